@@ -411,6 +411,106 @@ MAMBO_API size_t mambo_q4k_linear_group_workspace_bytes(const MamboQ4KItem* item
 MAMBO_API int mambo_q4k_linear_group(const MamboQ4KItem* items, int count, void* workspace, size_t workspace_bytes,
                                      mambo_stream_t stream);
 
+/*
+ * FP8 block-scaled linear (no counterpart in the reference, whose linears take
+ * GGUF blocks): weights E4M3 with one f32 scale per 128 x 128 block,
+ * activations E4M3 with one UE8M0 scale per 32 values along K (MXFP8) or per
+ * 128 (group = 32 or 128; exponents as mambo_quantize_mxfp8 forms them):
+ *   out[m, n] = sum_b sw[n/128, b] * sum_{k in block b} xq[m, k] * 2^e(m, k/group) * wq[n, k]
+ * with FP32 accumulation. Any N, K >= 1 (up to 2^24) and any M >= 1. A value
+ * group with NaN or infinity has the scale code 0xFF and makes its row NaN.
+ *
+ * A weight is packed once, from values [experts, N, K] and scales [experts,
+ * ceil(N/128), ceil(K/128)] with any strides (values in bytes, scales in
+ * elements). gate_up: rows [0, N/2) are a gate projection, [N/2, N) an up
+ * projection, each with its own row blocks of scales (2 * ceil(N/2/128) scale
+ * rows); such a weight is for mambo_moe_experts. The packed buffer is 16-byte
+ * aligned.
+ */
+typedef struct MamboFp8BlockWeight {
+  const void* packed;  /* mambo_fp8b_packed_bytes() */
+  const float* scales; /* mambo_fp8b_scales_bytes() */
+  int64_t n_rows;      /* N */
+  int64_t k;           /* K */
+  int64_t n_experts;   /* 1 for a plain linear, at most MAMBO_MOE_MAX_EXPERTS */
+  int gate_up;
+} MamboFp8BlockWeight;
+#define MAMBO_MOE_MAX_EXPERTS 1024
+#define MAMBO_MOE_MAX_TOP 32
+MAMBO_API size_t mambo_fp8b_packed_bytes(int64_t experts, int64_t n, int64_t k, int gate_up);
+MAMBO_API size_t mambo_fp8b_scales_bytes(int64_t experts, int64_t n, int64_t k, int gate_up);
+MAMBO_API int mambo_fp8b_pack(const uint8_t* values, int64_t experts, int64_t n, int64_t k, int64_t stride_expert,
+                              int64_t stride_row, int64_t stride_k, const float* block_scales,
+                              int64_t scale_stride_expert, int64_t scale_stride_row, int64_t scale_stride_k,
+                              int gate_up, void* packed, float* packed_scales, mambo_stream_t stream);
+
+/* Activation quantization alone: x [M, K] (f32 or bf16, row stride ldx elements, any K >= 1)
+ * -> q u8 [M, K] E4M3 and s u8 [M, ceil(K/group)] UE8M0. */
+MAMBO_API int mambo_fp8b_quantize(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, int group, uint8_t* q,
+                                  int64_t ldq, uint8_t* s, int64_t lds, mambo_stream_t stream);
+
+/*
+ * The linear on quantized activations, with the quantization in the call, and
+ * grouped by expert: rows [offsets[e], offsets[e+1]) of x times expert e's
+ * weight, offsets int32 [experts + 1] in device memory (0 first, then
+ * non-decreasing up to `rows`; segments may be empty; offsets outside [0, rows]
+ * are clamped and rows that no segment covers are not written). workspace:
+ * mambo_fp8b_linear_workspace_bytes(), zero-filled once, shared with the other
+ * linears of the stream.
+ */
+MAMBO_API size_t mambo_fp8b_linear_workspace_bytes(int64_t rows, int64_t experts, int64_t n, int64_t k);
+MAMBO_API int mambo_fp8b_linear(const uint8_t* xq, int64_t ldxq, const uint8_t* xs, int64_t ldxs, int group, int64_t m,
+                                const MamboFp8BlockWeight* w, void* out, int out_dtype, int64_t ldo, void* workspace,
+                                size_t workspace_bytes, mambo_stream_t stream);
+MAMBO_API int mambo_fp8b_linear_fused(const void* x, int x_dtype, int64_t ldx, int group, int64_t m,
+                                      const MamboFp8BlockWeight* w, void* out, int out_dtype, int64_t ldo,
+                                      void* workspace, size_t workspace_bytes, mambo_stream_t stream);
+MAMBO_API int mambo_fp8b_grouped_linear(const void* x, int x_dtype, int64_t ldx, int group, int64_t rows,
+                                        const int32_t* offsets, const MamboFp8BlockWeight* w, void* out, int out_dtype,
+                                        int64_t ldo, void* workspace, size_t workspace_bytes, mambo_stream_t stream);
+
+/*
+ * Expert routing of logits [tokens, experts] (f32 or bf16): per token the `top`
+ * experts with the highest selection score, highest first, equal scores to the
+ * lower expert. MAMBO_MOE_SOFTMAX: p = softmax(logits), selection by logit;
+ * MAMBO_MOE_SIGMOID: p = 1/(1+exp(-logit)), selection by p. bias (f32
+ * [experts] or NULL) is added to the selection score only. weights = p of the
+ * chosen, divided by their sum with renormalize, times scale. A logit of -inf
+ * or NaN masks its expert; +inf counts as the largest finite number; a token
+ * with fewer than `top` experts left gets ids -1, weights 0, positions -1.
+ * offsets [experts + 1]: first row of each expert in expert order (stable by
+ * token); positions [tokens, top]: row of each choice; rows (NULL or [tokens *
+ * top]): the choice token * top + j of each row, -1 past the last. workspace:
+ * mambo_moe_route_workspace_bytes().
+ */
+enum { MAMBO_MOE_SOFTMAX = 0, MAMBO_MOE_SIGMOID = 1 };
+MAMBO_API size_t mambo_moe_route_workspace_bytes(int64_t tokens, int64_t experts);
+MAMBO_API int mambo_moe_route(const void* logits, int dtype, int64_t ld, const float* bias, int64_t tokens,
+                              int64_t experts, int top, int scoring, int renormalize, float scale, int32_t* ids,
+                              float* weights, int32_t* offsets, int32_t* positions, int32_t* rows, void* workspace,
+                              size_t workspace_bytes, mambo_stream_t stream);
+
+/* out[t] = sum_j weights[t, j] * y[positions[t, j]] (positions < 0 are skipped), FP32 in the order of j. */
+MAMBO_API int mambo_moe_combine(const void* y, int y_dtype, int64_t ldy, int64_t rows, const int32_t* positions,
+                                const float* weights, int64_t tokens, int top, int64_t h, void* out, int out_dtype,
+                                int64_t ldo, mambo_stream_t stream);
+
+/*
+ * A layer of routed experts: x [tokens, H] -> MXFP8 -> gate and up of the
+ * chosen experts -> h = silu(gate) * up -> MXFP8 (from FP32) -> down -> the
+ * weighted sum of each token's rows. gate_up: a gate/up weight [experts, 2I,
+ * H]; down [experts, H, I]; ids, weights, positions and offsets from
+ * mambo_moe_route. Each expert row rounds once to out_dtype before the sum.
+ * workspace: mambo_moe_experts_workspace_bytes(), zero-filled once.
+ */
+MAMBO_API size_t mambo_moe_experts_workspace_bytes(int64_t tokens, int top, int64_t experts, int64_t h, int64_t i,
+                                                   int out_dtype);
+MAMBO_API int mambo_moe_experts(const void* x, int x_dtype, int64_t ldx, int64_t tokens, const int32_t* ids,
+                                const float* weights, const int32_t* positions, const int32_t* offsets, int top,
+                                const MamboFp8BlockWeight* gate_up, const MamboFp8BlockWeight* down, void* out,
+                                int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
+                                mambo_stream_t stream);
+
 /* Number of tunable configurations of a kernel kind, and the i-th one (for the autotuner).
  * Replaces the search spaces of make_benchmark_cases (src/python/mambo/kernels/iq3_s_fp8.py:402-465). */
 MAMBO_API int mambo_num_configs(int kernel);

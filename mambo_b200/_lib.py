@@ -75,6 +75,19 @@ EXPORTED_SYMBOLS = (
     "mambo_ar_comm_connect",
     "mambo_ar_comm_destroy",
     "mambo_iq3s_linear_fused_ar",
+    "mambo_fp8b_packed_bytes",
+    "mambo_fp8b_scales_bytes",
+    "mambo_fp8b_pack",
+    "mambo_fp8b_quantize",
+    "mambo_fp8b_linear_workspace_bytes",
+    "mambo_fp8b_linear",
+    "mambo_fp8b_linear_fused",
+    "mambo_fp8b_grouped_linear",
+    "mambo_moe_route_workspace_bytes",
+    "mambo_moe_route",
+    "mambo_moe_combine",
+    "mambo_moe_experts_workspace_bytes",
+    "mambo_moe_experts",
 )
 
 MAMBO_AR_HANDLE_BYTES = 64
@@ -137,6 +150,25 @@ class MamboQuantOut(ctypes.Structure):
         ("s", ctypes.c_void_p),
         ("lds", ctypes.c_int64),
     ]
+
+
+class MamboFp8BlockWeight(ctypes.Structure):
+    """A packed FP8 block-scaled weight [experts, N, K] (mambo_fp8b_pack)."""
+
+    _fields_ = [
+        ("packed", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("n_rows", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("n_experts", ctypes.c_int64),
+        ("gate_up", ctypes.c_int),
+    ]
+
+
+MAMBO_MOE_MAX_EXPERTS = 1024
+MAMBO_MOE_MAX_TOP = 32
+MAMBO_MOE_SOFTMAX = 0
+MAMBO_MOE_SIGMOID = 1
 
 
 class MamboLinearConfig(ctypes.Structure):
@@ -267,6 +299,37 @@ def load() -> ctypes.CDLL:
             "mambo_iq3s_linear_fused_ar": (
                 [vp, i32, i64, i64, ctypes.POINTER(MamboIQ3SWeight), vp, vp, i32, i64, vp,
                  ctypes.POINTER(MamboLinearConfig), vp, ctypes.c_size_t, vp],
+                i32,
+            ),
+            "mambo_fp8b_packed_bytes": ([i64, i64, i64, i32], ctypes.c_size_t),
+            "mambo_fp8b_scales_bytes": ([i64, i64, i64, i32], ctypes.c_size_t),
+            "mambo_fp8b_pack": ([vp, i64, i64, i64, i64, i64, i64, vp, i64, i64, i64, i32, vp, vp, vp], i32),
+            "mambo_fp8b_quantize": ([vp, i32, i64, i64, i64, i32, vp, i64, vp, i64, vp], i32),
+            "mambo_fp8b_linear_workspace_bytes": ([i64, i64, i64, i64], ctypes.c_size_t),
+            "mambo_fp8b_linear": (
+                [vp, i64, vp, i64, i32, i64, ctypes.POINTER(MamboFp8BlockWeight), vp, i32, i64, vp, ctypes.c_size_t, vp],
+                i32,
+            ),
+            "mambo_fp8b_linear_fused": (
+                [vp, i32, i64, i32, i64, ctypes.POINTER(MamboFp8BlockWeight), vp, i32, i64, vp, ctypes.c_size_t, vp],
+                i32,
+            ),
+            "mambo_fp8b_grouped_linear": (
+                [vp, i32, i64, i32, i64, vp, ctypes.POINTER(MamboFp8BlockWeight), vp, i32, i64, vp, ctypes.c_size_t,
+                 vp],
+                i32,
+            ),
+            "mambo_moe_route_workspace_bytes": ([i64, i64], ctypes.c_size_t),
+            "mambo_moe_route": (
+                [vp, i32, i64, vp, i64, i64, i32, i32, i32, ctypes.c_float, vp, vp, vp, vp, vp, vp, ctypes.c_size_t,
+                 vp],
+                i32,
+            ),
+            "mambo_moe_combine": ([vp, i32, i64, i64, vp, vp, i64, i32, i64, vp, i32, i64, vp], i32),
+            "mambo_moe_experts_workspace_bytes": ([i64, i32, i64, i64, i64, i32], ctypes.c_size_t),
+            "mambo_moe_experts": (
+                [vp, i32, i64, i64, vp, vp, vp, vp, i32, ctypes.POINTER(MamboFp8BlockWeight),
+                 ctypes.POINTER(MamboFp8BlockWeight), vp, i32, i64, vp, ctypes.c_size_t, vp],
                 i32,
             ),
         }

@@ -139,6 +139,30 @@ int require_sm100(DeviceInfo* info) {
   return MAMBO_OK;
 }
 
+}  // namespace
+
+namespace mambo {
+int api_fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return fail(code, "%s", buf);
+}
+int api_ok() { return ok(); }
+int api_cuda_fail(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+int api_require_sm100(int* sms, int* smem_optin) {
+  DeviceInfo info;
+  const int st = require_sm100(&info);
+  *sms = info.sms;
+  *smem_optin = info.max_smem_optin;
+  return st;
+}
+}  // namespace mambo
+
+namespace {
+
 // --- configurations ---------------------------------------------------------
 // tcgen05 GEMV (MAMBO_KERNEL_GEMV): {decoder warps, stages, prefetch}, each with split 0 and 1.
 struct TcChoice {
@@ -199,10 +223,10 @@ constexpr int kNumGemmF16Configs = kNumGemmConfigs * (int)(sizeof(kGemmSplits) /
 // Split-K counters live at the start of every workspace: 64 Ki ints, zero
 // between calls, a fixed region so that a call never finds another shape's
 // partials there. Shapes needing more are rejected.
-constexpr size_t kCounterBytes = 256 * 1024;
+constexpr size_t kCounterBytes = kWorkspaceCounterBytes;
 // The first half holds the GEMVs' counters (4 per 128-row tile), the second
 // the FP16 GEMM's K-split counters (8 per output tile).
-constexpr size_t kGemvCounterBytes = 128 * 1024;
+constexpr size_t kGemvCounterBytes = kWorkspaceSplitCounterOffset;
 constexpr size_t kGemmSplitCounterOffset = kGemvCounterBytes;
 constexpr size_t kGemmSplitCounterBytes = kCounterBytes - kGemmSplitCounterOffset;
 constexpr int kGemmMaxSplit = 8;

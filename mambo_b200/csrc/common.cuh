@@ -31,6 +31,8 @@ enum WaitSite : int {
   kSiteGemvEmpty = 2,
   kSiteSelfTest = 9,
   kSiteArPeer = 10,  // a peer rank's partial never arrived (fused all-reduce)
+  kSiteFbFull = 11,  // FP8 block product: operands or results
+  kSiteFbEmpty = 12,
 };
 
 __device__ __forceinline__ void record_timeout(int site) {

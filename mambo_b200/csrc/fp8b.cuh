@@ -1,0 +1,205 @@
+// Layouts and parameter blocks of the FP8 block-scaled linear (E4M3 weights
+// with one f32 scale per 128 x 128 block) and of its expert-grouped form.
+//
+// Weights, packed once: a 16 KB record per (128-row tile, 128-wide K block),
+// the tile's bytes in the tensor core's 128-byte-swizzled K-major layout (row
+// r at 128*r, its 16-byte chunk c at chunk c ^ (r & 7)), records K-block
+// consecutive per row tile, row tiles consecutive per expert. A record is one
+// bulk copy and needs no tensor map; rows past N and values past K are zero.
+// Scales: f32 [experts][row tiles][2][K blocks]; entry 0 scales the rows of
+// the tile's even 32-row quarters, entry 1 those of the odd ones (equal,
+// unless the tile interleaves gate and up rows by quarters).
+//
+// Activations, written by the quantizer for each call: E4M3 bytes [K block]
+// [padded row][128 bytes], swizzled by (padded row & 7), so any run of rows
+// that starts at a multiple of 8 is one bulk copy per K block; scale codes
+// (UE8M0, one per 32 values) as the tensor core's scale-factor atoms, 512
+// bytes per (token tile, K block, 128 rows of the tile).
+//
+// Ragged segments: expert e owns rows [o_e, o_{e+1}) of R. Its padded rows
+// start at floor8(o_e) + 8e and its token-tile slots at o_e / nt + e: since
+// floor(a + c) - floor(a) + 1 >= ceil(c) in units of 8 (of nt), consecutive
+// segments never overlap, and no prefix sum over the experts is needed.
+#pragma once
+
+#include "common.cuh"
+
+namespace mambo {
+
+constexpr int kFbBlock = 128;                // K block, rows of a weight tile
+constexpr uint32_t kFbRecord = 128u * 128u;  // bytes of a packed weight record
+constexpr uint32_t kFbAtom = 512u;           // bytes of a scale-factor atom (128 rows x 4 groups)
+constexpr int kFbMaxExperts = 1024;
+
+struct FbActivations {
+  uint8_t* x8;        // [kblocks][rows_pad][128]
+  uint8_t* atoms;     // [slots][kblocks][atoms per tile][512]
+  int64_t rows_pad;   // padded rows of x8
+  int64_t slots;      // token-tile slots
+  int kblocks;
+  int nt;             // most tokens of a tile
+};
+
+__host__ __device__ inline int fb_atoms_per_tile(int nt) { return (nt + 127) / 128; }
+__host__ __device__ inline int64_t fb_rows_pad(int64_t rows, int64_t experts) {
+  // The last tile is read in whole groups of 16 rows: 16 rows of slack.
+  return rows / 8 * 8 + 8 * experts + 16;
+}
+__host__ __device__ inline int64_t fb_slots(int64_t rows, int64_t experts, int nt) { return rows / nt + experts; }
+__host__ __device__ inline int64_t fb_row_start(int o, int e) { return (int64_t)(o / 8 * 8) + 8 * e; }
+__host__ __device__ inline int64_t fb_slot_start(int o, int e, int nt) { return o / nt + e; }
+// A segment of `count` rows is cut into equal tiles of at most nt tokens, a multiple of 16 each.
+__host__ __device__ inline int fb_tiles(int count, int nt) { return (count + nt - 1) / nt; }
+__host__ __device__ inline int fb_tile_rows(int count, int tiles) {
+  return tiles > 0 ? ((count + tiles - 1) / tiles + 15) / 16 * 16 : 16;
+}
+
+#ifdef __CUDACC__
+// Where row `local` of expert e (o_e, count) lies: its padded row, its tile's slot and its row in the tile.
+struct FbPlace {
+  int64_t prow, slot;
+  int in_tile;
+};
+__device__ __forceinline__ FbPlace fb_place(int o, int count, int e, int local, int nt) {
+  FbPlace pl;
+  const int tiles = fb_tiles(count, nt), tr = fb_tile_rows(count, tiles);
+  pl.prow = fb_row_start(o, e) + local;
+  pl.slot = fb_slot_start(o, e, nt) + local / tr;
+  pl.in_tile = local % tr;
+  return pl;
+}
+
+__device__ __forceinline__ void fb_store(const FbActivations& a, const FbPlace& pl, int64_t chunk8, uint2 q,
+                                         uint32_t word) {
+  // chunk8: index of the 8-value chunk in the row.
+  if (pl.prow < 0 || pl.prow >= a.rows_pad || pl.slot < 0 || pl.slot >= a.slots) return;
+  const int64_t kb = chunk8 >> 4;
+  const int c = (int)(chunk8 & 15);
+  uint8_t* d = a.x8 + (kb * a.rows_pad + pl.prow) * 128 + (((c >> 1) ^ (int)(pl.prow & 7)) << 4) + (c & 1) * 8;
+  *reinterpret_cast<uint2*>(d) = q;
+  if (c == 0) {
+    const int apt = fb_atoms_per_tile(a.nt), t = pl.in_tile & 127;
+    uint8_t* s = a.atoms + ((pl.slot * a.kblocks + kb) * apt + (pl.in_tile >> 7)) * kFbAtom + (t & 31) * 16 + (t >> 5) * 4;
+    *reinterpret_cast<uint32_t*>(s) = word;
+  }
+}
+
+__device__ __forceinline__ int clamp_offset(int o, int64_t total) { return o < 0 ? 0 : o > total ? (int)total : o; }
+#endif
+
+// --- weight packing ----------------------------------------------------------
+struct FbPackParams {
+  const uint8_t* w;  // E4M3 [experts][N][K] with any strides (bytes)
+  int64_t stride_e, stride_n, stride_k;
+  const float* s;    // [experts][row blocks][K blocks] with any strides (elements)
+  int64_t sstride_e, sstride_n, sstride_k;
+  int experts, n, k;
+  int gate_up;       // 1: rows [0, n/2) are gate, [n/2, n) up, interleaved by quarters of a tile
+  int row_tiles, kblocks;
+  uint8_t* packed;
+  float* scales;
+};
+cudaError_t launch_fb_pack(const FbPackParams& p, cudaStream_t stream);
+__host__ __device__ inline int fb_row_tiles(int64_t n, int gate_up) {
+  // Gate and up: 64 hidden features per tile, whole 128-feature blocks.
+  return gate_up ? (int)((n / 2 + 127) / 128) * 2 : (int)((n + 127) / 128);
+}
+
+// --- activation quantization ---------------------------------------------------
+enum { kFbDense = 0, kFbGrouped = 1, kFbRouted = 2 };
+struct FbQuantParams {
+  const void* x;  // [rows][k], row stride ldx elements
+  int x_kind;     // MAMBO_F32, MAMBO_BF16, or kFbCodes: already E4M3 with the scale codes of xs
+  const uint8_t* xs;
+  int64_t lds;
+  int64_t ldx;
+  int64_t rows, k;
+  int group;  // 32 or 128 values per scale
+  int mode;   // kFb*
+  int experts;
+  const int* offsets;    // [experts + 1] (kFbGrouped, kFbRouted)
+  const int* ids;        // [rows][top] (kFbRouted): expert of each copy of the row, < 0 for none
+  const int* positions;  // [rows][top]: its row in expert order
+  int top;
+  int64_t total_rows;    // rows in expert order (bounds every position)
+  FbActivations act;
+  // Row-major outputs instead of act (kFbDense, values != null).
+  uint8_t* values;
+  int64_t ldv;
+  uint8_t* scales;
+  int64_t ldsc;
+};
+constexpr int kFbCodes = 100;
+cudaError_t launch_fb_quant(const FbQuantParams& p, cudaStream_t stream);
+
+// --- the product -----------------------------------------------------------------
+struct FbGemmParams {
+  const uint8_t* packed;
+  const float* scales;
+  FbActivations act;
+  int experts;
+  int64_t rows;        // R (dense: M); bounds the offsets
+  const int* offsets;  // device [experts + 1], or null for a dense call
+  int n_rows;          // valid rows of the weight (output columns)
+  int row_tiles;
+  void* out;           // [R][ldo]
+  int out_bf16;
+  int64_t ldo;
+  int stages;
+  int evict_weights;   // 1: weights are read once (evict-first)
+  float* partials;     // [grid][2][128 * nt]
+  int* counters;       // [grid][8], zero on entry and left zero
+};
+// Token-tile sizes the kernel is built for.
+int fb_tile_for(int64_t expected_rows);
+uint32_t fb_gemm_smem(int nt, int experts, int stages);
+int fb_gemm_stages(int nt, int experts, int smem_optin);
+int fb_gemm_grid(int nt, int sms);
+size_t fb_partial_bytes(int nt, int sms);
+cudaError_t launch_fb_gemm(const FbGemmParams& p, int grid, cudaStream_t stream);
+
+// --- experts ----------------------------------------------------------------------
+struct FbHiddenParams {
+  const float* gu;  // [R][ld]: columns in the gate/up tile order
+  int64_t ld;
+  int64_t rows;     // R
+  int i;            // hidden features
+  int experts;
+  const int* offsets;
+  FbActivations act;
+};
+cudaError_t launch_fb_hidden(const FbHiddenParams& p, cudaStream_t stream);
+
+struct FbRouteParams {
+  const void* logits;
+  int bf16;
+  int64_t ld;
+  const float* bias;
+  int tokens, experts, top;
+  int sigmoid, renormalize;
+  float scale;
+  int* ids;
+  float* weights;
+  int* offsets;
+  int* positions;
+  int* rows;
+  int* chunk_counts;  // workspace [chunks][experts + 1]
+};
+int fb_route_chunks(int tokens);
+cudaError_t launch_fb_route(const FbRouteParams& p, cudaStream_t stream);
+
+struct FbCombineParams {
+  const void* y;  // [R][ldy]
+  int y_bf16;
+  int64_t ldy;
+  const int* positions;
+  const float* weights;
+  int tokens, top, h;
+  int64_t rows;   // R, bounds the positions
+  void* out;
+  int out_bf16;
+  int64_t ldo;
+};
+cudaError_t launch_fb_combine(const FbCombineParams& p, cudaStream_t stream);
+
+}  // namespace mambo

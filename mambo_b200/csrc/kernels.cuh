@@ -5,6 +5,16 @@
 
 namespace mambo {
 
+// Error channel and device check of the C ABI (api.cu), for its other files.
+int api_fail(int code, const char* fmt, ...);
+int api_ok();
+int api_cuda_fail(cudaError_t e, const char* what);
+int api_require_sm100(int* sms, int* smem_optin);
+// Counters at the start of every workspace: zero between calls. The second
+// half belongs to kernels that split K over tiles.
+constexpr size_t kWorkspaceCounterBytes = 256 * 1024;
+constexpr size_t kWorkspaceSplitCounterOffset = 128 * 1024;
+
 // Sets a kernel's dynamic shared memory limit once per (kernel, device).
 cudaError_t ensure_smem_attribute(const void* kernel, size_t smem_bytes);
 

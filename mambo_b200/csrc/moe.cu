@@ -1,0 +1,364 @@
+// Expert routing, the hidden activation of the experts' path and the weighted
+// sum of a token's expert outputs (layouts in fp8b.cuh).
+#include "fp8b.cuh"
+#include "kernels.cuh"
+#include "mxfp8.cuh"
+
+namespace mambo {
+
+namespace {
+
+constexpr int kRouteThreads = 256;
+constexpr int kRouteWarps = kRouteThreads / 32;
+// Tokens of a chunk: one CTA. A call of one chunk is one launch.
+constexpr int kRouteChunk = 128;
+
+// Monotone map of a float to an unsigned key (0 is free: it marks masked experts).
+__device__ __forceinline__ uint32_t order_key(float f) {
+  const uint32_t b = __float_as_uint(f);
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+
+// One token, a warp: expert 32*i + lane in slot i of the lane. Experts whose
+// logit is -inf or NaN are masked; +inf counts as the largest finite number.
+template <int NV>
+__device__ __forceinline__ void route_token(const FbRouteParams& p, int token, int lane, int* hist) {
+  float l[NV], prob[NV];
+  uint32_t key[NV];
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int e = 32 * i + lane;
+    l[i] = -INFINITY;
+    if (e < p.experts) {
+      const int64_t at = (int64_t)token * p.ld + e;
+      const float v = p.bf16 ? __uint_as_float((uint32_t)__ldg((const uint16_t*)p.logits + at) << 16)
+                             : __ldg((const float*)p.logits + at);
+      if (v == v) l[i] = fminf(v, 3.4028234663852886e38f);
+    }
+    top = fmaxf(top, l[i]);
+  }
+  if (p.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = 32 * i + lane;
+      prob[i] = 1.0f / (1.0f + expf(-l[i]));
+      const float s = prob[i] + (p.bias && e < p.experts ? __ldg(p.bias + e) : 0.f);
+      key[i] = l[i] == -INFINITY || s != s ? 0u : order_key(s);
+    }
+  } else {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      prob[i] = l[i] == -INFINITY ? 0.f : expf(l[i] - top);
+      sum += prob[i];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = 32 * i + lane;
+      prob[i] = sum > 0.f ? prob[i] / sum : 0.f;
+      const float s = l[i] + (p.bias && e < p.experts ? __ldg(p.bias + e) : 0.f);
+      key[i] = l[i] == -INFINITY || s != s ? 0u : order_key(s);
+    }
+  }
+  float total = 0.f, mine_w = 0.f;
+  int mine_id = -1;
+  for (int j = 0; j < p.top; ++j) {
+    uint32_t best = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (key[i] > best) {  // the first of equal keys: the lowest expert of the lane
+        best = key[i];
+        at = i;
+      }
+    const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, best);
+    if (m == 0) break;  // no expert left
+    const uint32_t cand = best == m ? (uint32_t)(32 * at + lane) : 0xFFFFFFFFu;
+    const uint32_t id = __reduce_min_sync(0xFFFFFFFFu, cand);
+    float w = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (cand == id && at == i) {
+        w = prob[i];
+        key[i] = 0;
+      }
+    w = __shfl_sync(0xFFFFFFFFu, w, (int)(id & 31));
+    total += w;
+    if (lane == j) {
+      mine_w = w;
+      mine_id = (int)id;
+    }
+  }
+  if (p.renormalize) mine_w = total > 0.f ? mine_w / total : 0.f;
+  if (lane < p.top) {
+    p.ids[(int64_t)token * p.top + lane] = mine_id;
+    p.weights[(int64_t)token * p.top + lane] = mine_w * p.scale;
+    atomicAdd(hist + (mine_id < 0 ? p.experts : mine_id), 1);  // whole numbers: the order does not matter
+  }
+}
+
+// In-place exclusive scan of n counts in shared memory by warp 0.
+__device__ __forceinline__ void scan_counts(int* v, int n, int lane) {
+  int carry = 0;
+  for (int b = 0; b < n; b += 32) {
+    const int x = b + lane < n ? v[b + lane] : 0;
+    int t = x;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xFFFFFFFFu, t, d);
+      if (lane >= d) t += up;
+    }
+    if (b + lane < n) v[b + lane] = carry + t - x;
+    carry += __shfl_sync(0xFFFFFFFFu, t, 31);
+  }
+}
+
+// The chunk's (token, choice) pairs in order, each to its row: base[e] holds
+// the first free row of expert e for this chunk (bucket `experts`: no expert).
+__device__ __forceinline__ void place_chunk(const FbRouteParams& p, int first, int count, const int* base, int* wcnt,
+                                            int warp, int lane) {
+  const int n = count * p.top, buckets = p.experts + 1;
+  const int per = (n + kRouteWarps * 32 - 1) / (kRouteWarps * 32) * 32;  // entries of a warp, whole groups of 32
+  const int b0 = min(n, warp * per), b1 = min(n, b0 + per);
+  const int* ids = p.ids + (int64_t)first * p.top;
+  for (int i = threadIdx.x; i < kRouteWarps * buckets; i += kRouteThreads) wcnt[i] = 0;
+  __syncthreads();
+  for (int i = b0 + lane; i < b1; i += 32) {
+    const int e = ids[i];
+    atomicAdd(wcnt + warp * buckets + (e < 0 ? p.experts : e), 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < buckets; e += kRouteThreads) {
+    int at = base[e];
+    for (int w = 0; w < kRouteWarps; ++w) {
+      const int c = wcnt[w * buckets + e];
+      wcnt[w * buckets + e] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  for (int i0 = b0; i0 < b1; i0 += 32) {
+    const int i = i0 + lane;
+    const bool have = i < b1;
+    const int id = have ? ids[i] : -2;
+    const int e = id < 0 ? p.experts : id;
+    const unsigned same = __match_any_sync(0xFFFFFFFFu, id);
+    int* c = wcnt + warp * buckets + e;
+    const int at = have ? *c + __popc(same & ((1u << lane) - 1u)) : 0;
+    __syncwarp();
+    if (have) {
+      if ((same >> lane) == 1u) *c = at + 1;  // the group's last lane
+      const int64_t slot = (int64_t)first * p.top + i;
+      p.positions[slot] = id < 0 ? -1 : at;
+      if (p.rows) p.rows[at] = id < 0 ? -1 : (int)slot;
+    }
+    __syncwarp();
+  }
+}
+
+}  // namespace
+
+// Selection of a chunk's tokens, a warp per token, and the chunk's counts per
+// expert; with one chunk also the placement. Latency-bound in decode.
+template <int NV>
+__global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const __grid_constant__ FbRouteParams p) {
+  extern __shared__ int route_sm[];
+  int* hist = route_sm;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, buckets = p.experts + 1;
+  const int first = blockIdx.x * kRouteChunk, count = min(kRouteChunk, p.tokens - first);
+  for (int i = threadIdx.x; i < buckets; i += kRouteThreads) hist[i] = 0;
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  for (int t = warp; t < count; t += kRouteWarps) route_token<NV>(p, first + t, lane, hist);
+  __syncthreads();
+  if (gridDim.x > 1) {
+    for (int i = threadIdx.x; i < buckets; i += kRouteThreads) p.chunk_counts[(int64_t)blockIdx.x * buckets + i] = hist[i];
+    return;
+  }
+  if (warp == 0) scan_counts(hist, buckets, lane);
+  __syncthreads();
+  for (int i = threadIdx.x; i < buckets; i += kRouteThreads) p.offsets[i] = hist[i];
+  place_chunk(p, first, count, hist, hist + buckets, warp, lane);
+}
+
+// Placement of one chunk: every CTA sums the chunks' counts itself (the counts
+// of a 16384-token call are 128 x 257 numbers in L2), so there is no third launch.
+__global__ void __launch_bounds__(kRouteThreads) moe_place_kernel(const __grid_constant__ FbRouteParams p) {
+  extern __shared__ int route_sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, buckets = p.experts + 1;
+  int* base = route_sm;            // totals, then first rows
+  int* before = base + buckets;    // counts of earlier chunks
+  int* wcnt = before + buckets;
+  const int first = blockIdx.x * kRouteChunk, count = min(kRouteChunk, p.tokens - first);
+  pdl_wait();
+  pdl_launch_dependents();
+  for (int e = threadIdx.x; e < buckets; e += kRouteThreads) {
+    int all = 0, prior = 0;
+#pragma unroll 8
+    for (int c = 0; c < (int)gridDim.x; ++c) {
+      const int v = p.chunk_counts[(int64_t)c * buckets + e];
+      all += v;
+      prior += c < (int)blockIdx.x ? v : 0;
+    }
+    base[e] = all;
+    before[e] = prior;
+  }
+  __syncthreads();
+  if (warp == 0) scan_counts(base, buckets, lane);
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < buckets; i += kRouteThreads) p.offsets[i] = base[i];
+  for (int e = threadIdx.x; e < buckets; e += kRouteThreads) before[e] += base[e];
+  __syncthreads();
+  place_chunk(p, first, count, before, wcnt, warp, lane);
+}
+
+int fb_route_chunks(int tokens) { return (tokens + kRouteChunk - 1) / kRouteChunk; }
+
+cudaError_t launch_fb_route(const FbRouteParams& p, cudaStream_t stream) {
+  const int chunks = fb_route_chunks(p.tokens), buckets = p.experts + 1;
+  const size_t smem = (size_t)buckets * (1 + kRouteWarps) * sizeof(int);
+  const int nv = (p.experts + 31) / 32;
+  const void* k = nv <= 2   ? (const void*)moe_route_kernel<2>
+                  : nv <= 4 ? (const void*)moe_route_kernel<4>
+                  : nv <= 8 ? (const void*)moe_route_kernel<8>
+                  : nv <= 16 ? (const void*)moe_route_kernel<16>
+                             : (const void*)moe_route_kernel<32>;
+  cudaError_t e = launch_pdl(k, dim3(chunks), dim3(kRouteThreads), smem, stream, p);
+  if (e != cudaSuccess || chunks == 1) return e;
+  return launch_pdl((const void*)moe_place_kernel, dim3(chunks), dim3(kRouteThreads),
+                    (size_t)buckets * (2 + kRouteWarps) * sizeof(int), stream, p);
+}
+
+// --------------------------------------------------------------------------
+// h = silu(gate) * up of each routed row, quantized to MXFP8 from FP32 into
+// the second product's activation layout: a rounding of h to bf16 in between
+// would move 1-2 % of its E4M3 codes.
+// --------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) moe_hidden_kernel(const __grid_constant__ FbHiddenParams p) {
+  const int64_t row = blockIdx.y + (int64_t)blockIdx.z * 65535;
+  if (row >= p.rows) return;
+  const int lane = threadIdx.x & 31;
+  const int chunks = (p.i + 127) / 128 * 16, c = blockIdx.x * 256 + threadIdx.x;
+  pdl_wait();
+  pdl_launch_dependents();
+  int e = 0;
+  for (int b = 0; b < p.experts; b += 32) {
+    const int end = b + lane < p.experts ? __ldg(p.offsets + b + lane + 1) : 0x7FFFFFFF;
+    e += __popc(__ballot_sync(0xFFFFFFFFu, end <= row));
+  }
+  if (e >= p.experts) return;
+  const bool in = c < chunks;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  if (in) {
+    const int f = c * 8;
+    const float* g = p.gu + row * p.ld + 128 * (f >> 6) + 64 * ((f >> 5) & 1) + (f & 31);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float gate = __ldg(g + i), up = __ldg(g + 32 + i);
+      v[i] = gate / (1.0f + expf(-gate)) * up;
+    }
+  }
+  uint2 q;
+  const uint32_t code = mxfp8_quad_rne(v, q);
+  uint32_t word = code << (8 * ((lane >> 2) & 3));
+  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
+  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
+  if (!in) return;
+  const int o = clamp_offset(__ldg(p.offsets + e), p.rows), end = clamp_offset(__ldg(p.offsets + e + 1), p.rows);
+  const int local = (int)row - o;
+  if (local < 0 || end <= o) return;
+  fb_store(p.act, fb_place(o, end - o, e, local, p.act.nt), c, q, word);
+}
+
+cudaError_t launch_fb_hidden(const FbHiddenParams& p, cudaStream_t stream) {
+  const int chunks = (p.i + 127) / 128 * 16;
+  const dim3 grid((unsigned)((chunks + 255) / 256), (unsigned)(p.rows < 65535 ? p.rows : 65535),
+                  (unsigned)((p.rows + 65534) / 65535));
+  return launch_pdl((const void*)moe_hidden_kernel, grid, dim3(256), 0, stream, p);
+}
+
+// --------------------------------------------------------------------------
+// out[t] = sum_j weights[t, j] * y[positions[t, j]], FP32 in the order of j,
+// rounded once; a token without experts gets zeros.
+// --------------------------------------------------------------------------
+template <bool kIn16, bool kVec>
+__global__ void __launch_bounds__(256) moe_combine_kernel(const __grid_constant__ FbCombineParams p) {
+  const int t = blockIdx.y + blockIdx.z * 65535;
+  if (t >= p.tokens) return;
+  const int c = (blockIdx.x * 256 + threadIdx.x) * 8;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (c >= p.h) return;
+  float acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+  for (int j = 0; j < p.top; ++j) {
+    const int pos = __ldg(p.positions + (int64_t)t * p.top + j);
+    if (pos < 0 || pos >= p.rows) continue;
+    const float w = __ldg(p.weights + (int64_t)t * p.top + j);
+    if constexpr (kIn16) {
+      const uint16_t* y = (const uint16_t*)p.y + (int64_t)pos * p.ldy + c;
+      if (kVec) {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(y));
+        const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[2 * i] = fmaf(w, __uint_as_float(u[i] << 16), acc[2 * i]);
+          acc[2 * i + 1] = fmaf(w, __uint_as_float(u[i] & 0xFFFF0000u), acc[2 * i + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i < p.h) acc[i] = fmaf(w, __uint_as_float((uint32_t)__ldg(y + i) << 16), acc[i]);
+      }
+    } else {
+      const float* y = (const float*)p.y + (int64_t)pos * p.ldy + c;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (kVec || c + i < p.h) acc[i] = fmaf(w, __ldg(y + i), acc[i]);
+    }
+  }
+  if (p.out_bf16) {
+    __nv_bfloat16* o = (__nv_bfloat16*)p.out + (int64_t)t * p.ldo + c;
+    if (kVec) {
+      uint32_t u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(acc[2 * i], acc[2 * i + 1]);
+        u[i] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+      *reinterpret_cast<uint4*>(o) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < p.h) o[i] = __float2bfloat16_rn(acc[i]);
+    }
+  } else {
+    float* o = (float*)p.out + (int64_t)t * p.ldo + c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (kVec || c + i < p.h) o[i] = acc[i];
+  }
+}
+
+cudaError_t launch_fb_combine(const FbCombineParams& p, cudaStream_t stream) {
+  const dim3 grid((unsigned)((p.h + 2047) / 2048), (unsigned)(p.tokens < 65535 ? p.tokens : 65535),
+                  (unsigned)((p.tokens + 65534) / 65535));
+  const int ys = p.y_bf16 ? 2 : 4, os = p.out_bf16 ? 2 : 4;
+  const bool vec = p.h % 8 == 0 && (uintptr_t)p.y % 16 == 0 && p.ldy * ys % 16 == 0 && (uintptr_t)p.out % 16 == 0 &&
+                   p.ldo * os % 16 == 0;
+  const void* k = p.y_bf16 ? (vec ? (const void*)moe_combine_kernel<true, true> : (const void*)moe_combine_kernel<true, false>)
+                           : (vec ? (const void*)moe_combine_kernel<false, true> : (const void*)moe_combine_kernel<false, false>);
+  return launch_pdl(k, grid, dim3(256), 0, stream, p);
+}
+
+}  // namespace mambo
