@@ -7,6 +7,7 @@
 #include <new>
 #include <string>
 
+#include "fp8b.cuh"
 #include "kernels.cuh"
 
 namespace mambo {
@@ -668,19 +669,30 @@ int mambo_device_status(int reset, int* code, int* where, int* block) {
   DeviceStatus st{};
   cudaError_t e = cudaMemcpyFromSymbol(&st, g_device_status, sizeof(st));
   if (e != cudaSuccess) return cuda_fail(e, "reading the device status");
+  // The FP8 block product is a program of its own with its own record.
+  void *fb_status = nullptr, *fb_limit = nullptr;
+  e = fb_status_symbols(&fb_status, &fb_limit);
+  DeviceStatus fb{};
+  if (e == cudaSuccess) e = cudaMemcpy(&fb, fb_status, sizeof(fb), cudaMemcpyDeviceToHost);
+  if (e != cudaSuccess) return cuda_fail(e, "reading the device status");
+  if (st.code == 0) st = fb;
   if (code) *code = st.code;
   if (where) *where = st.where;
   if (block) *block = st.block;
   if (reset) {
     DeviceStatus zero{};
     e = cudaMemcpyToSymbol(g_device_status, &zero, sizeof(zero));
+    if (e == cudaSuccess) e = cudaMemcpy(fb_status, &zero, sizeof(zero), cudaMemcpyHostToDevice);
     if (e != cudaSuccess) return cuda_fail(e, "resetting the device status");
   }
   return ok();
 }
 
 int mambo_set_wait_limit_ns(unsigned long long ns) {
+  void *fb_status = nullptr, *fb_limit = nullptr;
   cudaError_t e = cudaMemcpyToSymbol(g_wait_limit_ns, &ns, sizeof(ns));
+  if (e == cudaSuccess) e = fb_status_symbols(&fb_status, &fb_limit);
+  if (e == cudaSuccess) e = cudaMemcpy(fb_limit, &ns, sizeof(ns), cudaMemcpyHostToDevice);
   if (e != cudaSuccess) return cuda_fail(e, "setting the wait limit");
   return ok();
 }

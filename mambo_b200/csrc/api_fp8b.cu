@@ -29,8 +29,8 @@ int check_weight(const MamboFp8BlockWeight* w) {
 // One product's activations and partial sums in the workspace.
 struct Plan {
   int nt, kblocks, row_tiles;
-  int64_t rows_pad, slots;
-  size_t x8, atoms;  // bytes
+  int64_t slots;
+  size_t x8;  // bytes
 };
 Plan plan(int64_t rows, int64_t experts, int64_t bound, int64_t n, int64_t k, int gate_up) {
   Plan P;
@@ -41,19 +41,17 @@ Plan plan(int64_t rows, int64_t experts, int64_t bound, int64_t n, int64_t k, in
   P.nt = fb_tile_for(experts == 1 ? rows : share < bound ? share : bound);
   P.kblocks = (int)((k + 127) / 128);
   P.row_tiles = fb_row_tiles(n, gate_up);
-  P.rows_pad = fb_rows_pad(rows, experts);
   P.slots = fb_slots(rows, experts, P.nt);
-  P.x8 = align256((size_t)P.kblocks * P.rows_pad * 128);
-  P.atoms = align256((size_t)P.slots * P.kblocks * fb_atoms_per_tile(P.nt) * kFbAtom);
+  P.x8 = align256((size_t)P.slots * P.kblocks * fb_record_bytes(P.nt));
   return P;
 }
 FbActivations activations(const Plan& P, uint8_t* at) {
-  return FbActivations{at, at + P.x8, P.rows_pad, P.slots, P.kblocks, P.nt};
+  return FbActivations{at, P.slots, P.kblocks, P.nt};
 }
 
 constexpr int kSmsBound = 160;  // workspace sizes do not depend on the device: an upper bound of its SMs
 
-size_t product_bytes(const Plan& P) { return P.x8 + P.atoms + align256(fb_partial_bytes(P.nt, kSmsBound)); }
+size_t product_bytes(const Plan& P) { return P.x8 + align256(fb_partial_bytes(P.nt, kSmsBound)); }
 
 int check_workspace(void* ws, size_t have, size_t need) {
   if (!ws || have < need) return api_fail(MAMBO_EWORKSPACE, "workspace of %zu bytes needed, %zu given", need, have);
@@ -124,7 +122,7 @@ int linear_impl(const void* x, int x_kind, int64_t ldx, const uint8_t* xs, int64
   q.act = act;
   cudaError_t e = launch_fb_quant(q, stream);
   if (e != cudaSuccess) return api_cuda_fail(e, "fp8 block quantizer");
-  e = run_gemm(w, P, act, m, offsets, out, out_dtype == MAMBO_BF16, ldo, (int)w->n_rows, at + P.x8 + P.atoms, workspace,
+  e = run_gemm(w, P, act, m, offsets, out, out_dtype == MAMBO_BF16, ldo, (int)w->n_rows, at + P.x8, workspace,
                sms, smem, stream);
   if (e != cudaSuccess) return api_cuda_fail(e, "fp8 block product");
   return api_ok();
@@ -147,7 +145,7 @@ ExpertsPlan plan_experts(int64_t tokens, int64_t top, int64_t experts, int64_t h
   E.y = align256((size_t)E.rows * h * elem(out_dtype));
   const int nt = E.a.nt > E.b.nt ? E.a.nt : E.b.nt;
   E.partials = align256(fb_partial_bytes(nt, kSmsBound));
-  E.total = kWorkspaceCounterBytes + E.a.x8 + E.a.atoms + E.b.x8 + E.b.atoms + E.gu + E.y + E.partials;
+  E.total = kWorkspaceCounterBytes + E.a.x8 + E.b.x8 + E.gu + E.y + E.partials;
   return E;
 }
 
@@ -362,9 +360,9 @@ int mambo_moe_experts(const void* x, int x_dtype, int64_t ldx, int64_t tokens, c
   cudaStream_t stream = (cudaStream_t)stream_;
   uint8_t* at = (uint8_t*)workspace + kWorkspaceCounterBytes;
   const FbActivations xa = activations(E.a, at);
-  at += E.a.x8 + E.a.atoms;
+  at += E.a.x8;
   const FbActivations ha = activations(E.b, at);
-  at += E.b.x8 + E.b.atoms;
+  at += E.b.x8;
   float* gu = (float*)at;
   at += E.gu;
   void* y = at;

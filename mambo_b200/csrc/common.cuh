@@ -22,9 +22,15 @@ struct DeviceStatus {
   int reserved;
 };
 
+// Wall-clock limit of one bounded wait: g_wait_limit_ns, in nanoseconds (set by the host).
+#ifdef MAMBO_OWN_DEVICE_STATUS
+// A file compiled as a whole program: its own copies, which the host reads and sets with the others.
+static __device__ DeviceStatus g_device_status = {0, 0, 0, 0};
+static __device__ unsigned long long g_wait_limit_ns = 1000000000ull;
+#else
 extern __device__ DeviceStatus g_device_status;
-// Wall-clock limit of one bounded wait, in nanoseconds (set by the host).
 extern __device__ unsigned long long g_wait_limit_ns;
+#endif
 
 enum WaitSite : int {
   kSiteGemvFull = 1,

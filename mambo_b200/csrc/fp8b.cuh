@@ -10,16 +10,17 @@
 // the tile's even 32-row quarters, entry 1 those of the odd ones (equal,
 // unless the tile interleaves gate and up rows by quarters).
 //
-// Activations, written by the quantizer for each call: E4M3 bytes [K block]
-// [padded row][128 bytes], swizzled by (padded row & 7), so any run of rows
-// that starts at a multiple of 8 is one bulk copy per K block; scale codes
-// (UE8M0, one per 32 values) as the tensor core's scale-factor atoms, 512
-// bytes per (token tile, K block, 128 rows of the tile).
+// Activations, written by the quantizer for each call: a record per (token
+// tile, K block), again one bulk copy (per CTA): the tile's rows of 128 E4M3
+// bytes, swizzled, then its scale codes (UE8M0, one per 32 values) as the
+// tensor core's scale-factor atoms, 512 bytes per 128 tokens. For tiles of a
+// CTA pair a record has a part per CTA, each with its half of either MMA's
+// tokens (fb_split) and all the scale codes.
 //
-// Ragged segments: expert e owns rows [o_e, o_{e+1}) of R. Its padded rows
-// start at floor8(o_e) + 8e and its token-tile slots at o_e / nt + e: since
-// floor(a + c) - floor(a) + 1 >= ceil(c) in units of 8 (of nt), consecutive
-// segments never overlap, and no prefix sum over the experts is needed.
+// Ragged segments: expert e owns rows [o_e, o_{e+1}) of R; its token tiles have
+// the slots from o_e / nt + e on: since floor(a + c) - floor(a) + 1 >= ceil(c)
+// in units of nt, consecutive segments never overlap, and no prefix sum over
+// the experts is needed to place a row.
 #pragma once
 
 #include "common.cuh"
@@ -31,23 +32,28 @@ constexpr uint32_t kFbRecord = 128u * 128u;  // bytes of a packed weight record
 constexpr uint32_t kFbAtom = 512u;           // bytes of a scale-factor atom (128 rows x 4 groups)
 constexpr int kFbMaxExperts = 1024;
 
+// Tokens of a tile above which CTA pairs work on it (and the largest tile).
+constexpr int kFbPairTokens = 240;
+
 struct FbActivations {
-  uint8_t* x8;        // [kblocks][rows_pad][128]
-  uint8_t* atoms;     // [slots][kblocks][atoms per tile][512]
-  int64_t rows_pad;   // padded rows of x8
-  int64_t slots;      // token-tile slots
+  uint8_t* x8;    // [slots][kblocks][record]
+  int64_t slots;  // token-tile slots
   int kblocks;
-  int nt;             // most tokens of a tile
+  int nt;         // most tokens of a tile
 };
 
-__host__ __device__ inline int fb_atoms_per_tile(int nt) { return (nt + 127) / 128; }
-__host__ __device__ inline int64_t fb_rows_pad(int64_t rows, int64_t experts) {
-  // The last tile is read in whole groups of 16 rows: 16 rows of slack.
-  return rows / 8 * 8 + 8 * experts + 16;
+__host__ __device__ constexpr bool fb_is_pair(int nt) { return nt > 128; }
+__host__ __device__ constexpr int fb_atoms_per_tile(int nt) { return (nt + 127) / 128; }
+// Bytes of a CTA's part of a record, and of a record.
+__host__ __device__ constexpr uint32_t fb_part_bytes(int nt) {
+  return (uint32_t)((fb_is_pair(nt) ? nt / 2 : nt) * 128) + fb_atoms_per_tile(nt) * kFbAtom;
 }
+__host__ __device__ constexpr uint32_t fb_record_bytes(int nt) { return (fb_is_pair(nt) ? 2 : 1) * fb_part_bytes(nt); }
 __host__ __device__ inline int64_t fb_slots(int64_t rows, int64_t experts, int nt) { return rows / nt + experts; }
-__host__ __device__ inline int64_t fb_row_start(int o, int e) { return (int64_t)(o / 8 * 8) + 8 * e; }
 __host__ __device__ inline int64_t fb_slot_start(int o, int e, int nt) { return o / nt + e; }
+// Rows that a CTA holds of a tile of n tokens, before its scale codes: alone all (in groups of 8), of a pair half of
+// each MMA's N, the first MMA taking min(128, n) tokens rounded up to 16 and the second the rest.
+__host__ __device__ inline int fb_part_rows(int n, bool pair) { return pair ? (n + 15) / 16 * 8 : (n + 7) / 8 * 8; }
 // A segment of `count` rows is cut into equal tiles of at most nt tokens, a multiple of 16 each.
 __host__ __device__ inline int fb_tiles(int count, int nt) { return (count + nt - 1) / nt; }
 __host__ __device__ inline int fb_tile_rows(int count, int tiles) {
@@ -55,32 +61,48 @@ __host__ __device__ inline int fb_tile_rows(int count, int tiles) {
 }
 
 #ifdef __CUDACC__
-// Where row `local` of expert e (o_e, count) lies: its padded row, its tile's slot and its row in the tile.
+// Where row `local` of expert e (o_e, count) lies: its tile's slot, its row there and the tile's tokens.
 struct FbPlace {
-  int64_t prow, slot;
-  int in_tile;
+  int64_t slot;
+  int in_tile, n;
 };
 __device__ __forceinline__ FbPlace fb_place(int o, int count, int e, int local, int nt) {
   FbPlace pl;
   const int tiles = fb_tiles(count, nt), tr = fb_tile_rows(count, tiles);
-  pl.prow = fb_row_start(o, e) + local;
-  pl.slot = fb_slot_start(o, e, nt) + local / tr;
-  pl.in_tile = local % tr;
+  const int tt = local / tr;
+  pl.slot = fb_slot_start(o, e, nt) + tt;
+  pl.in_tile = local - tt * tr;
+  pl.n = min(tr, count - tt * tr);
   return pl;
 }
 
+// Stores 8 values (chunk8: their index in the row, in eights) and, with the first of a K block, its four scale codes.
 __device__ __forceinline__ void fb_store(const FbActivations& a, const FbPlace& pl, int64_t chunk8, uint2 q,
                                          uint32_t word) {
-  // chunk8: index of the 8-value chunk in the row.
-  if (pl.prow < 0 || pl.prow >= a.rows_pad || pl.slot < 0 || pl.slot >= a.slots) return;
+  if (pl.slot < 0 || pl.slot >= a.slots) return;
   const int64_t kb = chunk8 >> 4;
   const int c = (int)(chunk8 & 15);
-  uint8_t* d = a.x8 + (kb * a.rows_pad + pl.prow) * 128 + (((c >> 1) ^ (int)(pl.prow & 7)) << 4) + (c & 1) * 8;
+  const bool pair = fb_is_pair(a.nt);
+  uint8_t* rec = a.x8 + (pl.slot * a.kblocks + kb) * fb_record_bytes(a.nt);
+  int row = pl.in_tile, part = 0;
+  if (pair) {
+    const int nn = (pl.n + 15) / 16 * 16, n0 = min(nn, 128) / 2, n1 = nn / 2 - n0;
+    if (row < 2 * n0) {
+      part = row >= n0;
+      row -= part * n0;
+    } else {
+      row -= 2 * n0;
+      part = row >= n1;
+      row += n0 - part * n1;
+    }
+  }
+  uint8_t* d = rec + part * fb_part_bytes(a.nt) + row * 128 + (((c >> 1) ^ (row & 7)) << 4) + (c & 1) * 8;
   *reinterpret_cast<uint2*>(d) = q;
   if (c == 0) {
-    const int apt = fb_atoms_per_tile(a.nt), t = pl.in_tile & 127;
-    uint8_t* s = a.atoms + ((pl.slot * a.kblocks + kb) * apt + (pl.in_tile >> 7)) * kFbAtom + (t & 31) * 16 + (t >> 5) * 4;
+    const int t = pl.in_tile & 127;
+    uint8_t* s = rec + fb_part_rows(pl.n, pair) * 128 + (pl.in_tile >> 7) * kFbAtom + (t & 31) * 16 + (t >> 5) * 4;
     *reinterpret_cast<uint32_t*>(s) = word;
+    if (pair) *reinterpret_cast<uint32_t*>(s + fb_part_bytes(a.nt)) = word;
   }
 }
 
@@ -150,6 +172,8 @@ struct FbGemmParams {
   float* partials;     // [grid][2][128 * nt]
   int* counters;       // [grid][8], zero on entry and left zero
 };
+// Device addresses of the product kernels' status record and wait limit (the current device's).
+cudaError_t fb_status_symbols(void** status, void** limit);
 // Token-tile sizes the kernel is built for.
 int fb_tile_for(int64_t expected_rows);
 uint32_t fb_gemm_smem(int nt, int experts, int stages);

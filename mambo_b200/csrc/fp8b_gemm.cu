@@ -16,8 +16,13 @@
 // CTA (stream-K), so every CTA ends at the same time. A tile that several CTAs
 // share is summed in K order by whichever arrives last: nothing waits.
 //
-// Warps: 0 weights producer, 1 MMA, 2 activations producer, 3 idle, then the
+// Warps: 0 weights producer, 1 and 3 MMA, 2 activations producer, then the
 // epilogue warps, one per TMEM lane quadrant (and per half of the columns).
+//
+// Compiled as a whole program of its own (no relocatable device code): the
+// compiler takes setmaxnreg into account only then, and the pair kernel's
+// epilogue keeps 128 sums a thread. So it has its own device status.
+#define MAMBO_OWN_DEVICE_STATUS
 #include "fp8b.cuh"
 #include "iq3s_tm.cuh"
 #include "kernels.cuh"
@@ -28,24 +33,29 @@ namespace mambo {
 namespace {
 
 constexpr int kMaxStagesB = 12;
+constexpr int kPairTokens = kFbPairTokens;
 
-template <int NT>
+// kPair: CTA pairs. A tile is 256 weight rows (a row tile per CTA) x NT tokens; each CTA loads half of the
+// tokens and the pair's tensor cores read both halves. The tile's tokens are two MMAs (the first 128, the
+// rest) with D buffers and epilogue warps of their own: a buffer is then free for the next block but one
+// while the other half's MMAs run.
+template <int NT, bool kPair>
 struct FbCfg {
-  static constexpr int kEpiWarps = NT > 64 ? 8 : 4;
-  static constexpr int kCols = NT > 64 ? NT / 2 : NT;  // columns of an epilogue warp
-  static constexpr int kD = NT > 64 ? 3 : 4;           // D buffers
-  static constexpr uint32_t kDStride = NT;
-  static constexpr uint32_t kSfa = kD * kDStride;      // weights' scale factors, all 2^0
-  static constexpr uint32_t kSfb = kSfa + 16;          // activations' scale factors, 8 columns per D buffer
-  static constexpr uint32_t kTmem = kSfb + 8 * kD <= 128 ? 128 : kSfb + 8 * kD <= 256 ? 256 : 512;
+  static constexpr int kHalves = kPair ? 2 : 1;
+  static constexpr int kEpiWarps = 4 * kHalves;
+  static constexpr int kCols = kPair ? 128 : NT;  // columns of an epilogue warp
+  static constexpr int kD = kPair ? 2 : 4;        // D buffers (of each half)
+  static constexpr uint32_t kDStride = kPair ? 256 : NT;
+  // Scale factors: the weights' (all 2^0), and 8 columns of the activations' per D buffer. With 240 tokens
+  // they lie in the 16 columns that each 256-column half has left.
+  static constexpr uint32_t kSfa = kPair ? 496 : kD * kDStride;
+  static constexpr uint32_t kSfb = kPair ? 240 : kSfa + 16;
+  static constexpr uint32_t kTmem = kPair ? 512 : kSfb + 8 * kD <= 128 ? 128 : kSfb + 8 * kD <= 256 ? 256 : 512;
   static constexpr int kThreads = (4 + kEpiWarps) * 32;
   static constexpr int kApt = (NT + 127) / 128;
-  static constexpr uint32_t kXBytes = NT * 128u;
-  static constexpr uint32_t kStage = kFbRecord + kXBytes + kApt * kFbAtom;
-  static_assert(kStage % 512 == 0, "stage");
-  // Operand tiles start on 1024-byte boundaries: weights and tokens first, then all scale atoms.
-  static constexpr uint32_t kTiles = kFbRecord + kXBytes;
-  static_assert(kTiles % 1024 == 0, "swizzle atoms");
+  // A stage: the weight record and this CTA's part of the activation record, both on 1024-byte boundaries.
+  static constexpr uint32_t kStage = (kFbRecord + fb_part_bytes(NT) + 1023) / 1024 * 1024;
+  static_assert(kPair ? NT > 128 && NT <= 240 : NT <= 64, "scale factors need TMEM columns beside the D buffers");
 };
 
 constexpr uint32_t kFbBarBytes = 512;
@@ -100,13 +110,13 @@ struct FbWalk {
 // The tile's expert, row tile and tokens, from the prefix tables in shared memory.
 struct FbTile {
   int e, rt, row0, n;  // n tokens from row row0 of the expert's segment
-  int64_t prow, slot;
+  int64_t slot;
   int o;
 };
 struct FbCursor {
   const int* tiles;  // [experts + 1] first tile of each expert
   const int* offs;   // [experts + 1] clamped, non-decreasing
-  int experts, row_tiles, nt, e;
+  int experts, nt, e;
   __device__ __forceinline__ FbTile at(int tile) {
     while (e + 1 < experts && tile >= tiles[e + 1]) ++e;
     FbTile t;
@@ -115,15 +125,75 @@ struct FbCursor {
     const int count = offs[e + 1] - t.o;
     const int tt_n = fb_tiles(count, nt), tr = fb_tile_rows(count, tt_n);
     const int local = tile - tiles[e];
-    t.rt = local / tt_n;
+    t.rt = local / tt_n;  // row group: of the pair, in pairs
     const int tt = local - t.rt * tt_n;
     t.row0 = tt * tr;
     t.n = count - t.row0 < tr ? count - t.row0 : tr;
-    t.prow = fb_row_start(t.o, e) + t.row0;
     t.slot = fb_slot_start(t.o, e, nt) + tt;
     return t;
   }
 };
+
+// Bounded waits for a barrier phase, by one thread and by a whole warp (which agrees on the outcome). The main loop
+// is a chain of such waits, most of them for a phase that is over already: that path is one try and a vote inline
+// (47 + 20 clocks); with the loop around it inline the same wait took 260.
+__device__ __forceinline__ bool fb_wait_slow(uint32_t bar, uint32_t parity, int site) {
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_bounded(bar, parity, site);
+}
+__device__ __forceinline__ bool fb_wait(uint32_t bar, uint32_t parity, int site) {
+  return mbar_try_wait(bar, parity) || fb_wait_slow(bar, parity, site);
+}
+__device__ __forceinline__ bool fb_warp_wait(uint32_t bar, uint32_t parity, int site) {
+  if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xFFFFFFFFu, fb_wait_slow(bar, parity, site));
+}
+
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xFFFFFFFFu, v, 0); }
+
+// Arrival on a barrier of the pair's other CTA. What it announces is not memory that this thread wrote: bulk copies
+// that completed on a barrier, and TMEM loads that were waited for. So it needs no release at cluster scope, which
+// holds the thread up until its stores are visible there: with it a K block took 1.5 times as long (prefill of
+// 2048 x 14336 x 4096: 277 us, without 190 us).
+__device__ __forceinline__ void arrive_remote(uint32_t remote_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote_bar) : "memory");
+}
+// Packed FP32 pairs in 64-bit registers.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+// N (16 or 32) consecutive TMEM columns of this lane, and the wait that makes them readable (it names the registers,
+// so that no use is scheduled before it). The wait is for all of the thread's loads.
+template <int N>
+__device__ __forceinline__ void ld_cols(uint32_t taddr, uint32_t (&r)[N]) {
+  static_assert(N == 16 || N == 32, "16 or 32 columns");
+  if constexpr (N == 16) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+  } else {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr));
+  }
+}
+template <int N>
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[N]) {
+  if constexpr (N == 16) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) : : "memory");
+  } else {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) : : "memory");
+  }
+}
 
 // After a wait gave up: time for the bulk copies in flight to land before the CTA leaves its shared memory.
 __device__ __forceinline__ void settle_copies() {
@@ -132,49 +202,80 @@ __device__ __forceinline__ void settle_copies() {
 }
 
 // D[tmem] (+)= A[smem] x (B[smem] * 2^sfb)^T, block scaled (A's factors are 2^0), issued by one thread.
+template <bool kPair>
 __device__ __forceinline__ void mma_mx_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
                                           uint32_t tmem_sfa, uint32_t tmem_sfb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
-          tmem_d),
-      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb));
+  if constexpr (kPair) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
+            tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb));
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
+            tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb));
+  }
+}
+// A scale-factor atom from shared memory to 4 TMEM columns; for a pair each CTA's atom to its own TMEM.
+template <bool kPair>
+__device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t sdesc) {
+  if constexpr (kPair) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+  } else {
+    tc::cp_32x128b_warpx4(taddr, sdesc);
+  }
 }
 
 }  // namespace
 
-template <int NT>
-__global__ void __launch_bounds__(FbCfg<NT>::kThreads, 1) fb_gemm_kernel(const __grid_constant__ FbGemmParams p) {
-  using C = FbCfg<NT>;
+template <int NT, bool kPair>
+__global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(const __grid_constant__ FbGemmParams p) {
+  using C = FbCfg<NT, kPair>;
+  constexpr uint16_t kBoth = 0x3;  // CTA mask of a pair
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* tiles0 = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int S = p.stages;
-  uint8_t* atoms0 = tiles0 + (size_t)S * C::kTiles;
-  int* tile_start = reinterpret_cast<int*>(atoms0 + (size_t)S * C::kApt * kFbAtom);
+  int* tile_start = reinterpret_cast<int*>(tiles0 + (size_t)S * C::kStage);
   int* offs = tile_start + p.experts + 1;
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(tile_start) + fb_tables_bytes(p.experts));
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStagesB + 2 * 4 + 1);
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t kFull = bar0, kEmpty = bar0 + 8 * kMaxStagesB;
   const uint32_t kMdone = bar0 + 16 * kMaxStagesB, kEfree = kMdone + 8 * 4, kEdone = kEfree + 8 * 4;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  static_assert(C::kD * C::kHalves <= 4, "barriers");
+  // Values that the whole warp shares are broadcast from lane 0, so that the compiler keeps them, and what the MMAs
+  // take as operands, in uniform registers.
+  const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int KB = p.act.kblocks;
+  const int rank = kPair ? (int)cluster_ctarank() : 0;
+  const int row_groups = kPair ? (p.row_tiles + 1) / 2 : p.row_tiles;
+  // Rank 0's copy of a barrier: it issues the pair's MMAs, rank 1 arrives there.
+  auto lead = [&](uint32_t bar) { return mapa_shared(bar, 0); };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(kFull + 8 * s, 2);
-      mbar_init(kEmpty + 8 * s, 1);
+      // Both producers, and in rank 0 of a pair the other CTA's landed operands.
+      mbar_init(kFull + 8 * s, kPair && rank == 0 ? 3 : 2);
+      mbar_init(kEmpty + 8 * s, kPair ? 2 : 1);  // a pair's two issuers
     }
-    for (int d = 0; d < C::kD; ++d) {
+    for (int d = 0; d < C::kD * C::kHalves; ++d) {  // buffer d of half h: barrier h * kD + d
       mbar_init(kMdone + 8 * d, 1);
-      mbar_init(kEfree + 8 * d, C::kEpiWarps);
+      mbar_init(kEfree + 8 * d, kPair ? 8 : 4);
     }
     mbar_init(kEdone, C::kEpiWarps);
     fence_barrier_init();
   }
   if (warp == 1) {
-    tc::alloc(smem_u32(tmem_slot), C::kTmem);
-    tc::relinquish();
+    if constexpr (kPair) {
+      tc::alloc_pair(smem_u32(tmem_slot), C::kTmem);
+      tc::relinquish_pair();
+    } else {
+      tc::alloc(smem_u32(tmem_slot), C::kTmem);
+      tc::relinquish();
+    }
   }
   if (warp == 0) {
     // Row and tile prefix of the experts. Offsets are clamped to [0, rows] and
@@ -200,7 +301,7 @@ __global__ void __launch_bounds__(FbCfg<NT>::kThreads, 1) fb_gemm_kernel(const _
         }
         int before = __shfl_up_sync(0xFFFFFFFFu, o, 1);
         if (lane == 0) before = prev;
-        int t = fb_tiles(o - before, NT) * p.row_tiles;
+        int t = fb_tiles(o - before, NT) * row_groups;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
           const int up = __shfl_up_sync(0xFFFFFFFFu, t, d);
@@ -215,7 +316,7 @@ __global__ void __launch_bounds__(FbCfg<NT>::kThreads, 1) fb_gemm_kernel(const _
       }
     } else if (lane == 0) {
       tile_start[0] = 0;
-      tile_start[1] = fb_tiles((int)p.rows, NT) * p.row_tiles;
+      tile_start[1] = fb_tiles((int)p.rows, NT) * row_groups;
       offs[0] = 0;
       offs[1] = (int)p.rows;
     }
@@ -223,7 +324,7 @@ __global__ void __launch_bounds__(FbCfg<NT>::kThreads, 1) fb_gemm_kernel(const _
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = (uint32_t)uniform((int)*tmem_slot);
   // The weights' MMA scale factors: 2^0 in every lane and byte.
   if (warp >= 4 && warp < 8) {
     tc::st_x4(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + C::kSfa, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
@@ -231,11 +332,16 @@ __global__ void __launch_bounds__(FbCfg<NT>::kThreads, 1) fb_gemm_kernel(const _
   }
   tc::fence_before_sync();
   __syncthreads();
+  if constexpr (kPair) cluster_sync_all();  // both CTAs' barriers and TMEM are ready before any remote use
   tc::fence_after_sync();
 
-  FbWalk walk(tile_start[p.experts], KB, (int)blockIdx.x, (int)gridDim.x);
-  FbCursor cur{tile_start, offs, p.experts, p.row_tiles, NT, 0};
+  FbWalk walk(uniform(tile_start[p.experts]), KB, (int)blockIdx.x / (kPair ? 2 : 1), (int)gridDim.x / (kPair ? 2 : 1));
+  FbCursor cur{tile_start, offs, p.experts, NT, 0};
 
+  // Register split of the pair kernel, launched with 168 a thread (384 threads): 128 x 56 + 256 x 224 = 384 x 168.
+  // Each instruction opens its own branch, so that the compiler knows every role's count.
+  if (warp < 4) {
+    if constexpr (kPair) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp == 0) {
     // -------------------------------------------------------------- weights producer
     if (lane == 0) {
@@ -245,15 +351,22 @@ __global__ void __launch_bounds__(FbCfg<NT>::kThreads, 1) fb_gemm_kernel(const _
       bool ok = true;
       while (ok && walk.next()) {
         const FbTile t = cur.at(walk.tile);
-        const uint8_t* rec = p.packed + (((int64_t)t.e * p.row_tiles + t.rt) * KB) * kFbRecord;
+        const int rt = kPair ? 2 * t.rt + rank : t.rt;
+        const bool have = !kPair || rt < p.row_tiles;  // the second row tile of the last pair may not exist
+        const uint8_t* rec = p.packed + (((int64_t)t.e * p.row_tiles + rt) * KB) * kFbRecord;
         for (int kb = walk.kb0; kb < walk.kb1; ++kb, ++it) {
-          if (it >= S && !mbar_wait_bounded(kEmpty + 8 * s, ph ^ 1, kSiteFbEmpty)) {
+          if (it >= S && !fb_wait(kEmpty + 8 * s, ph ^ 1, kSiteFbEmpty)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(kFull + 8 * s, kFbRecord);
-          const uint32_t dst = smem_u32(tiles0 + (size_t)s * C::kTiles);
-          if (p.evict_weights) {
+          const uint32_t dst = smem_u32(tiles0 + (size_t)s * C::kStage);
+          if (have) {
+            mbar_arrive_expect_tx(kFull + 8 * s, kFbRecord);
+          } else {
+            mbar_arrive(kFull + 8 * s);  // whatever the stage holds: these rows are not stored
+          }
+          if (!have) {
+          } else if (p.evict_weights) {
             bulk_load_hint(dst, rec + (int64_t)kb * kFbRecord, kFbRecord, kFull + 8 * s, policy);
           } else {
             bulk_load(dst, rec + (int64_t)kb * kFbRecord, kFbRecord, kFull + 8 * s);
@@ -276,20 +389,17 @@ __global__ void __launch_bounds__(FbCfg<NT>::kThreads, 1) fb_gemm_kernel(const _
       bool ok = true;
       while (ok && walk.next()) {
         const FbTile t = cur.at(walk.tile);
-        const uint32_t xb = (uint32_t)((t.n + 7) / 8) * 1024u;
-        const uint8_t* x = p.act.x8 + t.prow * 128;
-        const uint8_t* sf = p.act.atoms + t.slot * KB * (C::kApt * kFbAtom);
+        const uint32_t bytes = (uint32_t)fb_part_rows(t.n, kPair) * 128u + C::kApt * kFbAtom;
+        const uint8_t* x = p.act.x8 + t.slot * KB * fb_record_bytes(NT) + (kPair ? rank * fb_part_bytes(NT) : 0u);
         for (int kb = walk.kb0; kb < walk.kb1; ++kb, ++it) {
-          if (it >= S && !mbar_wait_bounded(kEmpty + 8 * s, ph ^ 1, kSiteFbEmpty)) {
+          if (it >= S && !fb_wait(kEmpty + 8 * s, ph ^ 1, kSiteFbEmpty)) {
             ok = false;
             break;
           }
           const uint32_t full = kFull + 8 * s;
-          mbar_arrive_expect_tx(full, xb + C::kApt * kFbAtom);
-          bulk_load(smem_u32(tiles0 + (size_t)s * C::kTiles) + kFbRecord, x + (int64_t)kb * p.act.rows_pad * 128, xb,
+          mbar_arrive_expect_tx(full, bytes);
+          bulk_load(smem_u32(tiles0 + (size_t)s * C::kStage) + kFbRecord, x + (int64_t)kb * fb_record_bytes(NT), bytes,
                     full);
-          bulk_load(smem_u32(atoms0 + (size_t)s * C::kApt * kFbAtom), sf + (int64_t)kb * (C::kApt * kFbAtom),
-                    C::kApt * kFbAtom, full);
           if (++s == S) {
             s = 0;
             ph ^= 1;
@@ -299,92 +409,165 @@ __global__ void __launch_bounds__(FbCfg<NT>::kThreads, 1) fb_gemm_kernel(const _
       if (!ok) settle_copies();
     }
     __syncwarp();
-  } else if (warp == 1) {
+  } else {
     // -------------------------------------------------------------- MMA
-    int it = 0, s = 0, db = 0;
-    uint32_t ph = 0, dph = 0;
-    bool ok = true;
-    while (ok && walk.next()) {
-      const FbTile t = cur.at(walk.tile);
-      const uint32_t idesc = tc::idesc_mx_e4m3(128, (t.n + 15) / 16 * 16, 0, 0);
-      for (int kb = walk.kb0; kb < walk.kb1; ++kb, ++it) {
-        ok = tm::warp_wait(kFull + 8 * s, ph, kSiteFbFull);
-        if (ok && it >= C::kD) ok = tm::warp_wait(kEfree + 8 * db, dph ^ 1, kSiteFbEmpty);
-        if (!ok) break;
-        tc::fence_after_sync();
-        const uint32_t wt = smem_u32(tiles0 + (size_t)s * C::kTiles);
-        const uint32_t at = smem_u32(atoms0 + (size_t)s * C::kApt * kFbAtom);
-        const uint64_t adesc = tc::smem_desc_sw128(wt, 1024u), bdesc = tc::smem_desc_sw128(wt + kFbRecord, 1024u);
-        const uint32_t d = tmem + (uint32_t)db * C::kDStride, sfb = tmem + C::kSfb + 8u * (uint32_t)db;
-        if (tm::elect_one()) {
-#pragma unroll
-          for (int a = 0; a < C::kApt; ++a)
-            tc::cp_32x128b_warpx4(sfb + 4u * a, tc::smem_desc(at + a * kFbAtom, 128u, 128u));
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_mx_ss(d, adesc + (uint64_t)(2 * j), bdesc + (uint64_t)(2 * j), idesc | ((uint32_t)j << 4),
-                      tmem + C::kSfa, sfb, j != 0);
-          tc::commit(kEmpty + 8 * s);
-          tc::commit(kMdone + 8 * db);
+    // Two issuing warps, 1 and 3, each with D buffers of its own: of a pair's tile each issues one half, alone they
+    // take the K blocks in turn. A K block costs its issuer some 400 clocks (two waits, the scale copy, four MMAs,
+    // two commits), which alone would pace the kernel.
+    const int who = warp >> 1;
+    if (kPair && rank == 1 && who == 0) {
+      // Rank 1 of a pair: its operands have landed, told to rank 0, which issues the MMAs of both.
+      if (lane == 0) {
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        while (ok && walk.next()) {
+          for (int kb = walk.kb0; kb < walk.kb1; ++kb) {
+            ok = fb_wait(kFull + 8 * s, ph, kSiteFbFull);
+            if (!ok) break;
+            arrive_remote(lead(kFull + 8 * s));
+            if (++s == S) {
+              s = 0;
+              ph ^= 1;
+            }
+          }
         }
-        __syncwarp();
+      }
+      __syncwarp();
+    }
+    int s = 0, use = 0, it = 0;  // use: D buffers taken by this warp so far
+    uint32_t ph = 0;
+    bool ok = !kPair || rank == 0;
+    while (ok && walk.next()) {
+      const int n_tile = uniform(cur.at(walk.tile).n);
+      const int nn = (n_tile + 15) / 16 * 16;
+      const int n = !kPair ? nn : who == 0 ? (nn < 128 ? nn : 128) : nn - 128;
+      const uint32_t idesc = tc::idesc_mx_e4m3(kPair ? 256 : 128, n, 0, 0);
+      // Scale codes follow the rows that this CTA holds; the pair's second MMA starts at their row 64.
+      const uint32_t sf_at = kFbRecord + (uint32_t)fb_part_rows(n_tile, kPair) * 128u + (kPair ? who * kFbAtom : 0u);
+      const uint32_t b_at = kFbRecord + (kPair ? who * 64u * 128u : 0u);
+      for (int kb = walk.kb0; ok && kb < walk.kb1; ++kb, ++it) {
+        if (kPair ? n > 0 : (it & 1) == who) {
+          // Buffer `use % n`, and its barriers: of a pair, kD buffers per half; alone every other buffer of kD.
+          constexpr int kMine = kPair ? C::kD : C::kD / 2;
+          const int db = kPair ? use % kMine : use % kMine * 2 + who;
+          const uint32_t bar = 8u * (uint32_t)(kPair ? who * C::kD + db : db);
+          ok = fb_warp_wait(kFull + 8 * s, ph, kSiteFbFull);
+          if (ok && use >= kMine) ok = fb_warp_wait(kEfree + bar, (uint32_t)(use / kMine - 1) & 1u, kSiteFbEmpty);
+          if (!ok) break;
+          ++use;
+          tc::fence_after_sync();
+          const uint32_t wt = smem_u32(tiles0) + (uint32_t)s * C::kStage;
+          const uint64_t adesc = tc::smem_desc_sw128(wt, 1024u), bdesc = tc::smem_desc_sw128(wt + b_at, 1024u);
+          // The scale factors lie beside their D buffer: those of this buffer's last use are no longer read.
+          const uint32_t d = tmem + (uint32_t)db * C::kDStride + (kPair ? 128u * who : 0u);
+          const uint32_t sfb = tmem + C::kSfb + 8u * (uint32_t)db + (kPair ? 4u * who : 0u);
+          const uint64_t sdesc = tc::smem_desc(wt + sf_at, 128u, 128u);
+          if (tm::elect_one()) {
+            cp_scales<kPair>(sfb, sdesc);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              mma_mx_ss<kPair>(d, adesc + (uint64_t)(2 * j), bdesc + (uint64_t)(2 * j), idesc | ((uint32_t)j << 4),
+                               tmem + C::kSfa, sfb, j != 0);
+            if constexpr (kPair) {
+              tc::commit_pair(kMdone + bar, kBoth);
+              tc::commit_pair(kEmpty + 8 * s, kBoth);
+            } else {
+              tc::commit(kMdone + bar);
+              tc::commit(kEmpty + 8 * s);
+            }
+          }
+          __syncwarp();
+        } else if (kPair) {
+          // A tile of at most 128 tokens has no second half: the stage is released as if it had been read.
+          ok = fb_warp_wait(kFull + 8 * s, ph, kSiteFbFull);
+          if (!ok) break;
+          if (lane < 2) arrive_remote(mapa_shared(kEmpty + 8 * s, (uint32_t)lane));
+          __syncwarp();
+        }
         if (++s == S) {
           s = 0;
           ph ^= 1;
         }
-        if (++db == C::kD) {
-          db = 0;
-          dph ^= 1;
-        }
       }
     }
+    if (who == 0) {
     // Free the TMEM once every epilogue warp has read its last results.
-    mbar_wait_bounded(kEdone, 0, kSiteFbFull);
+    fb_wait(kEdone, 0, kSiteFbFull);
     __syncwarp();
     tc::fence_after_sync();
-    tc::dealloc(tmem, C::kTmem);
-  } else if (warp >= 4) {
+    if constexpr (kPair) {
+      tc::dealloc_pair(tmem, C::kTmem);
+    } else {
+      tc::dealloc(tmem, C::kTmem);
+    }
+    }
+  }
+  } else {
+    if constexpr (kPair) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // -------------------------------------------------------------- epilogue
     const int q = warp & 3, h = (warp - 4) >> 2;
     const int rl = 32 * q + lane;
     const int c0 = h * C::kCols;
     const uint32_t tq0 = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)c0;
-    float acc[C::kCols];
+    uint64_t acc2[C::kCols / 2];  // pairs of columns
+#pragma unroll
+    for (int i = 0; i < C::kCols / 2; ++i) acc2[i] = 0;
+    auto acc = [&](int c) {
+      return __uint_as_float((c & 1) ? (uint32_t)(acc2[c >> 1] >> 32) : (uint32_t)acc2[c >> 1]);
+    };
     pdl_wait();  // the output and the workspace may belong to the previous kernel
     pdl_launch_dependents();
+    const uint32_t efree0 = kPair ? lead(kEfree + 8 * h * C::kD) : 0u;
     int db = 0;
     uint32_t dph = 0;
     bool ok = true;
     while (ok && walk.next()) {
       const FbTile t = cur.at(walk.tile);
       const int cols = t.n - c0;  // this warp's valid columns (may be <= 0)
-      const float* sw = p.scales + (((int64_t)t.e * p.row_tiles + t.rt) * 2 + (q & 1)) * KB;
+      const int rt = kPair ? 2 * t.rt + rank : t.rt;
+      const bool have = !kPair || rt < p.row_tiles;
+      const float* sw = p.scales + (((int64_t)t.e * p.row_tiles + (have ? rt : 0)) * 2 + (q & 1)) * KB;
 #pragma unroll
-      for (int i = 0; i < C::kCols; ++i) acc[i] = 0.f;
+      for (int i = 0; i < C::kCols / 2; ++i) acc2[i] = 0;
+      if (cols <= 0) continue;  // this half's MMAs are not issued either
       float sv = 0.f;
       for (int kb = walk.kb0; kb < walk.kb1; ++kb) {
         if (kb == walk.kb0 || (kb & 31) == 0) sv = (kb & ~31) + lane < KB ? __ldg(sw + (kb & ~31) + lane) : 0.f;
         const float w = __shfl_sync(0xFFFFFFFFu, sv, kb & 31);
-        ok = tm::warp_wait(kMdone + 8 * db, dph, kSiteFbFull);
+        ok = fb_warp_wait(kMdone + 8 * (h * C::kD + db), dph, kSiteFbFull);
         if (!ok) break;
         tc::fence_after_sync();
         const uint32_t tq = tq0 + (uint32_t)db * C::kDStride;
+        const uint64_t w2 = pack2(w, w);
+        // Chunks of columns: the next chunk's load is in flight while this one's values are added, and the buffer is
+        // released once its last chunk is in registers.
+        constexpr int kCh = C::kCols < 32 ? C::kCols : 32;
+        uint32_t v[2][kCh];
+        ld_cols(tq, v[0]);
 #pragma unroll
-        for (int b = 0; b < C::kCols; b += 16) {
+        for (int b = 0; b < C::kCols; b += kCh) {
           if (b < cols) {
-            const uint32_t off[2] = {(uint32_t)b, (uint32_t)b + 8u};
-            float v[2][8];
-            tc::ld_x8_multi<2>(tq, off, v);
+            uint32_t(&x)[kCh] = v[(b / kCh) & 1];
+            wait_ld(x);
+            if (b + kCh < C::kCols && b + kCh < cols) {
+              ld_cols(tq + b + kCh, v[(b / kCh + 1) & 1]);
+            } else {
+              tc::fence_before_sync();
+              __syncwarp();
+              if (lane == 0) {
+                if (kPair && rank != 0) {
+                  arrive_remote(efree0 + 8 * db);
+                } else {
+                  mbar_arrive(kEfree + 8 * (h * C::kD + db));
+                }
+              }
+            }
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int i = 0; i < 8; i += 2)
-                fma2(acc[b + 8 * j + i], acc[b + 8 * j + i + 1], v[j][i], v[j][i + 1], w, w);
+            for (int i = 0; i < kCh / 2; ++i)
+              acc2[b / 2 + i] = fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), w2, acc2[b / 2 + i]);
           }
         }
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(kEfree + 8 * db);
         if (++db == C::kD) {
           db = 0;
           dph ^= 1;
@@ -399,16 +582,16 @@ __global__ void __launch_bounds__(FbCfg<NT>::kThreads, 1) fb_gemm_kernel(const _
         constexpr int kQuads = NT / 4;
         auto part = [&](int cta) {
           // Slot 1 holds the part that starts its tile (the CTA's last tile), slot 0 the others.
-          return reinterpret_cast<float4*>(p.partials) +
-                 (((int64_t)cta * 2 + (cta == first ? 1 : 0)) * kQuads + c0 / 4) * 128 + rl;
+          const int64_t at = kPair ? cta * 2 + rank : cta;
+          return reinterpret_cast<float4*>(p.partials) + ((at * 2 + (cta == first ? 1 : 0)) * kQuads + c0 / 4) * 128 + rl;
         };
         float4* mine = part(walk.cl);
 #pragma unroll
         for (int c = 0; c < C::kCols; c += 4)
-          if (c < cols) __stcg(mine + (c / 4) * 128, make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]));
+          if (c < cols) __stcg(mine + (c / 4) * 128, make_float4(acc(c), acc(c + 1), acc(c + 2), acc(c + 3)));
         __threadfence();
         __syncwarp();
-        int* counter = p.counters + first * 8 + (warp - 4);
+        int* counter = p.counters + (kPair ? first * 2 + rank : first) * 8 + (warp - 4);
         int done = 0;
         if (lane == 0) done = atomic_add_acq_rel_gpu(counter, 1) == last - first;
         done = __shfl_sync(0xFFFFFFFFu, done, 0);
@@ -416,34 +599,32 @@ __global__ void __launch_bounds__(FbCfg<NT>::kThreads, 1) fb_gemm_kernel(const _
         if (lane == 0) *counter = 0;  // all parts are in: zero again for the next launch
         __threadfence();
 #pragma unroll
-        for (int c = 0; c < C::kCols; ++c) acc[c] = 0.f;
+        for (int c = 0; c < C::kCols / 2; ++c) acc2[c] = 0;
         for (int cta = first; cta <= last; ++cta) {
           const float4* src = part(cta);
 #pragma unroll
           for (int c = 0; c < C::kCols; c += 4) {
             if (c < cols) {
               const float4 v = __ldcg(src + (c / 4) * 128);
-              acc[c] += v.x;
-              acc[c + 1] += v.y;
-              acc[c + 2] += v.z;
-              acc[c + 3] += v.w;
+              acc2[c / 2] = pack2(acc(c) + v.x, acc(c + 1) + v.y);
+              acc2[c / 2 + 1] = pack2(acc(c + 2) + v.z, acc(c + 3) + v.w);
             }
           }
         }
       }
-      const int row = t.rt * 128 + rl;
+      const int row = rt * 128 + rl;
       if (row < p.n_rows) {
         const int64_t at = ((int64_t)t.o + t.row0 + c0) * p.ldo + row;
         if (p.out_bf16) {
           __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.out) + at;
 #pragma unroll
           for (int c = 0; c < C::kCols; ++c)
-            if (c < cols) o[(int64_t)c * p.ldo] = __float2bfloat16_rn(acc[c]);
+            if (c < cols) o[(int64_t)c * p.ldo] = __float2bfloat16_rn(acc(c));
         } else {
           float* o = reinterpret_cast<float*>(p.out) + at;
 #pragma unroll
           for (int c = 0; c < C::kCols; ++c)
-            if (c < cols) o[(int64_t)c * p.ldo] = acc[c];
+            if (c < cols) o[(int64_t)c * p.ldo] = acc(c);
         }
       }
     }
@@ -452,34 +633,42 @@ __global__ void __launch_bounds__(FbCfg<NT>::kThreads, 1) fb_gemm_kernel(const _
     if (lane == 0) mbar_arrive(kEdone);
     __syncwarp();
   }
+  // Neither CTA of a pair leaves while the other may still use its shared memory or TMEM.
+  if constexpr (kPair) cluster_sync_all();
 }
 
 // --------------------------------------------------------------------------
 // Host side
 // --------------------------------------------------------------------------
 namespace {
-template <int NT>
+
+template <int NT, bool kPair>
 uint32_t smem_of(int experts, int stages) {
-  return 1024 + (uint32_t)stages * (FbCfg<NT>::kTiles + FbCfg<NT>::kApt * kFbAtom) + fb_tables_bytes(experts) +
-         kFbBarBytes;
+  using C = FbCfg<NT, kPair>;
+  return 1024 + (uint32_t)stages * C::kStage + fb_tables_bytes(experts) + kFbBarBytes;
 }
-template <int NT>
+template <int NT, bool kPair>
 cudaError_t launch_nt(const FbGemmParams& p, int grid, cudaStream_t stream) {
-  const uint32_t smem = smem_of<NT>(p.experts, p.stages);
-  const void* k = (const void*)fb_gemm_kernel<NT>;
+  const uint32_t smem = smem_of<NT, kPair>(p.experts, p.stages);
+  const void* k = (const void*)fb_gemm_kernel<NT, kPair>;
   cudaError_t e = ensure_smem_attribute(k, smem);
   if (e != cudaSuccess) return e;
-  return launch_pdl(k, dim3(grid), dim3(FbCfg<NT>::kThreads), smem, stream, p);
+  return launch_pdl_cluster(k, dim3(grid), dim3(FbCfg<NT, kPair>::kThreads), smem, stream, kPair ? 2 : 1, p);
 }
+
 }  // namespace
 
 int fb_tile_for(int64_t expected_rows) {
-  return expected_rows <= 16 ? 16 : expected_rows <= 32 ? 32 : expected_rows <= 64 ? 64 : 128;
+  return expected_rows <= 16 ? 16 : expected_rows <= 32 ? 32 : expected_rows <= 64 ? 64 : kPairTokens;
 }
 
 uint32_t fb_gemm_smem(int nt, int experts, int stages) {
-  return nt == 16 ? smem_of<16>(experts, stages) : nt == 32 ? smem_of<32>(experts, stages)
-         : nt == 64 ? smem_of<64>(experts, stages) : smem_of<128>(experts, stages);
+  switch (nt) {
+    case 16: return smem_of<16, false>(experts, stages);
+    case 32: return smem_of<32, false>(experts, stages);
+    case 64: return smem_of<64, false>(experts, stages);
+    default: return smem_of<kPairTokens, true>(experts, stages);
+  }
 }
 
 int fb_gemm_stages(int nt, int experts, int smem_optin) {
@@ -488,15 +677,20 @@ int fb_gemm_stages(int nt, int experts, int smem_optin) {
   return s;
 }
 
-int fb_gemm_grid(int, int sms) { return sms; }
+cudaError_t fb_status_symbols(void** status, void** limit) {
+  cudaError_t e = cudaGetSymbolAddress(status, g_device_status);
+  return e == cudaSuccess ? cudaGetSymbolAddress(limit, g_wait_limit_ns) : e;
+}
+
+int fb_gemm_grid(int nt, int sms) { return nt == kPairTokens ? sms / 2 * 2 : sms; }
 size_t fb_partial_bytes(int nt, int sms) { return (size_t)sms * 2 * 128 * nt * sizeof(float); }
 
 cudaError_t launch_fb_gemm(const FbGemmParams& p, int grid, cudaStream_t stream) {
   switch (p.act.nt) {
-    case 16: return launch_nt<16>(p, grid, stream);
-    case 32: return launch_nt<32>(p, grid, stream);
-    case 64: return launch_nt<64>(p, grid, stream);
-    default: return launch_nt<128>(p, grid, stream);
+    case 16: return launch_nt<16, false>(p, grid, stream);
+    case 32: return launch_nt<32, false>(p, grid, stream);
+    case 64: return launch_nt<64, false>(p, grid, stream);
+    default: return launch_nt<kPairTokens, true>(p, grid, stream);
   }
 }
 
