@@ -33,7 +33,7 @@ constexpr uint32_t kFbAtom = 512u;           // bytes of a scale-factor atom (12
 constexpr int kFbMaxExperts = 1024;
 
 // Tokens of a tile above which CTA pairs work on it (and the largest tile).
-constexpr int kFbPairTokens = 240;
+constexpr int kFbPairTokens = 224;
 
 struct FbActivations {
   uint8_t* x8;    // [slots][kblocks][record]
@@ -51,8 +51,10 @@ __host__ __device__ constexpr uint32_t fb_part_bytes(int nt) {
 __host__ __device__ constexpr uint32_t fb_record_bytes(int nt) { return (fb_is_pair(nt) ? 2 : 1) * fb_part_bytes(nt); }
 __host__ __device__ inline int64_t fb_slots(int64_t rows, int64_t experts, int nt) { return rows / nt + experts; }
 __host__ __device__ inline int64_t fb_slot_start(int o, int e, int nt) { return o / nt + e; }
+// A pair's tile of n tokens is two MMAs: the first takes this many tokens (a multiple of 16), the second the rest.
+__host__ __device__ inline int fb_split(int n) { return ((n + 15) / 16 + 1) / 2 * 16; }
 // Rows that a CTA holds of a tile of n tokens, before its scale codes: alone all (in groups of 8), of a pair half of
-// each MMA's N, the first MMA taking min(128, n) tokens rounded up to 16 and the second the rest.
+// each MMA's N (rounded up to 16).
 __host__ __device__ inline int fb_part_rows(int n, bool pair) { return pair ? (n + 15) / 16 * 8 : (n + 7) / 8 * 8; }
 // A segment of `count` rows is cut into equal tiles of at most nt tokens, a multiple of 16 each.
 __host__ __device__ inline int fb_tiles(int count, int nt) { return (count + nt - 1) / nt; }
@@ -84,23 +86,19 @@ __device__ __forceinline__ void fb_store(const FbActivations& a, const FbPlace& 
   const int c = (int)(chunk8 & 15);
   const bool pair = fb_is_pair(a.nt);
   uint8_t* rec = a.x8 + (pl.slot * a.kblocks + kb) * fb_record_bytes(a.nt);
-  int row = pl.in_tile, part = 0;
+  int row = pl.in_tile, part = 0, half = 0, t = pl.in_tile;  // t: place among its MMA's tokens
   if (pair) {
-    const int nn = (pl.n + 15) / 16 * 16, n0 = min(nn, 128) / 2, n1 = nn / 2 - n0;
-    if (row < 2 * n0) {
-      part = row >= n0;
-      row -= part * n0;
-    } else {
-      row -= 2 * n0;
-      part = row >= n1;
-      row += n0 - part * n1;
-    }
+    const int nn = (pl.n + 15) / 16 * 16, n0 = fb_split(pl.n), n1 = nn - n0;
+    half = t >= n0;
+    t -= half * n0;
+    const int per = (half ? n1 : n0) / 2;
+    part = t >= per;
+    row = t - part * per + half * (n0 / 2);
   }
   uint8_t* d = rec + part * fb_part_bytes(a.nt) + row * 128 + (((c >> 1) ^ (row & 7)) << 4) + (c & 1) * 8;
   *reinterpret_cast<uint2*>(d) = q;
   if (c == 0) {
-    const int t = pl.in_tile & 127;
-    uint8_t* s = rec + fb_part_rows(pl.n, pair) * 128 + (pl.in_tile >> 7) * kFbAtom + (t & 31) * 16 + (t >> 5) * 4;
+    uint8_t* s = rec + fb_part_rows(pl.n, pair) * 128 + half * kFbAtom + (t & 31) * 16 + (t >> 5) * 4;
     *reinterpret_cast<uint32_t*>(s) = word;
     if (pair) *reinterpret_cast<uint32_t*>(s + fb_part_bytes(a.nt)) = word;
   }

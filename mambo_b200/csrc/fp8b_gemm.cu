@@ -23,6 +23,8 @@
 // compiler takes setmaxnreg into account only then, and the pair kernel's
 // epilogue keeps 128 sums a thread. So it has its own device status.
 #define MAMBO_OWN_DEVICE_STATUS
+#include <type_traits>
+
 #include "fp8b.cuh"
 #include "iq3s_tm.cuh"
 #include "kernels.cuh"
@@ -33,29 +35,27 @@ namespace mambo {
 namespace {
 
 constexpr int kMaxStagesB = 12;
-constexpr int kPairTokens = kFbPairTokens;
 
 // kPair: CTA pairs. A tile is 256 weight rows (a row tile per CTA) x NT tokens; each CTA loads half of the
-// tokens and the pair's tensor cores read both halves. The tile's tokens are two MMAs (the first 128, the
-// rest) with D buffers and epilogue warps of their own: a buffer is then free for the next block but one
-// while the other half's MMAs run.
+// tokens and the pair's tensor cores read both halves. The tile's tokens are two MMAs of up to 112, each with D
+// buffers and epilogue warps of its own: a buffer's way through the epilogue then has the time of three other MMAs
+// (of one, as a single MMA of 224). 112 sums and two chunks of 32 loaded values are what an epilogue thread can hold:
+// with 2 x 128 sums it spilled, and a K block took 10 % longer.
 template <int NT, bool kPair>
 struct FbCfg {
   static constexpr int kHalves = kPair ? 2 : 1;
   static constexpr int kEpiWarps = 4 * kHalves;
-  static constexpr int kCols = kPair ? 128 : NT;  // columns of an epilogue warp
-  static constexpr int kD = kPair ? 2 : 4;        // D buffers (of each half)
-  static constexpr uint32_t kDStride = kPair ? 256 : NT;
-  // Scale factors: the weights' (all 2^0), and 8 columns of the activations' per D buffer. With 240 tokens
-  // they lie in the 16 columns that each 256-column half has left.
-  static constexpr uint32_t kSfa = kPair ? 496 : kD * kDStride;
-  static constexpr uint32_t kSfb = kPair ? 240 : kSfa + 16;
-  static constexpr uint32_t kTmem = kPair ? 512 : kSfb + 8 * kD <= 128 ? 128 : kSfb + 8 * kD <= 256 ? 256 : 512;
+  static constexpr int kCols = NT / kHalves;  // columns of an epilogue warp
+  static constexpr int kD = kPair ? 2 : 4;    // D buffers (of each half), kCols columns each
+  // Scale factors: the weights' (all 2^0), and 4 columns of the activations' per D buffer.
+  static constexpr uint32_t kSfa = kHalves * kD * kCols;
+  static constexpr uint32_t kSfb = kSfa + 16;
+  static constexpr uint32_t kTmemUsed = kSfb + 4 * kD * kHalves;
+  static constexpr uint32_t kTmem = kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
   static constexpr int kThreads = (4 + kEpiWarps) * 32;
-  static constexpr int kApt = (NT + 127) / 128;
   // A stage: the weight record and this CTA's part of the activation record, both on 1024-byte boundaries.
   static constexpr uint32_t kStage = (kFbRecord + fb_part_bytes(NT) + 1023) / 1024 * 1024;
-  static_assert(kPair ? NT > 128 && NT <= 240 : NT <= 64, "scale factors need TMEM columns beside the D buffers");
+  static_assert(kCols % 16 == 0 && kSfa % 16 == 0 && kTmemUsed <= 512, "TMEM plan");
 };
 
 constexpr uint32_t kFbBarBytes = 512;
@@ -68,7 +68,7 @@ __host__ __device__ inline uint32_t fb_tables_bytes(int experts) {
 // then one tile of each whole wave.
 struct FbWalk {
   int kb_n, sk, waves, ncl, cl, nsk;
-  int64_t u, u1, units;
+  int u, u1, units;  // the host keeps tiles * K blocks below 2^31
   int wave;
   int tile, kb0, kb1;  // the current segment
   __device__ __forceinline__ FbWalk(int tiles, int kblocks, int cl_, int ncl_) {
@@ -78,19 +78,18 @@ struct FbWalk {
     waves = tiles / ncl;
     if (tiles % ncl && waves > 0) --waves;
     sk = tiles - waves * ncl;
-    units = (int64_t)sk * kb_n;
-    nsk = (int)(units < ncl ? units : ncl);
-    u = cl < nsk ? cl * units / nsk : 0;
-    u1 = cl < nsk ? (cl + 1) * units / nsk : 0;
+    units = sk * kb_n;
+    nsk = units < ncl ? units : ncl;
+    u = cl < nsk ? (int)((int64_t)cl * units / nsk) : 0;
+    u1 = cl < nsk ? (int)((int64_t)(cl + 1) * units / nsk) : 0;
     wave = 0;
     tile = kb0 = kb1 = 0;
   }
   __device__ __forceinline__ bool next() {
     if (u < u1) {
-      tile = (int)(u / kb_n);
-      kb0 = (int)(u - (int64_t)tile * kb_n);
-      const int64_t left = u1 - u;
-      kb1 = left < kb_n - kb0 ? kb0 + (int)left : kb_n;
+      tile = u / kb_n;
+      kb0 = u - tile * kb_n;
+      kb1 = min(kb_n, kb0 + (u1 - u));
       u += kb1 - kb0;
       return true;
     }
@@ -104,7 +103,7 @@ struct FbWalk {
     return false;
   }
   // The CTA whose range holds unit x.
-  __device__ __forceinline__ int owner(int64_t x) const { return (int)(((x + 1) * nsk - 1) / units); }
+  __device__ __forceinline__ int owner(int x) const { return (int)((((int64_t)x + 1) * nsk - 1) / units); }
 };
 
 // The tile's expert, row tile and tokens, from the prefix tables in shared memory.
@@ -136,12 +135,21 @@ struct FbCursor {
 
 // Bounded waits for a barrier phase, by one thread and by a whole warp (which agrees on the outcome). The main loop
 // is a chain of such waits, most of them for a phase that is over already: that path is one try and a vote inline
-// (47 + 20 clocks); with the loop around it inline the same wait took 260.
+// (47 + 20 clocks); with a retry loop around the try the same wait took 260. The clock is read only every 256 tries.
 __device__ __forceinline__ bool fb_wait_slow(uint32_t bar, uint32_t parity, int site) {
+  unsigned long long t0 = 0;
 #pragma unroll 1
-  for (int i = 0; i < 64; ++i)
+  for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait_bounded(bar, parity, site);
+    if ((i & 255u) == 0) {
+      const unsigned long long now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (*(volatile int*)&g_device_status.code != 0 || now - t0 > g_wait_limit_ns) {
+        record_timeout(site);
+        return false;
+      }
+    }
+  }
 }
 __device__ __forceinline__ bool fb_wait(uint32_t bar, uint32_t parity, int site) {
   return mbar_try_wait(bar, parity) || fb_wait_slow(bar, parity, site);
@@ -201,31 +209,62 @@ __device__ __forceinline__ void settle_copies() {
   while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
 }
 
-// D[tmem] (+)= A[smem] x (B[smem] * 2^sfb)^T, block scaled (A's factors are 2^0), issued by one thread.
+// A K block by its issuing thread: the scale codes' atom to TMEM columns sfb (of a pair each CTA's to its own TMEM),
+// four MMAs D[d] (+)= A x (B * 2^sfb)^T of 32 K each, block scaled (A's factors, at sfa, are 2^0), and the arrivals
+// once they are done: on `done` (D may be read) and `empty` (the stage may be refilled), of a pair in both CTAs. a_lo,
+// b_lo, s_lo: the low words of the operands' shared-memory descriptors; idesc: the instruction descriptor, whose
+// bits 4-5 pick the scale code of the 32 K.
 template <bool kPair>
-__device__ __forceinline__ void mma_mx_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
-                                          uint32_t tmem_sfa, uint32_t tmem_sfb, uint32_t accumulate) {
+__device__ __forceinline__ void issue_block(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t s_lo, uint32_t idesc,
+                                            uint32_t sfa, uint32_t sfb, uint32_t done, uint32_t empty) {
+  // High words: 8-row groups 1024 bytes apart, 128-byte swizzle; and 128 bytes apart without one, descriptor version 1.
+  constexpr uint32_t kSwHi = (1024u >> 4) | (1u << 14) | (2u << 29), kSfHi = (128u >> 4) | (1u << 14);
+  const uint32_t al = (a_lo & 0x3FFFu) | (1u << 16), bl = (b_lo & 0x3FFFu) | (1u << 16);
+  const uint32_t sl = (s_lo & 0x3FFFu) | ((128u >> 4) << 16);
   if constexpr (kPair) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
-            tmem_d),
-        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb));
+        "{\n\t.reg .pred p;\n\t.reg .b32 a, b, id;\n\t.reg .b64 da, db, ds;\n\t"
+        "mov.b64 ds, {%3, %9};\n\t"
+        "tcgen05.cp.cta_group::2.32x128b.warpx4 [%6], ds;\n\t"
+        "setp.ne.b32 p, 0, 0;\n\t"
+        "mov.b64 da, {%1, %10};\n\tmov.b64 db, {%2, %10};\n\tmov.b32 id, %4;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, id, [%5], [%6], p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\tadd.u32 a, %1, 2;\n\tadd.u32 b, %2, 2;\n\tadd.u32 id, %4, 16;\n\t"
+        "mov.b64 da, {a, %10};\n\tmov.b64 db, {b, %10};\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, id, [%5], [%6], p;\n\t"
+        "add.u32 a, %1, 4;\n\tadd.u32 b, %2, 4;\n\tadd.u32 id, %4, 32;\n\t"
+        "mov.b64 da, {a, %10};\n\tmov.b64 db, {b, %10};\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, id, [%5], [%6], p;\n\t"
+        "add.u32 a, %1, 6;\n\tadd.u32 b, %2, 6;\n\tadd.u32 id, %4, 48;\n\t"
+        "mov.b64 da, {a, %10};\n\tmov.b64 db, {b, %10};\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, id, [%5], [%6], p;\n\t"
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%7], %11;\n\t"
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%8], %11;\n\t}"
+        ::"r"(d), "r"(al), "r"(bl), "r"(sl), "r"(idesc), "r"(sfa), "r"(sfb), "r"(done), "r"(empty), "r"(kSfHi),
+        "r"(kSwHi), "h"((uint16_t)0x3)
+        : "memory");
   } else {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
-            tmem_d),
-        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb));
-  }
-}
-// A scale-factor atom from shared memory to 4 TMEM columns; for a pair each CTA's atom to its own TMEM.
-template <bool kPair>
-__device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t sdesc) {
-  if constexpr (kPair) {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
-  } else {
-    tc::cp_32x128b_warpx4(taddr, sdesc);
+        "{\n\t.reg .pred p;\n\t.reg .b32 a, b, id;\n\t.reg .b64 da, db, ds;\n\t"
+        "mov.b64 ds, {%3, %9};\n\t"
+        "tcgen05.cp.cta_group::1.32x128b.warpx4 [%6], ds;\n\t"
+        "setp.ne.b32 p, 0, 0;\n\t"
+        "mov.b64 da, {%1, %10};\n\tmov.b64 db, {%2, %10};\n\tmov.b32 id, %4;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, id, [%5], [%6], p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\tadd.u32 a, %1, 2;\n\tadd.u32 b, %2, 2;\n\tadd.u32 id, %4, 16;\n\t"
+        "mov.b64 da, {a, %10};\n\tmov.b64 db, {b, %10};\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, id, [%5], [%6], p;\n\t"
+        "add.u32 a, %1, 4;\n\tadd.u32 b, %2, 4;\n\tadd.u32 id, %4, 32;\n\t"
+        "mov.b64 da, {a, %10};\n\tmov.b64 db, {b, %10};\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, id, [%5], [%6], p;\n\t"
+        "add.u32 a, %1, 6;\n\tadd.u32 b, %2, 6;\n\tadd.u32 id, %4, 48;\n\t"
+        "mov.b64 da, {a, %10};\n\tmov.b64 db, {b, %10};\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, id, [%5], [%6], p;\n\t"
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t"
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%8];\n\t}"
+        ::"r"(d), "r"(al), "r"(bl), "r"(sl), "r"(idesc), "r"(sfa), "r"(sfb), "r"(done), "r"(empty), "r"(kSfHi),
+        "r"(kSwHi)
+        : "memory");
   }
 }
 
@@ -234,7 +273,6 @@ __device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t sdesc) {
 template <int NT, bool kPair>
 __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(const __grid_constant__ FbGemmParams p) {
   using C = FbCfg<NT, kPair>;
-  constexpr uint16_t kBoth = 0x3;  // CTA mask of a pair
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* tiles0 = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int S = p.stages;
@@ -389,7 +427,7 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
       bool ok = true;
       while (ok && walk.next()) {
         const FbTile t = cur.at(walk.tile);
-        const uint32_t bytes = (uint32_t)fb_part_rows(t.n, kPair) * 128u + C::kApt * kFbAtom;
+        const uint32_t bytes = (uint32_t)fb_part_rows(t.n, kPair) * 128u + fb_atoms_per_tile(NT) * kFbAtom;
         const uint8_t* x = p.act.x8 + t.slot * KB * fb_record_bytes(NT) + (kPair ? rank * fb_part_bytes(NT) : 0u);
         for (int kb = walk.kb0; kb < walk.kb1; ++kb, ++it) {
           if (it >= S && !fb_wait(kEmpty + 8 * s, ph ^ 1, kSiteFbEmpty)) {
@@ -435,72 +473,68 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
       }
       __syncwarp();
     }
-    int s = 0, use = 0, it = 0;  // use: D buffers taken by this warp so far
-    uint32_t ph = 0;
-    bool ok = !kPair || rank == 0;
-    while (ok && walk.next()) {
-      const int n_tile = uniform(cur.at(walk.tile).n);
-      const int nn = (n_tile + 15) / 16 * 16;
-      const int n = !kPair ? nn : who == 0 ? (nn < 128 ? nn : 128) : nn - 128;
-      const uint32_t idesc = tc::idesc_mx_e4m3(kPair ? 256 : 128, n, 0, 0);
-      // Scale codes follow the rows that this CTA holds; the pair's second MMA starts at their row 64.
-      const uint32_t sf_at = kFbRecord + (uint32_t)fb_part_rows(n_tile, kPair) * 128u + (kPair ? who * kFbAtom : 0u);
-      const uint32_t b_at = kFbRecord + (kPair ? who * 64u * 128u : 0u);
-      for (int kb = walk.kb0; ok && kb < walk.kb1; ++kb, ++it) {
-        if (kPair ? n > 0 : (it & 1) == who) {
-          // Buffer `use % n`, and its barriers: of a pair, kD buffers per half; alone every other buffer of kD.
-          constexpr int kMine = kPair ? C::kD : C::kD / 2;
-          const int db = kPair ? use % kMine : use % kMine * 2 + who;
-          const uint32_t bar = 8u * (uint32_t)(kPair ? who * C::kD + db : db);
-          ok = fb_warp_wait(kFull + 8 * s, ph, kSiteFbFull);
-          if (ok && use >= kMine) ok = fb_warp_wait(kEfree + bar, (uint32_t)(use / kMine - 1) & 1u, kSiteFbEmpty);
-          if (!ok) break;
-          ++use;
-          tc::fence_after_sync();
-          const uint32_t wt = smem_u32(tiles0) + (uint32_t)s * C::kStage;
-          const uint64_t adesc = tc::smem_desc_sw128(wt, 1024u), bdesc = tc::smem_desc_sw128(wt + b_at, 1024u);
-          // The scale factors lie beside their D buffer: those of this buffer's last use are no longer read.
-          const uint32_t d = tmem + (uint32_t)db * C::kDStride + (kPair ? 128u * who : 0u);
-          const uint32_t sfb = tmem + C::kSfb + 8u * (uint32_t)db + (kPair ? 4u * who : 0u);
-          const uint64_t sdesc = tc::smem_desc(wt + sf_at, 128u, 128u);
-          if (tm::elect_one()) {
-            cp_scales<kPair>(sfb, sdesc);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              mma_mx_ss<kPair>(d, adesc + (uint64_t)(2 * j), bdesc + (uint64_t)(2 * j), idesc | ((uint32_t)j << 4),
-                               tmem + C::kSfa, sfb, j != 0);
-            if constexpr (kPair) {
-              tc::commit_pair(kMdone + bar, kBoth);
-              tc::commit_pair(kEmpty + 8 * s, kBoth);
-            } else {
-              tc::commit(kMdone + bar);
-              tc::commit(kEmpty + 8 * s);
+    // One thread issues: the chain from a free D buffer to its MMAs has no votes and no elections, and what the
+    // instructions take is ready before the waits.
+    if ((!kPair || rank == 0) && tm::elect_one()) {
+      // The loop is a chain of dependent instructions of one thread: everything that it can carry along is carried.
+      constexpr int kMine = kPair ? C::kD : C::kD / 2;  // D buffers of this issuer: a half's, or every other one
+      constexpr uint32_t kStep = kPair ? 1 : 2;
+      const uint32_t buf0 = kPair ? who * C::kD : who;
+      const uint32_t stage0 = smem_u32(tiles0) >> 4;
+      int s = 0, buf = 0;
+      uint32_t ph = 0, eph = 1, stage = stage0;  // eph: a fresh barrier's previous phase counts as over
+      bool ok = true, turn = kPair || who == 0;
+      while (ok && walk.next()) {
+        const int n_tile = cur.at(walk.tile).n;
+        const int nn = (n_tile + 15) / 16 * 16, n0 = kPair ? fb_split(n_tile) : nn;
+        const int n = who == 0 || !kPair ? n0 : nn - n0;
+        const uint32_t idesc = tc::idesc_mx_e4m3(kPair ? 256 : 128, n, 0, 0);
+        // This MMA's tokens, and the scale codes after all rows that the CTA holds.
+        const uint32_t b_at = (kFbRecord + (kPair && who ? n0 / 2 * 128u : 0u)) >> 4;
+        const uint32_t sf_at = (kFbRecord + (uint32_t)fb_part_rows(n_tile, kPair) * 128u + (kPair ? who * kFbAtom : 0u)) >> 4;
+        for (int left = walk.kb1 - walk.kb0; left > 0; --left) {
+          const uint32_t full = kFull + 8 * s;
+          if (kPair ? n > 0 : turn) {
+            const uint32_t b = buf0 + kStep * buf, bar = 8u * b;
+            uint32_t d = tmem + b * C::kCols, sfb = tmem + C::kSfb + 4u * b;
+            uint32_t a_lo = stage, b_lo = stage + b_at, s_lo = stage + sf_at;
+            asm volatile("" : "+r"(a_lo), "+r"(b_lo), "+r"(s_lo), "+r"(d), "+r"(sfb));  // before the waits
+            ok = fb_wait(full, ph, kSiteFbFull) && fb_wait(kEfree + bar, eph, kSiteFbEmpty);
+            if (!ok) break;
+            tc::fence_after_sync();
+            issue_block<kPair>(d, a_lo, b_lo, s_lo, idesc, tmem + C::kSfa, sfb, kMdone + bar, kEmpty + 8 * s);
+            if (++buf == kMine) {
+              buf = 0;
+              eph ^= 1;
             }
+          } else if (kPair) {
+            // A tile of at most 16 tokens has no second MMA: the stage is released as if it had been read.
+            ok = fb_wait(full, ph, kSiteFbFull);
+            if (!ok) break;
+            arrive_remote(mapa_shared(kEmpty + 8 * s, 0));
+            arrive_remote(mapa_shared(kEmpty + 8 * s, 1));
           }
-          __syncwarp();
-        } else if (kPair) {
-          // A tile of at most 128 tokens has no second half: the stage is released as if it had been read.
-          ok = fb_warp_wait(kFull + 8 * s, ph, kSiteFbFull);
-          if (!ok) break;
-          if (lane < 2) arrive_remote(mapa_shared(kEmpty + 8 * s, (uint32_t)lane));
-          __syncwarp();
-        }
-        if (++s == S) {
-          s = 0;
-          ph ^= 1;
+          if (!kPair) turn = !turn;
+          stage += C::kStage >> 4;
+          if (++s == S) {
+            s = 0;
+            ph ^= 1;
+            stage = stage0;
+          }
         }
       }
     }
-    if (who == 0) {
-    // Free the TMEM once every epilogue warp has read its last results.
-    fb_wait(kEdone, 0, kSiteFbFull);
     __syncwarp();
-    tc::fence_after_sync();
-    if constexpr (kPair) {
-      tc::dealloc_pair(tmem, C::kTmem);
-    } else {
-      tc::dealloc(tmem, C::kTmem);
-    }
+    if (who == 0) {
+      // Free the TMEM once every epilogue warp has read its last results.
+      fb_wait(kEdone, 0, kSiteFbFull);
+      __syncwarp();
+      tc::fence_after_sync();
+      if constexpr (kPair) {
+        tc::dealloc_pair(tmem, C::kTmem);
+      } else {
+        tc::dealloc(tmem, C::kTmem);
+      }
     }
   }
   } else {
@@ -508,8 +542,7 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
     // -------------------------------------------------------------- epilogue
     const int q = warp & 3, h = (warp - 4) >> 2;
     const int rl = 32 * q + lane;
-    const int c0 = h * C::kCols;
-    const uint32_t tq0 = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)c0;
+    const uint32_t tq0 = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(h * C::kD * C::kCols);
     uint64_t acc2[C::kCols / 2];  // pairs of columns
 #pragma unroll
     for (int i = 0; i < C::kCols / 2; ++i) acc2[i] = 0;
@@ -523,67 +556,93 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
     uint32_t dph = 0;
     bool ok = true;
     while (ok && walk.next()) {
-      const FbTile t = cur.at(walk.tile);
-      const int cols = t.n - c0;  // this warp's valid columns (may be <= 0)
-      const int rt = kPair ? 2 * t.rt + rank : t.rt;
-      const bool have = !kPair || rt < p.row_tiles;
-      const float* sw = p.scales + (((int64_t)t.e * p.row_tiles + (have ? rt : 0)) * 2 + (q & 1)) * KB;
+      const float* sw;
+      int cols;  // this warp's valid columns (may be <= 0)
+      {
+        const FbTile t = cur.at(walk.tile);
+        const int rt = kPair ? 2 * t.rt + rank : t.rt;
+        const int n = uniform(t.n), n0 = kPair ? fb_split(n) : n;
+        cols = h ? n - n0 : min(n, n0);
+        // A row tile past the end has no scales; its sums are not stored.
+        sw = p.scales + (((int64_t)t.e * p.row_tiles + (rt < p.row_tiles ? rt : 0)) * 2 + (q & 1)) * KB;
+      }
 #pragma unroll
       for (int i = 0; i < C::kCols / 2; ++i) acc2[i] = 0;
       if (cols <= 0) continue;  // this half's MMAs are not issued either
+      // The columns pass in chunks through two register buffers: while one chunk is added, the next one's load is in
+      // flight, across the K blocks too (the next block's first load is issued before this block's last additions).
+      // A D buffer is released once its last chunk is in registers. Columns past the tile's are added like the
+      // others (whatever they hold) and never stored: a branch around them costs every tile more.
+      constexpr int kCh = C::kCols < 64 ? 16 : 32;
+      constexpr int kChunks = (C::kCols + kCh - 1) / kCh;
+      constexpr int kLast = C::kCols - (kChunks - 1) * kCh;  // columns of the last chunk
+      uint32_t v[2][kCh];
       float sv = 0.f;
+      ok = fb_warp_wait(kMdone + 8 * (h * C::kD + db), dph, kSiteFbFull);
+      if (!ok) break;
+      tc::fence_after_sync();
+      ld_cols(tq0 + (uint32_t)db * C::kCols, v[0]);
+#pragma unroll 1
       for (int kb = walk.kb0; kb < walk.kb1; ++kb) {
         if (kb == walk.kb0 || (kb & 31) == 0) sv = (kb & ~31) + lane < KB ? __ldg(sw + (kb & ~31) + lane) : 0.f;
         const float w = __shfl_sync(0xFFFFFFFFu, sv, kb & 31);
-        ok = fb_warp_wait(kMdone + 8 * (h * C::kD + db), dph, kSiteFbFull);
-        if (!ok) break;
-        tc::fence_after_sync();
-        const uint32_t tq = tq0 + (uint32_t)db * C::kDStride;
         const uint64_t w2 = pack2(w, w);
-        // Chunks of columns: the next chunk's load is in flight while this one's values are added, and the buffer is
-        // released once its last chunk is in registers.
-        constexpr int kCh = C::kCols < 32 ? C::kCols : 32;
-        uint32_t v[2][kCh];
-        ld_cols(tq, v[0]);
+        const uint32_t tq = tq0 + (uint32_t)db * C::kCols;
 #pragma unroll
-        for (int b = 0; b < C::kCols; b += kCh) {
-          if (b < cols) {
-            uint32_t(&x)[kCh] = v[(b / kCh) & 1];
+        for (int c = 0; c < kChunks; ++c) {
+          uint32_t(&x)[kCh] = v[c & 1];
+          uint32_t(&y)[kCh] = v[(c + 1) & 1];
+          if (c + 1 < kChunks) {
             wait_ld(x);
-            if (b + kCh < C::kCols && b + kCh < cols) {
-              ld_cols(tq + b + kCh, v[(b / kCh + 1) & 1]);
+            if (c + 2 < kChunks || kLast == kCh) {
+              ld_cols(tq + (c + 1) * kCh, y);
             } else {
-              tc::fence_before_sync();
-              __syncwarp();
-              if (lane == 0) {
-                if (kPair && rank != 0) {
-                  arrive_remote(efree0 + 8 * db);
-                } else {
-                  mbar_arrive(kEfree + 8 * (h * C::kD + db));
-                }
+              ld_cols(tq + (c + 1) * kCh, *reinterpret_cast<uint32_t(*)[kLast]>(&y));
+            }
+          } else {
+            wait_ld(*reinterpret_cast<uint32_t(*)[kLast]>(&x));
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+              if (kPair && rank != 0) {
+                arrive_remote(efree0 + 8 * db);
+              } else {
+                mbar_arrive(kEfree + 8 * (h * C::kD + db));
               }
             }
-#pragma unroll
-            for (int i = 0; i < kCh / 2; ++i)
-              acc2[b / 2 + i] = fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), w2, acc2[b / 2 + i]);
+            if (++db == C::kD) {
+              db = 0;
+              dph ^= 1;
+            }
+            if (kChunks > 1 && kb + 1 < walk.kb1) {
+              ok = fb_warp_wait(kMdone + 8 * (h * C::kD + db), dph, kSiteFbFull);
+              tc::fence_after_sync();
+              if (ok) ld_cols(tq0 + (uint32_t)db * C::kCols, y);
+            }
           }
+#pragma unroll
+          for (int i = 0; i < (c + 1 < kChunks ? kCh : kLast) / 2; ++i)
+            acc2[c * kCh / 2 + i] =
+                fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), w2, acc2[c * kCh / 2 + i]);
         }
-        if (++db == C::kD) {
-          db = 0;
-          dph ^= 1;
+        if (kChunks == 1 && kb + 1 < walk.kb1) {  // one buffer
+          ok = fb_warp_wait(kMdone + 8 * (h * C::kD + db), dph, kSiteFbFull);
+          tc::fence_after_sync();
+          if (ok) ld_cols(tq0 + (uint32_t)db * C::kCols, v[0]);
         }
+        if (!ok) break;
       }
       if (!ok) break;
       if (walk.kb0 != 0 || walk.kb1 != KB) {
         // A tile shared between CTAs: publish this warp's part, and sum all
         // parts in K order if it is the last to arrive.
-        const int64_t u_tile = (int64_t)walk.tile * KB;
+        const int u_tile = walk.tile * KB;
         const int first = walk.owner(u_tile), last = walk.owner(u_tile + KB - 1);
         constexpr int kQuads = NT / 4;
         auto part = [&](int cta) {
           // Slot 1 holds the part that starts its tile (the CTA's last tile), slot 0 the others.
           const int64_t at = kPair ? cta * 2 + rank : cta;
-          return reinterpret_cast<float4*>(p.partials) + ((at * 2 + (cta == first ? 1 : 0)) * kQuads + c0 / 4) * 128 + rl;
+          return reinterpret_cast<float4*>(p.partials) + ((at * 2 + (cta == first ? 1 : 0)) * kQuads + h * C::kCols / 4) * 128 + rl;
         };
         float4* mine = part(walk.cl);
 #pragma unroll
@@ -612,9 +671,11 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
           }
         }
       }
-      const int row = rt * 128 + rl;
+      // Looked up again: held over the K loop, these would cost it registers.
+      const FbTile t = cur.at(walk.tile);
+      const int row = (kPair ? 2 * t.rt + rank : t.rt) * 128 + rl;
       if (row < p.n_rows) {
-        const int64_t at = ((int64_t)t.o + t.row0 + c0) * p.ldo + row;
+        const int64_t at = ((int64_t)t.o + t.row0 + (h ? fb_split(t.n) : 0)) * p.ldo + row;
         if (p.out_bf16) {
           __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.out) + at;
 #pragma unroll
@@ -659,7 +720,7 @@ cudaError_t launch_nt(const FbGemmParams& p, int grid, cudaStream_t stream) {
 }  // namespace
 
 int fb_tile_for(int64_t expected_rows) {
-  return expected_rows <= 16 ? 16 : expected_rows <= 32 ? 32 : expected_rows <= 64 ? 64 : kPairTokens;
+  return expected_rows <= 16 ? 16 : expected_rows <= 32 ? 32 : expected_rows <= 64 ? 64 : kFbPairTokens;
 }
 
 uint32_t fb_gemm_smem(int nt, int experts, int stages) {
@@ -667,7 +728,7 @@ uint32_t fb_gemm_smem(int nt, int experts, int stages) {
     case 16: return smem_of<16, false>(experts, stages);
     case 32: return smem_of<32, false>(experts, stages);
     case 64: return smem_of<64, false>(experts, stages);
-    default: return smem_of<kPairTokens, true>(experts, stages);
+    default: return smem_of<kFbPairTokens, true>(experts, stages);
   }
 }
 
@@ -682,7 +743,7 @@ cudaError_t fb_status_symbols(void** status, void** limit) {
   return e == cudaSuccess ? cudaGetSymbolAddress(limit, g_wait_limit_ns) : e;
 }
 
-int fb_gemm_grid(int nt, int sms) { return nt == kPairTokens ? sms / 2 * 2 : sms; }
+int fb_gemm_grid(int nt, int sms) { return nt == kFbPairTokens ? sms / 2 * 2 : sms; }
 size_t fb_partial_bytes(int nt, int sms) { return (size_t)sms * 2 * 128 * nt * sizeof(float); }
 
 cudaError_t launch_fb_gemm(const FbGemmParams& p, int grid, cudaStream_t stream) {
@@ -690,7 +751,7 @@ cudaError_t launch_fb_gemm(const FbGemmParams& p, int grid, cudaStream_t stream)
     case 16: return launch_nt<16, false>(p, grid, stream);
     case 32: return launch_nt<32, false>(p, grid, stream);
     case 64: return launch_nt<64, false>(p, grid, stream);
-    default: return launch_nt<kPairTokens, true>(p, grid, stream);
+    default: return launch_nt<kFbPairTokens, true>(p, grid, stream);
   }
 }
 
