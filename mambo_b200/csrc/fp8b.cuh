@@ -78,14 +78,19 @@ __device__ __forceinline__ FbPlace fb_place(int o, int count, int e, int local, 
   return pl;
 }
 
-// Stores 8 values (chunk8: their index in the row, in eights) and, with the first of a K block, its four scale codes.
-__device__ __forceinline__ void fb_store(const FbActivations& a, const FbPlace& pl, int64_t chunk8, uint2 q,
-                                         uint32_t word) {
-  if (pl.slot < 0 || pl.slot >= a.slots) return;
-  const int64_t kb = chunk8 >> 4;
-  const int c = (int)(chunk8 & 15);
+// Where a row goes in the records of its K blocks: its 128 bytes' address in the first one, its scale word's, and the
+// swizzle of its 16-byte chunks. row is null for a row that has no place.
+struct FbDst {
+  uint8_t* row;
+  uint8_t* sf;
+  int swz;
+};
+__device__ __forceinline__ FbDst fb_dst(const FbActivations& a, const FbPlace& pl) {
+  FbDst d;
+  d.row = nullptr;
+  if (pl.slot < 0 || pl.slot >= a.slots) return d;
   const bool pair = fb_is_pair(a.nt);
-  uint8_t* rec = a.x8 + (pl.slot * a.kblocks + kb) * fb_record_bytes(a.nt);
+  uint8_t* rec = a.x8 + pl.slot * a.kblocks * fb_record_bytes(a.nt);
   int row = pl.in_tile, part = 0, half = 0, t = pl.in_tile;  // t: place among its MMA's tokens
   if (pair) {
     const int nn = (pl.n + 15) / 16 * 16, n0 = fb_split(pl.n), n1 = nn - n0;
@@ -95,12 +100,21 @@ __device__ __forceinline__ void fb_store(const FbActivations& a, const FbPlace& 
     part = t >= per;
     row = t - part * per + half * (n0 / 2);
   }
-  uint8_t* d = rec + part * fb_part_bytes(a.nt) + row * 128 + (((c >> 1) ^ (row & 7)) << 4) + (c & 1) * 8;
-  *reinterpret_cast<uint2*>(d) = q;
+  d.row = rec + part * fb_part_bytes(a.nt) + row * 128;
+  d.sf = rec + fb_part_rows(pl.n, pair) * 128 + half * kFbAtom + (t & 31) * 16 + (t >> 5) * 4;
+  d.swz = row & 7;
+  return d;
+}
+// Stores the 8 values of chunk c (0..15) of K block kb, and with the first chunk the block's four scale codes (for
+// both CTAs of a pair).
+__device__ __forceinline__ void fb_store(const FbActivations& a, const FbDst& d, int64_t kb, int c, uint2 q,
+                                         uint32_t word) {
+  if (!d.row) return;
+  const int64_t at = kb * fb_record_bytes(a.nt);
+  *reinterpret_cast<uint2*>(d.row + at + (((c >> 1) ^ d.swz) << 4) + (c & 1) * 8) = q;
   if (c == 0) {
-    uint8_t* s = rec + fb_part_rows(pl.n, pair) * 128 + half * kFbAtom + (t & 31) * 16 + (t >> 5) * 4;
-    *reinterpret_cast<uint32_t*>(s) = word;
-    if (pair) *reinterpret_cast<uint32_t*>(s + fb_part_bytes(a.nt)) = word;
+    *reinterpret_cast<uint32_t*>(d.sf + at) = word;
+    if (fb_is_pair(a.nt)) *reinterpret_cast<uint32_t*>(d.sf + at + fb_part_bytes(a.nt)) = word;
   }
 }
 

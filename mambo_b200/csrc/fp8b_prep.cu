@@ -53,153 +53,198 @@ cudaError_t launch_fb_pack(const FbPackParams& p, cudaStream_t stream) {
 }
 
 // --------------------------------------------------------------------------
-// Quantization: 8 values per thread (one 16-byte load of bf16), a quad (16
-// lanes) per 32 (128) values, 2048 values of a row per CTA. Every row goes to
-// each of its places: one in expert order (kFbGrouped), up to `top` when its
-// token was routed, so that x is read once.
+// Quantization, bound by the bytes it moves. A warp takes kSpan values of one
+// row, kSteps loads in flight (a lane holds 8 values, a quad or 16 lanes a
+// scale group), and finds the row's places once for all of them: one place in
+// expert order (kFbGrouped), up to `top` when the row's token was routed, so
+// that x is read once. One 256-value step per lane and the place found by
+// every thread took 180 us for 4096 x 28672 bf16 rows, this one XX us.
 // --------------------------------------------------------------------------
+namespace {
+
+constexpr int kSteps = 4, kSpan = 256 * kSteps;
+
+__device__ __forceinline__ uint2 quantize8(const float (&v)[8], int group, int lane, uint32_t& word) {
+  // Largest magnitude as bits: NaN orders above infinity, so either gives the group the code 0xFF.
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+  m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+  if (group == 128) {
+    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 4));
+    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
+  }
+  const uint32_t code = mxfp8_scale_code(__uint_as_float(m));
+  const float inv = e8m0_to_float(code == 0xFFu ? 0u : 254u - code);
+  uint32_t packed[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    packed[h] = cvt_e4m3x2_rn(v[4 * h] * inv, v[4 * h + 1] * inv) |
+                (cvt_e4m3x2_rn(v[4 * h + 2] * inv, v[4 * h + 3] * inv) << 16);
+  word = code << (8 * ((lane >> 2) & 3));
+  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
+  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
+  return make_uint2(packed[0], packed[1]);
+}
+
+}  // namespace
+
 template <int kIn, bool kVec>
 __global__ void __launch_bounds__(256) fb_quant_kernel(const __grid_constant__ FbQuantParams p) {
-  const int64_t row = blockIdx.y + (int64_t)blockIdx.z * 65535;
-  if (row >= p.rows) return;
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;  // 8-value chunk of the row
-  const int64_t chunks = (p.k + 127) / 128 * 16;
   const int lane = threadIdx.x & 31;
+  const int64_t spans = (p.k + kSpan - 1) / kSpan;
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   pdl_wait();
   pdl_launch_dependents();
-  // Whole 16-lane groups are in range together (chunks is a multiple of 16).
-  const bool in = c < chunks;
-  uint2 q = make_uint2(0, 0);
-  uint32_t word = 0;
-  if (kIn == kFbCodes) {
-    if (in) {
-      const uint8_t* src = reinterpret_cast<const uint8_t*>(p.x) + row * p.ldx + c * 8;
-      if (kVec && c * 8 + 8 <= p.k) {
-        q = __ldg(reinterpret_cast<const uint2*>(src));
-      } else {
-        uint32_t b[2] = {0, 0};
+  if (item >= p.rows * spans) return;
+  const int64_t row = item / spans, span = item - row * spans;
+  const int64_t c0 = span * (kSpan / 8) + lane;        // first 8-value chunk of the lane
+  const int64_t chunks = (p.k + 127) / 128 * 16;       // whole K blocks
+  // All loads first.
+  uint4 raw[kSteps], raw2[kIn == MAMBO_F32 ? kSteps : 1];
+  (void)raw2;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c * 8 + i < p.k) b[i >> 2] |= (uint32_t)__ldg(src + i) << (8 * (i & 3));
-        q = make_uint2(b[0], b[1]);
+  for (int i = 0; i < kSteps; ++i) {
+    const int64_t k0 = (c0 + 32 * i) * 8;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if constexpr (kIn == MAMBO_F32) raw2[i] = make_uint4(0, 0, 0, 0);
+    if (k0 >= p.k) continue;
+    if constexpr (kIn == MAMBO_BF16) {
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(p.x) + row * p.ldx + k0;
+      if (kVec && k0 + 8 <= p.k) {
+        raw[i] = __ldg(reinterpret_cast<const uint4*>(src));
+      } else {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (k0 + j < p.k) w[j >> 1] |= (uint32_t)__ldg(src + j) << (16 * (j & 1));
+        raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      const uint8_t* s = p.xs + row * p.lds;
-      if (p.group == 128) {
-        word = (uint32_t)__ldg(s + (c >> 4)) * 0x01010101u;
+    } else if constexpr (kIn == MAMBO_F32) {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.x) + row * p.ldx + k0;
+      if (kVec && k0 + 8 <= p.k) {
+        raw[i] = __ldg(reinterpret_cast<const uint4*>(src));
+        raw2[i] = __ldg(reinterpret_cast<const uint4*>(src) + 1);
       } else {
-        const int64_t g0 = (c >> 4) * 4, groups = (p.k + 31) / 32;
+        uint32_t w[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) word |= (uint32_t)(g0 + j < groups ? __ldg(s + g0 + j) : 127) << (8 * j);
+        for (int j = 0; j < 8; ++j) w[j] = k0 + j < p.k ? __ldg(src + j) : 0u;
+        raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        raw2[i] = make_uint4(w[4], w[5], w[6], w[7]);
       }
-    }
-  } else {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    if (in) {
-      if constexpr (kIn == MAMBO_BF16) {
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(p.x) + row * p.ldx + c * 8;
-        if (kVec && c * 8 + 8 <= p.k) {
-          const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src));
-          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c * 8 + i < p.k) v[i] = __uint_as_float((uint32_t)__ldg(src + i) << 16);
-        }
+    } else {
+      const uint8_t* src = reinterpret_cast<const uint8_t*>(p.x) + row * p.ldx + k0;
+      if (kVec && k0 + 8 <= p.k) {
+        const uint2 t = __ldg(reinterpret_cast<const uint2*>(src));
+        raw[i] = make_uint4(t.x, t.y, 0, 0);
       } else {
-        const float* src = reinterpret_cast<const float*>(p.x) + row * p.ldx + c * 8;
-        if (kVec && c * 8 + 8 <= p.k) {
-          const float4 a = __ldg(reinterpret_cast<const float4*>(src));
-          const float4 b = __ldg(reinterpret_cast<const float4*>(src) + 1);
-          v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-          v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
+        uint32_t w[2] = {0, 0};
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c * 8 + i < p.k) v[i] = __ldg(src + i);
-        }
+        for (int j = 0; j < 8; ++j)
+          if (k0 + j < p.k) w[j >> 2] |= (uint32_t)__ldg(src + j) << (8 * (j & 3));
+        raw[i] = make_uint4(w[0], w[1], 0, 0);
       }
     }
-    // Largest magnitude as bits: NaN orders above infinity, so either gives the group the code 0xFF.
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-    if (p.group == 128) {
-      m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 4));
-      m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
-    }
-    const uint32_t code = mxfp8_scale_code(__uint_as_float(m));
-    const float inv = e8m0_to_float(code == 0xFFu ? 0u : 254u - code);
-    uint32_t packed[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      packed[h] = cvt_e4m3x2_rn(v[4 * h] * inv, v[4 * h + 1] * inv) |
-                  (cvt_e4m3x2_rn(v[4 * h + 2] * inv, v[4 * h + 3] * inv) << 16);
-    q = make_uint2(packed[0], packed[1]);
-    word = code << (8 * ((lane >> 2) & 3));
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
   }
-  // Grouped: the row's expert, by whole warps: how many segments end at or before it.
-  int expert = 0;
-  if (p.mode == kFbGrouped) {
+  // The row's places while they are on their way.
+  int copies = 1, expert = 0;
+  FbDst dst;
+  dst.row = nullptr;
+  if (p.mode == kFbDense) {
+    if (!p.values) dst = fb_dst(p.act, fb_place(0, (int)p.rows, 0, (int)row, p.act.nt));
+  } else if (p.mode == kFbGrouped) {
+    // The row's expert: how many segments end at or before it.
     for (int b = 0; b < p.experts; b += 32) {
       const int end = b + lane < p.experts ? __ldg(p.offsets + b + lane + 1) : 0x7FFFFFFF;
       expert += __popc(__ballot_sync(0xFFFFFFFFu, end <= row));
     }
+    if (expert < p.experts) {
+      const int o = clamp_offset(__ldg(p.offsets + expert), p.total_rows);
+      const int end = clamp_offset(__ldg(p.offsets + expert + 1), p.total_rows);
+      if (row >= o && end > o) dst = fb_dst(p.act, fb_place(o, end - o, expert, (int)row - o, p.act.nt));
+    }
+  } else {
+    copies = p.top;
   }
-  if (!in) return;
-  if (p.mode == kFbDense) {
-    if (p.values) {
+  uint2 q[kSteps];
+  uint32_t word[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    if constexpr (kIn == kFbCodes) {
+      q[i] = make_uint2(raw[i].x, raw[i].y);
+      const int64_t kb = (c0 + 32 * i) >> 4;
+      const uint8_t* s = p.xs + row * p.lds;
+      word[i] = 0;
+      if (c0 + 32 * i < chunks) {
+        if (p.group == 128) {
+          word[i] = (uint32_t)__ldg(s + kb) * 0x01010101u;
+        } else {
+          const int64_t groups = (p.k + 31) / 32;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) word[i] |= (uint32_t)(kb * 4 + j < groups ? __ldg(s + kb * 4 + j) : 127) << (8 * j);
+        }
+      }
+    } else {
+      float v[8];
+      if constexpr (kIn == MAMBO_BF16) {
+        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[2 * j] = __uint_as_float(w[j] << 16);
+          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        }
+      } else {
+        const uint32_t w[8] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w, raw2[i].x, raw2[i].y, raw2[i].z, raw2[i].w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+      }
+      q[i] = quantize8(v, p.group, lane, word[i]);
+    }
+  }
+  if (p.mode == kFbDense && p.values) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int64_t c = c0 + 32 * i;
+      if (c * 8 >= p.k) continue;
       uint8_t* d = p.values + row * p.ldv + c * 8;
       if (c * 8 + 8 <= p.k && (uintptr_t)d % 8 == 0) {
-        *reinterpret_cast<uint2*>(d) = q;
+        *reinterpret_cast<uint2*>(d) = q[i];
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c * 8 + i < p.k) d[i] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+        for (int j = 0; j < 8; ++j)
+          if (c * 8 + j < p.k) d[j] = (uint8_t)((j < 4 ? q[i].x : q[i].y) >> (8 * (j & 3)));
       }
       if (p.group == 128) {
-        if ((c & 15) == 0) p.scales[row * p.ldsc + (c >> 4)] = (uint8_t)word;
-      } else if ((c & 3) == 0 && c * 8 < p.k) {
-        p.scales[row * p.ldsc + (c >> 2)] = (uint8_t)(word >> (8 * ((c >> 2) & 3)));
+        if ((c & 15) == 0) p.scales[row * p.ldsc + (c >> 4)] = (uint8_t)word[i];
+      } else if ((c & 3) == 0) {
+        p.scales[row * p.ldsc + (c >> 2)] = (uint8_t)(word[i] >> (8 * ((c >> 2) & 3)));
       }
-      return;
     }
-    fb_store(p.act, fb_place(0, (int)p.rows, 0, (int)row, p.act.nt), c, q, word);
-  } else if (p.mode == kFbGrouped) {
-    const int e = expert;
-    if (e >= p.experts) return;  // past the last segment
-    const int o = clamp_offset(__ldg(p.offsets + e), p.total_rows);
-    const int end = clamp_offset(__ldg(p.offsets + e + 1), p.total_rows);
-    const int local = (int)row - o;
-    if (local < 0 || end <= o) return;
-    fb_store(p.act, fb_place(o, end - o, e, local, p.act.nt), c, q, word);
-  } else {
-    for (int j = 0; j < p.top; ++j) {
+    return;
+  }
+  for (int j = 0; j < copies; ++j) {
+    if (p.mode == kFbRouted) {
+      dst.row = nullptr;
       const int e = __ldg(p.ids + row * p.top + j);
       const int pos = __ldg(p.positions + row * p.top + j);
-      if (e < 0 || e >= p.experts || pos < 0 || pos >= p.total_rows) continue;
-      const int o = clamp_offset(__ldg(p.offsets + e), p.total_rows);
-      const int end = clamp_offset(__ldg(p.offsets + e + 1), p.total_rows);
-      if (pos < o || pos >= end) continue;
-      fb_store(p.act, fb_place(o, end - o, e, pos - o, p.act.nt), c, q, word);
+      if (e >= 0 && e < p.experts && pos >= 0 && pos < p.total_rows) {
+        const int o = clamp_offset(__ldg(p.offsets + e), p.total_rows);
+        const int end = clamp_offset(__ldg(p.offsets + e + 1), p.total_rows);
+        if (pos >= o && pos < end) dst = fb_dst(p.act, fb_place(o, end - o, e, pos - o, p.act.nt));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int64_t c = c0 + 32 * i;
+      if (c < chunks) fb_store(p.act, dst, c >> 4, (int)(c & 15), q[i], word[i]);
     }
   }
 }
 
 cudaError_t launch_fb_quant(const FbQuantParams& p, cudaStream_t stream) {
-  const int64_t chunks = (p.k + 127) / 128 * 16;
-  const dim3 grid((unsigned)((chunks + 255) / 256), (unsigned)(p.rows < 65535 ? p.rows : 65535),
-                  (unsigned)((p.rows + 65534) / 65535));
+  const int64_t items = p.rows * ((p.k + kSpan - 1) / kSpan);
+  const dim3 grid((unsigned)((items + 7) / 8));
   const int esize = p.x_kind == MAMBO_F32 ? 4 : p.x_kind == MAMBO_BF16 ? 2 : 1;
   const int align = p.x_kind == kFbCodes ? 8 : 16;
   const bool vec = (uintptr_t)p.x % align == 0 && (p.ldx * esize) % align == 0;

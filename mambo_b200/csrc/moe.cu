@@ -8,7 +8,7 @@ namespace mambo {
 
 namespace {
 
-constexpr int kRouteThreads = 256;
+constexpr int kRouteThreads = 512;
 constexpr int kRouteWarps = kRouteThreads / 32;
 // Tokens of a chunk: one CTA. A call of one chunk is one launch.
 constexpr int kRouteChunk = 128;
@@ -22,28 +22,37 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 // One token, a warp: expert 32*i + lane in slot i of the lane. Experts whose
 // logit is -inf or NaN are masked; +inf counts as the largest finite number.
 template <int NV>
-__device__ __forceinline__ void route_token(const FbRouteParams& p, int token, int lane, int* hist) {
+__device__ __forceinline__ void route_load(const FbRouteParams& p, int token, int lane, float (&raw)[NV]) {
+  const int64_t at = (int64_t)token * p.ld + lane;
+  if (p.bf16) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      raw[i] = 32 * i + lane < p.experts ? __uint_as_float((uint32_t)__ldg((const uint16_t*)p.logits + at + 32 * i) << 16)
+                                         : -INFINITY;
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      raw[i] = 32 * i + lane < p.experts ? __ldg((const float*)p.logits + at + 32 * i) : -INFINITY;
+  }
+}
+
+template <int NV>
+__device__ __forceinline__ void route_token(const FbRouteParams& p, int token, int lane, const float (&raw)[NV],
+                                            const float (&bias)[NV], int* hist) {
   float l[NV], prob[NV];
   uint32_t key[NV];
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int e = 32 * i + lane;
-    l[i] = -INFINITY;
-    if (e < p.experts) {
-      const int64_t at = (int64_t)token * p.ld + e;
-      const float v = p.bf16 ? __uint_as_float((uint32_t)__ldg((const uint16_t*)p.logits + at) << 16)
-                             : __ldg((const float*)p.logits + at);
-      if (v == v) l[i] = fminf(v, 3.4028234663852886e38f);
-    }
+    const float v = raw[i];
+    l[i] = v == v ? fminf(v, 3.4028234663852886e38f) : -INFINITY;
     top = fmaxf(top, l[i]);
   }
   if (p.sigmoid) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int e = 32 * i + lane;
       prob[i] = 1.0f / (1.0f + expf(-l[i]));
-      const float s = prob[i] + (p.bias && e < p.experts ? __ldg(p.bias + e) : 0.f);
+      const float s = prob[i] + bias[i];
       key[i] = l[i] == -INFINITY || s != s ? 0u : order_key(s);
     }
   } else {
@@ -59,34 +68,41 @@ __device__ __forceinline__ void route_token(const FbRouteParams& p, int token, i
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int e = 32 * i + lane;
       prob[i] = sum > 0.f ? prob[i] / sum : 0.f;
-      const float s = l[i] + (p.bias && e < p.experts ? __ldg(p.bias + e) : 0.f);
+      const float s = l[i] + bias[i];
       key[i] = l[i] == -INFINITY || s != s ? 0u : order_key(s);
     }
   }
+  // Each lane's best key and its slot (the first of equal keys: the lowest expert of the lane).
+  uint32_t best = 0;
+  int at = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (key[i] > best) {
+      best = key[i];
+      at = i;
+    }
   float total = 0.f, mine_w = 0.f;
   int mine_id = -1;
   for (int j = 0; j < p.top; ++j) {
-    uint32_t best = 0;
-    int at = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (key[i] > best) {  // the first of equal keys: the lowest expert of the lane
-        best = key[i];
-        at = i;
-      }
     const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, best);
     if (m == 0) break;  // no expert left
-    const uint32_t cand = best == m ? (uint32_t)(32 * at + lane) : 0xFFFFFFFFu;
-    const uint32_t id = __reduce_min_sync(0xFFFFFFFFu, cand);
+    const uint32_t id = __reduce_min_sync(0xFFFFFFFFu, best == m ? (uint32_t)(32 * at + lane) : 0xFFFFFFFFu);
     float w = 0.f;
+    if (lane == (int)(id & 31)) {  // the lane that had it takes its next best
+      best = 0;
+      const int taken = at;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (cand == id && at == i) {
-        w = prob[i];
-        key[i] = 0;
+      for (int i = 0; i < NV; ++i) {
+        if (i == taken) {
+          w = prob[i];
+          key[i] = 0;
+        } else if (key[i] > best) {
+          best = key[i];
+          at = i;
+        }
       }
+    }
     w = __shfl_sync(0xFFFFFFFFu, w, (int)(id & 31));
     total += w;
     if (lane == j) {
@@ -175,7 +191,16 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const __grid_c
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
-  for (int t = warp; t < count; t += kRouteWarps) route_token<NV>(p, first + t, lane, hist);
+  float bias[NV], raw[NV], next[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) bias[i] = p.bias && 32 * i + lane < p.experts ? __ldg(p.bias + 32 * i + lane) : 0.f;
+  if (warp < count) route_load<NV>(p, first + warp, lane, next);
+  for (int t = warp; t < count; t += kRouteWarps) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) raw[i] = next[i];
+    if (t + kRouteWarps < count) route_load<NV>(p, first + t + kRouteWarps, lane, next);  // while this one is ranked
+    route_token<NV>(p, first + t, lane, raw, bias, hist);
+  }
   __syncthreads();
   if (gridDim.x > 1) {
     for (int i = threadIdx.x; i < buckets; i += kRouteThreads) p.chunk_counts[(int64_t)blockIdx.x * buckets + i] = hist[i];
@@ -198,16 +223,24 @@ __global__ void __launch_bounds__(kRouteThreads) moe_place_kernel(const __grid_c
   const int first = blockIdx.x * kRouteChunk, count = min(kRouteChunk, p.tokens - first);
   pdl_wait();
   pdl_launch_dependents();
-  for (int e = threadIdx.x; e < buckets; e += kRouteThreads) {
+  // Warps take (32 buckets, part of the chunks), so that the loads of all are in flight.
+  for (int e = threadIdx.x; e < 2 * buckets; e += kRouteThreads) base[e] = 0;
+  __syncthreads();
+  const int groups = (buckets + 31) / 32, parts = max(1, kRouteWarps / groups), chunks = (int)gridDim.x;
+  for (int job = warp; job < groups * parts; job += kRouteWarps) {
+    const int e = job % groups * 32 + lane, part = job / groups;
+    const int c0 = part * chunks / parts, c1 = (part + 1) * chunks / parts;
     int all = 0, prior = 0;
-#pragma unroll 8
-    for (int c = 0; c < (int)gridDim.x; ++c) {
-      const int v = p.chunk_counts[(int64_t)c * buckets + e];
-      all += v;
-      prior += c < (int)blockIdx.x ? v : 0;
+    if (e < buckets) {
+#pragma unroll 16
+      for (int c = c0; c < c1; ++c) {
+        const int v = __ldg(p.chunk_counts + (int64_t)c * buckets + e);
+        all += v;
+        prior += c < (int)blockIdx.x ? v : 0;
+      }
+      atomicAdd(base + e, all);  // whole numbers: the order does not matter
+      atomicAdd(before + e, prior);
     }
-    base[e] = all;
-    before[e] = prior;
   }
   __syncthreads();
   if (warp == 0) scan_counts(base, buckets, lane);
@@ -230,10 +263,12 @@ cudaError_t launch_fb_route(const FbRouteParams& p, cudaStream_t stream) {
                   : nv <= 8 ? (const void*)moe_route_kernel<8>
                   : nv <= 16 ? (const void*)moe_route_kernel<16>
                              : (const void*)moe_route_kernel<32>;
-  cudaError_t e = launch_pdl(k, dim3(chunks), dim3(kRouteThreads), smem, stream, p);
+  cudaError_t e = ensure_smem_attribute(k, smem);
+  if (e == cudaSuccess) e = launch_pdl(k, dim3(chunks), dim3(kRouteThreads), smem, stream, p);
   if (e != cudaSuccess || chunks == 1) return e;
-  return launch_pdl((const void*)moe_place_kernel, dim3(chunks), dim3(kRouteThreads),
-                    (size_t)buckets * (2 + kRouteWarps) * sizeof(int), stream, p);
+  const size_t place = (size_t)buckets * (2 + kRouteWarps) * sizeof(int);
+  e = ensure_smem_attribute((const void*)moe_place_kernel, place);
+  return e != cudaSuccess ? e : launch_pdl((const void*)moe_place_kernel, dim3(chunks), dim3(kRouteThreads), place, stream, p);
 }
 
 // --------------------------------------------------------------------------
@@ -276,7 +311,7 @@ __global__ void __launch_bounds__(256) moe_hidden_kernel(const __grid_constant__
   const int o = clamp_offset(__ldg(p.offsets + e), p.rows), end = clamp_offset(__ldg(p.offsets + e + 1), p.rows);
   const int local = (int)row - o;
   if (local < 0 || end <= o) return;
-  fb_store(p.act, fb_place(o, end - o, e, local, p.act.nt), c, q, word);
+  fb_store(p.act, fb_dst(p.act, fb_place(o, end - o, e, local, p.act.nt)), c >> 4, c & 15, q, word);
 }
 
 cudaError_t launch_fb_hidden(const FbHiddenParams& p, cudaStream_t stream) {
