@@ -60,7 +60,7 @@ int check_workspace(void* ws, size_t have, size_t need) {
 }
 
 cudaError_t run_gemm(const MamboFp8BlockWeight* w, const Plan& P, const FbActivations& act, int64_t rows,
-                     const int* offsets, void* out, int out_bf16, int64_t ldo, int n_rows, uint8_t* partials,
+                     const int* offsets, void* out, int out_bf16, int64_t ldo, const FbActivations* hidden, uint8_t* partials,
                      void* workspace, int sms, int smem_optin, cudaStream_t stream) {
   FbGemmParams g{};
   g.packed = (const uint8_t*)w->packed;
@@ -69,12 +69,13 @@ cudaError_t run_gemm(const MamboFp8BlockWeight* w, const Plan& P, const FbActiva
   g.experts = offsets ? (int)w->n_experts : 1;
   g.rows = rows;
   g.offsets = offsets;
-  g.n_rows = n_rows;
+  g.n_rows = (int)w->n_rows;
   g.row_tiles = P.row_tiles;
   g.out = out;
   g.out_bf16 = out_bf16;
   g.ldo = ldo;
-  g.stages = fb_gemm_stages(P.nt, g.experts, smem_optin);
+  if (hidden) g.hidden = *hidden;
+  g.stages = fb_gemm_stages(P.nt, g.experts, smem_optin, hidden != nullptr);
   g.evict_weights = rows <= P.nt;
   g.partials = (float*)partials;
   g.counters = (int*)((uint8_t*)workspace + kWorkspaceSplitCounterOffset);
@@ -122,7 +123,7 @@ int linear_impl(const void* x, int x_kind, int64_t ldx, const uint8_t* xs, int64
   q.act = act;
   cudaError_t e = launch_fb_quant(q, stream);
   if (e != cudaSuccess) return api_cuda_fail(e, "fp8 block quantizer");
-  e = run_gemm(w, P, act, m, offsets, out, out_dtype == MAMBO_BF16, ldo, (int)w->n_rows, at + P.x8, workspace,
+  e = run_gemm(w, P, act, m, offsets, out, out_dtype == MAMBO_BF16, ldo, nullptr, at + P.x8, workspace,
                sms, smem, stream);
   if (e != cudaSuccess) return api_cuda_fail(e, "fp8 block product");
   return api_ok();
@@ -131,21 +132,19 @@ int linear_impl(const void* x, int x_kind, int64_t ldx, const uint8_t* xs, int64
 // The experts' path: regions of the workspace after the counters.
 struct ExpertsPlan {
   Plan a, b;
-  int64_t rows, gu_ld;
-  size_t gu, y, partials, total;
+  int64_t rows;
+  size_t y, partials, total;
 };
 ExpertsPlan plan_experts(int64_t tokens, int64_t top, int64_t experts, int64_t h, int64_t i, int out_dtype) {
   ExpertsPlan E;
   E.rows = tokens * top;
   // A token picks an expert at most once.
   E.a = plan(E.rows, experts, tokens, 2 * i, h, 1);
-  E.b = plan(E.rows, experts, tokens, h, i, 0);
-  E.gu_ld = (int64_t)E.a.row_tiles * 128;
-  E.gu = align256((size_t)E.rows * E.gu_ld * 4);
+  E.b = plan(E.rows, experts, tokens, h, i, 0);  // the same tiles: nt depends on the rows only
   E.y = align256((size_t)E.rows * h * elem(out_dtype));
   const int nt = E.a.nt > E.b.nt ? E.a.nt : E.b.nt;
   E.partials = align256(fb_partial_bytes(nt, kSmsBound));
-  E.total = kWorkspaceCounterBytes + E.a.x8 + E.b.x8 + E.gu + E.y + E.partials;
+  E.total = kWorkspaceCounterBytes + E.a.x8 + E.b.x8 + E.y + E.partials;
   return E;
 }
 
@@ -268,7 +267,8 @@ int mambo_fp8b_grouped_linear(const void* x, int x_dtype, int64_t ldx, int group
 
 size_t mambo_moe_route_workspace_bytes(int64_t tokens, int64_t experts) {
   if (tokens < 1 || experts < 1) return 0;
-  return kWorkspaceCounterBytes + align256((size_t)((tokens + 127) / 128) * (experts + 1) * sizeof(int));
+  const int64_t chunk = fb_route_chunk(tokens);
+  return kWorkspaceCounterBytes + align256((size_t)((tokens + chunk - 1) / chunk) * (experts + 1) * sizeof(int));
 }
 
 int mambo_moe_route(const void* logits, int dtype, int64_t ld, const float* bias, int64_t tokens, int64_t experts,
@@ -294,6 +294,7 @@ int mambo_moe_route(const void* logits, int dtype, int64_t ld, const float* bias
   p.ld = ld;
   p.bias = bias;
   p.tokens = (int)tokens;
+  p.chunk = fb_route_chunk(tokens);
   p.experts = (int)experts;
   p.top = top;
   p.sigmoid = scoring == MAMBO_MOE_SIGMOID;
@@ -363,8 +364,6 @@ int mambo_moe_experts(const void* x, int x_dtype, int64_t ldx, int64_t tokens, c
   at += E.a.x8;
   const FbActivations ha = activations(E.b, at);
   at += E.b.x8;
-  float* gu = (float*)at;
-  at += E.gu;
   void* y = at;
   at += E.y;
   uint8_t* partials = at;
@@ -386,13 +385,9 @@ int mambo_moe_experts(const void* x, int x_dtype, int64_t ldx, int64_t tokens, c
   q.act = xa;
   cudaError_t e = launch_fb_quant(q, stream);
   if (e == cudaSuccess)
-    e = run_gemm(gate_up, E.a, xa, E.rows, offsets, gu, 0, E.gu_ld, (int)E.gu_ld, partials, workspace, sms, smem, stream);
-  if (e == cudaSuccess) {
-    FbHiddenParams hp{gu, E.gu_ld, E.rows, (int)i, (int)experts, offsets, ha};
-    e = launch_fb_hidden(hp, stream);
-  }
+    e = run_gemm(gate_up, E.a, xa, E.rows, offsets, nullptr, 0, 0, &ha, partials, workspace, sms, smem, stream);
   if (e == cudaSuccess)
-    e = run_gemm(down, E.b, ha, E.rows, offsets, y, out_dtype == MAMBO_BF16, h, (int)h, partials, workspace, sms, smem,
+    e = run_gemm(down, E.b, ha, E.rows, offsets, y, out_dtype == MAMBO_BF16, h, nullptr, partials, workspace, sms, smem,
                  stream);
   if (e == cudaSuccess) {
     FbCombineParams c{y, out_dtype == MAMBO_BF16, h, positions, weights, (int)tokens, top, (int)h, E.rows, out,

@@ -105,19 +105,6 @@ __device__ __forceinline__ FbDst fb_dst(const FbActivations& a, const FbPlace& p
   d.swz = row & 7;
   return d;
 }
-// Stores the 8 values of chunk c (0..15) of K block kb, and with the first chunk the block's four scale codes (for
-// both CTAs of a pair).
-__device__ __forceinline__ void fb_store(const FbActivations& a, const FbDst& d, int64_t kb, int c, uint2 q,
-                                         uint32_t word) {
-  if (!d.row) return;
-  const int64_t at = kb * fb_record_bytes(a.nt);
-  *reinterpret_cast<uint2*>(d.row + at + (((c >> 1) ^ d.swz) << 4) + (c & 1) * 8) = q;
-  if (c == 0) {
-    *reinterpret_cast<uint32_t*>(d.sf + at) = word;
-    if (fb_is_pair(a.nt)) *reinterpret_cast<uint32_t*>(d.sf + at + fb_part_bytes(a.nt)) = word;
-  }
-}
-
 __device__ __forceinline__ int clamp_offset(int o, int64_t total) { return o < 0 ? 0 : o > total ? (int)total : o; }
 #endif
 
@@ -179,6 +166,9 @@ struct FbGemmParams {
   void* out;           // [R][ldo]
   int out_bf16;
   int64_t ldo;
+  // Gate/up weights: h = silu(gate) * up of each row, quantized (MXFP8) into the
+  // next product's activations, in place of out; its tiles are cut as act's.
+  FbActivations hidden;  // x8 null: none
   int stages;
   int evict_weights;   // 1: weights are read once (evict-first)
   float* partials;     // [grid][2][128 * nt]
@@ -188,25 +178,15 @@ struct FbGemmParams {
 cudaError_t fb_status_symbols(void** status, void** limit);
 // Token-tile sizes the kernel is built for.
 int fb_tile_for(int64_t expected_rows);
-uint32_t fb_gemm_smem(int nt, int experts, int stages);
-int fb_gemm_stages(int nt, int experts, int smem_optin);
+uint32_t fb_gemm_smem(int nt, int experts, int stages, bool hidden);
+int fb_gemm_stages(int nt, int experts, int smem_optin, bool hidden);
 int fb_gemm_grid(int nt, int sms);
 size_t fb_partial_bytes(int nt, int sms);
 cudaError_t launch_fb_gemm(const FbGemmParams& p, int grid, cudaStream_t stream);
 
 // --- experts ----------------------------------------------------------------------
-struct FbHiddenParams {
-  const float* gu;  // [R][ld]: columns in the gate/up tile order
-  int64_t ld;
-  int64_t rows;     // R
-  int i;            // hidden features
-  int experts;
-  const int* offsets;
-  FbActivations act;
-};
-cudaError_t launch_fb_hidden(const FbHiddenParams& p, cudaStream_t stream);
-
 struct FbRouteParams {
+  int chunk;  // tokens of a CTA (fb_route_chunk)
   const void* logits;
   int bf16;
   int64_t ld;
@@ -221,7 +201,7 @@ struct FbRouteParams {
   int* rows;
   int* chunk_counts;  // workspace [chunks][experts + 1]
 };
-int fb_route_chunks(int tokens);
+int fb_route_chunk(int64_t tokens);
 cudaError_t launch_fb_route(const FbRouteParams& p, cudaStream_t stream);
 
 struct FbCombineParams {

@@ -28,6 +28,7 @@
 #include "fp8b.cuh"
 #include "iq3s_tm.cuh"
 #include "kernels.cuh"
+#include "mxfp8.cuh"
 #include "tcgen05.cuh"
 
 namespace mambo {
@@ -270,7 +271,7 @@ __device__ __forceinline__ void issue_block(uint32_t d, uint32_t a_lo, uint32_t 
 
 }  // namespace
 
-template <int NT, bool kPair>
+template <int NT, bool kPair, bool kHidden>
 __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(const __grid_constant__ FbGemmParams p) {
   using C = FbCfg<NT, kPair>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -279,10 +280,12 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
   int* tile_start = reinterpret_cast<int*>(tiles0 + (size_t)S * C::kStage);
   int* offs = tile_start + p.experts + 1;
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(tile_start) + fb_tables_bytes(p.experts));
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStagesB + 2 * 4 + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStagesB + 2 * 4 + 1 + 4);
+  float* xchg = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + kFbBarBytes);  // kHidden: 4 KB per two warps
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t kFull = bar0, kEmpty = bar0 + 8 * kMaxStagesB;
   const uint32_t kMdone = bar0 + 16 * kMaxStagesB, kEfree = kMdone + 8 * 4, kEdone = kEfree + 8 * 4;
+  const uint32_t kPairBar = kEdone + 8;  // kHidden: two epilogue warps meet, 4 of them
   static_assert(C::kD * C::kHalves <= 4, "barriers");
   // Values that the whole warp shares are broadcast from lane 0, so that the compiler keeps them, and what the MMAs
   // take as operands, in uniform registers.
@@ -304,6 +307,7 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
       mbar_init(kEfree + 8 * d, kPair ? 8 : 4);
     }
     mbar_init(kEdone, C::kEpiWarps);
+    for (int i = 0; i < 4; ++i) mbar_init(kPairBar + 8 * i, 2);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -555,6 +559,16 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
     int db = 0;
     uint32_t dph = 0;
     bool ok = true;
+    // kHidden: this warp and the one with the other half of its features meet (a bounded wait, as every one).
+    const uint32_t meet = kPairBar + 8u * (uint32_t)(h * 2 + (q >> 1));
+    uint32_t mph = 0;
+    auto pair_sync = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(meet);
+      const bool met = fb_warp_wait(meet, mph, kSiteFbFull);
+      mph ^= 1;
+      return met;
+    };
     while (ok && walk.next()) {
       const float* sw;
       int cols;  // this warp's valid columns (may be <= 0)
@@ -652,10 +666,24 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
         __syncwarp();
         int* counter = p.counters + (kPair ? first * 2 + rank : first) * 8 + (warp - 4);
         int done = 0;
-        if (lane == 0) done = atomic_add_acq_rel_gpu(counter, 1) == last - first;
-        done = __shfl_sync(0xFFFFFFFFu, done, 0);
-        if (!done) continue;
-        if (lane == 0) *counter = 0;  // all parts are in: zero again for the next launch
+        if constexpr (kHidden) {
+          // The two warps finish a tile together, so one of them counts for both, once both have published.
+          if (!(ok = pair_sync())) break;
+          int* flag = reinterpret_cast<int*>(xchg + (h * 2 + (q >> 1)) * 1024);
+          if (lane == 0 && (q & 1) == 0) {
+            *flag = atomic_add_acq_rel_gpu(counter, 1) == last - first;
+            if (*flag) *counter = 0;  // all parts are in: zero again for the next launch
+          }
+          if (!(ok = pair_sync())) break;
+          done = *flag;
+          if (!(ok = pair_sync())) break;  // before the flag's place is used again
+          if (!done) continue;
+        } else {
+          if (lane == 0) done = atomic_add_acq_rel_gpu(counter, 1) == last - first;
+          done = __shfl_sync(0xFFFFFFFFu, done, 0);
+          if (!done) continue;
+          if (lane == 0) *counter = 0;  // all parts are in: zero again for the next launch
+        }
         __threadfence();
 #pragma unroll
         for (int c = 0; c < C::kCols / 2; ++c) acc2[c] = 0;
@@ -673,6 +701,51 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
       }
       // Looked up again: held over the K loop, these would cost it registers.
       const FbTile t = cur.at(walk.tile);
+      if constexpr (kHidden) {
+        // The even warps hold gate rows, the odd ones the up rows of the same 32 features (a MXFP8 group of the next
+        // product's K). Both put 16 columns into shared memory at a time; of those the even warp forms h for the
+        // first eight, the odd one for the others: a lane per feature, so the group's maximum is one warp reduction.
+        float* mine = xchg + (h * 2 + (q >> 1)) * 1024;
+        const FbActivations& hid = p.hidden;
+        const int n0 = fb_split(t.n), per = (h ? (t.n + 15) / 16 * 16 - n0 : n0) / 2;
+        uint8_t* rec = hid.x8 + (t.slot * hid.kblocks + (kPair ? t.rt : t.rt >> 1)) * fb_record_bytes(NT);
+        const int rt = kPair ? rank : t.rt & 1;  // half of the 128-feature block
+        const int chunk = 4 * rt + (q & 2) + (lane >> 4);  // this lane's 16-byte chunk of the row
+        uint8_t* sf = rec + fb_part_rows(t.n, kPair) * 128 + h * kFbAtom + 2 * rt + (q >> 1);
+#pragma unroll 1
+        for (int b = 0; b < cols; b += 16) {
+#pragma unroll
+          for (int k = 0; k < C::kCols; k += 16) {
+            if (k == b) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) mine[(q & 1) * 512 + i * 32 + lane] = acc(k + i);
+            }
+          }
+          if (!(ok = pair_sync())) break;
+          const float* own = mine + 8 * (q & 1) * 32 + lane;
+          const int c8 = b + 8 * (q & 1);  // this warp's eight tokens, among this half's
+          uint32_t codes[8], bytes[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float g = own[i * 32], u = own[512 + i * 32];
+            // A quotient within 2 units in the last place: h is rounded to E4M3 next.
+            const float v = __fdividef(g, 1.0f + expf(-g)) * u;
+            codes[i] =
+                mxfp8_scale_code(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu)));
+            bytes[i] = cvt_e4m3x2_rn(v * e8m0_to_float(codes[i] == 0xFFu ? 0u : 254u - codes[i]), 0.f) & 0xFFu;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int c = c8 + i;
+            if (c >= cols) break;
+            const int part = kPair && c >= per, row = kPair ? c - part * per + h * (n0 / 2) : c;
+            rec[part * fb_part_bytes(NT) + row * 128 + ((chunk ^ (row & 7)) << 4) + (lane & 15)] = (uint8_t)bytes[i];
+            if (lane < (kPair ? 2 : 1)) sf[lane * fb_part_bytes(NT) + (c & 31) * 16 + (c >> 5) * 4] = (uint8_t)codes[i];
+          }
+          if (!(ok = pair_sync())) break;
+        }
+        continue;
+      }
       const int row = (kPair ? 2 * t.rt + rank : t.rt) * 128 + rl;
       if (row < p.n_rows) {
         const int64_t at = ((int64_t)t.o + t.row0 + (h ? fb_split(t.n) : 0)) * p.ldo + row;
@@ -704,17 +777,22 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
 namespace {
 
 template <int NT, bool kPair>
-uint32_t smem_of(int experts, int stages) {
+uint32_t smem_of(int experts, int stages, bool hidden) {
   using C = FbCfg<NT, kPair>;
-  return 1024 + (uint32_t)stages * C::kStage + fb_tables_bytes(experts) + kFbBarBytes;
+  return 1024 + (uint32_t)stages * C::kStage + fb_tables_bytes(experts) + kFbBarBytes +
+         (hidden ? (uint32_t)C::kEpiWarps / 2 * 4096 : 0u);
 }
-template <int NT, bool kPair>
-cudaError_t launch_nt(const FbGemmParams& p, int grid, cudaStream_t stream) {
-  const uint32_t smem = smem_of<NT, kPair>(p.experts, p.stages);
-  const void* k = (const void*)fb_gemm_kernel<NT, kPair>;
+template <int NT, bool kPair, bool kHidden>
+cudaError_t launch_kernel(const FbGemmParams& p, int grid, cudaStream_t stream) {
+  const uint32_t smem = smem_of<NT, kPair>(p.experts, p.stages, kHidden);
+  const void* k = (const void*)fb_gemm_kernel<NT, kPair, kHidden>;
   cudaError_t e = ensure_smem_attribute(k, smem);
   if (e != cudaSuccess) return e;
   return launch_pdl_cluster(k, dim3(grid), dim3(FbCfg<NT, kPair>::kThreads), smem, stream, kPair ? 2 : 1, p);
+}
+template <int NT, bool kPair>
+cudaError_t launch_nt(const FbGemmParams& p, int grid, cudaStream_t stream) {
+  return p.hidden.x8 ? launch_kernel<NT, kPair, true>(p, grid, stream) : launch_kernel<NT, kPair, false>(p, grid, stream);
 }
 
 }  // namespace
@@ -723,18 +801,18 @@ int fb_tile_for(int64_t expected_rows) {
   return expected_rows <= 16 ? 16 : expected_rows <= 32 ? 32 : expected_rows <= 64 ? 64 : kFbPairTokens;
 }
 
-uint32_t fb_gemm_smem(int nt, int experts, int stages) {
+uint32_t fb_gemm_smem(int nt, int experts, int stages, bool hidden) {
   switch (nt) {
-    case 16: return smem_of<16, false>(experts, stages);
-    case 32: return smem_of<32, false>(experts, stages);
-    case 64: return smem_of<64, false>(experts, stages);
-    default: return smem_of<kFbPairTokens, true>(experts, stages);
+    case 16: return smem_of<16, false>(experts, stages, hidden);
+    case 32: return smem_of<32, false>(experts, stages, hidden);
+    case 64: return smem_of<64, false>(experts, stages, hidden);
+    default: return smem_of<kFbPairTokens, true>(experts, stages, hidden);
   }
 }
 
-int fb_gemm_stages(int nt, int experts, int smem_optin) {
+int fb_gemm_stages(int nt, int experts, int smem_optin, bool hidden) {
   int s = kMaxStagesB;
-  while (s > 2 && (int)fb_gemm_smem(nt, experts, s) > smem_optin) --s;
+  while (s > 2 && (int)fb_gemm_smem(nt, experts, s, hidden) > smem_optin) --s;
   return s;
 }
 

@@ -64,6 +64,35 @@ namespace {
 
 constexpr int kSteps = 4, kSpan = 256 * kSteps;
 
+// 8 values of a lane, of a scale group of 4 (32 values) or 16 lanes: their E4M3 bytes, and the K block's four scale
+// codes as a word.
+__device__ __forceinline__ uint32_t scale_word(uint32_t code, int lane) {
+  uint32_t word = code << (8 * ((lane >> 2) & 3));
+  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
+  return word | __shfl_xor_sync(0xFFFFFFFFu, word, 8);
+}
+// bf16 pairs: the maximum of packed magnitudes (NaN wins) and packed multiplications.
+__device__ __forceinline__ uint2 quantize8(const uint4& c, int group, int lane, uint32_t& word) {
+  uint32_t a = absmax_bf16x2(absmax_bf16x2(c.x, c.y), absmax_bf16x2(c.z, c.w));
+  a = absmax_bf16x2(a, __shfl_xor_sync(0xFFFFFFFFu, a, 1));
+  a = absmax_bf16x2(a, __shfl_xor_sync(0xFFFFFFFFu, a, 2));
+  if (group == 128) {
+    a = absmax_bf16x2(a, __shfl_xor_sync(0xFFFFFFFFu, a, 4));
+    a = absmax_bf16x2(a, __shfl_xor_sync(0xFFFFFFFFu, a, 8));
+  }
+  const uint32_t code = mxfp8_scale_code(__uint_as_float(max(a & 0x7FFFu, (a >> 16) & 0x7FFFu) << 16));
+  const float inv = e8m0_to_float(code == 0xFFu ? 0u : 254u - code);
+  const uint32_t w4[4] = {c.x, c.y, c.z, c.w};
+  uint32_t b[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float lo, hi;
+    mul2(lo, hi, __uint_as_float(w4[j] << 16), __uint_as_float(w4[j] & 0xFFFF0000u), inv, inv);
+    b[j] = cvt_e4m3x2_rn(lo, hi);
+  }
+  word = scale_word(code, lane);
+  return make_uint2(prmt(b[0], b[1], 0x5410u), prmt(b[2], b[3], 0x5410u));
+}
 __device__ __forceinline__ uint2 quantize8(const float (&v)[8], int group, int lane, uint32_t& word) {
   // Largest magnitude as bits: NaN orders above infinity, so either gives the group the code 0xFF.
   uint32_t m = 0;
@@ -82,28 +111,16 @@ __device__ __forceinline__ uint2 quantize8(const float (&v)[8], int group, int l
   for (int h = 0; h < 2; ++h)
     packed[h] = cvt_e4m3x2_rn(v[4 * h] * inv, v[4 * h + 1] * inv) |
                 (cvt_e4m3x2_rn(v[4 * h + 2] * inv, v[4 * h + 3] * inv) << 16);
-  word = code << (8 * ((lane >> 2) & 3));
-  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
-  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
+  word = scale_word(code, lane);
   return make_uint2(packed[0], packed[1]);
 }
 
 }  // namespace
 
+// One item's loads: a row's span, 8 values a lane and step.
 template <int kIn, bool kVec>
-__global__ void __launch_bounds__(256) fb_quant_kernel(const __grid_constant__ FbQuantParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t spans = (p.k + kSpan - 1) / kSpan;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  pdl_wait();
-  pdl_launch_dependents();
-  if (item >= p.rows * spans) return;
-  const int64_t row = item / spans, span = item - row * spans;
-  const int64_t c0 = span * (kSpan / 8) + lane;        // first 8-value chunk of the lane
-  const int64_t chunks = (p.k + 127) / 128 * 16;       // whole K blocks
-  // All loads first.
-  uint4 raw[kSteps], raw2[kIn == MAMBO_F32 ? kSteps : 1];
-  (void)raw2;
+__device__ __forceinline__ void quant_load(const FbQuantParams& p, int64_t row, int64_t c0, uint4 (&raw)[kSteps],
+                                           uint4 (&raw2)[kIn == MAMBO_F32 ? kSteps : 1]) {
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int64_t k0 = (c0 + 32 * i) * 8;
@@ -147,7 +164,23 @@ __global__ void __launch_bounds__(256) fb_quant_kernel(const __grid_constant__ F
       }
     }
   }
-  // The row's places while they are on their way.
+}
+
+template <int kIn, bool kVec>
+__global__ void __launch_bounds__(256) fb_quant_kernel(const __grid_constant__ FbQuantParams p) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t spans = (uint32_t)((p.k + kSpan - 1) / kSpan);
+  const uint32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);  // the host keeps rows * spans below 2^31
+  pdl_wait();
+  pdl_launch_dependents();
+  if (item >= (uint32_t)p.rows * spans) return;
+  const uint32_t r32 = item / spans;
+  const int64_t row = r32;
+  const int c0 = (int)(item - r32 * spans) * (kSpan / 8) + lane;  // first 8-value chunk of the lane
+  const int chunks = (int)((p.k + 127) / 128 * 16);               // whole K blocks
+  uint4 raw[kSteps], raw2[kIn == MAMBO_F32 ? kSteps : 1];
+  quant_load<kIn, kVec>(p, row, c0, raw, raw2);
+  // The row's places.
   int copies = 1, expert = 0;
   FbDst dst;
   dst.row = nullptr;
@@ -173,7 +206,7 @@ __global__ void __launch_bounds__(256) fb_quant_kernel(const __grid_constant__ F
   for (int i = 0; i < kSteps; ++i) {
     if constexpr (kIn == kFbCodes) {
       q[i] = make_uint2(raw[i].x, raw[i].y);
-      const int64_t kb = (c0 + 32 * i) >> 4;
+      const int kb = (c0 + 32 * i) >> 4;
       const uint8_t* s = p.xs + row * p.lds;
       word[i] = 0;
       if (c0 + 32 * i < chunks) {
@@ -186,20 +219,14 @@ __global__ void __launch_bounds__(256) fb_quant_kernel(const __grid_constant__ F
         }
       }
     } else {
-      float v[8];
       if constexpr (kIn == MAMBO_BF16) {
-        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[2 * j] = __uint_as_float(w[j] << 16);
-          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-        }
+        q[i] = quantize8(raw[i], p.group, lane, word[i]);
       } else {
-        const uint32_t w[8] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w, raw2[i].x, raw2[i].y, raw2[i].z, raw2[i].w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+        const float v[8] = {__uint_as_float(raw[i].x),  __uint_as_float(raw[i].y),  __uint_as_float(raw[i].z),
+                            __uint_as_float(raw[i].w),  __uint_as_float(raw2[i].x), __uint_as_float(raw2[i].y),
+                            __uint_as_float(raw2[i].z), __uint_as_float(raw2[i].w)};
+        q[i] = quantize8(v, p.group, lane, word[i]);
       }
-      q[i] = quantize8(v, p.group, lane, word[i]);
     }
   }
   if (p.mode == kFbDense && p.values) {
@@ -234,16 +261,32 @@ __global__ void __launch_bounds__(256) fb_quant_kernel(const __grid_constant__ F
         if (pos >= o && pos < end) dst = fb_dst(p.act, fb_place(o, end - o, e, pos - o, p.act.nt));
       }
     }
+    if (!dst.row) continue;
+    // The lane's chunk of its K block is the same in every step, two blocks on.
+    const uint32_t rec = fb_record_bytes(p.act.nt);
+    const int64_t at = (int64_t)(c0 >> 4) * rec;
+    uint8_t* d = dst.row + at + ((((c0 & 15) >> 1) ^ dst.swz) << 4) + (c0 & 1) * 8;
+    uint8_t* sf = dst.sf + at;
+    const bool first = (c0 & 15) == 0, pair = fb_is_pair(p.act.nt);
+    const uint32_t other = fb_part_bytes(p.act.nt);
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      const int64_t c = c0 + 32 * i;
-      if (c < chunks) fb_store(p.act, dst, c >> 4, (int)(c & 15), q[i], word[i]);
+      if (c0 + 32 * i < chunks) {
+        *reinterpret_cast<uint2*>(d) = q[i];
+        if (first) {
+          *reinterpret_cast<uint32_t*>(sf) = word[i];
+          if (pair) *reinterpret_cast<uint32_t*>(sf + other) = word[i];  // both CTAs' parts
+        }
+      }
+      d += 2 * rec;
+      sf += 2 * rec;
     }
   }
 }
 
 cudaError_t launch_fb_quant(const FbQuantParams& p, cudaStream_t stream) {
   const int64_t items = p.rows * ((p.k + kSpan - 1) / kSpan);
+  if (items >= (int64_t)1 << 31) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)((items + 7) / 8));
   const int esize = p.x_kind == MAMBO_F32 ? 4 : p.x_kind == MAMBO_BF16 ? 2 : 1;
   const int align = p.x_kind == kFbCodes ? 8 : 16;

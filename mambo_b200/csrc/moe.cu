@@ -10,8 +10,6 @@ namespace {
 
 constexpr int kRouteThreads = 512;
 constexpr int kRouteWarps = kRouteThreads / 32;
-// Tokens of a chunk: one CTA. A call of one chunk is one launch.
-constexpr int kRouteChunk = 128;
 
 // Monotone map of a float to an unsigned key (0 is free: it marks masked experts).
 __device__ __forceinline__ uint32_t order_key(float f) {
@@ -36,84 +34,90 @@ __device__ __forceinline__ void route_load(const FbRouteParams& p, int token, in
   }
 }
 
+// The probability of a logit, before any renormalization.
+__device__ __forceinline__ float route_prob(bool sigmoid, float l, float top, float sum) {
+  return sigmoid ? 1.0f / (1.0f + expf(-l)) : expf(l - top) / sum;
+}
+
 template <int NV>
 __device__ __forceinline__ void route_token(const FbRouteParams& p, int token, int lane, const float (&raw)[NV],
                                             const float (&bias)[NV], int* hist) {
-  float l[NV], prob[NV];
   uint32_t key[NV];
-  float top = -INFINITY;
+  float top = -INFINITY, sum = 0.f;
+  float l[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const float v = raw[i];
     l[i] = v == v ? fminf(v, 3.4028234663852886e38f) : -INFINITY;
     top = fmaxf(top, l[i]);
   }
-  if (p.sigmoid) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      prob[i] = 1.0f / (1.0f + expf(-l[i]));
-      const float s = prob[i] + bias[i];
-      key[i] = l[i] == -INFINITY || s != s ? 0u : order_key(s);
-    }
-  } else {
+  if (!p.sigmoid) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      prob[i] = l[i] == -INFINITY ? 0.f : expf(l[i] - top);
-      sum += prob[i];
-    }
+    for (int i = 0; i < NV; ++i) sum += l[i] == -INFINITY ? 0.f : expf(l[i] - top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      prob[i] = sum > 0.f ? prob[i] / sum : 0.f;
-      const float s = l[i] + bias[i];
-      key[i] = l[i] == -INFINITY || s != s ? 0u : order_key(s);
-    }
   }
-  // Each lane's best key and its slot (the first of equal keys: the lowest expert of the lane).
-  uint32_t best = 0;
-  int at = 0;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (key[i] > best) {
-      best = key[i];
-      at = i;
-    }
-  float total = 0.f, mine_w = 0.f;
+  for (int i = 0; i < NV; ++i) {
+    const float s = (p.sigmoid ? 1.0f / (1.0f + expf(-l[i])) : l[i]) + bias[i];
+    key[i] = l[i] == -INFINITY || s != s ? 0u : order_key(s);
+  }
+  // Each lane's best two keys and their slots (the first of equal keys: the lowest expert of the lane). A lane whose
+  // best is taken goes on with the second; only one that is taken again looks through its keys anew.
+  uint32_t best = 0, second = 0, taken = 0;
+  int at = 0, at2 = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const bool b1 = key[i] > best, b2 = key[i] > second;
+    second = b1 ? best : b2 ? key[i] : second;
+    at2 = b1 ? at : b2 ? i : at2;
+    best = b1 ? key[i] : best;
+    at = b1 ? i : at;
+  }
+  bool have2 = true;
   int mine_id = -1;
   for (int j = 0; j < p.top; ++j) {
     const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, best);
     if (m == 0) break;  // no expert left
     const uint32_t id = __reduce_min_sync(0xFFFFFFFFu, best == m ? (uint32_t)(32 * at + lane) : 0xFFFFFFFFu);
-    float w = 0.f;
-    if (lane == (int)(id & 31)) {  // the lane that had it takes its next best
-      best = 0;
-      const int taken = at;
+    if (lane == j) mine_id = (int)id;
+    const bool won = lane == (int)(id & 31);
+    if (won) taken |= 1u << at;
+    if (__any_sync(0xFFFFFFFFu, won && !have2)) {
+      if (won) {
+        best = 0;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (i == taken) {
-          w = prob[i];
-          key[i] = 0;
-        } else if (key[i] > best) {
-          best = key[i];
-          at = i;
-        }
+        for (int i = 0; i < NV; ++i)
+          if (!((taken >> i) & 1u) && key[i] > best) {
+            best = key[i];
+            at = i;
+          }
       }
-    }
-    w = __shfl_sync(0xFFFFFFFFu, w, (int)(id & 31));
-    total += w;
-    if (lane == j) {
-      mine_w = w;
-      mine_id = (int)id;
+    } else if (won) {
+      best = second;
+      at = at2;
+      have2 = false;
     }
   }
-  if (p.renormalize) mine_w = total > 0.f ? mine_w / total : 0.f;
+  // Lane j has the j-th choice: its probability from its logit, once more.
+  float w = 0.f;
+  if (mine_id >= 0) {
+    const int64_t from = (int64_t)token * p.ld + mine_id;
+    const float v = p.bf16 ? __uint_as_float((uint32_t)__ldg((const uint16_t*)p.logits + from) << 16)
+                           : __ldg((const float*)p.logits + from);
+    w = route_prob(p.sigmoid, fminf(v, 3.4028234663852886e38f), top, sum);
+  }
+  if (p.renormalize) {
+    float total = w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+    w = total > 0.f ? w / total : 0.f;
+  }
   if (lane < p.top) {
     p.ids[(int64_t)token * p.top + lane] = mine_id;
-    p.weights[(int64_t)token * p.top + lane] = mine_w * p.scale;
+    p.weights[(int64_t)token * p.top + lane] = w * p.scale;
     atomicAdd(hist + (mine_id < 0 ? p.experts : mine_id), 1);  // whole numbers: the order does not matter
   }
 }
@@ -182,11 +186,11 @@ __device__ __forceinline__ void place_chunk(const FbRouteParams& p, int first, i
 // Selection of a chunk's tokens, a warp per token, and the chunk's counts per
 // expert; with one chunk also the placement. Latency-bound in decode.
 template <int NV>
-__global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const __grid_constant__ FbRouteParams p) {
+__global__ void __launch_bounds__(kRouteThreads, NV <= 8 ? 2 : 1) moe_route_kernel(const __grid_constant__ FbRouteParams p) {
   extern __shared__ int route_sm[];
   int* hist = route_sm;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, buckets = p.experts + 1;
-  const int first = blockIdx.x * kRouteChunk, count = min(kRouteChunk, p.tokens - first);
+  const int first = blockIdx.x * p.chunk, count = min(p.chunk, p.tokens - first);
   for (int i = threadIdx.x; i < buckets; i += kRouteThreads) hist[i] = 0;
   __syncthreads();
   pdl_wait();
@@ -220,7 +224,7 @@ __global__ void __launch_bounds__(kRouteThreads) moe_place_kernel(const __grid_c
   int* base = route_sm;            // totals, then first rows
   int* before = base + buckets;    // counts of earlier chunks
   int* wcnt = before + buckets;
-  const int first = blockIdx.x * kRouteChunk, count = min(kRouteChunk, p.tokens - first);
+  const int first = blockIdx.x * p.chunk, count = min(p.chunk, p.tokens - first);
   pdl_wait();
   pdl_launch_dependents();
   // Warps take (32 buckets, part of the chunks), so that the loads of all are in flight.
@@ -252,10 +256,15 @@ __global__ void __launch_bounds__(kRouteThreads) moe_place_kernel(const __grid_c
   place_chunk(p, first, count, before, wcnt, warp, lane);
 }
 
-int fb_route_chunks(int tokens) { return (tokens + kRouteChunk - 1) / kRouteChunk; }
+// Tokens of a chunk, one CTA: up to 64 tokens are one chunk and one launch; beyond that about 256 chunks, so that
+// every SM ranks (a token's ranking is a chain of some 3000 clocks) and the placement still sums few counts.
+int fb_route_chunk(int64_t tokens) {
+  const int64_t per = (tokens + 255) / 256;
+  return tokens <= 64 ? 64 : (int)(per < 16 ? 16 : per);
+}
 
 cudaError_t launch_fb_route(const FbRouteParams& p, cudaStream_t stream) {
-  const int chunks = fb_route_chunks(p.tokens), buckets = p.experts + 1;
+  const int chunks = (p.tokens + p.chunk - 1) / p.chunk, buckets = p.experts + 1;
   const size_t smem = (size_t)buckets * (1 + kRouteWarps) * sizeof(int);
   const int nv = (p.experts + 31) / 32;
   const void* k = nv <= 2   ? (const void*)moe_route_kernel<2>
@@ -269,56 +278,6 @@ cudaError_t launch_fb_route(const FbRouteParams& p, cudaStream_t stream) {
   const size_t place = (size_t)buckets * (2 + kRouteWarps) * sizeof(int);
   e = ensure_smem_attribute((const void*)moe_place_kernel, place);
   return e != cudaSuccess ? e : launch_pdl((const void*)moe_place_kernel, dim3(chunks), dim3(kRouteThreads), place, stream, p);
-}
-
-// --------------------------------------------------------------------------
-// h = silu(gate) * up of each routed row, quantized to MXFP8 from FP32 into
-// the second product's activation layout: a rounding of h to bf16 in between
-// would move 1-2 % of its E4M3 codes.
-// --------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) moe_hidden_kernel(const __grid_constant__ FbHiddenParams p) {
-  const int64_t row = blockIdx.y + (int64_t)blockIdx.z * 65535;
-  if (row >= p.rows) return;
-  const int lane = threadIdx.x & 31;
-  const int chunks = (p.i + 127) / 128 * 16, c = blockIdx.x * 256 + threadIdx.x;
-  pdl_wait();
-  pdl_launch_dependents();
-  int e = 0;
-  for (int b = 0; b < p.experts; b += 32) {
-    const int end = b + lane < p.experts ? __ldg(p.offsets + b + lane + 1) : 0x7FFFFFFF;
-    e += __popc(__ballot_sync(0xFFFFFFFFu, end <= row));
-  }
-  if (e >= p.experts) return;
-  const bool in = c < chunks;
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  if (in) {
-    const int f = c * 8;
-    const float* g = p.gu + row * p.ld + 128 * (f >> 6) + 64 * ((f >> 5) & 1) + (f & 31);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float gate = __ldg(g + i), up = __ldg(g + 32 + i);
-      v[i] = gate / (1.0f + expf(-gate)) * up;
-    }
-  }
-  uint2 q;
-  const uint32_t code = mxfp8_quad_rne(v, q);
-  uint32_t word = code << (8 * ((lane >> 2) & 3));
-  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
-  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
-  if (!in) return;
-  const int o = clamp_offset(__ldg(p.offsets + e), p.rows), end = clamp_offset(__ldg(p.offsets + e + 1), p.rows);
-  const int local = (int)row - o;
-  if (local < 0 || end <= o) return;
-  fb_store(p.act, fb_dst(p.act, fb_place(o, end - o, e, local, p.act.nt)), c >> 4, c & 15, q, word);
-}
-
-cudaError_t launch_fb_hidden(const FbHiddenParams& p, cudaStream_t stream) {
-  const int chunks = (p.i + 127) / 128 * 16;
-  const dim3 grid((unsigned)((chunks + 255) / 256), (unsigned)(p.rows < 65535 ? p.rows : 65535),
-                  (unsigned)((p.rows + 65534) / 65535));
-  return launch_pdl((const void*)moe_hidden_kernel, grid, dim3(256), 0, stream, p);
 }
 
 // --------------------------------------------------------------------------
