@@ -703,47 +703,65 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
       const FbTile t = cur.at(walk.tile);
       if constexpr (kHidden) {
         // The even warps hold gate rows, the odd ones the up rows of the same 32 features (a MXFP8 group of the next
-        // product's K). Both put 16 columns into shared memory at a time; of those the even warp forms h for the
-        // first eight, the odd one for the others: a lane per feature, so the group's maximum is one warp reduction.
-        float* mine = xchg + (h * 2 + (q >> 1)) * 1024;
+        // product's K). Of 16 columns at a time the even warp forms h for the first eight, the odd one for the
+        // others: each sends the other eight over shared memory. Then a lane is a feature and a group's maximum is
+        // one warp reduction. Bound by instructions (some 25 a column), with the MMAs waiting: hence the packed
+        // code arithmetic below; a first version of 60 a column took 1073 us in all where this one takes XX.
         const FbActivations& hid = p.hidden;
+        const bool odd = q & 1;
         const int n0 = fb_split(t.n), per = (h ? (t.n + 15) / 16 * 16 - n0 : n0) / 2;
         uint8_t* rec = hid.x8 + (t.slot * hid.kblocks + (kPair ? t.rt : t.rt >> 1)) * fb_record_bytes(NT);
         const int rt = kPair ? rank : t.rt & 1;  // half of the 128-feature block
-        const int chunk = 4 * rt + (q & 2) + (lane >> 4);  // this lane's 16-byte chunk of the row
-        uint8_t* sf = rec + fb_part_rows(t.n, kPair) * 128 + h * kFbAtom + 2 * rt + (q >> 1);
+        uint8_t* row0 = rec + 64 * rt + 16 * (q & 2) + lane;  // the lane's byte of an unswizzled row
+        // Scale codes: lanes 0-7 store those of eight tokens, of a pair lanes 8-15 the other CTA's copy.
+        uint8_t* sf = rec + fb_part_rows(t.n, kPair) * 128 + h * kFbAtom + 2 * rt + (q >> 1) + (lane & 7) * 16 +
+                      (lane >= 8 ? fb_part_bytes(NT) : 0u);
+        float* xch = xchg + (h * 2 + (q >> 1)) * 1024 + lane;
 #pragma unroll 1
         for (int b = 0; b < cols; b += 16) {
+          float own[8], other[8];
+          float* buf = xch + (b & 16) * 32;  // two buffers: one meeting per turn
 #pragma unroll
           for (int k = 0; k < C::kCols; k += 16) {
             if (k == b) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) mine[(q & 1) * 512 + i * 32 + lane] = acc(k + i);
+              for (int i = 0; i < 8; ++i) {
+                own[i] = odd ? acc(k + 8 + i) : acc(k + i);
+                buf[(odd ? 256 : 0) + i * 32] = odd ? acc(k + i) : acc(k + 8 + i);
+              }
             }
           }
           if (!(ok = pair_sync())) break;
-          const float* own = mine + 8 * (q & 1) * 32 + lane;
-          const int c8 = b + 8 * (q & 1);  // this warp's eight tokens, among this half's
-          uint32_t codes[8], bytes[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) other[i] = buf[(odd ? 0 : 256) + i * 32];
+          const int c8 = b + (odd ? 8 : 0);  // this warp's eight tokens, among this half's
+          uint32_t most = 0;                 // lane i (mod 8): token i's largest magnitude
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float g = own[i * 32], u = own[512 + i * 32];
-            // A quotient within 2 units in the last place: h is rounded to E4M3 next.
-            const float v = __fdividef(g, 1.0f + expf(-g)) * u;
-            codes[i] =
-                mxfp8_scale_code(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu)));
-            bytes[i] = cvt_e4m3x2_rn(v * e8m0_to_float(codes[i] == 0xFFu ? 0u : 254u - codes[i]), 0.f) & 0xFFu;
+            const float g = odd ? other[i] : own[i], u = odd ? own[i] : other[i];
+            // The fast exponential and quotient: within some 2^-21 of the value, which E4M3 rounds by up to 2^-4.
+            own[i] = __fdividef(g, 1.0f + __expf(-g)) * u;
+            const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(own[i]) & 0x7FFFFFFFu);
+            if ((lane & 7) == i) most = m;
           }
+          const uint32_t code = mxfp8_scale_code(__uint_as_float(most));
+          const int part = kPair && c8 >= per;
+          // Eight tokens are eight rows of one swizzle group of one part: row i lies 128 i on, its chunks xor i.
+          uint8_t* r8 = row0 + part * fb_part_bytes(NT) + (kPair ? c8 - part * per + h * (n0 / 2) : c8) * 128;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int c = c8 + i;
-            if (c >= cols) break;
-            const int part = kPair && c >= per, row = kPair ? c - part * per + h * (n0 / 2) : c;
-            rec[part * fb_part_bytes(NT) + row * 128 + ((chunk ^ (row & 7)) << 4) + (lane & 15)] = (uint8_t)bytes[i];
-            if (lane < (kPair ? 2 : 1)) sf[lane * fb_part_bytes(NT) + (c & 31) * 16 + (c >> 5) * 4] = (uint8_t)codes[i];
+          for (int i = 0; i < 8; i += 2) {
+            const uint32_t k0 = __shfl_sync(0xFFFFFFFFu, code, i), k1 = __shfl_sync(0xFFFFFFFFu, code, i + 1);
+            // 2^-e, e = code - 127; the bytes of a NaN group (code 255) do not matter.
+            const uint32_t two = cvt_e4m3x2_rn(own[i] * __uint_as_float((254u - k0) << 23),
+                                               own[i + 1] * __uint_as_float((254u - k1) << 23));
+            if (c8 + i < cols) *reinterpret_cast<uint8_t*>(((uintptr_t)r8 ^ (i << 4)) + 128 * i) = (uint8_t)two;
+            if (c8 + i + 1 < cols)
+              *reinterpret_cast<uint8_t*>(((uintptr_t)r8 ^ ((i + 1) << 4)) + 128 * (i + 1)) = (uint8_t)(two >> 8);
           }
-          if (!(ok = pair_sync())) break;
+          if (lane < (kPair ? 16 : 8) && c8 + (lane & 7) < cols) sf[(c8 & 31) * 16 + (c8 >> 5) * 4] = (uint8_t)code;
         }
+        // The next tile's first turn may use either buffer: the other warp has read both.
+        if (ok) ok = pair_sync();
         continue;
       }
       const int row = (kPair ? 2 * t.rt + rank : t.rt) * 128 + rl;
