@@ -33,7 +33,7 @@ constexpr uint32_t kFbAtom = 512u;           // bytes of a scale-factor atom (12
 constexpr int kFbMaxExperts = 1024;
 
 // Tokens of a tile above which CTA pairs work on it (and the largest tile).
-constexpr int kFbPairTokens = 224;
+constexpr int kFbPairTokens = 192;
 
 struct FbActivations {
   uint8_t* x8;    // [slots][kblocks][record]

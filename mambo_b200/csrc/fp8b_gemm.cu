@@ -38,10 +38,9 @@ namespace {
 constexpr int kMaxStagesB = 12;
 
 // kPair: CTA pairs. A tile is 256 weight rows (a row tile per CTA) x NT tokens; each CTA loads half of the
-// tokens and the pair's tensor cores read both halves. The tile's tokens are two MMAs of up to 112, each with D
+// tokens and the pair's tensor cores read both halves. The tile's tokens are two MMAs of up to 96, each with D
 // buffers and epilogue warps of its own: a buffer's way through the epilogue then has the time of three other MMAs
-// (of one, as a single MMA of 224). 112 sums and two chunks of 32 loaded values are what an epilogue thread can hold:
-// with 2 x 128 sums it spilled, and a K block took 10 % longer.
+// (of one, as a single MMA of 192). 96 sums and 96 loaded values are what an epilogue thread can hold.
 template <int NT, bool kPair>
 struct FbCfg {
   static constexpr int kHalves = kPair ? 2 : 1;
@@ -202,6 +201,13 @@ __device__ __forceinline__ void wait_ld(uint32_t (&r)[N]) {
   } else {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) : : "memory");
   }
+}
+
+// Ties registers to the wait before: no use of them moves ahead of it.
+template <int N>
+__device__ __forceinline__ void tie(uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 
 // After a wait gave up: time for the bulk copies in flight to land before the CTA leaves its shared memory.
@@ -583,68 +589,45 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
 #pragma unroll
       for (int i = 0; i < C::kCols / 2; ++i) acc2[i] = 0;
       if (cols <= 0) continue;  // this half's MMAs are not issued either
-      // The columns pass in chunks through two register buffers: while one chunk is added, the next one's load is in
-      // flight, across the K blocks too (the next block's first load is issued before this block's last additions).
-      // A D buffer is released once its last chunk is in registers. Columns past the tile's are added like the
-      // others (whatever they hold) and never stored: a branch around them costs every tile more.
-      constexpr int kCh = C::kCols < 64 ? 16 : 32;
-      constexpr int kChunks = (C::kCols + kCh - 1) / kCh;
-      constexpr int kLast = C::kCols - (kChunks - 1) * kCh;  // columns of the last chunk
-      uint32_t v[2][kCh];
+      // A K block: all of the warp's columns to registers at once, the D buffer released, then the additions. The
+      // buffer's way back to the MMAs is what paces the kernel, and additions between its loads lengthen it: with
+      // chunks of 32 columns loaded ahead of their additions a K block of 224 tokens took 912 clocks, 505 without
+      // the additions. Columns past the tile's are added like the others (whatever they hold) and never stored.
       float sv = 0.f;
-      ok = fb_warp_wait(kMdone + 8 * (h * C::kD + db), dph, kSiteFbFull);
-      if (!ok) break;
-      tc::fence_after_sync();
-      ld_cols(tq0 + (uint32_t)db * C::kCols, v[0]);
 #pragma unroll 1
       for (int kb = walk.kb0; kb < walk.kb1; ++kb) {
         if (kb == walk.kb0 || (kb & 31) == 0) sv = (kb & ~31) + lane < KB ? __ldg(sw + (kb & ~31) + lane) : 0.f;
         const float w = __shfl_sync(0xFFFFFFFFu, sv, kb & 31);
         const uint64_t w2 = pack2(w, w);
-        const uint32_t tq = tq0 + (uint32_t)db * C::kCols;
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          uint32_t(&x)[kCh] = v[c & 1];
-          uint32_t(&y)[kCh] = v[(c + 1) & 1];
-          if (c + 1 < kChunks) {
-            wait_ld(x);
-            if (c + 2 < kChunks || kLast == kCh) {
-              ld_cols(tq + (c + 1) * kCh, y);
-            } else {
-              ld_cols(tq + (c + 1) * kCh, *reinterpret_cast<uint32_t(*)[kLast]>(&y));
-            }
-          } else {
-            wait_ld(*reinterpret_cast<uint32_t(*)[kLast]>(&x));
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-              if (kPair && rank != 0) {
-                arrive_remote(efree0 + 8 * db);
-              } else {
-                mbar_arrive(kEfree + 8 * (h * C::kD + db));
-              }
-            }
-            if (++db == C::kD) {
-              db = 0;
-              dph ^= 1;
-            }
-            if (kChunks > 1 && kb + 1 < walk.kb1) {
-              ok = fb_warp_wait(kMdone + 8 * (h * C::kD + db), dph, kSiteFbFull);
-              tc::fence_after_sync();
-              if (ok) ld_cols(tq0 + (uint32_t)db * C::kCols, y);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < (c + 1 < kChunks ? kCh : kLast) / 2; ++i)
-            acc2[c * kCh / 2 + i] =
-                fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), w2, acc2[c * kCh / 2 + i]);
-        }
-        if (kChunks == 1 && kb + 1 < walk.kb1) {  // one buffer
-          ok = fb_warp_wait(kMdone + 8 * (h * C::kD + db), dph, kSiteFbFull);
-          tc::fence_after_sync();
-          if (ok) ld_cols(tq0 + (uint32_t)db * C::kCols, v[0]);
-        }
+        ok = fb_warp_wait(kMdone + 8 * (h * C::kD + db), dph, kSiteFbFull);
         if (!ok) break;
+        tc::fence_after_sync();
+        constexpr int kCh = C::kCols < 32 ? C::kCols : 32;
+        uint32_t v[C::kCols / kCh][kCh];
+#pragma unroll
+        for (int c = 0; c < C::kCols / kCh; ++c) ld_cols(tq0 + (uint32_t)db * C::kCols + c * kCh, v[c]);
+        wait_ld(v[0]);
+#pragma unroll
+        for (int c = 1; c < C::kCols / kCh; ++c) tie(v[c]);
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if (kPair && rank != 0) {
+            arrive_remote(efree0 + 8 * db);
+          } else {
+            mbar_arrive(kEfree + 8 * (h * C::kD + db));
+          }
+        }
+        if (++db == C::kD) {
+          db = 0;
+          dph ^= 1;
+        }
+#pragma unroll
+        for (int c = 0; c < C::kCols / kCh; ++c)
+#pragma unroll
+          for (int i = 0; i < kCh / 2; ++i)
+            acc2[c * kCh / 2 + i] =
+                fma2(pack2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), w2, acc2[c * kCh / 2 + i]);
       }
       if (!ok) break;
       if (walk.kb0 != 0 || walk.kb1 != KB) {

@@ -53,6 +53,15 @@ class _NoGuard:
 
 
 _NO_GUARD = _NoGuard()
+
+
+def _stream(stream, device: torch.device) -> int:
+    """As _runtime.stream_handle; the current stream without building a torch.cuda.Stream (2 us of a call's 17)."""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    return _runtime.stream_handle(stream, device)
+
+
 _DTYPES = {torch.float32: _lib.MAMBO_F32, torch.bfloat16: _lib.MAMBO_BF16}
 
 
@@ -103,7 +112,7 @@ def prepare_fp8_block_fields(values, scales, *, gate_up: bool = False, stream=No
     out_scales = torch.empty(lib.mambo_fp8b_scales_bytes(experts, n, k, int(gate_up)) // 4, dtype=torch.float32,
                              device=dev)
     with _device_guard(dev):
-        st = _runtime.stream_handle(stream, dev)
+        st = _stream(stream, dev)
         _lib.check(lib.mambo_fp8b_pack(
             values.data_ptr(), experts, n, k, values.stride(0), values.stride(1), values.stride(2), scales.data_ptr(),
             scales.stride(0), scales.stride(1), scales.stride(2), int(gate_up), packed.data_ptr(),
@@ -127,7 +136,7 @@ def launch_quantize_fp8_block(x, *, group: int = BLOCK, stream=None) -> tuple[to
     scales = torch.empty((m, -(-k // group)), dtype=torch.uint8, device=x.device)
     if m:
         with _device_guard(x.device):
-            st = _runtime.stream_handle(stream, x.device)
+            st = _stream(stream, x.device)
             _lib.check(_lib.load().mambo_fp8b_quantize(
                 x.data_ptr(), _DTYPES[x.dtype], m, k, _row_stride(x), group, values.data_ptr(), k, scales.data_ptr(),
                 scales.shape[1], st), "launch_quantize_fp8_block")
@@ -191,7 +200,7 @@ def launch_fp8_block_matmul(x_values, x_scales, weight: Fp8BlockFields, *, strea
     out = _output(out, m, weight["n_rows"], out_dtype, dev)
     if m:
         with _device_guard(dev):
-            st = _runtime.stream_handle(stream, dev)
+            st = _stream(stream, dev)
             ws = _runtime.workspace(dev, st, _linear_workspace_bytes(m, 1, weight["n_rows"], k))
             _lib.check(_lib.load().mambo_fp8b_linear(
                 x_values.data_ptr(), _row_stride(x_values), x_scales.data_ptr(), _row_stride(x_scales), group, m,
@@ -218,7 +227,7 @@ def fp8_block_linear(x, weight: Fp8BlockFields, *, act_group: int = BLOCK, strea
     out = _output(out, m, n, out_dtype, dev)
     if m:
         with _device_guard(dev):
-            st = _runtime.stream_handle(stream, dev)
+            st = _stream(stream, dev)
             ws = _runtime.workspace(dev, st, _linear_workspace_bytes(m, 1, n, weight["k"]))
             _lib.check(_lib.load().mambo_fp8b_linear_fused(
                 x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), act_group, m, weight["weight"], out.data_ptr(),
@@ -244,7 +253,7 @@ def fp8_block_grouped_linear(x, offsets, weight: Fp8BlockFields, *, act_group: i
     out = _output(out, rows, n, out_dtype, dev)
     if rows:
         with _device_guard(dev):
-            st = _runtime.stream_handle(stream, dev)
+            st = _stream(stream, dev)
             ws = _runtime.workspace(dev, st, _linear_workspace_bytes(rows, experts, n, weight["k"]))
             _lib.check(_lib.load().mambo_fp8b_grouped_linear(
                 x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), act_group, rows, offsets.data_ptr(), weight["weight"],

@@ -21,7 +21,7 @@ from typing import TypedDict
 import torch
 
 from .. import _lib, _runtime
-from .fp8_block import _DTYPES, Fp8BlockFields, _device_guard, _output, _row_stride
+from .fp8_block import _DTYPES, Fp8BlockFields, _device_guard, _output, _row_stride, _stream
 
 _SCORING = {"softmax": _lib.MAMBO_MOE_SOFTMAX, "sigmoid": _lib.MAMBO_MOE_SIGMOID}
 
@@ -75,15 +75,13 @@ def launch_moe_route(logits, top_k: int, *, scoring: str = "softmax", bias=None,
     _runtime.require_device(dev)
     if logits.stride(1) != 1 and experts > 1:
         logits = logits.contiguous()
-    # One allocation: the float weights and the four integer outputs.
-    n = tokens * top_k
-    buf = torch.empty(4 * n + experts + 1, dtype=torch.int32, device=dev)
-    ids, weights, positions, rows, offsets = buf.split((n, n, n, n, experts + 1))
-    ids, positions = ids.view(tokens, top_k), positions.view(tokens, top_k)
-    weights = weights.view(torch.float32).view(tokens, top_k)
+    ids, positions, rows = torch.empty((3, tokens, top_k), dtype=torch.int32, device=dev).unbind(0)
+    rows = rows.view(-1)
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
     if tokens:
         with _device_guard(dev):
-            st = _runtime.stream_handle(stream, dev)
+            st = _stream(stream, dev)
             ws = _runtime.workspace(dev, st, _route_workspace_bytes(tokens, experts))
             _lib.check(_lib.load().mambo_moe_route(
                 logits.data_ptr(), _DTYPES[logits.dtype], _row_stride(logits), 0 if bias is None else bias.data_ptr(),
@@ -129,7 +127,7 @@ def launch_moe_combine(y, route: MoeRoute, *, stream=None, out_dtype: torch.dtyp
         out.zero_()
     elif tokens:
         with _device_guard(dev):
-            st = _runtime.stream_handle(stream, dev)
+            st = _stream(stream, dev)
             _lib.check(_lib.load().mambo_moe_combine(
                 y.data_ptr(), _DTYPES[y.dtype], _row_stride(y), rows, route["positions"].data_ptr(),
                 route["weights"].data_ptr(), tokens, top, h, out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), st),
@@ -171,7 +169,7 @@ def fp8_moe_experts(x, route: MoeRoute, gate_up: Fp8BlockFields, down: Fp8BlockF
     if tokens:
         code = _DTYPES[out.dtype]
         with _device_guard(dev):
-            st = _runtime.stream_handle(stream, dev)
+            st = _stream(stream, dev)
             ws = _runtime.workspace(dev, st, _experts_workspace_bytes(tokens, top, experts, h, i, code))
             _lib.check(_lib.load().mambo_moe_experts(
                 x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), tokens, route["ids"].data_ptr(),
