@@ -36,6 +36,12 @@ namespace mambo {
 namespace {
 
 constexpr int kMaxStagesB = 12;
+constexpr int kWorth = 12, kWorthPair = 30;
+// Whether the CTAs that the last wave leaves idle lose kWorth K blocks on average.
+__host__ __device__ inline bool fb_split_pays(int64_t tiles, int64_t kblocks, int64_t ctas) {
+  const int64_t rem = tiles % ctas;
+  return rem && (ctas - rem) * kblocks >= kWorth * ctas;
+}
 
 // kPair: CTA pairs. A tile is 256 weight rows (a row tile per CTA) x NT tokens; each CTA loads half of the
 // tokens and the pair's tensor cores read both halves. The tile's tokens are two MMAs of up to 96, each with D
@@ -64,25 +70,44 @@ __host__ __device__ inline uint32_t fb_tables_bytes(int experts) {
   return ((uint32_t)(experts + 1) * 8 + 127) / 128 * 128;  // tile and row prefix
 }
 
-// This CTA's share of the tiles: a stream-K range over the first sk tiles,
-// then one tile of each whole wave.
-struct FbWalk {
-  int kb_n, sk, waves, ncl, cl, nsk;
-  int u, u1, units;  // the host keeps tiles * K blocks below 2^31
-  int wave;
+// This CTA's share of the tiles. Whole: one tile of each wave. kSplit: where the last wave would leave too many CTAs idle
+// for too long, an equal range of the K blocks of the last one to two waves comes first (stream-K); the parts' sums
+// have to be published and added up, which is worth it once the idle CTAs lose some kWorth K blocks on average.
+template <bool kSplit>
+struct FbWalk;
+template <>
+struct FbWalk<false> {
+  int kb_n, tiles, ncl, at;
+  int tile, kb1;  // the current segment
+  static constexpr int kb0 = 0;
+  __device__ __forceinline__ FbWalk(int tiles_, int kblocks, int cl, int ncl_)
+      : kb_n(kblocks), tiles(tiles_), ncl(ncl_), at(cl), tile(0), kb1(kblocks) {}
+  __device__ __forceinline__ bool next() {
+    tile = at;
+    at += ncl;
+    return tile < tiles;
+  }
+};
+template <>
+struct FbWalk<true> {
+  int kb_n, sk, tiles, ncl, cl, nsk;
+  int u, u1, units;    // the host keeps tiles * K blocks below 2^31
+  int at;              // next whole tile
   int tile, kb0, kb1;  // the current segment
-  __device__ __forceinline__ FbWalk(int tiles, int kblocks, int cl_, int ncl_) {
+  __device__ __forceinline__ FbWalk(int tiles_, int kblocks, int cl_, int ncl_) {
     kb_n = kblocks;
+    tiles = tiles_;
     ncl = ncl_;
     cl = cl_;
-    waves = tiles / ncl;
-    if (tiles % ncl && waves > 0) --waves;
-    sk = tiles - waves * ncl;
+    const int rem = tiles % ncl;
+    sk = 0;
+    if (fb_split_pays(tiles, kb_n, ncl)) sk = tiles < ncl ? rem : rem + ncl;
     units = sk * kb_n;
-    nsk = units < ncl ? units : ncl;
+    // Each part at least four K blocks.
+    nsk = max(1, min(ncl, units / 4));
     u = cl < nsk ? (int)((int64_t)cl * units / nsk) : 0;
     u1 = cl < nsk ? (int)((int64_t)(cl + 1) * units / nsk) : 0;
-    wave = 0;
+    at = sk + cl;
     tile = kb0 = kb1 = 0;
   }
   __device__ __forceinline__ bool next() {
@@ -93,9 +118,9 @@ struct FbWalk {
       u += kb1 - kb0;
       return true;
     }
-    if (wave < waves) {
-      tile = sk + wave * ncl + cl;
-      ++wave;
+    if (at < tiles) {
+      tile = at;
+      at += ncl;
       kb0 = 0;
       kb1 = kb_n;
       return true;
@@ -115,7 +140,7 @@ struct FbTile {
 struct FbCursor {
   const int* tiles;  // [experts + 1] first tile of each expert
   const int* offs;   // [experts + 1] clamped, non-decreasing
-  int experts, nt, e;
+  int experts, nt, row_groups, e;
   __device__ __forceinline__ FbTile at(int tile) {
     while (e + 1 < experts && tile >= tiles[e + 1]) ++e;
     FbTile t;
@@ -123,9 +148,11 @@ struct FbCursor {
     t.o = offs[e];
     const int count = offs[e + 1] - t.o;
     const int tt_n = fb_tiles(count, nt), tr = fb_tile_rows(count, tt_n);
-    const int local = tile - tiles[e];
-    t.rt = local / tt_n;  // row group: of the pair, in pairs
-    const int tt = local - t.rt * tt_n;
+    // Blocks of 8 row groups; inside one, token tile by token tile: the tiles that run together then read the fewest
+    // weight and token rows (some 8 groups x 9 token tiles on 74 pairs, instead of 3 x all).
+    const int local = tile - tiles[e], per = 8 * tt_n, block = local / per, in = local - block * per;
+    const int rows = min(8, row_groups - 8 * block), tt = in / rows;
+    t.rt = 8 * block + (in - tt * rows);  // row group: of the pair, in pairs
     t.row0 = tt * tr;
     t.n = count - t.row0 < tr ? count - t.row0 : tr;
     t.slot = fb_slot_start(t.o, e, nt) + tt;
@@ -277,7 +304,7 @@ __device__ __forceinline__ void issue_block(uint32_t d, uint32_t a_lo, uint32_t 
 
 }  // namespace
 
-template <int NT, bool kPair, bool kHidden>
+template <int NT, bool kPair, bool kHidden, bool kSplit>
 __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(const __grid_constant__ FbGemmParams p) {
   using C = FbCfg<NT, kPair>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -383,8 +410,8 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
   if constexpr (kPair) cluster_sync_all();  // both CTAs' barriers and TMEM are ready before any remote use
   tc::fence_after_sync();
 
-  FbWalk walk(uniform(tile_start[p.experts]), KB, (int)blockIdx.x / (kPair ? 2 : 1), (int)gridDim.x / (kPair ? 2 : 1));
-  FbCursor cur{tile_start, offs, p.experts, NT, 0};
+  FbWalk<kSplit> walk(uniform(tile_start[p.experts]), KB, (int)blockIdx.x / (kPair ? 2 : 1), (int)gridDim.x / (kPair ? 2 : 1));
+  FbCursor cur{tile_start, offs, p.experts, NT, row_groups, 0};
 
   // Register split of the pair kernel, launched with 168 a thread (384 threads): 128 x 56 + 256 x 224 = 384 x 168.
   // Each instruction opens its own branch, so that the compiler knows every role's count.
@@ -630,7 +657,7 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
                 fma2(pack2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), w2, acc2[c * kCh / 2 + i]);
       }
       if (!ok) break;
-      if (walk.kb0 != 0 || walk.kb1 != KB) {
+      if constexpr (kSplit) if (walk.kb0 != 0 || walk.kb1 != KB) {
         // A tile shared between CTAs: publish this warp's part, and sum all
         // parts in K order if it is the last to arrive.
         const int u_tile = walk.tile * KB;
@@ -644,9 +671,9 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
         float4* mine = part(walk.cl);
 #pragma unroll
         for (int c = 0; c < C::kCols; c += 4)
-          if (c < cols) __stcg(mine + (c / 4) * 128, make_float4(acc(c), acc(c + 1), acc(c + 2), acc(c + 3)));
-        __threadfence();
-        __syncwarp();
+          if (C::kCols <= 32 || c < cols)
+            __stcg(mine + (c / 4) * 128, make_float4(acc(c), acc(c + 1), acc(c + 2), acc(c + 3)));
+        __syncwarp();  // orders the warp's stores before the counting lane's release
         int* counter = p.counters + (kPair ? first * 2 + rank : first) * 8 + (warp - 4);
         int done = 0;
         if constexpr (kHidden) {
@@ -667,17 +694,40 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
           if (!done) continue;
           if (lane == 0) *counter = 0;  // all parts are in: zero again for the next launch
         }
-        __threadfence();
+        __syncwarp();
 #pragma unroll
         for (int c = 0; c < C::kCols / 2; ++c) acc2[c] = 0;
-        for (int cta = first; cta <= last; ++cta) {
-          const float4* src = part(cta);
+        // The parts in K order. Of a small tile several parts' loads are in flight at once; a large one's columns are
+        // enough, and holding more would cost its K loop registers.
+        constexpr int kBatch = C::kCols <= 16 ? 8 : C::kCols <= 32 ? 4 : 1;
+        for (int cta = first; cta <= last; cta += kBatch) {
+          if constexpr (kBatch == 1) {
+            const float4* src = part(cta);
 #pragma unroll
-          for (int c = 0; c < C::kCols; c += 4) {
-            if (c < cols) {
-              const float4 v = __ldcg(src + (c / 4) * 128);
-              acc2[c / 2] = pack2(acc(c) + v.x, acc(c + 1) + v.y);
-              acc2[c / 2 + 1] = pack2(acc(c + 2) + v.z, acc(c + 3) + v.w);
+            for (int c = 0; c < C::kCols; c += 4) {
+              if (c < cols) {
+                const float4 v = __ldcg(src + (c / 4) * 128);
+                acc2[c / 2] = pack2(acc(c) + v.x, acc(c + 1) + v.y);
+                acc2[c / 2 + 1] = pack2(acc(c + 2) + v.z, acc(c + 3) + v.w);
+              }
+            }
+          } else {
+            float4 v[kBatch][C::kCols / 4];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+              const float4* src = part(min(cta + j, last));
+#pragma unroll
+              for (int c = 0; c < C::kCols; c += 4) v[j][c / 4] = __ldcg(src + (c / 4) * 128);
+            }
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+              if (cta + j <= last) {
+#pragma unroll
+                for (int c = 0; c < C::kCols; c += 4) {
+                  acc2[c / 2] = pack2(acc(c) + v[j][c / 4].x, acc(c + 1) + v[j][c / 4].y);
+                  acc2[c / 2 + 1] = pack2(acc(c + 2) + v[j][c / 4].z, acc(c + 3) + v[j][c / 4].w);
+                }
+              }
             }
           }
         }
@@ -783,17 +833,29 @@ uint32_t smem_of(int experts, int stages, bool hidden) {
   return 1024 + (uint32_t)stages * C::kStage + fb_tables_bytes(experts) + kFbBarBytes +
          (hidden ? (uint32_t)C::kEpiWarps / 2 * 4096 : 0u);
 }
-template <int NT, bool kPair, bool kHidden>
+template <int NT, bool kPair, bool kHidden, bool kSplit>
 cudaError_t launch_kernel(const FbGemmParams& p, int grid, cudaStream_t stream) {
   const uint32_t smem = smem_of<NT, kPair>(p.experts, p.stages, kHidden);
-  const void* k = (const void*)fb_gemm_kernel<NT, kPair, kHidden>;
+  const void* k = (const void*)fb_gemm_kernel<NT, kPair, kHidden, kSplit>;
   cudaError_t e = ensure_smem_attribute(k, smem);
   if (e != cudaSuccess) return e;
   return launch_pdl_cluster(k, dim3(grid), dim3(FbCfg<NT, kPair>::kThreads), smem, stream, kPair ? 2 : 1, p);
 }
-template <int NT, bool kPair>
-cudaError_t launch_nt(const FbGemmParams& p, int grid, cudaStream_t stream) {
-  return p.hidden.x8 ? launch_kernel<NT, kPair, true>(p, grid, stream) : launch_kernel<NT, kPair, false>(p, grid, stream);
+// Single CTAs decide on the device whether to split (an expert-grouped call's tiles are counted there). A CTA pair's
+// partial sums are large (98 KB a CTA): only a call whose tiles leave most pairs idle for long splits, and the others
+// run a kernel without that code, which also keeps its registers (14336 x 4096 at 2048 tokens: 131 us, with it 148).
+template <int NT>
+cudaError_t launch_one(const FbGemmParams& p, int grid, cudaStream_t stream) {
+  return p.hidden.x8 ? launch_kernel<NT, false, true, true>(p, grid, stream)
+                     : launch_kernel<NT, false, false, true>(p, grid, stream);
+}
+cudaError_t launch_pair(const FbGemmParams& p, int grid, cudaStream_t stream) {
+  constexpr int NT = kFbPairTokens;
+  if (p.hidden.x8) return launch_kernel<NT, true, true, false>(p, grid, stream);
+  const int64_t tiles = (int64_t)(p.row_tiles + 1) / 2 * fb_tiles((int)p.rows, NT), pairs = grid / 2;
+  if (!p.offsets && 2 * tiles <= pairs && (pairs - tiles) * p.act.kblocks >= kWorthPair * pairs)
+    return launch_kernel<NT, true, false, true>(p, grid, stream);
+  return launch_kernel<NT, true, false, false>(p, grid, stream);
 }
 
 }  // namespace
@@ -827,10 +889,10 @@ size_t fb_partial_bytes(int nt, int sms) { return (size_t)sms * 2 * 128 * nt * s
 
 cudaError_t launch_fb_gemm(const FbGemmParams& p, int grid, cudaStream_t stream) {
   switch (p.act.nt) {
-    case 16: return launch_nt<16, false>(p, grid, stream);
-    case 32: return launch_nt<32, false>(p, grid, stream);
-    case 64: return launch_nt<64, false>(p, grid, stream);
-    default: return launch_nt<kFbPairTokens, true>(p, grid, stream);
+    case 16: return launch_one<16>(p, grid, stream);
+    case 32: return launch_one<32>(p, grid, stream);
+    case 64: return launch_one<64>(p, grid, stream);
+    default: return launch_pair(p, grid, stream);
   }
 }
 
