@@ -499,17 +499,17 @@ MAMBO_API int mambo_moe_combine(const void* y, int y_dtype, int64_t ldy, int64_t
  * A layer of routed experts: x [tokens, H] -> MXFP8 -> gate and up of the
  * chosen experts -> h = silu(gate) * up -> MXFP8 (from FP32) -> down -> the
  * weighted sum of each token's rows. gate_up: a gate/up weight [experts, 2I,
- * H]; down [experts, H, I]; ids, weights, positions and offsets from
- * mambo_moe_route. Each expert row rounds once to out_dtype before the sum.
+ * H]; down [experts, H, I]; ids, weights, positions, offsets and rows (or
+ * NULL: without it a decode call takes one more launch) from mambo_moe_route. Each expert row rounds once to out_dtype before the sum.
  * workspace: mambo_moe_experts_workspace_bytes(), zero-filled once.
  */
 MAMBO_API size_t mambo_moe_experts_workspace_bytes(int64_t tokens, int top, int64_t experts, int64_t h, int64_t i,
                                                    int out_dtype);
 MAMBO_API int mambo_moe_experts(const void* x, int x_dtype, int64_t ldx, int64_t tokens, const int32_t* ids,
-                                const float* weights, const int32_t* positions, const int32_t* offsets, int top,
-                                const MamboFp8BlockWeight* gate_up, const MamboFp8BlockWeight* down, void* out,
-                                int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
-                                mambo_stream_t stream);
+                                const float* weights, const int32_t* positions, const int32_t* offsets,
+                                const int32_t* rows, int top, const MamboFp8BlockWeight* gate_up,
+                                const MamboFp8BlockWeight* down, void* out, int out_dtype, int64_t ldo,
+                                void* workspace, size_t workspace_bytes, mambo_stream_t stream);
 
 /* Number of tunable configurations of a kernel kind, and the i-th one (for the autotuner).
  * Replaces the search spaces of make_benchmark_cases (src/python/mambo/kernels/iq3_s_fp8.py:402-465). */

@@ -328,7 +328,7 @@ def load() -> ctypes.CDLL:
             "mambo_moe_combine": ([vp, i32, i64, i64, vp, vp, i64, i32, i64, vp, i32, i64, vp], i32),
             "mambo_moe_experts_workspace_bytes": ([i64, i32, i64, i64, i64, i32], ctypes.c_size_t),
             "mambo_moe_experts": (
-                [vp, i32, i64, i64, vp, vp, vp, vp, i32, ctypes.POINTER(MamboFp8BlockWeight),
+                [vp, i32, i64, i64, vp, vp, vp, vp, vp, i32, ctypes.POINTER(MamboFp8BlockWeight),
                  ctypes.POINTER(MamboFp8BlockWeight), vp, i32, i64, vp, ctypes.c_size_t, vp],
                 i32,
             ),

@@ -59,10 +59,25 @@ int check_workspace(void* ws, size_t have, size_t need) {
   return MAMBO_OK;
 }
 
-cudaError_t run_gemm(const MamboFp8BlockWeight* w, const Plan& P, const FbActivations& act, int64_t rows,
+FbSource source(const void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t k, int group) {
+  FbSource s{};
+  s.x = x;
+  s.bf16 = x_dtype == MAMBO_BF16;
+  s.vec = (uintptr_t)x % 16 == 0 && ldx * elem(x_dtype) % 16 == 0;
+  s.ldx = ldx;
+  s.k = k;
+  s.group = group;
+  s.top = 1;
+  s.last = (int)(rows - 1);
+  return s;
+}
+
+// src: activations that the product quantizes itself, else act holds them.
+cudaError_t run_gemm(const MamboFp8BlockWeight* w, const Plan& P, const FbSource* src, const FbActivations& act, int64_t rows,
                      const int* offsets, void* out, int out_bf16, int64_t ldo, const FbActivations* hidden, uint8_t* partials,
                      void* workspace, int sms, int smem_optin, cudaStream_t stream) {
   FbGemmParams g{};
+  if (src) g.src = *src;
   g.packed = (const uint8_t*)w->packed;
   g.scales = w->scales;
   g.act = act;
@@ -107,24 +122,31 @@ int linear_impl(const void* x, int x_kind, int64_t ldx, const uint8_t* xs, int64
   if (st != MAMBO_OK) return st;
   uint8_t* at = (uint8_t*)workspace + kWorkspaceCounterBytes;
   const FbActivations act = activations(P, at);
-  FbQuantParams q{};
-  q.x = x;
-  q.x_kind = x_kind;
-  q.xs = xs;
-  q.lds = lds;
-  q.ldx = ldx;
-  q.rows = m;
-  q.k = w->k;
-  q.group = group;
-  q.mode = offsets ? kFbGrouped : kFbDense;
-  q.experts = (int)experts;
-  q.offsets = offsets;
-  q.total_rows = m;
-  q.act = act;
-  cudaError_t e = launch_fb_quant(q, stream);
-  if (e != cudaSuccess) return api_cuda_fail(e, "fp8 block quantizer");
-  e = run_gemm(w, P, act, m, offsets, out, out_dtype == MAMBO_BF16, ldo, nullptr, at + P.x8, workspace,
-               sms, smem, stream);
+  cudaError_t e;
+  if (x_kind != kFbCodes && m <= kFbQuantTokens) {
+    const FbSource src = source(x, x_kind, ldx, m, w->k, group);
+    e = run_gemm(w, P, &src, act, m, offsets, out, out_dtype == MAMBO_BF16, ldo, nullptr, at + P.x8, workspace, sms, smem,
+                 stream);
+  } else {
+    FbQuantParams q{};
+    q.x = x;
+    q.x_kind = x_kind;
+    q.xs = xs;
+    q.lds = lds;
+    q.ldx = ldx;
+    q.rows = m;
+    q.k = w->k;
+    q.group = group;
+    q.mode = offsets ? kFbGrouped : kFbDense;
+    q.experts = (int)experts;
+    q.offsets = offsets;
+    q.total_rows = m;
+    q.act = act;
+    e = launch_fb_quant(q, stream);
+    if (e != cudaSuccess) return api_cuda_fail(e, "fp8 block quantizer");
+    e = run_gemm(w, P, nullptr, act, m, offsets, out, out_dtype == MAMBO_BF16, ldo, nullptr, at + P.x8, workspace, sms,
+                 smem, stream);
+  }
   if (e != cudaSuccess) return api_cuda_fail(e, "fp8 block product");
   return api_ok();
 }
@@ -336,8 +358,8 @@ size_t mambo_moe_experts_workspace_bytes(int64_t tokens, int top, int64_t expert
 }
 
 int mambo_moe_experts(const void* x, int x_dtype, int64_t ldx, int64_t tokens, const int32_t* ids,
-                      const float* weights, const int32_t* positions, const int32_t* offsets, int top,
-                      const MamboFp8BlockWeight* gate_up, const MamboFp8BlockWeight* down, void* out, int out_dtype,
+                      const float* weights, const int32_t* positions, const int32_t* offsets, const int32_t* rows,
+                      int top, const MamboFp8BlockWeight* gate_up, const MamboFp8BlockWeight* down, void* out, int out_dtype,
                       int64_t ldo, void* workspace, size_t workspace_bytes, mambo_stream_t stream_) {
   if (!x || !ids || !weights || !positions || !offsets || !out) return api_fail(MAMBO_EINVAL, "null pointer");
   int st = check_weight(gate_up);
@@ -368,27 +390,35 @@ int mambo_moe_experts(const void* x, int x_dtype, int64_t ldx, int64_t tokens, c
   at += E.y;
   uint8_t* partials = at;
 
-  FbQuantParams q{};
-  q.x = x;
-  q.x_kind = x_dtype;
-  q.ldx = ldx;
-  q.rows = tokens;
-  q.k = h;
-  q.group = 32;
-  q.mode = kFbRouted;
-  q.experts = (int)experts;
-  q.offsets = offsets;
-  q.ids = ids;
-  q.positions = positions;
-  q.top = top;
-  q.total_rows = E.rows;
-  q.act = xa;
-  cudaError_t e = launch_fb_quant(q, stream);
+  cudaError_t e;
+  if (rows && tokens <= kFbQuantTokens) {  // an expert has at most one row of a token
+    FbSource src = source(x, x_dtype, ldx, tokens, h, 32);
+    src.rows = rows;
+    src.top = top;
+    e = run_gemm(gate_up, E.a, &src, xa, E.rows, offsets, nullptr, 0, 0, &ha, partials, workspace, sms, smem, stream);
+  } else {
+    FbQuantParams q{};
+    q.x = x;
+    q.x_kind = x_dtype;
+    q.ldx = ldx;
+    q.rows = tokens;
+    q.k = h;
+    q.group = 32;
+    q.mode = kFbRouted;
+    q.experts = (int)experts;
+    q.offsets = offsets;
+    q.ids = ids;
+    q.positions = positions;
+    q.top = top;
+    q.total_rows = E.rows;
+    q.act = xa;
+    e = launch_fb_quant(q, stream);
+    if (e == cudaSuccess)
+      e = run_gemm(gate_up, E.a, nullptr, xa, E.rows, offsets, nullptr, 0, 0, &ha, partials, workspace, sms, smem, stream);
+  }
   if (e == cudaSuccess)
-    e = run_gemm(gate_up, E.a, xa, E.rows, offsets, nullptr, 0, 0, &ha, partials, workspace, sms, smem, stream);
-  if (e == cudaSuccess)
-    e = run_gemm(down, E.b, ha, E.rows, offsets, y, out_dtype == MAMBO_BF16, h, nullptr, partials, workspace, sms, smem,
-                 stream);
+    e = run_gemm(down, E.b, nullptr, ha, E.rows, offsets, y, out_dtype == MAMBO_BF16, h, nullptr, partials, workspace, sms,
+                 smem, stream);
   if (e == cudaSuccess) {
     FbCombineParams c{y, out_dtype == MAMBO_BF16, h, positions, weights, (int)tokens, top, (int)h, E.rows, out,
                       out_dtype == MAMBO_BF16, ldo};

@@ -47,7 +47,7 @@ __host__ __device__ inline bool fb_split_pays(int64_t tiles, int64_t kblocks, in
 // tokens and the pair's tensor cores read both halves. The tile's tokens are two MMAs of up to 96, each with D
 // buffers and epilogue warps of its own: a buffer's way through the epilogue then has the time of three other MMAs
 // (of one, as a single MMA of 192). 96 sums and 96 loaded values are what an epilogue thread can hold.
-template <int NT, bool kPair>
+template <int NT, bool kPair, bool kQuant = false>
 struct FbCfg {
   static constexpr int kHalves = kPair ? 2 : 1;
   static constexpr int kEpiWarps = 4 * kHalves;
@@ -58,7 +58,8 @@ struct FbCfg {
   static constexpr uint32_t kSfb = kSfa + 16;
   static constexpr uint32_t kTmemUsed = kSfb + 4 * kD * kHalves;
   static constexpr uint32_t kTmem = kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
-  static constexpr int kThreads = (4 + kEpiWarps) * 32;
+  static constexpr int kQuantWarps = kQuant ? 4 : 0;
+  static constexpr int kThreads = (4 + kEpiWarps + kQuantWarps) * 32;
   // A stage: the weight record and this CTA's part of the activation record, both on 1024-byte boundaries.
   static constexpr uint32_t kStage = (kFbRecord + fb_part_bytes(NT) + 1023) / 1024 * 1024;
   static_assert(kCols % 16 == 0 && kSfa % 16 == 0 && kTmemUsed <= 512, "TMEM plan");
@@ -304,9 +305,10 @@ __device__ __forceinline__ void issue_block(uint32_t d, uint32_t a_lo, uint32_t 
 
 }  // namespace
 
-template <int NT, bool kPair, bool kHidden, bool kSplit>
-__global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(const __grid_constant__ FbGemmParams p) {
-  using C = FbCfg<NT, kPair>;
+template <int NT, bool kPair, bool kHidden, bool kSplit, bool kQuant>
+__global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm_kernel(const __grid_constant__ FbGemmParams p) {
+  using C = FbCfg<NT, kPair, kQuant>;
+  static_assert(!kQuant || (!kPair && NT == 16), "quantizing warps: tiles of 16 tokens");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* tiles0 = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int S = p.stages;
@@ -420,6 +422,9 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
   if (warp == 0) {
     // -------------------------------------------------------------- weights producer
     if (lane == 0) {
+      // Weights may be read ahead of the previous kernel's end where that is the quantizer, which waited for all
+      // before it; a kernel that is the first of its call may follow the one that packed them.
+      if (kQuant) pdl_wait();
       const uint64_t policy = l2_policy_evict_first();
       int it = 0, s = 0;
       uint32_t ph = 0;
@@ -457,7 +462,7 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
     __syncwarp();
   } else if (warp == 2) {
     // -------------------------------------------------------------- activations producer
-    if (lane == 0) {
+    if (!kQuant && lane == 0) {
       pdl_wait();
       int it = 0, s = 0;
       uint32_t ph = 0;
@@ -574,6 +579,78 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair>::kThreads, 1) fb_gemm_kernel(
       }
     }
   }
+  } else if (kQuant && warp >= 8) {
+    // -------------------------------------------------------------- quantizing warps
+    // For tiles of one or two tokens: four warps take the K blocks in turn and write each block's E4M3 bytes and scale
+    // codes straight into its stage, a half warp a token, 8 values a lane. Every tile's CTA quantizes the tokens anew:
+    // for one token that is less than a launch of the quantizer (4096 x 4096: 11.2 -> 10.6 us, 64 experts of 2048 x
+    // 1408, six a token: 32.0 -> 27.9), for eight it held the weights up (28672 x 8192: 39 -> 54 us).
+    const FbSource& src = p.src;
+    const int who = warp - 8, col = (lane & 15) * 8, r = lane >> 4;
+    pdl_wait();
+    int it = 0;
+    bool ok = true;
+    while (ok && walk.next()) {
+      const FbTile t = cur.at(walk.tile);
+      const int mine = t.o + t.row0 + min(r, t.n - 1);
+      const int64_t row = min(src.rows ? max(__ldg(src.rows + mine), 0) / src.top : mine, src.last) * src.ldx;
+      const uint32_t sf_at = kFbRecord + (uint32_t)fb_part_rows(t.n, false) * 128u;
+      auto load = [&](int kb, uint4& lo, uint4& hi) {
+        const int64_t k0 = (int64_t)kb * 128 + col;
+        lo = hi = make_uint4(0, 0, 0, 0);
+        if (src.bf16) {
+          const uint16_t* x = reinterpret_cast<const uint16_t*>(src.x) + row + k0;
+          if (src.vec && k0 + 8 <= src.k) {
+            lo = __ldg(reinterpret_cast<const uint4*>(x));
+          } else {
+            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (k0 + i < src.k) w[i >> 1] |= (uint32_t)__ldg(x + i) << (16 * (i & 1));
+            lo = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else {
+          const uint32_t* x = reinterpret_cast<const uint32_t*>(src.x) + row + k0;
+          if (src.vec && k0 + 8 <= src.k) {
+            lo = __ldg(reinterpret_cast<const uint4*>(x));
+            hi = __ldg(reinterpret_cast<const uint4*>(x) + 1);
+          } else {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = k0 + i < src.k ? __ldg(x + i) : 0u;
+            lo = make_uint4(w[0], w[1], w[2], w[3]);
+            hi = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+        }
+      };
+      int kb = walk.kb0 + ((who - it) & 3);  // this warp's first block of the segment
+      uint4 lo, hi, lo2, hi2;
+      if (kb < walk.kb1) load(kb, lo, hi);
+      for (; kb < walk.kb1; kb += 4) {
+        if (kb + 4 < walk.kb1) load(kb + 4, lo2, hi2);
+        const int at = it + (kb - walk.kb0), s = at % S;
+        if (at >= S && !(ok = fb_warp_wait(kEmpty + 8 * s, (uint32_t)(at / S - 1) & 1u, kSiteFbEmpty))) break;
+        uint8_t* st = tiles0 + (size_t)s * C::kStage;
+        uint32_t word;
+        uint2 q;
+        if (src.bf16) {
+          q = quantize8(lo, src.group, lane, word);
+        } else {
+          const float v[8] = {__uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w),
+                              __uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w)};
+          q = quantize8(v, src.group, lane, word);
+        }
+        *reinterpret_cast<uint2*>(st + kFbRecord + r * 128 + ((((lane & 15) >> 1) ^ r) << 4) + (lane & 1) * 8) = q;
+        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(st + sf_at + r * 16) = word;
+        fence_proxy_async_shared();  // the tensor core reads the stage through the async proxy
+        __syncwarp();
+        if (lane == 0) mbar_arrive(kFull + 8 * s);
+        lo = lo2;
+        hi = hi2;
+      }
+      it += walk.kb1 - walk.kb0;
+    }
+    __syncwarp();
   } else {
     if constexpr (kPair) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // -------------------------------------------------------------- epilogue
@@ -833,21 +910,21 @@ uint32_t smem_of(int experts, int stages, bool hidden) {
   return 1024 + (uint32_t)stages * C::kStage + fb_tables_bytes(experts) + kFbBarBytes +
          (hidden ? (uint32_t)C::kEpiWarps / 2 * 4096 : 0u);
 }
-template <int NT, bool kPair, bool kHidden, bool kSplit>
+template <int NT, bool kPair, bool kHidden, bool kSplit, bool kQuant = false>
 cudaError_t launch_kernel(const FbGemmParams& p, int grid, cudaStream_t stream) {
   const uint32_t smem = smem_of<NT, kPair>(p.experts, p.stages, kHidden);
-  const void* k = (const void*)fb_gemm_kernel<NT, kPair, kHidden, kSplit>;
+  const void* k = (const void*)fb_gemm_kernel<NT, kPair, kHidden, kSplit, kQuant>;
   cudaError_t e = ensure_smem_attribute(k, smem);
   if (e != cudaSuccess) return e;
-  return launch_pdl_cluster(k, dim3(grid), dim3(FbCfg<NT, kPair>::kThreads), smem, stream, kPair ? 2 : 1, p);
+  return launch_pdl_cluster(k, dim3(grid), dim3(FbCfg<NT, kPair, kQuant>::kThreads), smem, stream, kPair ? 2 : 1, p);
 }
 // Single CTAs decide on the device whether to split (an expert-grouped call's tiles are counted there). A CTA pair's
 // partial sums are large (98 KB a CTA): only a call whose tiles leave most pairs idle for long splits, and the others
 // run a kernel without that code, which also keeps its registers (14336 x 4096 at 2048 tokens: 131 us, with it 148).
-template <int NT>
+template <int NT, bool kQuant = false>
 cudaError_t launch_one(const FbGemmParams& p, int grid, cudaStream_t stream) {
-  return p.hidden.x8 ? launch_kernel<NT, false, true, true>(p, grid, stream)
-                     : launch_kernel<NT, false, false, true>(p, grid, stream);
+  return p.hidden.x8 ? launch_kernel<NT, false, true, true, kQuant>(p, grid, stream)
+                     : launch_kernel<NT, false, false, true, kQuant>(p, grid, stream);
 }
 cudaError_t launch_pair(const FbGemmParams& p, int grid, cudaStream_t stream) {
   constexpr int NT = kFbPairTokens;
@@ -889,7 +966,7 @@ size_t fb_partial_bytes(int nt, int sms) { return (size_t)sms * 2 * 128 * nt * s
 
 cudaError_t launch_fb_gemm(const FbGemmParams& p, int grid, cudaStream_t stream) {
   switch (p.act.nt) {
-    case 16: return launch_one<16>(p, grid, stream);
+    case 16: return p.src.x ? launch_one<16, true>(p, grid, stream) : launch_one<16>(p, grid, stream);
     case 32: return launch_one<32>(p, grid, stream);
     case 64: return launch_one<64>(p, grid, stream);
     default: return launch_pair(p, grid, stream);

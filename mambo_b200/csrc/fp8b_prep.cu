@@ -64,57 +64,6 @@ namespace {
 
 constexpr int kSteps = 4, kSpan = 256 * kSteps;
 
-// 8 values of a lane, of a scale group of 4 (32 values) or 16 lanes: their E4M3 bytes, and the K block's four scale
-// codes as a word.
-__device__ __forceinline__ uint32_t scale_word(uint32_t code, int lane) {
-  uint32_t word = code << (8 * ((lane >> 2) & 3));
-  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
-  return word | __shfl_xor_sync(0xFFFFFFFFu, word, 8);
-}
-// bf16 pairs: the maximum of packed magnitudes (NaN wins) and packed multiplications.
-__device__ __forceinline__ uint2 quantize8(const uint4& c, int group, int lane, uint32_t& word) {
-  uint32_t a = absmax_bf16x2(absmax_bf16x2(c.x, c.y), absmax_bf16x2(c.z, c.w));
-  a = absmax_bf16x2(a, __shfl_xor_sync(0xFFFFFFFFu, a, 1));
-  a = absmax_bf16x2(a, __shfl_xor_sync(0xFFFFFFFFu, a, 2));
-  if (group == 128) {
-    a = absmax_bf16x2(a, __shfl_xor_sync(0xFFFFFFFFu, a, 4));
-    a = absmax_bf16x2(a, __shfl_xor_sync(0xFFFFFFFFu, a, 8));
-  }
-  const uint32_t code = mxfp8_scale_code(__uint_as_float(max(a & 0x7FFFu, (a >> 16) & 0x7FFFu) << 16));
-  const float inv = e8m0_to_float(code == 0xFFu ? 0u : 254u - code);
-  const uint32_t w4[4] = {c.x, c.y, c.z, c.w};
-  uint32_t b[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float lo, hi;
-    mul2(lo, hi, __uint_as_float(w4[j] << 16), __uint_as_float(w4[j] & 0xFFFF0000u), inv, inv);
-    b[j] = cvt_e4m3x2_rn(lo, hi);
-  }
-  word = scale_word(code, lane);
-  return make_uint2(prmt(b[0], b[1], 0x5410u), prmt(b[2], b[3], 0x5410u));
-}
-__device__ __forceinline__ uint2 quantize8(const float (&v)[8], int group, int lane, uint32_t& word) {
-  // Largest magnitude as bits: NaN orders above infinity, so either gives the group the code 0xFF.
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-  m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-  if (group == 128) {
-    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 4));
-    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
-  }
-  const uint32_t code = mxfp8_scale_code(__uint_as_float(m));
-  const float inv = e8m0_to_float(code == 0xFFu ? 0u : 254u - code);
-  uint32_t packed[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    packed[h] = cvt_e4m3x2_rn(v[4 * h] * inv, v[4 * h + 1] * inv) |
-                (cvt_e4m3x2_rn(v[4 * h + 2] * inv, v[4 * h + 3] * inv) << 16);
-  word = scale_word(code, lane);
-  return make_uint2(packed[0], packed[1]);
-}
-
 }  // namespace
 
 // One item's loads: a row's span, 8 values a lane and step.

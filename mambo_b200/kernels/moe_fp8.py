@@ -75,10 +75,13 @@ def launch_moe_route(logits, top_k: int, *, scoring: str = "softmax", bias=None,
     _runtime.require_device(dev)
     if logits.stride(1) != 1 and experts > 1:
         logits = logits.contiguous()
-    ids, positions, rows = torch.empty((3, tokens, top_k), dtype=torch.int32, device=dev).unbind(0)
-    rows = rows.view(-1)
-    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
-    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
+    # One allocation: the four integer outputs and the float weights between them.
+    n = tokens * top_k
+    buf = torch.empty(4 * n + experts + 1, dtype=torch.int32, device=dev)
+    shape, strides = (tokens, top_k), (top_k, 1)
+    ids, positions = buf.as_strided(shape, strides, 0), buf.as_strided(shape, strides, n)
+    weights = buf.view(torch.float32).as_strided(shape, strides, 2 * n)
+    rows, offsets = buf.as_strided((n,), (1,), 3 * n), buf.as_strided((experts + 1,), (1,), 4 * n)
     if tokens:
         with _device_guard(dev):
             st = _stream(stream, dev)
@@ -95,16 +98,16 @@ def launch_moe_route(logits, top_k: int, *, scoring: str = "softmax", bias=None,
 
 def _check_route(route: MoeRoute, tokens: int, device: torch.device) -> int:
     """top_k of a route for `tokens` tokens."""
-    ids, weights, positions = route["ids"], route["weights"], route["positions"]
+    ids, weights, positions, rows = route["ids"], route["weights"], route["positions"], route["rows"]
     if ids.ndim != 2 or ids.shape[0] != tokens or weights.shape != ids.shape or positions.shape != ids.shape:
         raise ValueError("route must have ids, weights and positions [T,top_k] for the activation's T")
     if ids.dtype != torch.int32 or positions.dtype != torch.int32 or weights.dtype != torch.float32 \
-            or route["offsets"].dtype != torch.int32:
-        raise ValueError("route must have int32 ids, positions and offsets and float32 weights")
-    if not (ids.is_contiguous() and weights.is_contiguous() and positions.is_contiguous()
+            or route["offsets"].dtype != torch.int32 or rows.dtype != torch.int32 or rows.numel() != ids.numel():
+        raise ValueError("route must have int32 ids, positions, rows and offsets and float32 weights")
+    if not (ids.is_contiguous() and rows.is_contiguous() and weights.is_contiguous() and positions.is_contiguous()
             and route["offsets"].is_contiguous()):
         raise ValueError("route tensors must be contiguous")
-    if ids.device != device or weights.device != device or positions.device != device \
+    if ids.device != device or rows.device != device or weights.device != device or positions.device != device \
             or route["offsets"].device != device:
         raise ValueError("route and activation must be on one device")
     return ids.shape[1]
@@ -173,7 +176,7 @@ def fp8_moe_experts(x, route: MoeRoute, gate_up: Fp8BlockFields, down: Fp8BlockF
             ws = _runtime.workspace(dev, st, _experts_workspace_bytes(tokens, top, experts, h, i, code))
             _lib.check(_lib.load().mambo_moe_experts(
                 x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), tokens, route["ids"].data_ptr(),
-                route["weights"].data_ptr(), route["positions"].data_ptr(), route["offsets"].data_ptr(), top,
-                gate_up["weight"], down["weight"], out.data_ptr(), code, _row_stride(out), ws.data_ptr(), ws.numel(),
+                route["weights"].data_ptr(), route["positions"].data_ptr(), route["offsets"].data_ptr(),
+                route["rows"].data_ptr(), top, gate_up["weight"], down["weight"], out.data_ptr(), code, _row_stride(out), ws.data_ptr(), ws.numel(),
                 st), "fp8_moe_experts")
     return out
