@@ -72,6 +72,14 @@ FbSource source(const void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t k
   return s;
 }
 
+// Tiles times K blocks are counted in 32 bits, and the quantizer's spans too.
+int check_size(const Plan& P, int64_t rows, int64_t experts, int64_t k) {
+  const double tiles = (double)(rows / P.nt + experts) * P.row_tiles;
+  if (tiles * P.kblocks >= 2147483647.0 || (double)rows * (double)((k + 1023) / 1024) >= 2147483647.0)
+    return api_fail(MAMBO_EINVAL, "the call is too large: split its rows");
+  return MAMBO_OK;
+}
+
 // src: activations that the product quantizes itself, else act holds them.
 cudaError_t run_gemm(const MamboFp8BlockWeight* w, const Plan& P, const FbSource* src, const FbActivations& act, int64_t rows,
                      const int* offsets, void* out, int out_bf16, int64_t ldo, const FbActivations* hidden, uint8_t* partials,
@@ -91,10 +99,11 @@ cudaError_t run_gemm(const MamboFp8BlockWeight* w, const Plan& P, const FbSource
   g.ldo = ldo;
   if (hidden) g.hidden = *hidden;
   g.stages = fb_gemm_stages(P.nt, g.experts, smem_optin, hidden != nullptr);
-  g.evict_weights = rows <= P.nt;
+  // Most experts have one token tile at most (twice the even share fits it): their weights are read once.
+  g.evict_weights = offsets ? !fb_is_pair(P.nt) : rows <= P.nt;
   g.partials = (float*)partials;
   g.counters = (int*)((uint8_t*)workspace + kWorkspaceSplitCounterOffset);
-  return launch_fb_gemm(g, fb_gemm_grid(P.nt, sms), stream);
+  return launch_fb_gemm(g, fb_gemm_grid(P.nt, sms < kSmsBound ? sms : kSmsBound), stream);
 }
 
 int check_linear(const void* x, int64_t m, int group, const MamboFp8BlockWeight* w, const void* out, int out_dtype,
@@ -118,6 +127,8 @@ int linear_impl(const void* x, int x_kind, int64_t ldx, const uint8_t* xs, int64
   if (st != MAMBO_OK) return st;
   const int64_t experts = offsets ? w->n_experts : 1;
   const Plan P = plan(m, experts, m, w->n_rows, w->k, 0);
+  st = check_size(P, m, experts, w->k);
+  if (st != MAMBO_OK) return st;
   st = check_workspace(workspace, workspace_bytes, kWorkspaceCounterBytes + product_bytes(P));
   if (st != MAMBO_OK) return st;
   uint8_t* at = (uint8_t*)workspace + kWorkspaceCounterBytes;
@@ -226,6 +237,7 @@ int mambo_fp8b_quantize(const void* x, int x_dtype, int64_t m, int64_t k, int64_
   if (m < 1 || m > kMaxRows || k < 1 || k > kMaxExtent) return api_fail(MAMBO_EINVAL, "activation must be [M,K] with M, K >= 1");
   if (group != 32 && group != 128) return api_fail(MAMBO_EINVAL, "activation scales are per 32 or per 128 values");
   if (ldx < k || ldq < k || lds < (k + group - 1) / group) return api_fail(MAMBO_EINVAL, "row stride smaller than the row");
+  if (m * ((k + 1023) / 1024) >= 2147483647) return api_fail(MAMBO_EINVAL, "the call is too large: split its rows");
   int sms, smem;
   const int st = api_require_sm100(&sms, &smem);
   if (st != MAMBO_OK) return st;
@@ -375,6 +387,9 @@ int mambo_moe_experts(const void* x, int x_dtype, int64_t ldx, int64_t tokens, c
   if (tokens < 1 || tokens * top > kMaxRows) return api_fail(MAMBO_EINVAL, "tokens must be at least 1, tokens * top at most 2^28");
   if (ldx < h || ldo < h) return api_fail(MAMBO_EINVAL, "row stride smaller than the row");
   const ExpertsPlan E = plan_experts(tokens, top, experts, h, i, out_dtype);
+  st = check_size(E.a, E.rows, experts, h);
+  if (st == MAMBO_OK) st = check_size(E.b, E.rows, experts, i);
+  if (st != MAMBO_OK) return st;
   st = check_workspace(workspace, workspace_bytes, E.total);
   if (st != MAMBO_OK) return st;
   int sms, smem;

@@ -7,21 +7,33 @@
 // activations' power-of-two scales itself (block-scaled MMA, one scale per 32
 // K); a K block's partial product then has one factor left, the f32 scale of
 // the 128 x 128 weight block: the epilogue warps add D * sw to their FP32
-// registers, one packed FMA per two values, while the next block's MMAs run
-// into another D buffer.
+// registers, one packed FMA per two values, while the next blocks' MMAs run
+// into other D buffers.
+//
+// Two forms. Tiles of 128 rows x 16, 32 or 64 tokens on single CTAs stream the
+// weights: 28672 x 8192 at 8 tokens 38-42 us, 0.85-0.94 of the measured HBM
+// bandwidth. Tiles of 256 rows x 192 tokens on CTA pairs carry prompts: 8192 x
+// 28672 at 4096 tokens runs at 2.1 PFLOP/s in its kernel under ncu and 1.9 with
+// the quantizer in a short burst, where the power limit holds the SMs at
+// 1.5-1.7 GHz. What paces them is the way of a D buffer through the epilogue
+// and back (a K block of 192 tokens: 384 clocks of MMAs, 750 in all), and the
+// power of the FP32 additions: without them the same launch took 880 us, with
+// them 1000.
 //
 // Work: the (row tile, token tile) tiles of all experts, numbered expert by
-// expert, token tiles inner. Whole waves of tiles go one per CTA; the rest
-// (between one and two waves) is cut at K blocks into equal ranges, one per
-// CTA (stream-K), so every CTA ends at the same time. A tile that several CTAs
-// share is summed in K order by whichever arrives last: nothing waits.
+// expert, one per CTA and wave. Where the last wave would leave many CTAs idle
+// for long, the last one to two waves are cut at K blocks into equal ranges
+// instead (stream-K); a tile that several CTAs share is summed in K order by
+// whichever arrives last: nothing waits, and the sums do not depend on who.
 //
 // Warps: 0 weights producer, 1 and 3 MMA, 2 activations producer, then the
-// epilogue warps, one per TMEM lane quadrant (and per half of the columns).
+// epilogue warps, one per TMEM lane quadrant (and per half of the columns),
+// and for one or two tokens four warps that quantize them.
 //
 // Compiled as a whole program of its own (no relocatable device code): the
 // compiler takes setmaxnreg into account only then, and the pair kernel's
-// epilogue keeps 128 sums a thread. So it has its own device status.
+// epilogue holds 96 sums and 96 loaded values a thread. So it has its own
+// device status.
 #define MAMBO_OWN_DEVICE_STATUS
 #include <type_traits>
 
@@ -36,8 +48,11 @@ namespace mambo {
 namespace {
 
 constexpr int kMaxStagesB = 12;
+// K blocks that the CTAs which the last wave leaves idle lose on average from which a K split pays for publishing and
+// adding up the parts. Measured: 4096 x 4096 at one token (25 blocks) 11.5 -> 11.2 us, 28672 x 8192 at 8 (31) 41.5 ->
+// 39.7; split all the same, 32 experts of 4096 x 2048 at 96 rows (5) 45.3 -> 49.4. CTA pairs, 8192 x 28672 at 200 tokens
+// (100 blocks) 99 -> 89; split all the same, 5003 x 3001 at 77 (18) 17.1 -> 25.4.
 constexpr int kWorth = 12, kWorthPair = 30;
-// Whether the CTAs that the last wave leaves idle lose kWorth K blocks on average.
 __host__ __device__ inline bool fb_split_pays(int64_t tiles, int64_t kblocks, int64_t ctas) {
   const int64_t rem = tiles % ctas;
   return rem && (ctas - rem) * kblocks >= kWorth * ctas;
@@ -80,7 +95,7 @@ template <>
 struct FbWalk<false> {
   int kb_n, tiles, ncl, at;
   int tile, kb1;  // the current segment
-  static constexpr int kb0 = 0;
+  static constexpr int kb0 = 0, cl = 0;
   __device__ __forceinline__ FbWalk(int tiles_, int kblocks, int cl, int ncl_)
       : kb_n(kblocks), tiles(tiles_), ncl(ncl_), at(cl), tile(0), kb1(kblocks) {}
   __device__ __forceinline__ bool next() {
@@ -88,6 +103,7 @@ struct FbWalk<false> {
     at += ncl;
     return tile < tiles;
   }
+  __device__ __forceinline__ int owner(int) const { return 0; }  // of no split tile
 };
 template <>
 struct FbWalk<true> {
@@ -213,21 +229,39 @@ template <int N>
 __device__ __forceinline__ void ld_cols(uint32_t taddr, uint32_t (&r)[N]) {
   static_assert(N == 16 || N == 32, "16 or 32 columns");
   if constexpr (N == 16) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,"
+        "%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr));
   } else {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr));
   }
 }
 template <int N>
 __device__ __forceinline__ void wait_ld(uint32_t (&r)[N]) {
   if constexpr (N == 16) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) : : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
   } else {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) : : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
   }
 }
 
@@ -419,166 +453,166 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
   // Each instruction opens its own branch, so that the compiler knows every role's count.
   if (warp < 4) {
     if constexpr (kPair) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-  if (warp == 0) {
-    // -------------------------------------------------------------- weights producer
-    if (lane == 0) {
-      // Weights may be read ahead of the previous kernel's end where that is the quantizer, which waited for all
-      // before it; a kernel that is the first of its call may follow the one that packed them.
-      if (kQuant) pdl_wait();
-      const uint64_t policy = l2_policy_evict_first();
-      int it = 0, s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      while (ok && walk.next()) {
-        const FbTile t = cur.at(walk.tile);
-        const int rt = kPair ? 2 * t.rt + rank : t.rt;
-        const bool have = !kPair || rt < p.row_tiles;  // the second row tile of the last pair may not exist
-        const uint8_t* rec = p.packed + (((int64_t)t.e * p.row_tiles + rt) * KB) * kFbRecord;
-        for (int kb = walk.kb0; kb < walk.kb1; ++kb, ++it) {
-          if (it >= S && !fb_wait(kEmpty + 8 * s, ph ^ 1, kSiteFbEmpty)) {
-            ok = false;
-            break;
-          }
-          const uint32_t dst = smem_u32(tiles0 + (size_t)s * C::kStage);
-          if (have) {
-            mbar_arrive_expect_tx(kFull + 8 * s, kFbRecord);
-          } else {
-            mbar_arrive(kFull + 8 * s);  // whatever the stage holds: these rows are not stored
-          }
-          if (!have) {
-          } else if (p.evict_weights) {
-            bulk_load_hint(dst, rec + (int64_t)kb * kFbRecord, kFbRecord, kFull + 8 * s, policy);
-          } else {
-            bulk_load(dst, rec + (int64_t)kb * kFbRecord, kFbRecord, kFull + 8 * s);
-          }
-          if (++s == S) {
-            s = 0;
-            ph ^= 1;
-          }
-        }
-      }
-      if (!ok) settle_copies();
-    }
-    __syncwarp();
-  } else if (warp == 2) {
-    // -------------------------------------------------------------- activations producer
-    if (!kQuant && lane == 0) {
-      pdl_wait();
-      int it = 0, s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      while (ok && walk.next()) {
-        const FbTile t = cur.at(walk.tile);
-        const uint32_t bytes = (uint32_t)fb_part_rows(t.n, kPair) * 128u + fb_atoms_per_tile(NT) * kFbAtom;
-        const uint8_t* x = p.act.x8 + t.slot * KB * fb_record_bytes(NT) + (kPair ? rank * fb_part_bytes(NT) : 0u);
-        for (int kb = walk.kb0; kb < walk.kb1; ++kb, ++it) {
-          if (it >= S && !fb_wait(kEmpty + 8 * s, ph ^ 1, kSiteFbEmpty)) {
-            ok = false;
-            break;
-          }
-          const uint32_t full = kFull + 8 * s;
-          mbar_arrive_expect_tx(full, bytes);
-          bulk_load(smem_u32(tiles0 + (size_t)s * C::kStage) + kFbRecord, x + (int64_t)kb * fb_record_bytes(NT), bytes,
-                    full);
-          if (++s == S) {
-            s = 0;
-            ph ^= 1;
-          }
-        }
-      }
-      if (!ok) settle_copies();
-    }
-    __syncwarp();
-  } else {
-    // -------------------------------------------------------------- MMA
-    // Two issuing warps, 1 and 3, each with D buffers of its own: of a pair's tile each issues one half, alone they
-    // take the K blocks in turn. A K block costs its issuer some 400 clocks (two waits, the scale copy, four MMAs,
-    // two commits), which alone would pace the kernel.
-    const int who = warp >> 1;
-    if (kPair && rank == 1 && who == 0) {
-      // Rank 1 of a pair: its operands have landed, told to rank 0, which issues the MMAs of both.
+    if (warp == 0) {
+      // -------------------------------------------------------------- weights producer
       if (lane == 0) {
-        int s = 0;
+        // Weights may be read ahead of the previous kernel's end where that is the quantizer, which waited for all
+        // before it; a kernel that is the first of its call may follow the one that packed them.
+        if (kQuant) pdl_wait();
+        const uint64_t policy = l2_policy_evict_first();
+        int it = 0, s = 0;
         uint32_t ph = 0;
         bool ok = true;
         while (ok && walk.next()) {
-          for (int kb = walk.kb0; kb < walk.kb1; ++kb) {
-            ok = fb_wait(kFull + 8 * s, ph, kSiteFbFull);
-            if (!ok) break;
-            arrive_remote(lead(kFull + 8 * s));
+          const FbTile t = cur.at(walk.tile);
+          const int rt = kPair ? 2 * t.rt + rank : t.rt;
+          const bool have = !kPair || rt < p.row_tiles;  // the second row tile of the last pair may not exist
+          const uint8_t* rec = p.packed + (((int64_t)t.e * p.row_tiles + rt) * KB) * kFbRecord;
+          for (int kb = walk.kb0; kb < walk.kb1; ++kb, ++it) {
+            if (it >= S && !fb_wait(kEmpty + 8 * s, ph ^ 1, kSiteFbEmpty)) {
+              ok = false;
+              break;
+            }
+            const uint32_t dst = smem_u32(tiles0 + (size_t)s * C::kStage);
+            if (have) {
+              mbar_arrive_expect_tx(kFull + 8 * s, kFbRecord);
+            } else {
+              mbar_arrive(kFull + 8 * s);  // whatever the stage holds: these rows are not stored
+            }
+            if (!have) {
+            } else if (p.evict_weights) {
+              bulk_load_hint(dst, rec + (int64_t)kb * kFbRecord, kFbRecord, kFull + 8 * s, policy);
+            } else {
+              bulk_load(dst, rec + (int64_t)kb * kFbRecord, kFbRecord, kFull + 8 * s);
+            }
             if (++s == S) {
               s = 0;
               ph ^= 1;
             }
           }
         }
+        if (!ok) settle_copies();
       }
       __syncwarp();
-    }
-    // One thread issues: the chain from a free D buffer to its MMAs has no votes and no elections, and what the
-    // instructions take is ready before the waits.
-    if ((!kPair || rank == 0) && tm::elect_one()) {
-      // The loop is a chain of dependent instructions of one thread: everything that it can carry along is carried.
-      constexpr int kMine = kPair ? C::kD : C::kD / 2;  // D buffers of this issuer: a half's, or every other one
-      constexpr uint32_t kStep = kPair ? 1 : 2;
-      const uint32_t buf0 = kPair ? who * C::kD : who;
-      const uint32_t stage0 = smem_u32(tiles0) >> 4;
-      int s = 0, buf = 0;
-      uint32_t ph = 0, eph = 1, stage = stage0;  // eph: a fresh barrier's previous phase counts as over
-      bool ok = true, turn = kPair || who == 0;
-      while (ok && walk.next()) {
-        const int n_tile = cur.at(walk.tile).n;
-        const int nn = (n_tile + 15) / 16 * 16, n0 = kPair ? fb_split(n_tile) : nn;
-        const int n = who == 0 || !kPair ? n0 : nn - n0;
-        const uint32_t idesc = tc::idesc_mx_e4m3(kPair ? 256 : 128, n, 0, 0);
-        // This MMA's tokens, and the scale codes after all rows that the CTA holds.
-        const uint32_t b_at = (kFbRecord + (kPair && who ? n0 / 2 * 128u : 0u)) >> 4;
-        const uint32_t sf_at = (kFbRecord + (uint32_t)fb_part_rows(n_tile, kPair) * 128u + (kPair ? who * kFbAtom : 0u)) >> 4;
-        for (int left = walk.kb1 - walk.kb0; left > 0; --left) {
-          const uint32_t full = kFull + 8 * s;
-          if (kPair ? n > 0 : turn) {
-            const uint32_t b = buf0 + kStep * buf, bar = 8u * b;
-            uint32_t d = tmem + b * C::kCols, sfb = tmem + C::kSfb + 4u * b;
-            uint32_t a_lo = stage, b_lo = stage + b_at, s_lo = stage + sf_at;
-            asm volatile("" : "+r"(a_lo), "+r"(b_lo), "+r"(s_lo), "+r"(d), "+r"(sfb));  // before the waits
-            ok = fb_wait(full, ph, kSiteFbFull) && fb_wait(kEfree + bar, eph, kSiteFbEmpty);
-            if (!ok) break;
-            tc::fence_after_sync();
-            issue_block<kPair>(d, a_lo, b_lo, s_lo, idesc, tmem + C::kSfa, sfb, kMdone + bar, kEmpty + 8 * s);
-            if (++buf == kMine) {
-              buf = 0;
-              eph ^= 1;
+    } else if (warp == 2) {
+      // -------------------------------------------------------------- activations producer
+      if (!kQuant && lane == 0) {
+        pdl_wait();
+        int it = 0, s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        while (ok && walk.next()) {
+          const FbTile t = cur.at(walk.tile);
+          const uint32_t bytes = (uint32_t)fb_part_rows(t.n, kPair) * 128u + fb_atoms_per_tile(NT) * kFbAtom;
+          const uint8_t* x = p.act.x8 + t.slot * KB * fb_record_bytes(NT) + (kPair ? rank * fb_part_bytes(NT) : 0u);
+          for (int kb = walk.kb0; kb < walk.kb1; ++kb, ++it) {
+            if (it >= S && !fb_wait(kEmpty + 8 * s, ph ^ 1, kSiteFbEmpty)) {
+              ok = false;
+              break;
             }
-          } else if (kPair) {
-            // A tile of at most 16 tokens has no second MMA: the stage is released as if it had been read.
-            ok = fb_wait(full, ph, kSiteFbFull);
-            if (!ok) break;
-            arrive_remote(mapa_shared(kEmpty + 8 * s, 0));
-            arrive_remote(mapa_shared(kEmpty + 8 * s, 1));
+            const uint32_t full = kFull + 8 * s;
+            mbar_arrive_expect_tx(full, bytes);
+            bulk_load(smem_u32(tiles0 + (size_t)s * C::kStage) + kFbRecord, x + (int64_t)kb * fb_record_bytes(NT), bytes,
+                      full);
+            if (++s == S) {
+              s = 0;
+              ph ^= 1;
+            }
           }
-          if (!kPair) turn = !turn;
-          stage += C::kStage >> 4;
-          if (++s == S) {
-            s = 0;
-            ph ^= 1;
-            stage = stage0;
+        }
+        if (!ok) settle_copies();
+      }
+      __syncwarp();
+    } else {
+      // -------------------------------------------------------------- MMA
+      // Two issuing warps, 1 and 3, each with D buffers of its own: of a pair's tile each issues one half, alone they
+      // take the K blocks in turn. A K block costs its issuer some 400 clocks (two waits, the scale copy, four MMAs,
+      // two commits), which alone would pace the kernel.
+      const int who = warp >> 1;
+      if (kPair && rank == 1 && who == 0) {
+        // Rank 1 of a pair: its operands have landed, told to rank 0, which issues the MMAs of both.
+        if (lane == 0) {
+          int s = 0;
+          uint32_t ph = 0;
+          bool ok = true;
+          while (ok && walk.next()) {
+            for (int kb = walk.kb0; kb < walk.kb1; ++kb) {
+              ok = fb_wait(kFull + 8 * s, ph, kSiteFbFull);
+              if (!ok) break;
+              arrive_remote(lead(kFull + 8 * s));
+              if (++s == S) {
+                s = 0;
+                ph ^= 1;
+              }
+            }
+          }
+        }
+        __syncwarp();
+      }
+      // One thread issues: the chain from a free D buffer to its MMAs has no votes and no elections, and what the
+      // instructions take is ready before the waits.
+      if ((!kPair || rank == 0) && tm::elect_one()) {
+        // The loop is a chain of dependent instructions of one thread: everything that it can carry along is carried.
+        constexpr int kMine = kPair ? C::kD : C::kD / 2;  // D buffers of this issuer: a half's, or every other one
+        constexpr uint32_t kStep = kPair ? 1 : 2;
+        const uint32_t buf0 = kPair ? who * C::kD : who;
+        const uint32_t stage0 = smem_u32(tiles0) >> 4;
+        int s = 0, buf = 0;
+        uint32_t ph = 0, eph = 1, stage = stage0;  // eph: a fresh barrier's previous phase counts as over
+        bool ok = true, turn = kPair || who == 0;
+        while (ok && walk.next()) {
+          const int n_tile = cur.at(walk.tile).n;
+          const int nn = (n_tile + 15) / 16 * 16, n0 = kPair ? fb_split(n_tile) : nn;
+          const int n = who == 0 || !kPair ? n0 : nn - n0;
+          const uint32_t idesc = tc::idesc_mx_e4m3(kPair ? 256 : 128, n, 0, 0);
+          // This MMA's tokens, and the scale codes after all rows that the CTA holds.
+          const uint32_t b_at = (kFbRecord + (kPair && who ? n0 / 2 * 128u : 0u)) >> 4;
+          const uint32_t sf_at = (kFbRecord + (uint32_t)fb_part_rows(n_tile, kPair) * 128u + (kPair ? who * kFbAtom : 0u)) >> 4;
+          for (int left = walk.kb1 - walk.kb0; left > 0; --left) {
+            const uint32_t full = kFull + 8 * s;
+            if (kPair ? n > 0 : turn) {
+              const uint32_t b = buf0 + kStep * buf, bar = 8u * b;
+              uint32_t d = tmem + b * C::kCols, sfb = tmem + C::kSfb + 4u * b;
+              uint32_t a_lo = stage, b_lo = stage + b_at, s_lo = stage + sf_at;
+              asm volatile("" : "+r"(a_lo), "+r"(b_lo), "+r"(s_lo), "+r"(d), "+r"(sfb));  // before the waits
+              ok = fb_wait(full, ph, kSiteFbFull) && fb_wait(kEfree + bar, eph, kSiteFbEmpty);
+              if (!ok) break;
+              tc::fence_after_sync();
+              issue_block<kPair>(d, a_lo, b_lo, s_lo, idesc, tmem + C::kSfa, sfb, kMdone + bar, kEmpty + 8 * s);
+              if (++buf == kMine) {
+                buf = 0;
+                eph ^= 1;
+              }
+            } else if (kPair) {
+              // A tile of at most 16 tokens has no second MMA: the stage is released as if it had been read.
+              ok = fb_wait(full, ph, kSiteFbFull);
+              if (!ok) break;
+              arrive_remote(mapa_shared(kEmpty + 8 * s, 0));
+              arrive_remote(mapa_shared(kEmpty + 8 * s, 1));
+            }
+            if (!kPair) turn = !turn;
+            stage += C::kStage >> 4;
+            if (++s == S) {
+              s = 0;
+              ph ^= 1;
+              stage = stage0;
+            }
           }
         }
       }
-    }
-    __syncwarp();
-    if (who == 0) {
-      // Free the TMEM once every epilogue warp has read its last results.
-      fb_wait(kEdone, 0, kSiteFbFull);
       __syncwarp();
-      tc::fence_after_sync();
-      if constexpr (kPair) {
-        tc::dealloc_pair(tmem, C::kTmem);
-      } else {
-        tc::dealloc(tmem, C::kTmem);
+      if (who == 0) {
+        // Free the TMEM once every epilogue warp has read its last results.
+        fb_wait(kEdone, 0, kSiteFbFull);
+        __syncwarp();
+        tc::fence_after_sync();
+        if constexpr (kPair) {
+          tc::dealloc_pair(tmem, C::kTmem);
+        } else {
+          tc::dealloc(tmem, C::kTmem);
+        }
       }
     }
-  }
   } else if (kQuant && warp >= 8) {
     // -------------------------------------------------------------- quantizing warps
     // For tiles of one or two tokens: four warps take the K blocks in turn and write each block's E4M3 bytes and scale
@@ -734,7 +768,7 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
                 fma2(pack2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), w2, acc2[c * kCh / 2 + i]);
       }
       if (!ok) break;
-      if constexpr (kSplit) if (walk.kb0 != 0 || walk.kb1 != KB) {
+      if (kSplit && (walk.kb0 != 0 || walk.kb1 != KB)) {
         // A tile shared between CTAs: publish this warp's part, and sum all
         // parts in K order if it is the last to arrive.
         const int u_tile = walk.tile * KB;
@@ -816,7 +850,8 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
         // product's K). Of 16 columns at a time the even warp forms h for the first eight, the odd one for the
         // others: each sends the other eight over shared memory. Then a lane is a feature and a group's maximum is
         // one warp reduction. Bound by instructions (some 25 a column), with the MMAs waiting: hence the packed
-        // code arithmetic below; a first version of 60 a column took 1073 us in all where this one takes XX.
+        // code arithmetic below; a first version of 60 a column took 1073 us in all where this one takes 805
+        // (gate/up product of 4096 tokens, 64 experts of 2048 x 4096, eight a token).
         const FbActivations& hid = p.hidden;
         const bool odd = q & 1;
         const int n0 = fb_split(t.n), per = (h ? (t.n + 15) / 16 * 16 - n0 : n0) / 2;
@@ -849,7 +884,7 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float g = odd ? other[i] : own[i], u = odd ? own[i] : other[i];
-            // The fast exponential and quotient: within some 2^-21 of the value, which E4M3 rounds by up to 2^-4.
+            // The fast exponential and quotient: within some 2^-20 of the value, which E4M3 rounds by up to 2^-4.
             own[i] = __fdividef(g, 1.0f + __expf(-g)) * u;
             const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(own[i]) & 0x7FFFFFFFu);
             if ((lane & 7) == i) most = m;

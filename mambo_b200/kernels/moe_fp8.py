@@ -177,6 +177,6 @@ def fp8_moe_experts(x, route: MoeRoute, gate_up: Fp8BlockFields, down: Fp8BlockF
             _lib.check(_lib.load().mambo_moe_experts(
                 x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), tokens, route["ids"].data_ptr(),
                 route["weights"].data_ptr(), route["positions"].data_ptr(), route["offsets"].data_ptr(),
-                route["rows"].data_ptr(), top, gate_up["weight"], down["weight"], out.data_ptr(), code, _row_stride(out), ws.data_ptr(), ws.numel(),
-                st), "fp8_moe_experts")
+                route["rows"].data_ptr(), top, gate_up["weight"], down["weight"], out.data_ptr(), code,
+                _row_stride(out), ws.data_ptr(), ws.numel(), st), "fp8_moe_experts")
     return out

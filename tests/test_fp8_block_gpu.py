@@ -344,3 +344,60 @@ def test_refusals(cuda_device):
             pytest.fail(f"case {i} was accepted")
     with pytest.raises(TypeError):
         fp8_block_linear(x, c)
+
+
+@pytest.mark.parametrize("m,n,k", [(192, 256, 128), (193, 300, 200), (385, 4100, 256), (2000, 3000, 640),
+                                   (4096, 1030, 384), (200, 512, 8192), (100, 130, 6000), (1, 20000, 300), (2, 9000, 777)])
+def test_linear_waves_and_splits(cuda_device, m, n, k):
+    """Several waves of pair tiles, pair tiles split along K, row groups past a block of 8, one and two tokens."""
+    codes, scales = make_weight(n, k, m + 1)
+    w = prepared(cuda_device, codes, scales)
+    x = make_x(m, k, n).bfloat16()
+    ref = quantize64(x.double().numpy(), 128)[0] @ weight64(codes, scales).T
+    out = fp8_block_linear(x.to(cuda_device), w, out_dtype=torch.float32)
+    check(out, ref)
+    assert torch.equal(out, fp8_block_linear(x.to(cuda_device), w, out_dtype=torch.float32))
+    assert torch.equal(out.bfloat16(), fp8_block_linear(x.to(cuda_device), w))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m", [1, 2])
+def test_one_and_two_tokens_equal_the_quantizer(cuda_device, m, dtype):
+    """The product's own quantization of one or two tokens gives what the quantizer gives, whatever the rows' alignment."""
+    n, k = 300, 1003
+    codes, scales = make_weight(n, k, 2)
+    w = prepared(cuda_device, codes, scales)
+    wide = torch.zeros(m, k + 9, dtype=dtype, device=cuda_device)
+    wide[:, 5:5 + k] = make_x(m, k, 1).to(dtype).to(cuda_device)
+    x = wide[:, 5:5 + k]
+    for group in (32, 128):
+        v, s = launch_quantize_fp8_block(x, group=group)
+        assert torch.equal(fp8_block_linear(x, w, act_group=group, out_dtype=torch.float32), launch_fp8_block_matmul(v, s, w))
+    off = torch.tensor([0, 0, m], dtype=torch.int32, device=cuda_device)
+    w2 = prepared(cuda_device, np.stack([codes, codes]), np.stack([scales, scales]))
+    assert torch.equal(fp8_block_grouped_linear(x, off, w2), fp8_block_linear(x, w))
+
+
+def test_more_than_2_31_elements(cuda_device):
+    """Output and weight offsets past 32 bits."""
+    dev = cuda_device
+    codes, scales = make_weight(8192, 128, 3)
+    w = prepared(dev, codes, scales)
+    m = 300_000
+    x = torch.randn(m, 128, device=dev, dtype=torch.bfloat16)
+    out = fp8_block_linear(x, w)
+    assert out.numel() > 2 ** 31
+    for a in (0, 131_072, m - 40):
+        # Which tokens share a tile does not change a sum of one K block.
+        assert torch.equal(out[a:a + 40], fp8_block_linear(x[a:a + 40].contiguous(), w))
+    del out, x
+    experts, n, k = 40, 8192, 8192
+    big = torch.randint(0, 120, (experts, n, k), dtype=torch.uint8, device=dev)
+    s = torch.full((experts, 64, 64), 2.0 ** -8, device=dev)
+    wg = prepare_fp8_block_fields(big, s)
+    x = torch.randn(experts * 3, k, device=dev, dtype=torch.bfloat16)
+    off = torch.arange(experts + 1, dtype=torch.int32, device=dev) * 3
+    out = fp8_block_grouped_linear(x, off, wg, out_dtype=torch.float32)
+    for e in (0, 39):
+        one = fp8_block_linear(x[3 * e:3 * e + 3], prepare_fp8_block_fields(big[e], s[e]), out_dtype=torch.float32)
+        assert frob(out[3 * e:3 * e + 3].cpu(), one.cpu()) < F32_TOL

@@ -238,3 +238,76 @@ def test_refusals(cuda_device):
             pytest.fail(f"case {n} was accepted")
     with pytest.raises(TypeError):
         fp8_moe_experts(x, r, gu, wd)
+
+
+@pytest.mark.parametrize("t,e,k,h,i", [(1, 8, 2, 4096, 64), (3, 8, 2, 4096, 64), (5, 4, 1, 256, 4096), (40, 2, 1, 2304, 130)])
+def test_experts_split_along_k(cuda_device, t, e, k, h, i):
+    """Few tiles of many K blocks: several CTAs share a tile, also where its epilogue forms the hidden activations."""
+    gu, gus, down, downs = make_experts(e, h, i, t + i)
+    dev = cuda_device
+    wg = prepare_fp8_block_fields(torch.from_numpy(gu).to(dev), torch.from_numpy(gus).to(dev), gate_up=True)
+    wd = prepare_fp8_block_fields(torch.from_numpy(down).to(dev), torch.from_numpy(downs).to(dev))
+    logits = np.random.default_rng(t).standard_normal((t, e)).astype(np.float32)
+    x = torch.zeros(t, h + 3, device=dev)
+    x[:, 1:1 + h] = make_x(t, h, 3).to(dev) * 0.5
+    x = x[:, 1:1 + h]
+    route = launch_moe_route(torch.from_numpy(logits).to(dev), k)
+    ref = experts_ref(x.cpu().numpy(), route_ref(logits, k), gu, gus, down, downs)
+    out = fp8_moe_experts(x, route, wg, wd, out_dtype=torch.float32)
+    assert frob(out.cpu(), ref) < EXPERTS_F32_TOL
+    for _ in range(3):
+        assert torch.equal(out, fp8_moe_experts(x, route, wg, wd, out_dtype=torch.float32))
+
+
+def test_experts_in_a_graph(cuda_device):
+    """Route and experts captured once and replayed on new inputs: nothing goes through the host."""
+    dev = cuda_device
+    t, e, k, h, i = 6, 16, 2, 256, 128
+    gu, gus, down, downs = make_experts(e, h, i, 4)
+    wg = prepare_fp8_block_fields(torch.from_numpy(gu).to(dev), torch.from_numpy(gus).to(dev), gate_up=True)
+    wd = prepare_fp8_block_fields(torch.from_numpy(down).to(dev), torch.from_numpy(downs).to(dev))
+    x, logits = torch.zeros(t, h, device=dev, dtype=torch.bfloat16), torch.zeros(t, e, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fp8_moe_experts(x, launch_moe_route(logits, k), wg, wd)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = fp8_moe_experts(x, launch_moe_route(logits, k), wg, wd)
+    for seed in range(3):
+        gen = torch.Generator().manual_seed(seed)
+        x.copy_(torch.randn(t, h, generator=gen))
+        logits.copy_(torch.randn(t, e, generator=gen))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, fp8_moe_experts(x, launch_moe_route(logits, k), wg, wd))
+
+
+def test_example_layer(cuda_device):
+    """The example's layer gives the sum of its shared and routed experts, computed in float64."""
+    import sys
+
+    from conftest import ROOT
+
+    sys.path.insert(0, str(ROOT / "examples"))
+    from fp8_expert_layer import ExpertLayer, random_fp8_weight
+
+    hidden, features, experts, top = 256, 128, 8, 2
+    layer = ExpertLayer(hidden, features, experts, top, seed=3)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    router = torch.randn((experts, hidden), generator=gen, device="cuda") / hidden ** 0.5
+    plain = []
+    for shape in ((2 * features, hidden), (hidden, features), (experts, 2 * features, hidden), (experts, hidden, features)):
+        v, s = random_fp8_weight(shape, gen)
+        plain.append((v.view(torch.uint8).cpu().numpy(), s.cpu().numpy()))
+    x = torch.randn(20, hidden, device=cuda_device).bfloat16()
+    xq = quantize64(x.double().cpu().numpy(), 128)[0]
+    a = xq @ weight64(*plain[0]).T
+    g, u = a[:, :features], a[:, features:]
+    shared = quantize64(g / (1 + np.exp(-g)) * u, 128)[0] @ weight64(*plain[1]).T
+    logits = (x.float() @ router.t()).cpu().numpy()
+    routed = experts_ref(x.float().cpu().numpy(), route_ref(logits, top), *plain[2], *plain[3])
+    # The shared hidden activations pass through bf16 here: two roundings of 2^-8 and the codes they move (2^-4 of
+    # about 2^-8 / 2^-4 of them), under 2e-2 in the norm.
+    assert frob(layer(x).float().cpu(), shared + routed) < 2e-2
