@@ -699,7 +699,7 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
     };
     pdl_wait();  // the output and the workspace may belong to the previous kernel
     pdl_launch_dependents();
-    const uint32_t efree0 = kPair ? lead(kEfree + 8 * h * C::kD) : 0u;
+    const uint32_t efree0 = kPair ? lead(kEfree + 8 * h * C::kD) : 0u;  // this half's, in rank 0
     int db = 0;
     uint32_t dph = 0;
     bool ok = true;
@@ -748,13 +748,11 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
 #pragma unroll
         for (int c = 1; c < C::kCols / kCh; ++c) tie(v[c]);
         tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          if (kPair && rank != 0) {
-            arrive_remote(efree0 + 8 * db);
-          } else {
-            mbar_arrive(kEfree + 8 * (h * C::kD + db));
-          }
+        // The loads' wait was the whole warp's, so one lane may speak for it; in both CTAs of a pair to rank 0.
+        if (kPair) {
+          if (lane == 0) arrive_remote(efree0 + 8 * db);
+        } else {
+          if (lane == 0) mbar_arrive(kEfree + 8 * db);
         }
         if (++db == C::kD) {
           db = 0;
