@@ -51,11 +51,12 @@ constexpr int kMaxStagesB = 12;
 // K blocks that the CTAs which the last wave leaves idle lose on average from which a K split pays for publishing and
 // adding up the parts. Measured: 4096 x 4096 at one token (25 blocks) 11.5 -> 11.2 us, 28672 x 8192 at 8 (31) 41.5 ->
 // 39.7; split all the same, 32 experts of 4096 x 2048 at 96 rows (5) 45.3 -> 49.4. CTA pairs, 8192 x 28672 at 200 tokens
-// (100 blocks) 99 -> 89; split all the same, 5003 x 3001 at 77 (18) 17.1 -> 25.4.
-constexpr int kWorth = 12, kWorthPair = 30;
+// (100 blocks) 99 -> 89; split all the same, 5003 x 3001 at 77 (18) 17.1 -> 25.4. After several waves the CTAs have drifted
+// apart and the last ones run faster alone: 8 experts of 28672 x 4096 at 32 tokens (12 waves) 227 us unsplit, 233 split.
+constexpr int kWorth = 12, kWorthPair = 30, kWorthWaves = 4;
 __host__ __device__ inline bool fb_split_pays(int64_t tiles, int64_t kblocks, int64_t ctas) {
   const int64_t rem = tiles % ctas;
-  return rem && (ctas - rem) * kblocks >= kWorth * ctas;
+  return rem && tiles < kWorthWaves * ctas && (ctas - rem) * kblocks >= kWorth * ctas;
 }
 
 // kPair: CTA pairs. A tile is 256 weight rows (a row tile per CTA) x NT tokens; each CTA loads half of the
@@ -118,7 +119,7 @@ struct FbWalk<true> {
     cl = cl_;
     const int rem = tiles % ncl;
     sk = 0;
-    if (fb_split_pays(tiles, kb_n, ncl)) sk = tiles < ncl ? rem : rem + ncl;
+    if (fb_split_pays(tiles, kb_n, ncl)) sk = rem;
     units = sk * kb_n;
     // Each part at least four K blocks.
     nsk = max(1, min(ncl, units / 4));

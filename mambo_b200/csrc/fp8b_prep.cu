@@ -117,7 +117,7 @@ __device__ __forceinline__ void quant_load(const FbQuantParams& p, int64_t row, 
 }
 
 template <int kIn, bool kVec>
-__global__ void __launch_bounds__(256) fb_quant_kernel(const __grid_constant__ FbQuantParams p) {
+__global__ void __launch_bounds__(256, 5) fb_quant_kernel(const __grid_constant__ FbQuantParams p) {
   const int lane = threadIdx.x & 31;
   const uint32_t spans = (uint32_t)((p.k + kSpan - 1) / kSpan);
   const uint32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);  // the host keeps rows * spans below 2^31
