@@ -731,40 +731,54 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
       // A K block: all of the warp's columns to registers at once, the D buffer released, then the additions. The
       // buffer's way back to the MMAs is what paces the kernel, and additions between its loads lengthen it: with
       // chunks of 32 columns loaded ahead of their additions a K block of 224 tokens took 912 clocks, 505 without
-      // the additions. Columns past the tile's are added like the others (whatever they hold) and never stored.
-      float sv = 0.f;
+      // the additions. Columns past the tile's in a chunk are added like the others (whatever they hold), never stored.
+      constexpr int kCh = C::kCols < 32 ? C::kCols : 32;
+      // One loop per number of column chunks, so that a ragged tile loads and adds no more than it has: branches inside
+      // one loop made every tile slower (14336 x 4096 at 2048 tokens 150 -> 183 us).
+      auto k_loop = [&](auto chunks) {
+        constexpr int kChunks = decltype(chunks)::value;
+        float sv = 0.f;
 #pragma unroll 1
-      for (int kb = walk.kb0; kb < walk.kb1; ++kb) {
-        if (kb == walk.kb0 || (kb & 31) == 0) sv = (kb & ~31) + lane < KB ? __ldg(sw + (kb & ~31) + lane) : 0.f;
-        const float w = __shfl_sync(0xFFFFFFFFu, sv, kb & 31);
-        const uint64_t w2 = pack2(w, w);
-        ok = fb_warp_wait(kMdone + 8 * (h * C::kD + db), dph, kSiteFbFull);
-        if (!ok) break;
-        tc::fence_after_sync();
-        constexpr int kCh = C::kCols < 32 ? C::kCols : 32;
-        uint32_t v[C::kCols / kCh][kCh];
+        for (int kb = walk.kb0; kb < walk.kb1; ++kb) {
+          if (kb == walk.kb0 || (kb & 31) == 0) sv = (kb & ~31) + lane < KB ? __ldg(sw + (kb & ~31) + lane) : 0.f;
+          const float w = __shfl_sync(0xFFFFFFFFu, sv, kb & 31);
+          const uint64_t w2 = pack2(w, w);
+          ok = fb_warp_wait(kMdone + 8 * (h * C::kD + db), dph, kSiteFbFull);
+          if (!ok) return;
+          tc::fence_after_sync();
+          uint32_t v[kChunks][kCh];
 #pragma unroll
-        for (int c = 0; c < C::kCols / kCh; ++c) ld_cols(tq0 + (uint32_t)db * C::kCols + c * kCh, v[c]);
-        wait_ld(v[0]);
+          for (int c = 0; c < kChunks; ++c) ld_cols(tq0 + (uint32_t)db * C::kCols + c * kCh, v[c]);
+          wait_ld(v[0]);
 #pragma unroll
-        for (int c = 1; c < C::kCols / kCh; ++c) tie(v[c]);
-        tc::fence_before_sync();
-        // The loads' wait was the whole warp's, so one lane may speak for it; in both CTAs of a pair to rank 0.
-        if (kPair) {
-          if (lane == 0) arrive_remote(efree0 + 8 * db);
+          for (int c = 1; c < kChunks; ++c) tie(v[c]);
+          tc::fence_before_sync();
+          // The loads' wait was the whole warp's, so one lane may speak for it; in both CTAs of a pair to rank 0.
+          if (kPair) {
+            if (lane == 0) arrive_remote(efree0 + 8 * db);
+          } else {
+            if (lane == 0) mbar_arrive(kEfree + 8 * db);
+          }
+          if (++db == C::kD) {
+            db = 0;
+            dph ^= 1;
+          }
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < kCh / 2; ++i)
+              acc2[c * kCh / 2 + i] =
+                  fma2(pack2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), w2, acc2[c * kCh / 2 + i]);
+        }
+      };
+      if constexpr (C::kCols == 3 * kCh) {
+        if (cols > 2 * kCh) {
+          k_loop(std::integral_constant<int, 3>{});
         } else {
-          if (lane == 0) mbar_arrive(kEfree + 8 * db);
+          k_loop(std::integral_constant<int, 2>{});
         }
-        if (++db == C::kD) {
-          db = 0;
-          dph ^= 1;
-        }
-#pragma unroll
-        for (int c = 0; c < C::kCols / kCh; ++c)
-#pragma unroll
-          for (int i = 0; i < kCh / 2; ++i)
-            acc2[c * kCh / 2 + i] =
-                fma2(pack2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), w2, acc2[c * kCh / 2 + i]);
+      } else {
+        k_loop(std::integral_constant<int, C::kCols / kCh>{});
       }
       if (!ok) break;
       if (kSplit && (walk.kb0 != 0 || walk.kb1 != KB)) {
