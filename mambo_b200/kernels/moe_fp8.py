@@ -32,6 +32,7 @@ class MoeRoute(TypedDict):
     offsets: torch.Tensor  # int32 [E+1]: first row of each expert in expert order
     positions: torch.Tensor  # int32 [T,top]: row of each choice in expert order, -1: none
     rows: torch.Tensor  # int32 [T*top]: the choice (token * top + j) of each row, -1 past the last
+    made: tuple  # the tensors above as launch_moe_route made them: calls that get these very ones skip their checks
 
 
 @functools.lru_cache(maxsize=1024)
@@ -93,12 +94,17 @@ def launch_moe_route(logits, top_k: int, *, scoring: str = "softmax", bias=None,
                 ws.numel(), st), "launch_moe_route")
     else:
         offsets.zero_()
-    return {"ids": ids, "weights": weights, "offsets": offsets, "positions": positions, "rows": rows}
+    return {"ids": ids, "weights": weights, "offsets": offsets, "positions": positions, "rows": rows,
+            "made": (ids, weights, positions, rows, offsets)}
 
 
 def _check_route(route: MoeRoute, tokens: int, device: torch.device) -> int:
     """top_k of a route for `tokens` tokens."""
     ids, weights, positions, rows = route["ids"], route["weights"], route["positions"], route["rows"]
+    made = route.get("made")
+    if made and made[0] is ids and made[1] is weights and made[2] is positions and made[3] is rows \
+            and made[4] is route["offsets"] and ids.shape[0] == tokens and ids.device == device:
+        return ids.shape[1]
     if ids.ndim != 2 or ids.shape[0] != tokens or weights.shape != ids.shape or positions.shape != ids.shape:
         raise ValueError("route must have ids, weights and positions [T,top_k] for the activation's T")
     if ids.dtype != torch.int32 or positions.dtype != torch.int32 or weights.dtype != torch.float32 \
