@@ -48,7 +48,8 @@ class ExpertLayer:
         self.down = prepare_fp8_block_fields(*random_fp8_weight((experts, hidden, features), gen))
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
-        gate, up = fp8_block_linear(x, self.shared_up).chunk(2, dim=1)
+        # float32 until it is quantized again: rounded to bf16 first, one E4M3 code in twenty would be another.
+        gate, up = fp8_block_linear(x, self.shared_up, out_dtype=torch.float32).chunk(2, dim=1)
         shared = fp8_block_linear(torch.nn.functional.silu(gate) * up, self.shared_down)
         route = launch_moe_route(x.float() @ self.router.t(), self.top)
         return shared + fp8_moe_experts(x, route, self.gate_up, self.down)
