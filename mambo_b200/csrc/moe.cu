@@ -8,8 +8,10 @@ namespace mambo {
 
 namespace {
 
-constexpr int kRouteThreads = 512;
-constexpr int kRouteWarps = kRouteThreads / 32;
+// Threads of a routing CTA: as many warps as its registers allow, a token each at a time (more than 256 experts need
+// more registers a thread).
+constexpr int kPlaceThreads = 1024;
+__host__ __device__ constexpr int route_threads(int nv) { return nv <= 8 ? 1024 : 512; }
 
 // Monotone map of a float to an unsigned key (0 is free: it marks masked experts).
 __device__ __forceinline__ uint32_t order_key(float f) {
@@ -140,8 +142,10 @@ __device__ __forceinline__ void scan_counts(int* v, int n, int lane) {
 
 // The chunk's (token, choice) pairs in order, each to its row: base[e] holds
 // the first free row of expert e for this chunk (bucket `experts`: no expert).
+template <int kRouteThreads>
 __device__ __forceinline__ void place_chunk(const FbRouteParams& p, int first, int count, const int* base, int* wcnt,
                                             int warp, int lane) {
+  constexpr int kRouteWarps = kRouteThreads / 32;
   const int n = count * p.top, buckets = p.experts + 1;
   const int per = (n + kRouteWarps * 32 - 1) / (kRouteWarps * 32) * 32;  // entries of a warp, whole groups of 32
   const int b0 = min(n, warp * per), b1 = min(n, b0 + per);
@@ -186,7 +190,8 @@ __device__ __forceinline__ void place_chunk(const FbRouteParams& p, int first, i
 // Selection of a chunk's tokens, a warp per token, and the chunk's counts per
 // expert; with one chunk also the placement. Latency-bound in decode.
 template <int NV>
-__global__ void __launch_bounds__(kRouteThreads, NV <= 8 ? 2 : 1) moe_route_kernel(const __grid_constant__ FbRouteParams p) {
+__global__ void __launch_bounds__(route_threads(NV), 1) moe_route_kernel(const __grid_constant__ FbRouteParams p) {
+  constexpr int kRouteThreads = route_threads(NV), kRouteWarps = kRouteThreads / 32;
   extern __shared__ int route_sm[];
   int* hist = route_sm;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, buckets = p.experts + 1;
@@ -213,12 +218,13 @@ __global__ void __launch_bounds__(kRouteThreads, NV <= 8 ? 2 : 1) moe_route_kern
   if (warp == 0) scan_counts(hist, buckets, lane);
   __syncthreads();
   for (int i = threadIdx.x; i < buckets; i += kRouteThreads) p.offsets[i] = hist[i];
-  place_chunk(p, first, count, hist, hist + buckets, warp, lane);
+  place_chunk<kRouteThreads>(p, first, count, hist, hist + buckets, warp, lane);
 }
 
 // Placement of one chunk: every CTA sums the chunks' counts itself (the counts
 // of a 16384-token call are 128 x 257 numbers in L2), so there is no third launch.
-__global__ void __launch_bounds__(kRouteThreads) moe_place_kernel(const __grid_constant__ FbRouteParams p) {
+__global__ void __launch_bounds__(kPlaceThreads, 1) moe_place_kernel(const __grid_constant__ FbRouteParams p) {
+  constexpr int kRouteThreads = kPlaceThreads, kRouteWarps = kRouteThreads / 32;
   extern __shared__ int route_sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, buckets = p.experts + 1;
   int* base = route_sm;            // totals, then first rows
@@ -253,31 +259,32 @@ __global__ void __launch_bounds__(kRouteThreads) moe_place_kernel(const __grid_c
     for (int i = threadIdx.x; i < buckets; i += kRouteThreads) p.offsets[i] = base[i];
   for (int e = threadIdx.x; e < buckets; e += kRouteThreads) before[e] += base[e];
   __syncthreads();
-  place_chunk(p, first, count, before, wcnt, warp, lane);
+  place_chunk<kRouteThreads>(p, first, count, before, wcnt, warp, lane);
 }
 
-// Tokens of a chunk, one CTA: up to 64 tokens are one chunk and one launch; beyond that about 256 chunks, so that
-// every SM ranks (a token's ranking is a chain of some 3000 clocks) and the placement still sums few counts.
+// Tokens of a chunk, one CTA: up to 32 tokens are one chunk and one launch; beyond that at most 128 chunks, so that
+// each has an SM (a token's ranking is a chain of some 2000 clocks) and the placement sums few counts: 16384 tokens
+// over 256 experts take 30 us, with 256 chunks of half the warps 35 (64 tokens in one chunk 13, in two 11).
 int fb_route_chunk(int64_t tokens) {
-  const int64_t per = (tokens + 255) / 256;
-  return tokens <= 64 ? 64 : (int)(per < 16 ? 16 : per);
+  const int64_t per = (tokens + 127) / 128;
+  return per < 32 ? 32 : (int)per;
 }
 
 cudaError_t launch_fb_route(const FbRouteParams& p, cudaStream_t stream) {
   const int chunks = (p.tokens + p.chunk - 1) / p.chunk, buckets = p.experts + 1;
-  const size_t smem = (size_t)buckets * (1 + kRouteWarps) * sizeof(int);
-  const int nv = (p.experts + 31) / 32;
+  const int nv = (p.experts + 31) / 32, threads = route_threads(nv);
+  const size_t smem = (size_t)buckets * (1 + threads / 32) * sizeof(int);
   const void* k = nv <= 2   ? (const void*)moe_route_kernel<2>
                   : nv <= 4 ? (const void*)moe_route_kernel<4>
                   : nv <= 8 ? (const void*)moe_route_kernel<8>
                   : nv <= 16 ? (const void*)moe_route_kernel<16>
                              : (const void*)moe_route_kernel<32>;
   cudaError_t e = ensure_smem_attribute(k, smem);
-  if (e == cudaSuccess) e = launch_pdl(k, dim3(chunks), dim3(kRouteThreads), smem, stream, p);
+  if (e == cudaSuccess) e = launch_pdl(k, dim3(chunks), dim3(threads), smem, stream, p);
   if (e != cudaSuccess || chunks == 1) return e;
-  const size_t place = (size_t)buckets * (2 + kRouteWarps) * sizeof(int);
+  const size_t place = (size_t)buckets * (2 + kPlaceThreads / 32) * sizeof(int);
   e = ensure_smem_attribute((const void*)moe_place_kernel, place);
-  return e != cudaSuccess ? e : launch_pdl((const void*)moe_place_kernel, dim3(chunks), dim3(kRouteThreads), place, stream, p);
+  return e != cudaSuccess ? e : launch_pdl((const void*)moe_place_kernel, dim3(chunks), dim3(kPlaceThreads), place, stream, p);
 }
 
 // --------------------------------------------------------------------------
