@@ -11,14 +11,13 @@
 // into other D buffers.
 //
 // Two forms. Tiles of 128 rows x 16, 32 or 64 tokens on single CTAs stream the
-// weights: 28672 x 8192 at 8 tokens 38-42 us, 0.85-0.94 of the measured HBM
-// bandwidth. Tiles of 256 rows x 192 tokens on CTA pairs carry prompts: 8192 x
-// 28672 at 4096 tokens runs at 2.1 PFLOP/s in its kernel under ncu and 1.9 with
-// the quantizer in a short burst, where the power limit holds the SMs at
-// 1.5-1.7 GHz. What paces them is the way of a D buffer through the epilogue
-// and back (a K block of 192 tokens: 384 clocks of MMAs, 750 in all), and the
-// power of the FP32 additions: without them the same launch took 880 us, with
-// them 1000.
+// weights: 28672 x 8192 at 8 tokens 40-42 us, 0.86-0.90 of the measured HBM
+// bandwidth (38 repeated on one input). Tiles of 256 rows x 192 tokens on CTA pairs carry prompts: 8192 x
+// 28672 at 4096 tokens takes 910-930 us with its quantizer in short bursts (2.1
+// PFLOP/s) and 1060-1180 in long runs (1.6-1.8), where the power limit holds the
+// SMs near 1.5 GHz. 14336 x 4096 at 2048 tokens: 120 us, the tensor pipe active
+// 60 % of the time. What paces them is the way of a D buffer through the
+// epilogue and back, and power.
 //
 // Work: the (row tile, token tile) tiles of all experts, numbered expert by
 // expert, one per CTA and wave. Where the last wave would leave many CTAs idle
@@ -49,7 +48,7 @@ namespace {
 
 constexpr int kMaxStagesB = 12;
 // K blocks that the CTAs which the last wave leaves idle lose on average from which a K split pays for publishing and
-// adding up the parts. Measured: 4096 x 4096 at one token (25 blocks) 11.5 -> 11.2 us, 28672 x 8192 at 8 (31) 41.5 ->
+// adding up the parts. Measured: 4096 x 4096 at one token (25 blocks, weights in L2) 11.5 -> 11.2 us, 28672 x 8192 at 8 (31) 41.5 ->
 // 39.7; split all the same, 32 experts of 4096 x 2048 at 96 rows (5) 45.3 -> 49.4. CTA pairs, 8192 x 28672 at 200 tokens
 // (100 blocks) 99 -> 89; split all the same, 5003 x 3001 at 77 (18) 17.1 -> 25.4. After several waves the CTAs have drifted
 // apart and the last ones run faster alone: 8 experts of 28672 x 4096 at 32 tokens (12 waves) 227 us unsplit, 233 split.
@@ -618,7 +617,7 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
     // -------------------------------------------------------------- quantizing warps
     // For tiles of one or two tokens: four warps take the K blocks in turn and write each block's E4M3 bytes and scale
     // codes straight into its stage, a half warp a token, 8 values a lane. Every tile's CTA quantizes the tokens anew:
-    // for one token that is less than a launch of the quantizer (4096 x 4096: 11.2 -> 10.6 us, 64 experts of 2048 x
+    // for one token that is less than a launch of the quantizer (repeated, weights in L2: 4096 x 4096 11.2 -> 10.6 us, 64 experts of 2048 x
     // 1408, six a token: 32.0 -> 27.9), for eight it held the weights up (28672 x 8192: 39 -> 54 us).
     const FbSource& src = p.src;
     const int who = warp - 8, col = (lane & 15) * 8, r = lane >> 4;

@@ -57,8 +57,8 @@ cudaError_t launch_fb_pack(const FbPackParams& p, cudaStream_t stream) {
 // row, kSteps loads in flight (a lane holds 8 values, a quad or 16 lanes a
 // scale group), and finds the row's places once for all of them: one place in
 // expert order (kFbGrouped), up to `top` when the row's token was routed, so
-// that x is read once. 4096 x 28672 bf16 values take 79 us, 4.4 TB/s read and
-// written (0.68 of the measured bandwidth); one step of 256 values a warp with
+// that x is read once. 4096 x 28672 bf16 values take 75 us, 4.7 TB/s read and
+// written (0.72 of the measured bandwidth); one step of 256 values a warp with
 // the place found by every thread took 180 us under ncu where this takes 99.
 // --------------------------------------------------------------------------
 namespace {
