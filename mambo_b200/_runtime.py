@@ -13,6 +13,8 @@ from . import _lib
 
 _checked_devices: dict[int, int] = {}
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_captured: set[tuple[int, int]] = set()  # workspaces that a CUDA graph may use
+_kept: list[torch.Tensor] = []  # ... and such as a larger one has replaced
 _ws_lock = threading.Lock()
 
 
@@ -59,25 +61,48 @@ def require_device(device: torch.device) -> None:
         raise RuntimeError(f"IQ3_S FP8 kernels have no build for sm{major}{minor} (this library targets sm_100a)")
 
 
+def _stream_is_capturing(device: torch.device, stream: int) -> bool:
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """Zero-filled scratch for split-K partials and counters, one per (device, stream).
 
     The kernels leave the counter region zeroed again, so the buffer is reused
     across calls on the same stream; calls on different streams get their own.
+
+    A CUDA graph keeps the address of the buffer that its calls were captured
+    with. So a buffer that was handed out during a capture is never freed, also
+    when a later call on the stream needs a larger one; each is at least twice
+    the one before, so what is kept adds up to less than the newest. A capture
+    itself cannot make the buffer grow (it could neither be zero-filled at once
+    nor outlive the graph): that raises, and the capture goes on undisturbed.
     """
     index = device.index if device.index is not None else torch.cuda.current_device()
     key = (index, stream)
+    # Only the current stream's capture is a cheap question: any other stream counts as capturing.
+    captured = index != torch.cuda.current_device() or stream != torch._C._cuda_getCurrentRawStream(index) \
+        or torch.cuda.is_current_stream_capturing()
     with _ws_lock:
         ws = _workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
+            dev = torch.device("cuda", index)
+            if captured and _stream_is_capturing(dev, stream):
+                raise RuntimeError(f"the stream's workspace has {0 if ws is None else ws.numel()} bytes and this call needs "
+                                   f"{nbytes}: run it once on the stream before capturing it")
             size = max(nbytes, 1 << 20)
             if ws is not None:
                 size = max(size, 2 * ws.numel())
-            dev = torch.device("cuda", index)
             # Drain pending work before swapping buffers: a kernel on `stream`
             # may still use the old one, and the zero-fill runs on torch's stream.
             torch.cuda.synchronize(dev)
+            if key in _captured:
+                _captured.remove(key)
+                _kept.append(ws)
             ws = torch.zeros(size, dtype=torch.uint8, device=dev)
             torch.cuda.synchronize(dev)
             _workspaces[key] = ws
+        if captured:
+            _captured.add(key)
         return ws
