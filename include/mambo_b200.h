@@ -500,7 +500,9 @@ MAMBO_API int mambo_moe_combine(const void* y, int y_dtype, int64_t ldy, int64_t
  * chosen experts -> h = silu(gate) * up -> MXFP8 (from FP32) -> down -> the
  * weighted sum of each token's rows. gate_up: a gate/up weight [experts, 2I,
  * H]; down [experts, H, I]; ids, weights, positions, offsets and rows (or
- * NULL: without it a decode call takes one more launch) from mambo_moe_route. Each expert row rounds once to out_dtype before the sum.
+ * NULL: without it a decode call takes one more launch) from mambo_moe_route
+ * or laid out as it lays them out; a token may name an expert more than once.
+ * Each expert row rounds once to out_dtype before the sum.
  * workspace: mambo_moe_experts_workspace_bytes(), zero-filled once.
  */
 MAMBO_API size_t mambo_moe_experts_workspace_bytes(int64_t tokens, int top, int64_t experts, int64_t h, int64_t i,

@@ -171,7 +171,7 @@ struct ExpertsPlan {
 ExpertsPlan plan_experts(int64_t tokens, int64_t top, int64_t experts, int64_t h, int64_t i, int out_dtype) {
   ExpertsPlan E;
   E.rows = tokens * top;
-  // A token picks an expert at most once.
+  // A token mostly picks an expert once; where a route repeats one, its rows take several tiles.
   E.a = plan(E.rows, experts, tokens, 2 * i, h, 1);
   E.b = plan(E.rows, experts, tokens, h, i, 0);  // the same tiles: nt depends on the rows only
   E.y = align256((size_t)E.rows * h * elem(out_dtype));
@@ -406,7 +406,8 @@ int mambo_moe_experts(const void* x, int x_dtype, int64_t ldx, int64_t tokens, c
   uint8_t* partials = at;
 
   cudaError_t e;
-  if (rows && tokens <= kFbQuantTokens) {  // an expert has at most one row of a token
+  // Tiles of 16 tokens, the form that quantizes them: of more only where one expert has more than 16 rows of two tokens.
+  if (rows && tokens <= kFbQuantTokens && E.a.nt == 16) {
     FbSource src = source(x, x_dtype, ldx, tokens, h, 32);
     src.rows = rows;
     src.top = top;

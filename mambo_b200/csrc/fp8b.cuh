@@ -206,7 +206,7 @@ constexpr int kFbCodes = 100;
 cudaError_t launch_fb_quant(const FbQuantParams& p, cudaStream_t stream);
 
 // --- the product -----------------------------------------------------------------
-// Unquantized activations that the product's own warps quantize (tiles of at most kFbQuantTokens).
+// Unquantized activations that the product's own warps quantize (tiles of 16 tokens, calls of at most kFbQuantTokens).
 struct FbSource {
   const void* x;     // [rows][k], row stride ldx; null: none
   int bf16;          // else f32
@@ -216,7 +216,7 @@ struct FbSource {
   const int* rows;   // row r of the product is row rows[r] / top of x; null: row r
   int top, last;     // last: x's last row, which bounds the others
 };
-constexpr int kFbQuantTokens = 2;  // most tokens of a tile that the product quantizes itself
+constexpr int kFbQuantTokens = 2;  // most tokens of a call that the product quantizes itself
 struct FbGemmParams {
   FbSource src;
   const uint8_t* packed;

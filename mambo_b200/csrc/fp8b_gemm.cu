@@ -619,7 +619,9 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
     // For tiles of one or two tokens: four warps take the K blocks in turn and write each block's E4M3 bytes and scale
     // codes straight into its stage, a half warp a token, 8 values a lane. Every tile's CTA quantizes the tokens anew:
     // for one token that is less than a launch of the quantizer (repeated, weights in L2: 4096 x 4096 11.2 -> 10.6 us, 64 experts of 2048 x
-    // 1408, six a token: 32.0 -> 27.9), for eight it held the weights up (28672 x 8192: 39 -> 54 us).
+    // 1408, six a token: 32.0 -> 27.9), for eight it held the weights up (28672 x 8192: 39 -> 54 us). A call of one or two
+    // tokens has tiles of more rows only where a route names an expert repeatedly: those follow two at a time (the loop
+    // for them costs the others 0.5 %: one token of 64 experts, weights from HBM, 28.8 -> 28.95 us).
     const FbSource& src = p.src;
     const int who = warp - 8, col = (lane & 15) * 8, r = lane >> 4;
     pdl_wait();
@@ -627,10 +629,13 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
     bool ok = true;
     while (ok && walk.next()) {
       const FbTile t = cur.at(walk.tile);
-      const int mine = t.o + t.row0 + min(r, t.n - 1);
-      const int64_t row = min(src.rows ? max(__ldg(src.rows + mine), 0) / src.top : mine, src.last) * src.ldx;
       const uint32_t sf_at = kFbRecord + (uint32_t)fb_part_rows(t.n, false) * 128u;
-      auto load = [&](int kb, uint4& lo, uint4& hi) {
+      // Where row i of the tile starts in x (the last row for one past it).
+      auto row_at = [&](int i) {
+        const int mine = t.o + t.row0 + min(i, t.n - 1);
+        return min(src.rows ? max(__ldg(src.rows + mine), 0) / src.top : mine, src.last) * src.ldx;
+      };
+      auto load = [&](int64_t row, int kb, uint4& lo, uint4& hi) {
         const int64_t k0 = (int64_t)kb * 128 + col;
         lo = hi = make_uint4(0, 0, 0, 0);
         if (src.bf16) {
@@ -658,14 +663,8 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
           }
         }
       };
-      int kb = walk.kb0 + ((who - it) & 3);  // this warp's first block of the segment
-      uint4 lo, hi, lo2, hi2;
-      if (kb < walk.kb1) load(kb, lo, hi);
-      for (; kb < walk.kb1; kb += 4) {
-        if (kb + 4 < walk.kb1) load(kb + 4, lo2, hi2);
-        const int at = it + (kb - walk.kb0), s = at % S;
-        if (at >= S && !(ok = fb_warp_wait(kEmpty + 8 * s, (uint32_t)(at / S - 1) & 1u, kSiteFbEmpty))) break;
-        uint8_t* st = tiles0 + (size_t)s * C::kStage;
+      // A half warp's values to row i of the stage (a row past the tile's holds the last one again; nothing stores it).
+      auto store = [&](uint8_t* st, int i, const uint4& lo, const uint4& hi) {
         uint32_t word;
         uint2 q;
         if (src.bf16) {
@@ -675,8 +674,25 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
                               __uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w)};
           q = quantize8(v, src.group, lane, word);
         }
-        *reinterpret_cast<uint2*>(st + kFbRecord + r * 128 + ((((lane & 15) >> 1) ^ r) << 4) + (lane & 1) * 8) = q;
-        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(st + sf_at + r * 16) = word;
+        *reinterpret_cast<uint2*>(st + kFbRecord + i * 128 + ((((lane & 15) >> 1) ^ (i & 7)) << 4) + (lane & 1) * 8) = q;
+        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(st + sf_at + i * 16) = word;
+      };
+      const int64_t row = row_at(r);
+      int kb = walk.kb0 + ((who - it) & 3);  // this warp's first block of the segment
+      uint4 lo, hi, lo2, hi2;
+      if (kb < walk.kb1) load(row, kb, lo, hi);
+      for (; kb < walk.kb1; kb += 4) {
+        if (kb + 4 < walk.kb1) load(row, kb + 4, lo2, hi2);
+        const int at = it + (kb - walk.kb0), s = at % S;
+        if (at >= S && !(ok = fb_warp_wait(kEmpty + 8 * s, (uint32_t)(at / S - 1) & 1u, kSiteFbEmpty))) break;
+        uint8_t* st = tiles0 + (size_t)s * C::kStage;
+        store(st, r, lo, hi);
+#pragma unroll 1
+        for (int i = 2; i < t.n; i += 2) {
+          uint4 more_lo, more_hi;
+          load(row_at(i + r), kb, more_lo, more_hi);
+          store(st, i + r, more_lo, more_hi);
+        }
         fence_proxy_async_shared();  // the tensor core reads the stage through the async proxy
         __syncwarp();
         if (lane == 0) mbar_arrive(kFull + 8 * s);
