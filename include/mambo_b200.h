@@ -6,6 +6,12 @@
  * never throws or aborts. On failure a message is kept per host thread and
  * can be read with mambo_last_error().
  *
+ * A call with a workspace may be several launches that hand data on through
+ * it. So calls that share one must not overlap on the GPU, and host threads
+ * that share one must not enter such calls at the same time (their launches
+ * could alternate on the stream). A workspace outlives the CUDA graphs that
+ * were captured with it.
+ *
  * Each declaration cites the reference interface it replaces (paths relative
  * to the Menooker/Mambo tree). The reference launches cuTile kernels from
  * Python through CuPy; these functions are what its launch wrappers

@@ -12,10 +12,8 @@ import torch
 from . import _lib
 
 _checked_devices: dict[int, int] = {}
-_workspaces: dict[tuple[int, int], torch.Tensor] = {}
-_captured: set[tuple[int, int]] = set()  # workspaces that a CUDA graph may use
-_kept: list[torch.Tensor] = []  # ... and such as a larger one has replaced
-_ws_lock = threading.Lock()
+_workspaces: dict[tuple[int, int], "_Workspace"] = {}
+_kept: list[torch.Tensor] = []  # buffers that a CUDA graph may use and a larger one has replaced
 
 
 def as_cuda_tensor(obj) -> torch.Tensor:
@@ -66,11 +64,45 @@ def _stream_is_capturing(device: torch.device, stream: int) -> bool:
         return torch.cuda.is_current_stream_capturing()
 
 
-def workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    """Zero-filled scratch for split-K partials and counters, one per (device, stream).
+class _Workspace:
+    """The scratch buffer of one (device, stream), at ``ptr`` with ``size`` bytes; while it is entered, the calling thread's."""
+
+    __slots__ = ("lock", "buffer", "ptr", "size", "captured")
+
+    def __init__(self):
+        self.lock = threading.Lock()
+        self.buffer: torch.Tensor | None = None
+        self.ptr = self.size = 0
+        self.captured = False  # a CUDA graph may use the buffer
+
+    def __enter__(self) -> "_Workspace":
+        return self
+
+    def __exit__(self, *exc) -> None:
+        self.lock.release()
+
+    def grow(self, device: torch.device, nbytes: int) -> None:
+        size = max(nbytes, 1 << 20, 2 * self.size)
+        # Drain pending work before swapping buffers: a kernel on the stream
+        # may still use the old one, and the zero-fill runs on torch's stream.
+        torch.cuda.synchronize(device)
+        new = torch.zeros(size, dtype=torch.uint8, device=device)
+        torch.cuda.synchronize(device)
+        if self.captured:
+            _kept.append(self.buffer)
+        self.buffer, self.ptr, self.size, self.captured = new, new.data_ptr(), size, False
+
+
+def workspace(device: torch.device, stream: int, nbytes: int) -> _Workspace:
+    """Zero-filled scratch for split-K partials and counters, one buffer per (device, stream), to be used as
+
+        with workspace(device, stream, nbytes) as ws:
+            ...  # the C call that gets ws.ptr and ws.size
 
     The kernels leave the counter region zeroed again, so the buffer is reused
     across calls on the same stream; calls on different streams get their own.
+    A call may be several launches that hand data on through the buffer, so
+    another host thread's call on the stream waits here until they are queued.
 
     A CUDA graph keeps the address of the buffer that its calls were captured
     with. So a buffer that was handed out during a capture is never freed, also
@@ -79,30 +111,27 @@ def workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     itself cannot make the buffer grow (it could neither be zero-filled at once
     nor outlive the graph): that raises, and the capture goes on undisturbed.
     """
-    index = device.index if device.index is not None else torch.cuda.current_device()
-    key = (index, stream)
+    current = torch._C._cuda_getDevice()  # torch.cuda.current_device() without its 0.2 us of initialization checks
+    index = device.index
+    if index is None:
+        index = current
+    ws = _workspaces.get((index, stream))
+    if ws is None:
+        ws = _workspaces.setdefault((index, stream), _Workspace())
     # Only the current stream's capture is a cheap question: any other stream counts as capturing.
-    captured = index != torch.cuda.current_device() or stream != torch._C._cuda_getCurrentRawStream(index) \
-        or torch.cuda.is_current_stream_capturing()
-    with _ws_lock:
-        ws = _workspaces.get(key)
-        if ws is None or ws.numel() < nbytes:
+    captured = index != current or stream != torch._C._cuda_getCurrentRawStream(index) \
+        or torch._C._cuda_isCurrentStreamCapturing()
+    ws.lock.acquire()
+    try:
+        if ws.size < nbytes:
             dev = torch.device("cuda", index)
             if captured and _stream_is_capturing(dev, stream):
-                raise RuntimeError(f"the stream's workspace has {0 if ws is None else ws.numel()} bytes and this call needs "
-                                   f"{nbytes}: run it once on the stream before capturing it")
-            size = max(nbytes, 1 << 20)
-            if ws is not None:
-                size = max(size, 2 * ws.numel())
-            # Drain pending work before swapping buffers: a kernel on `stream`
-            # may still use the old one, and the zero-fill runs on torch's stream.
-            torch.cuda.synchronize(dev)
-            if key in _captured:
-                _captured.remove(key)
-                _kept.append(ws)
-            ws = torch.zeros(size, dtype=torch.uint8, device=dev)
-            torch.cuda.synchronize(dev)
-            _workspaces[key] = ws
+                raise RuntimeError(f"the stream's workspace has {ws.size} bytes and this call needs {nbytes}: run it once on "
+                                   "the stream before capturing it")
+            ws.grow(dev, nbytes)
         if captured:
-            _captured.add(key)
-        return ws
+            ws.captured = True
+    except BaseException:
+        ws.lock.release()
+        raise
+    return ws

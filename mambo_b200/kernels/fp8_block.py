@@ -39,7 +39,7 @@ class Fp8BlockFields(TypedDict):
 
 def _device_guard(device: torch.device):
     """torch.cuda.device, or nothing when the device is current already."""
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         return _NO_GUARD
     return torch.cuda.device(device)
 
@@ -201,11 +201,11 @@ def launch_fp8_block_matmul(x_values, x_scales, weight: Fp8BlockFields, *, strea
     if m:
         with _device_guard(dev):
             st = _stream(stream, dev)
-            ws = _runtime.workspace(dev, st, _linear_workspace_bytes(m, 1, weight["n_rows"], k))
-            _lib.check(_lib.load().mambo_fp8b_linear(
-                x_values.data_ptr(), _row_stride(x_values), x_scales.data_ptr(), _row_stride(x_scales), group, m,
-                weight["weight"], out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), ws.data_ptr(), ws.numel(), st),
-                "launch_fp8_block_matmul")
+            with _runtime.workspace(dev, st, _linear_workspace_bytes(m, 1, weight["n_rows"], k)) as ws:
+                _lib.check(_lib.load().mambo_fp8b_linear(
+                    x_values.data_ptr(), _row_stride(x_values), x_scales.data_ptr(), _row_stride(x_scales), group, m,
+                    weight["weight"], out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), ws.ptr, ws.size, st),
+                    "launch_fp8_block_matmul")
     return out
 
 
@@ -228,10 +228,10 @@ def fp8_block_linear(x, weight: Fp8BlockFields, *, act_group: int = BLOCK, strea
     if m:
         with _device_guard(dev):
             st = _stream(stream, dev)
-            ws = _runtime.workspace(dev, st, _linear_workspace_bytes(m, 1, n, weight["k"]))
-            _lib.check(_lib.load().mambo_fp8b_linear_fused(
-                x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), act_group, m, weight["weight"], out.data_ptr(),
-                _DTYPES[out.dtype], _row_stride(out), ws.data_ptr(), ws.numel(), st), "fp8_block_linear")
+            with _runtime.workspace(dev, st, _linear_workspace_bytes(m, 1, n, weight["k"])) as ws:
+                _lib.check(_lib.load().mambo_fp8b_linear_fused(
+                    x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), act_group, m, weight["weight"], out.data_ptr(),
+                    _DTYPES[out.dtype], _row_stride(out), ws.ptr, ws.size, st), "fp8_block_linear")
     return out
 
 
@@ -254,9 +254,9 @@ def fp8_block_grouped_linear(x, offsets, weight: Fp8BlockFields, *, act_group: i
     if rows:
         with _device_guard(dev):
             st = _stream(stream, dev)
-            ws = _runtime.workspace(dev, st, _linear_workspace_bytes(rows, experts, n, weight["k"]))
-            _lib.check(_lib.load().mambo_fp8b_grouped_linear(
-                x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), act_group, rows, offsets.data_ptr(), weight["weight"],
-                out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), ws.data_ptr(), ws.numel(), st),
-                "fp8_block_grouped_linear")
+            with _runtime.workspace(dev, st, _linear_workspace_bytes(rows, experts, n, weight["k"])) as ws:
+                _lib.check(_lib.load().mambo_fp8b_grouped_linear(
+                    x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), act_group, rows, offsets.data_ptr(), weight["weight"],
+                    out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), ws.ptr, ws.size, st),
+                    "fp8_block_grouped_linear")
     return out

@@ -283,16 +283,16 @@ def linear_into(x_values: torch.Tensor, x_scales: torch.Tensor, iq3_weight: IQ3S
     with torch.cuda.device(dev):
         st = _runtime.stream_handle(stream, dev)
         need = lib.mambo_iq3s_linear_workspace_bytes(m, n_rows, blocks, cfg)
-        ws = _runtime.workspace(dev, st, need)
-        out_dtype = _lib.MAMBO_BF16 if out.dtype == torch.bfloat16 else _lib.MAMBO_F32
-        _lib.check(
-            lib.mambo_iq3s_linear_q(
-                x_values.data_ptr(), x_values.stride(0), x_scales.data_ptr(), x_scales.stride(0), m, w,
-                _get_iq3_table(dev).data_ptr(), out.data_ptr(), out_dtype, out.stride(0), _quant_out_struct(qout),
-                cfg, ws.data_ptr(), ws.numel(), st,
-            ),
-            "launch_iq3_s_fp8_matmul",
-        )
+        with _runtime.workspace(dev, st, need) as ws:
+            out_dtype = _lib.MAMBO_BF16 if out.dtype == torch.bfloat16 else _lib.MAMBO_F32
+            _lib.check(
+                lib.mambo_iq3s_linear_q(
+                    x_values.data_ptr(), x_values.stride(0), x_scales.data_ptr(), x_scales.stride(0), m, w,
+                    _get_iq3_table(dev).data_ptr(), out.data_ptr(), out_dtype, out.stride(0), _quant_out_struct(qout),
+                    cfg, ws.ptr, ws.size, st,
+                ),
+                "launch_iq3_s_fp8_matmul",
+            )
     return out
 
 
@@ -350,16 +350,16 @@ def fused_linear_into(x: torch.Tensor, iq3_weight: IQ3SFields, out: torch.Tensor
     with torch.cuda.device(dev):
         st = _runtime.stream_handle(stream, dev)
         need = lib.mambo_iq3s_linear_fused_workspace_bytes(m, n_rows, blocks, cfg)
-        ws = _runtime.workspace(dev, st, need)
-        x_dtype = _lib.MAMBO_BF16 if x.dtype == torch.bfloat16 else _lib.MAMBO_F32
-        out_dtype = _lib.MAMBO_BF16 if out.dtype == torch.bfloat16 else _lib.MAMBO_F32
-        _lib.check(
-            lib.mambo_iq3s_linear_fused_q(
-                x.data_ptr(), x_dtype, x.stride(0), m, w, _get_iq3_table(dev).data_ptr(), out.data_ptr(), out_dtype,
-                out.stride(0), _quant_out_struct(qout), cfg, ws.data_ptr(), ws.numel(), st,
-            ),
-            "iq3_s_fp8_linear",
-        )
+        with _runtime.workspace(dev, st, need) as ws:
+            x_dtype = _lib.MAMBO_BF16 if x.dtype == torch.bfloat16 else _lib.MAMBO_F32
+            out_dtype = _lib.MAMBO_BF16 if out.dtype == torch.bfloat16 else _lib.MAMBO_F32
+            _lib.check(
+                lib.mambo_iq3s_linear_fused_q(
+                    x.data_ptr(), x_dtype, x.stride(0), m, w, _get_iq3_table(dev).data_ptr(), out.data_ptr(), out_dtype,
+                    out.stride(0), _quant_out_struct(qout), cfg, ws.ptr, ws.size, st,
+                ),
+                "iq3_s_fp8_linear",
+            )
     return out
 
 
@@ -381,15 +381,15 @@ def fused_linear_ar_into(x: torch.Tensor, iq3_weight: IQ3SFields, out: torch.Ten
     with torch.cuda.device(dev):
         st = _runtime.stream_handle(stream, dev)
         need = lib.mambo_iq3s_linear_fused_workspace_bytes(m, n_rows, blocks, cfg)
-        ws = _runtime.workspace(dev, st, need)
-        out_dtype = _lib.MAMBO_BF16 if out.dtype == torch.bfloat16 else _lib.MAMBO_F32
-        _lib.check(
-            lib.mambo_iq3s_linear_fused_ar(
-                x.data_ptr(), _lib.MAMBO_BF16, x.stride(0), m, w, _get_iq3_table(dev).data_ptr(), out.data_ptr(),
-                out_dtype, out.stride(0), comm.handle, cfg, ws.data_ptr(), ws.numel(), st,
-            ),
-            "fused all-reduce linear",
-        )
+        with _runtime.workspace(dev, st, need) as ws:
+            out_dtype = _lib.MAMBO_BF16 if out.dtype == torch.bfloat16 else _lib.MAMBO_F32
+            _lib.check(
+                lib.mambo_iq3s_linear_fused_ar(
+                    x.data_ptr(), _lib.MAMBO_BF16, x.stride(0), m, w, _get_iq3_table(dev).data_ptr(), out.data_ptr(),
+                    out_dtype, out.stride(0), comm.handle, cfg, ws.ptr, ws.size, st,
+                ),
+                "fused all-reduce linear",
+            )
     return out
 
 
@@ -458,15 +458,15 @@ def group_linear_into(xs, iq3_weights, outs, stream=None, qouts=None) -> list:
     with torch.cuda.device(dev):
         st = _runtime.stream_handle(stream, dev)
         need = lib.mambo_iq3s_linear_group_workspace_bytes(items, count)
-        ws = _runtime.workspace(dev, st, need)
-        qarr = None
-        if qouts is not None:
-            qarr = (_lib.MamboQuantOut * count)()
-            for i, qo in enumerate(qouts):
-                if qo is not None:
-                    qarr[i] = _quant_out_struct(qo)
-        _lib.check(lib.mambo_iq3s_linear_group_q(items, qarr, count, _get_iq3_table(dev).data_ptr(), ws.data_ptr(),
-                                                 ws.numel(), st), "iq3_s_fp8_linear_group")
+        with _runtime.workspace(dev, st, need) as ws:
+            qarr = None
+            if qouts is not None:
+                qarr = (_lib.MamboQuantOut * count)()
+                for i, qo in enumerate(qouts):
+                    if qo is not None:
+                        qarr[i] = _quant_out_struct(qo)
+            _lib.check(lib.mambo_iq3s_linear_group_q(items, qarr, count, _get_iq3_table(dev).data_ptr(), ws.ptr,
+                                                     ws.size, st), "iq3_s_fp8_linear_group")
     return outs
 
 

@@ -86,12 +86,12 @@ def launch_moe_route(logits, top_k: int, *, scoring: str = "softmax", bias=None,
     if tokens:
         with _device_guard(dev):
             st = _stream(stream, dev)
-            ws = _runtime.workspace(dev, st, _route_workspace_bytes(tokens, experts))
-            _lib.check(_lib.load().mambo_moe_route(
-                logits.data_ptr(), _DTYPES[logits.dtype], _row_stride(logits), 0 if bias is None else bias.data_ptr(),
-                tokens, experts, top_k, _SCORING[scoring], int(renormalize), scale, ids.data_ptr(),
-                weights.data_ptr(), offsets.data_ptr(), positions.data_ptr(), rows.data_ptr(), ws.data_ptr(),
-                ws.numel(), st), "launch_moe_route")
+            with _runtime.workspace(dev, st, _route_workspace_bytes(tokens, experts)) as ws:
+                _lib.check(_lib.load().mambo_moe_route(
+                    logits.data_ptr(), _DTYPES[logits.dtype], _row_stride(logits), 0 if bias is None else bias.data_ptr(),
+                    tokens, experts, top_k, _SCORING[scoring], int(renormalize), scale, ids.data_ptr(),
+                    weights.data_ptr(), offsets.data_ptr(), positions.data_ptr(), rows.data_ptr(), ws.ptr,
+                    ws.size, st), "launch_moe_route")
     else:
         offsets.zero_()
     return {"ids": ids, "weights": weights, "offsets": offsets, "positions": positions, "rows": rows,
@@ -179,10 +179,10 @@ def fp8_moe_experts(x, route: MoeRoute, gate_up: Fp8BlockFields, down: Fp8BlockF
         code = _DTYPES[out.dtype]
         with _device_guard(dev):
             st = _stream(stream, dev)
-            ws = _runtime.workspace(dev, st, _experts_workspace_bytes(tokens, top, experts, h, i, code))
-            _lib.check(_lib.load().mambo_moe_experts(
-                x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), tokens, route["ids"].data_ptr(),
-                route["weights"].data_ptr(), route["positions"].data_ptr(), route["offsets"].data_ptr(),
-                route["rows"].data_ptr(), top, gate_up["weight"], down["weight"], out.data_ptr(), code,
-                _row_stride(out), ws.data_ptr(), ws.numel(), st), "fp8_moe_experts")
+            with _runtime.workspace(dev, st, _experts_workspace_bytes(tokens, top, experts, h, i, code)) as ws:
+                _lib.check(_lib.load().mambo_moe_experts(
+                    x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), tokens, route["ids"].data_ptr(),
+                    route["weights"].data_ptr(), route["positions"].data_ptr(), route["offsets"].data_ptr(),
+                    route["rows"].data_ptr(), top, gate_up["weight"], down["weight"], out.data_ptr(), code,
+                    _row_stride(out), ws.ptr, ws.size, st), "fp8_moe_experts")
     return out

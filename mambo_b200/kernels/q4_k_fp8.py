@@ -116,12 +116,12 @@ def launch_q4_k_fp8_matmul(x_values, x_scales, x_sums, weight: Q4KFields, *, str
     lib = _lib.load()
     with torch.cuda.device(dev):
         st = _runtime.stream_handle(stream, dev)
-        ws = _runtime.workspace(dev, st, lib.mambo_q4k_linear_workspace_bytes(m, n_rows, n_blocks, cfg))
-        _lib.check(lib.mambo_q4k_linear(
-            x_values.data_ptr(), x_values.stride(0), x_scales.data_ptr(), x_scales.stride(0), x_sums.data_ptr(),
-            x_sums.stride(0), m, weight["packed"].data_ptr(), n_rows, n_blocks, out.data_ptr(),
-            _lib.MAMBO_BF16 if out.dtype == torch.bfloat16 else _lib.MAMBO_F32, out.stride(0), cfg, ws.data_ptr(),
-            ws.numel(), st), "launch_q4_k_fp8_matmul")
+        with _runtime.workspace(dev, st, lib.mambo_q4k_linear_workspace_bytes(m, n_rows, n_blocks, cfg)) as ws:
+            _lib.check(lib.mambo_q4k_linear(
+                x_values.data_ptr(), x_values.stride(0), x_scales.data_ptr(), x_scales.stride(0), x_sums.data_ptr(),
+                x_sums.stride(0), m, weight["packed"].data_ptr(), n_rows, n_blocks, out.data_ptr(),
+                _lib.MAMBO_BF16 if out.dtype == torch.bfloat16 else _lib.MAMBO_F32, out.stride(0), cfg, ws.ptr,
+                ws.size, st), "launch_q4_k_fp8_matmul")
     return out
 
 
@@ -146,12 +146,12 @@ def q4_k_fp8_linear(x, weight: Q4KFields, *, stream=None, out_dtype: torch.dtype
     lib = _lib.load()
     with torch.cuda.device(dev):
         st = _runtime.stream_handle(stream, dev)
-        ws = _runtime.workspace(dev, st, lib.mambo_q4k_linear_fused_workspace_bytes(m, n_rows, n_blocks, cfg))
-        _lib.check(lib.mambo_q4k_linear_fused(
-            x.data_ptr(), _lib.MAMBO_BF16 if x.dtype == torch.bfloat16 else _lib.MAMBO_F32, x.stride(0), m,
-            weight["packed"].data_ptr(), n_rows, n_blocks, out.data_ptr(),
-            _lib.MAMBO_BF16 if out.dtype == torch.bfloat16 else _lib.MAMBO_F32, out.stride(0), cfg, ws.data_ptr(),
-            ws.numel(), st), "q4_k_fp8_linear")
+        with _runtime.workspace(dev, st, lib.mambo_q4k_linear_fused_workspace_bytes(m, n_rows, n_blocks, cfg)) as ws:
+            _lib.check(lib.mambo_q4k_linear_fused(
+                x.data_ptr(), _lib.MAMBO_BF16 if x.dtype == torch.bfloat16 else _lib.MAMBO_F32, x.stride(0), m,
+                weight["packed"].data_ptr(), n_rows, n_blocks, out.data_ptr(),
+                _lib.MAMBO_BF16 if out.dtype == torch.bfloat16 else _lib.MAMBO_F32, out.stride(0), cfg, ws.ptr,
+                ws.size, st), "q4_k_fp8_linear")
     return out
 
 
@@ -188,8 +188,8 @@ def q4_k_linear_group_into(xs, weights, outs, *, stream=None) -> list:
     lib = _lib.load()
     with torch.cuda.device(dev):
         st = _runtime.stream_handle(stream, dev)
-        ws = _runtime.workspace(dev, st, lib.mambo_q4k_linear_group_workspace_bytes(items, count))
-        _lib.check(lib.mambo_q4k_linear_group(items, count, ws.data_ptr(), ws.numel(), st), "q4_k_linear_group")
+        with _runtime.workspace(dev, st, lib.mambo_q4k_linear_group_workspace_bytes(items, count)) as ws:
+            _lib.check(lib.mambo_q4k_linear_group(items, count, ws.ptr, ws.size, st), "q4_k_linear_group")
     return outs
 
 

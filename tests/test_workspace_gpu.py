@@ -1,6 +1,8 @@
-"""CUDA graphs over calls whose per-stream workspace is replaced by a larger one after the capture."""
+"""The per-stream workspaces on the GPU: graphs captured before a larger one replaces them, and host threads that share one."""
 
 from __future__ import annotations
+
+import threading
 
 import pytest
 import torch
@@ -16,8 +18,7 @@ pytestmark = pytest.mark.gpu
 @pytest.fixture(autouse=True)
 def _fresh_workspaces(monkeypatch):
     """Streams come from a pool: without this, an earlier test's large buffer may already be there."""
-    for name in ("_workspaces", "_captured"):
-        monkeypatch.setattr(_runtime, name, type(getattr(_runtime, name))())
+    monkeypatch.setattr(_runtime, "_workspaces", {})
     yield
     torch.cuda.synchronize()
     assert _lib.device_status()[0] == 0
@@ -25,7 +26,8 @@ def _fresh_workspaces(monkeypatch):
 
 def workspace_bytes(stream) -> int:
     """The size of the stream's buffer once a call that needs next to nothing has got it."""
-    return _runtime.workspace(torch.device("cuda", 0), stream.cuda_stream, 1).numel()
+    with _runtime.workspace(torch.device("cuda", 0), stream.cuda_stream, 1) as ws:
+        return ws.size
 
 
 def prepared(dev, n, k, seed, experts=None, **kw):
@@ -100,3 +102,32 @@ def test_a_capture_that_would_grow_the_workspace_is_refused(cuda_device):
     assert torch.equal(out, ref) and torch.equal(again, ref)
     with torch.cuda.stream(side):
         assert fp8_block_linear(large, w).shape == (700, 768)
+
+
+def test_two_threads_on_one_stream(cuda_device):
+    """Each thread gets its own results, whatever the other one calls in between."""
+    dev = cuda_device
+    w = prepared(dev, 768, 1024, 3)
+    gate_up, down = prepared(dev, 512, 1024, 4, experts=8, gate_up=True), prepared(dev, 1024, 256, 5, experts=8)
+
+    def layer(x, logits):
+        return fp8_block_linear(x, w), fp8_moe_experts(x, launch_moe_route(logits, 3), gate_up, down)
+
+    inputs = [(torch.randn(m, 1024, device=dev, dtype=torch.bfloat16), torch.randn(m, 8, device=dev)) for m in (40, 57, 3, 300)]
+    refs = [layer(*i) for i in inputs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def many(n):
+        for _ in range(60):
+            got = layer(*inputs[n])
+            torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, refs[n])):
+                wrong.append(n)
+
+    threads = [threading.Thread(target=many, args=(n,)) for n in range(len(inputs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
