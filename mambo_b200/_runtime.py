@@ -5,6 +5,8 @@ PyTorch provides device memory and streams; the compute is in libmambo_b200.
 
 from __future__ import annotations
 
+import dataclasses
+import functools
 import threading
 
 import torch
@@ -45,6 +47,55 @@ def stream_handle(stream, device: torch.device) -> int:
     raise TypeError(f"unsupported stream object {type(stream).__name__}")
 
 
+def _tensors(obj):
+    """The tensors of an argument or a result: one, or a list, tuple, dict or dataclass of them."""
+    if isinstance(obj, torch.Tensor):
+        yield obj
+    elif isinstance(obj, (list, tuple)):
+        for v in obj:
+            yield from _tensors(v)
+    elif isinstance(obj, dict):
+        for v in obj.values():
+            yield from _tensors(v)
+    elif dataclasses.is_dataclass(obj) and not isinstance(obj, type):
+        for f in dataclasses.fields(obj):
+            yield from _tensors(getattr(obj, f.name))
+
+
+def with_stream(operator):
+    """Runs an operator with its ``stream=`` (a torch stream or any handle) as the current one.
+
+    So what it allocates, copies (rows without unit stride) and fills belongs to
+    the stream that its kernels run on. The caller orders that stream with the
+    work that made the arguments, and his own with the results. Memory may be
+    let go of at any time: arguments are not used again before the stream is
+    done with them, nor results before the caller's current stream is.
+    """
+
+    @functools.wraps(operator)
+    def call(*args, stream=None, **kwargs):
+        if stream is None:
+            return operator(*args, **kwargs)
+        given = list(_tensors((args, kwargs)))
+        device = next((t.device for t in given if t.is_cuda), None)
+        if device is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        caller, handle = torch.cuda.current_stream(device), stream_handle(stream, device)
+        if handle == caller.cuda_stream:
+            return operator(*args, **kwargs)
+        target = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(handle, device=device)
+        with torch.cuda.stream(target):
+            result = operator(*args, **kwargs)
+        for t in given:
+            if t.is_cuda:
+                t.record_stream(target)
+        for t in _tensors(result):
+            t.record_stream(caller)
+        return result
+
+    return call
+
+
 def require_device(device: torch.device) -> None:
     """Raise RuntimeError unless `device` is an sm_100 GPU this library runs on."""
     index = device.index if device.index is not None else torch.cuda.current_device()
@@ -65,11 +116,12 @@ def _stream_is_capturing(device: torch.device, stream: int) -> bool:
 
 
 class _Workspace:
-    """The scratch buffer of one (device, stream), at ``ptr`` with ``size`` bytes; while it is entered, the calling thread's."""
+    """The scratch buffer of ``stream``, at ``ptr`` with ``size`` bytes; while it is entered, the calling thread's."""
 
-    __slots__ = ("lock", "buffer", "ptr", "size", "captured")
+    __slots__ = ("stream", "lock", "buffer", "ptr", "size", "captured")
 
-    def __init__(self):
+    def __init__(self, stream: int):
+        self.stream = stream
         self.lock = threading.Lock()
         self.buffer: torch.Tensor | None = None
         self.ptr = self.size = 0
@@ -93,12 +145,13 @@ class _Workspace:
         self.buffer, self.ptr, self.size, self.captured = new, new.data_ptr(), size, False
 
 
-def workspace(device: torch.device, stream: int, nbytes: int) -> _Workspace:
+def workspace(device: torch.device, stream: int | None, nbytes: int) -> _Workspace:
     """Zero-filled scratch for split-K partials and counters, one buffer per (device, stream), to be used as
 
         with workspace(device, stream, nbytes) as ws:
-            ...  # the C call that gets ws.ptr and ws.size
+            ...  # the C call that gets ws.ptr, ws.size and ws.stream
 
+    ``stream`` None: the current stream of ``device``, which is the current device.
     The kernels leave the counter region zeroed again, so the buffer is reused
     across calls on the same stream; calls on different streams get their own.
     A call may be several launches that hand data on through the buffer, so
@@ -111,16 +164,18 @@ def workspace(device: torch.device, stream: int, nbytes: int) -> _Workspace:
     itself cannot make the buffer grow (it could neither be zero-filled at once
     nor outlive the graph): that raises, and the capture goes on undisturbed.
     """
-    current = torch._C._cuda_getDevice()  # torch.cuda.current_device() without its 0.2 us of initialization checks
-    index = device.index
-    if index is None:
-        index = current
+    if stream is None:
+        index = device.index
+        stream, here = torch._C._cuda_getCurrentRawStream(index), True
+    else:
+        current = torch.cuda.current_device()
+        index = device.index if device.index is not None else current
+        here = index == current and stream == torch._C._cuda_getCurrentRawStream(index)
     ws = _workspaces.get((index, stream))
     if ws is None:
-        ws = _workspaces.setdefault((index, stream), _Workspace())
+        ws = _workspaces.setdefault((index, stream), _Workspace(stream))
     # Only the current stream's capture is a cheap question: any other stream counts as capturing.
-    captured = index != current or stream != torch._C._cuda_getCurrentRawStream(index) \
-        or torch._C._cuda_isCurrentStreamCapturing()
+    captured = not here or torch._C._cuda_isCurrentStreamCapturing()
     ws.lock.acquire()
     try:
         if ws.size < nbytes:

@@ -55,11 +55,9 @@ class _NoGuard:
 _NO_GUARD = _NoGuard()
 
 
-def _stream(stream, device: torch.device) -> int:
-    """As _runtime.stream_handle; the current stream without building a torch.cuda.Stream (2 us of a call's 17)."""
-    if stream is None:
-        return torch._C._cuda_getCurrentRawStream(device.index)
-    return _runtime.stream_handle(stream, device)
+def _stream(device: torch.device) -> int:
+    """The current stream's handle, without building a torch.cuda.Stream (2 us of a call's 17)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 _DTYPES = {torch.float32: _lib.MAMBO_F32, torch.bfloat16: _lib.MAMBO_BF16}
@@ -77,6 +75,7 @@ def _check_group(group: int) -> None:
         raise ValueError("activation scales are per 32 or per 128 values")
 
 
+@_runtime.with_stream
 def prepare_fp8_block_fields(values, scales, *, gate_up: bool = False, stream=None) -> Fp8BlockFields:
     """E4M3 weights [N,K] or [E,N,K] and their float32 block scales -> the packed copy the kernels stream.
 
@@ -112,7 +111,7 @@ def prepare_fp8_block_fields(values, scales, *, gate_up: bool = False, stream=No
     out_scales = torch.empty(lib.mambo_fp8b_scales_bytes(experts, n, k, int(gate_up)) // 4, dtype=torch.float32,
                              device=dev)
     with _device_guard(dev):
-        st = _stream(stream, dev)
+        st = _stream(dev)
         _lib.check(lib.mambo_fp8b_pack(
             values.data_ptr(), experts, n, k, values.stride(0), values.stride(1), values.stride(2), scales.data_ptr(),
             scales.stride(0), scales.stride(1), scales.stride(2), int(gate_up), packed.data_ptr(),
@@ -122,6 +121,7 @@ def prepare_fp8_block_fields(values, scales, *, gate_up: bool = False, stream=No
             "gate_up": bool(gate_up), "weight": weight}
 
 
+@_runtime.with_stream
 def launch_quantize_fp8_block(x, *, group: int = BLOCK, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
     """Return [M,K] E4M3 bytes and [M,ceil(K/group)] UE8M0 scale bytes of x (float32 or bfloat16 [M,K], any K)."""
     x = _runtime.as_cuda_tensor(x)
@@ -136,7 +136,7 @@ def launch_quantize_fp8_block(x, *, group: int = BLOCK, stream=None) -> tuple[to
     scales = torch.empty((m, -(-k // group)), dtype=torch.uint8, device=x.device)
     if m:
         with _device_guard(x.device):
-            st = _stream(stream, x.device)
+            st = _stream(x.device)
             _lib.check(_lib.load().mambo_fp8b_quantize(
                 x.data_ptr(), _DTYPES[x.dtype], m, k, _row_stride(x), group, values.data_ptr(), k, scales.data_ptr(),
                 scales.shape[1], st), "launch_quantize_fp8_block")
@@ -174,6 +174,7 @@ def _check_weight(weight: Fp8BlockFields, device: torch.device, grouped: bool) -
         raise ValueError("weight and activation must be on one device")
 
 
+@_runtime.with_stream
 def launch_fp8_block_matmul(x_values, x_scales, weight: Fp8BlockFields, *, stream=None,
                             out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """Quantized activations times a prepared weight -> out [M,N].
@@ -200,11 +201,10 @@ def launch_fp8_block_matmul(x_values, x_scales, weight: Fp8BlockFields, *, strea
     out = _output(out, m, weight["n_rows"], out_dtype, dev)
     if m:
         with _device_guard(dev):
-            st = _stream(stream, dev)
-            with _runtime.workspace(dev, st, _linear_workspace_bytes(m, 1, weight["n_rows"], k)) as ws:
+            with _runtime.workspace(dev, None, _linear_workspace_bytes(m, 1, weight["n_rows"], k)) as ws:
                 _lib.check(_lib.load().mambo_fp8b_linear(
                     x_values.data_ptr(), _row_stride(x_values), x_scales.data_ptr(), _row_stride(x_scales), group, m,
-                    weight["weight"], out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), ws.ptr, ws.size, st),
+                    weight["weight"], out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), ws.ptr, ws.size, ws.stream),
                     "launch_fp8_block_matmul")
     return out
 
@@ -219,6 +219,7 @@ def _activation(x, weight: Fp8BlockFields, act_group: int, grouped: bool) -> tor
     return x if x.stride(1) == 1 else x.contiguous()
 
 
+@_runtime.with_stream
 def fp8_block_linear(x, weight: Fp8BlockFields, *, act_group: int = BLOCK, stream=None,
                      out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """bf16/f32 activations [M,K] -> E4M3 with one scale per ``act_group`` values -> the linear, one C-ABI call."""
@@ -227,14 +228,14 @@ def fp8_block_linear(x, weight: Fp8BlockFields, *, act_group: int = BLOCK, strea
     out = _output(out, m, n, out_dtype, dev)
     if m:
         with _device_guard(dev):
-            st = _stream(stream, dev)
-            with _runtime.workspace(dev, st, _linear_workspace_bytes(m, 1, n, weight["k"])) as ws:
+            with _runtime.workspace(dev, None, _linear_workspace_bytes(m, 1, n, weight["k"])) as ws:
                 _lib.check(_lib.load().mambo_fp8b_linear_fused(
                     x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), act_group, m, weight["weight"], out.data_ptr(),
-                    _DTYPES[out.dtype], _row_stride(out), ws.ptr, ws.size, st), "fp8_block_linear")
+                    _DTYPES[out.dtype], _row_stride(out), ws.ptr, ws.size, ws.stream), "fp8_block_linear")
     return out
 
 
+@_runtime.with_stream
 def fp8_block_grouped_linear(x, offsets, weight: Fp8BlockFields, *, act_group: int = BLOCK, stream=None,
                              out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """Rows offsets[e] .. offsets[e+1]-1 of x [R,K] times expert e's weight, for every expert in one call.
@@ -253,10 +254,9 @@ def fp8_block_grouped_linear(x, offsets, weight: Fp8BlockFields, *, act_group: i
     out = _output(out, rows, n, out_dtype, dev)
     if rows:
         with _device_guard(dev):
-            st = _stream(stream, dev)
-            with _runtime.workspace(dev, st, _linear_workspace_bytes(rows, experts, n, weight["k"])) as ws:
+            with _runtime.workspace(dev, None, _linear_workspace_bytes(rows, experts, n, weight["k"])) as ws:
                 _lib.check(_lib.load().mambo_fp8b_grouped_linear(
                     x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), act_group, rows, offsets.data_ptr(), weight["weight"],
-                    out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), ws.ptr, ws.size, st),
+                    out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), ws.ptr, ws.size, ws.stream),
                     "fp8_block_grouped_linear")
     return out

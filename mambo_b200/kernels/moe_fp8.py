@@ -45,6 +45,7 @@ def _experts_workspace_bytes(tokens: int, top: int, experts: int, h: int, i: int
     return _lib.load().mambo_moe_experts_workspace_bytes(tokens, top, experts, h, i, out)
 
 
+@_runtime.with_stream
 def launch_moe_route(logits, top_k: int, *, scoring: str = "softmax", bias=None, renormalize: bool = True,
                      scale: float = 1.0, stream=None) -> MoeRoute:
     """The ``top_k`` experts of each token of logits [T,E] (float32 or bfloat16) and the order of their rows.
@@ -85,13 +86,12 @@ def launch_moe_route(logits, top_k: int, *, scoring: str = "softmax", bias=None,
     rows, offsets = buf.as_strided((n,), (1,), 3 * n), buf.as_strided((experts + 1,), (1,), 4 * n)
     if tokens:
         with _device_guard(dev):
-            st = _stream(stream, dev)
-            with _runtime.workspace(dev, st, _route_workspace_bytes(tokens, experts)) as ws:
+            with _runtime.workspace(dev, None, _route_workspace_bytes(tokens, experts)) as ws:
                 _lib.check(_lib.load().mambo_moe_route(
                     logits.data_ptr(), _DTYPES[logits.dtype], _row_stride(logits), 0 if bias is None else bias.data_ptr(),
                     tokens, experts, top_k, _SCORING[scoring], int(renormalize), scale, ids.data_ptr(),
                     weights.data_ptr(), offsets.data_ptr(), positions.data_ptr(), rows.data_ptr(), ws.ptr,
-                    ws.size, st), "launch_moe_route")
+                    ws.size, ws.stream), "launch_moe_route")
     else:
         offsets.zero_()
     return {"ids": ids, "weights": weights, "offsets": offsets, "positions": positions, "rows": rows,
@@ -119,6 +119,7 @@ def _check_route(route: MoeRoute, tokens: int, device: torch.device) -> int:
     return ids.shape[1]
 
 
+@_runtime.with_stream
 def launch_moe_combine(y, route: MoeRoute, *, stream=None, out_dtype: torch.dtype = torch.bfloat16,
                        out: torch.Tensor | None = None) -> torch.Tensor:
     """out[t] = sum_j weights[t,j] * y[positions[t,j]] for expert rows y [R,H] in expert order, summed in float32."""
@@ -136,7 +137,7 @@ def launch_moe_combine(y, route: MoeRoute, *, stream=None, out_dtype: torch.dtyp
         out.zero_()
     elif tokens:
         with _device_guard(dev):
-            st = _stream(stream, dev)
+            st = _stream(dev)
             _lib.check(_lib.load().mambo_moe_combine(
                 y.data_ptr(), _DTYPES[y.dtype], _row_stride(y), rows, route["positions"].data_ptr(),
                 route["weights"].data_ptr(), tokens, top, h, out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), st),
@@ -144,6 +145,7 @@ def launch_moe_combine(y, route: MoeRoute, *, stream=None, out_dtype: torch.dtyp
     return out
 
 
+@_runtime.with_stream
 def fp8_moe_experts(x, route: MoeRoute, gate_up: Fp8BlockFields, down: Fp8BlockFields, *, stream=None,
                     out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """A layer of routed experts, x [T,H] -> out [T,H], in one C-ABI call.
@@ -178,11 +180,10 @@ def fp8_moe_experts(x, route: MoeRoute, gate_up: Fp8BlockFields, down: Fp8BlockF
     if tokens:
         code = _DTYPES[out.dtype]
         with _device_guard(dev):
-            st = _stream(stream, dev)
-            with _runtime.workspace(dev, st, _experts_workspace_bytes(tokens, top, experts, h, i, code)) as ws:
+            with _runtime.workspace(dev, None, _experts_workspace_bytes(tokens, top, experts, h, i, code)) as ws:
                 _lib.check(_lib.load().mambo_moe_experts(
                     x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), tokens, route["ids"].data_ptr(),
                     route["weights"].data_ptr(), route["positions"].data_ptr(), route["offsets"].data_ptr(),
                     route["rows"].data_ptr(), top, gate_up["weight"], down["weight"], out.data_ptr(), code,
-                    _row_stride(out), ws.ptr, ws.size, st), "fp8_moe_experts")
+                    _row_stride(out), ws.ptr, ws.size, ws.stream), "fp8_moe_experts")
     return out

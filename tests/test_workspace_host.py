@@ -25,7 +25,7 @@ def device(monkeypatch):
     real_zeros, state = torch.zeros, Device()
     monkeypatch.setattr(torch, "zeros", lambda *shape, dtype=None, device=None: real_zeros(*shape, dtype=dtype))
     monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
-    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: state.capturing, raising=False)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 7, raising=False)
     monkeypatch.setattr(_runtime, "_stream_is_capturing", lambda device, stream: state.capturing, raising=False)
@@ -118,7 +118,6 @@ def test_calls_of_several_threads_on_a_stream_take_turns(device, monkeypatch, op
     monkeypatch.setattr(_runtime, "require_device", lambda dev: None)
     for module in (fp8_block, moe_fp8):
         monkeypatch.setattr(module, "_device_guard", lambda dev: fp8_block._NO_GUARD)
-        monkeypatch.setattr(module, "_stream", lambda stream, dev: 7)
     for f in (fp8_block._linear_workspace_bytes, moe_fp8._route_workspace_bytes, moe_fp8._experts_workspace_bytes):
         f.cache_clear()  # the sizes here are not the library's
     packed = torch.zeros(1)
