@@ -160,6 +160,7 @@ def _power_of_two(value: int, name: str) -> None:
 # ----------------------------------------------------------------------------
 # Standalone decoder
 # ----------------------------------------------------------------------------
+@_runtime.with_stream
 def launch_dequant_iq3_s(iq3_weight: IQ3SFields, *, tile_n: int = 1, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
     """Return [N,K] E4M3 bit patterns and [N,K/32] original F32 scales (iq3_s_fp8.py:341-351)."""
     _power_of_two(tile_n, "tile_n")
@@ -296,6 +297,7 @@ def linear_into(x_values: torch.Tensor, x_scales: torch.Tensor, iq3_weight: IQ3S
     return out
 
 
+@_runtime.with_stream
 def launch_iq3_s_fp8_matmul(x_values, x_scales, iq3_weight: IQ3SFields, *, stream=None,
                             out_dtype: torch.dtype = torch.float32, config: dict | None = None,
                             quantize_output: bool = False):
@@ -393,6 +395,7 @@ def fused_linear_ar_into(x: torch.Tensor, iq3_weight: IQ3SFields, out: torch.Ten
     return out
 
 
+@_runtime.with_stream
 def iq3_s_fp8_linear(x, iq3_weight: IQ3SFields, *, stream=None, out_dtype: torch.dtype = torch.bfloat16,
                      rounding: str = "nearest_even", config: dict | None = None, quantize_output: bool = False):
     """bf16/f32 activations [M,K] -> MXFP8 -> IQ3_S linear -> out_dtype [M,N] (quantize + matmul).
@@ -470,6 +473,7 @@ def group_linear_into(xs, iq3_weights, outs, stream=None, qouts=None) -> list:
     return outs
 
 
+@_runtime.with_stream
 def iq3_s_fp8_linear_group(xs, iq3_weights, *, stream=None, out_dtype: torch.dtype = torch.bfloat16) -> list:
     """Several independent ``iq3_s_fp8_linear`` calls as one (see ``group_linear_into``).
 

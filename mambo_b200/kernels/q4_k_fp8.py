@@ -36,6 +36,7 @@ class Q4KFields(TypedDict):
     n_blocks: int
 
 
+@_runtime.with_stream
 def prepare_q4_k_fields(raw: torch.Tensor, *, stream=None) -> Q4KFields:
     """GGUF Q4_K bytes [N, B, 144] or [N, B*144] (uint8, any strides) -> the packed copy the GEMV streams."""
     raw = _runtime.as_cuda_tensor(raw)
@@ -60,6 +61,7 @@ def prepare_q4_k_fields(raw: torch.Tensor, *, stream=None) -> Q4KFields:
     return {"packed": packed, "n_rows": n_rows, "n_blocks": n_blocks}
 
 
+@_runtime.with_stream
 def launch_quantize_fp8_sums(x, *, stream=None, rounding: str = "nearest_even"):
     """MXFP8 quantization plus each 32-value group's sum of its quantized values.
 
@@ -91,6 +93,7 @@ def _config(config: dict | None) -> _lib.MamboLinearConfig | None:
     return None if config is None else _lib.MamboLinearConfig.from_dict(config)
 
 
+@_runtime.with_stream
 def launch_q4_k_fp8_matmul(x_values, x_scales, x_sums, weight: Q4KFields, *, stream=None,
                            out_dtype: torch.dtype = torch.float32, config: dict | None = None,
                            out: torch.Tensor | None = None) -> torch.Tensor:
@@ -125,6 +128,7 @@ def launch_q4_k_fp8_matmul(x_values, x_scales, x_sums, weight: Q4KFields, *, str
     return out
 
 
+@_runtime.with_stream
 def q4_k_fp8_linear(x, weight: Q4KFields, *, stream=None, out_dtype: torch.dtype = torch.bfloat16,
                     config: dict | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """bf16/f32 activations [M,K] -> MXFP8 (round to nearest even, with group sums) -> Q4_K linear, one C-ABI call."""
@@ -193,6 +197,7 @@ def q4_k_linear_group_into(xs, weights, outs, *, stream=None) -> list:
     return outs
 
 
+@_runtime.with_stream
 def q4_k_fp8_linear_group(xs, weights, *, stream=None, out_dtype: torch.dtype = torch.bfloat16) -> list:
     """Several independent ``q4_k_fp8_linear`` calls as one (see ``q4_k_linear_group_into``)."""
     if out_dtype not in (torch.float32, torch.bfloat16):

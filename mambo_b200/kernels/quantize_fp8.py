@@ -47,6 +47,7 @@ def _activation_config(m: int, device: torch.device) -> dict:
     return BEST_CONFIGS[sm]["large" if m >= LARGE_TOKEN_THRESHOLD else "medium"]
 
 
+@_runtime.with_stream
 def launch_quantize_fp8(x, *, tile_m: int | None = None, tile_k_groups: int | None = None, stream=None,
                         rounding: str = "nearest_even", out=None) -> tuple[torch.Tensor, torch.Tensor]:
     """Return [M,K] E4M3 bytes and [M,K/32] E8M0 scale bytes (quantize_fp8.py:67-84).

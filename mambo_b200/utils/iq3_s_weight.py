@@ -43,6 +43,7 @@ class IQ3SFields:
     packed: torch.Tensor | None = None
 
 
+@_runtime.with_stream
 def prepare_iq3_s_fields(iq3_weight, *, stream=None, packed: bool = True, soa: bool = True) -> IQ3SFields:
     """Split GGUF uint8 [N,B,110] blocks into aligned SoA fields once (iq3_s_weight.py:25-54).
 
@@ -100,6 +101,7 @@ def has_soa_fields(iq3_weight: IQ3SFields) -> bool:
     return iq3_weight.qs.numel() > 0
 
 
+@_runtime.with_stream
 def pack_iq3_s_fields(fields: IQ3SFields, *, stream=None) -> IQ3SFields:
     """Return ``fields`` with the tile-major packed copy built (mambo_iq3s_pack)."""
     n, blocks = _weight_dimensions(fields)
