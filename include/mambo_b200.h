@@ -423,7 +423,8 @@ MAMBO_API int mambo_q4k_linear_group(const MamboQ4KItem* items, int count, void*
  * activations E4M3 with one UE8M0 scale per 32 values along K (MXFP8) or per
  * 128 (group = 32 or 128; exponents as mambo_quantize_mxfp8 forms them):
  *   out[m, n] = sum_b sw[n/128, b] * sum_{k in block b} xq[m, k] * 2^e(m, k/group) * wq[n, k]
- * with FP32 accumulation. Any N, K >= 1 (up to 2^24) and any M >= 1. A value
+ * with FP32 accumulation. Any N, K >= 1 (up to 2^24) and any M >= 1 (up to
+ * 2^28); the size functions return 0 for what the calls refuse. A value
  * group with NaN or infinity has the scale code 0xFF and makes its row NaN.
  *
  * A weight is packed once, from values [experts, N, K] and scales [experts,

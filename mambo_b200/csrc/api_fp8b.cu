@@ -10,6 +10,10 @@ namespace {
 constexpr int64_t kMaxRows = (int64_t)1 << 28;   // rows of a call (32-bit row arithmetic with padding)
 constexpr int64_t kMaxExtent = (int64_t)1 << 24; // N and K
 
+bool extent_ok(int64_t v) { return v >= 1 && v <= kMaxExtent; }
+bool experts_ok(int64_t v) { return v >= 1 && v <= kFbMaxExperts; }
+// tokens * top choices, without forming a product that may not fit.
+bool choices_ok(int64_t tokens, int64_t top) { return tokens >= 1 && top >= 1 && tokens <= kMaxRows / top; }
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 bool dtype_ok(int d) { return d == MAMBO_F32 || d == MAMBO_BF16; }
 int elem(int d) { return d == MAMBO_BF16 ? 2 : 4; }
@@ -18,9 +22,9 @@ int check_weight(const MamboFp8BlockWeight* w) {
   if (!w || !w->packed || !w->scales) return api_fail(MAMBO_EINVAL, "null weight field");
   if ((uintptr_t)w->packed % 16 || (uintptr_t)w->scales % 4)
     return api_fail(MAMBO_EINVAL, "packed weight must be 16-byte aligned, its scales 4-byte");
-  if (w->n_rows < 1 || w->k < 1 || w->n_rows > kMaxExtent || w->k > kMaxExtent)
+  if (!extent_ok(w->n_rows) || !extent_ok(w->k))
     return api_fail(MAMBO_EINVAL, "weight must have N and K in [1, 2^24]");
-  if (w->n_experts < 1 || w->n_experts > kFbMaxExperts)
+  if (!experts_ok(w->n_experts))
     return api_fail(MAMBO_EINVAL, "a weight has 1 to %d experts", kFbMaxExperts);
   if (w->gate_up && w->n_rows % 2) return api_fail(MAMBO_EINVAL, "a gate/up weight has an even number of rows");
   return MAMBO_OK;
@@ -186,7 +190,7 @@ ExpertsPlan plan_experts(int64_t tokens, int64_t top, int64_t experts, int64_t h
 extern "C" {
 
 size_t mambo_fp8b_packed_bytes(int64_t experts, int64_t n, int64_t k, int gate_up) {
-  if (experts < 1 || experts > kFbMaxExperts || n < 1 || k < 1 || n > kMaxExtent || k > kMaxExtent) return 0;
+  if (!experts_ok(experts) || !extent_ok(n) || !extent_ok(k)) return 0;
   return (size_t)experts * fb_row_tiles(n, gate_up) * ((k + 127) / 128) * kFbRecord;
 }
 
@@ -199,8 +203,8 @@ int mambo_fp8b_pack(const uint8_t* values, int64_t experts, int64_t n, int64_t k
                     int64_t scale_stride_row, int64_t scale_stride_k, int gate_up, void* packed, float* packed_scales,
                     mambo_stream_t stream) {
   if (!values || !block_scales || !packed || !packed_scales) return api_fail(MAMBO_EINVAL, "null pointer");
-  if (experts < 1 || experts > kFbMaxExperts) return api_fail(MAMBO_EINVAL, "a weight has 1 to %d experts", kFbMaxExperts);
-  if (n < 1 || k < 1 || n > kMaxExtent || k > kMaxExtent)
+  if (!experts_ok(experts)) return api_fail(MAMBO_EINVAL, "a weight has 1 to %d experts", kFbMaxExperts);
+  if (!extent_ok(n) || !extent_ok(k))
     return api_fail(MAMBO_EINVAL, "weight must have N and K in [1, 2^24]");
   if (gate_up && n % 2) return api_fail(MAMBO_EINVAL, "a gate/up weight has an even number of rows");
   if ((uintptr_t)packed % 16) return api_fail(MAMBO_EINVAL, "packed buffer must be 16-byte aligned");
@@ -234,7 +238,7 @@ int mambo_fp8b_quantize(const void* x, int x_dtype, int64_t m, int64_t k, int64_
                         int64_t ldq, uint8_t* s, int64_t lds, mambo_stream_t stream) {
   if (!x || !q || !s) return api_fail(MAMBO_EINVAL, "null pointer");
   if (!dtype_ok(x_dtype)) return api_fail(MAMBO_EINVAL, "activation must be f32 or bf16");
-  if (m < 1 || m > kMaxRows || k < 1 || k > kMaxExtent) return api_fail(MAMBO_EINVAL, "activation must be [M,K] with M, K >= 1");
+  if (m < 1 || m > kMaxRows || !extent_ok(k)) return api_fail(MAMBO_EINVAL, "activation must be [M,K] with M, K >= 1");
   if (group != 32 && group != 128) return api_fail(MAMBO_EINVAL, "activation scales are per 32 or per 128 values");
   if (ldx < k || ldq < k || lds < (k + group - 1) / group) return api_fail(MAMBO_EINVAL, "row stride smaller than the row");
   if (m * ((k + 1023) / 1024) >= 2147483647) return api_fail(MAMBO_EINVAL, "the call is too large: split its rows");
@@ -259,7 +263,7 @@ int mambo_fp8b_quantize(const void* x, int x_dtype, int64_t m, int64_t k, int64_
 }
 
 size_t mambo_fp8b_linear_workspace_bytes(int64_t rows, int64_t experts, int64_t n, int64_t k) {
-  if (rows < 1 || experts < 1 || n < 1 || k < 1) return 0;
+  if (rows < 1 || rows > kMaxRows || !experts_ok(experts) || !extent_ok(n) || !extent_ok(k)) return 0;
   return kWorkspaceCounterBytes + product_bytes(plan(rows, experts, rows, n, k, 0));
 }
 
@@ -300,7 +304,7 @@ int mambo_fp8b_grouped_linear(const void* x, int x_dtype, int64_t ldx, int group
 }
 
 size_t mambo_moe_route_workspace_bytes(int64_t tokens, int64_t experts) {
-  if (tokens < 1 || experts < 1) return 0;
+  if (!choices_ok(tokens, 1) || !experts_ok(experts)) return 0;
   const int64_t chunk = fb_route_chunk(tokens);
   return kWorkspaceCounterBytes + align256((size_t)((tokens + chunk - 1) / chunk) * (experts + 1) * sizeof(int));
 }
@@ -311,10 +315,10 @@ int mambo_moe_route(const void* logits, int dtype, int64_t ld, const float* bias
                     mambo_stream_t stream) {
   if (!logits || !ids || !weights || !offsets || !positions) return api_fail(MAMBO_EINVAL, "null pointer");
   if (!dtype_ok(dtype)) return api_fail(MAMBO_EINVAL, "logits must be f32 or bf16");
-  if (experts < 1 || experts > kFbMaxExperts) return api_fail(MAMBO_EINVAL, "1 to %d experts", kFbMaxExperts);
+  if (!experts_ok(experts)) return api_fail(MAMBO_EINVAL, "1 to %d experts", kFbMaxExperts);
   if (top < 1 || top > MAMBO_MOE_MAX_TOP || top > experts)
     return api_fail(MAMBO_EINVAL, "top must be in [1, min(%d, experts)]", MAMBO_MOE_MAX_TOP);
-  if (tokens < 1 || tokens * top > kMaxRows) return api_fail(MAMBO_EINVAL, "tokens must be at least 1, tokens * top at most 2^28");
+  if (!choices_ok(tokens, top)) return api_fail(MAMBO_EINVAL, "tokens must be at least 1, tokens * top at most 2^28");
   if (ld < experts) return api_fail(MAMBO_EINVAL, "row stride smaller than the row");
   if (scoring != MAMBO_MOE_SOFTMAX && scoring != MAMBO_MOE_SIGMOID) return api_fail(MAMBO_EINVAL, "unknown scoring %d", scoring);
   int st = check_workspace(workspace, workspace_bytes, mambo_moe_route_workspace_bytes(tokens, experts));
@@ -350,7 +354,7 @@ int mambo_moe_combine(const void* y, int y_dtype, int64_t ldy, int64_t rows, con
                       mambo_stream_t stream) {
   if (!y || !positions || !weights || !out) return api_fail(MAMBO_EINVAL, "null pointer");
   if (!dtype_ok(y_dtype) || !dtype_ok(out_dtype)) return api_fail(MAMBO_EINVAL, "y and out must be f32 or bf16");
-  if (tokens < 1 || top < 1 || tokens * top > kMaxRows || rows < 1 || h < 1 || h > kMaxExtent)
+  if (!choices_ok(tokens, top) || rows < 1 || !extent_ok(h))
     return api_fail(MAMBO_EINVAL, "bad tokens, top, rows or width");
   if (ldy < h || ldo < h) return api_fail(MAMBO_EINVAL, "row stride smaller than the row");
   int sms, smem;
@@ -365,7 +369,7 @@ int mambo_moe_combine(const void* y, int y_dtype, int64_t ldy, int64_t rows, con
 
 size_t mambo_moe_experts_workspace_bytes(int64_t tokens, int top, int64_t experts, int64_t h, int64_t i,
                                          int out_dtype) {
-  if (tokens < 1 || top < 1 || experts < 1 || h < 1 || i < 1) return 0;
+  if (top > MAMBO_MOE_MAX_TOP || !choices_ok(tokens, top) || !experts_ok(experts) || !extent_ok(h) || !extent_ok(i)) return 0;
   return plan_experts(tokens, top, experts, h, i, out_dtype).total;
 }
 
@@ -384,7 +388,7 @@ int mambo_moe_experts(const void* x, int x_dtype, int64_t ldx, int64_t tokens, c
     return api_fail(MAMBO_EINVAL, "down must be [experts, hidden size, features] to the gate/up weight's [experts, 2 * features, hidden size]");
   if (!dtype_ok(x_dtype) || !dtype_ok(out_dtype)) return api_fail(MAMBO_EINVAL, "x and out must be f32 or bf16");
   if (top < 1 || top > MAMBO_MOE_MAX_TOP) return api_fail(MAMBO_EINVAL, "top must be in [1, %d]", MAMBO_MOE_MAX_TOP);
-  if (tokens < 1 || tokens * top > kMaxRows) return api_fail(MAMBO_EINVAL, "tokens must be at least 1, tokens * top at most 2^28");
+  if (!choices_ok(tokens, top)) return api_fail(MAMBO_EINVAL, "tokens must be at least 1, tokens * top at most 2^28");
   if (ldx < h || ldo < h) return api_fail(MAMBO_EINVAL, "row stride smaller than the row");
   const ExpertsPlan E = plan_experts(tokens, top, experts, h, i, out_dtype);
   st = check_size(E.a, E.rows, experts, h);
