@@ -6,6 +6,7 @@
  * never throws or aborts. On failure a message is kept per host thread and
  * can be read with mambo_last_error().
  *
+ * Pointers are aligned to their elements (and further where a call says so).
  * A call with a workspace may be several launches that hand data on through
  * it. So calls that share one must not overlap on the GPU, and host threads
  * that share one must not enter such calls at the same time (their launches

@@ -18,6 +18,10 @@ size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 bool dtype_ok(int d) { return d == MAMBO_F32 || d == MAMBO_BF16; }
 int elem(int d) { return d == MAMBO_BF16 ? 2 : 4; }
 
+// Pointers are read and written element by element at least: one off its elements' alignment would fault.
+bool aligned(const void* p, int bytes) { return (uintptr_t)p % bytes == 0; }
+constexpr const char* kUnaligned = "a pointer is not aligned to its elements";
+
 int check_weight(const MamboFp8BlockWeight* w) {
   if (!w || !w->packed || !w->scales) return api_fail(MAMBO_EINVAL, "null weight field");
   if ((uintptr_t)w->packed % 16 || (uintptr_t)w->scales % 4)
@@ -120,6 +124,7 @@ int check_linear(const void* x, int64_t m, int group, const MamboFp8BlockWeight*
   if (group != 32 && group != 128) return api_fail(MAMBO_EINVAL, "activation scales are per 32 or per 128 values");
   if (!dtype_ok(out_dtype)) return api_fail(MAMBO_EINVAL, "out must be f32 or bf16");
   if (ldo < w->n_rows) return api_fail(MAMBO_EINVAL, "out row stride is smaller than N");
+  if (!aligned(out, elem(out_dtype))) return api_fail(MAMBO_EINVAL, kUnaligned);
   return MAMBO_OK;
 }
 
@@ -207,7 +212,8 @@ int mambo_fp8b_pack(const uint8_t* values, int64_t experts, int64_t n, int64_t k
   if (!extent_ok(n) || !extent_ok(k))
     return api_fail(MAMBO_EINVAL, "weight must have N and K in [1, 2^24]");
   if (gate_up && n % 2) return api_fail(MAMBO_EINVAL, "a gate/up weight has an even number of rows");
-  if ((uintptr_t)packed % 16) return api_fail(MAMBO_EINVAL, "packed buffer must be 16-byte aligned");
+  if (!aligned(packed, 16)) return api_fail(MAMBO_EINVAL, "packed buffer must be 16-byte aligned");
+  if (!aligned(block_scales, 4) || !aligned(packed_scales, 4)) return api_fail(MAMBO_EINVAL, kUnaligned);
   FbPackParams p{};
   p.w = values;
   p.stride_e = stride_expert;
@@ -241,6 +247,7 @@ int mambo_fp8b_quantize(const void* x, int x_dtype, int64_t m, int64_t k, int64_
   if (m < 1 || m > kMaxRows || !extent_ok(k)) return api_fail(MAMBO_EINVAL, "activation must be [M,K] with M, K >= 1");
   if (group != 32 && group != 128) return api_fail(MAMBO_EINVAL, "activation scales are per 32 or per 128 values");
   if (ldx < k || ldq < k || lds < (k + group - 1) / group) return api_fail(MAMBO_EINVAL, "row stride smaller than the row");
+  if (!aligned(x, elem(x_dtype))) return api_fail(MAMBO_EINVAL, kUnaligned);
   if (m * ((k + 1023) / 1024) >= 2147483647) return api_fail(MAMBO_EINVAL, "the call is too large: split its rows");
   int sms, smem;
   const int st = api_require_sm100(&sms, &smem);
@@ -287,6 +294,7 @@ int mambo_fp8b_linear_fused(const void* x, int x_dtype, int64_t ldx, int group, 
   if (w->n_experts != 1) return api_fail(MAMBO_EINVAL, "a weight of several experts needs mambo_fp8b_grouped_linear");
   if (!dtype_ok(x_dtype)) return api_fail(MAMBO_EINVAL, "activation must be f32 or bf16");
   if (ldx < w->k) return api_fail(MAMBO_EINVAL, "row stride smaller than the row");
+  if (!aligned(x, elem(x_dtype))) return api_fail(MAMBO_EINVAL, kUnaligned);
   return linear_impl(x, x_dtype, ldx, nullptr, 0, group, m, nullptr, w, out, out_dtype, ldo, workspace,
                      workspace_bytes, (cudaStream_t)stream);
 }
@@ -299,6 +307,7 @@ int mambo_fp8b_grouped_linear(const void* x, int x_dtype, int64_t ldx, int group
   if (st != MAMBO_OK) return st;
   if (!dtype_ok(x_dtype)) return api_fail(MAMBO_EINVAL, "activation must be f32 or bf16");
   if (ldx < w->k) return api_fail(MAMBO_EINVAL, "row stride smaller than the row");
+  if (!aligned(x, elem(x_dtype)) || !aligned(offsets, 4)) return api_fail(MAMBO_EINVAL, kUnaligned);
   return linear_impl(x, x_dtype, ldx, nullptr, 0, group, rows, offsets, w, out, out_dtype, ldo, workspace,
                      workspace_bytes, (cudaStream_t)stream);
 }
@@ -323,6 +332,9 @@ int mambo_moe_route(const void* logits, int dtype, int64_t ld, const float* bias
   if (scoring != MAMBO_MOE_SOFTMAX && scoring != MAMBO_MOE_SIGMOID) return api_fail(MAMBO_EINVAL, "unknown scoring %d", scoring);
   int st = check_workspace(workspace, workspace_bytes, mambo_moe_route_workspace_bytes(tokens, experts));
   if (st != MAMBO_OK) return st;
+  if (!aligned(logits, elem(dtype)) || !aligned(bias, 4) || !aligned(ids, 4) || !aligned(weights, 4) || !aligned(offsets, 4) ||
+      !aligned(positions, 4) || !aligned(rows, 4))
+    return api_fail(MAMBO_EINVAL, kUnaligned);
   int sms, smem;
   st = api_require_sm100(&sms, &smem);
   if (st != MAMBO_OK) return st;
@@ -357,6 +369,8 @@ int mambo_moe_combine(const void* y, int y_dtype, int64_t ldy, int64_t rows, con
   if (!choices_ok(tokens, top) || rows < 1 || !extent_ok(h))
     return api_fail(MAMBO_EINVAL, "bad tokens, top, rows or width");
   if (ldy < h || ldo < h) return api_fail(MAMBO_EINVAL, "row stride smaller than the row");
+  if (!aligned(y, elem(y_dtype)) || !aligned(positions, 4) || !aligned(weights, 4) || !aligned(out, elem(out_dtype)))
+    return api_fail(MAMBO_EINVAL, kUnaligned);
   int sms, smem;
   const int st = api_require_sm100(&sms, &smem);
   if (st != MAMBO_OK) return st;
@@ -390,6 +404,9 @@ int mambo_moe_experts(const void* x, int x_dtype, int64_t ldx, int64_t tokens, c
   if (top < 1 || top > MAMBO_MOE_MAX_TOP) return api_fail(MAMBO_EINVAL, "top must be in [1, %d]", MAMBO_MOE_MAX_TOP);
   if (!choices_ok(tokens, top)) return api_fail(MAMBO_EINVAL, "tokens must be at least 1, tokens * top at most 2^28");
   if (ldx < h || ldo < h) return api_fail(MAMBO_EINVAL, "row stride smaller than the row");
+  if (!aligned(x, elem(x_dtype)) || !aligned(ids, 4) || !aligned(weights, 4) || !aligned(positions, 4) || !aligned(offsets, 4) ||
+      !aligned(rows, 4) || !aligned(out, elem(out_dtype)))
+    return api_fail(MAMBO_EINVAL, kUnaligned);
   const ExpertsPlan E = plan_experts(tokens, top, experts, h, i, out_dtype);
   st = check_size(E.a, E.rows, experts, h);
   if (st == MAMBO_OK) st = check_size(E.b, E.rows, experts, i);

@@ -1,4 +1,4 @@
-"""CPU: size functions and argument checks of the FP8 block and expert entry points at the ends of 64 bits."""
+"""CPU: size functions and argument checks of the FP8 block and expert entry points: huge sizes, unaligned pointers."""
 
 from __future__ import annotations
 
@@ -63,3 +63,43 @@ assert lib.mambo_moe_combine(4096, 0, 8, 4, 4096, 4096, 4, (1 << 31) - 1, 8, 409
 print("done")
 """)
     assert out.strip() == "done"
+
+
+def test_unaligned_pointers_are_refused():
+    """A pointer off its elements' alignment is an error of the call, never a fault of the GPU (no device is needed)."""
+    lib, e, f32, bf16 = _lib.load(), _lib.MAMBO_EINVAL, _lib.MAMBO_F32, _lib.MAMBO_BF16
+    big = (1 << 63) - 1
+    w = _lib.MamboFp8BlockWeight(4096, 4096, 256, 256, 1, 0)
+    grouped = _lib.MamboFp8BlockWeight(4096, 4096, 256, 256, 4, 0)
+    gate_up = _lib.MamboFp8BlockWeight(4096, 4096, 256, 256, 4, 1)
+    down = _lib.MamboFp8BlockWeight(4096, 4096, 256, 128, 4, 0)
+
+    def refused(call, good, pointers):
+        for name, off in pointers:
+            assert call(**{**good, name: 4096 + off}) == e, (name, off)
+            assert "aligned" in _lib.last_error()
+
+    refused(lambda s, ps: lib.mambo_fp8b_pack(4096, 1, 256, 256, 0, 256, 1, s, 0, 2, 1, 0, 4096, ps, None),
+            dict(s=4096, ps=4096), [("s", 2), ("ps", 2)])
+    refused(lambda x, t: lib.mambo_fp8b_quantize(x, t, 4, 256, 256, 128, 4096, 256, 4096, 2, None), dict(x=4096, t=f32),
+            [("x", 1), ("x", 2)])
+    refused(lambda x, t: lib.mambo_fp8b_quantize(x, t, 4, 256, 256, 128, 4096, 256, 4096, 2, None), dict(x=4096, t=bf16),
+            [("x", 1)])
+    for t, off in ((f32, 2), (bf16, 1)):
+        refused(lambda x, out: lib.mambo_fp8b_linear_fused(x, t, 256, 128, 4, w, out, t, 256, 4096, big, None),  # noqa: B023
+                dict(x=4096, out=4096), [("x", off), ("out", off)])
+        refused(lambda out: lib.mambo_fp8b_linear(4097, 256, 4097, 2, 128, 4, w, out, t, 256, 4096, big, None),  # noqa: B023
+                dict(out=4096), [("out", off)])
+        refused(lambda x, o, out: lib.mambo_fp8b_grouped_linear(x, t, 256, 128, 4, o, grouped, out, t, 256, 4096,  # noqa: B023
+                                                                big, None),
+                dict(x=4096, o=4096, out=4096), [("x", off), ("o", 2), ("out", off)])
+        refused(lambda l, b, i, wt, o, p, r: lib.mambo_moe_route(l, t, 8, b, 4, 8, 2, 0, 1, 1.0, i, wt, o, p, r, 4096,  # noqa: B023
+                                                                 big, None),
+                dict(l=4096, b=4096, i=4096, wt=4096, o=4096, p=4096, r=4096),
+                [("l", off), ("b", 2), ("i", 2), ("wt", 2), ("o", 2), ("p", 2), ("r", 2)])
+        refused(lambda y, p, wt, out: lib.mambo_moe_combine(y, t, 8, 8, p, wt, 4, 2, 8, out, t, 8, None),  # noqa: B023
+                dict(y=4096, p=4096, wt=4096, out=4096), [("y", off), ("p", 2), ("wt", 2), ("out", off)])
+        refused(lambda x, i, wt, p, o, r, out: lib.mambo_moe_experts(x, t, 256, 4, i, wt, p, o, r, 2, gate_up, down,  # noqa: B023
+                                                                     out, t, 256, 4096, big, None),
+                dict(x=4096, i=4096, wt=4096, p=4096, o=4096, r=4096, out=4096),
+                [("x", off), ("i", 2), ("wt", 2), ("p", 2), ("o", 2), ("r", 2), ("out", off)])
