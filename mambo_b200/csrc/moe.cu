@@ -13,10 +13,10 @@ namespace {
 constexpr int kPlaceThreads = 1024;
 __host__ __device__ constexpr int route_threads(int nv) { return nv <= 8 ? 1024 : 512; }
 
-// Monotone map of a float to an unsigned key (0 is free: it marks masked experts).
+// Monotone map of a number to an unsigned key: 0 is free (it marks masked experts), zeros of either sign have one key.
 __device__ __forceinline__ uint32_t order_key(float f) {
   const uint32_t b = __float_as_uint(f);
-  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+  return (b & 0x80000000u) ? 0u - b : b | 0x80000000u;
 }
 
 // One token, a warp: expert 32*i + lane in slot i of the lane. Experts whose
