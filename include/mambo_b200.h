@@ -510,7 +510,8 @@ MAMBO_API int mambo_moe_combine(const void* y, int y_dtype, int64_t ldy, int64_t
  * H]; down [experts, H, I]; ids, weights, positions, offsets and rows (or
  * NULL: without it a decode call takes one more launch) from mambo_moe_route
  * or laid out as it lays them out; a token may name an expert more than once.
- * Each expert row rounds once to out_dtype before the sum.
+ * Each expert row rounds once to out_dtype before the sum, which is FP32: for
+ * a bf16 result with one rounding take MAMBO_F32 and round that.
  * workspace: mambo_moe_experts_workspace_bytes(), zero-filled once.
  */
 MAMBO_API size_t mambo_moe_experts_workspace_bytes(int64_t tokens, int top, int64_t experts, int64_t h, int64_t i,

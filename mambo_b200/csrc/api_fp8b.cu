@@ -453,6 +453,10 @@ int mambo_moe_experts(const void* x, int x_dtype, int64_t ldx, int64_t tokens, c
     if (e == cudaSuccess)
       e = run_gemm(gate_up, E.a, nullptr, xa, E.rows, offsets, nullptr, 0, 0, &ha, partials, workspace, sms, smem, stream);
   }
+  // An expert's row rounds once to the output type before the weighted sum, which is FP32 and rounds once more. Kept in
+  // f32 for a bf16 output, the rows cost 8 % of a prompt (4096 tokens, 64 experts of 2048 x 4096, eight a token: 1,340 ->
+  // 1,442 us) and 2 % of a token (28.8 -> 29.5); the error against float64 is 2.35e-3 of the norm as it is, 1.66e-3 with
+  // the output's rounding alone. Who wants the latter takes an f32 output and rounds it.
   if (e == cudaSuccess)
     e = run_gemm(down, E.b, nullptr, ha, E.rows, offsets, y, out_dtype == MAMBO_BF16, h, nullptr, partials, workspace, sms,
                  smem, stream);
