@@ -22,8 +22,8 @@
 //
 // Work: the (row tile, token tile) tiles of all experts, numbered expert by
 // expert, one per CTA and wave. Where the last wave would leave many CTAs idle
-// for long, the last one to two waves are cut at K blocks into equal ranges
-// instead (stream-K); a tile that several CTAs share is summed in K order by
+// for long, its tiles are cut at K blocks into equal ranges instead (stream-K),
+// which come first; a tile that several CTAs share is summed in K order by
 // whichever arrives last: nothing waits, and the sums do not depend on who.
 //
 // Warps: 0 weights producer, 1 and 3 MMA, 2 activations producer, then the
@@ -48,15 +48,27 @@ namespace mambo {
 namespace {
 
 constexpr int kMaxStagesB = 12;
-// K blocks that the CTAs which the last wave leaves idle lose on average from which a K split pays for publishing and
-// adding up the parts. Measured: 4096 x 4096 at one token (25 blocks, weights in L2) 11.5 -> 11.2 us, 28672 x 8192 at 8 (31) 41.5 ->
-// 39.7; split all the same, 32 experts of 4096 x 2048 at 96 rows (5) 45.3 -> 49.4. CTA pairs, 8192 x 28672 at 200 tokens
-// (100 blocks) 99 -> 89; split all the same, 5003 x 3001 at 77 (18) 17.1 -> 25.4. After several waves the CTAs have drifted
-// apart and the last ones run faster alone: 8 experts of 28672 x 4096 at 32 tokens (12 waves) 227 us unsplit, 233 split.
-constexpr int kWorth = 12, kWorthPair = 30, kWorthWaves = 4;
-__host__ __device__ inline bool fb_split_pays(int64_t tiles, int64_t kblocks, int64_t ctas) {
-  const int64_t rem = tiles % ctas;
-  return rem && tiles < kWorthWaves * ctas && (ctas - rem) * kblocks >= kWorth * ctas;
+// Whether the last wave's tiles are split along K: publishing and adding up the parts has to cost less than the CTAs that
+// the wave leaves idle could do. All of it in K blocks of a CTA that streams its weights alone, 0.225 us (a pair 0.285);
+// measured with and without the split over 1 to 420 tiles of 8 to 192 blocks, weights from HBM.
+// Single wave. All CTAs at once take 1.65 times as long a block, for HBM, so a split saves K * (1 - 1.65 * tiles / CTAs).
+// It costs some 20 blocks for tiles of 16 tokens, 30 for 32, and for 64, whose parts are added one by one, 35 and 4 a part.
+// One token of 4096 x 4096 10.2 us unsplit, 10.4 split, x 14336 28.3 and 17.5, 8192 x 4096 10.3 and 13.2; 64 tokens of
+// 4096 x 4096 12.9 and 21.6, x 14336 30.5 and 26.9.
+// After a whole wave the parts are added up under the tiles that follow, so that a loss of 30 blocks on average is enough:
+// 8 tokens of 28672 x 8192 (31) 41.9 and 40.9, x 4096 (15) 24.0 and 26.8. After two the CTAs have drifted apart and the last
+// ones run faster alone: 340 tiles of 48 blocks lose 1 us, 380 lose 2.
+// CTA pairs: 55 and 5 a part of what the idle pairs lose, and only where they are most of them. 192 tokens of 4096 x 8192
+// (50, 5 parts) 25.4 unsplit, 32.2 split, x 14336 (87) 39.8 and 37.4, x 28672 (175) 72.9 and 45.5.
+template <int NT>
+__host__ __device__ inline bool fb_split_pays(int tiles, int kblocks, int ctas) {  // kblocks up to 2^17: all fits 32 bits
+  const int rem = tiles < ctas ? tiles : tiles - ctas;
+  if (rem <= 0 || rem >= ctas) return false;
+  const int parts = ctas * 4 < rem * kblocks ? ctas / rem : kblocks / 4;  // of a tile: at least 4 blocks each
+  const int idle = (ctas - rem) * kblocks;
+  if (NT > 64) return 2 * tiles <= ctas && idle >= (55 + 5 * parts) * ctas;
+  if (NT <= 32 && tiles > ctas) return idle >= 30 * ctas;
+  return (20 * ctas - 33 * rem) * kblocks >= 20 * ctas * (NT <= 16 ? 20 : NT <= 32 ? 30 : 35 + 4 * parts);
 }
 
 // kPair: CTA pairs. A tile is 256 weight rows (a row tile per CTA) x NT tokens; each CTA loads half of the
@@ -87,13 +99,12 @@ __host__ __device__ inline uint32_t fb_tables_bytes(int experts) {
   return ((uint32_t)(experts + 1) * 8 + 127) / 128 * 128;  // tile and row prefix
 }
 
-// This CTA's share of the tiles. Whole: one tile of each wave. kSplit: where the last wave would leave too many CTAs idle
-// for too long, an equal range of the K blocks of the last one to two waves comes first (stream-K); the parts' sums
-// have to be published and added up, which is worth it once the idle CTAs lose some kWorth K blocks on average.
-template <bool kSplit>
+// This CTA's share of the tiles. Whole: one tile of each wave. kSplit: where it pays (above), an equal range of the K
+// blocks of the last wave's tiles comes first (stream-K); the parts' sums are published and added up.
+template <bool kSplit, int NT>
 struct FbWalk;
-template <>
-struct FbWalk<false> {
+template <int NT>
+struct FbWalk<false, NT> {
   int kb_n, tiles, ncl, at;
   int tile, kb1;  // the current segment
   static constexpr int kb0 = 0, cl = 0;
@@ -106,8 +117,8 @@ struct FbWalk<false> {
   }
   __device__ __forceinline__ int owner(int) const { return 0; }  // of no split tile
 };
-template <>
-struct FbWalk<true> {
+template <int NT>
+struct FbWalk<true, NT> {
   int kb_n, sk, tiles, ncl, cl, nsk;
   int u, u1, units;    // the host keeps tiles * K blocks below 2^31
   int at;              // next whole tile
@@ -117,9 +128,7 @@ struct FbWalk<true> {
     tiles = tiles_;
     ncl = ncl_;
     cl = cl_;
-    const int rem = tiles % ncl;
-    sk = 0;
-    if (fb_split_pays(tiles, kb_n, ncl)) sk = rem;
+    sk = fb_split_pays<NT>(tiles, kb_n, ncl) ? (tiles < ncl ? tiles : tiles - ncl) : 0;  // the last wave's tiles
     units = sk * kb_n;
     // Each part at least four K blocks.
     nsk = max(1, min(ncl, units / 4));
@@ -447,7 +456,7 @@ __global__ void __launch_bounds__(FbCfg<NT, kPair, kQuant>::kThreads, 1) fb_gemm
   if constexpr (kPair) cluster_sync_all();  // both CTAs' barriers and TMEM are ready before any remote use
   tc::fence_after_sync();
 
-  FbWalk<kSplit> walk(uniform(tile_start[p.experts]), KB, (int)blockIdx.x / (kPair ? 2 : 1), (int)gridDim.x / (kPair ? 2 : 1));
+  FbWalk<kSplit, NT> walk(uniform(tile_start[p.experts]), KB, (int)blockIdx.x / (kPair ? 2 : 1), (int)gridDim.x / (kPair ? 2 : 1));
   FbCursor cur{tile_start, offs, p.experts, NT, row_groups, 0};
 
   // Register split of the pair kernel, launched with 168 a thread (384 threads): 128 x 56 + 256 x 224 = 384 x 168.
@@ -983,8 +992,10 @@ cudaError_t launch_kernel(const FbGemmParams& p, int grid, cudaStream_t stream) 
   return launch_pdl_cluster(k, dim3(grid), dim3(FbCfg<NT, kPair, kQuant>::kThreads), smem, stream, kPair ? 2 : 1, p);
 }
 // Single CTAs decide on the device whether to split (an expert-grouped call's tiles are counted there). A CTA pair's
-// partial sums are large (98 KB a CTA): only a call whose tiles leave most pairs idle for long splits, and the others
-// run a kernel without that code, which also keeps its registers (14336 x 4096 at 2048 tokens: 131 us, with it 148).
+// partial sums are large (98 KB a CTA), and the code for them costs its K loop registers, used or not (14336 x 4096 at 2048
+// tokens: 131 us without it, 148 with), so the host decides, and a grouped call does not split. That one would gain little
+// and lose more: 4 experts of 1024 x 14336 at 800 rows 49.3 us, with the split kernel 46.8; one of 8 experts of 14336 x 4096
+// at 512 rows 45.3 and 62.4; 64 of 4096 x 4096 at 16384 rows 474 and 490.
 template <int NT, bool kQuant = false>
 cudaError_t launch_one(const FbGemmParams& p, int grid, cudaStream_t stream) {
   return p.hidden.x8 ? launch_kernel<NT, false, true, true, kQuant>(p, grid, stream)
@@ -993,8 +1004,8 @@ cudaError_t launch_one(const FbGemmParams& p, int grid, cudaStream_t stream) {
 cudaError_t launch_pair(const FbGemmParams& p, int grid, cudaStream_t stream) {
   constexpr int NT = kFbPairTokens;
   if (p.hidden.x8) return launch_kernel<NT, true, true, false>(p, grid, stream);
-  const int64_t tiles = (int64_t)(p.row_tiles + 1) / 2 * fb_tiles((int)p.rows, NT), pairs = grid / 2;
-  if (!p.offsets && 2 * tiles <= pairs && (pairs - tiles) * p.act.kblocks >= kWorthPair * pairs)
+  const int tiles = (p.row_tiles + 1) / 2 * fb_tiles((int)p.rows, NT), pairs = grid / 2;  // the host's size check: they fit
+  if (!p.offsets && fb_split_pays<NT>(tiles, p.act.kblocks, pairs))
     return launch_kernel<NT, true, false, true>(p, grid, stream);
   return launch_kernel<NT, true, false, false>(p, grid, stream);
 }
