@@ -107,7 +107,9 @@ cudaError_t run_gemm(const MamboFp8BlockWeight* w, const Plan& P, const FbSource
   g.ldo = ldo;
   if (hidden) g.hidden = *hidden;
   g.stages = fb_gemm_stages(P.nt, g.experts, smem_optin, hidden != nullptr);
-  // Most experts have one token tile at most (twice the even share fits it): their weights are read once.
+  // Weights are read once where a call has one token tile, or as a rule an expert has (its tile holds twice the even share):
+  // evict-first keeps the rest in the L2. 64 experts of 4096 x 4096 at 16 rows each 166 us with it, 174 without, of 1024 x
+  // 2048 33.1 and 35.6. With all 1024 rows in one expert its weights are read by 32 tiles, 64-65 us and 19.6 either way.
   g.evict_weights = offsets ? !fb_is_pair(P.nt) : rows <= P.nt;
   g.partials = (float*)partials;
   g.counters = (int*)((uint8_t*)workspace + kWorkspaceSplitCounterOffset);

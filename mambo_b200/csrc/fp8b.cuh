@@ -33,7 +33,7 @@ constexpr uint32_t kFbRecord = 128u * 128u;  // bytes of a packed weight record
 constexpr uint32_t kFbAtom = 512u;           // bytes of a scale-factor atom (128 rows x 4 groups)
 constexpr int kFbMaxExperts = 1024;
 
-// Tokens of a tile above which CTA pairs work on it (and the largest tile).
+// Tokens of a CTA pair's tile, the largest; single CTAs take tiles of 16, 32 and 64 (fb_tile_for).
 constexpr int kFbPairTokens = 192;
 
 struct FbActivations {
@@ -234,13 +234,13 @@ struct FbGemmParams {
   // next product's activations, in place of out; its tiles are cut as act's.
   FbActivations hidden;  // x8 null: none
   int stages;
-  int evict_weights;   // 1: weights are read once (evict-first)
+  int evict_weights;   // 1: weights are mostly read once (evict-first)
   float* partials;     // [grid][2][128 * nt]
   int* counters;       // [grid][8], zero on entry and left zero
 };
 // Device addresses of the product kernels' status record and wait limit (the current device's).
 cudaError_t fb_status_symbols(void** status, void** limit);
-// Token-tile sizes the kernel is built for.
+// The tile, of those that the kernel is built for, for a call or an expert of so many rows.
 int fb_tile_for(int64_t expected_rows);
 uint32_t fb_gemm_smem(int nt, int experts, int stages, bool hidden);
 int fb_gemm_stages(int nt, int experts, int smem_optin, bool hidden);

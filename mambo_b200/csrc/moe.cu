@@ -1,5 +1,5 @@
-// Expert routing, the hidden activation of the experts' path and the weighted
-// sum of a token's expert outputs (layouts in fp8b.cuh).
+// Expert routing and the weighted sum of a token's expert outputs (layouts in
+// fp8b.cuh; the hidden activation is formed in the product, fp8b_gemm.cu).
 #include "fp8b.cuh"
 #include "kernels.cuh"
 #include "mxfp8.cuh"
