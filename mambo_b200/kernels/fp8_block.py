@@ -153,14 +153,15 @@ def _linear_workspace_bytes(rows: int, experts: int, n: int, k: int) -> int:
     return _lib.load().mambo_fp8b_linear_workspace_bytes(rows, experts, n, k)
 
 
-def _output(out, rows: int, n: int, out_dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+def _output(out, rows: int, n: int, out_dtype: torch.dtype, device: torch.device) -> tuple[torch.Tensor, int]:
+    """The output [rows, n], the given one or a new one, and its row stride."""
     if out is None:
         _out_code(out_dtype)
-        return torch.empty((rows, n), dtype=out_dtype, device=device)
+        return torch.empty((rows, n), dtype=out_dtype, device=device), n
     if tuple(out.shape) != (rows, n) or out.dtype not in _DTYPES or (n > 1 and out.stride(1) != 1) \
             or out.device != device:
         raise ValueError("out must be float32 or bfloat16 [M,N] with unit column stride on the activation's device")
-    return out
+    return out, _row_stride(out)
 
 
 def _check_weight(weight: Fp8BlockFields, device: torch.device, grouped: bool) -> None:
@@ -198,40 +199,46 @@ def launch_fp8_block_matmul(x_values, x_scales, weight: Fp8BlockFields, *, strea
         x_values = x_values.contiguous()
     if x_scales.stride(1) != 1:
         x_scales = x_scales.contiguous()
-    out = _output(out, m, weight["n_rows"], out_dtype, dev)
+    out, ldo = _output(out, m, weight["n_rows"], out_dtype, dev)
     if m:
         with _device_guard(dev):
             with _runtime.workspace(dev, None, _linear_workspace_bytes(m, 1, weight["n_rows"], k)) as ws:
                 _lib.check(_lib.load().mambo_fp8b_linear(
                     x_values.data_ptr(), _row_stride(x_values), x_scales.data_ptr(), _row_stride(x_scales), group, m,
-                    weight["weight"], out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), ws.ptr, ws.size, ws.stream),
+                    weight["weight"], out.data_ptr(), _DTYPES[out.dtype], ldo, ws.ptr, ws.size, ws.stream),
                     "launch_fp8_block_matmul")
     return out
 
 
-def _activation(x, weight: Fp8BlockFields, act_group: int, grouped: bool) -> torch.Tensor:
+def _activation(x, weight: Fp8BlockFields, act_group: int, grouped: bool) -> tuple[torch.Tensor, torch.device, int, int]:
+    """x [M,K] with unit column stride, its device, M and row stride."""
     x = _runtime.as_cuda_tensor(x)
+    dev = x.device
     _check_group(act_group)
-    _check_weight(weight, x.device, grouped)
+    _check_weight(weight, dev, grouped)
     if x.ndim != 2 or x.dtype not in _DTYPES or x.shape[1] != weight["k"]:
         raise ValueError("activation must be float32 or bfloat16 [M,K] with the weight's K")
-    _runtime.require_device(x.device)
-    return x if x.stride(1) == 1 else x.contiguous()
+    _runtime.require_device(dev)
+    m, (ldx, unit) = x.shape[0], x.stride()
+    if unit != 1:
+        x = x.contiguous()
+        ldx = weight["k"]
+    return x, dev, m, ldx if m > 1 else weight["k"]
 
 
 @_runtime.with_stream
 def fp8_block_linear(x, weight: Fp8BlockFields, *, act_group: int = BLOCK, stream=None,
                      out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """bf16/f32 activations [M,K] -> E4M3 with one scale per ``act_group`` values -> the linear, one C-ABI call."""
-    x = _activation(x, weight, act_group, False)
-    dev, m, n = x.device, x.shape[0], weight["n_rows"]
-    out = _output(out, m, n, out_dtype, dev)
+    x, dev, m, ldx = _activation(x, weight, act_group, False)
+    n = weight["n_rows"]
+    out, ldo = _output(out, m, n, out_dtype, dev)
     if m:
         with _device_guard(dev):
             with _runtime.workspace(dev, None, _linear_workspace_bytes(m, 1, n, weight["k"])) as ws:
                 _lib.check(_lib.load().mambo_fp8b_linear_fused(
-                    x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), act_group, m, weight["weight"], out.data_ptr(),
-                    _DTYPES[out.dtype], _row_stride(out), ws.ptr, ws.size, ws.stream), "fp8_block_linear")
+                    x.data_ptr(), _DTYPES[x.dtype], ldx, act_group, m, weight["weight"], out.data_ptr(), _DTYPES[out.dtype],
+                    ldo, ws.ptr, ws.size, ws.stream), "fp8_block_linear")
     return out
 
 
@@ -244,19 +251,19 @@ def fp8_block_grouped_linear(x, offsets, weight: Fp8BlockFields, *, act_group: i
     non-decreasing up to R; it is not read on the host. Segments may be empty;
     output rows that no segment covers are not written.
     """
-    x = _activation(x, weight, act_group, True)
+    x, dev, rows, ldx = _activation(x, weight, act_group, True)
     offsets = _runtime.as_cuda_tensor(offsets)
-    dev, rows, n, experts = x.device, x.shape[0], weight["n_rows"], weight["n_experts"]
+    n, experts = weight["n_rows"], weight["n_experts"]
     if offsets.dtype != torch.int32 or tuple(offsets.shape) != (experts + 1,) or offsets.device != dev:
         raise ValueError("offsets must be int32 [E+1] on the activation's device")
     if offsets.stride(0) != 1:
         offsets = offsets.contiguous()
-    out = _output(out, rows, n, out_dtype, dev)
+    out, ldo = _output(out, rows, n, out_dtype, dev)
     if rows:
         with _device_guard(dev):
             with _runtime.workspace(dev, None, _linear_workspace_bytes(rows, experts, n, weight["k"])) as ws:
                 _lib.check(_lib.load().mambo_fp8b_grouped_linear(
-                    x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), act_group, rows, offsets.data_ptr(), weight["weight"],
-                    out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), ws.ptr, ws.size, ws.stream),
+                    x.data_ptr(), _DTYPES[x.dtype], ldx, act_group, rows, offsets.data_ptr(), weight["weight"],
+                    out.data_ptr(), _DTYPES[out.dtype], ldo, ws.ptr, ws.size, ws.stream),
                     "fp8_block_grouped_linear")
     return out

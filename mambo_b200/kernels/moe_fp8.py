@@ -88,7 +88,8 @@ def launch_moe_route(logits, top_k: int, *, scoring: str = "softmax", bias=None,
         with _device_guard(dev):
             with _runtime.workspace(dev, None, _route_workspace_bytes(tokens, experts)) as ws:
                 _lib.check(_lib.load().mambo_moe_route(
-                    logits.data_ptr(), _DTYPES[logits.dtype], _row_stride(logits), 0 if bias is None else bias.data_ptr(),
+                    logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0) if tokens > 1 else experts,
+                    0 if bias is None else bias.data_ptr(),
                     tokens, experts, top_k, _SCORING[scoring], int(renormalize), scale, ids.data_ptr(),
                     weights.data_ptr(), offsets.data_ptr(), positions.data_ptr(), rows.data_ptr(), ws.ptr,
                     ws.size, ws.stream), "launch_moe_route")
@@ -132,7 +133,7 @@ def launch_moe_combine(y, route: MoeRoute, *, stream=None, out_dtype: torch.dtyp
     if y.stride(1) != 1:
         y = y.contiguous()
     rows, h = y.shape
-    out = _output(out, tokens, h, out_dtype, dev)
+    out, ldo = _output(out, tokens, h, out_dtype, dev)
     if tokens and not rows:
         out.zero_()
     elif tokens:
@@ -140,7 +141,7 @@ def launch_moe_combine(y, route: MoeRoute, *, stream=None, out_dtype: torch.dtyp
             st = _stream(dev)
             _lib.check(_lib.load().mambo_moe_combine(
                 y.data_ptr(), _DTYPES[y.dtype], _row_stride(y), rows, route["positions"].data_ptr(),
-                route["weights"].data_ptr(), tokens, top, h, out.data_ptr(), _DTYPES[out.dtype], _row_stride(out), st),
+                route["weights"].data_ptr(), tokens, top, h, out.data_ptr(), _DTYPES[out.dtype], ldo, st),
                 "launch_moe_combine")
     return out
 
@@ -178,14 +179,14 @@ def fp8_moe_experts(x, route: MoeRoute, gate_up: Fp8BlockFields, down: Fp8BlockF
     _runtime.require_device(dev)
     if x.stride(1) != 1:
         x = x.contiguous()
-    out = _output(out, tokens, h, out_dtype, dev)
+    out, ldo = _output(out, tokens, h, out_dtype, dev)
     if tokens:
         code = _DTYPES[out.dtype]
         with _device_guard(dev):
             with _runtime.workspace(dev, None, _experts_workspace_bytes(tokens, top, experts, h, i, code)) as ws:
                 _lib.check(_lib.load().mambo_moe_experts(
-                    x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), tokens, route["ids"].data_ptr(),
+                    x.data_ptr(), _DTYPES[x.dtype], x.stride(0) if tokens > 1 else h, tokens, route["ids"].data_ptr(),
                     route["weights"].data_ptr(), route["positions"].data_ptr(), route["offsets"].data_ptr(),
                     route["rows"].data_ptr(), top, gate_up["weight"], down["weight"], out.data_ptr(), code,
-                    _row_stride(out), ws.ptr, ws.size, ws.stream), "fp8_moe_experts")
+                    ldo, ws.ptr, ws.size, ws.stream), "fp8_moe_experts")
     return out
