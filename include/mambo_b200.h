@@ -535,7 +535,8 @@ MAMBO_API int mambo_default_config(int64_t m, int64_t n_rows, int64_t n_blocks, 
  * have no waits). Every wait of the pipelined kernels is bounded: when one
  * gives up it records MAMBO_ETIMEOUT with a site id and returns instead of
  * hanging. mambo_device_status reads (and with reset != 0 clears) that record;
- * it synchronizes with the device.
+ * it synchronizes with the device. A call that gave up may leave counters in
+ * its workspace that are not zero: zero-fill the workspace before its next use.
  */
 MAMBO_API int mambo_device_status(int reset, int* code, int* where, int* block);
 /* Wall-clock limit of one bounded device wait (default 1 s). */

@@ -362,6 +362,15 @@ def check(status: int, what: str = "") -> None:
 
 
 def device_status(reset: bool = False) -> tuple[int, int, int]:
+    """(code, site, block) of the first wait that gave up on the current device, (0, 0, 0) if none did.
+
+    ``reset`` clears the record, and after a failure the device's workspaces too:
+    a call that gave up may have left counters there that are not zero.
+    """
     code, where, block = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
     check(load().mambo_device_status(1 if reset else 0, ctypes.byref(code), ctypes.byref(where), ctypes.byref(block)))
+    if reset and code.value != MAMBO_OK:
+        from . import _runtime
+
+        _runtime.zero_workspaces()
     return code.value, where.value, block.value

@@ -190,3 +190,17 @@ def workspace(device: torch.device, stream: int | None, nbytes: int) -> _Workspa
         ws.lock.release()
         raise
     return ws
+
+
+def zero_workspaces() -> None:
+    """Zero-fill the current device's workspaces, those that only CUDA graphs use among them; nothing may be running there."""
+    index = torch.cuda.current_device()
+    for (device, _), ws in list(_workspaces.items()):
+        if device == index:
+            with ws.lock:
+                if ws.buffer is not None:
+                    ws.buffer.zero_()
+    for buffer in _kept:
+        if buffer.device.index in (index, None):
+            buffer.zero_()
+    torch.cuda.synchronize(index)

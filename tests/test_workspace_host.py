@@ -170,3 +170,31 @@ def test_a_failed_call_gives_the_workspace_back(device):
     t.start()
     t.join(timeout=10)
     assert done
+
+
+def test_a_reset_after_a_failure_zeroes_the_workspaces(device, monkeypatch):
+    """Counters that a call left behind when it gave up would keep later calls from summing their parts."""
+    class Status:
+        code = 0
+
+        def mambo_device_status(self, reset, code, where, block):
+            code._obj.value = self.code
+            return _lib.MAMBO_OK
+
+    lib = Status()
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    first, size = handed_out(7, 1)
+    device.capturing = True
+    handed_out(7, 1)
+    device.capturing = False
+    handed_out(7, size + 1)  # the first one stays with the graph
+    buffers = [first(), _runtime.workspace(DEV, 9, 1), _runtime.workspace(DEV, 7, 1)]
+    for b in buffers[1:]:
+        b.lock.release()
+    buffers = [buffers[0], buffers[1].buffer, buffers[2].buffer]
+    for code, reset, left in ((_lib.MAMBO_ETIMEOUT, True, 0), (_lib.MAMBO_ETIMEOUT, False, 1), (0, True, 1)):
+        for b in buffers:
+            b.fill_(1)
+        lib.code = code
+        assert _lib.device_status(reset=reset)[0] == code
+        assert all(bool((b == left).all()) for b in buffers)
