@@ -11,11 +11,11 @@
 // into other D buffers.
 //
 // Two forms. Tiles of 128 rows x 16, 32 or 64 tokens on single CTAs stream the
-// weights: 28672 x 8192 at 8 tokens 40-42 us, 0.86-0.90 of the measured HBM
-// bandwidth (38 repeated on one input). Tiles of 256 rows x 192 tokens on CTA
-// pairs carry prompts: 8192 x 28672 at 4096 tokens takes 910-945 us with its
-// quantizer in short bursts (2.0-2.1 PFLOP/s) and 1060-1180 in long runs
-// (1.6-1.8), where the power limit holds the SMs near 1.5 GHz.
+// weights: 28672 x 8192 at 8 tokens 40.4-41.4 us, 0.87-0.89 of the measured
+// HBM bandwidth (38 repeated on one input). Tiles of 256 rows x 192 tokens on
+// CTA pairs carry prompts: 8192 x 28672 at 4096 tokens takes 910-945 us with
+// its quantizer in short bursts (2.0-2.1 PFLOP/s) and 1046-1103 in long runs
+// (1.7-1.8), where the power limit holds the SMs near 1.5 GHz.
 // 14336 x 4096 at 2048 tokens: 120 us, the tensor pipe active
 // 60 % of the time. What paces them is the way of a D buffer through the
 // epilogue and back, and power.
