@@ -5,7 +5,6 @@ PyTorch provides device memory and streams; the compute is in libmambo_b200.
 
 from __future__ import annotations
 
-import dataclasses
 import functools
 import threading
 
@@ -47,19 +46,42 @@ def stream_handle(stream, device: torch.device) -> int:
     raise TypeError(f"unsupported stream object {type(stream).__name__}")
 
 
-def _tensors(obj):
-    """The tensors of an argument or a result: one, or a list, tuple, dict or dataclass of them."""
-    if isinstance(obj, torch.Tensor):
-        yield obj
-    elif isinstance(obj, (list, tuple)):
-        for v in obj:
-            yield from _tensors(v)
-    elif isinstance(obj, dict):
-        for v in obj.values():
-            yield from _tensors(v)
-    elif dataclasses.is_dataclass(obj) and not isinstance(obj, type):
-        for f in dataclasses.fields(obj):
-            yield from _tensors(getattr(obj, f.name))
+def _parts(obj):
+    """What a container of tensors holds: a list, tuple, dict or dataclass (prepared weights, routes)."""
+    if isinstance(obj, (list, tuple)):
+        return obj
+    if isinstance(obj, dict):
+        return obj.values()
+    if hasattr(obj, "__dataclass_fields__"):
+        return [getattr(obj, name) for name in obj.__dataclass_fields__]
+    return ()
+
+
+def _device_of(parts) -> torch.device | None:
+    for v in parts:
+        if isinstance(v, torch.Tensor):
+            if v.is_cuda:
+                return v.device
+        elif (device := _device_of(_parts(v))) is not None:
+            return device
+    return None
+
+
+def _record_use(parts, stream: torch.cuda.Stream) -> None:
+    """The allocator keeps the tensors' memory until what is queued on ``stream`` now is done."""
+    for v in parts:
+        if isinstance(v, torch.Tensor):
+            if v.is_cuda:
+                v.record_stream(stream)
+        elif v is not None and not isinstance(v, (int, str)):
+            _record_use(_parts(v), stream)
+
+
+@functools.lru_cache(maxsize=256)
+def _external_stream(handle: int, device: torch.device) -> torch.cuda.Stream:
+    if handle in (0, 1):  # the legacy default stream by either of its names
+        return torch.cuda.default_stream(device)
+    return torch.cuda.ExternalStream(handle, device=device)
 
 
 def with_stream(operator):
@@ -67,30 +89,31 @@ def with_stream(operator):
 
     So what it allocates, copies (rows without unit stride) and fills belongs to
     the stream that its kernels run on. The caller orders that stream with the
-    work that made the arguments, and his own with the results. Memory may be
-    let go of at any time: arguments are not used again before the stream is
-    done with them, nor results before the caller's current stream is.
+    work that made the arguments, and his own with the results. Either may be
+    dropped at any time: memory is not used again before both streams are done
+    with it.
     """
 
     @functools.wraps(operator)
     def call(*args, stream=None, **kwargs):
         if stream is None:
             return operator(*args, **kwargs)
-        given = list(_tensors((args, kwargs)))
-        device = next((t.device for t in given if t.is_cuda), None)
-        if device is None:
-            device = torch.device("cuda", torch.cuda.current_device())
-        caller, handle = torch.cuda.current_stream(device), stream_handle(stream, device)
-        if handle == caller.cuda_stream:
+        device = _device_of(args) or _device_of(kwargs.values()) or torch.device("cuda", torch.cuda.current_device())
+        handle, here = stream_handle(stream, device), torch._C._cuda_getCurrentRawStream(device.index)
+        if handle == here or (handle == 1 and here == 0):
             return operator(*args, **kwargs)
-        target = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(handle, device=device)
-        with torch.cuda.stream(target):
+        target = stream if isinstance(stream, torch.cuda.Stream) else _external_stream(handle, device)
+        current_device, caller = torch.cuda.current_device(), torch.cuda.current_stream(device)
+        torch.cuda.set_stream(target)
+        try:
             result = operator(*args, **kwargs)
-        for t in given:
-            if t.is_cuda:
-                t.record_stream(target)
-        for t in _tensors(result):
-            t.record_stream(caller)
+        finally:
+            torch.cuda.set_stream(caller)
+            if current_device != device.index:
+                torch.cuda.set_device(current_device)
+        _record_use(args, target)
+        _record_use(kwargs.values(), target)
+        _record_use((result,), caller)
         return result
 
     return call
@@ -111,7 +134,7 @@ def require_device(device: torch.device) -> None:
 
 
 def _stream_is_capturing(device: torch.device, stream: int) -> bool:
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+    with torch.cuda.stream(_external_stream(stream, device)):
         return torch.cuda.is_current_stream_capturing()
 
 

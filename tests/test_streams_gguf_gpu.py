@@ -6,8 +6,8 @@ import numpy as np
 import pytest
 import torch
 
-from mambo_b200 import _lib
-from mambo_b200.kernels.iq3_s_fp8 import iq3_s_fp8_linear, iq3_s_fp8_linear_group
+from mambo_b200 import _lib, _runtime
+from mambo_b200.kernels.iq3_s_fp8 import fused_linear_into, iq3_s_fp8_linear, iq3_s_fp8_linear_group
 from mambo_b200.kernels.q4_k_fp8 import launch_quantize_fp8_sums, prepare_q4_k_fields, q4_k_fp8_linear
 from mambo_b200.kernels.quantize_fp8 import launch_quantize_fp8
 from mambo_b200.utils.iq3_s_weight import prepare_iq3_s_fields
@@ -93,3 +93,17 @@ def test_results_do_not_overwrite_memory_in_use(operators, name):
     torch.cuda.synchronize()
     assert all(bool((c == 3).all()) for c in copies)
     assert equal(out, ref)
+
+
+@pytest.mark.parametrize("handle", [0, 1, 2])
+def test_into_calls_with_the_default_streams_handles(cuda_device, handle, monkeypatch):
+    """The calls into given outputs take raw handles too, whose workspaces then come and grow."""
+    monkeypatch.setattr(_runtime, "_workspaces", {})
+    w = prepare_iq3_s_fields(torch.from_numpy(O.make_synthetic_iq3s(N, K, seed=3)).to(cuda_device))
+    for m in (2, 12, 600):
+        x = torch.randn(m, K, generator=torch.Generator().manual_seed(m)).bfloat16().to(cuda_device)
+        ref, out = iq3_s_fp8_linear(x, w), torch.zeros(m, N, dtype=torch.bfloat16, device=cuda_device)
+        torch.cuda.synchronize()
+        fused_linear_into(x, w, out, stream=handle)
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref)

@@ -178,3 +178,26 @@ def test_empty_results_on_another_stream(cuda_device):
     side.synchronize()
     with torch.cuda.stream(side):
         assert bool((empty["offsets"] == 0).all()) and bool((out == 0).all())
+
+
+@pytest.mark.parametrize("handle", [0, 1, 2])
+def test_the_default_streams_handles(operators, handle):
+    """The legacy default stream as 0 and 1, the per-thread one as 2, from the current stream and from another."""
+    x = make_x(M, K, 9).cuda()
+    ref = operators["linear"](x, None)
+    torch.cuda.synchronize()
+    out = operators["linear"](x, handle)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        other = operators["linear"](x, handle)
+        assert torch.cuda.current_stream() == side
+    torch.cuda.synchronize()
+    assert torch.equal(out, ref) and torch.equal(other, ref)
+
+
+def test_a_refused_call_leaves_the_current_stream(operators):
+    side = torch.cuda.Stream()
+    before = torch.cuda.current_stream()
+    with pytest.raises(ValueError):
+        operators["linear"](torch.zeros(3, K + 1, device="cuda"), side)
+    assert torch.cuda.current_stream() == before
