@@ -34,8 +34,8 @@ def as_cuda_tensor(obj) -> torch.Tensor:
 
 def stream_handle(stream, device: torch.device) -> int:
     """cudaStream_t of `stream` (None = torch's current stream on `device`)."""
-    if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
+    if stream is None:  # without building a torch.cuda.Stream, which takes 2 us
+        return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else torch.cuda.current_device())
     if isinstance(stream, torch.cuda.Stream):
         return stream.cuda_stream
     if isinstance(stream, int):

@@ -55,11 +55,6 @@ class _NoGuard:
 _NO_GUARD = _NoGuard()
 
 
-def _stream(device: torch.device) -> int:
-    """The current stream's handle, without building a torch.cuda.Stream (2 us of a call's 17)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
 _DTYPES = {torch.float32: _lib.MAMBO_F32, torch.bfloat16: _lib.MAMBO_BF16}
 
 
@@ -111,7 +106,7 @@ def prepare_fp8_block_fields(values, scales, *, gate_up: bool = False, stream=No
     out_scales = torch.empty(lib.mambo_fp8b_scales_bytes(experts, n, k, int(gate_up)) // 4, dtype=torch.float32,
                              device=dev)
     with _device_guard(dev):
-        st = _stream(dev)
+        st = _runtime.stream_handle(None, dev)
         _lib.check(lib.mambo_fp8b_pack(
             values.data_ptr(), experts, n, k, values.stride(0), values.stride(1), values.stride(2), scales.data_ptr(),
             scales.stride(0), scales.stride(1), scales.stride(2), int(gate_up), packed.data_ptr(),
@@ -136,7 +131,7 @@ def launch_quantize_fp8_block(x, *, group: int = BLOCK, stream=None) -> tuple[to
     scales = torch.empty((m, -(-k // group)), dtype=torch.uint8, device=x.device)
     if m:
         with _device_guard(x.device):
-            st = _stream(x.device)
+            st = _runtime.stream_handle(None, x.device)
             _lib.check(_lib.load().mambo_fp8b_quantize(
                 x.data_ptr(), _DTYPES[x.dtype], m, k, _row_stride(x), group, values.data_ptr(), k, scales.data_ptr(),
                 scales.shape[1], st), "launch_quantize_fp8_block")

@@ -21,7 +21,7 @@ from typing import TypedDict
 import torch
 
 from .. import _lib, _runtime
-from .fp8_block import _DTYPES, Fp8BlockFields, _device_guard, _output, _row_stride, _stream
+from .fp8_block import _DTYPES, Fp8BlockFields, _device_guard, _output, _row_stride
 
 _SCORING = {"softmax": _lib.MAMBO_MOE_SOFTMAX, "sigmoid": _lib.MAMBO_MOE_SIGMOID}
 
@@ -138,7 +138,7 @@ def launch_moe_combine(y, route: MoeRoute, *, stream=None, out_dtype: torch.dtyp
         out.zero_()
     elif tokens:
         with _device_guard(dev):
-            st = _stream(dev)
+            st = _runtime.stream_handle(None, dev)
             _lib.check(_lib.load().mambo_moe_combine(
                 y.data_ptr(), _DTYPES[y.dtype], _row_stride(y), rows, route["positions"].data_ptr(),
                 route["weights"].data_ptr(), tokens, top, h, out.data_ptr(), _DTYPES[out.dtype], ldo, st),
