@@ -582,6 +582,91 @@ MAMBO_API int mambo_iq3s_linear_fused_ar(const void* x, int x_dtype, int64_t ldx
                                          MamboArComm* comm, const MamboLinearConfig* cfg, void* workspace,
                                          size_t workspace_bytes, mambo_stream_t stream);
 
+/*
+ * Rotary positions (no counterpart in the reference). Pair p of the first
+ * rotary_dim dimensions of a head, (a, b) at 2p, 2p + 1 (interleaved) or p,
+ * p + rotary_dim / 2, becomes
+ *   magnitude * (a cos t - b sin t, a sin t + b cos t), t = position * turns[p] / 2^64 turns;
+ * the other dimensions are copied. turns[p] is the frequency as a 64-bit
+ * fraction of a turn per position, so that no position is too far. x and out
+ * [tokens, heads, dim], f32 or bf16 with unit stride along dim; out may be x.
+ * inverse turns back (the transposed rotation with the same magnitude, which
+ * is also the gradient). positions: int32 or int64 in device memory.
+ */
+typedef struct MamboRotary {
+  const uint64_t* turns; /* device, [rotary_dim / 2] */
+  int rotary_dim;
+  int interleaved;
+  float magnitude;
+} MamboRotary;
+MAMBO_API int mambo_rotary(const void* x, int dtype, int64_t tokens, int64_t heads, int64_t dim, int64_t stride_token,
+                           int64_t stride_head, const void* positions, int positions_64, const MamboRotary* rotary,
+                           int inverse, void* out, int64_t out_stride_token, int64_t out_stride_head,
+                           mambo_stream_t stream);
+
+/*
+ * A paged key/value cache in FP8 (no counterpart in the reference): E4M3 codes
+ * [pages, kv_heads, page_tokens, head_dim] and one UE8M0 scale per page and
+ * head, for keys and for values, all contiguous, the codes 16-byte aligned.
+ * page_tokens is 16, 32, 64 or 128; head_dim a multiple of 16 up to 128. Scale
+ * exponents are -64 .. 127 (codes 63 .. 254); 255 marks a page of a head in
+ * which a value was NaN or infinite.
+ *
+ * A call's sequences: sequence b's tokens lie in the pages that row b of
+ * page_table names (int32; an entry outside the cache has no tokens), and
+ * tokens offsets[b] .. offsets[b + 1] of the call are its own (offsets null:
+ * token b). Everything is in device memory and clamped to the buffers;
+ * nothing is read back to the host.
+ */
+typedef struct MamboKvCache {
+  uint8_t* keys;
+  uint8_t* values;
+  uint8_t* key_scales;
+  uint8_t* value_scales;
+  int64_t pages;
+  int kv_heads;
+  int page_tokens;
+  int head_dim;
+} MamboKvCache;
+typedef struct MamboKvSequences {
+  const int32_t* page_table; /* [batch, table_pages], row stride table_stride */
+  int64_t table_stride;
+  int64_t table_pages;
+  const int32_t* lengths;    /* [batch] tokens in the cache: before an append, with the call's own for attention */
+  const int32_t* offsets;    /* [batch + 1], or null */
+  int64_t batch;
+} MamboKvSequences;
+
+/*
+ * Keys and values [tokens, kv_heads, head_dim] (f32 or bf16, unit stride along
+ * head_dim) to the positions lengths[b] on of their sequences, keys turned by
+ * their positions on the way (rotary null: not). A page's scale is the
+ * smallest power of two that holds its new values, or the one that it has if
+ * that is larger and the page was begun before; where it grows, the page's
+ * older codes are rounded anew. Tokens behind the table's last page are
+ * dropped. A page that is appended to belongs to one sequence.
+ */
+MAMBO_API int mambo_kv_append(const MamboKvCache* cache, const void* k, int64_t k_stride_token, int64_t k_stride_head,
+                              const void* v, int64_t v_stride_token, int64_t v_stride_head, int dtype, int64_t tokens,
+                              const MamboKvSequences* seq, const MamboRotary* rotary, mambo_stream_t stream);
+
+/*
+ * Causal attention of bf16 queries [tokens, heads, head_dim] over the cache;
+ * query head h reads key head h / (heads / kv_heads). A sequence's n queries
+ * stand at its last n positions; a query sees the positions up to its own, the
+ * last `window` of them where window is not 0:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j   (bf16),   lse = log sum_j exp(scale * q . k_j)   (f32, may be null).
+ * A query that sees nothing has zeros and an lse of minus infinity; rows that
+ * no sequence covers are not written. workspace: zero-filled once, shared with
+ * the other calls of the stream.
+ */
+MAMBO_API size_t mambo_kv_attention_workspace_bytes(int64_t tokens, int64_t heads, const MamboKvCache* cache);
+MAMBO_API int mambo_kv_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, int64_t tokens,
+                                 int64_t heads, const MamboKvCache* cache, const MamboKvSequences* seq, int64_t window,
+                                 float scale, void* out, int64_t out_stride_token, int64_t out_stride_head, float* lse,
+                                 int64_t lse_stride_token, int64_t lse_stride_head, void* workspace,
+                                 size_t workspace_bytes, mambo_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

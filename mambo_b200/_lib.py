@@ -88,6 +88,10 @@ EXPORTED_SYMBOLS = (
     "mambo_moe_combine",
     "mambo_moe_experts_workspace_bytes",
     "mambo_moe_experts",
+    "mambo_rotary",
+    "mambo_kv_append",
+    "mambo_kv_attention_workspace_bytes",
+    "mambo_kv_attention",
 )
 
 MAMBO_AR_HANDLE_BYTES = 64
@@ -162,6 +166,45 @@ class MamboFp8BlockWeight(ctypes.Structure):
         ("k", ctypes.c_int64),
         ("n_experts", ctypes.c_int64),
         ("gate_up", ctypes.c_int),
+    ]
+
+
+class MamboRotary(ctypes.Structure):
+    """Rotary frequencies: a 64-bit fraction of a turn per position for each pair."""
+
+    _fields_ = [
+        ("turns", ctypes.c_void_p),
+        ("rotary_dim", ctypes.c_int),
+        ("interleaved", ctypes.c_int),
+        ("magnitude", ctypes.c_float),
+    ]
+
+
+class MamboKvCache(ctypes.Structure):
+    """A paged FP8 key/value cache [pages, kv_heads, page_tokens, head_dim] and its scales [pages, kv_heads]."""
+
+    _fields_ = [
+        ("keys", ctypes.c_void_p),
+        ("values", ctypes.c_void_p),
+        ("key_scales", ctypes.c_void_p),
+        ("value_scales", ctypes.c_void_p),
+        ("pages", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int),
+        ("page_tokens", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+    ]
+
+
+class MamboKvSequences(ctypes.Structure):
+    """The sequences of an append or an attention call."""
+
+    _fields_ = [
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("table_pages", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p),
+        ("batch", ctypes.c_int64),
     ]
 
 
@@ -330,6 +373,19 @@ def load() -> ctypes.CDLL:
             "mambo_moe_experts": (
                 [vp, i32, i64, i64, vp, vp, vp, vp, vp, i32, ctypes.POINTER(MamboFp8BlockWeight),
                  ctypes.POINTER(MamboFp8BlockWeight), vp, i32, i64, vp, ctypes.c_size_t, vp],
+                i32,
+            ),
+            "mambo_rotary": (
+                [vp, i32, i64, i64, i64, i64, i64, vp, i32, ctypes.POINTER(MamboRotary), i32, vp, i64, i64, vp], i32),
+            "mambo_kv_append": (
+                [ctypes.POINTER(MamboKvCache), vp, i64, i64, vp, i64, i64, i32, i64, ctypes.POINTER(MamboKvSequences),
+                 ctypes.POINTER(MamboRotary), vp],
+                i32,
+            ),
+            "mambo_kv_attention_workspace_bytes": ([i64, i64, ctypes.POINTER(MamboKvCache)], ctypes.c_size_t),
+            "mambo_kv_attention": (
+                [vp, i64, i64, i64, i64, ctypes.POINTER(MamboKvCache), ctypes.POINTER(MamboKvSequences), i64,
+                 ctypes.c_float, vp, i64, i64, vp, i64, i64, vp, ctypes.c_size_t, vp],
                 i32,
             ),
         }

@@ -1,0 +1,187 @@
+// C ABI of rotary positions, the append to the paged FP8 key/value cache and
+// attention over it (declared in include/mambo_b200.h).
+#include "kernels.cuh"
+#include "kv.cuh"
+
+using namespace mambo;
+
+namespace {
+
+constexpr int64_t kMaxTokens = (int64_t)1 << 24, kMaxHeads = 1024, kMaxBatch = 1 << 16, kMaxPages = (int64_t)1 << 31;
+
+bool dtype_ok(int d) { return d == MAMBO_F32 || d == MAMBO_BF16; }
+bool aligned(const void* p, int bytes) { return (uintptr_t)p % bytes == 0; }
+constexpr const char* kUnaligned = "a pointer is not aligned to its elements";
+
+int check_rotary(const MamboRotary* r, int64_t dim) {
+  if (!r->turns) return api_fail(MAMBO_EINVAL, "null pointer");
+  if (r->rotary_dim < 2 || r->rotary_dim % 2 || r->rotary_dim > dim)
+    return api_fail(MAMBO_EINVAL, "the rotated part must be an even number of dimensions of the head");
+  if (!aligned(r->turns, 8)) return api_fail(MAMBO_EINVAL, kUnaligned);
+  return MAMBO_OK;
+}
+
+RotaryParams rotary_params(const MamboRotary* r, int inverse) {
+  RotaryParams p{};
+  if (r) p = {r->turns, r->rotary_dim / 2, r->interleaved != 0, r->magnitude, inverse ? -1.f : 1.f};
+  return p;
+}
+
+int check_cache(const MamboKvCache* c) {
+  if (!c || !c->keys || !c->values || !c->key_scales || !c->value_scales) return api_fail(MAMBO_EINVAL, "null cache field");
+  if (c->page_tokens != 16 && c->page_tokens != 32 && c->page_tokens != 64 && c->page_tokens != 128)
+    return api_fail(MAMBO_EINVAL, "a page has 16, 32, 64 or 128 tokens");
+  if (c->head_dim < 16 || c->head_dim % 16 || c->head_dim > kKvMaxDim)
+    return api_fail(MAMBO_EINVAL, "the head size must be a multiple of 16, at most %d", kKvMaxDim);
+  if (c->kv_heads < 1 || c->kv_heads > kMaxHeads) return api_fail(MAMBO_EINVAL, "1 to %d heads", (int)kMaxHeads);
+  if (c->pages < 1 || c->pages * c->kv_heads > kMaxPages) return api_fail(MAMBO_EINVAL, "pages * heads must be in [1, 2^31]");
+  if (!aligned(c->keys, 16) || !aligned(c->values, 16)) return api_fail(MAMBO_EINVAL, "the cache must be 16-byte aligned");
+  return MAMBO_OK;
+}
+
+KvCache cache_params(const MamboKvCache* c) {
+  KvCache p{};
+  p.codes[0] = c->keys;
+  p.codes[1] = c->values;
+  p.scales[0] = c->key_scales;
+  p.scales[1] = c->value_scales;
+  p.pages = c->pages;
+  p.heads = c->kv_heads;
+  p.page = c->page_tokens;
+  p.dim = c->head_dim;
+  p.log_page = c->page_tokens == 16 ? 4 : c->page_tokens == 32 ? 5 : c->page_tokens == 64 ? 6 : 7;
+  return p;
+}
+
+int check_sequences(const MamboKvSequences* s, int64_t tokens) {
+  if (!s || !s->page_table || !s->lengths) return api_fail(MAMBO_EINVAL, "null pointer");
+  if (s->batch < 1 || s->batch > kMaxBatch) return api_fail(MAMBO_EINVAL, "1 to 2^16 sequences");
+  if (s->table_pages < 1 || s->table_pages > (1 << 24)) return api_fail(MAMBO_EINVAL, "the page table has 1 to 2^24 columns");
+  if (s->table_stride < s->table_pages && s->batch > 1) return api_fail(MAMBO_EINVAL, "page table row stride smaller than the row");
+  if (tokens < 1 || tokens > kMaxTokens) return api_fail(MAMBO_EINVAL, "1 to 2^24 tokens");
+  if (!s->offsets && tokens != s->batch) return api_fail(MAMBO_EINVAL, "without offsets a sequence has one token");
+  if (!aligned(s->page_table, 4) || !aligned(s->lengths, 4) || !aligned(s->offsets, 4)) return api_fail(MAMBO_EINVAL, kUnaligned);
+  return MAMBO_OK;
+}
+
+KvSequences sequence_params(const MamboKvSequences* s, int64_t tokens) {
+  return {s->page_table, s->table_stride, (int)s->table_pages, s->lengths, s->offsets, (int)s->batch, (int)tokens};
+}
+
+}  // namespace
+
+extern "C" {
+
+int mambo_rotary(const void* x, int dtype, int64_t tokens, int64_t heads, int64_t dim, int64_t stride_token,
+                 int64_t stride_head, const void* positions, int positions_64, const MamboRotary* rotary, int inverse,
+                 void* out, int64_t out_stride_token, int64_t out_stride_head, mambo_stream_t stream) {
+  if (!x || !out || !positions || !rotary) return api_fail(MAMBO_EINVAL, "null pointer");
+  if (!dtype_ok(dtype)) return api_fail(MAMBO_EINVAL, "x must be f32 or bf16");
+  if (tokens < 1 || tokens > kMaxTokens || heads < 1 || heads > kMaxHeads || dim < 2 || dim > 65536)
+    return api_fail(MAMBO_EINVAL, "x must be [1..2^24 tokens, 1..1024 heads, 2..65536]");
+  const int es = dtype == MAMBO_BF16 ? 2 : 4;
+  if (!aligned(x, es) || !aligned(out, es) || !aligned(positions, positions_64 ? 8 : 4)) return api_fail(MAMBO_EINVAL, kUnaligned);
+  int st = check_rotary(rotary, dim);
+  if (st != MAMBO_OK) return st;
+  if ((double)tokens * (double)heads * (double)(dim / 16 + 2) >= 2147483647.0 * 128)
+    return api_fail(MAMBO_EINVAL, "the call is too large: split its tokens");
+  int sms, smem;
+  st = api_require_sm100(&sms, &smem);
+  if (st != MAMBO_OK) return st;
+  RotaryCall p{};
+  p.rot = rotary_params(rotary, inverse);
+  p.x = x;
+  p.out = out;
+  p.bf16 = dtype == MAMBO_BF16;
+  p.tokens = (int)tokens;
+  p.heads = (int)heads;
+  p.dim = (int)dim;
+  p.xs_t = stride_token;
+  p.xs_h = stride_head;
+  p.os_t = out_stride_token;
+  p.os_h = out_stride_head;
+  p.positions = positions;
+  p.positions64 = positions_64 != 0;
+  const cudaError_t e = launch_rotary(p, (cudaStream_t)stream);
+  if (e != cudaSuccess) return api_cuda_fail(e, "rotary positions");
+  return api_ok();
+}
+
+int mambo_kv_append(const MamboKvCache* cache, const void* k, int64_t k_stride_token, int64_t k_stride_head, const void* v,
+                    int64_t v_stride_token, int64_t v_stride_head, int dtype, int64_t tokens, const MamboKvSequences* seq,
+                    const MamboRotary* rotary, mambo_stream_t stream) {
+  int st = check_cache(cache);
+  if (st == MAMBO_OK) st = check_sequences(seq, tokens);
+  if (st != MAMBO_OK) return st;
+  if (!k || !v) return api_fail(MAMBO_EINVAL, "null pointer");
+  if (!dtype_ok(dtype)) return api_fail(MAMBO_EINVAL, "k and v must be f32 or bf16");
+  if (rotary) st = check_rotary(rotary, cache->head_dim);
+  if (st != MAMBO_OK) return st;
+  const int es = dtype == MAMBO_BF16 ? 2 : 4;
+  if (!aligned(k, es) || !aligned(v, es)) return api_fail(MAMBO_EINVAL, kUnaligned);
+  int sms, smem;
+  st = api_require_sm100(&sms, &smem);
+  if (st != MAMBO_OK) return st;
+  KvAppendCall p{};
+  p.rot = rotary_params(rotary, 0);
+  p.cache = cache_params(cache);
+  p.seq = sequence_params(seq, tokens);
+  p.x[0] = k;
+  p.x[1] = v;
+  p.xs_t[0] = k_stride_token;
+  p.xs_t[1] = v_stride_token;
+  p.xs_h[0] = k_stride_head;
+  p.xs_h[1] = v_stride_head;
+  p.bf16 = dtype == MAMBO_BF16;
+  const cudaError_t e = launch_kv_append(p, (cudaStream_t)stream);
+  if (e != cudaSuccess) return api_cuda_fail(e, "key/value append");
+  return api_ok();
+}
+
+size_t mambo_kv_attention_workspace_bytes(int64_t tokens, int64_t heads, const MamboKvCache* cache) {
+  if (!cache || tokens < 1 || tokens > kMaxTokens || cache->kv_heads < 1 || heads < 1 || heads > kMaxHeads ||
+      heads % cache->kv_heads)
+    return 0;
+  return kWorkspaceCounterBytes;
+}
+
+int mambo_kv_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, int64_t tokens, int64_t heads,
+                       const MamboKvCache* cache, const MamboKvSequences* seq, int64_t window, float scale, void* out,
+                       int64_t out_stride_token, int64_t out_stride_head, float* lse, int64_t lse_stride_token,
+                       int64_t lse_stride_head, void* workspace, size_t workspace_bytes, mambo_stream_t stream) {
+  int st = check_cache(cache);
+  if (st == MAMBO_OK) st = check_sequences(seq, tokens);
+  if (st != MAMBO_OK) return st;
+  if (!q || !out) return api_fail(MAMBO_EINVAL, "null pointer");
+  if (heads < 1 || heads > kMaxHeads || heads % cache->kv_heads)
+    return api_fail(MAMBO_EINVAL, "query heads must be a multiple of the cache's heads, at most %d", (int)kMaxHeads);
+  if (window < 0) return api_fail(MAMBO_EINVAL, "the window must not be negative");
+  if (!aligned(q, 2) || !aligned(out, 2) || !aligned(lse, 4)) return api_fail(MAMBO_EINVAL, kUnaligned);
+  const size_t need = mambo_kv_attention_workspace_bytes(tokens, heads, cache);
+  if (!workspace || workspace_bytes < need)
+    return api_fail(MAMBO_EWORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  if (!aligned(workspace, 256)) return api_fail(MAMBO_EINVAL, "workspace must be 256-byte aligned");
+  int sms, smem;
+  st = api_require_sm100(&sms, &smem);
+  if (st != MAMBO_OK) return st;
+  KvAttentionCall p{};
+  p.cache = cache_params(cache);
+  p.seq = sequence_params(seq, tokens);
+  p.q = (const uint16_t*)q;
+  p.qs_t = q_stride_token;
+  p.qs_h = q_stride_head;
+  p.out = (uint16_t*)out;
+  p.os_t = out_stride_token;
+  p.os_h = out_stride_head;
+  p.lse = lse;
+  p.ls_t = lse_stride_token;
+  p.ls_h = lse_stride_head;
+  p.group = (int)(heads / cache->kv_heads);
+  p.window = window <= 0x7FFFFFFF ? (int)window : 0;
+  p.scale = scale;
+  const cudaError_t e = launch_kv_attention_simple(p, (cudaStream_t)stream);
+  if (e != cudaSuccess) return api_cuda_fail(e, "attention");
+  return api_ok();
+}
+
+}  // extern "C"
