@@ -7,7 +7,8 @@ using namespace mambo;
 
 namespace {
 
-constexpr int64_t kMaxTokens = (int64_t)1 << 24, kMaxHeads = 1024, kMaxBatch = 1 << 16, kMaxPages = (int64_t)1 << 31;
+constexpr int kSmsBound = 160;  // workspace sizes do not depend on the device: an upper bound of its SMs
+constexpr int64_t kMaxTokens = (int64_t)1 << 24, kMaxHeads = 1024, kMaxBatch = 4096, kMaxPages = (int64_t)1 << 31;
 
 bool dtype_ok(int d) { return d == MAMBO_F32 || d == MAMBO_BF16; }
 bool aligned(const void* p, int bytes) { return (uintptr_t)p % bytes == 0; }
@@ -55,7 +56,7 @@ KvCache cache_params(const MamboKvCache* c) {
 
 int check_sequences(const MamboKvSequences* s, int64_t tokens) {
   if (!s || !s->page_table || !s->lengths) return api_fail(MAMBO_EINVAL, "null pointer");
-  if (s->batch < 1 || s->batch > kMaxBatch) return api_fail(MAMBO_EINVAL, "1 to 2^16 sequences");
+  if (s->batch < 1 || s->batch > kMaxBatch) return api_fail(MAMBO_EINVAL, "1 to 4096 sequences");
   if (s->table_pages < 1 || s->table_pages > (1 << 24)) return api_fail(MAMBO_EINVAL, "the page table has 1 to 2^24 columns");
   if (s->table_stride < s->table_pages && s->batch > 1) return api_fail(MAMBO_EINVAL, "page table row stride smaller than the row");
   if (tokens < 1 || tokens > kMaxTokens) return api_fail(MAMBO_EINVAL, "1 to 2^24 tokens");
@@ -142,7 +143,7 @@ size_t mambo_kv_attention_workspace_bytes(int64_t tokens, int64_t heads, const M
   if (!cache || tokens < 1 || tokens > kMaxTokens || cache->kv_heads < 1 || heads < 1 || heads > kMaxHeads ||
       heads % cache->kv_heads)
     return 0;
-  return kWorkspaceCounterBytes;
+  return kWorkspaceCounterBytes + kv_decode_partial_bytes((int)(heads / cache->kv_heads), kSmsBound);
 }
 
 int mambo_kv_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, int64_t tokens, int64_t heads,
@@ -157,6 +158,9 @@ int mambo_kv_attention(const void* q, int64_t q_stride_token, int64_t q_stride_h
     return api_fail(MAMBO_EINVAL, "query heads must be a multiple of the cache's heads, at most %d", (int)kMaxHeads);
   if (window < 0) return api_fail(MAMBO_EINVAL, "the window must not be negative");
   if (!aligned(q, 2) || !aligned(out, 2) || !aligned(lse, 4)) return api_fail(MAMBO_EINVAL, kUnaligned);
+  // Tiles of 128 positions, over all sequences and heads, are counted in 32 bits.
+  if ((double)seq->batch * cache->kv_heads * ((double)seq->table_pages * cache->page_tokens / 128 + 1) >= 2147483647.0)
+    return api_fail(MAMBO_EINVAL, "the call is too large: split its sequences");
   const size_t need = mambo_kv_attention_workspace_bytes(tokens, heads, cache);
   if (!workspace || workspace_bytes < need)
     return api_fail(MAMBO_EWORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
@@ -179,7 +183,16 @@ int mambo_kv_attention(const void* q, int64_t q_stride_token, int64_t q_stride_h
   p.group = (int)(heads / cache->kv_heads);
   p.window = window <= 0x7FFFFFFF ? (int)window : 0;
   p.scale = scale;
-  const cudaError_t e = launch_kv_attention_simple(p, (cudaStream_t)stream);
+  p.few = p.group <= 16 ? 16 : p.group <= 32 ? 32 : 0;
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i)
+    if (!kv_page_map(p.cache, i, &maps[i])) return api_fail(MAMBO_EINVAL, "the cache has no tensor map");
+  cudaError_t e = cudaSuccess;
+  if (p.few)
+    e = launch_kv_decode(p, maps[0], maps[1], sms < kSmsBound ? sms : kSmsBound, smem,
+                         (float*)((uint8_t*)workspace + kWorkspaceCounterBytes),
+                         (int*)((uint8_t*)workspace + kWorkspaceSplitCounterOffset), (cudaStream_t)stream);
+  if (e == cudaSuccess && (p.seq.offsets || !p.few)) e = launch_kv_attention_simple(p, (cudaStream_t)stream);
   if (e != cudaSuccess) return api_cuda_fail(e, "attention");
   return api_ok();
 }

@@ -39,6 +39,8 @@ enum WaitSite : int {
   kSiteArPeer = 10,  // a peer rank's partial never arrived (fused all-reduce)
   kSiteFbFull = 11,  // FP8 block product: operands or results
   kSiteFbEmpty = 12,
+  kSiteKvFull = 13,   // attention over the FP8 cache: operands or results
+  kSiteKvEmpty = 14,
 };
 
 __device__ __forceinline__ void record_timeout(int site) {

@@ -85,8 +85,13 @@ struct KvAttentionCall {
   int group;           // query heads of a key head
   int window;          // 0: none
   float scale;         // of the scores
+  int few;             // rows (tokens * group) of a sequence up to which the decode kernel has it; 0: it has none
 };
 cudaError_t launch_kv_attention_simple(const KvAttentionCall& p, cudaStream_t stream);
+bool kv_page_map(const KvCache& c, int which, CUtensorMap* map);
+size_t kv_decode_partial_bytes(int group, int sms);
+cudaError_t launch_kv_decode(const KvAttentionCall& p, const CUtensorMap& k, const CUtensorMap& v, int sms, int smem_optin,
+                             float* partials, int* counters, cudaStream_t stream);
 
 #ifdef __CUDACC__
 // The call's tokens of sequence b: [first, first + count), clamped to the call.

@@ -33,6 +33,7 @@ __global__ void __launch_bounds__(128) kv_attention_simple_kernel(const __grid_c
     }
     if (b == p.seq.batch) return;
   }
+  if (count * p.group <= p.few) return;
   const int64_t place = (int64_t)kv_length(p.seq, b, cache.page) - count + at;
   const int64_t first = p.window ? max(place - p.window + 1, (int64_t)0) : 0;
   const int kv = h / p.group, dim = cache.dim;
