@@ -50,9 +50,9 @@ struct Cfg {
   static constexpr uint32_t kQ = N * 128u;            // bytes of a term of the queries
   static constexpr uint32_t kW = 128u * N;            // of the weights: [N / 16][128 positions][16]
   static constexpr uint32_t kTmem = 128;              // O: N columns, S: two of N
-  static constexpr uint32_t kMeta = 2 * N * 8;        // two units' row factors and places
+  static constexpr uint32_t kMeta = 2 * N * 16;       // two units' row factors, places, tokens and heads
   static constexpr uint32_t kScales = 2 * 32 * 16;    // two batches of pages
-  static constexpr uint32_t kRed = (4 * N + 12) * 4;  // maxima or sums of the warps; the first tile's place, a flag
+  static constexpr uint32_t kRed = (4 * N + 16) * 4;  // maxima or sums of the warps; the first tile, a flag
   static constexpr int kNumBars = 3 * kMaxStages + 15;
   static constexpr uint32_t kFixed = 1024 + 4 * kQ + 2 * kW + kMeta + kScales + kRed + kNumBars * 8 + 16;
   static constexpr int kPart = N * 130;               // floats of a part: O [N][128], m, l
@@ -74,14 +74,9 @@ struct Walk {
     const int end = (int)((len + kKvTile - 1) / kKvTile);
     return end > start ? end - start : 1;  // one (of masked positions) where nothing is seen
   }
-  // local: tile x0 among those of sequence b's heads.
-  __device__ __forceinline__ Walk(const KvAttentionCall& call, int rows_, int x0, int end, int b0, int local)
-      : p(call), rows(rows_), x(x0), x1(end), b(b0), h(0), t(0), tiles(1), start(0), first(true) {
-    if (x >= x1) return;
-    tiles = tiles_of(p, rows, b, start);
-    h = local / tiles;
-    t = local - h * tiles;
-  }
+  // at: the first tile's sequence, head, tile, tiles and start.
+  __device__ __forceinline__ Walk(const KvAttentionCall& call, int rows_, int x0, int end, const int* at)
+      : p(call), rows(rows_), x(x0), x1(end), b(at[0]), h(at[1]), t(at[2]), tiles(at[3]), start(at[4]), first(true) {}
   __device__ __forceinline__ bool valid() const { return x < x1; }
   __device__ __forceinline__ bool last() const { return t == tiles - 1 || x == x1 - 1; }
   __device__ __forceinline__ void next() {
@@ -125,6 +120,27 @@ __device__ __forceinline__ void mma_values(uint32_t d, uint32_t v, uint32_t w0, 
       : "memory");
 }
 
+// The reduction of N columns over the warp, each lane with a value of each: every step halves the columns that a lane
+// goes on with, N - 1 + 32 / N shuffles in all. The result is that of column `column_of(lane)`.
+template <int N, typename Op>
+__device__ __forceinline__ float reduce_columns(float (&v)[N], int lane, Op op) {
+#pragma unroll
+  for (int w = N / 2, bit = 1; w >= 1; w >>= 1, bit <<= 1) {
+    const bool up = lane & bit;
+#pragma unroll
+    for (int i = 0; i < w; ++i) {
+      const float other = __shfl_xor_sync(0xFFFFFFFFu, up ? v[i] : v[i + w], bit);
+      v[i] = op(up ? v[i + w] : v[i], other);
+    }
+  }
+  if constexpr (N == 16) v[0] = op(v[0], __shfl_xor_sync(0xFFFFFFFFu, v[0], 16));
+  return v[0];
+}
+template <int N>
+__device__ __forceinline__ int column_of(int lane) {
+  return (int)(__brev((uint32_t)lane) >> (N == 16 ? 28 : 27));
+}
+
 }  // namespace
 
 template <int N>
@@ -138,10 +154,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
   uint8_t* ws = qs + 4 * C::kQ;                       // [hi, lo][N / 16][128][16]
   float* factors = reinterpret_cast<float*>(ws + 2 * C::kW);   // [2][N]
   int* places = reinterpret_cast<int*>(factors + 2 * N);       // [2][N]
-  float4* scales = reinterpret_cast<float4*>(places + 2 * N);  // [2][32]: key factor, value exponent, 2^-exponent, is there
+  int2* owners = reinterpret_cast<int2*>(places + 2 * N);      // [2][N]: the row's token and query head
+  float4* scales = reinterpret_cast<float4*>(owners + 2 * N);  // [2][32]: key factor, value exponent, 2^-exponent, is there
   float* red = reinterpret_cast<float*>(scales + 2 * 32);      // [4][N]
-  int* begin = reinterpret_cast<int*>(red + 4 * N);            // all tiles, the first one's sequence and place in it; a flag
-  int* warp_sums = begin + 4;                                  // [8]
+  int* begin = reinterpret_cast<int*>(red + 4 * N);            // the first tile: sequence, head, tile, tiles, start; a flag
+  int* warp_sums = begin + 8;                                  // [8]
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(red) + C::kRed);
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
   const uint32_t kFullK = smem_u32(bars), kFullV = kFullK + 8 * kMaxStages, kEmpty = kFullV + 8 * kMaxStages;
@@ -205,13 +222,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
   const int x0 = has ? (int)((int64_t)blockIdx.x * total / ctas) : 0;
   const int x1 = has ? (int)(((int64_t)blockIdx.x + 1) * total / ctas) : 0;
   if (x0 < x1 && x0 >= before && x0 < before + sum) {
-    int b = mine0;
-    for (int n; x0 >= before + (n = Walk::tiles_of(p, N, b, unused) * p.cache.heads); ++b) before += n;
+    int b = mine0, start, n;
+    while (x0 >= before + (n = Walk::tiles_of(p, N, b, start)) * p.cache.heads) {
+      before += n * p.cache.heads;
+      ++b;
+    }
     begin[0] = b;
-    begin[1] = x0 - before;
+    begin[1] = (x0 - before) / n;
+    begin[2] = (x0 - before) % n;
+    begin[3] = n;
+    begin[4] = start;
   }
   __syncthreads();
-  Walk walk(p, N, x0, x1, begin[0], begin[1]);
+  Walk walk(p, N, x0, x1, begin);
   const int log_page = p.cache.log_page, per_tile = kKvTile >> log_page, batch = 32 / per_tile;
 
   if (warp == 4) {
@@ -307,49 +330,65 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
     // -------------------------------------------------------------- queries
     KvRing ring;
     bool ok = true;
-    const bool vec = p.cache.dim % 4 == 0 && (uintptr_t)p.q % 8 == 0 && p.qs_t % 4 == 0 && p.qs_h % 4 == 0;
+    const bool vec = (uintptr_t)p.q % 16 == 0 && p.qs_t % 8 == 0 && p.qs_h % 8 == 0;
+    const int half = lane >> 4, d0 = 8 * (lane & 15);  // two rows at a time, 8 dimensions a lane
     for (int unit = 0; walk.valid(); ++unit) {
       const KvSpan span = kv_span(p.seq, walk.b);
       const int place0 = kv_length(p.seq, walk.b, p.cache.page) - span.count, rows = span.count * p.group;
       if (unit >= 2 && !(ok = kv_warp_wait(kQfree + 8 * ring.at, ring.phase ^ 1, kSiteKvEmpty))) break;
+      // Rows behind the last keep whatever is there: their columns are not read, and their factor is 0.
+      if (lane < N) {
+        const int t = min(lane, rows - 1) / p.group;
+        factors[ring.at * N + lane] = 0.f;
+        places[ring.at * N + lane] = place0 + t;
+        owners[ring.at * N + lane] = make_int2(span.first + t, walk.h * p.group + lane - t * p.group);
+      }
+      __syncwarp();
       uint8_t* hi = qs + ring.at * 2 * C::kQ;
-      for (int n0 = 0; n0 < N; n0 += 8) {
-        uint32_t raw[8][2];
+      // A loop, four rows a step, and not unrolled: code that runs once is paced by the fetch of its instructions.
+#pragma unroll 1
+      for (int n0 = 0; n0 < rows; n0 += 4) {
+        uint4 raw[2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int n = n0 + i;
-          raw[i][0] = raw[i][1] = 0;
-          if (n < rows && 4 * lane < p.cache.dim) {
-            const int t = n / p.group;
-            const uint16_t* q = p.q + (span.first + t) * p.qs_t + (walk.h * p.group + n - t * p.group) * p.qs_h + 4 * lane;
+        for (int i = 0; i < 2; ++i) {
+          const int n = n0 + 2 * i + half;
+          raw[i] = make_uint4(0, 0, 0, 0);
+          if (n < rows && d0 < p.cache.dim) {
+            const int2 own = owners[ring.at * N + n];
+            const uint16_t* q = p.q + own.x * p.qs_t + own.y * p.qs_h + d0;
             if (vec) {
-              const uint2 v = __ldg(reinterpret_cast<const uint2*>(q));
-              raw[i][0] = v.x;
-              raw[i][1] = v.y;
+              raw[i] = __ldg(reinterpret_cast<const uint4*>(q));
             } else {
-              raw[i][0] = (uint32_t)__ldg(q) | (uint32_t)__ldg(q + 1) << 16;
-              raw[i][1] = (uint32_t)__ldg(q + 2) | (uint32_t)__ldg(q + 3) << 16;
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[k] = (uint32_t)__ldg(q + 2 * k) | (uint32_t)__ldg(q + 2 * k + 1) << 16;
+              raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int n = n0 + i;
-          const uint32_t m = max(max(raw[i][0] & 0x7FFFu, raw[i][0] >> 16 & 0x7FFFu),
-                                 max(raw[i][1] & 0x7FFFu, raw[i][1] >> 16 & 0x7FFFu));
-          const uint32_t code = mxfp8_scale_code(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, m) << 16));
+        for (int i = 0; i < 2; ++i) {
+          const int n = n0 + 2 * i + half;
+          uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          uint32_t top = absmax_bf16x2(absmax_bf16x2(w[0], w[1]), absmax_bf16x2(w[2], w[3]));
+#pragma unroll
+          for (int o = 8; o; o >>= 1) top = absmax_bf16x2(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+          const uint32_t code = mxfp8_scale_code(__uint_as_float(max(top & 0x7FFFu, (top >> 16) & 0x7FFFu) << 16));
           const float inv = code == 255u ? 0.f : e8m0_to_float(254u - code);
-          const float v[4] = {__uint_as_float(raw[i][0] << 16) * inv, __uint_as_float(raw[i][0] & 0xFFFF0000u) * inv,
-                              __uint_as_float(raw[i][1] << 16) * inv, __uint_as_float(raw[i][1] & 0xFFFF0000u) * inv};
-          uint32_t h, l;
-          split_e4m3x4(v, h, l);
-          if (code == 255u) h = l = 0u;
-          const uint32_t to = n * 128 + (((lane >> 2) ^ (n & 7)) << 4) + (lane & 3) * 4;
-          *reinterpret_cast<uint32_t*>(hi + to) = h;
-          *reinterpret_cast<uint32_t*>(hi + C::kQ + to) = l;
-          if (lane == 0) {
-            factors[ring.at * N + n] = n >= rows ? 0.f : code == 255u ? NAN : p.scale * 1.4426950408889634f * e8m0_to_float(code);
-            places[ring.at * N + n] = place0 + min(n, rows - 1) / p.group;
+          uint32_t h[2], l[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float v[4] = {__uint_as_float(w[2 * k] << 16) * inv, __uint_as_float(w[2 * k] & 0xFFFF0000u) * inv,
+                                __uint_as_float(w[2 * k + 1] << 16) * inv, __uint_as_float(w[2 * k + 1] & 0xFFFF0000u) * inv};
+            split_e4m3x4(v, h[k], l[k]);
+            if (code == 255u) h[k] = l[k] = 0u;
+          }
+          if (n < rows) {
+            const uint32_t to = n * 128 + (((lane & 15) >> 1 ^ (n & 7)) << 4) + (lane & 1) * 8;
+            *reinterpret_cast<uint2*>(hi + to) = make_uint2(h[0], h[1]);
+            *reinterpret_cast<uint2*>(hi + C::kQ + to) = make_uint2(l[0], l[1]);
+            if (d0 == 0)
+              factors[ring.at * N + n] = code == 255u ? NAN : p.scale * 1.4426950408889634f * e8m0_to_float(code);
           }
         }
       }
@@ -392,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
     }
   } else {
     // -------------------------------------------------------------- softmax
-    const int j = threadIdx.x;
+    const int j = threadIdx.x, column = column_of<N>(lane);
     const uint32_t tq = tmem + ((uint32_t)(32 * warp) << 16);
     KvRing sr, vr, qr;
     uint32_t wphase = 1;  // of the last tile's MMAs on the values: a fresh barrier's previous phase counts as over
@@ -452,22 +491,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
       for (int n = 0; n < N; ++n) up |= x[n] > m[n] + kHeadroom;
       if (kv_bar_any(1, 128, up)) {
         if (kv_bar_any(1, 128, failed)) break;  // all four warps leave together
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-          float t = x[n];
-#pragma unroll
-          for (int o = 16; o; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, o));
-          if (lane == 0) red[warp * N + n] = t;
-        }
-        kv_bar_sync(1, 128);
         float f[N];
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-          const float t = fmaxf(fmaxf(red[n], red[N + n]), fmaxf(red[2 * N + n], red[3 * N + n])) - kStart;
-          const float to = fmaxf(m[n], t);
-          f[n] = ex2(m[n] - to);
-          m[n] = to;
-          l[n] *= f[n];
+        for (int n = 0; n < N; ++n) f[n] = x[n];
+        red[warp * N + column] = reduce_columns<N>(f, lane, [](float a, float b) { return fmaxf(a, b); });
+        kv_bar_sync(1, 128);
+#pragma unroll
+        for (int n = 0; n < N; n += 4) {
+          float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float4 r = *reinterpret_cast<const float4*>(red + w * N + n);
+            t[0] = fmaxf(t[0], r.x), t[1] = fmaxf(t[1], r.y), t[2] = fmaxf(t[2], r.z), t[3] = fmaxf(t[3], r.w);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float to = fmaxf(m[n + k], t[k] - kStart);
+            f[n + k] = ex2(m[n + k] - to);
+            m[n + k] = to;
+            l[n + k] *= f[n + k];
+          }
         }
         if (!first) {
           // O holds all tiles before once the last one's MMAs are done.
@@ -523,108 +566,91 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
 
       if (walk.last()) {
         // The unit's end, or this CTA's part of it: O^T has a dimension of the head a lane, a row a column.
-        const KvSpan span = kv_span(p.seq, walk.b);
-        const int rows = span.count * p.group;
+        const int2* own = owners + qr.at * N;
+        const int rows = kv_span(p.seq, walk.b).count * p.group;
+        const int unit0 = walk.x - walk.t, unit1 = unit0 + walk.tiles - 1;  // the unit's tiles
+        auto result = [&](int n, int d, float sum, float total_, float top) {  // of row n, dimension d
+          const int2 to = own[n];
+          const __nv_bfloat16 v = __float2bfloat16_rn(total_ == 0.f ? 0.f : sum / total_);
+          if (d < p.cache.dim) p.out[to.x * p.os_t + to.y * p.os_h + d] = *reinterpret_cast<const uint16_t*>(&v);
+          if (p.lse && d == 0)
+            p.lse[to.x * p.ls_t + to.y * p.ls_h] = total_ == 0.f ? -INFINITY : (top + log2f(total_)) * 0.6931471805599453f;
+        };
+        red[warp * N + column] = reduce_columns<N>(l, lane, [](float a, float b) { return a + b; });
         failed |= !kv_warp_wait(kWfree, wphase, kSiteKvFull);
         tc::fence_after_sync();
         kv_ld<N>(tq, raw);
         kv_wait_ld();
         kv_tie(raw);
         tc::fence_before_sync();
-        if (lane == 0) {
-          mbar_arrive(kOfree);
-          mbar_arrive(kQfree + 8 * qr.at);
-        }
-        qr.next(2);
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-          float t = l[n];
-#pragma unroll
-          for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
-          if (lane == 0) red[warp * N + n] = t;
-        }
+        if (lane == 0) mbar_arrive(kOfree);
         kv_bar_sync(1, 128);
-        float o[N];
+        if (unit0 >= x0 && unit1 < x1) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-          l[n] = (red[n] + red[N + n]) + (red[2 * N + n] + red[3 * N + n]);
-          o[n] = __uint_as_float(raw[n]);
-        }
-        bool done = true;
-        const int unit0 = walk.x - walk.t, unit1 = unit0 + walk.tiles - 1;  // the unit's tiles
-        if (unit0 < x0 || unit1 >= x1) {
+          for (int n = 0; n < N; ++n)
+            if (n < rows) result(n, j, __uint_as_float(raw[n]), (red[n] + red[N + n]) + (red[2 * N + n] + red[3 * N + n]), m[n]);
+        } else {
+          // Published: O [N][128], m [N], l [N]. The last to arrive joins all parts, in the order of the positions.
           const int cta0 = kv_owner(unit0, total, ctas), cta1 = kv_owner(unit1, total, ctas);
           auto part = [&](int cta) { return partials + (int64_t)(cta * 2 + (cta == cta0)) * C::kPart; };
-          float* mine_at = part(blockIdx.x);
+          float* mine = part(blockIdx.x);
 #pragma unroll
-          for (int n = 0; n < N; ++n) {
-            if (n < rows) __stcg(mine_at + n * 128 + j, o[n]);
-            if (j == n) {
-              __stcg(mine_at + N * 128 + n, m[n]);
-              __stcg(mine_at + N * 129 + n, l[n]);
-            }
+          for (int n = 0; n < N; ++n)
+            if (n < rows) __stcg(mine + n * 128 + j, __uint_as_float(raw[n]));
+          if (j < N) __stcg(mine + N * 129 + j, (red[j] + red[N + j]) + (red[2 * N + j] + red[3 * N + j]));
+          if (j == 32) {
+#pragma unroll
+            for (int n = 0; n < N; n += 4)
+              __stcg(reinterpret_cast<float4*>(mine + N * 128 + n), make_float4(m[n], m[n + 1], m[n + 2], m[n + 3]));
           }
-          __threadfence();
-          kv_bar_sync(1, 128);
-          int* flag = begin + 2;
+          kv_bar_sync(1, 128);  // orders the warps' stores before the counting thread's release
           if (j == 0) {
-            *flag = atomic_add_acq_rel_gpu(counters + cta0, 1) == cta1 - cta0;
-            if (*flag) counters[cta0] = 0;  // all parts are in: zero again for the next launch
+            begin[5] = atomic_add_acq_rel_gpu(counters + cta0, 1) == cta1 - cta0;
+            if (begin[5]) counters[cta0] = 0;  // all parts are in: zero again for the next launch
           }
           kv_bar_sync(1, 128);
-          done = *flag;
-          if (done) {
-            __threadfence();
-#pragma unroll
-            for (int n = 0; n < N; ++n) m[n] = kNone;
-            for (int c = cta0; c <= cta1; ++c) {
-              const float4* pm = reinterpret_cast<const float4*>(part(c) + N * 128);
-#pragma unroll
-              for (int n = 0; n < N; n += 4) {
-                const float4 v = __ldcg(pm + n / 4);
-                m[n] = fmaxf(m[n], v.x);
-                m[n + 1] = fmaxf(m[n + 1], v.y);
-                m[n + 2] = fmaxf(m[n + 2], v.z);
-                m[n + 3] = fmaxf(m[n + 3], v.w);
-              }
-            }
-#pragma unroll
-            for (int n = 0; n < N; ++n) o[n] = l[n] = 0.f;
-#pragma unroll
-            for (int n = 0; n < N; n += 4) {
-              if (n >= rows) break;
+          if (begin[5]) {
+            // Rows' maxima and sums, 128 / N threads a row (over the weights' buffer: the MMAs are done with it).
+            constexpr int kSplit = 128 / N;
+            float* tops = reinterpret_cast<float*>(ws);  // [kSplit][N], then [kSplit][N] sums
+            const int n = j % N;
+            float top = kNone, sum = 0.f;
 #pragma unroll 4
+            for (int c = cta0 + j / N; c <= cta1; c += kSplit) top = fmaxf(top, __ldcg(part(c) + N * 128 + n));
+            tops[j] = top;
+            kv_bar_sync(1, 128);
+            for (int i = 0; i < kSplit; ++i) top = fmaxf(top, tops[i * N + n]);
+#pragma unroll 4
+            for (int c = cta0 + j / N; c <= cta1; c += kSplit)
+              sum = fmaf(ex2(__ldcg(part(c) + N * 128 + n) - top), __ldcg(part(c) + N * 129 + n), sum);
+            tops[128 + j] = sum;
+            kv_bar_sync(1, 128);
+            if (j < N) {
+              float all = 0.f;
+              for (int i = 0; i < kSplit; ++i) all += tops[128 + i * N + n];
+              red[n] = top;
+              red[N + n] = all;
+            }
+            kv_bar_sync(1, 128);
+            // A warp a row, four dimensions a lane: many parts' loads are in flight at once.
+#pragma unroll 1
+            for (int r = warp; r < rows; r += 4) {
+              const float at = red[r], all = red[N + r];
+              float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
               for (int c = cta0; c <= cta1; ++c) {
-                const float* pp = part(c);
-                const float4 pm = __ldcg(reinterpret_cast<const float4*>(pp + N * 128 + n));
-                const float4 pl4 = __ldcg(reinterpret_cast<const float4*>(pp + N * 129 + n));
-                const float f[4] = {ex2(pm.x - m[n]), ex2(pm.y - m[n + 1]), ex2(pm.z - m[n + 2]), ex2(pm.w - m[n + 3])};
-                const float ls[4] = {pl4.x, pl4.y, pl4.z, pl4.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const float v = n + k < rows ? __ldcg(pp + (n + k) * 128 + j) : 0.f;
-                  o[n + k] = fmaf(f[k], v, o[n + k]);
-                  l[n + k] = fmaf(f[k], ls[k], l[n + k]);
-                }
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(part(c) + r * 128) + lane);
+                const float f = ex2(__ldcg(part(c) + N * 128 + r) - at);
+                o[0] = fmaf(f, v.x, o[0]), o[1] = fmaf(f, v.y, o[1]), o[2] = fmaf(f, v.z, o[2]), o[3] = fmaf(f, v.w, o[3]);
               }
-            }
-          }
-        } else {
-          kv_bar_sync(1, 128);  // before red is used again
-        }
-        if (done) {
 #pragma unroll
-          for (int n = 0; n < N; ++n) {
-            if (n < rows) {
-              const int t = n / p.group;
-              const int64_t token = span.first + t, head = walk.h * p.group + n - t * p.group;
-              const __nv_bfloat16 v = __float2bfloat16_rn(l[n] == 0.f ? 0.f : o[n] / l[n]);
-              if (j < p.cache.dim) p.out[token * p.os_t + head * p.os_h + j] = *reinterpret_cast<const uint16_t*>(&v);
-              if (p.lse && j == 0)
-                p.lse[token * p.ls_t + head * p.ls_h] = l[n] == 0.f ? -INFINITY : (m[n] + log2f(l[n])) * 0.6931471805599453f;
+              for (int k = 0; k < 4; ++k) result(r, 4 * lane + k, o[k], all, at);
             }
           }
         }
+        kv_bar_sync(1, 128);  // before red and the weights' buffer are used again
+        if (lane == 0) mbar_arrive(kQfree + 8 * qr.at);
+        qr.next(2);
       }
       walk.next();
     }
