@@ -657,10 +657,11 @@ MAMBO_API int mambo_kv_append(const MamboKvCache* cache, const void* k, int64_t 
  * last `window` of them where window is not 0:
  *   out = sum_j softmax_j(scale * q . k_j) v_j   (bf16),   lse = log sum_j exp(scale * q . k_j)   (f32, may be null).
  * A query that sees nothing has zeros and an lse of minus infinity; rows that
- * no sequence covers are not written. workspace: zero-filled once, shared with
- * the other calls of the stream.
+ * no sequence covers are not written. scale: a positive number. workspace:
+ * mambo_kv_attention_workspace_bytes(ragged: with offsets), zero-filled once,
+ * shared with the other calls of the stream.
  */
-MAMBO_API size_t mambo_kv_attention_workspace_bytes(int64_t tokens, int64_t heads, const MamboKvCache* cache);
+MAMBO_API size_t mambo_kv_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int ragged);
 MAMBO_API int mambo_kv_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, int64_t tokens,
                                  int64_t heads, const MamboKvCache* cache, const MamboKvSequences* seq, int64_t window,
                                  float scale, void* out, int64_t out_stride_token, int64_t out_stride_head, float* lse,

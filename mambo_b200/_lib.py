@@ -382,7 +382,7 @@ def load() -> ctypes.CDLL:
                  ctypes.POINTER(MamboRotary), vp],
                 i32,
             ),
-            "mambo_kv_attention_workspace_bytes": ([i64, i64, ctypes.POINTER(MamboKvCache)], ctypes.c_size_t),
+            "mambo_kv_attention_workspace_bytes": ([i64, i64, i32], ctypes.c_size_t),
             "mambo_kv_attention": (
                 [vp, i64, i64, i64, i64, ctypes.POINTER(MamboKvCache), ctypes.POINTER(MamboKvSequences), i64,
                  ctypes.c_float, vp, i64, i64, vp, i64, i64, vp, ctypes.c_size_t, vp],

@@ -69,6 +69,12 @@ KvSequences sequence_params(const MamboKvSequences* s, int64_t tokens) {
   return {s->page_table, s->table_stride, (int)s->table_pages, s->lengths, s->offsets, (int)s->batch, (int)tokens};
 }
 
+// Rows of a sequence (tokens times query heads of a key head) that the decode kernel takes at most: it has forms for 16
+// and for 32 rows, and where the heads alone are more, none.
+int few_rows(int group) { return group <= 16 ? 16 : group <= 32 ? 32 : 0; }
+size_t decode_bytes(int group) { return few_rows(group) ? (kv_decode_partial_bytes(group, kSmsBound) + 255) / 256 * 256 : 0; }
+constexpr int kPromptCounters = 4096;  // of the split counters: the prompt kernel's, behind the decode kernel's
+
 }  // namespace
 
 extern "C" {
@@ -139,11 +145,10 @@ int mambo_kv_append(const MamboKvCache* cache, const void* k, int64_t k_stride_t
   return api_ok();
 }
 
-size_t mambo_kv_attention_workspace_bytes(int64_t tokens, int64_t heads, const MamboKvCache* cache) {
-  if (!cache || tokens < 1 || tokens > kMaxTokens || cache->kv_heads < 1 || heads < 1 || heads > kMaxHeads ||
-      heads % cache->kv_heads)
-    return 0;
-  return kWorkspaceCounterBytes + kv_decode_partial_bytes((int)(heads / cache->kv_heads), kSmsBound);
+size_t mambo_kv_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int ragged) {
+  if (kv_heads < 1 || kv_heads > kMaxHeads || heads < 1 || heads > kMaxHeads || heads % kv_heads) return 0;
+  const int group = (int)(heads / kv_heads);
+  return kWorkspaceCounterBytes + decode_bytes(group) + (ragged || !few_rows(group) ? kv_prompt_partial_bytes(kSmsBound) : 0);
 }
 
 int mambo_kv_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, int64_t tokens, int64_t heads,
@@ -158,10 +163,15 @@ int mambo_kv_attention(const void* q, int64_t q_stride_token, int64_t q_stride_h
     return api_fail(MAMBO_EINVAL, "query heads must be a multiple of the cache's heads, at most %d", (int)kMaxHeads);
   if (window < 0) return api_fail(MAMBO_EINVAL, "the window must not be negative");
   if (!aligned(q, 2) || !aligned(out, 2) || !aligned(lse, 4)) return api_fail(MAMBO_EINVAL, kUnaligned);
-  // Tiles of 128 positions, over all sequences and heads, are counted in 32 bits.
-  if ((double)seq->batch * cache->kv_heads * ((double)seq->table_pages * cache->page_tokens / 128 + 1) >= 2147483647.0)
+  // Rows, and tiles of 128 positions over all sequences, heads and units of rows, are counted in 32 bits.
+  const int64_t group = heads / cache->kv_heads;
+  const double units = (double)tokens * group / 256 + (double)seq->batch;
+  if (tokens * group > (1 << 30) ||
+      units * cache->kv_heads * ((double)seq->table_pages * cache->page_tokens / 128 + 1) >= 2147483647.0)
     return api_fail(MAMBO_EINVAL, "the call is too large: split its sequences");
-  const size_t need = mambo_kv_attention_workspace_bytes(tokens, heads, cache);
+  if (!(scale > 0.f) || !(scale <= 3.4028234663852886e38f)) return api_fail(MAMBO_EINVAL, "the scale must be a positive number");
+  const bool prompt = seq->offsets || !few_rows((int)group);
+  const size_t need = mambo_kv_attention_workspace_bytes(heads, cache->kv_heads, seq->offsets != nullptr);
   if (!workspace || workspace_bytes < need)
     return api_fail(MAMBO_EWORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   if (!aligned(workspace, 256)) return api_fail(MAMBO_EINVAL, "workspace must be 256-byte aligned");
@@ -183,16 +193,18 @@ int mambo_kv_attention(const void* q, int64_t q_stride_token, int64_t q_stride_h
   p.group = (int)(heads / cache->kv_heads);
   p.window = window <= 0x7FFFFFFF ? (int)window : 0;
   p.scale = scale;
-  p.few = p.group <= 16 ? 16 : p.group <= 32 ? 32 : 0;
+  p.few = few_rows(p.group);
   CUtensorMap maps[2];
   for (int i = 0; i < 2; ++i)
     if (!kv_page_map(p.cache, i, &maps[i])) return api_fail(MAMBO_EINVAL, "the cache has no tensor map");
+  if (sms > kSmsBound) sms = kSmsBound;
+  uint8_t* parts = (uint8_t*)workspace + kWorkspaceCounterBytes;
+  int* counters = (int*)((uint8_t*)workspace + kWorkspaceSplitCounterOffset);
   cudaError_t e = cudaSuccess;
-  if (p.few)
-    e = launch_kv_decode(p, maps[0], maps[1], sms < kSmsBound ? sms : kSmsBound, smem,
-                         (float*)((uint8_t*)workspace + kWorkspaceCounterBytes),
-                         (int*)((uint8_t*)workspace + kWorkspaceSplitCounterOffset), (cudaStream_t)stream);
-  if (e == cudaSuccess && (p.seq.offsets || !p.few)) e = launch_kv_attention_simple(p, (cudaStream_t)stream);
+  if (p.few) e = launch_kv_decode(p, maps[0], maps[1], sms, smem, (float*)parts, counters, (cudaStream_t)stream);
+  if (e == cudaSuccess && prompt)
+    e = launch_kv_prompt(p, maps[0], maps[1], sms, (float*)(parts + decode_bytes(p.group)), counters + kPromptCounters,
+                         (cudaStream_t)stream);
   if (e != cudaSuccess) return api_cuda_fail(e, "attention");
   return api_ok();
 }

@@ -87,11 +87,15 @@ struct KvAttentionCall {
   float scale;         // of the scores
   int few;             // rows (tokens * group) of a sequence up to which the decode kernel has it; 0: it has none
 };
-cudaError_t launch_kv_attention_simple(const KvAttentionCall& p, cudaStream_t stream);
 bool kv_page_map(const KvCache& c, int which, CUtensorMap* map);
 size_t kv_decode_partial_bytes(int group, int sms);
 cudaError_t launch_kv_decode(const KvAttentionCall& p, const CUtensorMap& k, const CUtensorMap& v, int sms, int smem_optin,
                              float* partials, int* counters, cudaStream_t stream);
+size_t kv_prompt_partial_bytes(int sms);
+cudaError_t launch_kv_prompt(const KvAttentionCall& p, const CUtensorMap& k, const CUtensorMap& v, int sms, float* partials,
+                             int* counters, cudaStream_t stream);
+// Device addresses of the prompt kernel's status record and wait limit (the current device's).
+cudaError_t kv_prompt_status_symbols(void** status, void** limit);
 
 #ifdef __CUDACC__
 // The call's tokens of sequence b: [first, first + count), clamped to the call.

@@ -142,9 +142,8 @@ def launch_fp8_kv_append(cache: Fp8KvCache, k, v, page_table, lengths, *, offset
 
 
 @functools.lru_cache(maxsize=1024)
-def _attention_workspace_bytes(tokens: int, heads: int, kv_heads: int, page: int, dim: int) -> int:
-    return _lib.load().mambo_kv_attention_workspace_bytes(
-        tokens, heads, _lib.MamboKvCache(None, None, None, None, 1, kv_heads, page, dim))
+def _attention_workspace_bytes(heads: int, kv_heads: int, ragged: bool) -> int:
+    return _lib.load().mambo_kv_attention_workspace_bytes(heads, kv_heads, int(ragged))
 
 
 @_runtime.with_stream
@@ -183,7 +182,7 @@ def fp8_paged_attention(q, cache: Fp8KvCache, page_table, lengths, *, offsets=No
         raise ValueError("out must be bfloat16 of q's shape with unit stride along the head, on its device")
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if return_lse else None
     if tokens:
-        need = _attention_workspace_bytes(tokens, heads, view.kv_heads, view.page_tokens, dim)
+        need = _attention_workspace_bytes(heads, view.kv_heads, offsets is not None)
         with _device_guard(dev):
             with _runtime.workspace(dev, None, need) as ws:
                 _lib.check(_lib.load().mambo_kv_attention(
