@@ -24,10 +24,8 @@
 // several CTAs share is joined by the last to arrive, in the order of the
 // positions.
 //
-// Warps 0-3 and 4-7 softmax of either tile, 8-11 queries and values, 12 copies,
-// 13 MMA, 14 the pages' scales. Compiled as a whole program of its own, for
-// setmaxnreg; so it has its own device status.
-#define MAMBO_OWN_DEVICE_STATUS
+// Warps 0-3 and 4-7 softmax of either tile, 8-11 queries and values, 12 copies, 13 MMA, 14 the pages' scales, 15 the
+// units to come, which it describes to the others.
 #include "iq3s_tm.cuh"
 #include "kernels.cuh"
 #include "kv_tc.cuh"
@@ -42,75 +40,68 @@ constexpr int kUnitRows = 2 * kRows;
 constexpr int kKStages = 3, kVStages = 2;
 constexpr float kNone = -1e30f;       // m of a row that has seen nothing
 constexpr float kHeadroom = 8.f;
+// What a unit costs besides its tiles, in tiles: where the ranges of the CTAs are cut, units count as this much longer.
+constexpr int kUnitCost = 2;
 
 // Shared memory: queries [2 tiles][hi, lo][128][128], keys, values as they come and in f16 [2 halves of D][128][128 bytes].
 constexpr uint32_t kQ = 4 * kKvTileBytes, kVf = 2 * kKvTileBytes;
 constexpr uint32_t kAtK = kQ, kAtV = kAtK + kKStages * kKvTileBytes, kAtVf = kAtV + kVStages * kKvTileBytes;
-constexpr uint32_t kAtFactors = kAtVf + 2 * kVf, kAtScales = kAtFactors + kUnitRows * 4, kAtBegin = kAtScales + 2 * 32 * 16;
-constexpr uint32_t kAtBars = kAtBegin + 128;
-constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 4 + 8 + 2 + 4;
+constexpr uint32_t kAtFactors = kAtVf + 2 * kVf, kAtScales = kAtFactors + kUnitRows * 4, kAtUnits = kAtScales + 2 * 32 * 16;
+constexpr int kUnitStages = 4;
+constexpr uint32_t kAtBegin = kAtUnits + (kUnitStages + 1) * 64, kAtBars = kAtBegin + 128;
+constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 4 + 8 + 4 + 4 + 2 * kUnitStages;
 constexpr uint32_t kSmem = 1024 + kAtBars + kNumBars * 8 + 16;
 constexpr int kPart = kRows * 130;    // floats of a tile's part: O [32][128][4], m, l
 
-// The unit that a CTA is at, and its tiles. b, h: sequence and key head; u: the unit's number in them.
-struct Walk {
+// A CTA's part of a unit, as one warp works it out and the others read it.
+struct alignas(64) Unit {
+  int tile, n;        // tiles [tile, tile + n) of the sequence's positions; n == 0: there is no further unit
+  int b, h;           // sequence, key head
+  int row0, rows;     // the unit's first row, all rows of the sequence
+  int token, place0;  // the sequence's first token and its position
+  int lo[2], hi[2];   // positions of the first and last rows of either tile of rows; hi < lo: it has no rows
+  int x, tiles;       // the unit's tiles in the work: [x, x + tiles); this part is all of it where n == tiles
+  __device__ __forceinline__ bool has(int q) const { return row0 + kRows * q < rows; }
+};
+// Whether rows at the positions lo .. hi see any of the 128 positions from tile j on: the MMA and the softmax go by it.
+__device__ __forceinline__ bool sees(int lo, int hi, int j, int window) {
+  const int64_t j0 = (int64_t)j * kKvTile;
+  return j0 <= hi && (window == 0 || j0 + kKvTile - 1 > (int64_t)lo - window);
+}
+
+// The units of a call: sequence b, key head h, unit u of `units` of that head.
+struct Plan {
   const KvAttentionCall& p;
-  int x, x1, b, h, u, t, tiles, start;
-  int first_token, place0, rows;  // of the sequence: its first token, the position of that, its rows
-  bool first;                     // tile of the CTA's part of the unit
+  int b, h, u, units, token, place0, rows;
   __device__ __forceinline__ void sequence() {
     const KvSpan s = kv_span(p.seq, b);
-    first_token = s.first;
+    token = s.first;
     rows = (int64_t)s.count * p.group > p.few ? s.count * p.group : 0;
     place0 = kv_length(p.seq, b, p.cache.page) - s.count;
+    units = (rows + kUnitRows - 1) / kUnitRows;
   }
-  __device__ __forceinline__ int units() const { return (rows + kUnitRows - 1) / kUnitRows; }
   __device__ __forceinline__ int place(int row) const { return place0 + min(row, rows - 1) / p.group; }
-  // Tiles of unit i, at least one.
-  __device__ __forceinline__ int tiles_of(int i, int& at) const {
+  // Tiles of positions of unit i, at least one (of masked ones), and the first of them.
+  __device__ __forceinline__ int tiles_of(int i, int& first) const {
     const int64_t low = p.window ? place(kUnitRows * i) + 1 - (int64_t)p.window : 0;
-    at = low > 0 ? (int)(low / kKvTile) : 0;
+    first = low > 0 ? (int)(low / kKvTile) : 0;
     const int high = place(kUnitRows * i + kUnitRows - 1);
-    const int end = high >= 0 ? high / kKvTile + 1 : 0;
-    return max(end - at, 1);
+    return max((high >= 0 ? high / kKvTile + 1 : 0) - first, 1);
   }
-  __device__ __forceinline__ Walk(const KvAttentionCall& call, int x0, int end, const int* at)
-      : p(call), x(x0), x1(end), b(at[0]), h(at[1]), u(at[2]), t(at[3]), tiles(1), start(0), first(true) {
-    if (x >= x1) return;
-    sequence();
-    tiles = tiles_of(u, start);
+  // Its share of the work: the tiles come last.
+  __device__ __forceinline__ int cost_of(int i) const {
+    int first;
+    return tiles_of(i, first) + kUnitCost;
   }
-  __device__ __forceinline__ bool valid() const { return x < x1; }
-  __device__ __forceinline__ bool last() const { return t == tiles - 1 || x == x1 - 1; }
   __device__ __forceinline__ void next() {
-    ++x;
-    first = false;
-    if (++t < tiles) return;
-    t = 0;
-    first = true;
-    if (x >= x1) return;
-    if (++u == units()) {
-      u = 0;
-      if (++h == p.cache.heads) {
-        h = 0;
-        do {
-          ++b;
-          sequence();
-        } while (rows == 0);  // x < x1: there is one
-      }
-    }
-    tiles = tiles_of(u, start);
-  }
-  // Places of a tile's first and last rows (lo > hi: it has no rows), and whether its rows see any of the 128 positions
-  // from j0 on: what the MMA and the softmax both go by.
-  __device__ __forceinline__ void bounds(int q, int& lo, int& hi) const {
-    const int r = kUnitRows * u + kRows * q;
-    lo = r < rows ? place(r) : 0;
-    hi = r < rows ? place(r + kRows - 1) : -1;
-  }
-  __device__ __forceinline__ int64_t j0() const { return (int64_t)(start + t) * kKvTile; }
-  __device__ __forceinline__ bool sees(int lo, int hi) const {
-    return j0() <= hi && (p.window == 0 || j0() + kKvTile - 1 > (int64_t)lo - p.window);
+    if (++u < units) return;
+    u = 0;
+    if (++h < p.cache.heads) return;
+    h = 0;
+    do {
+      ++b;
+      sequence();
+    } while (rows == 0);  // called only where there is one
   }
 };
 
@@ -167,6 +158,40 @@ __device__ __forceinline__ void mma_values(uint32_t d, uint32_t w, uint32_t v, u
       : "memory");
 }
 
+// Packed FP32 pairs in 64-bit registers.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma_2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float low_of(uint64_t a) { return __uint_as_float((uint32_t)a); }
+__device__ __forceinline__ float high_of(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
+// 2^x of a pair in the FMA pipe, which has room where the special function unit has none. x = n + f with n the nearest
+// integer (read off the low bits of x + 1.5 * 2^23), f in [-1/2, 1/2]; 2^f is the minimax polynomial of degree 4 (by
+// Remez' exchange, relative error 2.6e-6); n is added to its exponent. x is at most about 10; below -126 it counts as that.
+__device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
+  float a, b;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(low_of(x)), "f"(-126.f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(high_of(x)), "f"(-126.f));
+  x = pack2(a, b);
+  const uint64_t n = add_2(x, pack2(12582912.f, 12582912.f));
+  const uint64_t f = add_2(x, fma_2(n, pack2(-1.f, -1.f), pack2(12582912.f, 12582912.f)));
+  uint64_t y = fma_2(pack2(0.009570102f, 0.009570102f), f, pack2(0.05591786f, 0.05591786f));
+  y = fma_2(y, f, pack2(0.24024744f, 0.24024744f));
+  y = fma_2(y, f, pack2(0.6931218f, 0.6931218f));
+  y = fma_2(y, f, pack2(0.9999993f, 0.9999993f));
+  return pack2(__uint_as_float((uint32_t)y + ((uint32_t)n << 23)), __uint_as_float((uint32_t)(y >> 32) + ((uint32_t)(n >> 32) << 23)));
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -182,7 +207,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* factors = reinterpret_cast<float*>(sm + kAtFactors);   // of the unit's rows
   float4* scales = reinterpret_cast<float4*>(sm + kAtScales);   // [2][4 tiles][8]: key factor, value exponent, 2^-exponent
-  int* begin = reinterpret_cast<int*>(sm + kAtBegin);           // the first tile: sequence, head, unit, tile; [8] flags
+  Unit* units = reinterpret_cast<Unit*>(sm + kAtUnits);         // [kUnitStages], and an empty one
+  int* begin = reinterpret_cast<int*>(sm + kAtBegin);           // where the share begins: sequence, head, unit, place in its work; [8] flags
   int* warp_sums = begin + 16;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kAtBars);
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
@@ -190,7 +216,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t kKfull = smem_u32(bars), kKfree = kKfull + 8 * kKStages, kVfull = kKfree + 8 * kKStages;
   const uint32_t kVfree = kVfull + 8 * kVStages, kFfull = kVfree + 8 * kVStages, kFfree = kFfull + 16;  // values in f16
   const uint32_t kSfull = kFfree + 16, kWfull = kSfull + 16, kOdone = kWfull + 16, kOfree = kOdone + 16;
-  const uint32_t kQfull = kOfree + 16, kQfree = kQfull + 8, kMfull = kQfree + 8, kMfree = kMfull + 16;
+  const uint32_t kQfull = kOfree + 16, kQfree = kQfull + 16, kMfull = kQfree + 16, kMfree = kMfull + 16;
+  const uint32_t kUfull = kMfree + 16, kUfree = kUfull + 8 * kUnitStages;
   const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -212,8 +239,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(kMfull + 8 * i, 1);
       mbar_init(kMfree + 8 * i, 8);
     }
-    mbar_init(kQfull, 4);
-    mbar_init(kQfree, 9);  // the MMAs and the softmax warps
+    for (int i = 0; i < kUnitStages; ++i) {
+      mbar_init(kUfull + 8 * i, 1);
+      mbar_init(kUfree + 8 * i, 15);  // copies, MMA, scales, 4 warps of values, 8 of the softmax
+    }
+    units[kUnitStages] = Unit{};
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(kQfull + 8 * i, 4);
+      mbar_init(kQfree + 8 * i, 5);  // the MMAs and the tile's softmax warps
+    }
     fence_barrier_init();
   }
   if (warp == 13) {
@@ -226,21 +260,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   pdl_wait();
   pdl_launch_dependents();
-  // All tiles, and where this CTA's first one lies: a warp has a run of sequences, a lane every 32nd unit of one.
+  // The whole work, and where this CTA's share begins: a warp has a run of sequences, a lane every 32nd unit of one.
   const int each = (p.seq.batch + 15) / 16, mine0 = min(p.seq.batch, warp * each), mine1 = min(p.seq.batch, mine0 + each);
-  const int zeros[4] = {0, 0, 0, 0};
-  Walk scan(p, 0, 0, zeros);
-  auto tiles_of_head = [&](int b) {
-    scan.b = b;
-    scan.sequence();
-    int n = 0, at;
-    for (int i = lane; i < scan.units(); i += 32) n += scan.tiles_of(i, at);
+  Plan plan{p, 0, 0, 0, 0, 0, 0, 0};
+  auto cost_of_head = [&](int b) {
+    plan.b = b;
+    plan.sequence();
+    int n = 0;
+    for (int i = lane; i < plan.units; i += 32) n += plan.cost_of(i);
 #pragma unroll
     for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
     return n;
   };
   int sum = 0;
-  for (int b = mine0; b < mine1; ++b) sum += tiles_of_head(b) * p.cache.heads;
+  for (int b = mine0; b < mine1; ++b) sum += cost_of_head(b) * p.cache.heads;
   if (lane == 0) warp_sums[warp] = sum;
   tc::fence_before_sync();
   __syncthreads();
@@ -251,22 +284,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     total += warp_sums[w];
     before += w < warp ? warp_sums[w] : 0;
   }
-  // Each of the CTAs that take part has a tile at least: those of a unit's parts are all that the join waits for.
+  // Each share is a tile at least, so that of the CTAs between a unit's first and last tile each has one: those are all
+  // that the join waits for.
   const int ctas = max(1, min((int)gridDim.x, total));
   const bool has = (int)blockIdx.x < ctas;
   const int x0 = has ? (int)((int64_t)blockIdx.x * total / ctas) : 0;
   const int x1 = has ? (int)(((int64_t)blockIdx.x + 1) * total / ctas) : 0;
   if (x0 < x1 && x0 >= before && x0 < before + sum) {
     int b = mine0, n;
-    while (x0 >= before + (n = tiles_of_head(b)) * p.cache.heads) {
+    while (x0 >= before + (n = cost_of_head(b)) * p.cache.heads) {
       before += n * p.cache.heads;
       ++b;
     }
-    const int h = (x0 - before) / n, units = scan.units();
-    int rest = (x0 - before) % n;  // tiles of the head before the first one
+    const int h = (x0 - before) / n;
+    int rest = (x0 - before) % n;  // what comes before in the head
     for (int i0 = 0;; i0 += 32) {
-      int at;
-      const int mine = i0 + lane < units ? scan.tiles_of(i0 + lane, at) : 0;
+      const int mine = i0 + lane < plan.units ? plan.cost_of(i0 + lane) : 0;
       int upto = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -280,173 +313,238 @@ __global__ void __launch_bounds__(kThreads, 1)
         begin[3] = rest - (upto - mine);
       }
       const int all = __shfl_sync(0xFFFFFFFFu, upto, 31);
-      if (rest < all || i0 + 32 >= units) break;
+      if (rest < all || i0 + 32 >= plan.units) break;
       rest -= all;
     }
   }
   __syncthreads();
-  Walk walk(p, x0, x1, begin);
+  // The next unit of this CTA, told by its ring's barrier; a role gives it back once it is through with it.
+  auto unit_of = [&](const KvRing& ring) -> const Unit& {
+    return units[kv_wait(kUfull + 8 * ring.at, ring.phase, kSiteKvFull) ? ring.at : kUnitStages];
+  };
   const int log_page = p.cache.log_page, per_tile = kKvTile >> log_page;
 
-  // Register split, launched with 128 a thread: 256 x 192 + 128 x 80 + 128 x 48 = 512 x 128.
   if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 12) {
       // ------------------------------------------------------------ copies
-      KvRing kr, vr;
-      auto page_of = [&](const Walk& w) {
-        const int64_t i = (int64_t)(w.start + w.t) * per_tile + lane;
-        return w.valid() && lane < per_tile && i < p.seq.table_pages ? __ldg(p.seq.table + w.b * p.seq.table_stride + i) : -1;
-      };
+      KvRing kr, vr, ur;
       const uint64_t policy = l2_policy_evict_last();
-      int page = page_of(walk);
       bool ok = true;
-      for (int it = 0; walk.valid(); ++it) {
-        const int h = walk.h;
-        walk.next();
-        const int next_page = page_of(walk);
-        // A page outside the cache: a box outside the tensor, which reads zeros.
-        const int row = page >= 0 && page < p.cache.pages ? page * p.cache.heads + h : -1;
-        if (it >= kKStages && !(ok = kv_warp_wait(kKfree + 8 * kr.at, kr.phase ^ 1, kSiteKvEmpty))) break;
-        if (lane == 0) mbar_arrive_expect_tx(kKfull + 8 * kr.at, kKvTileBytes);
+      for (int it = 0; ok;) {
+        const Unit& unit = unit_of(ur);
+        const int n = unit.n, h = unit.h;
+        if (n <= 0) break;
+        const int64_t i0 = (int64_t)unit.tile * per_tile + lane;
+        const int* row_pages = p.seq.table + unit.b * p.seq.table_stride + i0;
+        auto page_of = [&](int t) {
+          return t < n && lane < per_tile && i0 + t * per_tile < p.seq.table_pages ? __ldg(row_pages + t * per_tile) : -1;
+        };
+        int page = page_of(0);
+        for (int t = 0; t < n; ++t, ++it) {
+          const int next_page = page_of(t + 1);
+          // A page outside the cache: a box outside the tensor, which reads zeros.
+          const int row = page >= 0 && page < p.cache.pages ? page * p.cache.heads + h : -1;
+          if (it >= kKStages && !(ok = kv_warp_wait(kKfree + 8 * kr.at, kr.phase ^ 1, kSiteKvEmpty))) break;
+          if (lane == 0) mbar_arrive_expect_tx(kKfull + 8 * kr.at, kKvTileBytes);
+          __syncwarp();
+          if (lane < per_tile)
+            tma_load_3d(sm0 + kAtK + kr.at * kKvTileBytes + lane * (128u << log_page), &kmap, 0, 0, row, kKfull + 8 * kr.at, policy);
+          if (it >= kVStages && !(ok = kv_warp_wait(kVfree + 8 * vr.at, vr.phase ^ 1, kSiteKvEmpty))) break;
+          if (lane == 0) mbar_arrive_expect_tx(kVfull + 8 * vr.at, kKvTileBytes);
+          __syncwarp();
+          if (lane < per_tile)
+            tma_load_3d(sm0 + kAtV + vr.at * kKvTileBytes + lane * (128u << log_page), &vmap, 0, 0, row, kVfull + 8 * vr.at, policy);
+          page = next_page;
+          kr.next(kKStages);
+          vr.next(kVStages);
+        }
         __syncwarp();
-        if (lane < per_tile)
-          tma_load_3d(sm0 + kAtK + kr.at * kKvTileBytes + lane * (128u << log_page), &kmap, 0, 0, row, kKfull + 8 * kr.at, policy);
-        if (it >= kVStages && !(ok = kv_warp_wait(kVfree + 8 * vr.at, vr.phase ^ 1, kSiteKvEmpty))) break;
-        if (lane == 0) mbar_arrive_expect_tx(kVfull + 8 * vr.at, kKvTileBytes);
-        __syncwarp();
-        if (lane < per_tile)
-          tma_load_3d(sm0 + kAtV + vr.at * kKvTileBytes + lane * (128u << log_page), &vmap, 0, 0, row, kVfull + 8 * vr.at, policy);
-        page = next_page;
-        kr.next(kKStages);
-        vr.next(kVStages);
+        if (lane == 0) mbar_arrive(kUfree + 8 * ur.at);
+        ur.next(kUnitStages);
       }
       if (!ok) kv_settle();
     } else if (warp == 13) {
       // ------------------------------------------------------------ MMA
-      if (walk.valid() && tm::elect_one()) {
+      if (tm::elect_one()) {
         const uint32_t idesc_o = tc::idesc_f16_f32(kRows, p.cache.dim) | kIdescAlongN;
         const bool wide = p.cache.dim > 64;
         const uint32_t q0 = desc_low(sm0, 16), k0 = desc_low(sm0 + kAtK, 16), v0 = desc_low(sm0 + kAtVf, kKvTileBytes);
-        KvRing kr, fr;
-        uint32_t qphase = 0, wphase[2] = {0, 0}, ophase[2] = {1, 1};
-        bool ok = true, started[2] = {false, false};
-        // The scores of a tile; those of a tile of positions that a tile of rows does not see are left out.
-        auto scores = [&](const Walk& w, int q) {
-          int lo, hi;
-          w.bounds(q, lo, hi);
-          if (w.sees(lo, hi))
-            mma_scores(tmem + q * 128, q0 + q * (2 * kKvTileBytes >> 4), k0 + kr.at * (kKvTileBytes >> 4), wide, kSfull + 8 * q);
-        };
-        auto values = [&](const Walk& w, int q) {
-          int lo, hi;
-          w.bounds(q, lo, hi);
-          if (!w.sees(lo, hi)) return true;
-          if (!kv_wait(kWfull + 8 * q, wphase[q], kSiteKvFull)) return false;
-          wphase[q] ^= 1;
-          if (!started[q]) {
-            // The softmax has read the last unit's O.
-            if (!kv_wait(kOfree + 8 * q, ophase[q], kSiteKvEmpty)) return false;
+        // The unit and tile whose values come next (cur), and whose scores do (one tile ahead of it).
+        struct Cursor {
+          int tile, left, lo0, hi0, lo1, hi1;
+          __device__ __forceinline__ void load(const Unit& u) {
+            tile = u.tile;
+            left = u.n;
+            lo0 = u.lo[0], hi0 = u.hi[0], lo1 = u.lo[1], hi1 = u.hi[1];
           }
+          __device__ __forceinline__ bool sees(int q, int window) const {
+            return q ? mambo::sees(lo1, hi1, tile, window) : mambo::sees(lo0, hi0, tile, window);
+          }
+        } cur, ahead;
+        KvRing kr, fr, cu, au;
+        uint32_t qphase = 0, wphase0 = 0, wphase1 = 0, ophase0 = 1, ophase1 = 1;
+        bool ok = true, started0 = false, started1 = false, begins = true;  // begins: ahead is at a unit's first tile
+        auto scores = [&](int q) {
+          if (begins && !kv_wait(kQfull + 8 * q, qphase, kSiteKvFull)) return false;
+          if (q == 0 && !kv_wait(kKfull + 8 * kr.at, kr.phase, kSiteKvFull)) return false;
           tc::fence_after_sync();
-          mma_values(tmem + 256 + q * 128, tmem + q * 128, v0 + fr.at * (kVf >> 4), idesc_o, started[q], kOdone + 8 * q);
-          started[q] = true;
-          return true;
-        };
-        Walk ahead = walk;
-        auto next_scores = [&](int q) {  // of the tile after, while the softmax works on the other tile of rows
-          if (!ahead.valid()) return true;
-          if (q == 0) {
-            if (ahead.first) {
-              if (!kv_wait(kQfull, qphase, kSiteKvFull)) return false;
-              qphase ^= 1;
-            }
-            if (!kv_wait(kKfull + 8 * kr.at, kr.phase, kSiteKvFull)) return false;
-            tc::fence_after_sync();
-          }
-          scores(ahead, q);
+          if (ahead.sees(q, p.window))
+            mma_scores(tmem + q * 128, q0 + q * (2 * kKvTileBytes >> 4), k0 + kr.at * (kKvTileBytes >> 4), wide, kSfull + 8 * q);
+          if (ahead.left == 1) tc::commit(kQfree + 8 * q);
           if (q == 1) {
             tc::commit(kKfree + 8 * kr.at);
-            if (ahead.last()) tc::commit(kQfree);
             kr.next(kKStages);
+            ++ahead.tile;
+            qphase ^= begins;
+            begins = --ahead.left == 0;
+            if (begins) {
+              au.next(kUnitStages);
+              ahead.load(unit_of(au));
+            }
           }
           return true;
         };
-        ok = next_scores(0) && next_scores(1);
-        ahead.next();
-        while (ok && walk.valid()) {
-          if (walk.first) started[0] = started[1] = false;
+        auto values = [&](int q, uint32_t& wphase, uint32_t ophase, bool& started) {
+          if (!cur.sees(q, p.window)) return true;
+          if (!kv_wait(kWfull + 8 * q, wphase, kSiteKvFull)) return false;
+          wphase ^= 1;
+          // The softmax has read the last unit's O.
+          if (!started && !kv_wait(kOfree + 8 * q, ophase, kSiteKvEmpty)) return false;
+          tc::fence_after_sync();
+          mma_values(tmem + 256 + q * 128, tmem + q * 128, v0 + fr.at * (kVf >> 4), idesc_o, started, kOdone + 8 * q);
+          started = true;
+          return true;
+        };
+        ahead.load(unit_of(au));
+        cur = ahead;
+        if (cur.left > 0) ok = scores(0) && scores(1);
+        while (ok && cur.left > 0) {
           ok = kv_wait(kFfull + 8 * fr.at, fr.phase, kSiteKvFull);
           if (!ok) break;
           // The next unit's queries may still be on their way: both tiles' values come first then.
-          const bool turn = ahead.valid() && ahead.first;
-          ok = values(walk, 0) && (turn || next_scores(0)) && values(walk, 1) && (!turn || next_scores(0)) && next_scores(1);
+          const bool more = ahead.left > 0, turn = begins;
+          ok = values(0, wphase0, ophase0, started0) && (!more || turn || scores(0)) &&
+               values(1, wphase1, ophase1, started1) && (!more || !turn || scores(0)) && (!more || scores(1));
           if (!ok) break;
           tc::commit(kFfree + 8 * fr.at);
           fr.next(2);
-          if (walk.last()) {
-            for (int q = 0; q < 2; ++q)
-              if (started[q]) ophase[q] ^= 1;
+          ++cur.tile;
+          if (--cur.left == 0) {
+            ophase0 ^= started0;
+            ophase1 ^= started1;
+            started0 = started1 = false;
+            mbar_arrive(kUfree + 8 * cu.at);
+            cu.next(kUnitStages);
+            cur.load(unit_of(cu));
           }
-          walk.next();
-          ahead.next();
         }
         if (!ok) kv_settle();
       }
     } else if (warp == 14) {
       // ------------------------------------------------------------ scales: four tiles at a time, 16 positions a lane
-      KvRing ring;
-      for (int step = 0; walk.valid(); ++step) {
-        int64_t at = -1;
-        int h = 0;
-        for (int i = 0; i < 4 && walk.valid(); ++i) {
-          if (i == lane >> 3) {
-            const int64_t k = (walk.j0() + 16 * (lane & 7)) >> log_page;
-            at = k < p.seq.table_pages ? walk.b * p.seq.table_stride + k : -1;
-            h = walk.h;
-          }
-          walk.next();
-        }
+      KvRing ring, ur;
+      int step = 0, fill = 0;  // tiles in the current batch
+      int64_t at = -1;         // of this lane's tile: place in the table; and its head
+      int head = 0;
+      auto publish = [&]() {
         const int page = at >= 0 ? __ldg(p.seq.table + at) : -1;
         float4 v = make_float4(0.f, -INFINITY, 0.f, 0.f);  // positions without a page: x is minus infinity
         if (page >= 0 && page < p.cache.pages) {
-          const int64_t row = (int64_t)page * p.cache.heads + h;
+          const int64_t row = (int64_t)page * p.cache.heads + head;
           const uint32_t kc = max((uint32_t)__ldg(p.cache.scales[0] + row), kKvMinCode);
           const uint32_t vc = max((uint32_t)__ldg(p.cache.scales[1] + row), kKvMinCode);
           v = make_float4(kc == 255u ? NAN : e8m0_to_float(kc), vc == 255u ? NAN : (float)((int)vc - 127),
                           vc == 255u ? 1.f : e8m0_to_float(254u - vc), 0.f);
         }
-        if (step >= 2 && !kv_warp_wait(kMfree + 8 * ring.at, ring.phase ^ 1, kSiteKvEmpty)) break;
+        if (step >= 2) kv_warp_wait(kMfree + 8 * ring.at, ring.phase ^ 1, kSiteKvEmpty);
+        ++step;
         scales[ring.at * 32 + lane] = v;
         __syncwarp();
         if (lane == 0) mbar_arrive(kMfull + 8 * ring.at);
         ring.next(2);
+        fill = 0;
+        at = -1;
+      };
+      for (;;) {
+        const Unit& unit = unit_of(ur);
+        const int n = unit.n, tile = unit.tile, b = unit.b, h = unit.h;
+        if (n <= 0) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(kUfree + 8 * ur.at);
+        ur.next(kUnitStages);
+        for (int t = 0; t < n;) {
+          const int take = min(4 - fill, n - t), mine = (lane >> 3) - fill;  // tiles t .. t + take - 1 join the batch
+          if (mine >= 0 && mine < take) {
+            const int64_t k = ((int64_t)(tile + t + mine) * kKvTile + 16 * (lane & 7)) >> log_page;
+            at = k < p.seq.table_pages ? b * p.seq.table_stride + k : -1;
+            head = h;
+          }
+          t += take;
+          fill += take;
+          if (fill == 4) publish();
+        }
+      }
+      if (fill) publish();
+    } else if (lane == 0) {
+      // ------------------------------------------------------------ units
+      KvRing ur;
+      plan.b = begin[0];
+      plan.h = begin[1];
+      plan.u = begin[2];
+      if (x0 < x1) plan.sequence();
+      int x = x0, at = begin[3];  // place in the work, and in the unit's
+      for (int it = 0;;) {
+        Unit u{};
+        if (x < x1) {
+          u.tiles = plan.tiles_of(plan.u, u.tile);
+          const int t = max(at - kUnitCost, 0), left = x1 - x - max(kUnitCost - at, 0);
+          u.x = x - at + kUnitCost;
+          u.n = max(min(u.tiles - t, left), 0);
+          x = u.x + u.tiles;
+          at = 0;
+          u.tile += t;
+          u.b = plan.b;
+          u.h = plan.h;
+          u.row0 = kUnitRows * plan.u;
+          u.rows = plan.rows;
+          u.token = plan.token;
+          u.place0 = plan.place0;
+          for (int q = 0; q < 2; ++q) {
+            const bool has_rows = u.row0 + kRows * q < plan.rows;
+            u.lo[q] = has_rows ? plan.place(u.row0 + kRows * q) : 0;
+            u.hi[q] = has_rows ? plan.place(u.row0 + kRows * q + kRows - 1) : -1;
+          }
+          if (x < x1) plan.next();
+        }
+        if (it >= kUnitStages && !kv_wait(kUfree + 8 * ur.at, ur.phase ^ 1, kSiteKvEmpty)) u.n = 0;
+        units[ur.at] = u;
+        mbar_arrive(kUfull + 8 * ur.at);
+        ur.next(kUnitStages);
+        if (u.n == 0) break;  // of the last unit only the work besides its tiles may fall to this CTA
+        ++it;
       }
     }
   } else if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // -------------------------------------------------------------- queries and values
     const int i = threadIdx.x - 256;  // position of the tile
     const bool vec = (uintptr_t)p.q % 16 == 0 && p.qs_t % 8 == 0 && p.qs_h % 8 == 0;
-    KvRing vr, fr;
-    int unit = 0;
-    // A half warp a row, eight dimensions a lane.
-    auto queries = [&](const Walk& w) {
-      if (unit > 0) kv_warp_wait(kQfree, (unit & 1) ^ 1, kSiteKvEmpty);
-      ++unit;
-      const int d0 = 8 * (lane & 15), r0 = kUnitRows * w.u;
-      const int rows = min(kUnitRows, w.rows - r0);
-#pragma unroll 1
-      for (int n0 = 2 * (warp - 8) + (lane >> 4); n0 < kUnitRows; n0 += 32) {
-        uint4 raw[4];
+    KvRing vr, fr, ur;
+    uint32_t qphase = 1;  // a fresh barrier's previous phase counts as over
+    // Rows 8 apart: tokens and query heads on.
+    const int step_t = 8 / p.group, step_h = 8 % p.group;
+    // A half warp a row, eight dimensions a lane; the next four rows are loaded while four are split.
+    auto queries = [&](const Unit& u) {
+      const int d0 = 8 * (lane & 15), first = 2 * (warp - 8) + (lane >> 4);
+      const int rows = d0 < p.cache.dim ? min(kUnitRows, u.rows - u.row0) : 0;
+      const int end = u.has(1) ? kUnitRows : kRows;
+      int t = (u.row0 + first) / p.group, hh = u.row0 + first - t * p.group;
+      const uint16_t* q0 = p.q + (int64_t)u.token * p.qs_t + (int64_t)u.h * p.group * p.qs_h + d0;
+      auto load = [&](int n0, uint4 (&raw)[4]) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int n = n0 + 8 * k;
           raw[k] = make_uint4(0, 0, 0, 0);
-          if (n < rows && d0 < p.cache.dim) {
-            const int t = (r0 + n) / p.group;
-            const uint16_t* q = p.q + (int64_t)(w.first_token + t) * p.qs_t +
-                                (int64_t)(w.h * p.group + (r0 + n) - t * p.group) * p.qs_h + d0;
+          if (n0 + 8 * k < rows) {
+            const uint16_t* q = q0 + t * p.qs_t + hh * p.qs_h;
             if (vec) {
               raw[k] = __ldg(reinterpret_cast<const uint4*>(q));
             } else {
@@ -456,7 +554,22 @@ __global__ void __launch_bounds__(kThreads, 1)
               raw[k] = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
+          t += step_t;
+          hh += step_h;
+          if (hh >= p.group) {
+            hh -= p.group;
+            ++t;
+          }
         }
+      };
+      uint4 raw[4], ahead[4];
+      load(first, ahead);
+#pragma unroll 1
+      for (int n0 = first; n0 < end; n0 += 32) {
+        if ((n0 & (kRows - 1)) == first) kv_warp_wait(kQfree + 8 * (n0 >> 7), qphase, kSiteKvEmpty);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) raw[k] = ahead[k];
+        load(n0 + 32, ahead);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int n = n0 + 8 * k;
@@ -479,19 +592,32 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<uint2*>(to + kKvTileBytes) = make_uint2(l[0], l[1]);
           if (d0 == 0) factors[n] = code == 255u ? NAN : p.scale * 1.4426950408889634f * e8m0_to_float(code);
         }
+        if ((n0 & (kRows - 1)) == first + 96) {  // a tile's last rows
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(kQfull + 8 * (n0 >> 7));
+        }
       }
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(kQfull);
+      if (end == kRows) {  // a second tile without rows
+        kv_warp_wait(kQfree + 8, qphase, kSiteKvEmpty);
+        if (lane == 0) mbar_arrive(kQfull + 8);
+      }
+      qphase ^= 1;
     };
-    if (walk.valid()) queries(walk);
-    for (int it = 0; walk.valid(); ++it) {
+    int it = 0;
+    for (;;) {
+      const Unit& unit = unit_of(ur);
+      const int n = unit.n;
+      if (n <= 0) break;
+      queries(unit);
       // A position that no row sees: its value may be anything, and zero times NaN is NaN.
-      int lo, hi, lo1, hi1;
-      walk.bounds(0, lo, hi);
-      walk.bounds(1, lo1, hi1);
-      const int64_t j = walk.j0() + i;
-      const bool none = j > max(hi, hi1) || (p.window && j <= (int64_t)lo - p.window);
+      const int64_t above = max(unit.hi[0], unit.hi[1]), below = p.window ? (int64_t)unit.lo[0] - p.window : -1;
+      int64_t j = (int64_t)unit.tile * kKvTile + i;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kUfree + 8 * ur.at);
+      ur.next(kUnitStages);
+      for (int tile = 0; tile < n; ++tile, ++it, j += kKvTile) {
+      const bool none = j > above || j <= below;
       kv_warp_wait(kVfull + 8 * vr.at, vr.phase, kSiteKvFull);
       if (it >= 2) kv_warp_wait(kFfree + 8 * fr.at, fr.phase ^ 1, kSiteKvEmpty);
       const uint8_t* from = sm + kAtV + vr.at * kKvTileBytes + i * 128;
@@ -515,76 +641,78 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       vr.next(kVStages);
       fr.next(2);
-      const bool more = walk.last();
-      walk.next();
-      if (more && walk.valid()) queries(walk);
+      }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // -------------------------------------------------------------- softmax
     const int q = warp >> 2, r = threadIdx.x & 127;
     const uint32_t ts = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + q * 128, to_ = ts + 256;
-    KvRing mr;
+    KvRing mr, ur;
     int in_batch = 0;
     uint32_t sphase = 0, ophase = 1;  // ophase: of the last MMAs on the values
     uint32_t qphase = 0;
-    float m = kNone, l = 0.f, cq = 0.f;
-    int lo = 0, hi = -1, place = -1;
-    bool started = false;
-    while (walk.valid()) {
-      if (walk.first) {
-        kv_warp_wait(kQfull, qphase, kSiteKvFull);
-        qphase ^= 1;
-        cq = factors[kRows * q + r];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(kQfree);
-        walk.bounds(q, lo, hi);
-        const int row = kUnitRows * walk.u + kRows * q + r;
-        place = row < walk.rows ? walk.place(row) : -1;
-        m = kNone;
-        l = 0.f;
-        started = false;
-      }
+    for (;;) {
+      const Unit& unit = unit_of(ur);
+      const int n = unit.n;
+      if (n <= 0) break;
+      kv_warp_wait(kQfull + 8 * q, qphase, kSiteKvFull);
+      qphase ^= 1;
+      const float cq = factors[kRows * q + r];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kQfree + 8 * q);
+      const int lo = unit.lo[q], hi = unit.hi[q], row = unit.row0 + kRows * q + r;
+      const int place = row < unit.rows ? unit.place0 + row / p.group : -1;
+      float m = kNone, l = 0.f;
+      bool started = false;
+      for (int tile = unit.tile, left = n; left > 0; ++tile, --left) {
       if (in_batch == 0) kv_warp_wait(kMfull + 8 * mr.at, mr.phase, kSiteKvFull);
       const float4* sc = scales + mr.at * 32 + in_batch * 8;
-      if (walk.sees(lo, hi)) {
+      if (sees(lo, hi, tile, p.window)) {
         kv_warp_wait(kSfull + 8 * q, sphase, kSiteKvFull);
         sphase ^= 1;
         tc::fence_after_sync();
-        uint32_t raw[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) kv_ld<32>(ts + 32 * c, raw[c]);
-        kv_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) kv_tie(raw[c]);
-        const int64_t j0 = walk.j0();
+        const int64_t j0 = (int64_t)tile * kKvTile;
         const bool edge = j0 + kKvTile - 1 > lo || (p.window && j0 <= (int64_t)hi - p.window);
+        // The scores are read from TMEM twice, 64 columns at a time, for the maximum and for the weights: held between, they
+        // would need more registers than 512 threads have. Loops that are not unrolled keep the code in the SM's cache.
         float top = -INFINITY;
+        // Of an edge tile: the last position that the row sees, and the one before the first, in the tile.
+        int high = kKvTile, low = -1;
         if (!edge) {
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t raw[2][32];
+            kv_ld<32>(ts + 64 * c, raw[0]);
+            kv_ld<32>(ts + 64 * c + 32, raw[1]);
+            kv_wait_ld();
+            kv_tie(raw[0]);
+            kv_tie(raw[1]);
 #pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            const float4 v = sc[g];
-            auto s = [&](int k) { return __uint_as_float(raw[g >> 1][16 * (g & 1) + k]); };
-            float a = max3(s(0), s(1), s(2)), b = max3(s(3), s(4), s(5));
-            a = max3(a, s(6), s(7)), b = max3(b, s(8), s(9));
-            a = max3(a, s(10), s(11)), b = max3(b, s(12), s(13));
-            a = max3(a, s(14), s(15));
-            top = fmaxf(top, fmaf(fmaxf(a, b), cq * v.x, v.y));
+            for (int g = 0; g < 4; ++g) {
+              const float4 v = sc[4 * c + g];
+              auto s = [&](int k) { return __uint_as_float(raw[g >> 1][16 * (g & 1) + k]); };
+              float a = max3(s(0), s(1), s(2)), b = max3(s(3), s(4), s(5));
+              a = max3(a, s(6), s(7)), b = max3(b, s(8), s(9));
+              a = max3(a, s(10), s(11)), b = max3(b, s(12), s(13));
+              a = max3(a, s(14), s(15));
+              top = fmaxf(top, fmaf(fmaxf(a, b), cq * v.x, v.y));
+            }
           }
         } else {
-          // x in place of the score, minus infinity where the row does not see.
-          const int high = (int)min((int64_t)kKvTile, place - j0);  // last position of the tile that the row sees
-          const int low = p.window ? (int)max((int64_t)-1, min((int64_t)kKvTile, place - (int64_t)p.window - j0)) : -1;
-#pragma unroll
+          high = (int)min((int64_t)kKvTile, place - j0);
+          if (p.window) low = (int)max((int64_t)-1, min((int64_t)kKvTile, place - (int64_t)p.window - j0));
+#pragma unroll 1
           for (int g = 0; g < 8; ++g) {
+            uint32_t raw[16];
+            kv_ld<16>(ts + 16 * g, raw);
+            kv_wait_ld();
+            kv_tie(raw);
             const float4 v = sc[g];
             const float c = cq * v.x;
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               const int at = 16 * g + k;
-              const float x = at <= high && at > low ? fmaf(__uint_as_float(raw[g >> 1][16 * (g & 1) + k]), c, v.y) : -INFINITY;
-              raw[g >> 1][16 * (g & 1) + k] = __float_as_uint(x);
-              top = fmaxf(top, x);
+              if (at <= high && at > low) top = fmaxf(top, fmaf(__uint_as_float(raw[k]), c, v.y));
             }
           }
         }
@@ -607,27 +735,54 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
+        // The weights replace the scores from the left, half as wide, behind the columns that have been read.
+        if (!edge) {
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t raw[2][32], w[32];
+            kv_ld<32>(ts + 64 * c, raw[0]);
+            kv_ld<32>(ts + 64 * c + 32, raw[1]);
+            kv_wait_ld();
+            kv_tie(raw[0]);
+            kv_tie(raw[1]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[16];
+            for (int g = 0; g < 4; ++g) {
+              const float4 v = sc[4 * c + g];
+              const uint64_t k2 = pack2(cq * v.x, cq * v.x), add2 = pack2(v.y - m, v.y - m);
+              uint64_t sum2 = 0;
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float4 v = sc[2 * c + g];
-            const float k = edge ? 1.f : cq * v.x, add = edge ? -m : v.y - m;
-            float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float a = add, b = add;
-              fma2(a, b, __uint_as_float(raw[c][16 * g + 2 * i]), __uint_as_float(raw[c][16 * g + 2 * i + 1]), k, k);
-              a = ex2(a);
-              b = ex2(b);
-              s0 += a;
-              s1 += b;
-              w[8 * g + i] = f16x2_of(a, b);
+              for (int i = 0; i < 8; ++i) {
+                const int at = 16 * (g & 1) + 2 * i;
+                const uint64_t x = fma_2(pack2(__uint_as_float(raw[g >> 1][at]), __uint_as_float(raw[g >> 1][at + 1])), k2, add2);
+                const uint64_t e = (i & 3) == 3 ? ex2_poly(x) : pack2(ex2(low_of(x)), ex2(high_of(x)));
+                sum2 = add_2(sum2, e);
+                w[8 * g + i] = f16x2_of(low_of(e), high_of(e));
+              }
+              l = fmaf(low_of(sum2) + high_of(sum2), v.z, l);
             }
-            l = fmaf(s0 + s1, v.z, l);
+            tc::st_cols<32>(ts + 32 * c, w);
           }
-          tc::st_cols<16>(ts + 16 * c, w);
+        } else {
+#pragma unroll 1
+          for (int g = 0; g < 8; ++g) {
+            uint32_t raw[16], w[8];
+            kv_ld<16>(ts + 16 * g, raw);
+            kv_wait_ld();
+            kv_tie(raw);
+            const float4 v = sc[g];
+            const float c = cq * v.x, add = v.y - m;
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+              const int at = 16 * g + k;
+              const float a = at <= high && at > low ? ex2(fmaf(__uint_as_float(raw[k]), c, add)) : 0.f;
+              const float b = at + 1 <= high && at + 1 > low ? ex2(fmaf(__uint_as_float(raw[k + 1]), c, add)) : 0.f;
+              sum += a + b;
+              w[k >> 1] = f16x2_of(a, b);
+            }
+            l = fmaf(sum, v.z, l);
+            tc::st_x8(ts + 8 * g, w);
+          }
         }
         tc::wait_st();
         tc::fence_before_sync();
@@ -643,16 +798,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         mr.next(2);
       }
 
-      if (walk.last() && kUnitRows * walk.u + kRows * q < walk.rows) {
+      }
+
+      if (unit.has(q)) {
         // The unit's end, or this CTA's part of it.
         if (started) {
           kv_warp_wait(kOdone + 8 * q, ophase, kSiteKvFull);
           tc::fence_after_sync();
         }
-        const int unit0 = walk.x - walk.t, unit1 = unit0 + walk.tiles - 1;  // the unit's tiles
-        const int row = kUnitRows * walk.u + kRows * q + r, t = row / p.group;
-        const bool valid = row < walk.rows;
-        const int64_t token = walk.first_token + t, head = walk.h * p.group + row - t * p.group;
+        const int t = row / p.group;
+        const bool valid = row < unit.rows;
+        const int64_t token = unit.token + t, head = unit.h * p.group + row - t * p.group;
         uint16_t* out = p.out + token * p.os_t + head * p.os_h;
         const bool vec = (uintptr_t)p.out % 16 == 0 && p.os_t % 8 == 0 && p.os_h % 8 == 0;
         auto store = [&](int d, const float (&v)[16]) {  // 16 dimensions of the thread's row
@@ -675,8 +831,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (valid && p.lse)
             p.lse[token * p.ls_t + head * p.ls_h] = all == 0.f ? -INFINITY : (top + log2f(all)) * 0.6931471805599453f;
         };
-        const bool whole = unit0 >= x0 && unit1 < x1;
-        const int cta0 = whole ? 0 : kv_owner(unit0, total, ctas), cta1 = whole ? 0 : kv_owner(unit1, total, ctas);
+        const bool whole = n == unit.tiles;
+        const int cta0 = whole ? 0 : kv_owner(unit.x, total, ctas);
+        const int cta1 = whole ? 0 : kv_owner(unit.x + unit.tiles - 1, total, ctas);
         auto part = [&](int cta) { return partials + ((int64_t)(cta * 2 + (cta == cta0)) * 2 + q) * kPart; };
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
@@ -752,7 +909,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           kv_bar_sync(1 + q, 128);  // before the flag is used again
         }
       }
-      walk.next();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kUfree + 8 * ur.at);
+      ur.next(kUnitStages);
     }
   }
   __syncwarp();
@@ -772,11 +931,6 @@ cudaError_t launch_kv_prompt(const KvAttentionCall& p, const CUtensorMap& k, con
   const cudaError_t e = ensure_smem_attribute(kernel, kSmem);
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(sms), dim3(kThreads), kSmem, stream, p, k, v, partials, counters);
-}
-
-cudaError_t kv_prompt_status_symbols(void** status, void** limit) {
-  const cudaError_t e = cudaGetSymbolAddress(status, g_device_status);
-  return e != cudaSuccess ? e : cudaGetSymbolAddress(limit, g_wait_limit_ns);
 }
 
 }  // namespace mambo
