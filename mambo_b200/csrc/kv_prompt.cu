@@ -24,8 +24,8 @@
 // several CTAs share is joined by the last to arrive, in the order of the
 // positions.
 //
-// Warps 0-3 and 4-7 softmax of either tile, 8-11 queries and values, 12 copies, 13 MMA, 14 the pages' scales, 15 the
-// units to come, which it describes to the others.
+// Warps 0-3 and 4-7 softmax of either tile, and its queries; 8-11 values; 12 copies and the units to come, which it
+// describes to the others; 13 and 14 the MMAs of either tile; 15 the pages' scales.
 #include "iq3s_tm.cuh"
 #include "kernels.cuh"
 #include "kv_tc.cuh"
@@ -46,28 +46,25 @@ constexpr int kUnitCost = 2;
 // Shared memory: queries [2 tiles][hi, lo][128][128], keys, values as they come and in f16 [2 halves of D][128][128 bytes].
 constexpr uint32_t kQ = 4 * kKvTileBytes, kVf = 2 * kKvTileBytes;
 constexpr uint32_t kAtK = kQ, kAtV = kAtK + kKStages * kKvTileBytes, kAtVf = kAtV + kVStages * kKvTileBytes;
-constexpr uint32_t kAtFactors = kAtVf + 2 * kVf, kAtScales = kAtFactors + kUnitRows * 4, kAtUnits = kAtScales + 2 * 32 * 16;
+constexpr uint32_t kAtScales = kAtVf + 2 * kVf, kAtUnits = kAtScales + 2 * 32 * 16;
 constexpr int kUnitStages = 4;
-constexpr uint32_t kAtBegin = kAtUnits + (kUnitStages + 1) * 64, kAtBars = kAtBegin + 128;
+constexpr uint32_t kAtBegin = kAtUnits + (kUnitStages + 1) * 96, kAtBars = kAtBegin + 128;
 constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 4 + 8 + 4 + 4 + 2 * kUnitStages;
 constexpr uint32_t kSmem = 1024 + kAtBars + kNumBars * 8 + 16;
 constexpr int kPart = kRows * 130;    // floats of a tile's part: O [32][128][4], m, l
 
 // A CTA's part of a unit, as one warp works it out and the others read it.
-struct alignas(64) Unit {
+struct alignas(16) Unit {
   int tile, n;        // tiles [tile, tile + n) of the sequence's positions; n == 0: there is no further unit
   int b, h;           // sequence, key head
   int row0, rows;     // the unit's first row, all rows of the sequence
   int token, place0;  // the sequence's first token and its position
-  int lo[2], hi[2];   // positions of the first and last rows of either tile of rows; hi < lo: it has no rows
+  int lo[2], hi[2];   // positions of the first and last rows of either tile of rows
+  int from[2], to[2]; // tiles that any of them sees: [from, to)
   int x, tiles;       // the unit's tiles in the work: [x, x + tiles); this part is all of it where n == tiles
   __device__ __forceinline__ bool has(int q) const { return row0 + kRows * q < rows; }
 };
-// Whether rows at the positions lo .. hi see any of the 128 positions from tile j on: the MMA and the softmax go by it.
-__device__ __forceinline__ bool sees(int lo, int hi, int j, int window) {
-  const int64_t j0 = (int64_t)j * kKvTile;
-  return j0 <= hi && (window == 0 || j0 + kKvTile - 1 > (int64_t)lo - window);
-}
+static_assert(sizeof(Unit) <= 96, "shared memory");
 
 // The units of a call: sequence b, key head h, unit u of `units` of that head.
 struct Plan {
@@ -205,7 +202,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                      const __grid_constant__ CUtensorMap vmap, float* partials, int* counters) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float* factors = reinterpret_cast<float*>(sm + kAtFactors);   // of the unit's rows
   float4* scales = reinterpret_cast<float4*>(sm + kAtScales);   // [2][4 tiles][8]: key factor, value exponent, 2^-exponent
   Unit* units = reinterpret_cast<Unit*>(sm + kAtUnits);         // [kUnitStages], and an empty one
   int* begin = reinterpret_cast<int*>(sm + kAtBegin);           // where the share begins: sequence, head, unit, place in its work; [8] flags
@@ -223,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kKStages; ++s) {
       mbar_init(kKfull + 8 * s, 1);
-      mbar_init(kKfree + 8 * s, 1);
+      mbar_init(kKfree + 8 * s, 2);
     }
     for (int s = 0; s < kVStages; ++s) {
       mbar_init(kVfull + 8 * s, 1);
@@ -231,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(kFfull + 8 * i, 4);
-      mbar_init(kFfree + 8 * i, 1);
+      mbar_init(kFfree + 8 * i, 2);
       mbar_init(kSfull + 8 * i, 1);
       mbar_init(kWfull + 8 * i, 4);
       mbar_init(kOdone + 8 * i, 1);
@@ -241,12 +237,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kUnitStages; ++i) {
       mbar_init(kUfull + 8 * i, 1);
-      mbar_init(kUfree + 8 * i, 15);  // copies, MMA, scales, 4 warps of values, 8 of the softmax
+      mbar_init(kUfree + 8 * i, 15);  // MMAs, scales, 4 warps of values, 8 of the softmax
     }
     units[kUnitStages] = Unit{};
     for (int i = 0; i < 2; ++i) {
       mbar_init(kQfull + 8 * i, 4);
-      mbar_init(kQfree + 8 * i, 5);  // the MMAs and the tile's softmax warps
+      mbar_init(kQfree + 8 * i, 1);
     }
     fence_barrier_init();
   }
@@ -326,16 +322,59 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp >= 12) {
     if (warp == 12) {
-      // ------------------------------------------------------------ copies
+      // ------------------------------------------------------------ copies, and the units
       KvRing kr, vr, ur;
       const uint64_t policy = l2_policy_evict_last();
       bool ok = true;
-      for (int it = 0; ok;) {
-        const Unit& unit = unit_of(ur);
-        const int n = unit.n, h = unit.h;
-        if (n <= 0) break;
-        const int64_t i0 = (int64_t)unit.tile * per_tile + lane;
-        const int* row_pages = p.seq.table + unit.b * p.seq.table_stride + i0;
+      plan.b = begin[0];
+      plan.h = begin[1];
+      plan.u = begin[2];
+      if (x0 < x1) plan.sequence();
+      int x = x0, at = begin[3];  // place in the work, and in the unit's
+      int count = 0;
+      // The next unit of this CTA's share (one with n == 0 behind the last), told to the others.
+      auto unit_ahead = [&]() {
+        Unit u{};
+        if (x < x1) {
+          u.tiles = plan.tiles_of(plan.u, u.tile);
+          const int t = max(at - kUnitCost, 0), left = x1 - x - max(kUnitCost - at, 0);
+          u.x = x - at + kUnitCost;
+          u.n = max(min(u.tiles - t, left), 0);  // of the last unit only the work besides its tiles may fall to this CTA
+          x = u.x + u.tiles;
+          at = 0;
+          u.tile += t;
+          u.b = plan.b;
+          u.h = plan.h;
+          u.row0 = kUnitRows * plan.u;
+          u.rows = plan.rows;
+          u.token = plan.token;
+          u.place0 = plan.place0;
+          for (int q = 0; q < 2; ++q) {
+            if (!u.has(q)) continue;
+            u.lo[q] = plan.place(u.row0 + kRows * q);
+            u.hi[q] = plan.place(u.row0 + kRows * q + kRows - 1);
+            const int64_t low = p.window ? u.lo[q] + 1 - (int64_t)p.window : 0;
+            u.from[q] = low > 0 ? (int)(low / kKvTile) : 0;
+            u.to[q] = u.hi[q] >= 0 ? u.hi[q] / kKvTile + 1 : 0;
+          }
+          if (x < x1) plan.next();
+        }
+        if (count >= kUnitStages && !(ok = kv_warp_wait(kUfree + 8 * ur.at, ur.phase ^ 1, kSiteKvEmpty))) u.n = 0;
+        if (lane == 0) {
+          units[ur.at] = u;
+          mbar_arrive(kUfull + 8 * ur.at);
+        }
+        ur.next(kUnitStages);
+        ++count;
+        return u;
+      };
+      Unit ahead = unit_ahead();
+      for (int it = 0; ok && ahead.n > 0;) {
+        const Unit u = ahead;
+        ahead = unit_ahead();
+        const int n = u.n, h = u.h;
+        const int64_t i0 = (int64_t)u.tile * per_tile + lane;
+        const int* row_pages = p.seq.table + u.b * p.seq.table_stride + i0;
         auto page_of = [&](int t) {
           return t < n && lane < per_tile && i0 + t * per_tile < p.seq.table_pages ? __ldg(row_pages + t * per_tile) : -1;
         };
@@ -358,89 +397,88 @@ __global__ void __launch_bounds__(kThreads, 1)
           kr.next(kKStages);
           vr.next(kVStages);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(kUfree + 8 * ur.at);
-        ur.next(kUnitStages);
       }
       if (!ok) kv_settle();
-    } else if (warp == 13) {
-      // ------------------------------------------------------------ MMA
+    } else if (warp < 15) {
+      // ------------------------------------------------------------ MMA: a thread for each tile of rows. A tile's weights
+      // lie over its scores, and its next scores over them: in the order in which they are issued.
       if (tm::elect_one()) {
+        const int q = warp - 13;
         const uint32_t idesc_o = tc::idesc_f16_f32(kRows, p.cache.dim) | kIdescAlongN;
         const bool wide = p.cache.dim > 64;
-        const uint32_t q0 = desc_low(sm0, 16), k0 = desc_low(sm0 + kAtK, 16), v0 = desc_low(sm0 + kAtVf, kKvTileBytes);
-        // The unit and tile whose values come next (cur), and whose scores do (one tile ahead of it).
-        struct Cursor {
-          int tile, left, lo0, hi0, lo1, hi1;
-          __device__ __forceinline__ void load(const Unit& u) {
-            tile = u.tile;
-            left = u.n;
-            lo0 = u.lo[0], hi0 = u.hi[0], lo1 = u.lo[1], hi1 = u.hi[1];
-          }
-          __device__ __forceinline__ bool sees(int q, int window) const {
-            return q ? mambo::sees(lo1, hi1, tile, window) : mambo::sees(lo0, hi0, tile, window);
-          }
-        } cur, ahead;
-        KvRing kr, fr, cu, au;
-        uint32_t qphase = 0, wphase0 = 0, wphase1 = 0, ophase0 = 1, ophase1 = 1;
-        bool ok = true, started0 = false, started1 = false, begins = true;  // begins: ahead is at a unit's first tile
-        auto scores = [&](int q) {
-          if (begins && !kv_wait(kQfull + 8 * q, qphase, kSiteKvFull)) return false;
-          if (q == 0 && !kv_wait(kKfull + 8 * kr.at, kr.phase, kSiteKvFull)) return false;
-          tc::fence_after_sync();
-          if (ahead.sees(q, p.window))
-            mma_scores(tmem + q * 128, q0 + q * (2 * kKvTileBytes >> 4), k0 + kr.at * (kKvTileBytes >> 4), wide, kSfull + 8 * q);
-          if (ahead.left == 1) tc::commit(kQfree + 8 * q);
-          if (q == 1) {
-            tc::commit(kKfree + 8 * kr.at);
-            kr.next(kKStages);
-            ++ahead.tile;
-            qphase ^= begins;
-            begins = --ahead.left == 0;
-            if (begins) {
-              au.next(kUnitStages);
-              ahead.load(unit_of(au));
-            }
-          }
-          return true;
+        const uint32_t ds = tmem + q * 128, dout = ds + 256, a = desc_low(sm0 + q * 2 * kKvTileBytes, 16);
+        const uint32_t k0 = desc_low(sm0 + kAtK, 16), v0 = desc_low(sm0 + kAtVf, kKvTileBytes);
+        const uint32_t sfull = kSfull + 8 * q, wfull = kWfull + 8 * q, odone = kOdone + 8 * q, ofree = kOfree + 8 * q;
+        const uint32_t qfull = kQfull + 8 * q, qfree = kQfree + 8 * q;
+        KvRing kr, fr, ur;
+        uint32_t qphase = 0, wphase = 0, ophase = 1;
+        // The tile whose scores come next, one ahead of the tile whose values do: the unit's tiles left, and those that
+        // these rows see.
+        int tile = 0, left = 0, from = 0, to = 0;
+        bool begins = true;  // at a unit's first tile
+        auto enter = [&]() {
+          const Unit& u = unit_of(ur);
+          tile = u.tile;
+          left = u.n;
+          from = u.from[q];
+          to = u.to[q];
+          if (left > 0) mbar_arrive(kUfree + 8 * ur.at);
+          ur.next(kUnitStages);
+          begins = true;
         };
-        auto values = [&](int q, uint32_t& wphase, uint32_t ophase, bool& started) {
-          if (!cur.sees(q, p.window)) return true;
-          if (!kv_wait(kWfull + 8 * q, wphase, kSiteKvFull)) return false;
-          wphase ^= 1;
-          // The softmax has read the last unit's O.
-          if (!started && !kv_wait(kOfree + 8 * q, ophase, kSiteKvEmpty)) return false;
-          tc::fence_after_sync();
-          mma_values(tmem + 256 + q * 128, tmem + q * 128, v0 + fr.at * (kVf >> 4), idesc_o, started, kOdone + 8 * q);
-          started = true;
-          return true;
+        bool ok = true;
+        auto scores = [&]() {  // whether these rows see the tile
+          if (begins) {
+            ok = kv_wait(qfull, qphase, kSiteKvFull);
+            qphase ^= 1;
+            begins = false;
+          }
+          const bool seen = tile >= from && tile < to;
+          ok = ok && kv_wait(kKfull + 8 * kr.at, kr.phase, kSiteKvFull);
+          if (ok && seen) {
+            tc::fence_after_sync();
+            mma_scores(ds, a, k0 + kr.at * (kKvTileBytes >> 4), wide, sfull);
+          }
+          tc::commit(kKfree + 8 * kr.at);
+          kr.next(kKStages);
+          ++tile;
+          if (--left == 0) {
+            tc::commit(qfree);
+            enter();
+          }
+          return seen;
         };
-        ahead.load(unit_of(au));
-        cur = ahead;
-        if (cur.left > 0) ok = scores(0) && scores(1);
-        while (ok && cur.left > 0) {
+        enter();
+        bool started = false, ends = left == 1, some = left > 0, seen = some && scores();
+        while (ok && some) {
+          // The tile's values; the next tile's scores follow at once, unless its queries are still on their way.
+          const bool last = ends, go = seen;
           ok = kv_wait(kFfull + 8 * fr.at, fr.phase, kSiteKvFull);
-          if (!ok) break;
-          // The next unit's queries may still be on their way: both tiles' values come first then.
-          const bool more = ahead.left > 0, turn = begins;
-          ok = values(0, wphase0, ophase0, started0) && (!more || turn || scores(0)) &&
-               values(1, wphase1, ophase1, started1) && (!more || !turn || scores(0)) && (!more || scores(1));
+          if (ok && go) {
+            ok = kv_wait(wfull, wphase, kSiteKvFull);
+            wphase ^= 1;
+            // The softmax has read the last unit's O.
+            if (ok && !started) {
+              ok = kv_wait(ofree, ophase, kSiteKvEmpty);
+              ophase ^= 1;
+            }
+            if (ok) {
+              tc::fence_after_sync();
+              mma_values(dout, ds, v0 + fr.at * (kVf >> 4), idesc_o, started, odone);
+            }
+            started = true;
+          }
           if (!ok) break;
           tc::commit(kFfree + 8 * fr.at);
           fr.next(2);
-          ++cur.tile;
-          if (--cur.left == 0) {
-            ophase0 ^= started0;
-            ophase1 ^= started1;
-            started0 = started1 = false;
-            mbar_arrive(kUfree + 8 * cu.at);
-            cu.next(kUnitStages);
-            cur.load(unit_of(cu));
-          }
+          if (last) started = false;
+          some = left > 0;
+          ends = left == 1;
+          if (some) seen = scores();
         }
         if (!ok) kv_settle();
       }
-    } else if (warp == 14) {
+    } else {
       // ------------------------------------------------------------ scales: four tiles at a time, 16 positions a lane
       KvRing ring, ur;
       int step = 0, fill = 0;  // tiles in the current batch
@@ -485,133 +523,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (fill) publish();
-    } else if (lane == 0) {
-      // ------------------------------------------------------------ units
-      KvRing ur;
-      plan.b = begin[0];
-      plan.h = begin[1];
-      plan.u = begin[2];
-      if (x0 < x1) plan.sequence();
-      int x = x0, at = begin[3];  // place in the work, and in the unit's
-      for (int it = 0;;) {
-        Unit u{};
-        if (x < x1) {
-          u.tiles = plan.tiles_of(plan.u, u.tile);
-          const int t = max(at - kUnitCost, 0), left = x1 - x - max(kUnitCost - at, 0);
-          u.x = x - at + kUnitCost;
-          u.n = max(min(u.tiles - t, left), 0);
-          x = u.x + u.tiles;
-          at = 0;
-          u.tile += t;
-          u.b = plan.b;
-          u.h = plan.h;
-          u.row0 = kUnitRows * plan.u;
-          u.rows = plan.rows;
-          u.token = plan.token;
-          u.place0 = plan.place0;
-          for (int q = 0; q < 2; ++q) {
-            const bool has_rows = u.row0 + kRows * q < plan.rows;
-            u.lo[q] = has_rows ? plan.place(u.row0 + kRows * q) : 0;
-            u.hi[q] = has_rows ? plan.place(u.row0 + kRows * q + kRows - 1) : -1;
-          }
-          if (x < x1) plan.next();
-        }
-        if (it >= kUnitStages && !kv_wait(kUfree + 8 * ur.at, ur.phase ^ 1, kSiteKvEmpty)) u.n = 0;
-        units[ur.at] = u;
-        mbar_arrive(kUfull + 8 * ur.at);
-        ur.next(kUnitStages);
-        if (u.n == 0) break;  // of the last unit only the work besides its tiles may fall to this CTA
-        ++it;
-      }
     }
   } else if (warp >= 8) {
-    // -------------------------------------------------------------- queries and values
+    // -------------------------------------------------------------- values
     const int i = threadIdx.x - 256;  // position of the tile
-    const bool vec = (uintptr_t)p.q % 16 == 0 && p.qs_t % 8 == 0 && p.qs_h % 8 == 0;
     KvRing vr, fr, ur;
-    uint32_t qphase = 1;  // a fresh barrier's previous phase counts as over
-    // Rows 8 apart: tokens and query heads on.
-    const int step_t = 8 / p.group, step_h = 8 % p.group;
-    // A half warp a row, eight dimensions a lane; the next four rows are loaded while four are split.
-    auto queries = [&](const Unit& u) {
-      const int d0 = 8 * (lane & 15), first = 2 * (warp - 8) + (lane >> 4);
-      const int rows = d0 < p.cache.dim ? min(kUnitRows, u.rows - u.row0) : 0;
-      const int end = u.has(1) ? kUnitRows : kRows;
-      int t = (u.row0 + first) / p.group, hh = u.row0 + first - t * p.group;
-      const uint16_t* q0 = p.q + (int64_t)u.token * p.qs_t + (int64_t)u.h * p.group * p.qs_h + d0;
-      auto load = [&](int n0, uint4 (&raw)[4]) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          raw[k] = make_uint4(0, 0, 0, 0);
-          if (n0 + 8 * k < rows) {
-            const uint16_t* q = q0 + t * p.qs_t + hh * p.qs_h;
-            if (vec) {
-              raw[k] = __ldg(reinterpret_cast<const uint4*>(q));
-            } else {
-              uint32_t v[4];
-#pragma unroll
-              for (int c = 0; c < 4; ++c) v[c] = (uint32_t)__ldg(q + 2 * c) | (uint32_t)__ldg(q + 2 * c + 1) << 16;
-              raw[k] = make_uint4(v[0], v[1], v[2], v[3]);
-            }
-          }
-          t += step_t;
-          hh += step_h;
-          if (hh >= p.group) {
-            hh -= p.group;
-            ++t;
-          }
-        }
-      };
-      uint4 raw[4], ahead[4];
-      load(first, ahead);
-#pragma unroll 1
-      for (int n0 = first; n0 < end; n0 += 32) {
-        if ((n0 & (kRows - 1)) == first) kv_warp_wait(kQfree + 8 * (n0 >> 7), qphase, kSiteKvEmpty);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) raw[k] = ahead[k];
-        load(n0 + 32, ahead);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int n = n0 + 8 * k;
-          const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-          uint32_t top = absmax_bf16x2(absmax_bf16x2(v[0], v[1]), absmax_bf16x2(v[2], v[3]));
-#pragma unroll
-          for (int o = 8; o; o >>= 1) top = absmax_bf16x2(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-          const uint32_t code = mxfp8_scale_code(__uint_as_float(max(top & 0x7FFFu, (top >> 16) & 0x7FFFu) << 16));
-          const float inv = code == 255u ? 0.f : e8m0_to_float(254u - code);
-          uint32_t h[2], l[2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float e[4] = {__uint_as_float(v[2 * c] << 16) * inv, __uint_as_float(v[2 * c] & 0xFFFF0000u) * inv,
-                                __uint_as_float(v[2 * c + 1] << 16) * inv, __uint_as_float(v[2 * c + 1] & 0xFFFF0000u) * inv};
-            split_e4m3x4(e, h[c], l[c]);
-            if (code == 255u) h[c] = l[c] = 0u;
-          }
-          uint8_t* to = sm + (n >> 7) * 2 * kKvTileBytes + (n & 127) * 128 + (((lane & 15) >> 1 ^ (n & 7)) << 4) + (lane & 1) * 8;
-          *reinterpret_cast<uint2*>(to) = make_uint2(h[0], h[1]);
-          *reinterpret_cast<uint2*>(to + kKvTileBytes) = make_uint2(l[0], l[1]);
-          if (d0 == 0) factors[n] = code == 255u ? NAN : p.scale * 1.4426950408889634f * e8m0_to_float(code);
-        }
-        if ((n0 & (kRows - 1)) == first + 96) {  // a tile's last rows
-          fence_proxy_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(kQfull + 8 * (n0 >> 7));
-        }
-      }
-      if (end == kRows) {  // a second tile without rows
-        kv_warp_wait(kQfree + 8, qphase, kSiteKvEmpty);
-        if (lane == 0) mbar_arrive(kQfull + 8);
-      }
-      qphase ^= 1;
-    };
     int it = 0;
     for (;;) {
       const Unit& unit = unit_of(ur);
       const int n = unit.n;
       if (n <= 0) break;
-      queries(unit);
       // A position that no row sees: its value may be anything, and zero times NaN is NaN.
-      const int64_t above = max(unit.hi[0], unit.hi[1]), below = p.window ? (int64_t)unit.lo[0] - p.window : -1;
+      const int64_t above = unit.has(1) ? unit.hi[1] : unit.hi[0], below = p.window ? (int64_t)unit.lo[0] - p.window : -1;
       int64_t j = (int64_t)unit.tile * kKvTile + i;
       __syncwarp();
       if (lane == 0) mbar_arrive(kUfree + 8 * ur.at);
@@ -651,15 +574,64 @@ __global__ void __launch_bounds__(kThreads, 1)
     int in_batch = 0;
     uint32_t sphase = 0, ophase = 1;  // ophase: of the last MMAs on the values
     uint32_t qphase = 0;
+    // This thread's row of the unit's queries, split into two terms, to shared memory; its factor of the scores.
+    const bool qvec = (uintptr_t)p.q % 16 == 0 && p.qs_t % 8 == 0 && p.qs_h % 8 == 0;
+    auto queries = [&](const Unit& u) {
+      const int row = u.row0 + kRows * q + r, t = row / p.group;
+      const uint16_t* from = p.q + (int64_t)(u.token + t) * p.qs_t + (int64_t)(u.h * p.group + row - t * p.group) * p.qs_h;
+      const int dims = row < u.rows ? p.cache.dim : 0;
+      uint4 raw[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        raw[c] = make_uint4(0, 0, 0, 0);
+        if (8 * c < dims) {
+          if (qvec) {
+            raw[c] = __ldg(reinterpret_cast<const uint4*>(from) + c);
+          } else {
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = (uint32_t)__ldg(from + 8 * c + 2 * k) | (uint32_t)__ldg(from + 8 * c + 2 * k + 1) << 16;
+            raw[c] = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        top = absmax_bf16x2(top, absmax_bf16x2(absmax_bf16x2(raw[c].x, raw[c].y), absmax_bf16x2(raw[c].z, raw[c].w)));
+      const uint32_t code = mxfp8_scale_code(__uint_as_float(max(top & 0x7FFFu, (top >> 16) & 0x7FFFu) << 16));
+      const float inv = code == 255u ? 0.f : e8m0_to_float(254u - code);
+      uint8_t* to = sm + q * 2 * kKvTileBytes + r * 128;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const uint32_t v[8] = {raw[2 * c].x, raw[2 * c].y, raw[2 * c].z, raw[2 * c].w,
+                               raw[2 * c + 1].x, raw[2 * c + 1].y, raw[2 * c + 1].z, raw[2 * c + 1].w};
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // 8 significant bits up to 448: exact in f16 (down to 2^-17), and so is what the first term leaves.
+          const uint32_t e0 = f16x2_of(__uint_as_float(v[2 * k] << 16) * inv, __uint_as_float(v[2 * k] & 0xFFFF0000u) * inv);
+          const uint32_t e1 = f16x2_of(__uint_as_float(v[2 * k + 1] << 16) * inv, __uint_as_float(v[2 * k + 1] & 0xFFFF0000u) * inv);
+          const uint32_t h0 = e4m3x2_of_f16x2(e0), h1 = e4m3x2_of_f16x2(e1);
+          h[k] = h0 | (h1 << 16);
+          l[k] = e4m3x2_of_f16x2(sub_f16x2(e0, f16x2_of_e4m3x2(h0))) | (e4m3x2_of_f16x2(sub_f16x2(e1, f16x2_of_e4m3x2(h1))) << 16);
+          if (code == 255u) h[k] = l[k] = 0u;
+        }
+        *reinterpret_cast<uint4*>(to + ((c ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(to + kKvTileBytes + ((c ^ (r & 7)) << 4)) = make_uint4(l[0], l[1], l[2], l[3]);
+      }
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kQfull + 8 * q);
+      return code == 255u ? NAN : p.scale * 1.4426950408889634f * e8m0_to_float(code);
+    };
+    float cq = 0.f;
+    if (unit_of(ur).n > 0) cq = queries(unit_of(ur));
     for (;;) {
       const Unit& unit = unit_of(ur);
       const int n = unit.n;
       if (n <= 0) break;
-      kv_warp_wait(kQfull + 8 * q, qphase, kSiteKvFull);
-      qphase ^= 1;
-      const float cq = factors[kRows * q + r];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(kQfree + 8 * q);
+      const int from = unit.from[q], end = unit.to[q];
       const int lo = unit.lo[q], hi = unit.hi[q], row = unit.row0 + kRows * q + r;
       const int place = row < unit.rows ? unit.place0 + row / p.group : -1;
       float m = kNone, l = 0.f;
@@ -667,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int tile = unit.tile, left = n; left > 0; ++tile, --left) {
       if (in_batch == 0) kv_warp_wait(kMfull + 8 * mr.at, mr.phase, kSiteKvFull);
       const float4* sc = scales + mr.at * 32 + in_batch * 8;
-      if (sees(lo, hi, tile, p.window)) {
+      if (tile >= from && tile < end) {
         kv_warp_wait(kSfull + 8 * q, sphase, kSiteKvFull);
         sphase ^= 1;
         tc::fence_after_sync();
@@ -800,6 +772,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 
       }
 
+      // The next unit's queries, before this one's results are waited for.
+      KvRing after = ur;
+      after.next(kUnitStages);
+      const Unit& next = unit_of(after);
+      float next_cq = 0.f;
+      if (next.n > 0) {
+        kv_warp_wait(kQfree + 8 * q, qphase, kSiteKvEmpty);
+        qphase ^= 1;
+        next_cq = queries(next);
+      }
       if (unit.has(q)) {
         // The unit's end, or this CTA's part of it.
         if (started) {
@@ -912,6 +894,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(kUfree + 8 * ur.at);
       ur.next(kUnitStages);
+      cq = next_cq;
     }
   }
   __syncwarp();
