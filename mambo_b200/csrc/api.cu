@@ -8,6 +8,7 @@
 #include <string>
 
 #include "fp8b.cuh"
+#include "kv.cuh"
 #include "kernels.cuh"
 
 namespace mambo {
@@ -669,30 +670,34 @@ int mambo_device_status(int reset, int* code, int* where, int* block) {
   DeviceStatus st{};
   cudaError_t e = cudaMemcpyFromSymbol(&st, g_device_status, sizeof(st));
   if (e != cudaSuccess) return cuda_fail(e, "reading the device status");
-  // The FP8 block product is a program of its own with its own record.
-  void *fb_status = nullptr, *fb_limit = nullptr;
-  e = fb_status_symbols(&fb_status, &fb_limit);
-  DeviceStatus fb{};
-  if (e == cudaSuccess) e = cudaMemcpy(&fb, fb_status, sizeof(fb), cudaMemcpyDeviceToHost);
+  // The FP8 block product and the prompt attention are programs of their own with their own records.
+  void *status[2] = {}, *limit = nullptr;
+  e = fb_status_symbols(&status[0], &limit);
+  if (e == cudaSuccess) e = kv_prompt_status_symbols(&status[1], &limit);
+  for (int i = 0; i < 2 && e == cudaSuccess; ++i) {
+    DeviceStatus own{};
+    e = cudaMemcpy(&own, status[i], sizeof(own), cudaMemcpyDeviceToHost);
+    if (st.code == 0) st = own;
+  }
   if (e != cudaSuccess) return cuda_fail(e, "reading the device status");
-  if (st.code == 0) st = fb;
   if (code) *code = st.code;
   if (where) *where = st.where;
   if (block) *block = st.block;
   if (reset) {
     DeviceStatus zero{};
     e = cudaMemcpyToSymbol(g_device_status, &zero, sizeof(zero));
-    if (e == cudaSuccess) e = cudaMemcpy(fb_status, &zero, sizeof(zero), cudaMemcpyHostToDevice);
+    for (int i = 0; i < 2 && e == cudaSuccess; ++i) e = cudaMemcpy(status[i], &zero, sizeof(zero), cudaMemcpyHostToDevice);
     if (e != cudaSuccess) return cuda_fail(e, "resetting the device status");
   }
   return ok();
 }
 
 int mambo_set_wait_limit_ns(unsigned long long ns) {
-  void *fb_status = nullptr, *fb_limit = nullptr;
+  void *status = nullptr, *limit[2] = {};
   cudaError_t e = cudaMemcpyToSymbol(g_wait_limit_ns, &ns, sizeof(ns));
-  if (e == cudaSuccess) e = fb_status_symbols(&fb_status, &fb_limit);
-  if (e == cudaSuccess) e = cudaMemcpy(fb_limit, &ns, sizeof(ns), cudaMemcpyHostToDevice);
+  if (e == cudaSuccess) e = fb_status_symbols(&status, &limit[0]);
+  if (e == cudaSuccess) e = kv_prompt_status_symbols(&status, &limit[1]);
+  for (int i = 0; i < 2 && e == cudaSuccess; ++i) e = cudaMemcpy(limit[i], &ns, sizeof(ns), cudaMemcpyHostToDevice);
   if (e != cudaSuccess) return cuda_fail(e, "setting the wait limit");
   return ok();
 }

@@ -162,7 +162,9 @@ int mambo_kv_attention(const void* q, int64_t q_stride_token, int64_t q_stride_h
   if (heads < 1 || heads > kMaxHeads || heads % cache->kv_heads)
     return api_fail(MAMBO_EINVAL, "query heads must be a multiple of the cache's heads, at most %d", (int)kMaxHeads);
   if (window < 0) return api_fail(MAMBO_EINVAL, "the window must not be negative");
-  if (!aligned(q, 2) || !aligned(out, 2) || !aligned(lse, 4)) return api_fail(MAMBO_EINVAL, kUnaligned);
+  if (!aligned(lse, 4)) return api_fail(MAMBO_EINVAL, kUnaligned);
+  if (!aligned(q, 16) || !aligned(out, 16) || q_stride_token % 8 || q_stride_head % 8 || out_stride_token % 8 || out_stride_head % 8)
+    return api_fail(MAMBO_EINVAL, "the heads of q and out must be 16-byte aligned");
   // Rows, and tiles of 128 positions over all sequences, heads and units of rows, are counted in 32 bits.
   const int64_t group = heads / cache->kv_heads;
   const double units = (double)tokens * group / 256 + (double)seq->batch;

@@ -94,6 +94,8 @@ cudaError_t launch_kv_decode(const KvAttentionCall& p, const CUtensorMap& k, con
 size_t kv_prompt_partial_bytes(int sms);
 cudaError_t launch_kv_prompt(const KvAttentionCall& p, const CUtensorMap& k, const CUtensorMap& v, int sms, float* partials,
                              int* counters, cudaStream_t stream);
+// Device addresses of the prompt kernel's status record and wait limit (the current device's).
+cudaError_t kv_prompt_status_symbols(void** status, void** limit);
 
 #ifdef __CUDACC__
 // The call's tokens of sequence b: [first, first + count), clamped to the call.

@@ -330,7 +330,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
     // -------------------------------------------------------------- queries
     KvRing ring;
     bool ok = true;
-    const bool vec = (uintptr_t)p.q % 16 == 0 && p.qs_t % 8 == 0 && p.qs_h % 8 == 0;
     const int half = lane >> 4, d0 = 8 * (lane & 15);  // two rows at a time, 8 dimensions a lane
     for (int unit = 0; walk.valid(); ++unit) {
       const KvSpan span = kv_span(p.seq, walk.b);
@@ -356,14 +355,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
           if (n < rows && d0 < p.cache.dim) {
             const int2 own = owners[ring.at * N + n];
             const uint16_t* q = p.q + own.x * p.qs_t + own.y * p.qs_h + d0;
-            if (vec) {
-              raw[i] = __ldg(reinterpret_cast<const uint4*>(q));
-            } else {
-              uint32_t w[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) w[k] = (uint32_t)__ldg(q + 2 * k) | (uint32_t)__ldg(q + 2 * k + 1) << 16;
-              raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            raw[i] = __ldg(reinterpret_cast<const uint4*>(q));
           }
         }
 #pragma unroll

@@ -14,8 +14,9 @@
 //
 // A softmax thread has a row: no reductions over lanes. As in the decode kernel
 // x = score * log2(e) + exponent of the position's value scale, w = 2^(x - m),
-// l += w * 2^-exponent, and m moves (O is rescaled) only when a weight would
-// pass 2^8. What paces the kernel: the tensor core (2048 clocks for both tiles
+// l += w * 2^-exponent, and m moves (O is rescaled) only when weights pass 2^7
+// to 2^11, which shows in their sums: the common tile has no pass for its
+// maximum. What paces the kernel: the tensor core (2048 clocks for both tiles
 // and 128 positions of head size 128), then the softmax, whose 2^x take as long
 // on the special function unit alone.
 //
@@ -26,6 +27,12 @@
 //
 // Warps 0-3 and 4-7 softmax of either tile, and its queries; 8-11 values; 12 copies and the units to come, which it
 // describes to the others; 13 and 14 the MMAs of either tile; 15 the pages' scales.
+//
+// Compiled as a whole program of its own (no relocatable device code): the compiler takes setmaxnreg into account only
+// then. Without it the softmax's 128 registers were too few, and registers spilled to local memory come back from the L2,
+// as the shared memory leaves next to no L1: that alone made a tile's softmax twice as long. So it has its own device
+// status.
+#define MAMBO_OWN_DEVICE_STATUS
 #include "iq3s_tm.cuh"
 #include "kernels.cuh"
 #include "kv_tc.cuh"
@@ -39,14 +46,15 @@ constexpr int kRows = 128;            // of an MMA tile
 constexpr int kUnitRows = 2 * kRows;
 constexpr int kKStages = 3, kVStages = 2;
 constexpr float kNone = -1e30f;       // m of a row that has seen nothing
-constexpr float kHeadroom = 8.f;
+constexpr float kMostSum = 2048.f;    // of 16 weights, before m is moved: f16 holds 2^16
 // What a unit costs besides its tiles, in tiles: where the ranges of the CTAs are cut, units count as this much longer.
 constexpr int kUnitCost = 2;
 
 // Shared memory: queries [2 tiles][hi, lo][128][128], keys, values as they come and in f16 [2 halves of D][128][128 bytes].
 constexpr uint32_t kQ = 4 * kKvTileBytes, kVf = 2 * kKvTileBytes;
 constexpr uint32_t kAtK = kQ, kAtV = kAtK + kKStages * kKvTileBytes, kAtVf = kAtV + kVStages * kKvTileBytes;
-constexpr uint32_t kAtScales = kAtVf + 2 * kVf, kAtUnits = kAtScales + 2 * 32 * 16;
+// Of each softmax warp 2 KB: rows' factors, and results on their way out.
+constexpr uint32_t kAtStage = kAtVf + 2 * kVf, kAtScales = kAtStage + 8 * 2048, kAtUnits = kAtScales + 2 * 32 * 16;
 constexpr int kUnitStages = 4;
 constexpr uint32_t kAtBegin = kAtUnits + (kUnitStages + 1) * 96, kAtBars = kAtBegin + 128;
 constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 4 + 8 + 4 + 4 + 2 * kUnitStages;
@@ -189,11 +197,6 @@ __device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
   y = fma_2(y, f, pack2(0.9999993f, 0.9999993f));
   return pack2(__uint_as_float((uint32_t)y + ((uint32_t)n << 23)), __uint_as_float((uint32_t)(y >> 32) + ((uint32_t)(n >> 32) << 23)));
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 
 }  // namespace
 
@@ -240,6 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(kUfree + 8 * i, 15);  // MMAs, scales, 4 warps of values, 8 of the softmax
     }
     units[kUnitStages] = Unit{};
+    begin[12] = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(kQfull + 8 * i, 4);
       mbar_init(kQfree + 8 * i, 1);
@@ -276,6 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after_sync();
   const uint32_t tmem = (uint32_t)__shfl_sync(0xFFFFFFFFu, (int)*slot, 0);
   int total = 0, before = 0;
+  #pragma unroll 1
   for (int w = 0; w < 16; ++w) {
     total += warp_sums[w];
     before += w < warp ? warp_sums[w] : 0;
@@ -320,7 +325,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   const int log_page = p.cache.log_page, per_tile = kKvTile >> log_page;
 
+  // Register split, launched with 128 a thread: 256 x 176 + 256 x 80 = 512 x 128.
   if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == 12) {
       // ------------------------------------------------------------ copies, and the units
       KvRing kr, vr, ur;
@@ -356,6 +363,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int64_t low = p.window ? u.lo[q] + 1 - (int64_t)p.window : 0;
             u.from[q] = low > 0 ? (int)(low / kKvTile) : 0;
             u.to[q] = u.hi[q] >= 0 ? u.hi[q] / kKvTile + 1 : 0;
+          }
+          // The unit's queries on their way to the L2.
+#pragma unroll 1
+          for (int i = lane; i < kUnitRows && u.row0 + i < u.rows; i += 32) {
+            const int row = u.row0 + i, tok = row / p.group;
+            bulk_prefetch_l2(p.q + (int64_t)(u.token + tok) * p.qs_t + (int64_t)(u.h * p.group + row - tok * p.group) * p.qs_h, p.cache.dim * 2);
           }
           if (x < x1) plan.next();
         }
@@ -426,9 +439,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           ur.next(kUnitStages);
           begins = true;
         };
+        // One thread's values and next scores are issued together: the MMAs run in the order of their issue, and mixed they
+        // would end together, so that both tiles' softmax would run at once and then wait at once. The wait is for pace only
+        // and gives up after a while.
+        int* turn = begin + 12;
+        bool mine = false;
+        auto take_turn = [&]() {
+#pragma unroll 1
+          for (int i = 0; i < 64 && !mine; ++i) mine = atomicCAS(turn, 0, 1) == 0;
+        };
+        auto end_turn = [&]() {
+          if (mine) atomicExch(turn, 0);
+          mine = false;
+        };
         bool ok = true;
         auto scores = [&]() {  // whether these rows see the tile
           if (begins) {
+            end_turn();  // the next unit's queries may still be on their way
             ok = kv_wait(qfull, qphase, kSiteKvFull);
             qphase ^= 1;
             begins = false;
@@ -464,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (ok) {
               tc::fence_after_sync();
+              take_turn();
               mma_values(dout, ds, v0 + fr.at * (kVf >> 4), idesc_o, started, odone);
             }
             started = true;
@@ -475,7 +503,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           some = left > 0;
           ends = left == 1;
           if (some) seen = scores();
+          end_turn();
         }
+        end_turn();
         if (!ok) kv_settle();
       }
     } else {
@@ -525,6 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (fill) publish();
     }
   } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // -------------------------------------------------------------- values
     const int i = threadIdx.x - 256;  // position of the tile
     KvRing vr, fr, ur;
@@ -567,214 +598,206 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     // -------------------------------------------------------------- softmax
     const int q = warp >> 2, r = threadIdx.x & 127;
     const uint32_t ts = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + q * 128, to_ = ts + 256;
+    uint8_t* stage = sm + kAtStage + warp * 2048;
     KvRing mr, ur;
     int in_batch = 0;
     uint32_t sphase = 0, ophase = 1;  // ophase: of the last MMAs on the values
-    uint32_t qphase = 0;
-    // This thread's row of the unit's queries, split into two terms, to shared memory; its factor of the scores.
-    const bool qvec = (uintptr_t)p.q % 16 == 0 && p.qs_t % 8 == 0 && p.qs_h % 8 == 0;
+    uint32_t qphase = 1;              // a fresh barrier's previous phase counts as over
+    // Of the unit's queries this warp's 32 rows, split into two terms, to shared memory: a half warp a row, eight dimensions
+    // a lane. The factor of this thread's row is returned.
+    const int step_t = 2 / p.group, step_h = 2 - step_t * p.group;  // two rows on: tokens and heads
     auto queries = [&](const Unit& u) {
-      const int row = u.row0 + kRows * q + r, t = row / p.group;
-      const uint16_t* from = p.q + (int64_t)(u.token + t) * p.qs_t + (int64_t)(u.h * p.group + row - t * p.group) * p.qs_h;
-      const int dims = row < u.rows ? p.cache.dim : 0;
-      uint4 raw[16];
+      const int d0 = 8 * (lane & 15), r0 = 32 * (warp & 3) + (lane >> 4);
+      const int rows = d0 < p.cache.dim ? u.rows - u.row0 - kRows * q : 0;
+      const int row = u.row0 + kRows * q + r0;
+      int t = row / p.group, hh = row - t * p.group;
+      const uint16_t* from = p.q + (int64_t)u.token * p.qs_t + (int64_t)u.h * p.group * p.qs_h + d0;
+      uint4 ahead[8];
+      auto load = [&](int n) {
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        raw[c] = make_uint4(0, 0, 0, 0);
-        if (8 * c < dims) {
-          if (qvec) {
-            raw[c] = __ldg(reinterpret_cast<const uint4*>(from) + c);
-          } else {
-            uint32_t v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = (uint32_t)__ldg(from + 8 * c + 2 * k) | (uint32_t)__ldg(from + 8 * c + 2 * k + 1) << 16;
-            raw[c] = make_uint4(v[0], v[1], v[2], v[3]);
+        for (int k = 0; k < 8; ++k) {
+          ahead[k] = make_uint4(0, 0, 0, 0);
+          if (n + 2 * k < rows) ahead[k] = __ldg(reinterpret_cast<const uint4*>(from + t * p.qs_t + hh * p.qs_h));
+          t += step_t;
+          hh += step_h;
+          if (hh >= p.group) {
+            hh -= p.group;
+            ++t;
           }
         }
-      }
-      uint32_t top = 0;
+      };
+      load(r0);
+#pragma unroll 1
+      for (int n = r0; n < r0 + 32; n += 16) {
+        uint4 raw[8];
 #pragma unroll
-      for (int c = 0; c < 16; ++c)
-        top = absmax_bf16x2(top, absmax_bf16x2(absmax_bf16x2(raw[c].x, raw[c].y), absmax_bf16x2(raw[c].z, raw[c].w)));
-      const uint32_t code = mxfp8_scale_code(__uint_as_float(max(top & 0x7FFFu, (top >> 16) & 0x7FFFu) << 16));
-      const float inv = code == 255u ? 0.f : e8m0_to_float(254u - code);
-      uint8_t* to = sm + q * 2 * kKvTileBytes + r * 128;
+        for (int k = 0; k < 8; ++k) raw[k] = ahead[k];
+        if (n < r0 + 16) load(n + 16);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const uint32_t v[8] = {raw[2 * c].x, raw[2 * c].y, raw[2 * c].z, raw[2 * c].w,
-                               raw[2 * c + 1].x, raw[2 * c + 1].y, raw[2 * c + 1].z, raw[2 * c + 1].w};
-        uint32_t h[4], l[4];
+      for (int k = 0; k < 8; ++k) {
+        const int r1 = n + 2 * k;
+        const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+        uint32_t top = absmax_bf16x2(absmax_bf16x2(v[0], v[1]), absmax_bf16x2(v[2], v[3]));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int o = 8; o; o >>= 1) top = absmax_bf16x2(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const uint32_t code = mxfp8_scale_code(__uint_as_float(max(top & 0x7FFFu, (top >> 16) & 0x7FFFu) << 16));
+        const float inv = code == 255u ? 0.f : e8m0_to_float(254u - code);
+        uint32_t h[2], l[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
           // 8 significant bits up to 448: exact in f16 (down to 2^-17), and so is what the first term leaves.
-          const uint32_t e0 = f16x2_of(__uint_as_float(v[2 * k] << 16) * inv, __uint_as_float(v[2 * k] & 0xFFFF0000u) * inv);
-          const uint32_t e1 = f16x2_of(__uint_as_float(v[2 * k + 1] << 16) * inv, __uint_as_float(v[2 * k + 1] & 0xFFFF0000u) * inv);
+          const uint32_t e0 = f16x2_of(__uint_as_float(v[2 * c] << 16) * inv, __uint_as_float(v[2 * c] & 0xFFFF0000u) * inv);
+          const uint32_t e1 = f16x2_of(__uint_as_float(v[2 * c + 1] << 16) * inv, __uint_as_float(v[2 * c + 1] & 0xFFFF0000u) * inv);
           const uint32_t h0 = e4m3x2_of_f16x2(e0), h1 = e4m3x2_of_f16x2(e1);
-          h[k] = h0 | (h1 << 16);
-          l[k] = e4m3x2_of_f16x2(sub_f16x2(e0, f16x2_of_e4m3x2(h0))) | (e4m3x2_of_f16x2(sub_f16x2(e1, f16x2_of_e4m3x2(h1))) << 16);
-          if (code == 255u) h[k] = l[k] = 0u;
+          h[c] = h0 | (h1 << 16);
+          l[c] = e4m3x2_of_f16x2(sub_f16x2(e0, f16x2_of_e4m3x2(h0))) | (e4m3x2_of_f16x2(sub_f16x2(e1, f16x2_of_e4m3x2(h1))) << 16);
+          if (code == 255u) h[c] = l[c] = 0u;
         }
-        *reinterpret_cast<uint4*>(to + ((c ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(to + kKvTileBytes + ((c ^ (r & 7)) << 4)) = make_uint4(l[0], l[1], l[2], l[3]);
+        uint8_t* to = sm + q * 2 * kKvTileBytes + r1 * 128 + (((lane & 15) >> 1 ^ (r1 & 7)) << 4) + (lane & 1) * 8;
+        *reinterpret_cast<uint2*>(to) = make_uint2(h[0], h[1]);
+        *reinterpret_cast<uint2*>(to + kKvTileBytes) = make_uint2(l[0], l[1]);
+        if (d0 == 0)
+          *reinterpret_cast<float*>(stage + 4 * (r1 & 31)) = code == 255u ? NAN : p.scale * 1.4426950408889634f * e8m0_to_float(code);
+      }
       }
       fence_proxy_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(kQfull + 8 * q);
-      return code == 255u ? NAN : p.scale * 1.4426950408889634f * e8m0_to_float(code);
+      return *reinterpret_cast<const float*>(stage + 4 * lane);
     };
-    float cq = 0.f;
-    if (unit_of(ur).n > 0) cq = queries(unit_of(ur));
+    // Through the units, one behind: the next one's queries are on their way before this one's results are waited for.
+    float m = kNone, l = 0.f, cq = 0.f;
+    int n = 0, first = 0, from = 0, end = 0, lo = 0, hi = 0, place = -1;
+    bool started = false;
     for (;;) {
-      const Unit& unit = unit_of(ur);
-      const int n = unit.n;
-      if (n <= 0) break;
-      const int from = unit.from[q], end = unit.to[q];
-      const int lo = unit.lo[q], hi = unit.hi[q], row = unit.row0 + kRows * q + r;
-      const int place = row < unit.rows ? unit.place0 + row / p.group : -1;
-      float m = kNone, l = 0.f;
-      bool started = false;
-      for (int tile = unit.tile, left = n; left > 0; ++tile, --left) {
-      if (in_batch == 0) kv_warp_wait(kMfull + 8 * mr.at, mr.phase, kSiteKvFull);
-      const float4* sc = scales + mr.at * 32 + in_batch * 8;
-      if (tile >= from && tile < end) {
-        kv_warp_wait(kSfull + 8 * q, sphase, kSiteKvFull);
-        sphase ^= 1;
-        tc::fence_after_sync();
-        const int64_t j0 = (int64_t)tile * kKvTile;
-        const bool edge = j0 + kKvTile - 1 > lo || (p.window && j0 <= (int64_t)hi - p.window);
-        // The scores are read from TMEM twice, 64 columns at a time, for the maximum and for the weights: held between, they
-        // would need more registers than 512 threads have. Loops that are not unrolled keep the code in the SM's cache.
-        float top = -INFINITY;
-        // Of an edge tile: the last position that the row sees, and the one before the first, in the tile.
-        int high = kKvTile, low = -1;
-        if (!edge) {
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
+      for (int tile = first, left = n; left > 0; ++tile, --left) {
+        if (in_batch == 0) kv_warp_wait(kMfull + 8 * mr.at, mr.phase, kSiteKvFull);
+        const float4* sc = scales + mr.at * 32 + in_batch * 8;
+        if (tile >= from && tile < end) {
+          kv_warp_wait(kSfull + 8 * q, sphase, kSiteKvFull);
+          sphase ^= 1;
+          tc::fence_after_sync();
+          const int64_t j0 = (int64_t)tile * kKvTile;
+          const bool edge = j0 + kKvTile - 1 > lo || (p.window && j0 <= (int64_t)hi - p.window);
+          bool plain = started && !edge;
+          if (plain) {
+            // One pass with m as it is. A weight that is too large shows in the sums; then the tile is done over.
+            uint32_t w[2][32];
+            float sum = 0.f, most = 0.f;
             uint32_t raw[2][32];
-            kv_ld<32>(ts + 64 * c, raw[0]);
-            kv_ld<32>(ts + 64 * c + 32, raw[1]);
-            kv_wait_ld();
-            kv_tie(raw[0]);
-            kv_tie(raw[1]);
+            kv_ld<32>(ts, raw[0]);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const float4 v = sc[4 * c + g];
-              auto s = [&](int k) { return __uint_as_float(raw[g >> 1][16 * (g & 1) + k]); };
-              float a = max3(s(0), s(1), s(2)), b = max3(s(3), s(4), s(5));
-              a = max3(a, s(6), s(7)), b = max3(b, s(8), s(9));
-              a = max3(a, s(10), s(11)), b = max3(b, s(12), s(13));
-              a = max3(a, s(14), s(15));
-              top = fmaxf(top, fmaf(fmaxf(a, b), cq * v.x, v.y));
-            }
-          }
-        } else {
-          high = (int)min((int64_t)kKvTile, place - j0);
-          if (p.window) low = (int)max((int64_t)-1, min((int64_t)kKvTile, place - (int64_t)p.window - j0));
-#pragma unroll 1
-          for (int g = 0; g < 8; ++g) {
-            uint32_t raw[16];
-            kv_ld<16>(ts + 16 * g, raw);
-            kv_wait_ld();
-            kv_tie(raw);
-            const float4 v = sc[g];
-            const float c = cq * v.x;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const int at = 16 * g + k;
-              if (at <= high && at > low) top = fmaxf(top, fmaf(__uint_as_float(raw[k]), c, v.y));
-            }
-          }
-        }
-        if (__any_sync(0xFFFFFFFFu, top > m + kHeadroom)) {
-          const float to = top > m + kHeadroom ? top : m, f = ex2(m - to);
-          m = to;
-          l *= f;
-          if (started) {
-            kv_warp_wait(kOdone + 8 * q, ophase, kSiteKvFull);
-            tc::fence_after_sync();
-#pragma unroll 1
-            for (int c = 0; c < p.cache.dim; c += 16) {
-              uint32_t o[16];
-              kv_ld<16>(to_ + c, o);
+            for (int c = 0; c < 4; ++c) {
               kv_wait_ld();
-              kv_tie(o);
+              kv_tie(raw[c & 1]);
+              if (c < 3) kv_ld<32>(ts + 32 * c + 32, raw[(c + 1) & 1]);
 #pragma unroll
-              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tc::st_cols<16>(to_ + c, o);
-            }
-          }
-        }
-        // The weights replace the scores from the left, half as wide, behind the columns that have been read.
-        if (!edge) {
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t raw[2][32], w[32];
-            kv_ld<32>(ts + 64 * c, raw[0]);
-            kv_ld<32>(ts + 64 * c + 32, raw[1]);
-            kv_wait_ld();
-            kv_tie(raw[0]);
-            kv_tie(raw[1]);
+              for (int g = 0; g < 2; ++g) {
+                const float4 v = sc[2 * c + g];
+                const uint64_t k2 = pack2(cq * v.x, cq * v.x), add2 = pack2(v.y - m, v.y - m);
+                uint64_t sum2 = 0;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const float4 v = sc[4 * c + g];
-              const uint64_t k2 = pack2(cq * v.x, cq * v.x), add2 = pack2(v.y - m, v.y - m);
-              uint64_t sum2 = 0;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int at = 16 * (g & 1) + 2 * i;
-                const uint64_t x = fma_2(pack2(__uint_as_float(raw[g >> 1][at]), __uint_as_float(raw[g >> 1][at + 1])), k2, add2);
-                const uint64_t e = (i & 3) == 3 ? ex2_poly(x) : pack2(ex2(low_of(x)), ex2(high_of(x)));
-                sum2 = add_2(sum2, e);
-                w[8 * g + i] = f16x2_of(low_of(e), high_of(e));
+                for (int i = 0; i < 8; ++i) {
+                  const int at = 16 * g + 2 * i;
+                  const uint64_t x = fma_2(pack2(__uint_as_float(raw[c & 1][at]), __uint_as_float(raw[c & 1][at + 1])), k2, add2);
+                  const uint64_t e = (i & 3) == 3 ? ex2_poly(x) : pack2(ex2(low_of(x)), ex2(high_of(x)));
+                  sum2 = add_2(sum2, e);
+                  w[c >> 1][16 * (c & 1) + 8 * g + i] = f16x2_of(low_of(e), high_of(e));
+                }
+                const float part = low_of(sum2) + high_of(sum2);
+                most = fmaxf(most, part);
+                sum = fmaf(part, v.z, sum);
               }
-              l = fmaf(low_of(sum2) + high_of(sum2), v.z, l);
             }
-            tc::st_cols<32>(ts + 32 * c, w);
+            plain = !__any_sync(0xFFFFFFFFu, most > kMostSum);
+            if (plain) {
+              l += sum;
+              tc::st_cols<32>(ts, w[0]);
+              tc::st_cols<32>(ts + 32, w[1]);
+            }
           }
-        } else {
+          if (!plain) {
+            // The last position that the row sees, and the one before the first, in the tile; their largest x; then the
+            // weights, which replace the scores from the left, half as wide, behind the columns that have been read.
+            const int high = (int)max((int64_t)-1, min((int64_t)kKvTile, place - j0));
+            const int low = p.window ? (int)max((int64_t)-1, min((int64_t)kKvTile, place - (int64_t)p.window - j0)) : -1;
+            float top = -INFINITY;
 #pragma unroll 1
-          for (int g = 0; g < 8; ++g) {
-            uint32_t raw[16], w[8];
-            kv_ld<16>(ts + 16 * g, raw);
-            kv_wait_ld();
-            kv_tie(raw);
-            const float4 v = sc[g];
-            const float c = cq * v.x, add = v.y - m;
-            float sum = 0.f;
+            for (int c = 0; c < 4; ++c) {
+              uint32_t raw[32];
+              kv_ld<32>(ts + 32 * c, raw);
+              const float4 v[2] = {sc[2 * c], sc[2 * c + 1]};
+              kv_wait_ld();
+              kv_tie(raw);
+              float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-              const int at = 16 * g + k;
-              const float a = at <= high && at > low ? ex2(fmaf(__uint_as_float(raw[k]), c, add)) : 0.f;
-              const float b = at + 1 <= high && at + 1 > low ? ex2(fmaf(__uint_as_float(raw[k + 1]), c, add)) : 0.f;
-              sum += a + b;
-              w[k >> 1] = f16x2_of(a, b);
+              for (int k = 0; k < 32; ++k) {
+                const int at = 32 * c + k;
+                if (at <= high && at > low) t4[k & 3] = fmaxf(t4[k & 3], fmaf(__uint_as_float(raw[k]), cq * v[k >> 4].x, v[k >> 4].y));
+              }
+              top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
             }
-            l = fmaf(sum, v.z, l);
-            tc::st_x8(ts + 8 * g, w);
+            const float up = fmaxf(m, top), f = ex2(m - up);
+            m = up;
+            l *= f;
+            if (started) {
+              kv_warp_wait(kOdone + 8 * q, ophase, kSiteKvFull);
+              tc::fence_after_sync();
+              if (__any_sync(0xFFFFFFFFu, f != 1.f)) {
+#pragma unroll 1
+                for (int c = 0; c < p.cache.dim; c += 16) {
+                  uint32_t o[16];
+                  kv_ld<16>(to_ + c, o);
+                  kv_wait_ld();
+                  kv_tie(o);
+#pragma unroll
+                  for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                  tc::st_cols<16>(to_ + c, o);
+                }
+              }
+            }
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t raw[32], w[16];
+              kv_ld<32>(ts + 32 * c, raw);
+              const float4 v[2] = {sc[2 * c], sc[2 * c + 1]};
+              kv_wait_ld();
+              kv_tie(raw);
+              float sums[2] = {0.f, 0.f};
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                const int at = 32 * c + k, g = k >> 4;
+                const float a = at <= high && at > low ? ex2(fmaf(__uint_as_float(raw[k]), cq * v[g].x, v[g].y - m)) : 0.f;
+                const float b = at + 1 <= high && at + 1 > low ? ex2(fmaf(__uint_as_float(raw[k + 1]), cq * v[g].x, v[g].y - m)) : 0.f;
+                sums[g] += a + b;
+                w[k >> 1] = f16x2_of(a, b);
+              }
+              l = fmaf(sums[0], v[0].z, fmaf(sums[1], v[1].z, l));
+              tc::st_cols<16>(ts + 16 * c, w);
+            }
           }
+          tc::wait_st();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(kWfull + 8 * q);
+          started = true;
+          ophase ^= 1;
         }
-        tc::wait_st();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(kWfull + 8 * q);
-        started = true;
-        ophase ^= 1;
-      }
-      if (++in_batch == 4) {
-        in_batch = 0;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(kMfree + 8 * mr.at);
-        mr.next(2);
-      }
-
+        if (++in_batch == 4) {
+          in_batch = 0;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(kMfree + 8 * mr.at);
+          mr.next(2);
+        }
       }
 
       // The next unit's queries, before this one's results are waited for.
       KvRing after = ur;
-      after.next(kUnitStages);
+      if (n > 0) after.next(kUnitStages);
       const Unit& next = unit_of(after);
       float next_cq = 0.f;
       if (next.n > 0) {
@@ -782,35 +805,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         qphase ^= 1;
         next_cq = queries(next);
       }
-      if (unit.has(q)) {
+      const Unit& unit = units[ur.at];
+      if (n > 0 && unit.has(q)) {
         // The unit's end, or this CTA's part of it.
         if (started) {
           kv_warp_wait(kOdone + 8 * q, ophase, kSiteKvFull);
           tc::fence_after_sync();
         }
-        const int t = row / p.group;
-        const bool valid = row < unit.rows;
+        const int row = unit.row0 + kRows * q + r, t = row / p.group;
         const int64_t token = unit.token + t, head = unit.h * p.group + row - t * p.group;
-        uint16_t* out = p.out + token * p.os_t + head * p.os_h;
-        const bool vec = (uintptr_t)p.out % 16 == 0 && p.os_t % 8 == 0 && p.os_h % 8 == 0;
-        auto store = [&](int d, const float (&v)[16]) {  // 16 dimensions of the thread's row
-          uint32_t u[8];
+        const int64_t out_at = row < unit.rows ? token * p.os_t + head * p.os_h : -1;
+        // 32 dimensions of the warp's rows to memory, through the stage: 64 bytes of each of eight rows at a time.
+        auto store = [&](int c, const float (&v)[32]) {
+          __syncwarp();
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-            u[k] = *reinterpret_cast<const uint32_t*>(&b);
+          for (int k = 0; k < 4; ++k) {
+            uint32_t u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(v[8 * k + 2 * i], v[8 * k + 2 * i + 1]);
+              u[i] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
           }
-          if (!valid) return;
-          if (vec) {
-            reinterpret_cast<uint4*>(out + d)[0] = make_uint4(u[0], u[1], u[2], u[3]);
-            reinterpret_cast<uint4*>(out + d)[1] = make_uint4(u[4], u[5], u[6], u[7]);
-          } else {
+          __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 16; ++k) out[d + k] = (uint16_t)(u[k >> 1] >> (16 * (k & 1)));
+          for (int k = 0; k < 4; ++k) {
+            const int rr = (lane >> 2) + 8 * k, d = c + 8 * (lane & 3);
+            const int64_t at = __shfl_sync(0xFFFFFFFFu, out_at, rr);
+            const uint4 u = *reinterpret_cast<const uint4*>(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
+            if (at >= 0 && d < p.cache.dim) *reinterpret_cast<uint4*>(p.out + at + d) = u;
           }
         };
         auto store_lse = [&](float top, float all) {
-          if (valid && p.lse)
+          if (out_at >= 0 && p.lse)
             p.lse[token * p.ls_t + head * p.ls_h] = all == 0.f ? -INFINITY : (top + log2f(all)) * 0.6931471805599453f;
         };
         const bool whole = n == unit.tiles;
@@ -819,24 +847,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto part = [&](int cta) { return partials + ((int64_t)(cta * 2 + (cta == cta0)) * 2 + q) * kPart; };
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-        for (int d = 0; d < p.cache.dim; d += 16) {
-          uint32_t o[16];
-          float v[16];
+        for (int c = 0; c < p.cache.dim; c += 32) {
+          uint32_t o[32];
+          float v[32];
           if (started) {
-            kv_ld<16>(to_ + d, o);
+            kv_ld<32>(to_ + c, o);
             kv_wait_ld();
             kv_tie(o);
           }
 #pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] = started ? __uint_as_float(o[k]) : 0.f;
+          for (int k = 0; k < 32; ++k) v[k] = started ? __uint_as_float(o[k]) : 0.f;
           if (whole) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = l == 0.f ? 0.f : v[k] * inv;
-            store(d, v);
+            for (int k = 0; k < 32; ++k) v[k] = l == 0.f ? 0.f : v[k] * inv;
+            store(c, v);
           } else {
-            float4* at = reinterpret_cast<float4*>(part(blockIdx.x)) + (d >> 2) * kRows + r;
+            float4* at = reinterpret_cast<float4*>(part(blockIdx.x)) + (c >> 2) * kRows + r;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) __stcg(at + k * kRows, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
+            for (int k = 0; k < 8; ++k) __stcg(at + k * kRows, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
           }
         }
         tc::fence_before_sync();
@@ -859,42 +887,54 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (begin[8 + q]) {
             float top = kNone, all = 0.f;
 #pragma unroll 4
-            for (int c = cta0; c <= cta1; ++c) top = fmaxf(top, __ldcg(part(c) + kRows * 128 + r));
+            for (int k = cta0; k <= cta1; ++k) top = fmaxf(top, __ldcg(part(k) + kRows * 128 + r));
 #pragma unroll 4
-            for (int c = cta0; c <= cta1; ++c)
-              all = fmaf(ex2(__ldcg(part(c) + kRows * 128 + r) - top), __ldcg(part(c) + kRows * 129 + r), all);
+            for (int k = cta0; k <= cta1; ++k)
+              all = fmaf(ex2(__ldcg(part(k) + kRows * 128 + r) - top), __ldcg(part(k) + kRows * 129 + r), all);
             const float inv_all = all == 0.f ? 0.f : 1.f / all;
 #pragma unroll 1
-            for (int d = 0; d < p.cache.dim; d += 16) {
-              float v[16];
+            for (int c = 0; c < p.cache.dim; c += 32) {
+              float v[32];
 #pragma unroll
-              for (int k = 0; k < 16; ++k) v[k] = 0.f;
-#pragma unroll 2
-              for (int c = cta0; c <= cta1; ++c) {
-                const float f = ex2(__ldcg(part(c) + kRows * 128 + r) - top);
-                const float4* at = reinterpret_cast<const float4*>(part(c)) + (d >> 2) * kRows + r;
+              for (int k = 0; k < 32; ++k) v[k] = 0.f;
+#pragma unroll 1
+              for (int k = cta0; k <= cta1; ++k) {
+                const float f = ex2(__ldcg(part(k) + kRows * 128 + r) - top) * inv_all;
+                const float4* at = reinterpret_cast<const float4*>(part(k)) + (c >> 2) * kRows + r;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const float4 a = __ldcg(at + k * kRows);
-                  v[4 * k] = fmaf(f, a.x, v[4 * k]);
-                  v[4 * k + 1] = fmaf(f, a.y, v[4 * k + 1]);
-                  v[4 * k + 2] = fmaf(f, a.z, v[4 * k + 2]);
-                  v[4 * k + 3] = fmaf(f, a.w, v[4 * k + 3]);
+                for (int i = 0; i < 8; ++i) {
+                  const float4 a = __ldcg(at + i * kRows);
+                  v[4 * i] = fmaf(f, a.x, v[4 * i]);
+                  v[4 * i + 1] = fmaf(f, a.y, v[4 * i + 1]);
+                  v[4 * i + 2] = fmaf(f, a.z, v[4 * i + 2]);
+                  v[4 * i + 3] = fmaf(f, a.w, v[4 * i + 3]);
                 }
               }
+              if (all == 0.f) {
 #pragma unroll
-              for (int k = 0; k < 16; ++k) v[k] = all == 0.f ? 0.f : v[k] * inv_all;
-              store(d, v);
+                for (int k = 0; k < 32; ++k) v[k] = 0.f;
+              }
+              store(c, v);
             }
             store_lse(top, all);
           }
-          kv_bar_sync(1 + q, 128);  // before the flag is used again
         }
+        if (!whole) kv_bar_sync(1 + q, 128);  // before the flag is used again
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(kUfree + 8 * ur.at);
-      ur.next(kUnitStages);
+      if (n > 0 && lane == 0) mbar_arrive(kUfree + 8 * ur.at);
+      ur = after;
+      n = next.n;
+      if (n <= 0) break;
+      first = next.tile;
+      from = next.from[q], end = next.to[q];
+      lo = next.lo[q], hi = next.hi[q];
+      const int next_row = next.row0 + kRows * q + r;
+      place = next_row < next.rows ? next.place0 + next_row / p.group : -1;
       cq = next_cq;
+      m = place >= 0 ? kNone : -kNone;  // rows that see nothing have weights of zero whatever the scores are
+      l = 0.f;
+      started = false;
     }
   }
   __syncwarp();
@@ -914,6 +954,11 @@ cudaError_t launch_kv_prompt(const KvAttentionCall& p, const CUtensorMap& k, con
   const cudaError_t e = ensure_smem_attribute(kernel, kSmem);
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(sms), dim3(kThreads), kSmem, stream, p, k, v, partials, counters);
+}
+
+cudaError_t kv_prompt_status_symbols(void** status, void** limit) {
+  const cudaError_t e = cudaGetSymbolAddress(status, g_device_status);
+  return e != cudaSuccess ? e : cudaGetSymbolAddress(limit, g_wait_limit_ns);
 }
 
 }  // namespace mambo

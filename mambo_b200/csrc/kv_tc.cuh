@@ -13,7 +13,8 @@ namespace mambo {
 constexpr int kKvTile = 128;
 constexpr uint32_t kKvTileBytes = 128u * 128u;  // rows of 128 bytes, zero behind the head size
 
-// Waits for a barrier phase, bounded in time (the clock is read every 256 tries).
+// Waits for a barrier phase, bounded in time (the clock is read every 256 tries). The slow part is a function of its own:
+// it is in every role, and code that does not fit the SM's instruction cache is what these kernels lose most time to.
 __device__ __forceinline__ bool kv_wait_slow(uint32_t bar, uint32_t parity, int site) {
   unsigned long long t0 = 0;
 #pragma unroll 1

@@ -141,6 +141,12 @@ def launch_fp8_kv_append(cache: Fp8KvCache, k, v, page_table, lengths, *, offset
             None if rope is None else rope["rotary"], _runtime.stream_handle(None, dev)), "launch_fp8_kv_append")
 
 
+def _rows_aligned(t: torch.Tensor) -> bool:
+    """Whether every head of [T,H,D] is 16-byte aligned with unit stride."""
+    st, sh, unit = t.stride()
+    return unit == 1 and not (st % 8 or sh % 8 or t.data_ptr() % 16)
+
+
 @functools.lru_cache(maxsize=1024)
 def _attention_workspace_bytes(heads: int, kv_heads: int, ragged: bool) -> int:
     return _lib.load().mambo_kv_attention_workspace_bytes(heads, kv_heads, int(ragged))
@@ -174,12 +180,15 @@ def fp8_paged_attention(q, cache: Fp8KvCache, page_table, lengths, *, offsets=No
         raise ValueError("window must not be negative")
     seq, held = _sequences(page_table, lengths, offsets, tokens, dev)
     _runtime.require_device(dev)
-    if q.stride(2) != 1:
-        q = q.contiguous()
+    if not _rows_aligned(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    given = out
     if out is None:
         out = torch.empty((tokens, heads, dim), dtype=torch.bfloat16, device=dev)
-    elif tuple(out.shape) != (tokens, heads, dim) or out.dtype != torch.bfloat16 or out.stride(2) != 1 or out.device != dev:
-        raise ValueError("out must be bfloat16 of q's shape with unit stride along the head, on its device")
+    elif tuple(out.shape) != (tokens, heads, dim) or out.dtype != torch.bfloat16 or out.device != dev:
+        raise ValueError("out must be bfloat16 of q's shape on its device")
+    elif not _rows_aligned(out):
+        out = out.clone(memory_format=torch.contiguous_format)  # rows that no sequence covers keep what they hold
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if return_lse else None
     if tokens:
         need = _attention_workspace_bytes(heads, view.kv_heads, offsets is not None)
@@ -190,4 +199,7 @@ def fp8_paged_attention(q, cache: Fp8KvCache, page_table, lengths, *, offsets=No
                     dim ** -0.5 if scale is None else scale, out.data_ptr(), *_head_strides(out),
                     None if lse is None else lse.data_ptr(), heads, 1, ws.ptr, ws.size, ws.stream),
                     "fp8_paged_attention")
+    if given is not None and given is not out:
+        given.copy_(out)
+        out = given
     return (out, lse) if return_lse else out
