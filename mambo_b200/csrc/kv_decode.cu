@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
           uint32_t top = absmax_bf16x2(absmax_bf16x2(w[0], w[1]), absmax_bf16x2(w[2], w[3]));
 #pragma unroll
           for (int o = 8; o; o >>= 1) top = absmax_bf16x2(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-          const uint32_t code = mxfp8_scale_code(__uint_as_float(max(top & 0x7FFFu, (top >> 16) & 0x7FFFu) << 16));
+          const uint32_t code = bf16_scale_code(max(top & 0x7FFFu, (top >> 16) & 0x7FFFu));
           const float inv = code == 255u ? 0.f : e8m0_to_float(254u - code);
           uint32_t h[2], l[2];
 #pragma unroll

@@ -48,7 +48,7 @@ constexpr int kKStages = 3, kVStages = 2;
 constexpr float kNone = -1e30f;       // m of a row that has seen nothing
 constexpr float kMostSum = 2048.f;    // of 16 weights, before m is moved: f16 holds 2^16
 // What a unit costs besides its tiles, in tiles: where the ranges of the CTAs are cut, units count as this much longer.
-constexpr int kUnitCost = 2;
+constexpr int kUnitCost = 6;
 
 // Shared memory: queries [2 tiles][hi, lo][128][128], keys, values as they come and in f16 [2 halves of D][128][128 bytes].
 constexpr uint32_t kQ = 4 * kKvTileBytes, kVf = 2 * kKvTileBytes;
@@ -243,7 +243,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(kUfree + 8 * i, 15);  // MMAs, scales, 4 warps of values, 8 of the softmax
     }
     units[kUnitStages] = Unit{};
-    begin[12] = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(kQfull + 8 * i, 4);
       mbar_init(kQfree + 8 * i, 1);
@@ -439,23 +438,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           ur.next(kUnitStages);
           begins = true;
         };
-        // One thread's values and next scores are issued together: the MMAs run in the order of their issue, and mixed they
-        // would end together, so that both tiles' softmax would run at once and then wait at once. The wait is for pace only
-        // and gives up after a while.
-        int* turn = begin + 12;
-        bool mine = false;
-        auto take_turn = [&]() {
-#pragma unroll 1
-          for (int i = 0; i < 64 && !mine; ++i) mine = atomicCAS(turn, 0, 1) == 0;
-        };
-        auto end_turn = [&]() {
-          if (mine) atomicExch(turn, 0);
-          mine = false;
-        };
         bool ok = true;
         auto scores = [&]() {  // whether these rows see the tile
           if (begins) {
-            end_turn();  // the next unit's queries may still be on their way
             ok = kv_wait(qfull, qphase, kSiteKvFull);
             qphase ^= 1;
             begins = false;
@@ -491,7 +476,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (ok) {
               tc::fence_after_sync();
-              take_turn();
               mma_values(dout, ds, v0 + fr.at * (kVf >> 4), idesc_o, started, odone);
             }
             started = true;
@@ -503,9 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           some = left > 0;
           ends = left == 1;
           if (some) seen = scores();
-          end_turn();
         }
-        end_turn();
         if (!ok) kv_settle();
       }
     } else {
@@ -608,61 +590,74 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t sphase = 0, ophase = 1;  // ophase: of the last MMAs on the values
     uint32_t qphase = 1;              // a fresh barrier's previous phase counts as over
     // Of the unit's queries this warp's 32 rows, split into two terms, to shared memory: a half warp a row, eight dimensions
-    // a lane. The factor of this thread's row is returned.
+    // a lane. The rows come as they are to where their terms go (a row of bf16 is as large as both), all at once and
+    // asynchronously, and are split in place. The factor of this thread's row is returned.
     const int step_t = 2 / p.group, step_h = 2 - step_t * p.group;  // two rows on: tokens and heads
     auto queries = [&](const Unit& u) {
-      const int d0 = 8 * (lane & 15), r0 = 32 * (warp & 3) + (lane >> 4);
-      const int rows = d0 < p.cache.dim ? u.rows - u.row0 - kRows * q : 0;
+      const int c = lane & 15, r0 = 32 * (warp & 3) + (lane >> 4);
+      const int rows = 8 * c < p.cache.dim ? u.rows - u.row0 - kRows * q : 0;
       const int row = u.row0 + kRows * q + r0;
-      int t = row / p.group, hh = row - t * p.group;
-      const uint16_t* from = p.q + (int64_t)u.token * p.qs_t + (int64_t)u.h * p.group * p.qs_h + d0;
-      uint4 ahead[8];
-      auto load = [&](int n) {
+      const int t = row / p.group;
+      int hh = row - t * p.group;
+      // Two rows on: step_t tokens and step_h query heads, and where that passes the group another token and a group back.
+      const int64_t on = step_t * p.qs_t + step_h * p.qs_h, wrap = p.qs_t - p.group * p.qs_h;
+      const uint16_t* from = p.q + (int64_t)(u.token + t) * p.qs_t + (int64_t)(u.h * p.group + hh) * p.qs_h + 8 * c;
+      // Chunk c of a row: eight in the first term's place, eight in the second's.
+      const uint32_t tile0 = q * 2 * kKvTileBytes, mine = tile0 + (c >> 3) * kKvTileBytes;
+#pragma unroll 4
+      for (int r1 = r0; r1 < r0 + 32; r1 += 2) {
+        const bool have = r1 < rows;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sm0 + mine + r1 * 128 + (((c ^ r1) & 7) << 4)),
+                     "l"(have ? from : p.q), "r"(have ? 16 : 0)
+                     : "memory");
+        hh += step_h;
+        const bool over = hh >= p.group;
+        from += over ? on + wrap : on;
+        hh -= over ? p.group : 0;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      // Four rows at a time, whose chains (350 clocks each) overlap.
+#pragma unroll 1
+      for (int n = r0; n < r0 + 32; n += 8) {
+        uint32_t v[4][4], code[4], h[4][2], l[4][2];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          ahead[k] = make_uint4(0, 0, 0, 0);
-          if (n + 2 * k < rows) ahead[k] = __ldg(reinterpret_cast<const uint4*>(from + t * p.qs_t + hh * p.qs_h));
-          t += step_t;
-          hh += step_h;
-          if (hh >= p.group) {
-            hh -= p.group;
-            ++t;
+        for (int k = 0; k < 4; ++k) {
+          const int r1 = n + 2 * k;
+          const uint4 raw = *reinterpret_cast<const uint4*>(sm + mine + r1 * 128 + (((c ^ r1) & 7) << 4));
+          v[k][0] = raw.x, v[k][1] = raw.y, v[k][2] = raw.z, v[k][3] = raw.w;
+          code[k] = absmax_bf16x2(absmax_bf16x2(raw.x, raw.y), absmax_bf16x2(raw.z, raw.w));
+        }
+#pragma unroll
+        for (int o = 8; o; o >>= 1)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) code[k] = absmax_bf16x2(code[k], __shfl_xor_sync(0xFFFFFFFFu, code[k], o));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          code[k] = bf16_scale_code(max(code[k] & 0x7FFFu, (code[k] >> 16) & 0x7FFFu));
+          const float inv = code[k] == 255u ? 0.f : e8m0_to_float(254u - code[k]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            // 8 significant bits up to 448: exact in f16 (down to 2^-17), and so is what the first term leaves.
+            const uint32_t a = v[k][2 * i], b = v[k][2 * i + 1];
+            const uint32_t e0 = f16x2_of(__uint_as_float(a << 16) * inv, __uint_as_float(a & 0xFFFF0000u) * inv);
+            const uint32_t e1 = f16x2_of(__uint_as_float(b << 16) * inv, __uint_as_float(b & 0xFFFF0000u) * inv);
+            const uint32_t h0 = e4m3x2_of_f16x2(e0), h1 = e4m3x2_of_f16x2(e1);
+            h[k][i] = h0 | (h1 << 16);
+            l[k][i] = e4m3x2_of_f16x2(sub_f16x2(e0, f16x2_of_e4m3x2(h0))) | (e4m3x2_of_f16x2(sub_f16x2(e1, f16x2_of_e4m3x2(h1))) << 16);
+            if (code[k] == 255u) h[k][i] = l[k][i] = 0u;
           }
         }
-      };
-      load(r0);
-#pragma unroll 1
-      for (int n = r0; n < r0 + 32; n += 16) {
-        uint4 raw[8];
+        __syncwarp();  // both halves of the rows have been read
 #pragma unroll
-        for (int k = 0; k < 8; ++k) raw[k] = ahead[k];
-        if (n < r0 + 16) load(n + 16);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int r1 = n + 2 * k;
-        const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-        uint32_t top = absmax_bf16x2(absmax_bf16x2(v[0], v[1]), absmax_bf16x2(v[2], v[3]));
-#pragma unroll
-        for (int o = 8; o; o >>= 1) top = absmax_bf16x2(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        const uint32_t code = mxfp8_scale_code(__uint_as_float(max(top & 0x7FFFu, (top >> 16) & 0x7FFFu) << 16));
-        const float inv = code == 255u ? 0.f : e8m0_to_float(254u - code);
-        uint32_t h[2], l[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          // 8 significant bits up to 448: exact in f16 (down to 2^-17), and so is what the first term leaves.
-          const uint32_t e0 = f16x2_of(__uint_as_float(v[2 * c] << 16) * inv, __uint_as_float(v[2 * c] & 0xFFFF0000u) * inv);
-          const uint32_t e1 = f16x2_of(__uint_as_float(v[2 * c + 1] << 16) * inv, __uint_as_float(v[2 * c + 1] & 0xFFFF0000u) * inv);
-          const uint32_t h0 = e4m3x2_of_f16x2(e0), h1 = e4m3x2_of_f16x2(e1);
-          h[c] = h0 | (h1 << 16);
-          l[c] = e4m3x2_of_f16x2(sub_f16x2(e0, f16x2_of_e4m3x2(h0))) | (e4m3x2_of_f16x2(sub_f16x2(e1, f16x2_of_e4m3x2(h1))) << 16);
-          if (code == 255u) h[c] = l[c] = 0u;
+        for (int k = 0; k < 4; ++k) {
+          const int r1 = n + 2 * k;
+          uint8_t* to = sm + tile0 + r1 * 128 + ((((c >> 1) ^ r1) & 7) << 4) + (c & 1) * 8;
+          *reinterpret_cast<uint2*>(to) = make_uint2(h[k][0], h[k][1]);
+          *reinterpret_cast<uint2*>(to + kKvTileBytes) = make_uint2(l[k][0], l[k][1]);
+          if (c == 0)
+            *reinterpret_cast<float*>(stage + 4 * (r1 & 31)) = code[k] == 255u ? NAN : p.scale * 1.4426950408889634f * e8m0_to_float(code[k]);
         }
-        uint8_t* to = sm + q * 2 * kKvTileBytes + r1 * 128 + (((lane & 15) >> 1 ^ (r1 & 7)) << 4) + (lane & 1) * 8;
-        *reinterpret_cast<uint2*>(to) = make_uint2(h[0], h[1]);
-        *reinterpret_cast<uint2*>(to + kKvTileBytes) = make_uint2(l[0], l[1]);
-        if (d0 == 0)
-          *reinterpret_cast<float*>(stage + 4 * (r1 & 31)) = code == 255u ? NAN : p.scale * 1.4426950408889634f * e8m0_to_float(code);
-      }
       }
       fence_proxy_async_shared();
       __syncwarp();
@@ -727,17 +722,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int low = p.window ? (int)max((int64_t)-1, min((int64_t)kKvTile, place - (int64_t)p.window - j0)) : -1;
             float top = -INFINITY;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t raw[32];
-              kv_ld<32>(ts + 32 * c, raw);
-              const float4 v[2] = {sc[2 * c], sc[2 * c + 1]};
+            for (int g = 0; g < 8; ++g) {
+              uint32_t raw[16];
+              kv_ld<16>(ts + 16 * g, raw);
+              const float4 v = sc[g];
+              const float c = cq * v.x;
               kv_wait_ld();
               kv_tie(raw);
               float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                const int at = 32 * c + k;
-                if (at <= high && at > low) t4[k & 3] = fmaxf(t4[k & 3], fmaf(__uint_as_float(raw[k]), cq * v[k >> 4].x, v[k >> 4].y));
+              for (int k = 0; k < 16; ++k) {
+                const int at = 16 * g + k;
+                if (at <= high && at > low) t4[k & 3] = fmaxf(t4[k & 3], fmaf(__uint_as_float(raw[k]), c, v.y));
               }
               top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
             }
@@ -761,23 +757,25 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t raw[32], w[16];
-              kv_ld<32>(ts + 32 * c, raw);
-              const float4 v[2] = {sc[2 * c], sc[2 * c + 1]};
+            for (int g = 0; g < 8; ++g) {
+              uint32_t raw[16], w[8];
+              kv_ld<16>(ts + 16 * g, raw);
+              const float4 v = sc[g];
+              const float c = cq * v.x, add = v.y - m;
               kv_wait_ld();
               kv_tie(raw);
-              float sums[2] = {0.f, 0.f};
+              float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
-              for (int k = 0; k < 32; k += 2) {
-                const int at = 32 * c + k, g = k >> 4;
-                const float a = at <= high && at > low ? ex2(fmaf(__uint_as_float(raw[k]), cq * v[g].x, v[g].y - m)) : 0.f;
-                const float b = at + 1 <= high && at + 1 > low ? ex2(fmaf(__uint_as_float(raw[k + 1]), cq * v[g].x, v[g].y - m)) : 0.f;
-                sums[g] += a + b;
+              for (int k = 0; k < 16; k += 2) {
+                const int at = 16 * g + k;
+                const float a = at <= high && at > low ? ex2(fmaf(__uint_as_float(raw[k]), c, add)) : 0.f;
+                const float b = at + 1 <= high && at + 1 > low ? ex2(fmaf(__uint_as_float(raw[k + 1]), c, add)) : 0.f;
+                sum0 += a;
+                sum1 += b;
                 w[k >> 1] = f16x2_of(a, b);
               }
-              l = fmaf(sums[0], v[0].z, fmaf(sums[1], v[1].z, l));
-              tc::st_cols<16>(ts + 16 * c, w);
+              l = fmaf(sum0 + sum1, v.z, l);
+              tc::st_x8(ts + 8 * g, w);
             }
           }
           tc::wait_st();

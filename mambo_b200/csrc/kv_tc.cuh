@@ -13,22 +13,18 @@ namespace mambo {
 constexpr int kKvTile = 128;
 constexpr uint32_t kKvTileBytes = 128u * 128u;  // rows of 128 bytes, zero behind the head size
 
-// Waits for a barrier phase, bounded in time (the clock is read every 256 tries). The slow part is a function of its own:
-// it is in every role, and code that does not fit the SM's instruction cache is what these kernels lose most time to.
+// Waits for a barrier phase, bounded in time. A waiting warp sleeps in the try (up to 20 us, or until the phase is over):
+// tries in a loop fill the pipe that also takes the other warps' shuffles and shared-memory accesses.
 __device__ __forceinline__ bool kv_wait_slow(uint32_t bar, uint32_t parity, int site) {
-  unsigned long long t0 = 0;
+  const unsigned long long t0 = globaltimer_ns();
 #pragma unroll 1
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 255u) == 0) {
-      const unsigned long long now = globaltimer_ns();
-      if (t0 == 0) t0 = now;
-      if (*(volatile int*)&g_device_status.code != 0 || now - t0 > g_wait_limit_ns) {
-        record_timeout(site);
-        return false;
-      }
+  while (!mbar_try_wait_sleep(bar, parity, 20000u)) {
+    if (*(volatile int*)&g_device_status.code != 0 || globaltimer_ns() - t0 > g_wait_limit_ns) {
+      record_timeout(site);
+      return false;
     }
   }
+  return true;
 }
 __device__ __forceinline__ bool kv_wait(uint32_t bar, uint32_t parity, int site) {
   return mbar_try_wait(bar, parity) || kv_wait_slow(bar, parity, site);
@@ -80,6 +76,15 @@ __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
+}
+
+// The UE8M0 code of the power of two that brings a bf16 magnitude (its bits) to at most 448, 255 for NaN and infinity; as
+// mxfp8_scale_code, but for zero, and without branches: those keep the compiler from overlapping the chains of several
+// rows, and a row's chain (shuffles, code, conversions) is some 400 clocks.
+__device__ __forceinline__ uint32_t bf16_scale_code(uint32_t bits) {
+  const int biased = (int)(bits >> 7);
+  const int code = max(biased - ((bits & 0x7Fu) <= 0x60u ? 8 : 7), 0);
+  return biased == 255 ? 255u : (uint32_t)code;
 }
 
 // A row of queries as two E4M3 terms: q * 2^-e = hi + lo with e the power of two that brings its largest magnitude to at
