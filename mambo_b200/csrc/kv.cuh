@@ -69,7 +69,7 @@ struct KvAppendCall {
   const void* x[2];    // keys, values [tokens][heads][dim]
   int64_t xs_t[2], xs_h[2];
   int bf16;
-  int slots;           // CTAs: an upper bound of the pages that the call touches
+  int heads_each;      // heads of a CTA
 };
 cudaError_t launch_kv_append(KvAppendCall p, cudaStream_t stream);
 

@@ -34,26 +34,31 @@ __device__ __forceinline__ void turn_cos_sin(uint64_t phase, float& c, float& s)
   s = quarter & 2 ? -b : b;
 }
 
-// Where the 16 dimensions of a unit lie in a head. A rotated unit is 8 pairs: dimensions a .. a+7 and b .. b+7 (halves),
-// or a .. a+15 (interleaved); one behind the rotated part is a .. a+15, unchanged. `n`: its valid pairs or dimensions.
+// Where the 16 dimensions of a unit lie in a head. Interleaved pairs: dimensions a .. a+15, of which the first `turned`
+// pairs turn. Halves: dimensions a .. a+7 and b .. b+7, `turned` pairs; behind the rotated part a .. a+15, unchanged.
+// n: valid dimensions from a on (adjacent units).
 struct RotaryUnit {
-  int a, b, n;
-  bool turned, adjacent;  // adjacent: 16 dimensions in a row
+  int a, b, n, turned;
+  bool adjacent;
 };
-__host__ __device__ __forceinline__ int rotary_units(int pairs) { return (pairs + 7) / 8; }
+__host__ __device__ __forceinline__ int rotary_units(const RotaryParams& r, int dim) {
+  const int pairs = r.turns ? r.pairs : 0;
+  return r.interleaved ? (dim + 15) / 16 : (pairs + 7) / 8 + (dim - 2 * pairs + 15) / 16;
+}
 __device__ __forceinline__ RotaryUnit rotary_unit(const RotaryParams& r, int dim, int u) {
   RotaryUnit v;
-  const int pairs = r.turns ? r.pairs : 0, turned = rotary_units(pairs);
-  v.turned = u < turned;
-  v.adjacent = !v.turned || r.interleaved;
-  if (v.turned) {
-    v.a = r.interleaved ? 16 * u : 8 * u;
-    v.b = r.interleaved ? v.a + 8 : pairs + 8 * u;
-    v.n = min(8, pairs - 8 * u);
-  } else {
-    v.a = 2 * pairs + 16 * (u - turned);
+  const int pairs = r.turns ? r.pairs : 0, first = r.interleaved ? 0 : (pairs + 7) / 8;
+  v.adjacent = u >= first;
+  if (v.adjacent) {
+    v.a = (r.interleaved ? 0 : 2 * pairs) + 16 * (u - first);
     v.b = v.a + 8;
     v.n = min(16, dim - v.a);
+    v.turned = r.interleaved ? max(min(8, pairs - 8 * u), 0) : 0;
+  } else {
+    v.a = 8 * u;
+    v.b = pairs + 8 * u;
+    v.n = 0;
+    v.turned = min(8, pairs - 8 * u);
   }
   return v;
 }
@@ -85,23 +90,24 @@ __device__ __forceinline__ void unit_load(const void* x, int64_t at, const Rotar
       if constexpr (k16) return __uint_as_float((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(x) + at + d) << 16);
       return __ldg(reinterpret_cast<const float*>(x) + at + d);
     };
-    const int n0 = u.adjacent ? (u.turned ? 2 * u.n : u.n) : u.n;  // values from a on
+    const int n0 = u.adjacent ? u.n : u.turned, n1 = u.adjacent ? u.n - 8 : u.turned;  // values from a and from b on
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       lo[i] = i < n0 ? one(u.a + i) : 0.f;
-      hi[i] = u.adjacent ? (i + 8 < n0 ? one(u.a + 8 + i) : 0.f) : (i < u.n ? one(u.b + i) : 0.f);
+      hi[i] = i < n1 ? one(u.b + i) : 0.f;
     }
   }
 }
 
-// cos and sin of the unit's pairs, times the magnitude. Pairs behind the last are not turned.
+// cos and sin of the unit's pairs, times the magnitude; 1 and 0 for those that do not turn.
 __device__ __forceinline__ void unit_angles(const RotaryParams& r, const RotaryUnit& u, int pair0, int64_t position,
                                             float (&c)[8], float (&s)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint64_t f = i < u.n ? __ldg(reinterpret_cast<const unsigned long long*>(r.turns) + pair0 + i) : 0ull;
-    turn_cos_sin((uint64_t)position * f, c[i], s[i]);
-    c[i] *= r.magnitude;
+    const bool turns = i < u.turned;
+    const uint64_t f = turns ? __ldg(reinterpret_cast<const unsigned long long*>(r.turns) + pair0 + i) : 0ull;
+    turn_cos_sin((uint64_t)position * f, c[i], s[i]);  // of nothing: 1 and 0
+    c[i] *= turns ? r.magnitude : 1.f;
     s[i] *= r.magnitude * r.sign;
   }
 }
@@ -152,15 +158,11 @@ __device__ __forceinline__ void unit_store(void* out, int64_t at, const RotaryUn
       if constexpr (k16) reinterpret_cast<__nv_bfloat16*>(out)[at + d] = __float2bfloat16_rn(v);
       else reinterpret_cast<float*>(out)[at + d] = v;
     };
-    const int n0 = u.adjacent ? (u.turned ? 2 * u.n : u.n) : u.n;
+    const int n0 = u.adjacent ? u.n : u.turned, n1 = u.adjacent ? u.n - 8 : u.turned;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (i < n0) one(u.a + i, lo[i]);
-      if (u.adjacent) {
-        if (i + 8 < n0) one(u.a + 8 + i, hi[i]);
-      } else if (i < u.n) {
-        one(u.b + i, hi[i]);
-      }
+      if (i < n1) one(u.b + i, hi[i]);
     }
   }
 }
@@ -182,7 +184,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
     const int h = g + i * p.groups;
     if (h < p.heads) unit_load<kVec, k16>(p.x, token * p.xs_t + h * p.xs_h, u, lo[i], hi[i]);
   }
-  if (u.turned) {
+  if (u.turned > 0) {
     const int64_t position = p.positions64 ? __ldg(reinterpret_cast<const long long*>(p.positions) + token)
                                            : (int64_t)__ldg(reinterpret_cast<const int*>(p.positions) + token);
     float c[8], s[8];
@@ -204,15 +206,67 @@ const void* rotary_variant(int per) {
 }
 
 // ---------------------------------------------------------------------------
-// Append. A CTA has one page, one head, and its keys or its values: it takes
-// the new tokens' values into registers (turned), finds their largest
-// magnitude, decides the page's scale, rescales what the page already holds
-// where the scale has grown, and writes the codes. One pass over the input.
+// Append. A CTA has one page and its keys or its values of some heads, one
+// after the other: it takes the head's new values into registers (turned),
+// finds their largest magnitude, decides the page's scale, rescales what the
+// page already holds where the scale has grown, and writes the codes. One pass
+// over the input. A thread has the same tokens and dimensions in every head,
+// so that it keeps their cosines and sines; the next head's values are on
+// their way while one is quantized.
 // ---------------------------------------------------------------------------
-constexpr int kAppendThreads = 256;
-// Units of a thread: a page has at most 128 tokens x 8 units of 16 dimensions, or 9 where the rotated part ends inside one.
+// Units of a thread: one in the vector form, which keeps its registers at 64 (a page of 64 tokens with two units a thread
+// and 128 registers took 42 us for 16384 tokens).
 template <bool kVec>
-constexpr int kAppendPasses = kVec ? 4 : 5;
+constexpr int kAppendPasses = kVec ? 1 : 2;
+template <bool kVec>
+constexpr int kAppendThreads = kVec ? 1024 : 640;  // most, of a CTA: 128 tokens x 8 units, or 9 where the rotated part ends inside one
+
+// A unit's values as they come: 16 bf16, or 16 floats.
+template <bool kVec, bool k16>
+struct RawUnit {
+  static constexpr bool kPacked = kVec && k16;
+  uint4 w[kPacked ? 2 : 4];
+  __device__ __forceinline__ void load(const void* x, int64_t at, const RotaryUnit& u) {
+    if constexpr (kPacked) {
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(x) + at;
+      w[0] = __ldg(reinterpret_cast<const uint4*>(p + u.a));
+      w[1] = __ldg(reinterpret_cast<const uint4*>(p + u.b));
+    } else {
+      float lo[8], hi[8];
+      unit_load<kVec, k16>(x, at, u, lo, hi);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        w[i] = make_uint4(__float_as_uint(lo[4 * i]), __float_as_uint(lo[4 * i + 1]), __float_as_uint(lo[4 * i + 2]), __float_as_uint(lo[4 * i + 3]));
+        w[2 + i] = make_uint4(__float_as_uint(hi[4 * i]), __float_as_uint(hi[4 * i + 1]), __float_as_uint(hi[4 * i + 2]), __float_as_uint(hi[4 * i + 3]));
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&lo)[8], float (&hi)[8]) const {
+    if constexpr (kPacked) {
+      const uint32_t l[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, h[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo[2 * i] = __uint_as_float(l[i] << 16);
+        lo[2 * i + 1] = __uint_as_float(l[i] & 0xFFFF0000u);
+        hi[2 * i] = __uint_as_float(h[i] << 16);
+        hi[2 * i + 1] = __uint_as_float(h[i] & 0xFFFF0000u);
+      }
+    } else {
+      const uint32_t* f = reinterpret_cast<const uint32_t*>(w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        lo[i] = __uint_as_float(f[i]);
+        hi[i] = __uint_as_float(f[8 + i]);
+      }
+    }
+  }
+};
+// The larger magnitude of three, NaN if any is.
+__device__ __forceinline__ float absmax3(float m, float a, float b) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(a), "f"(b));
+  return d;
+}
 
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return cvt_e4m3x2_rn(a, b) | (cvt_e4m3x2_rn(c, d) << 16);
@@ -233,11 +287,12 @@ __device__ __forceinline__ int append_slot(const KvSequences& s, int b, int log_
 }
 
 template <bool kVec, bool k16>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ KvAppendCall p) {
-  __shared__ uint32_t sm_max[kAppendThreads / 32];
-  const int which = blockIdx.z, head = blockIdx.y, threads = blockDim.x;
+__global__ void __launch_bounds__(kAppendThreads<kVec>) kv_append_kernel(const __grid_constant__ KvAppendCall p) {
+  __shared__ float sm_max[2][32];
+  const int which = blockIdx.z, threads = blockDim.x;
   const KvCache& cache = p.cache;
   const int page = cache.page, dim = cache.dim;
+  const int head0 = blockIdx.y * p.heads_each, head1 = min(head0 + p.heads_each, cache.heads);
   pdl_wait();
   pdl_launch_dependents();
   int b = blockIdx.x, at = 0;
@@ -263,102 +318,101 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
   const int64_t where = __ldg(p.seq.table + b * p.seq.table_stride + block);
   if (where < 0 || where >= cache.pages) return;
   const int begun = (int)(t0 & (page - 1)), count = (int)(t1 - t0);  // tokens before the call's, and the call's
-  const int64_t token0 = span.first + (t0 - past);
 
-  const RotaryParams rot = which == 0 ? p.rot : RotaryParams{nullptr, 0, 0, 1.f, 1.f};
-  const int pairs = rot.turns ? rot.pairs : 0;
-  const int units = rotary_units(pairs) + (dim - 2 * pairs + 15) / 16, all = count * units;
-  const int64_t xs_t = p.xs_t[which], xs_h = p.xs_h[which];
+  RotaryParams rot = p.rot;
+  if (which == 1) rot = RotaryParams{nullptr, 0, 0, 1.f, 1.f};
+  const int units = rotary_units(rot, dim), all = count * units;
+  const int64_t xs_h = p.xs_h[which];
   constexpr int kPasses = kAppendPasses<kVec>;
-  float lo[kPasses][8], hi[kPasses][8];
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int f = threadIdx.x + i * threads;
-    if (f < all) {
-      const int row = f / units;
-      unit_load<kVec, k16>(p.x[which], (token0 + row) * xs_t + head * xs_h, rotary_unit(rot, dim, f - row * units), lo[i], hi[i]);
-    }
-  }
-  uint32_t top = 0;  // magnitudes as integers: NaN and infinity order above every number
+  int64_t from[kPasses];
+  RotaryUnit u[kPasses];
+  float c[kPasses][8], s[kPasses][8];
+  RawUnit<kVec, k16> raw[kPasses];
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const int f = threadIdx.x + i * threads;
     if (f < all) {
       const int row = f / units, unit = f - row * units;
-      const RotaryUnit u = rotary_unit(rot, dim, unit);
-      if (u.turned) {
-        float c[8], s[8];
-        unit_angles(rot, u, 8 * unit, t0 + row, c, s);
-        unit_turn(rot.interleaved, c, s, lo[i], hi[i]);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        top = max(top, max(__float_as_uint(lo[i][j]) & 0x7FFFFFFFu, __float_as_uint(hi[i][j]) & 0x7FFFFFFFu));
+      u[i] = rotary_unit(rot, dim, unit);
+      from[i] = (span.first + (t0 - past) + row) * p.xs_t[which];
+      raw[i].load(p.x[which], from[i] + head0 * xs_h, u[i]);
+      if (u[i].turned > 0) unit_angles(rot, u[i], 8 * unit, t0 + row, c[i], s[i]);
     }
   }
-  top = __reduce_max_sync(0xFFFFFFFFu, top);
-  if ((threadIdx.x & 31) == 0) sm_max[threadIdx.x >> 5] = top;
-  uint8_t* scale_at = cache.scales[which] + where * cache.heads + head;
-  const uint32_t old = begun ? *scale_at : 0u;
-  __syncthreads();
-  for (int w = 0; w < threads / 32; ++w) top = max(top, sm_max[w]);
-  const uint32_t need = top ? max(mxfp8_scale_code(__uint_as_float(top)), kKvMinCode) : kKvMinCode;
-  const uint32_t code = max(need, old);  // 255 stays
-  uint8_t* codes = cache.codes[which] + (where * cache.heads + head) * (int64_t)(page * dim);
-  if (begun && code > old && code != 255u) {
-    const int d = (int)old - (int)code;  // < 0
-    const float f = d < -126 ? 0.f : __uint_as_float((uint32_t)(127 + d) << 23);
-    for (int i = threadIdx.x; i < begun * dim / 16; i += threads) {
-      uint4 v = reinterpret_cast<uint4*>(codes)[i];
-      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+  for (int head = head0; head < head1; ++head) {
+    uint8_t* scale_at = cache.scales[which] + where * cache.heads + head;
+    const uint32_t old = begun ? *scale_at : 0u;
+    float lo[kPasses][8], hi[kPasses][8];
+    float top = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = rescale_e4m3x2(w[j], f) | (rescale_e4m3x2(w[j] >> 16, f) << 16);
-      reinterpret_cast<uint4*>(codes)[i] = v;
-    }
-  }
-  const float inv = code == 255u ? 0.f : e8m0_to_float(254u - code);
+    for (int i = 0; i < kPasses; ++i) {
+      if ((int)threadIdx.x + i * threads < all) {
+        raw[i].get(lo[i], hi[i]);
+        if (head + 1 < head1) raw[i].load(p.x[which], from[i] + (head + 1) * xs_h, u[i]);
+        if (u[i].turned > 0) unit_turn(rot.interleaved, c[i], s[i], lo[i], hi[i]);
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int f = threadIdx.x + i * threads;
-    if (f < all) {
-      const int row = f / units;
-      const RotaryUnit u = rotary_unit(rot, dim, f - row * units);
-      uint8_t* to = codes + (begun + row) * dim;
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        w[j] = e4m3x4(lo[i][4 * j] * inv, lo[i][4 * j + 1] * inv, lo[i][4 * j + 2] * inv, lo[i][4 * j + 3] * inv);
-        w[2 + j] = e4m3x4(hi[i][4 * j] * inv, hi[i][4 * j + 1] * inv, hi[i][4 * j + 2] * inv, hi[i][4 * j + 3] * inv);
+        for (int j = 0; j < 8; ++j) top = absmax3(top, lo[i][j], hi[i][j]);
       }
-      if (code == 255u) w[0] = w[1] = w[2] = w[3] = 0u;  // zero times NaN has a code of its own
-      if constexpr (kVec) {
-        *reinterpret_cast<uint2*>(to + u.a) = make_uint2(w[0], w[1]);
-        *reinterpret_cast<uint2*>(to + u.b) = make_uint2(w[2], w[3]);
-      } else {
-        const int n0 = u.adjacent ? (u.turned ? 2 * u.n : u.n) : u.n;
+    }
+    // As integers: NaN and infinity order above every number.
+    const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top) & 0x7FFFFFFFu);
+    float* maxima = sm_max[head & 1];
+    if ((threadIdx.x & 31) == 0) maxima[threadIdx.x >> 5] = __uint_as_float(most);
+    __syncthreads();
+    uint32_t bits = 0;
+    for (int w = 0; w < threads / 32; ++w) bits = max(bits, __float_as_uint(maxima[w]));
+    const uint32_t need = bits ? max(mxfp8_scale_code(__uint_as_float(bits)), kKvMinCode) : kKvMinCode;
+    const uint32_t code = max(need, old);  // 255 stays
+    uint8_t* codes = cache.codes[which] + (where * cache.heads + head) * (int64_t)(page * dim);
+    if (begun && code > old && code != 255u) {
+      const int d = (int)old - (int)code;  // < 0
+      const float f = d < -126 ? 0.f : __uint_as_float((uint32_t)(127 + d) << 23);
+      for (int i = threadIdx.x; i < begun * dim / 16; i += threads) {
+        uint4 v = reinterpret_cast<uint4*>(codes)[i];
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint8_t l = (uint8_t)(w[j >> 2] >> (8 * (j & 3))), h = (uint8_t)(w[2 + (j >> 2)] >> (8 * (j & 3)));
-          if (j < n0) to[u.a + j] = l;
-          if (u.adjacent) {
-            if (j + 8 < n0) to[u.a + 8 + j] = h;
-          } else if (j < u.n) {
-            to[u.b + j] = h;
+        for (int j = 0; j < 4; ++j) w[j] = rescale_e4m3x2(w[j], f) | (rescale_e4m3x2(w[j] >> 16, f) << 16);
+        reinterpret_cast<uint4*>(codes)[i] = v;
+      }
+    }
+    const float inv = code == 255u ? 0.f : e8m0_to_float(254u - code);
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int f = threadIdx.x + i * threads;
+      if (f < all) {
+        uint8_t* to = codes + (begun + f / units) * dim;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          w[j] = e4m3x4(lo[i][4 * j] * inv, lo[i][4 * j + 1] * inv, lo[i][4 * j + 2] * inv, lo[i][4 * j + 3] * inv);
+          w[2 + j] = e4m3x4(hi[i][4 * j] * inv, hi[i][4 * j + 1] * inv, hi[i][4 * j + 2] * inv, hi[i][4 * j + 3] * inv);
+        }
+        if (code == 255u) w[0] = w[1] = w[2] = w[3] = 0u;  // zero times NaN has a code of its own
+        if constexpr (kVec) {
+          *reinterpret_cast<uint2*>(to + u[i].a) = make_uint2(w[0], w[1]);
+          *reinterpret_cast<uint2*>(to + u[i].b) = make_uint2(w[2], w[3]);
+        } else {
+          const int n0 = u[i].adjacent ? u[i].n : u[i].turned, n1 = u[i].adjacent ? u[i].n - 8 : u[i].turned;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (j < n0) to[u[i].a + j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+            if (j < n1) to[u[i].b + j] = (uint8_t)(w[2 + (j >> 2)] >> (8 * (j & 3)));
           }
         }
       }
     }
+    if (threadIdx.x == 0) *scale_at = (uint8_t)code;
   }
-  if (threadIdx.x == 0) *scale_at = (uint8_t)code;
 }
 
 }  // namespace
 
 cudaError_t launch_rotary(RotaryCall p, cudaStream_t stream) {
-  const int pairs = p.rot.pairs, es = p.bf16 ? 2 : 4;
-  p.units = rotary_units(pairs) + (p.dim - 2 * pairs + 15) / 16;
-  const bool vec = p.dim % 16 == 0 && pairs % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.out % 16 == 0 &&
-                   p.xs_t * es % 16 == 0 && p.xs_h * es % 16 == 0 && p.os_t * es % 16 == 0 && p.os_h * es % 16 == 0;
+  const int es = p.bf16 ? 2 : 4;
+  p.units = rotary_units(p.rot, p.dim);
+  const bool vec = p.dim % 16 == 0 && (p.rot.interleaved || p.rot.pairs % 8 == 0) && (uintptr_t)p.x % 16 == 0 &&
+                   (uintptr_t)p.out % 16 == 0 && p.xs_t * es % 16 == 0 && p.xs_h * es % 16 == 0 && p.os_t * es % 16 == 0 &&
+                   p.os_h * es % 16 == 0;
   const int64_t head_units = (int64_t)p.tokens * p.heads * p.units;
   const int per = head_units >= 4ll << 18 ? 4 : head_units >= 2ll << 18 ? 2 : 1;
   p.groups = (p.heads + per - 1) / per;
@@ -369,16 +423,20 @@ cudaError_t launch_rotary(RotaryCall p, cudaStream_t stream) {
 }
 
 cudaError_t launch_kv_append(KvAppendCall p, cudaStream_t stream) {
-  const int es = p.bf16 ? 2 : 4, pairs = p.rot.turns ? p.rot.pairs : 0;
-  bool vec = pairs % 8 == 0;
+  const int es = p.bf16 ? 2 : 4;
+  bool vec = !p.rot.turns || p.rot.interleaved || p.rot.pairs % 8 == 0;
   for (int i = 0; i < 2; ++i)
     vec = vec && (uintptr_t)p.x[i] % 16 == 0 && p.xs_t[i] * es % 16 == 0 && p.xs_h[i] * es % 16 == 0;
-  p.slots = p.seq.offsets ? (p.seq.tokens >> p.cache.log_page) + 2 * p.seq.batch : p.seq.batch;
-  // One token a sequence is at most 9 units and needs a warp; a page's tokens keep 256 threads busy.
-  const int threads = p.seq.offsets ? kAppendThreads : 32;
+  const int slots = p.seq.offsets ? (p.seq.tokens >> p.cache.log_page) + 2 * p.seq.batch : p.seq.batch;
+  // One token a sequence is at most 9 units and needs a warp.
+  const int units = max(rotary_units(p.rot, p.cache.dim), (p.cache.dim + 15) / 16), page_units = p.cache.page * units;
+  const int threads = !p.seq.offsets ? 32 : ((vec ? page_units : (page_units + 1) / 2) + 31) / 32 * 32;
+  // Heads of a CTA: as many as leave 8 CTAs an SM.
+  p.heads_each = max(1, min(p.cache.heads, (int)((int64_t)slots * p.cache.heads * 2 / (148 * 8))));
+  const unsigned groups = (unsigned)((p.cache.heads + p.heads_each - 1) / p.heads_each);
   const void* k = p.bf16 ? (vec ? (const void*)kv_append_kernel<true, true> : (const void*)kv_append_kernel<false, true>)
                          : (vec ? (const void*)kv_append_kernel<true, false> : (const void*)kv_append_kernel<false, false>);
-  return launch_pdl(k, dim3((unsigned)p.slots, (unsigned)p.cache.heads, 2), dim3(threads), 0, stream, p);
+  return launch_pdl(k, dim3((unsigned)slots, groups, 2), dim3(threads), 0, stream, p);
 }
 
 }  // namespace mambo
