@@ -99,6 +99,46 @@ __device__ __forceinline__ void unit_load(const void* x, int64_t at, const Rotar
   }
 }
 
+// A unit's values as they come: 16 bf16, or 16 floats.
+template <bool kVec, bool k16>
+struct RawUnit {
+  static constexpr bool kPacked = kVec && k16;
+  uint4 w[kPacked ? 2 : 4];
+  __device__ __forceinline__ void load(const void* x, int64_t at, const RotaryUnit& u) {
+    if constexpr (kPacked) {
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(x) + at;
+      w[0] = __ldg(reinterpret_cast<const uint4*>(p + u.a));
+      w[1] = __ldg(reinterpret_cast<const uint4*>(p + u.b));
+    } else {
+      float lo[8], hi[8];
+      unit_load<kVec, k16>(x, at, u, lo, hi);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        w[i] = make_uint4(__float_as_uint(lo[4 * i]), __float_as_uint(lo[4 * i + 1]), __float_as_uint(lo[4 * i + 2]), __float_as_uint(lo[4 * i + 3]));
+        w[2 + i] = make_uint4(__float_as_uint(hi[4 * i]), __float_as_uint(hi[4 * i + 1]), __float_as_uint(hi[4 * i + 2]), __float_as_uint(hi[4 * i + 3]));
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&lo)[8], float (&hi)[8]) const {
+    if constexpr (kPacked) {
+      const uint32_t l[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, h[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo[2 * i] = __uint_as_float(l[i] << 16);
+        lo[2 * i + 1] = __uint_as_float(l[i] & 0xFFFF0000u);
+        hi[2 * i] = __uint_as_float(h[i] << 16);
+        hi[2 * i + 1] = __uint_as_float(h[i] & 0xFFFF0000u);
+      }
+    } else {
+      const uint32_t* f = reinterpret_cast<const uint32_t*>(w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        lo[i] = __uint_as_float(f[i]);
+        hi[i] = __uint_as_float(f[8 + i]);
+      }
+    }
+  }
+};
 // cos and sin of the unit's pairs, times the magnitude; 1 and 0 for those that do not turn.
 __device__ __forceinline__ void unit_angles(const RotaryParams& r, const RotaryUnit& u, int pair0, int64_t position,
                                             float (&c)[8], float (&s)[8]) {
@@ -169,7 +209,7 @@ __device__ __forceinline__ void unit_store(void* out, int64_t at, const RotaryUn
 
 // A unit's angles need its first pair's number: 8 per rotated unit.
 template <bool kVec, bool k16, int kPer>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryCall p) {
+__global__ void __launch_bounds__(256, kPer == 4 && kVec && k16 ? 3 : 1) rotary_kernel(const __grid_constant__ RotaryCall p) {
   const int64_t job = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int per_token = p.units * p.groups;
   const int64_t token = job / per_token;
@@ -178,24 +218,29 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
   if (token >= p.tokens) return;
   const int in = (int)(job - token * per_token), g = in / p.units, unit = in - g * p.units;
   const RotaryUnit u = rotary_unit(p.rot, p.dim, unit);
-  float lo[kPer][8], hi[kPer][8];
+  RawUnit<kVec, k16> raw[kPer];
+  const int64_t from = token * p.xs_t, to = token * p.os_t;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int h = g + i * p.groups;
-    if (h < p.heads) unit_load<kVec, k16>(p.x, token * p.xs_t + h * p.xs_h, u, lo[i], hi[i]);
+    if (h < p.heads) raw[i].load(p.x, from + h * p.xs_h, u);
   }
-  if (u.turned > 0) {
+  float c[8], s[8];
+  const bool turns = u.turned > 0;
+  if (turns) {
     const int64_t position = p.positions64 ? __ldg(reinterpret_cast<const long long*>(p.positions) + token)
                                            : (int64_t)__ldg(reinterpret_cast<const int*>(p.positions) + token);
-    float c[8], s[8];
     unit_angles(p.rot, u, 8 * unit, position, c, s);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) unit_turn(p.rot.interleaved, c, s, lo[i], hi[i]);
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int h = g + i * p.groups;
-    if (h < p.heads) unit_store<kVec, k16>(p.out, token * p.os_t + h * p.os_h, u, lo[i], hi[i]);
+    if (h < p.heads) {
+      float lo[8], hi[8];
+      raw[i].get(lo, hi);
+      if (turns) unit_turn(p.rot.interleaved, c, s, lo, hi);
+      unit_store<kVec, k16>(p.out, to + h * p.os_h, u, lo, hi);
+    }
   }
 }
 
@@ -221,46 +266,11 @@ constexpr int kAppendPasses = kVec ? 1 : 2;
 template <bool kVec>
 constexpr int kAppendThreads = kVec ? 1024 : 640;  // most, of a CTA: 128 tokens x 8 units, or 9 where the rotated part ends inside one
 
-// A unit's values as they come: 16 bf16, or 16 floats.
-template <bool kVec, bool k16>
-struct RawUnit {
-  static constexpr bool kPacked = kVec && k16;
-  uint4 w[kPacked ? 2 : 4];
-  __device__ __forceinline__ void load(const void* x, int64_t at, const RotaryUnit& u) {
-    if constexpr (kPacked) {
-      const uint16_t* p = reinterpret_cast<const uint16_t*>(x) + at;
-      w[0] = __ldg(reinterpret_cast<const uint4*>(p + u.a));
-      w[1] = __ldg(reinterpret_cast<const uint4*>(p + u.b));
-    } else {
-      float lo[8], hi[8];
-      unit_load<kVec, k16>(x, at, u, lo, hi);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        w[i] = make_uint4(__float_as_uint(lo[4 * i]), __float_as_uint(lo[4 * i + 1]), __float_as_uint(lo[4 * i + 2]), __float_as_uint(lo[4 * i + 3]));
-        w[2 + i] = make_uint4(__float_as_uint(hi[4 * i]), __float_as_uint(hi[4 * i + 1]), __float_as_uint(hi[4 * i + 2]), __float_as_uint(hi[4 * i + 3]));
-      }
-    }
-  }
-  __device__ __forceinline__ void get(float (&lo)[8], float (&hi)[8]) const {
-    if constexpr (kPacked) {
-      const uint32_t l[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, h[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lo[2 * i] = __uint_as_float(l[i] << 16);
-        lo[2 * i + 1] = __uint_as_float(l[i] & 0xFFFF0000u);
-        hi[2 * i] = __uint_as_float(h[i] << 16);
-        hi[2 * i + 1] = __uint_as_float(h[i] & 0xFFFF0000u);
-      }
-    } else {
-      const uint32_t* f = reinterpret_cast<const uint32_t*>(w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        lo[i] = __uint_as_float(f[i]);
-        hi[i] = __uint_as_float(f[8 + i]);
-      }
-    }
-  }
-};
+// mxfp8_scale_code from a magnitude's bits, without branches; of zero 0.
+__device__ __forceinline__ uint32_t f32_scale_code(uint32_t bits) {
+  const int biased = (int)(bits >> 23), code = max(biased - ((bits & 0x7FFFFFu) <= 0x600000u ? 8 : 7), 0);
+  return biased == 255 ? 255u : (uint32_t)code;
+}
 // The larger magnitude of three, NaN if any is.
 __device__ __forceinline__ float absmax3(float m, float a, float b) {
   float d;
@@ -316,7 +326,6 @@ __global__ void __launch_bounds__(kAppendThreads<kVec>) kv_append_kernel(const _
   const int64_t t0 = max(past, block << cache.log_page), t1 = min(past + span.count, (block + 1) << cache.log_page);
   if (at < 0 || t0 >= t1 || block >= p.seq.table_pages) return;
   const int64_t where = __ldg(p.seq.table + b * p.seq.table_stride + block);
-  if (where < 0 || where >= cache.pages) return;
   const int begun = (int)(t0 & (page - 1)), count = (int)(t1 - t0);  // tokens before the call's, and the call's
 
   RotaryParams rot = p.rot;
@@ -324,7 +333,9 @@ __global__ void __launch_bounds__(kAppendThreads<kVec>) kv_append_kernel(const _
   const int units = rotary_units(rot, dim), all = count * units;
   const int64_t xs_h = p.xs_h[which];
   constexpr int kPasses = kAppendPasses<kVec>;
-  int64_t from[kPasses];
+  constexpr bool kAhead = kVec && k16;  // the other forms have no registers for it
+  int64_t from[kPasses];  // this thread's tokens: in the input, and their codes in the page
+  int to[kPasses];
   RotaryUnit u[kPasses];
   float c[kPasses][8], s[kPasses][8];
   RawUnit<kVec, k16> raw[kPasses];
@@ -335,20 +346,27 @@ __global__ void __launch_bounds__(kAppendThreads<kVec>) kv_append_kernel(const _
       const int row = f / units, unit = f - row * units;
       u[i] = rotary_unit(rot, dim, unit);
       from[i] = (span.first + (t0 - past) + row) * p.xs_t[which];
-      raw[i].load(p.x[which], from[i] + head0 * xs_h, u[i]);
+      to[i] = (begun + row) * dim;
+      if constexpr (kAhead) raw[i].load(p.x[which], from[i] + head0 * xs_h, u[i]);
       if (u[i].turned > 0) unit_angles(rot, u[i], 8 * unit, t0 + row, c[i], s[i]);
     }
   }
-  for (int head = head0; head < head1; ++head) {
-    uint8_t* scale_at = cache.scales[which] + where * cache.heads + head;
+  if (where < 0 || where >= cache.pages) return;  // (after the values' loads, which do not wait for the page)
+  uint8_t* scale_at = cache.scales[which] + where * cache.heads + head0;
+  uint8_t* codes = cache.codes[which] + (where * cache.heads + head0) * (int64_t)(page * dim);
+  const int lane = threadIdx.x & 31, warps = threads / 32;
+  for (int head = head0; head < head1; ++head, ++scale_at, codes += page * dim) {
     const uint32_t old = begun ? *scale_at : 0u;
     float lo[kPasses][8], hi[kPasses][8];
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       if ((int)threadIdx.x + i * threads < all) {
+        if constexpr (!kAhead) raw[i].load(p.x[which], from[i] + head * xs_h, u[i]);
         raw[i].get(lo[i], hi[i]);
-        if (head + 1 < head1) raw[i].load(p.x[which], from[i] + (head + 1) * xs_h, u[i]);
+        if constexpr (kAhead) {
+          if (head + 1 < head1) raw[i].load(p.x[which], from[i] + (head + 1) * xs_h, u[i]);
+        }
         if (u[i].turned > 0) unit_turn(rot.interleaved, c[i], s[i], lo[i], hi[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = absmax3(top, lo[i][j], hi[i][j]);
@@ -357,13 +375,11 @@ __global__ void __launch_bounds__(kAppendThreads<kVec>) kv_append_kernel(const _
     // As integers: NaN and infinity order above every number.
     const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top) & 0x7FFFFFFFu);
     float* maxima = sm_max[head & 1];
-    if ((threadIdx.x & 31) == 0) maxima[threadIdx.x >> 5] = __uint_as_float(most);
+    if (lane == 0) maxima[threadIdx.x >> 5] = __uint_as_float(most);
     __syncthreads();
-    uint32_t bits = 0;
-    for (int w = 0; w < threads / 32; ++w) bits = max(bits, __float_as_uint(maxima[w]));
-    const uint32_t need = bits ? max(mxfp8_scale_code(__uint_as_float(bits)), kKvMinCode) : kKvMinCode;
-    const uint32_t code = max(need, old);  // 255 stays
-    uint8_t* codes = cache.codes[which] + (where * cache.heads + head) * (int64_t)(page * dim);
+    const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? __float_as_uint(maxima[lane]) : 0u);
+    // 255 stays; zero takes the smallest scale.
+    const uint32_t code = max(max(f32_scale_code(bits), kKvMinCode), old);
     if (begun && code > old && code != 255u) {
       const int d = (int)old - (int)code;  // < 0
       const float f = d < -126 ? 0.f : __uint_as_float((uint32_t)(127 + d) << 23);
@@ -380,7 +396,7 @@ __global__ void __launch_bounds__(kAppendThreads<kVec>) kv_append_kernel(const _
     for (int i = 0; i < kPasses; ++i) {
       const int f = threadIdx.x + i * threads;
       if (f < all) {
-        uint8_t* to = codes + (begun + f / units) * dim;
+        uint8_t* at = codes + to[i];
         uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -389,14 +405,14 @@ __global__ void __launch_bounds__(kAppendThreads<kVec>) kv_append_kernel(const _
         }
         if (code == 255u) w[0] = w[1] = w[2] = w[3] = 0u;  // zero times NaN has a code of its own
         if constexpr (kVec) {
-          *reinterpret_cast<uint2*>(to + u[i].a) = make_uint2(w[0], w[1]);
-          *reinterpret_cast<uint2*>(to + u[i].b) = make_uint2(w[2], w[3]);
+          *reinterpret_cast<uint2*>(at + u[i].a) = make_uint2(w[0], w[1]);
+          *reinterpret_cast<uint2*>(at + u[i].b) = make_uint2(w[2], w[3]);
         } else {
           const int n0 = u[i].adjacent ? u[i].n : u[i].turned, n1 = u[i].adjacent ? u[i].n - 8 : u[i].turned;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            if (j < n0) to[u[i].a + j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
-            if (j < n1) to[u[i].b + j] = (uint8_t)(w[2 + (j >> 2)] >> (8 * (j & 3)));
+            if (j < n0) at[u[i].a + j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+            if (j < n1) at[u[i].b + j] = (uint8_t)(w[2 + (j >> 2)] >> (8 * (j & 3)));
           }
         }
       }
@@ -414,7 +430,8 @@ cudaError_t launch_rotary(RotaryCall p, cudaStream_t stream) {
                    (uintptr_t)p.out % 16 == 0 && p.xs_t * es % 16 == 0 && p.xs_h * es % 16 == 0 && p.os_t * es % 16 == 0 &&
                    p.os_h * es % 16 == 0;
   const int64_t head_units = (int64_t)p.tokens * p.heads * p.units;
-  const int per = head_units >= 4ll << 18 ? 4 : head_units >= 2ll << 18 ? 2 : 1;
+  // Heads of a thread, which share its cosines and sines: four or two where that leaves 512 threads an SM.
+  const int per = head_units >= 4 * 148 * 512 ? 4 : head_units >= 2 * 148 * 512 ? 2 : 1;
   p.groups = (p.heads + per - 1) / per;
   const int64_t jobs = (int64_t)p.tokens * p.groups * p.units;
   const void* k = p.bf16 ? (vec ? rotary_variant<true, true>(per) : rotary_variant<false, true>(per))
@@ -431,8 +448,8 @@ cudaError_t launch_kv_append(KvAppendCall p, cudaStream_t stream) {
   // One token a sequence is at most 9 units and needs a warp.
   const int units = max(rotary_units(p.rot, p.cache.dim), (p.cache.dim + 15) / 16), page_units = p.cache.page * units;
   const int threads = !p.seq.offsets ? 32 : ((vec ? page_units : (page_units + 1) / 2) + 31) / 32 * 32;
-  // Heads of a CTA: as many as leave 8 CTAs an SM.
-  p.heads_each = max(1, min(p.cache.heads, (int)((int64_t)slots * p.cache.heads * 2 / (148 * 8))));
+  // Heads of a CTA: as many as leave six CTAs an SM.
+  p.heads_each = max(1, min(p.cache.heads, (int)((int64_t)slots * p.cache.heads * 2 / (148 * 6))));
   const unsigned groups = (unsigned)((p.cache.heads + p.heads_each - 1) / p.heads_each);
   const void* k = p.bf16 ? (vec ? (const void*)kv_append_kernel<true, true> : (const void*)kv_append_kernel<false, true>)
                          : (vec ? (const void*)kv_append_kernel<true, false> : (const void*)kv_append_kernel<false, false>);
