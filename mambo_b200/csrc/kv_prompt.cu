@@ -47,6 +47,7 @@ constexpr int kUnitRows = 2 * kRows;
 constexpr int kKStages = 3, kVStages = 2;
 constexpr float kNone = -1e30f;       // m of a row that has seen nothing
 constexpr float kMostSum = 2048.f;    // of 16 weights, before m is moved: f16 holds 2^16
+constexpr float kMostPoly = 100.f;    // of the exponents that the polynomial takes: a larger one would not show in its sum
 // What a unit costs besides its tiles, in tiles: where the ranges of the CTAs are cut, units count as this much longer.
 constexpr int kUnitCost = 6;
 
@@ -183,11 +184,13 @@ __device__ __forceinline__ float low_of(uint64_t a) { return __uint_as_float((ui
 __device__ __forceinline__ float high_of(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
 // 2^x of a pair in the FMA pipe, which has room where the special function unit has none. x = n + f with n the nearest
 // integer (read off the low bits of x + 1.5 * 2^23), f in [-1/2, 1/2]; 2^f is the minimax polynomial of degree 4 (by
-// Remez' exchange, relative error 2.6e-6); n is added to its exponent. x is at most about 10; below -126 it counts as that.
-__device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
+// Remez' exchange, relative error 2.6e-6); n is added to its exponent, which holds for x up to 127: `top` tells the caller.
+// Below -126 x counts as that.
+__device__ __forceinline__ uint64_t ex2_poly(uint64_t x, float& top) {
   float a, b;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(low_of(x)), "f"(-126.f));
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(high_of(x)), "f"(-126.f));
+  asm("max.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(a), "f"(b));
   x = pack2(a, b);
   const uint64_t n = add_2(x, pack2(12582912.f, 12582912.f));
   const uint64_t f = add_2(x, fma_2(n, pack2(-1.f, -1.f), pack2(12582912.f, 12582912.f)));
@@ -553,30 +556,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(kUfree + 8 * ur.at);
       ur.next(kUnitStages);
       for (int tile = 0; tile < n; ++tile, ++it, j += kKvTile) {
-      const bool none = j > above || j <= below;
-      kv_warp_wait(kVfull + 8 * vr.at, vr.phase, kSiteKvFull);
-      if (it >= 2) kv_warp_wait(kFfree + 8 * fr.at, fr.phase ^ 1, kSiteKvEmpty);
-      const uint8_t* from = sm + kAtV + vr.at * kKvTileBytes + i * 128;
-      uint8_t* to = sm + kAtVf + fr.at * kVf + i * 128;
+        const bool none = j > above || j <= below;
+        kv_warp_wait(kVfull + 8 * vr.at, vr.phase, kSiteKvFull);
+        if (it >= 2) kv_warp_wait(kFfree + 8 * fr.at, fr.phase ^ 1, kSiteKvEmpty);
+        const uint8_t* from = sm + kAtV + vr.at * kKvTileBytes + i * 128;
+        uint8_t* to = sm + kAtVf + fr.at * kVf + i * 128;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint4 v = *reinterpret_cast<const uint4*>(from + ((c ^ (i & 7)) << 4));
-        if (none) v = make_uint4(0, 0, 0, 0);
-        uint8_t* half = to + (c >> 2) * kKvTileBytes;
-        const int c0 = 2 * (c & 3);
-        *reinterpret_cast<uint4*>(half + ((c0 ^ (i & 7)) << 4)) =
-            make_uint4(f16x2_of_e4m3x2(v.x & 0xFFFFu), f16x2_of_e4m3x2(v.x >> 16), f16x2_of_e4m3x2(v.y & 0xFFFFu), f16x2_of_e4m3x2(v.y >> 16));
-        *reinterpret_cast<uint4*>(half + (((c0 + 1) ^ (i & 7)) << 4)) =
-            make_uint4(f16x2_of_e4m3x2(v.z & 0xFFFFu), f16x2_of_e4m3x2(v.z >> 16), f16x2_of_e4m3x2(v.w & 0xFFFFu), f16x2_of_e4m3x2(v.w >> 16));
-      }
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(kVfree + 8 * vr.at);
-        mbar_arrive(kFfull + 8 * fr.at);
-      }
-      vr.next(kVStages);
-      fr.next(2);
+        for (int c = 0; c < 8; ++c) {
+          uint4 v = *reinterpret_cast<const uint4*>(from + ((c ^ (i & 7)) << 4));
+          if (none) v = make_uint4(0, 0, 0, 0);
+          uint8_t* half = to + (c >> 2) * kKvTileBytes;
+          const int c0 = 2 * (c & 3);
+          *reinterpret_cast<uint4*>(half + ((c0 ^ (i & 7)) << 4)) =
+              make_uint4(f16x2_of_e4m3x2(v.x & 0xFFFFu), f16x2_of_e4m3x2(v.x >> 16), f16x2_of_e4m3x2(v.y & 0xFFFFu), f16x2_of_e4m3x2(v.y >> 16));
+          *reinterpret_cast<uint4*>(half + (((c0 + 1) ^ (i & 7)) << 4)) =
+              make_uint4(f16x2_of_e4m3x2(v.z & 0xFFFFu), f16x2_of_e4m3x2(v.z >> 16), f16x2_of_e4m3x2(v.w & 0xFFFFu), f16x2_of_e4m3x2(v.w >> 16));
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(kVfree + 8 * vr.at);
+          mbar_arrive(kFfull + 8 * fr.at);
+        }
+        vr.next(kVStages);
+        fr.next(2);
       }
     }
   } else {
@@ -682,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (plain) {
             // One pass with m as it is. A weight that is too large shows in the sums; then the tile is done over.
             uint32_t w[2][32];
-            float sum = 0.f, most = 0.f;
+            float sum = 0.f, most = 0.f, top = 0.f;
             uint32_t raw[2][32];
             kv_ld<32>(ts, raw[0]);
 #pragma unroll
@@ -699,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int i = 0; i < 8; ++i) {
                   const int at = 16 * g + 2 * i;
                   const uint64_t x = fma_2(pack2(__uint_as_float(raw[c & 1][at]), __uint_as_float(raw[c & 1][at + 1])), k2, add2);
-                  const uint64_t e = (i & 3) == 3 ? ex2_poly(x) : pack2(ex2(low_of(x)), ex2(high_of(x)));
+                  const uint64_t e = (i & 3) == 3 ? ex2_poly(x, top) : pack2(ex2(low_of(x)), ex2(high_of(x)));
                   sum2 = add_2(sum2, e);
                   w[c >> 1][16 * (c & 1) + 8 * g + i] = f16x2_of(low_of(e), high_of(e));
                 }
@@ -708,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 sum = fmaf(part, v.z, sum);
               }
             }
-            plain = !__any_sync(0xFFFFFFFFu, most > kMostSum);
+            plain = !__any_sync(0xFFFFFFFFu, most > kMostSum || top > kMostPoly);
             if (plain) {
               l += sum;
               tc::st_cols<32>(ts, w[0]);
@@ -761,15 +764,16 @@ __global__ void __launch_bounds__(kThreads, 1)
               uint32_t raw[16], w[8];
               kv_ld<16>(ts + 16 * g, raw);
               const float4 v = sc[g];
-              const float c = cq * v.x, add = v.y - m;
+              const float c = cq * v.x;
               kv_wait_ld();
               kv_tie(raw);
+              // x first and then less m: the row's largest is 2^0 exactly, however large its score and its rounding are.
               float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
               for (int k = 0; k < 16; k += 2) {
                 const int at = 16 * g + k;
-                const float a = at <= high && at > low ? ex2(fmaf(__uint_as_float(raw[k]), c, add)) : 0.f;
-                const float b = at + 1 <= high && at + 1 > low ? ex2(fmaf(__uint_as_float(raw[k + 1]), c, add)) : 0.f;
+                const float a = at <= high && at > low ? ex2(fmaf(__uint_as_float(raw[k]), c, v.y) - m) : 0.f;
+                const float b = at + 1 <= high && at + 1 > low ? ex2(fmaf(__uint_as_float(raw[k + 1]), c, v.y) - m) : 0.f;
                 sum0 += a;
                 sum1 += b;
                 w[k >> 1] = f16x2_of(a, b);
