@@ -55,12 +55,12 @@ def prepare_fp8_kv_cache(pages: int, kv_heads: int, page_tokens: int, head_dim: 
     return {"keys": keys, "values": values, "key_scales": key_scales, "value_scales": value_scales}
 
 
-def _cache_view(cache: Fp8KvCache) -> tuple[_lib.MamboKvCache, torch.device]:
+def _cache_view(cache: Fp8KvCache) -> _lib.MamboKvCache:
     try:
         keys, values, ks, vs = cache["keys"], cache["values"], cache["key_scales"], cache["value_scales"]
-    except (KeyError, TypeError):
+    except (KeyError, TypeError, IndexError):
         raise TypeError("cache must have keys, values, key_scales and value_scales (prepare_fp8_kv_cache)") from None
-    shape, dev = keys.shape, keys.device
+    shape, dev = keys.shape, keys.get_device()
     if len(shape) != 4 or values.shape != shape or ks.shape != shape[:2] or vs.shape != shape[:2]:
         raise ValueError("cache must be [pages, kv_heads, page_tokens, head_dim] with scales [pages, kv_heads]")
     u8 = torch.uint8
@@ -68,36 +68,37 @@ def _cache_view(cache: Fp8KvCache) -> tuple[_lib.MamboKvCache, torch.device]:
         raise ValueError("cache codes and scales must be uint8")
     if not (keys.is_contiguous() and values.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("cache tensors must be contiguous")
-    if not keys.is_cuda or values.device != dev or ks.device != dev or vs.device != dev:
+    if dev < 0 or values.get_device() != dev or ks.get_device() != dev or vs.get_device() != dev:
         raise ValueError("cache tensors must be on one CUDA device")
-    return _lib.MamboKvCache(keys.data_ptr(), values.data_ptr(), ks.data_ptr(), vs.data_ptr(), *shape), dev
+    return _lib.MamboKvCache(keys.data_ptr(), values.data_ptr(), ks.data_ptr(), vs.data_ptr(), *shape)
 
 
-def _sequences(page_table, lengths, offsets, tokens: int, dev: torch.device) -> tuple[_lib.MamboKvSequences, tuple]:
+def _sequences(page_table, lengths, offsets, tokens: int, device: int) -> tuple[_lib.MamboKvSequences, tuple]:
     """The C ABI's view of a call's sequences, and the tensors that it points to."""
     table, lengths = _runtime.as_cuda_tensor(page_table), _runtime.as_cuda_tensor(lengths)
-    if table.ndim != 2 or table.dtype != torch.int32 or table.shape[1] < 1 or table.device != dev:
+    if table.ndim != 2 or table.dtype is not torch.int32 or table.shape[1] < 1 or table.get_device() != device:
         raise ValueError("page_table must be int32 [B, pages of a sequence] on the cache's device")
     batch, columns = table.shape
-    if lengths.dtype != torch.int32 or tuple(lengths.shape) != (batch,) or lengths.device != dev:
+    if lengths.dtype is not torch.int32 or lengths.shape != (batch,) or lengths.get_device() != device:
         raise ValueError("lengths must be int32 [B] on the cache's device")
-    if columns > 1 and table.stride(1) != 1:
-        table = table.contiguous()
-    if batch > 1 and lengths.stride(0) != 1:
+    if not lengths.is_contiguous():
         lengths = lengths.contiguous()
-    if offsets is None:
-        if tokens != batch:
-            raise ValueError("without offsets there is one token for each sequence")
-        at = None
-    else:
+    stride, unit = table.stride()
+    if unit != 1 and columns > 1:
+        table = table.contiguous()
+        stride = columns
+    at = None
+    if offsets is not None:
         offsets = _runtime.as_cuda_tensor(offsets)
-        if offsets.dtype != torch.int32 or tuple(offsets.shape) != (batch + 1,) or offsets.device != dev:
+        if offsets.dtype is not torch.int32 or offsets.shape != (batch + 1,) or offsets.get_device() != device:
             raise ValueError("offsets must be int32 [B+1] on the cache's device")
-        if offsets.stride(0) != 1:
+        if not offsets.is_contiguous():
             offsets = offsets.contiguous()
         at = offsets.data_ptr()
-    stride = table.stride(0) if batch > 1 else columns
-    return (_lib.MamboKvSequences(table.data_ptr(), stride, columns, lengths.data_ptr(), at, batch), (table, lengths, offsets))
+    elif tokens != batch:
+        raise ValueError("without offsets there is one token for each sequence")
+    return (_lib.MamboKvSequences(table.data_ptr(), stride if batch > 1 else columns, columns, lengths.data_ptr(), at, batch),
+            (table, lengths, offsets))
 
 
 @_runtime.with_stream
@@ -118,14 +119,14 @@ def launch_fp8_kv_append(cache: Fp8KvCache, k, v, page_table, lengths, *, offset
     Tokens without a page (behind the table's end, or an entry outside the
     cache) are dropped. A page that is appended to belongs to one sequence.
     """
-    view, dev = _cache_view(cache)
+    view, dev = _cache_view(cache), cache["keys"].device
     k, v = _runtime.as_cuda_tensor(k), _runtime.as_cuda_tensor(v)
     if k.ndim != 3 or k.dtype not in _DTYPES or k.shape[1] != view.kv_heads or k.shape[2] != view.head_dim:
         raise ValueError("k must be float32 or bfloat16 [T,H,D] with the cache's heads and head size")
-    if v.shape != k.shape or v.dtype != k.dtype or k.device != dev or v.device != dev:
+    if v.shape != k.shape or v.dtype is not k.dtype or k.get_device() != dev.index or v.get_device() != dev.index:
         raise ValueError("v must have k's shape and type, both on the cache's device")
     tokens = k.shape[0]
-    seq, held = _sequences(page_table, lengths, offsets, tokens, dev)
+    seq, held = _sequences(page_table, lengths, offsets, tokens, dev.index)
     if rope is not None:
         _check_rope(rope, view.head_dim, dev)
     _runtime.require_device(dev)
@@ -169,22 +170,22 @@ def fp8_paged_attention(q, cache: Fp8KvCache, page_table, lengths, *, offsets=No
     exponentials (minus infinity where a query sees nothing), with which
     results over parts of a context are joined.
     """
-    view, dev = _cache_view(cache)
+    view, dev = _cache_view(cache), cache["keys"].device
     q = _runtime.as_cuda_tensor(q)
-    if q.ndim != 3 or q.dtype != torch.bfloat16 or q.shape[2] != view.head_dim or q.device != dev:
+    if q.ndim != 3 or q.dtype is not torch.bfloat16 or q.shape[2] != view.head_dim or q.get_device() != dev.index:
         raise ValueError("q must be bfloat16 [T,Hq,D] with the cache's head size on its device")
     tokens, heads, dim = q.shape
     if heads < 1 or heads % view.kv_heads:
         raise ValueError("the query heads must be a multiple of the cache's heads")
     if window < 0:
         raise ValueError("window must not be negative")
-    seq, held = _sequences(page_table, lengths, offsets, tokens, dev)
+    seq, held = _sequences(page_table, lengths, offsets, tokens, dev.index)
     _runtime.require_device(dev)
     if not _rows_aligned(q):
         q = q.clone(memory_format=torch.contiguous_format)
     given = out
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=torch.bfloat16, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif tuple(out.shape) != (tokens, heads, dim) or out.dtype != torch.bfloat16 or out.device != dev:
         raise ValueError("out must be bfloat16 of q's shape on its device")
     elif not _rows_aligned(out):

@@ -105,7 +105,7 @@ def _check_rope(rope: RotaryFields, dim: int, device: torch.device) -> None:
         raise TypeError("rope must come from prepare_rotary_fields")
     if rope["rotary_dim"] > dim:
         raise ValueError("the rotated part is larger than the head")
-    if rope["turns"].device != device:
+    if rope["turns"].get_device() != device.index:
         raise ValueError("rope and values must be on one device")
 
 
@@ -130,7 +130,7 @@ def launch_rotary(x, positions, rope: RotaryFields, *, inverse: bool = False, st
     if x.ndim != 3 or x.dtype not in _DTYPES or x.shape[1] < 1:
         raise ValueError("x must be float32 or bfloat16 [T,H,D]")
     tokens, heads, dim = x.shape
-    if positions.dtype not in _POSITIONS or tuple(positions.shape) != (tokens,) or positions.device != dev:
+    if positions.dtype not in _POSITIONS or positions.shape != (tokens,) or positions.get_device() != dev.index:
         raise ValueError("positions must be int32 or int64 [T] on x's device")
     _check_rope(rope, dim, dev)
     _runtime.require_device(dev)
@@ -139,7 +139,7 @@ def launch_rotary(x, positions, rope: RotaryFields, *, inverse: bool = False, st
             raise ValueError("x must have unit stride along the head to turn in place")
         x = x.contiguous()
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=dev)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif tuple(out.shape) != (tokens, heads, dim) or out.dtype != x.dtype or out.stride(2) != 1 or out.device != dev:
         raise ValueError("out must have x's shape, type and device and unit stride along the head")
     if tokens:
