@@ -4,9 +4,14 @@
 //
 // A unit is 256 rows of one key head (row r of a sequence: token r / group,
 // query head r % group) as two MMA tiles of 128, which share the keys and
-// values that pass by. For each 128 positions and tile:
-//   S [128 x 128] = Q K^T       8-bit MMAs, the queries in two exact terms (kv_tc.cuh)
-//   O [128 x D]  += W V         f16 MMAs, the weights W from TMEM (over S, which they replace)
+// values that pass by. For each 64 positions and tile:
+//   S [128 x 64] = Q K^T        8-bit MMAs, the queries in two exact terms (kv_tc.cuh)
+//   O [128 x D] += W V          f16 MMAs, the weights W from TMEM (over S, which they replace)
+// TMEM holds two S of 64 positions for each tile of rows (and O), so that one is
+// filled while the softmax works on the other. With one S of 128 positions every
+// tile waited for its MMAs in turn: 732 us for a prompt of 8192 tokens instead of
+// 596, although scores of 64 positions read the queries from shared memory twice
+// as often.
 // Two 8-bit terms cost what one 16-bit product does and need no conversion of
 // the keys. The values are converted to f16 (exactly) by a warpgroup of their
 // own: weights in f16 have 11 bits, where two more terms would have cost the
@@ -58,7 +63,7 @@ constexpr uint32_t kAtK = kQ, kAtV = kAtK + kKStages * kKvTileBytes, kAtVf = kAt
 constexpr uint32_t kAtStage = kAtVf + 2 * kVf, kAtScales = kAtStage + 8 * 2048, kAtUnits = kAtScales + 2 * 32 * 16;
 constexpr int kUnitStages = 4;
 constexpr uint32_t kAtBegin = kAtUnits + (kUnitStages + 1) * 96, kAtBars = kAtBegin + 128;
-constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 4 + 8 + 4 + 4 + 2 * kUnitStages;
+constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 4 + 14 + 4 + 4 + 2 * kUnitStages;
 constexpr uint32_t kSmem = 1024 + kAtBars + kNumBars * 8 + 16;
 constexpr int kPart = kRows * 130;    // floats of a tile's part: O [32][128][4], m, l
 
@@ -111,9 +116,9 @@ struct Plan {
   }
 };
 
-// One tile's S = Q K^T: head size up to 64 or 128, two terms of A.
+// Half a tile's S = Q K^T, 64 positions: head size up to 64 or 128, two terms of A.
 __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b, bool wide, uint32_t done) {
-  constexpr uint32_t kId = tc::idesc_e4m3_f32(kRows, kKvTile);
+  constexpr uint32_t kId = tc::idesc_e4m3_f32(kRows, kKvTile / 2);
   asm volatile(
       "{\n\t.reg .pred p, t, w;\n\t.reg .b32 x, y, z;\n\t.reg .b64 dx, dy, db;\n\t"
       "setp.ne.b32 p, 0, 0;\n\tsetp.eq.b32 t, 0, 0;\n\tsetp.ne.b32 w, %5, 0;\n\t"
@@ -137,7 +142,7 @@ __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b, b
       "r"(a), "r"(b), "r"(kId), "r"(desc_high(1024, true)), "r"((int)wide), "r"(done)
       : "memory");
 }
-// One tile's O (+)= W V: weights f16 at TMEM column w (8 columns for 16 positions), values f16 along N (16 positions in
+// Half a tile's O (+)= W V, 64 positions: weights f16 at TMEM column w (8 columns for 16 positions), values f16 along N (16 positions in
 // 2048 bytes).
 __device__ __forceinline__ void mma_values(uint32_t d, uint32_t w, uint32_t v, uint32_t idesc, uint32_t acc, uint32_t done) {
   asm volatile(
@@ -150,14 +155,6 @@ __device__ __forceinline__ void mma_values(uint32_t d, uint32_t w, uint32_t v, u
       "add.u32 a, %1, 16;\n\tadd.u32 b, %2, 256;\n\tmov.b64 db, {b, %5};\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %3, t;\n\t"
       "add.u32 a, %1, 24;\n\tadd.u32 b, %2, 384;\n\tmov.b64 db, {b, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %3, t;\n\t"
-      "add.u32 a, %1, 32;\n\tadd.u32 b, %2, 512;\n\tmov.b64 db, {b, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %3, t;\n\t"
-      "add.u32 a, %1, 40;\n\tadd.u32 b, %2, 640;\n\tmov.b64 db, {b, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %3, t;\n\t"
-      "add.u32 a, %1, 48;\n\tadd.u32 b, %2, 768;\n\tmov.b64 db, {b, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %3, t;\n\t"
-      "add.u32 a, %1, 56;\n\tadd.u32 b, %2, 896;\n\tmov.b64 db, {b, %5};\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], db, %3, t;\n\t"
       "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t}" ::"r"(d),
       "r"(w), "r"(v), "r"(idesc), "r"(acc), "r"(desc_high(1024, true)), "r"(done)
@@ -217,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t sm0 = smem_u32(sm);
   const uint32_t kKfull = smem_u32(bars), kKfree = kKfull + 8 * kKStages, kVfull = kKfree + 8 * kKStages;
   const uint32_t kVfree = kVfull + 8 * kVStages, kFfull = kVfree + 8 * kVStages, kFfree = kFfull + 16;  // values in f16
-  const uint32_t kSfull = kFfree + 16, kWfull = kSfull + 16, kOdone = kWfull + 16, kOfree = kOdone + 16;
+  const uint32_t kSfull = kFfree + 16, kWfull = kSfull + 32, kOdone = kWfull + 32, kOfree = kOdone + 32;
   const uint32_t kQfull = kOfree + 16, kQfree = kQfull + 16, kMfull = kQfree + 16, kMfree = kMfull + 16;
   const uint32_t kUfull = kMfree + 16, kUfree = kUfull + 8 * kUnitStages;
   const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -234,9 +231,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(kFfull + 8 * i, 4);
       mbar_init(kFfree + 8 * i, 2);
-      mbar_init(kSfull + 8 * i, 1);
-      mbar_init(kWfull + 8 * i, 4);
-      mbar_init(kOdone + 8 * i, 1);
+      mbar_init(kSfull + 16 * i, 1);  // of either tile of rows: two halves
+      mbar_init(kSfull + 16 * i + 8, 1);
+      mbar_init(kWfull + 16 * i, 4);
+      mbar_init(kWfull + 16 * i + 8, 4);
+      mbar_init(kOdone + 16 * i, 1);
+      mbar_init(kOdone + 16 * i + 8, 1);
       mbar_init(kOfree + 8 * i, 4);
       mbar_init(kMfull + 8 * i, 1);
       mbar_init(kMfree + 8 * i, 8);
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool wide = p.cache.dim > 64;
         const uint32_t ds = tmem + q * 128, dout = ds + 256, a = desc_low(sm0 + q * 2 * kKvTileBytes, 16);
         const uint32_t k0 = desc_low(sm0 + kAtK, 16), v0 = desc_low(sm0 + kAtVf, kKvTileBytes);
-        const uint32_t sfull = kSfull + 8 * q, wfull = kWfull + 8 * q, odone = kOdone + 8 * q, ofree = kOfree + 8 * q;
+        const uint32_t sfull = kSfull + 16 * q, wfull = kWfull + 16 * q, odone = kOdone + 16 * q, ofree = kOfree + 8 * q;
         const uint32_t qfull = kQfull + 8 * q, qfree = kQfree + 8 * q;
         KvRing kr, fr, ur;
         uint32_t qphase = 0, wphase = 0, ophase = 1;
@@ -442,18 +442,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           begins = true;
         };
         bool ok = true;
-        auto scores = [&]() {  // whether these rows see the tile
-          if (begins) {
-            ok = kv_wait(qfull, qphase, kSiteKvFull);
-            qphase ^= 1;
-            begins = false;
-          }
-          const bool seen = tile >= from && tile < to;
-          ok = ok && kv_wait(kKfull + 8 * kr.at, kr.phase, kSiteKvFull);
-          if (ok && seen) {
+        bool seen = false;  // whether these rows see the tile
+        auto scores = [&](int half) {
+          if (seen) {
             tc::fence_after_sync();
-            mma_scores(ds, a, k0 + kr.at * (kKvTileBytes >> 4), wide, sfull);
+            mma_scores(ds + 64 * half, a, k0 + kr.at * (kKvTileBytes >> 4) + half * (kKvTileBytes >> 5), wide, sfull + 8 * half);
           }
+          if (half == 0) return;
           tc::commit(kKfree + 8 * kr.at);
           kr.next(kKStages);
           ++tile;
@@ -461,35 +456,55 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::commit(qfree);
             enter();
           }
-          return seen;
+        };
+        auto both = [&]() {  // a unit's first tile
+          ok = kv_wait(qfull, qphase, kSiteKvFull) && kv_wait(kKfull + 8 * kr.at, kr.phase, kSiteKvFull);
+          qphase ^= 1;
+          begins = false;
+          seen = tile >= from && tile < to;
+          if (!ok) return;
+          scores(0);
+          scores(1);
         };
         enter();
-        bool started = false, ends = left == 1, some = left > 0, seen = some && scores();
+        bool started = false, ends = left == 1, some = left > 0;
+        if (some) both();
         while (ok && some) {
-          // The tile's values; the next tile's scores follow at once, unless its queries are still on their way.
+          // Half a tile's values, and over its weights the scores of the next tile's half: the softmax works on the other
+          // half meanwhile. A next unit's queries may still be on their way; then its scores come at the end.
           const bool last = ends, go = seen;
+          some = left > 0;
+          ends = left == 1;
+          const bool next = some && !begins;
           ok = kv_wait(kFfull + 8 * fr.at, fr.phase, kSiteKvFull);
-          if (ok && go) {
-            ok = kv_wait(wfull, wphase, kSiteKvFull);
-            wphase ^= 1;
-            // The softmax has read the last unit's O.
-            if (ok && !started) {
-              ok = kv_wait(ofree, ophase, kSiteKvEmpty);
-              ophase ^= 1;
-            }
-            if (ok) {
-              tc::fence_after_sync();
-              mma_values(dout, ds, v0 + fr.at * (kVf >> 4), idesc_o, started, odone);
-            }
-            started = true;
+          if (ok && next) ok = kv_wait(kKfull + 8 * kr.at, kr.phase, kSiteKvFull);
+          // The softmax has read the last unit's O.
+          if (ok && go && !started) {
+            ok = kv_wait(ofree, ophase, kSiteKvEmpty);
+            ophase ^= 1;
+          }
+          if (next) seen = tile >= from && tile < to;
+          const uint32_t values = v0 + fr.at * (kVf >> 4);
+          if (go) {
+            ok = ok && kv_wait(wfull, wphase, kSiteKvFull);
+            if (!ok) break;
+            tc::fence_after_sync();
+            mma_values(dout, ds, values, idesc_o, started, odone);
           }
           if (!ok) break;
+          if (next) scores(0);
+          if (go) {
+            if (!(ok = kv_wait(wfull + 8, wphase, kSiteKvFull))) break;
+            wphase ^= 1;
+            tc::fence_after_sync();
+            mma_values(dout, ds + 64, values + 512, idesc_o, 1, odone + 8);
+            started = true;
+          }
           tc::commit(kFfree + 8 * fr.at);
           fr.next(2);
           if (last) started = false;
-          some = left > 0;
-          ends = left == 1;
-          if (some) seen = scores();
+          if (next) scores(1);
+          if (some && !next) both();
         }
         if (!ok) kv_settle();
       }
@@ -590,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* stage = sm + kAtStage + warp * 2048;
     KvRing mr, ur;
     int in_batch = 0;
-    uint32_t sphase = 0, ophase = 1;  // ophase: of the last MMAs on the values
+    uint32_t sphase = 0;              // of the tile: its scores, and the MMAs on its values
     uint32_t qphase = 1;              // a fresh barrier's previous phase counts as over
     // Of the unit's queries this warp's 32 rows, split into two terms, to shared memory: a half warp a row, eight dimensions
     // a lane. The rows come as they are to where their terms go (a row of bf16 is as large as both), all at once and
@@ -676,118 +691,122 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (in_batch == 0) kv_warp_wait(kMfull + 8 * mr.at, mr.phase, kSiteKvFull);
         const float4* sc = scales + mr.at * 32 + in_batch * 8;
         if (tile >= from && tile < end) {
-          kv_warp_wait(kSfull + 8 * q, sphase, kSiteKvFull);
-          sphase ^= 1;
-          tc::fence_after_sync();
-          const int64_t j0 = (int64_t)tile * kKvTile;
-          const bool edge = j0 + kKvTile - 1 > lo || (p.window && j0 <= (int64_t)hi - p.window);
-          bool plain = started && !edge;
-          if (plain) {
-            // One pass with m as it is. A weight that is too large shows in the sums; then the tile is done over.
-            uint32_t w[2][32];
-            float sum = 0.f, most = 0.f, top = 0.f;
-            uint32_t raw[2][32];
-            kv_ld<32>(ts, raw[0]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              kv_wait_ld();
-              kv_tie(raw[c & 1]);
-              if (c < 3) kv_ld<32>(ts + 32 * c + 32, raw[(c + 1) & 1]);
-#pragma unroll
-              for (int g = 0; g < 2; ++g) {
-                const float4 v = sc[2 * c + g];
-                const uint64_t k2 = pack2(cq * v.x, cq * v.x), add2 = pack2(v.y - m, v.y - m);
-                uint64_t sum2 = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  const int at = 16 * g + 2 * i;
-                  const uint64_t x = fma_2(pack2(__uint_as_float(raw[c & 1][at]), __uint_as_float(raw[c & 1][at + 1])), k2, add2);
-                  const uint64_t e = (i & 3) == 3 ? ex2_poly(x, top) : pack2(ex2(low_of(x)), ex2(high_of(x)));
-                  sum2 = add_2(sum2, e);
-                  w[c >> 1][16 * (c & 1) + 8 * g + i] = f16x2_of(low_of(e), high_of(e));
-                }
-                const float part = low_of(sum2) + high_of(sum2);
-                most = fmaxf(most, part);
-                sum = fmaf(part, v.z, sum);
-              }
-            }
-            plain = !__any_sync(0xFFFFFFFFu, most > kMostSum || top > kMostPoly);
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t th = ts + 64 * half;
+            const float4* sh = sc + 4 * half;
+            kv_warp_wait(kSfull + 16 * q + 8 * half, sphase, kSiteKvFull);
+            tc::fence_after_sync();
+            const int64_t j0 = (int64_t)tile * kKvTile + 64 * half;
+            const bool edge = j0 + 63 > lo || (p.window && j0 <= (int64_t)hi - p.window);
+            bool plain = started && !edge;
             if (plain) {
-              l += sum;
-              tc::st_cols<32>(ts, w[0]);
-              tc::st_cols<32>(ts + 32, w[1]);
-            }
-          }
-          if (!plain) {
-            // The last position that the row sees, and the one before the first, in the tile; their largest x; then the
-            // weights, which replace the scores from the left, half as wide, behind the columns that have been read.
-            const int high = (int)max((int64_t)-1, min((int64_t)kKvTile, place - j0));
-            const int low = p.window ? (int)max((int64_t)-1, min((int64_t)kKvTile, place - (int64_t)p.window - j0)) : -1;
-            float top = -INFINITY;
-#pragma unroll 1
-            for (int g = 0; g < 8; ++g) {
-              uint32_t raw[16];
-              kv_ld<16>(ts + 16 * g, raw);
-              const float4 v = sc[g];
-              const float c = cq * v.x;
-              kv_wait_ld();
-              kv_tie(raw);
-              float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+              // One pass with m as it is. A weight that is too large shows in the sums; then the half is done over.
+              uint32_t w[32];
+              float sum = 0.f, most = 0.f, top = 0.f;
+              uint32_t raw[2][32];
+              kv_ld<32>(th, raw[0]);
 #pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                const int at = 16 * g + k;
-                if (at <= high && at > low) t4[k & 3] = fmaxf(t4[k & 3], fmaf(__uint_as_float(raw[k]), c, v.y));
-              }
-              top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
-            }
-            const float up = fmaxf(m, top), f = ex2(m - up);
-            m = up;
-            l *= f;
-            if (started) {
-              kv_warp_wait(kOdone + 8 * q, ophase, kSiteKvFull);
-              tc::fence_after_sync();
-              if (__any_sync(0xFFFFFFFFu, f != 1.f)) {
-#pragma unroll 1
-                for (int c = 0; c < p.cache.dim; c += 16) {
-                  uint32_t o[16];
-                  kv_ld<16>(to_ + c, o);
-                  kv_wait_ld();
-                  kv_tie(o);
+              for (int c = 0; c < 2; ++c) {
+                kv_wait_ld();
+                kv_tie(raw[c]);
+                if (c == 0) kv_ld<32>(th + 32, raw[1]);
 #pragma unroll
-                  for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                  tc::st_cols<16>(to_ + c, o);
+                for (int g = 0; g < 2; ++g) {
+                  const float4 v = sh[2 * c + g];
+                  const uint64_t k2 = pack2(cq * v.x, cq * v.x), add2 = pack2(v.y - m, v.y - m);
+                  uint64_t sum2 = 0;
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) {
+                    const int at = 16 * g + 2 * i;
+                    const uint64_t x = fma_2(pack2(__uint_as_float(raw[c][at]), __uint_as_float(raw[c][at + 1])), k2, add2);
+                    const uint64_t e = (i & 3) == 3 ? ex2_poly(x, top) : pack2(ex2(low_of(x)), ex2(high_of(x)));
+                    sum2 = add_2(sum2, e);
+                    w[16 * c + 8 * g + i] = f16x2_of(low_of(e), high_of(e));
+                  }
+                  const float part = low_of(sum2) + high_of(sum2);
+                  most = fmaxf(most, part);
+                  sum = fmaf(part, v.z, sum);
                 }
               }
-            }
-#pragma unroll 1
-            for (int g = 0; g < 8; ++g) {
-              uint32_t raw[16], w[8];
-              kv_ld<16>(ts + 16 * g, raw);
-              const float4 v = sc[g];
-              const float c = cq * v.x;
-              kv_wait_ld();
-              kv_tie(raw);
-              // x first and then less m: the row's largest is 2^0 exactly, however large its score and its rounding are.
-              float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-              for (int k = 0; k < 16; k += 2) {
-                const int at = 16 * g + k;
-                const float a = at <= high && at > low ? ex2(fmaf(__uint_as_float(raw[k]), c, v.y) - m) : 0.f;
-                const float b = at + 1 <= high && at + 1 > low ? ex2(fmaf(__uint_as_float(raw[k + 1]), c, v.y) - m) : 0.f;
-                sum0 += a;
-                sum1 += b;
-                w[k >> 1] = f16x2_of(a, b);
+              plain = !__any_sync(0xFFFFFFFFu, most > kMostSum || top > kMostPoly);
+              if (plain) {
+                l += sum;
+                tc::st_cols<32>(th, w);
               }
-              l = fmaf(sum0 + sum1, v.z, l);
-              tc::st_x8(ts + 8 * g, w);
             }
+            if (!plain) {
+              // The last position that the row sees, and the one before the first, in the half; their largest x; then the
+              // weights, which replace the scores from the left, half as wide, behind the columns that have been read.
+              const int high = (int)max((int64_t)-1, min((int64_t)64, place - j0));
+              const int low = p.window ? (int)max((int64_t)-1, min((int64_t)64, place - (int64_t)p.window - j0)) : -1;
+              float top = -INFINITY;
+#pragma unroll 1
+              for (int g = 0; g < 4; ++g) {
+                uint32_t raw[16];
+                kv_ld<16>(th + 16 * g, raw);
+                const float4 v = sh[g];
+                const float c = cq * v.x;
+                kv_wait_ld();
+                kv_tie(raw);
+                float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  const int at = 16 * g + k;
+                  if (at <= high && at > low) t4[k & 3] = fmaxf(t4[k & 3], fmaf(__uint_as_float(raw[k]), c, v.y));
+                }
+                top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
+              }
+              const float up = fmaxf(m, top), f = ex2(m - up);
+              m = up;
+              l *= f;
+              if (started) {
+                // The half before: this tile's first, or the last tile's second.
+                kv_warp_wait(kOdone + 16 * q + 8 * (half ^ 1), sphase ^ half ^ 1, kSiteKvFull);
+                tc::fence_after_sync();
+                if (__any_sync(0xFFFFFFFFu, f != 1.f)) {
+#pragma unroll 1
+                  for (int c = 0; c < p.cache.dim; c += 16) {
+                    uint32_t o[16];
+                    kv_ld<16>(to_ + c, o);
+                    kv_wait_ld();
+                    kv_tie(o);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                    tc::st_cols<16>(to_ + c, o);
+                  }
+                }
+              }
+#pragma unroll 1
+              for (int g = 0; g < 4; ++g) {
+                uint32_t raw[16], w[8];
+                kv_ld<16>(th + 16 * g, raw);
+                const float4 v = sh[g];
+                const float c = cq * v.x;
+                kv_wait_ld();
+                kv_tie(raw);
+                // x first and then less m: the row's largest is 2^0 exactly, however large its score and its rounding are.
+                float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) {
+                  const int at = 16 * g + k;
+                  const float a = at <= high && at > low ? ex2(fmaf(__uint_as_float(raw[k]), c, v.y) - m) : 0.f;
+                  const float b = at + 1 <= high && at + 1 > low ? ex2(fmaf(__uint_as_float(raw[k + 1]), c, v.y) - m) : 0.f;
+                  sum0 += a;
+                  sum1 += b;
+                  w[k >> 1] = f16x2_of(a, b);
+                }
+                l = fmaf(sum0 + sum1, v.z, l);
+                tc::st_x8(th + 8 * g, w);
+              }
+            }
+            tc::wait_st();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(kWfull + 16 * q + 8 * half);
+            started = true;
           }
-          tc::wait_st();
-          tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(kWfull + 8 * q);
-          started = true;
-          ophase ^= 1;
+          sphase ^= 1;
         }
         if (++in_batch == 4) {
           in_batch = 0;
@@ -811,7 +830,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (n > 0 && unit.has(q)) {
         // The unit's end, or this CTA's part of it.
         if (started) {
-          kv_warp_wait(kOdone + 8 * q, ophase, kSiteKvFull);
+          kv_warp_wait(kOdone + 16 * q, sphase ^ 1, kSiteKvFull);
+          kv_warp_wait(kOdone + 16 * q + 8, sphase ^ 1, kSiteKvFull);
           tc::fence_after_sync();
         }
         const int row = unit.row0 + kRows * q + r, t = row / p.group;
