@@ -260,7 +260,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
   }
-  pdl_wait();
+  // Behind the decode kernel (which waits for what came before it, and then lets this one start) there is nothing to wait
+  // for: they share nothing but the arguments. Its end is waited for at the end, so that this kernel's is the call's.
+  if (p.few == 0) pdl_wait();
   pdl_launch_dependents();
   // The whole work, and where this CTA's share begins: a warp has a run of sequences, a lane every 32nd unit of one.
   const int each = (p.seq.batch + 15) / 16, mine0 = min(p.seq.batch, warp * each), mine1 = min(p.seq.batch, mine0 + each);
@@ -706,11 +708,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               float sum = 0.f, most = 0.f, top = 0.f;
               uint32_t raw[2][32];
               kv_ld<32>(th, raw[0]);
+              kv_ld<32>(th + 32, raw[1]);
+              kv_wait_ld();
+              kv_tie(raw[0]);
+              kv_tie(raw[1]);
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                kv_wait_ld();
-                kv_tie(raw[c]);
-                if (c == 0) kv_ld<32>(th + 32, raw[1]);
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                   const float4 v = sh[2 * c + g];
@@ -720,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   for (int i = 0; i < 8; ++i) {
                     const int at = 16 * g + 2 * i;
                     const uint64_t x = fma_2(pack2(__uint_as_float(raw[c][at]), __uint_as_float(raw[c][at + 1])), k2, add2);
-                    const uint64_t e = (i & 3) == 3 ? ex2_poly(x, top) : pack2(ex2(low_of(x)), ex2(high_of(x)));
+                    const uint64_t e = i == 3 ? ex2_poly(x, top) : pack2(ex2(low_of(x)), ex2(high_of(x)));
                     sum2 = add_2(sum2, e);
                     w[16 * c + 8 * g + i] = f16x2_of(low_of(e), high_of(e));
                   }
@@ -966,6 +969,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::fence_after_sync();
     tc::dealloc(tmem, 512);
   }
+  if (p.few) pdl_wait();
 }
 
 size_t kv_prompt_partial_bytes(int sms) { return (size_t)sms * 4 * kPart * sizeof(float); }
