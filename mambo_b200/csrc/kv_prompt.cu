@@ -637,52 +637,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
-      // Four rows at a time, whose chains (350 clocks each) overlap.
-#pragma unroll 1
-      for (int n = r0; n < r0 + 32; n += 8) {
-        uint32_t v[4][4], code[4], h[4][2], l[4][2];
+      // A lane has a row: no shuffles, and one scale for it. (16 lanes a row took 6000 clocks and more.)
+      const int r1 = 32 * (warp & 3) + lane;
+      uint8_t* const to = sm + tile0 + r1 * 128;
+      uint32_t v[64], top[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r1 = n + 2 * k;
-          const uint4 raw = *reinterpret_cast<const uint4*>(sm + mine + r1 * 128 + (((c ^ r1) & 7) << 4));
-          v[k][0] = raw.x, v[k][1] = raw.y, v[k][2] = raw.z, v[k][3] = raw.w;
-          code[k] = absmax_bf16x2(absmax_bf16x2(raw.x, raw.y), absmax_bf16x2(raw.z, raw.w));
+      for (int i = 0; i < 16; ++i) {
+        const uint4 raw4 = *reinterpret_cast<const uint4*>(to + (i >> 3) * kKvTileBytes + (((i ^ r1) & 7) << 4));
+        v[4 * i] = raw4.x, v[4 * i + 1] = raw4.y, v[4 * i + 2] = raw4.z, v[4 * i + 3] = raw4.w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top[k] = absmax_bf16x2(top[k], v[4 * i + k]);
+      }
+      top[0] = absmax_bf16x2(absmax_bf16x2(top[0], top[1]), absmax_bf16x2(top[2], top[3]));
+      const uint32_t code = bf16_scale_code(max(top[0] & 0x7FFFu, (top[0] >> 16) & 0x7FFFu));
+      const bool bad = code == 255u;
+      const float inv = bad ? 0.f : e8m0_to_float(254u - code);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // 8 significant bits up to 448: exact in f16 (down to 2^-17), and so is what the first term leaves.
+          const uint32_t x = v[8 * d + 2 * i], y = v[8 * d + 2 * i + 1];
+          const uint32_t e0 = f16x2_of(__uint_as_float(x << 16) * inv, __uint_as_float(x & 0xFFFF0000u) * inv);
+          const uint32_t e1 = f16x2_of(__uint_as_float(y << 16) * inv, __uint_as_float(y & 0xFFFF0000u) * inv);
+          const uint32_t h0 = e4m3x2_of_f16x2(e0), h1 = e4m3x2_of_f16x2(e1);
+          h[i] = h0 | (h1 << 16);
+          l[i] = e4m3x2_of_f16x2(sub_f16x2(e0, f16x2_of_e4m3x2(h0))) | (e4m3x2_of_f16x2(sub_f16x2(e1, f16x2_of_e4m3x2(h1))) << 16);
         }
-#pragma unroll
-        for (int o = 8; o; o >>= 1)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) code[k] = absmax_bf16x2(code[k], __shfl_xor_sync(0xFFFFFFFFu, code[k], o));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          code[k] = bf16_scale_code(max(code[k] & 0x7FFFu, (code[k] >> 16) & 0x7FFFu));
-          const float inv = code[k] == 255u ? 0.f : e8m0_to_float(254u - code[k]);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            // 8 significant bits up to 448: exact in f16 (down to 2^-17), and so is what the first term leaves.
-            const uint32_t a = v[k][2 * i], b = v[k][2 * i + 1];
-            const uint32_t e0 = f16x2_of(__uint_as_float(a << 16) * inv, __uint_as_float(a & 0xFFFF0000u) * inv);
-            const uint32_t e1 = f16x2_of(__uint_as_float(b << 16) * inv, __uint_as_float(b & 0xFFFF0000u) * inv);
-            const uint32_t h0 = e4m3x2_of_f16x2(e0), h1 = e4m3x2_of_f16x2(e1);
-            h[k][i] = h0 | (h1 << 16);
-            l[k][i] = e4m3x2_of_f16x2(sub_f16x2(e0, f16x2_of_e4m3x2(h0))) | (e4m3x2_of_f16x2(sub_f16x2(e1, f16x2_of_e4m3x2(h1))) << 16);
-            if (code[k] == 255u) h[k][i] = l[k][i] = 0u;
-          }
-        }
-        __syncwarp();  // both halves of the rows have been read
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r1 = n + 2 * k;
-          uint8_t* to = sm + tile0 + r1 * 128 + ((((c >> 1) ^ r1) & 7) << 4) + (c & 1) * 8;
-          *reinterpret_cast<uint2*>(to) = make_uint2(h[k][0], h[k][1]);
-          *reinterpret_cast<uint2*>(to + kKvTileBytes) = make_uint2(l[k][0], l[k][1]);
-          if (c == 0)
-            *reinterpret_cast<float*>(stage + 4 * (r1 & 31)) = code[k] == 255u ? NAN : p.scale * 1.4426950408889634f * e8m0_to_float(code[k]);
-        }
+        const int at = ((d ^ r1) & 7) << 4;
+        *reinterpret_cast<uint4*>(to + at) = bad ? make_uint4(0, 0, 0, 0) : make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(to + kKvTileBytes + at) = bad ? make_uint4(0, 0, 0, 0) : make_uint4(l[0], l[1], l[2], l[3]);
       }
       fence_proxy_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(kQfull + 8 * q);
-      return *reinterpret_cast<const float*>(stage + 4 * lane);
+      return bad ? NAN : p.scale * 1.4426950408889634f * e8m0_to_float(code);
     };
     // Through the units, one behind: the next one's queries are on their way before this one's results are waited for.
     float m = kNone, l = 0.f, cq = 0.f;
