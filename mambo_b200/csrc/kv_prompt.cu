@@ -729,27 +729,32 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             if (!plain) {
-              // The last position that the row sees, and the one before the first, in the half; their largest x; then the
-              // weights, which replace the scores from the left, half as wide, behind the columns that have been read.
-              const int high = (int)max((int64_t)-1, min((int64_t)64, place - j0));
-              const int low = p.window ? (int)max((int64_t)-1, min((int64_t)64, place - (int64_t)p.window - j0)) : -1;
-              float top = -INFINITY;
-#pragma unroll 1
+              // The positions that the row sees, a bit each; their x, minus infinity for the others, and the largest of them.
+              const int64_t behind = place + 1 - j0;
+              const int high = (int)max((int64_t)0, min((int64_t)64, behind));
+              const int low = p.window ? (int)max((int64_t)0, min((int64_t)64, behind - p.window)) : 0;
+              const uint64_t bits = (high < 64 ? (1ull << high) - 1 : ~0ull) & (low < 64 ? ~0ull << low : 0ull);
+              const uint32_t seen[2] = {(uint32_t)bits, (uint32_t)(bits >> 32)};
+              uint32_t x[2][32];
+              kv_ld<32>(th, x[0]);
+              kv_ld<32>(th + 32, x[1]);
+              kv_wait_ld();
+              kv_tie(x[0]);
+              kv_tie(x[1]);
+              float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
               for (int g = 0; g < 4; ++g) {
-                uint32_t raw[16];
-                kv_ld<16>(th + 16 * g, raw);
                 const float4 v = sh[g];
                 const float c = cq * v.x;
-                kv_wait_ld();
-                kv_tie(raw);
-                float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                  const int at = 16 * g + k;
-                  if (at <= high && at > low) t4[k & 3] = fmaxf(t4[k & 3], fmaf(__uint_as_float(raw[k]), c, v.y));
+                  uint32_t& at = x[g >> 1][16 * (g & 1) + k];
+                  const bool in = (g < 2 ? seen[0] : seen[1]) >> (16 * (g & 1) + k) & 1;
+                  at = in ? __float_as_uint(fmaf(__uint_as_float(at), c, v.y)) : 0xFF800000u;
+                  t4[k & 3] = fmaxf(t4[k & 3], __uint_as_float(at));
                 }
-                top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
               }
+              const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
               const float up = fmaxf(m, top), f = ex2(m - up);
               m = up;
               l *= f;
@@ -770,28 +775,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                   }
                 }
               }
-#pragma unroll 1
+              // x first and then less m: the row's largest is 2^0 exactly, however large its score and its rounding are.
+#pragma unroll
               for (int g = 0; g < 4; ++g) {
-                uint32_t raw[16], w[8];
-                kv_ld<16>(th + 16 * g, raw);
-                const float4 v = sh[g];
-                const float c = cq * v.x;
-                kv_wait_ld();
-                kv_tie(raw);
-                // x first and then less m: the row's largest is 2^0 exactly, however large its score and its rounding are.
                 float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
                 for (int k = 0; k < 16; k += 2) {
-                  const int at = 16 * g + k;
-                  const float a = at <= high && at > low ? ex2(fmaf(__uint_as_float(raw[k]), c, v.y) - m) : 0.f;
-                  const float b = at + 1 <= high && at + 1 > low ? ex2(fmaf(__uint_as_float(raw[k + 1]), c, v.y) - m) : 0.f;
-                  sum0 += a;
-                  sum1 += b;
-                  w[k >> 1] = f16x2_of(a, b);
+                  uint32_t (&at)[32] = x[g >> 1];
+                  const float e0 = ex2(__uint_as_float(at[16 * (g & 1) + k]) - m), e1 = ex2(__uint_as_float(at[16 * (g & 1) + k + 1]) - m);
+                  sum0 += e0;
+                  sum1 += e1;
+                  x[0][8 * g + (k >> 1)] = f16x2_of(e0, e1);  // behind what has been read
                 }
-                l = fmaf(sum0 + sum1, v.z, l);
-                tc::st_x8(th + 8 * g, w);
+                l = fmaf(sum0 + sum1, sh[g].z, l);
               }
+              tc::st_cols<32>(th, x[0]);
             }
             tc::wait_st();
             tc::fence_before_sync();
