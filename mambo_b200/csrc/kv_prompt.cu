@@ -859,17 +859,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int cta1 = whole ? 0 : kv_owner(unit.x + unit.tiles - 1, total, ctas);
         auto part = [&](int cta) { return partials + ((int64_t)(cta * 2 + (cta == cta0)) * 2 + q) * kPart; };
         const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint32_t o[32];
+        if (started) kv_ld<32>(to_, o);
 #pragma unroll 1
         for (int c = 0; c < p.cache.dim; c += 32) {
-          uint32_t o[32];
           float v[32];
-          if (started) {
-            kv_ld<32>(to_ + c, o);
-            kv_wait_ld();
-            kv_tie(o);
-          }
+          if (started) kv_wait_ld();
+          kv_tie(o);
 #pragma unroll
           for (int k = 0; k < 32; ++k) v[k] = started ? __uint_as_float(o[k]) : 0.f;
+          if (started && c + 32 < p.cache.dim) kv_ld<32>(to_ + c + 32, o);
           if (whole) {
 #pragma unroll
             for (int k = 0; k < 32; ++k) v[k] = l == 0.f ? 0.f : v[k] * inv;
