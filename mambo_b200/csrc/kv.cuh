@@ -70,6 +70,8 @@ struct KvAppendCall {
   int64_t xs_t[2], xs_h[2];
   int bf16;
   int heads_each;      // heads of a CTA
+  int rows_each;       // tokens of a CTA's threads at a time
+  int first;           // of the launch: 0 keys (and values), 1 values
 };
 cudaError_t launch_kv_append(KvAppendCall p, cudaStream_t stream);
 

@@ -10,6 +10,8 @@
 #include "kv.cuh"
 #include "mxfp8.cuh"
 
+#include <type_traits>
+
 namespace mambo {
 
 namespace {
@@ -63,64 +65,21 @@ __device__ __forceinline__ RotaryUnit rotary_unit(const RotaryParams& r, int dim
   return v;
 }
 
-// 16 values of a unit: lo[i] at a + i, hi[i] at b + i. Vectors where everything is a multiple of 8 elements and 16 bytes.
-template <bool kVec, bool k16>
-__device__ __forceinline__ void unit_load(const void* x, int64_t at, const RotaryUnit& u, float (&lo)[8], float (&hi)[8]) {
-  if constexpr (kVec && k16) {
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(x) + at;
-    const uint4 l = __ldg(reinterpret_cast<const uint4*>(p + u.a)), h = __ldg(reinterpret_cast<const uint4*>(p + u.b));
-    const uint32_t lw[4] = {l.x, l.y, l.z, l.w}, hw[4] = {h.x, h.y, h.z, h.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      lo[2 * i] = __uint_as_float(lw[i] << 16);
-      lo[2 * i + 1] = __uint_as_float(lw[i] & 0xFFFF0000u);
-      hi[2 * i] = __uint_as_float(hw[i] << 16);
-      hi[2 * i + 1] = __uint_as_float(hw[i] & 0xFFFF0000u);
-    }
-  } else if constexpr (kVec) {
-    const float* p = reinterpret_cast<const float*>(x) + at;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float4 l = __ldg(reinterpret_cast<const float4*>(p + u.a) + i), h = __ldg(reinterpret_cast<const float4*>(p + u.b) + i);
-      lo[4 * i] = l.x, lo[4 * i + 1] = l.y, lo[4 * i + 2] = l.z, lo[4 * i + 3] = l.w;
-      hi[4 * i] = h.x, hi[4 * i + 1] = h.y, hi[4 * i + 2] = h.z, hi[4 * i + 3] = h.w;
-    }
-  } else {
-    auto one = [&](int d) {
-      if constexpr (k16) return __uint_as_float((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(x) + at + d) << 16);
-      return __ldg(reinterpret_cast<const float*>(x) + at + d);
-    };
-    const int n0 = u.adjacent ? u.n : u.turned, n1 = u.adjacent ? u.n - 8 : u.turned;  // values from a and from b on
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      lo[i] = i < n0 ? one(u.a + i) : 0.f;
-      hi[i] = i < n1 ? one(u.b + i) : 0.f;
-    }
-  }
-}
-
-// A unit's values as they come: 16 bf16, or 16 floats.
-template <bool kVec, bool k16>
+// The 16 values of a unit as they come: eight from a on, eight from b on. Everything is a multiple of 8 elements and 16 bytes.
+template <bool k16>
 struct RawUnit {
-  static constexpr bool kPacked = kVec && k16;
-  uint4 w[kPacked ? 2 : 4];
+  uint4 w[k16 ? 2 : 4];
   __device__ __forceinline__ void load(const void* x, int64_t at, const RotaryUnit& u) {
-    if constexpr (kPacked) {
-      const uint16_t* p = reinterpret_cast<const uint16_t*>(x) + at;
-      w[0] = __ldg(reinterpret_cast<const uint4*>(p + u.a));
-      w[1] = __ldg(reinterpret_cast<const uint4*>(p + u.b));
-    } else {
-      float lo[8], hi[8];
-      unit_load<kVec, k16>(x, at, u, lo, hi);
+    const uint8_t* p = reinterpret_cast<const uint8_t*>(x) + at * (k16 ? 2 : 4);
+    constexpr int kHalf = k16 ? 1 : 2;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        w[i] = make_uint4(__float_as_uint(lo[4 * i]), __float_as_uint(lo[4 * i + 1]), __float_as_uint(lo[4 * i + 2]), __float_as_uint(lo[4 * i + 3]));
-        w[2 + i] = make_uint4(__float_as_uint(hi[4 * i]), __float_as_uint(hi[4 * i + 1]), __float_as_uint(hi[4 * i + 2]), __float_as_uint(hi[4 * i + 3]));
-      }
+    for (int i = 0; i < kHalf; ++i) {
+      w[i] = __ldg(reinterpret_cast<const uint4*>(p + u.a * (k16 ? 2 : 4)) + i);
+      w[kHalf + i] = __ldg(reinterpret_cast<const uint4*>(p + u.b * (k16 ? 2 : 4)) + i);
     }
   }
   __device__ __forceinline__ void get(float (&lo)[8], float (&hi)[8]) const {
-    if constexpr (kPacked) {
+    if constexpr (k16) {
       const uint32_t l[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, h[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -139,6 +98,29 @@ struct RawUnit {
     }
   }
 };
+// A pair of values of a row that is not made of aligned vectors: pairs that turn, then neighbours that do not.
+struct RotaryPair {
+  int a, b;
+  bool turns, halves;
+};
+__host__ __device__ __forceinline__ int rotary_pairs(const RotaryParams& r, int dim) {
+  const int pairs = r.turns ? r.pairs : 0;
+  return r.interleaved ? (dim + 1) / 2 : pairs + (dim - 2 * pairs + 1) / 2;
+}
+__device__ __forceinline__ RotaryPair rotary_pair(const RotaryParams& r, int i) {
+  const int pairs = r.turns ? r.pairs : 0;
+  RotaryPair v;
+  v.turns = i < pairs;
+  v.halves = v.turns && !r.interleaved;
+  v.a = v.halves ? i : r.interleaved ? 2 * i : 2 * pairs + 2 * (i - pairs);
+  v.b = v.halves ? i + pairs : v.a + 1;
+  return v;
+}
+template <bool k16>
+__device__ __forceinline__ float one_value(const void* x, int64_t at) {
+  if constexpr (k16) return __uint_as_float((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(x) + at) << 16);
+  else return __ldg(reinterpret_cast<const float*>(x) + at);
+}
 // cos and sin of the unit's pairs, times the magnitude; 1 and 0 for those that do not turn.
 __device__ __forceinline__ void unit_angles(const RotaryParams& r, const RotaryUnit& u, int pair0, int64_t position,
                                             float (&c)[8], float (&s)[8]) {
@@ -177,39 +159,28 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&b);
 }
 
-template <bool kVec, bool k16>
+template <bool k16>
 __device__ __forceinline__ void unit_store(void* out, int64_t at, const RotaryUnit& u, const float (&lo)[8],
                                            const float (&hi)[8]) {
-  if constexpr (kVec && k16) {
+  if constexpr (k16) {
     uint16_t* p = reinterpret_cast<uint16_t*>(out) + at;
     *reinterpret_cast<uint4*>(p + u.a) =
         make_uint4(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7]));
     *reinterpret_cast<uint4*>(p + u.b) =
         make_uint4(pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3]), pack_bf16(hi[4], hi[5]), pack_bf16(hi[6], hi[7]));
-  } else if constexpr (kVec) {
+  } else {
     float* p = reinterpret_cast<float*>(out) + at;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       reinterpret_cast<float4*>(p + u.a)[i] = make_float4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
       reinterpret_cast<float4*>(p + u.b)[i] = make_float4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
     }
-  } else {
-    auto one = [&](int d, float v) {
-      if constexpr (k16) reinterpret_cast<__nv_bfloat16*>(out)[at + d] = __float2bfloat16_rn(v);
-      else reinterpret_cast<float*>(out)[at + d] = v;
-    };
-    const int n0 = u.adjacent ? u.n : u.turned, n1 = u.adjacent ? u.n - 8 : u.turned;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i < n0) one(u.a + i, lo[i]);
-      if (i < n1) one(u.b + i, hi[i]);
-    }
   }
 }
 
 // A unit's angles need its first pair's number: 8 per rotated unit.
-template <bool kVec, bool k16, int kPer>
-__global__ void __launch_bounds__(256, kPer == 4 && kVec && k16 ? 3 : 1) rotary_kernel(const __grid_constant__ RotaryCall p) {
+template <bool k16, int kPer>
+__global__ void __launch_bounds__(256, kPer == 4 && k16 ? 3 : 1) rotary_kernel(const __grid_constant__ RotaryCall p) {
   const int64_t job = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int per_token = p.units * p.groups;
   const int64_t token = job / per_token;
@@ -218,7 +189,7 @@ __global__ void __launch_bounds__(256, kPer == 4 && kVec && k16 ? 3 : 1) rotary_
   if (token >= p.tokens) return;
   const int in = (int)(job - token * per_token), g = in / p.units, unit = in - g * p.units;
   const RotaryUnit u = rotary_unit(p.rot, p.dim, unit);
-  RawUnit<kVec, k16> raw[kPer];
+  RawUnit<k16> raw[kPer];
   const int64_t from = token * p.xs_t, to = token * p.os_t;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
@@ -239,15 +210,74 @@ __global__ void __launch_bounds__(256, kPer == 4 && kVec && k16 ? 3 : 1) rotary_
       float lo[8], hi[8];
       raw[i].get(lo, hi);
       if (turns) unit_turn(p.rot.interleaved, c, s, lo, hi);
-      unit_store<kVec, k16>(p.out, to + h * p.os_h, u, lo, hi);
+      unit_store<k16>(p.out, to + h * p.os_h, u, lo, hi);
     }
   }
 }
 
-template <bool kVec, bool k16>
-const void* rotary_variant(int per) {
-  return per == 4 ? (const void*)rotary_kernel<kVec, k16, 4> : per == 2 ? (const void*)rotary_kernel<kVec, k16, 2>
-                                                                        : (const void*)rotary_kernel<kVec, k16, 1>;
+// The same where rows are not made of aligned vectors (a half of odd size, an odd address): a thread has one pair of
+// values of its heads, neighbours in the row for neighbours in the warp. 10926 tokens x 24 heads of 80, 34 of them turned
+// in halves: 38 us; 16 dimensions a thread as above, value by value, took 116.
+template <bool k16, int kPer>
+__global__ void __launch_bounds__(256) rotary_pairs_kernel(const __grid_constant__ RotaryCall p) {
+  using T = typename std::conditional<k16, uint16_t, float>::type;
+  const int64_t job = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per_token = p.units * p.groups;
+  const int64_t token = job / per_token;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (token >= p.tokens) return;
+  const int in = (int)(job - token * per_token), g = in / p.units, pair = in - g * p.units;
+  const RotaryPair at = rotary_pair(p.rot, pair);
+  const int a = at.a, b = at.b;
+  const bool turns = at.turns;
+  const bool two = b < p.dim;  // of an odd number of dimensions the last is alone
+  const T* x = reinterpret_cast<const T*>(p.x) + token * p.xs_t;
+  T lo[kPer], hi[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int h = g + i * p.groups;
+    if (h < p.heads) {
+      lo[i] = __ldg(x + h * p.xs_h + a);
+      if (two) hi[i] = __ldg(x + h * p.xs_h + b);
+    }
+  }
+  float c = 1.f, s = 0.f;
+  if (turns) {
+    const int64_t position = p.positions64 ? __ldg(reinterpret_cast<const long long*>(p.positions) + token)
+                                           : (int64_t)__ldg(reinterpret_cast<const int*>(p.positions) + token);
+    turn_cos_sin((uint64_t)position * __ldg(reinterpret_cast<const unsigned long long*>(p.rot.turns) + pair), c, s);
+    c *= p.rot.magnitude;
+    s *= p.rot.magnitude * p.rot.sign;
+  }
+  T* out = reinterpret_cast<T*>(p.out) + token * p.os_t;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int h = g + i * p.groups;
+    if (h >= p.heads) continue;
+    if (turns) {
+      float u, v;
+      if constexpr (k16) u = __uint_as_float((uint32_t)lo[i] << 16), v = __uint_as_float((uint32_t)hi[i] << 16);
+      else u = lo[i], v = hi[i];
+      const float first = fmaf(u, c, -v * s), second = fmaf(u, s, v * c);
+      if constexpr (k16) {
+        const uint32_t both = pack_bf16(first, second);
+        lo[i] = (uint16_t)both, hi[i] = (uint16_t)(both >> 16);
+      } else {
+        lo[i] = first, hi[i] = second;
+      }
+    }
+    out[h * p.os_h + a] = lo[i];
+    if (two) out[h * p.os_h + b] = hi[i];
+  }
+}
+
+template <bool k16>
+const void* rotary_variant(bool vec, int per) {
+  if (vec)
+    return per == 4 ? (const void*)rotary_kernel<k16, 4> : per == 2 ? (const void*)rotary_kernel<k16, 2> : (const void*)rotary_kernel<k16, 1>;
+  return per == 4 ? (const void*)rotary_pairs_kernel<k16, 4>
+                  : per == 2 ? (const void*)rotary_pairs_kernel<k16, 2> : (const void*)rotary_pairs_kernel<k16, 1>;
 }
 
 // ---------------------------------------------------------------------------
@@ -259,12 +289,10 @@ const void* rotary_variant(int per) {
 // so that it keeps their cosines and sines; the next head's values are on
 // their way while one is quantized.
 // ---------------------------------------------------------------------------
-// Units of a thread: one in the vector form, which keeps its registers at 64 (a page of 64 tokens with two units a thread
-// and 128 registers took 42 us for 16384 tokens).
-template <bool kVec>
-constexpr int kAppendPasses = kVec ? 1 : 2;
-template <bool kVec>
-constexpr int kAppendThreads = kVec ? 1024 : 640;  // most, of a CTA: 128 tokens x 8 units, or 9 where the rotated part ends inside one
+// In the vector form a thread has one unit, which keeps its registers at 64 (a page of 64 tokens with two units a thread
+// and 128 registers took 42 us for 16384 tokens). Otherwise it has one pair of values of every `rows_each`th token.
+constexpr int kAppendThreads = 1024;  // most, of a CTA: 128 tokens x 8 units
+constexpr int kAppendRows = 8;        // most, of a thread: 128 tokens x 64 pairs
 
 // mxfp8_scale_code from a magnitude's bits, without branches; of zero 0.
 __device__ __forceinline__ uint32_t f32_scale_code(uint32_t bits) {
@@ -297,9 +325,9 @@ __device__ __forceinline__ int append_slot(const KvSequences& s, int b, int log_
 }
 
 template <bool kVec, bool k16>
-__global__ void __launch_bounds__(kAppendThreads<kVec>) kv_append_kernel(const __grid_constant__ KvAppendCall p) {
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ KvAppendCall p) {
   __shared__ float sm_max[2][32];
-  const int which = blockIdx.z, threads = blockDim.x;
+  const int which = p.first + blockIdx.z, threads = blockDim.x;
   const KvCache& cache = p.cache;
   const int page = cache.page, dim = cache.dim;
   const int head0 = blockIdx.y * p.heads_each, head1 = min(head0 + p.heads_each, cache.heads);
@@ -330,25 +358,33 @@ __global__ void __launch_bounds__(kAppendThreads<kVec>) kv_append_kernel(const _
 
   RotaryParams rot = p.rot;
   if (which == 1) rot = RotaryParams{nullptr, 0, 0, 1.f, 1.f};
-  const int units = rotary_units(rot, dim), all = count * units;
-  const int64_t xs_h = p.xs_h[which];
-  constexpr int kPasses = kAppendPasses<kVec>;
+  const int64_t xs_h = p.xs_h[which], xs_t = p.xs_t[which];
+  const int units = kVec ? rotary_units(rot, dim) : rotary_pairs(rot, dim);
+  const int row = threadIdx.x / units, unit = threadIdx.x - row * units;
+  const int64_t from = (span.first + (t0 - past) + row) * xs_t;  // this thread's token: in the input, and its codes in the page
+  const int to = (begun + row) * dim;
   constexpr bool kAhead = kVec && k16;  // the other forms have no registers for it
-  int64_t from[kPasses];  // this thread's tokens: in the input, and their codes in the page
-  int to[kPasses];
-  RotaryUnit u[kPasses];
-  float c[kPasses][8], s[kPasses][8];
-  RawUnit<kVec, k16> raw[kPasses];
+  RotaryUnit u{};
+  RotaryPair pair{};
+  RawUnit<k16> raw;
+  float c[8], s[8];  // of the unit's pairs, or of the pair for each token
+  const int rows = row < p.rows_each ? (count - row + p.rows_each - 1) / p.rows_each : 0;  // of this thread
+  if constexpr (kVec) {
+    if (rows > 0) {
+      u = rotary_unit(rot, dim, unit);
+      if constexpr (kAhead) raw.load(p.x[which], from + head0 * xs_h, u);
+      if (u.turned > 0) unit_angles(rot, u, 8 * unit, t0 + row, c, s);
+    }
+  } else {
+    pair = rotary_pair(rot, unit);
+    const uint64_t f = pair.turns ? __ldg(reinterpret_cast<const unsigned long long*>(rot.turns) + unit) : 0ull;
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int f = threadIdx.x + i * threads;
-    if (f < all) {
-      const int row = f / units, unit = f - row * units;
-      u[i] = rotary_unit(rot, dim, unit);
-      from[i] = (span.first + (t0 - past) + row) * p.xs_t[which];
-      to[i] = (begun + row) * dim;
-      if constexpr (kAhead) raw[i].load(p.x[which], from[i] + head0 * xs_h, u[i]);
-      if (u[i].turned > 0) unit_angles(rot, u[i], 8 * unit, t0 + row, c[i], s[i]);
+    for (int i = 0; i < kAppendRows; ++i) {
+      if (i < rows && pair.turns) {
+        turn_cos_sin((uint64_t)(t0 + row + i * p.rows_each) * f, c[i], s[i]);
+        c[i] *= rot.magnitude;
+        s[i] *= rot.magnitude;
+      }
     }
   }
   if (where < 0 || where >= cache.pages) return;  // (after the values' loads, which do not wait for the page)
@@ -357,19 +393,38 @@ __global__ void __launch_bounds__(kAppendThreads<kVec>) kv_append_kernel(const _
   const int lane = threadIdx.x & 31, warps = threads / 32;
   for (int head = head0; head < head1; ++head, ++scale_at, codes += page * dim) {
     const uint32_t old = begun ? *scale_at : 0u;
-    float lo[kPasses][8], hi[kPasses][8];
+    float lo[8], hi[8];
     float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      if ((int)threadIdx.x + i * threads < all) {
-        if constexpr (!kAhead) raw[i].load(p.x[which], from[i] + head * xs_h, u[i]);
-        raw[i].get(lo[i], hi[i]);
+    if constexpr (kVec) {
+      if (rows > 0) {
+        if constexpr (!kAhead) raw.load(p.x[which], from + head * xs_h, u);
+        raw.get(lo, hi);
         if constexpr (kAhead) {
-          if (head + 1 < head1) raw[i].load(p.x[which], from[i] + (head + 1) * xs_h, u[i]);
+          if (head + 1 < head1) raw.load(p.x[which], from + (head + 1) * xs_h, u);
         }
-        if (u[i].turned > 0) unit_turn(rot.interleaved, c[i], s[i], lo[i], hi[i]);
+        if (u.turned > 0) unit_turn(rot.interleaved, c, s, lo, hi);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = absmax3(top, lo[i][j], hi[i][j]);
+        for (int j = 0; j < 8; ++j) top = absmax3(top, lo[j], hi[j]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kAppendRows; ++i) {
+        if (i < rows) {
+          const int64_t at = from + head * xs_h + i * p.rows_each * xs_t;
+          lo[i] = one_value<k16>(p.x[which], at + pair.a);
+          hi[i] = one_value<k16>(p.x[which], at + pair.b);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAppendRows; ++i) {
+        if (i < rows) {
+          if (pair.turns) {
+            const float a = lo[i], b2 = hi[i];
+            lo[i] = fmaf(a, c[i], -b2 * s[i]);
+            hi[i] = fmaf(a, s[i], b2 * c[i]);
+          }
+          top = absmax3(top, lo[i], hi[i]);
+        }
       }
     }
     // As integers: NaN and infinity order above every number.
@@ -392,27 +447,29 @@ __global__ void __launch_bounds__(kAppendThreads<kVec>) kv_append_kernel(const _
       }
     }
     const float inv = code == 255u ? 0.f : e8m0_to_float(254u - code);
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int f = threadIdx.x + i * threads;
-      if (f < all) {
-        uint8_t* at = codes + to[i];
+    if constexpr (kVec) {
+      if (rows > 0) {
         uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          w[j] = e4m3x4(lo[i][4 * j] * inv, lo[i][4 * j + 1] * inv, lo[i][4 * j + 2] * inv, lo[i][4 * j + 3] * inv);
-          w[2 + j] = e4m3x4(hi[i][4 * j] * inv, hi[i][4 * j + 1] * inv, hi[i][4 * j + 2] * inv, hi[i][4 * j + 3] * inv);
+          w[j] = e4m3x4(lo[4 * j] * inv, lo[4 * j + 1] * inv, lo[4 * j + 2] * inv, lo[4 * j + 3] * inv);
+          w[2 + j] = e4m3x4(hi[4 * j] * inv, hi[4 * j + 1] * inv, hi[4 * j + 2] * inv, hi[4 * j + 3] * inv);
         }
         if (code == 255u) w[0] = w[1] = w[2] = w[3] = 0u;  // zero times NaN has a code of its own
-        if constexpr (kVec) {
-          *reinterpret_cast<uint2*>(at + u[i].a) = make_uint2(w[0], w[1]);
-          *reinterpret_cast<uint2*>(at + u[i].b) = make_uint2(w[2], w[3]);
-        } else {
-          const int n0 = u[i].adjacent ? u[i].n : u[i].turned, n1 = u[i].adjacent ? u[i].n - 8 : u[i].turned;
+        *reinterpret_cast<uint2*>(codes + to + u.a) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(codes + to + u.b) = make_uint2(w[2], w[3]);
+      }
+    } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (j < n0) at[u[i].a + j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
-            if (j < n1) at[u[i].b + j] = (uint8_t)(w[2 + (j >> 2)] >> (8 * (j & 3)));
+      for (int i = 0; i < kAppendRows; ++i) {
+        if (i < rows) {
+          uint8_t* at = codes + to + i * p.rows_each * dim;
+          const uint32_t w = code == 255u ? 0u : cvt_e4m3x2_rn(lo[i] * inv, hi[i] * inv);
+          if (pair.halves) {
+            at[pair.a] = (uint8_t)w;
+            at[pair.b] = (uint8_t)(w >> 8);
+          } else {
+            *reinterpret_cast<uint16_t*>(at + pair.a) = (uint16_t)w;
           }
         }
       }
@@ -425,35 +482,43 @@ __global__ void __launch_bounds__(kAppendThreads<kVec>) kv_append_kernel(const _
 
 cudaError_t launch_rotary(RotaryCall p, cudaStream_t stream) {
   const int es = p.bf16 ? 2 : 4;
-  p.units = rotary_units(p.rot, p.dim);
   const bool vec = p.dim % 16 == 0 && (p.rot.interleaved || p.rot.pairs % 8 == 0) && (uintptr_t)p.x % 16 == 0 &&
                    (uintptr_t)p.out % 16 == 0 && p.xs_t * es % 16 == 0 && p.xs_h * es % 16 == 0 && p.os_t * es % 16 == 0 &&
                    p.os_h * es % 16 == 0;
+  p.units = vec ? rotary_units(p.rot, p.dim) : rotary_pairs(p.rot, p.dim);
   const int64_t head_units = (int64_t)p.tokens * p.heads * p.units;
   // Heads of a thread, which share its cosines and sines: four or two where that leaves 512 threads an SM.
   const int per = head_units >= 4 * 148 * 512 ? 4 : head_units >= 2 * 148 * 512 ? 2 : 1;
   p.groups = (p.heads + per - 1) / per;
   const int64_t jobs = (int64_t)p.tokens * p.groups * p.units;
-  const void* k = p.bf16 ? (vec ? rotary_variant<true, true>(per) : rotary_variant<false, true>(per))
-                         : (vec ? rotary_variant<true, false>(per) : rotary_variant<false, false>(per));
+  const void* k = p.bf16 ? rotary_variant<true>(vec, per) : rotary_variant<false>(vec, per);
   return launch_pdl(k, dim3((unsigned)((jobs + 255) / 256)), dim3(256), 0, stream, p);
 }
 
 cudaError_t launch_kv_append(KvAppendCall p, cudaStream_t stream) {
   const int es = p.bf16 ? 2 : 4;
-  bool vec = !p.rot.turns || p.rot.interleaved || p.rot.pairs % 8 == 0;
+  bool vec[2];
   for (int i = 0; i < 2; ++i)
-    vec = vec && (uintptr_t)p.x[i] % 16 == 0 && p.xs_t[i] * es % 16 == 0 && p.xs_h[i] * es % 16 == 0;
+    vec[i] = (i == 1 || !p.rot.turns || p.rot.interleaved || p.rot.pairs % 8 == 0) && (uintptr_t)p.x[i] % 16 == 0 &&
+             p.xs_t[i] * es % 16 == 0 && p.xs_h[i] * es % 16 == 0;
   const int slots = p.seq.offsets ? (p.seq.tokens >> p.cache.log_page) + 2 * p.seq.batch : p.seq.batch;
-  // One token a sequence is at most 9 units and needs a warp.
-  const int units = max(rotary_units(p.rot, p.cache.dim), (p.cache.dim + 15) / 16), page_units = p.cache.page * units;
-  const int threads = !p.seq.offsets ? 32 : ((vec ? page_units : (page_units + 1) / 2) + 31) / 32 * 32;
   // Heads of a CTA: as many as leave six CTAs an SM.
   p.heads_each = max(1, min(p.cache.heads, (int)((int64_t)slots * p.cache.heads * 2 / (148 * 6))));
   const unsigned groups = (unsigned)((p.cache.heads + p.heads_each - 1) / p.heads_each);
-  const void* k = p.bf16 ? (vec ? (const void*)kv_append_kernel<true, true> : (const void*)kv_append_kernel<false, true>)
-                         : (vec ? (const void*)kv_append_kernel<true, false> : (const void*)kv_append_kernel<false, false>);
-  return launch_pdl(k, dim3((unsigned)slots, groups, 2), dim3(threads), 0, stream, p);
+  // Keys and values in one launch where both have the same form.
+  for (int i = 0; i < 2; ++i) {
+    const bool both = vec[0] == vec[1];
+    if (both && i == 1) break;
+    const int units = vec[i] ? p.cache.dim / 16 : p.cache.dim / 2, page = p.seq.offsets ? p.cache.page : 1;
+    p.rows_each = vec[i] ? page : (page + kAppendRows - 1) / kAppendRows;
+    p.first = i;
+    const int threads = (p.rows_each * units + 31) / 32 * 32;
+    const void* k = p.bf16 ? (vec[i] ? (const void*)kv_append_kernel<true, true> : (const void*)kv_append_kernel<false, true>)
+                           : (vec[i] ? (const void*)kv_append_kernel<true, false> : (const void*)kv_append_kernel<false, false>);
+    const cudaError_t e = launch_pdl(k, dim3((unsigned)slots, groups, both ? 2 : 1), dim3(threads), 0, stream, p);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace mambo
