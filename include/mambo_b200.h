@@ -657,7 +657,9 @@ MAMBO_API int mambo_kv_append(const MamboKvCache* cache, const void* k, int64_t 
  * last `window` of them where window is not 0:
  *   out = sum_j softmax_j(scale * q . k_j) v_j   (bf16),   lse = log sum_j exp(scale * q . k_j)   (f32, may be null).
  * A query that sees nothing has zeros and an lse of minus infinity; rows that
- * no sequence covers are not written. The heads of q and out are 16-byte
+ * no sequence covers are not written. Positions of a page outside the cache do
+ * not exist; what no query sees may hold anything. Value scales of the pages
+ * that a query sees may be 2^100 apart. out may be q, with its strides. The heads of q and out are 16-byte
  * aligned (strides in multiples of 8). scale: a positive number. workspace:
  * mambo_kv_attention_workspace_bytes(ragged: with offsets), zero-filled once,
  * shared with the other calls of the stream.

@@ -6,7 +6,7 @@
 // is as precise as the first; its cosine and sine are the Taylor polynomials
 // on an eighth of a turn to either side (below). A cosine and sine serve
 // several heads of the token where there is enough to do. 8192 tokens x 32
-// heads of 128 in bf16: 23.5 us, 0.87 of a measured copy. Append of 16384
+// heads of 128 in bf16: 23.5 us, 0.87 of a measured copy. Append of 17059
 // tokens x 8 heads of 128: 28 us, 0.57 of a copy's rate: 110 instructions a
 // unit of 16 values for the turn, the largest magnitude and the conversions.
 #include "kernels.cuh"
@@ -293,7 +293,7 @@ const void* rotary_variant(bool vec, int per) {
 // their way while one is quantized.
 // ---------------------------------------------------------------------------
 // In the vector form a thread has one unit, which keeps its registers at 64 (a page of 64 tokens with two units a thread
-// and 128 registers took 42 us for 16384 tokens). Otherwise it has one pair of values of every `rows_each`th token.
+// and 128 registers took 42 us for 17059 tokens). Otherwise it has one pair of values of every `rows_each`th token.
 constexpr int kAppendThreads = 1024;  // most, of a CTA: 128 tokens x 8 units
 constexpr int kAppendRows = 8;        // most, of a thread: 128 tokens x 64 pairs
 
@@ -514,7 +514,7 @@ cudaError_t launch_kv_append(KvAppendCall p, cudaStream_t stream) {
     p.first = i;
     const int threads = (p.rows_each * units + 31) / 32 * 32;
     // A CTA has all heads of its page, for which it forms the cosines and sines once, where that leaves 1536 threads an SM,
-    // and fewer otherwise. 16384 tokens, 8 heads: all eight 28 us, four 32, one 56; 64 single tokens: one 2.9, all 5.7.
+    // and fewer otherwise. 17059 tokens, 8 heads: all eight 28 us, four 32, one 56; 64 single tokens: one 2.9, all 5.7.
     const int64_t page_threads = (int64_t)slots * 2 * threads;
     const int most = (int)min((int64_t)p.cache.heads, (148 * 1536 + page_threads - 1) / page_threads);
     p.heads_each = (p.cache.heads + most - 1) / most;

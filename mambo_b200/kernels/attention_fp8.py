@@ -165,6 +165,10 @@ def fp8_paged_attention(q, cache: Fp8KvCache, page_table, lengths, *, offsets=No
     A query sees the positions up to its own, with ``window`` the last
     ``window`` of them. Query head h reads key head h // (Hq / H). ``scale``
     (1/sqrt(D)) multiplies the scores. A query that sees nothing has zeros.
+    Positions of a page outside the cache do not exist. The value scales of the
+    pages that a query sees may be 2^100 apart: positions whose scale is smaller
+    by more are lost from the sum. ``out`` may be q; tokens that no sequence has
+    keep what it holds.
 
     ``return_lse``: also the float32 [T,Hq] logarithms of the sums of the
     exponentials (minus infinity where a query sees nothing), with which

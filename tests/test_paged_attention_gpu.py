@@ -423,6 +423,28 @@ def test_graphs_that_share_a_workspace(cuda_device):
                 assert torch.equal(got[i], want[i])
 
 
+def test_example_layer(cuda_device):
+    """A chunk at a time or all at once, a layer's last token sees the same context."""
+    import sys
+    from pathlib import Path
+
+    sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "examples"))
+    from fp8_attention_layer import AttentionLayer
+
+    x = torch.randn(2 * 40, 256, dtype=BF16, device="cuda")
+    outs = []
+    for cuts in ([40], [17, 22, 1]):
+        layer, at = AttentionLayer(256, 4, 2, 64, batch=2, most=64, page=16), 0
+        for n in cuts:
+            rows = torch.cat([x[at:at + n], x[40 + at:40 + at + n]])
+            positions = torch.arange(at, at + n, device="cuda").repeat(2)
+            out = layer(rows, positions, i32([0, n, 2 * n]) if n > 1 else None)
+            at += n
+        assert layer.lengths.tolist() == [40, 40] and out.isfinite().all()
+        outs.append(out)
+    assert outs[0].shape == (80, 256) and outs[1].shape == (2, 256)
+
+
 def test_refusals(cuda_device):
     cache = prepare_fp8_kv_cache(4, 2, 16, 64)
     q, table, lengths = torch.zeros(2, 4, 64, dtype=BF16, device="cuda"), i32([[0], [1]]), i32([1, 1])
