@@ -167,11 +167,12 @@ int mambo_kv_attention(const void* q, int64_t q_stride_token, int64_t q_stride_h
   if (!aligned(lse, 4)) return api_fail(MAMBO_EINVAL, kUnaligned);
   if (!aligned(q, 16) || !aligned(out, 16) || q_stride_token % 8 || q_stride_head % 8 || out_stride_token % 8 || out_stride_head % 8)
     return api_fail(MAMBO_EINVAL, "the heads of q and out must be 16-byte aligned");
-  // Rows, and tiles of 128 positions over all sequences, heads and units of rows, are counted in 32 bits.
+  // Rows, and tiles of 128 positions over all sequences, heads and units of rows (which count as six more), are counted in
+  // 32 bits.
   const int64_t group = heads / cache->kv_heads;
   const double units = (double)tokens * group / 256 + (double)seq->batch;
   if (tokens * group > (1 << 30) ||
-      units * cache->kv_heads * ((double)seq->table_pages * cache->page_tokens / 128 + 1) >= 2147483647.0)
+      units * cache->kv_heads * ((double)seq->table_pages * cache->page_tokens / 128 + 8) >= 2147483647.0)
     return api_fail(MAMBO_EINVAL, "the call is too large: split its sequences");
   if (!(scale > 0.f) || !(scale <= 3.4028234663852886e38f)) return api_fail(MAMBO_EINVAL, "the scale must be a positive number");
   const bool prompt = seq->offsets || !few_rows((int)group);

@@ -42,7 +42,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxStages = 8;
-constexpr float kNone = -1e30f;      // m of a row that has seen nothing
+constexpr float kNone = -3e38f;      // m of a row that has seen nothing
 constexpr float kHeadroom = 8.7f;    // 2^8.7 < 448
 constexpr float kStart = 4.f;
 

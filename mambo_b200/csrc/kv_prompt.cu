@@ -54,7 +54,7 @@ constexpr int kThreads = 512;
 constexpr int kRows = 128;            // of an MMA tile
 constexpr int kUnitRows = 2 * kRows;
 constexpr int kKStages = 3, kVStages = 2;
-constexpr float kNone = -1e30f;       // m of a row that has seen nothing
+constexpr float kNone = -3e38f;       // m of a row that has seen nothing
 constexpr float kMostSum = 2048.f;    // of 16 weights, before m is moved: f16 holds 2^16
 constexpr float kMostPoly = 100.f;    // of the exponents that the polynomial takes: a larger one would not show in its sum
 // What a unit costs besides its tiles, in tiles: where the ranges of the CTAs are cut, units count as this much longer.

@@ -168,7 +168,7 @@ def fp8_paged_attention(q, cache: Fp8KvCache, page_table, lengths, *, offsets=No
     Positions of a page outside the cache do not exist. The value scales of the
     pages that a query sees may be 2^100 apart: positions whose scale is smaller
     by more are lost from the sum. ``out`` may be q; tokens that no sequence has
-    keep what it holds.
+    keep what it holds (without it, and in the logarithms, anything).
 
     ``return_lse``: also the float32 [T,Hq] logarithms of the sums of the
     exponentials (minus infinity where a query sees nothing), with which

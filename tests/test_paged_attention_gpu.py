@@ -159,6 +159,21 @@ def test_one_score_far_above(cuda_device, jump, counts):
         check(got, lse, q, cache, table, [n], [0, counts[0]])
 
 
+@pytest.mark.parametrize("counts", [[1], [150]])
+def test_scores_near_the_ends_of_float32(cuda_device, counts):
+    """All scores far below zero, one of them above the others; values of one, so that the weights' sum shows."""
+    n, page, dim = 200, 16, 16
+    k = torch.zeros(n, 1, dim)
+    k[:, 0, 0] = -1e18
+    k[130, 0, 0] = -0.5e18
+    cache, table = prepare_fp8_kv_cache(13, 1, page, dim), torch.arange(13, dtype=torch.int32, device="cuda")[None]
+    launch_fp8_kv_append(cache, k.cuda(), torch.ones(n, 1, dim, device="cuda"), table, i32([0]), offsets=i32([0, n]))
+    q = torch.zeros(counts[0], 2, dim, dtype=BF16, device="cuda")
+    q[..., 0] = 1e18
+    got = fp8_paged_attention(q, cache, table, i32([n]), offsets=i32([0, counts[0]]), scale=1.0)
+    assert (got == 1).all()
+
+
 @pytest.mark.parametrize("counts", [[1, 1, 1], [40, 1, 200]])
 @pytest.mark.parametrize("window", [0, 90])
 def test_anything_in_masked_places(cuda_device, counts, window):
