@@ -88,7 +88,8 @@ def attention64(q, cache, table, lengths, offsets=None, window=0, scale=None):
     The queries are exact but for what is below 2^-18 of the row's largest value, so a score is off by that times the
     keys, and by the float32 sums (2^-20 of the products' sum with room). The weights, scaled by their positions' value
     scales, are two E4M3 terms: off by 2^-8 of their value, or by 2^-14 of the row's largest where that is more and the
-    weight not less. The result is rounded to bf16: 2^-8.
+    weight not less. The result is rounded to bf16: 2^-8, or half the smallest step, 2^-133, which is what a result that
+    is not zero in 64 bits alone may be off by.
     """
     dev, (tokens, heads, dim) = q.device, q.shape
     keys, values = (cache[n].view(torch.float8_e4m3fn).double() for n in ("keys", "values"))
@@ -143,7 +144,7 @@ def attention64(q, cache, table, lengths, offsets=None, window=0, scale=None):
         codes = vv.abs() * torch.exp2(-torch.nan_to_num(e))[..., None]
         ob = torch.einsum("hgnj,hjd->hgnd", off, codes) / safe[..., None]
         ob = ob + 2 * es[..., None] * torch.einsum("hgnj,hjd->hgnd", p, vv.abs()) / safe[..., None]
-        ob = ob * (1 + 2.0 ** -7) + 2.0 ** -8 * o.abs()
+        ob = ob * (1 + 2.0 ** -7) + 2.0 ** -8 * o.abs() + 2.0 ** -134
         span = slice(offsets[b], offsets[b + 1])
         back = lambda x: x.permute(2, 0, 1, *range(3, x.ndim)).reshape(n, heads, *x.shape[3:])  # noqa: E731
         out[span], lse[span] = back(o), back(torch.where(some, top[..., 0] + torch.log(safe), torch.full_like(total, -math.inf)))
