@@ -112,7 +112,7 @@ constexpr uint32_t kIdescAlongM = 1u << 15, kIdescAlongN = 1u << 16;
 // took 130 clocks an MMA. So the groups of MMAs below are one asm statement each, which steps the descriptors' low words
 // (start address and leading offset) itself.
 __device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lbo) { return ((saddr & 0x3FFFFu) >> 4) | (lbo >> 4) << 16; }
-constexpr uint32_t desc_high(uint32_t sbo, bool swizzled) { return (sbo >> 4) | 1u << 14 | (swizzled ? 2u << 29 : 0u); }
+__host__ __device__ constexpr uint32_t desc_high(uint32_t sbo, bool swizzled) { return (sbo >> 4) | 1u << 14 | (swizzled ? 2u << 29 : 0u); }
 
 // Two 32-wide steps of E4M3 operands along K (128-byte swizzle, 32 bytes a step), for two terms of B.
 __device__ __forceinline__ void mma_along_k_2x2(uint32_t d, uint32_t a, uint32_t b0, uint32_t b1, uint32_t idesc, uint32_t acc) {
