@@ -645,38 +645,51 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
       // A lane has a row: no shuffles, and one scale for it. (With 16 lanes a row this took 6000 clocks and more, and the
-      // prompt of 8192 tokens 590 us for 575.)
+      // prompt of 8192 tokens 590 us for 575.) In loops, because a short call is paced by the fetch of its instructions: all
+      // at once from registers took 5400 clocks there.
       const int r1 = 32 * (warp & 3) + lane;
       uint8_t* const to = sm + tile0 + r1 * 128;
-      uint32_t v[64], top[4] = {0, 0, 0, 0};
-#pragma unroll
+      uint32_t top[4] = {0, 0, 0, 0};
+#pragma unroll 2
       for (int i = 0; i < 16; ++i) {
-        const uint4 raw4 = *reinterpret_cast<const uint4*>(to + (i >> 3) * kKvTileBytes + (((i ^ r1) & 7) << 4));
-        v[4 * i] = raw4.x, v[4 * i + 1] = raw4.y, v[4 * i + 2] = raw4.z, v[4 * i + 3] = raw4.w;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top[k] = absmax_bf16x2(top[k], v[4 * i + k]);
+        const uint4 x = *reinterpret_cast<const uint4*>(to + (i >> 3) * kKvTileBytes + (((i ^ r1) & 7) << 4));
+        top[0] = absmax_bf16x2(top[0], x.x), top[1] = absmax_bf16x2(top[1], x.y);
+        top[2] = absmax_bf16x2(top[2], x.z), top[3] = absmax_bf16x2(top[3], x.w);
       }
       top[0] = absmax_bf16x2(absmax_bf16x2(top[0], top[1]), absmax_bf16x2(top[2], top[3]));
       const uint32_t code = bf16_scale_code(max(top[0] & 0x7FFFu, (top[0] >> 16) & 0x7FFFu));
       const bool bad = code == 255u;
       const float inv = bad ? 0.f : e8m0_to_float(254u - code);
+      // 16 dimensions d at a time: chunks 2d and 2d + 1 of the row as it came, of which the first terms go to chunk d and the
+      // second ones to chunk 8 + d. In the order 0 to 3, 7 to 4 no chunk is written that is still to be read, but for the
+      // second terms of 0 to 3, which wait in the stage.
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        const int d = i < 4 ? i : 11 - i;
+        uint32_t v[8], h[4], l[4];
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        uint32_t h[4], l[4];
+        for (int k = 0; k < 2; ++k) {
+          const int c2 = 2 * d + k;
+          const uint4 x = *reinterpret_cast<const uint4*>(to + (c2 >> 3) * kKvTileBytes + (((c2 ^ r1) & 7) << 4));
+          v[4 * k] = x.x, v[4 * k + 1] = x.y, v[4 * k + 2] = x.z, v[4 * k + 3] = x.w;
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int k = 0; k < 4; ++k) {
           // 8 significant bits up to 448: exact in f16 (down to 2^-17), and so is what the first term leaves.
-          const uint32_t x = v[8 * d + 2 * i], y = v[8 * d + 2 * i + 1];
+          const uint32_t x = v[2 * k], y = v[2 * k + 1];
           const uint32_t e0 = f16x2_of(__uint_as_float(x << 16) * inv, __uint_as_float(x & 0xFFFF0000u) * inv);
           const uint32_t e1 = f16x2_of(__uint_as_float(y << 16) * inv, __uint_as_float(y & 0xFFFF0000u) * inv);
           const uint32_t h0 = e4m3x2_of_f16x2(e0), h1 = e4m3x2_of_f16x2(e1);
-          h[i] = h0 | (h1 << 16);
-          l[i] = e4m3x2_of_f16x2(sub_f16x2(e0, f16x2_of_e4m3x2(h0))) | (e4m3x2_of_f16x2(sub_f16x2(e1, f16x2_of_e4m3x2(h1))) << 16);
+          h[k] = bad ? 0u : h0 | (h1 << 16);
+          l[k] = bad ? 0u : e4m3x2_of_f16x2(sub_f16x2(e0, f16x2_of_e4m3x2(h0))) | (e4m3x2_of_f16x2(sub_f16x2(e1, f16x2_of_e4m3x2(h1))) << 16);
         }
         const int at = ((d ^ r1) & 7) << 4;
-        *reinterpret_cast<uint4*>(to + at) = bad ? make_uint4(0, 0, 0, 0) : make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(to + kKvTileBytes + at) = bad ? make_uint4(0, 0, 0, 0) : make_uint4(l[0], l[1], l[2], l[3]);
+        *reinterpret_cast<uint4*>(to + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(i < 4 ? stage + d * 512 + lane * 16 : to + kKvTileBytes + at) = make_uint4(l[0], l[1], l[2], l[3]);
       }
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        *reinterpret_cast<uint4*>(to + kKvTileBytes + (((d ^ r1) & 7) << 4)) = *reinterpret_cast<const uint4*>(stage + d * 512 + lane * 16);
       fence_proxy_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(kQfull + 8 * q);
