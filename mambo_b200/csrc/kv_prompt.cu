@@ -375,18 +375,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             u.from[q] = low > 0 ? (int)(low / kKvTile) : 0;
             u.to[q] = u.hi[q] >= 0 ? u.hi[q] / kKvTile + 1 : 0;
           }
-          // The unit's queries on their way to the L2.
-#pragma unroll 1
-          for (int i = lane; i < kUnitRows && u.row0 + i < u.rows; i += 32) {
-            const int row = u.row0 + i, tok = row / p.group;
-            bulk_prefetch_l2(p.q + (int64_t)(u.token + tok) * p.qs_t + (int64_t)(u.h * p.group + row - tok * p.group) * p.qs_h, p.cache.dim * 2);
-          }
           if (x < x1) plan.next();
         }
         if (count >= kUnitStages && !(ok = kv_warp_wait(kUfree + 8 * ur.at, ur.phase ^ 1, kSiteKvEmpty))) u.n = 0;
         if (lane == 0) {
           units[ur.at] = u;
           mbar_arrive(kUfull + 8 * ur.at);
+        }
+        // The unit's queries on their way to the L2; those of the first are fetched at once.
+        if (count > 0 && u.n > 0) {
+#pragma unroll 1
+          for (int i = lane; i < kUnitRows && u.row0 + i < u.rows; i += 32) {
+            const int row = u.row0 + i, tok = row / p.group;
+            bulk_prefetch_l2(p.q + (int64_t)(u.token + tok) * p.qs_t + (int64_t)(u.h * p.group + row - tok * p.group) * p.qs_h, p.cache.dim * 2);
+          }
         }
         ur.next(kUnitStages);
         ++count;
