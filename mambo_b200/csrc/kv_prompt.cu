@@ -397,7 +397,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       Unit ahead = unit_ahead();
       for (int it = 0; ok && ahead.n > 0;) {
         const Unit u = ahead;
-        ahead = unit_ahead();
         const int n = u.n, h = u.h;
         const int64_t i0 = (int64_t)u.tile * per_tile + lane;
         const int* row_pages = p.seq.table + u.b * p.seq.table_stride + i0;
@@ -422,6 +421,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           page = next_page;
           kr.next(kKStages);
           vr.next(kVStages);
+          if (t == 0) ahead = unit_ahead();  // the next unit, behind the first loads of this one
+          if (!ok) break;
         }
       }
       if (!ok) kv_settle();
