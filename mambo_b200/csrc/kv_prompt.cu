@@ -27,7 +27,8 @@
 // none, a quarter and a half took 602, 596 and 629 us where an eighth took 588)
 // and the tensor core 2050 (2700 with what scores of 64 positions read from
 // shared memory). 32 query heads over 8 key heads of 128, 8192 tokens of a
-// prompt: 551-562 us, 980-1000 TFLOP/s.
+// prompt: 528 us, 1041 TFLOP/s, 0.63 of the measured rate of 16-bit products
+// (584 us where calls follow larger ones, at the power limit).
 //
 // Work: all units' tiles in a row, one equal range per SM (units have unequal
 // lengths under the causal mask, and there may be few of them). A unit that
@@ -59,7 +60,7 @@ constexpr float kMostSum = 2048.f;    // of 16 weights, before m is moved: f16 h
 constexpr float kMostPoly = 100.f;    // of the exponents that the polynomial takes: a larger one would not show in its sum
 // What a unit costs besides its tiles, in tiles: where the ranges of the CTAs are cut, units count as this much longer.
 // Queries, the first scores, masked halves and the results are some 15000 clocks. Prompt of 8192 tokens and a mixed step:
-// 4 551 and 113 us, 5 545 and 113, 6 549 and 106-111.
+// 3 552 and 100 us, 4 529 and 102, 5 525 and 102, 6 528 and 100.
 constexpr int kUnitCost = 6;
 
 // Shared memory: queries [2 tiles][hi, lo][128][128], keys, values as they come and in f16 [2 halves of D][128][128 bytes].
