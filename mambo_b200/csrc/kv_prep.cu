@@ -7,7 +7,7 @@
 // on an eighth of a turn to either side (below). A cosine and sine serve
 // several heads of the token where there is enough to do. 8192 tokens x 32
 // heads of 128 in bf16: 23.5 us, 0.87 of a measured copy. Append of 17059
-// tokens x 8 heads of 128: 28 us, 0.57 of a copy's rate: 110 instructions a
+// tokens x 8 heads of 128: 28 us, 0.57 of a copy's rate: 260 instructions a
 // unit of 16 values for the turn, the largest magnitude and the conversions.
 #include "kernels.cuh"
 #include "kv.cuh"

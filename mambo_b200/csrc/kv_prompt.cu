@@ -59,7 +59,7 @@ constexpr float kNone = -3e38f;       // m of a row that has seen nothing
 constexpr float kMostSum = 2048.f;    // of 16 weights, before m is moved: f16 holds 2^16
 constexpr float kMostPoly = 100.f;    // of the exponents that the polynomial takes: a larger one would not show in its sum
 // What a unit costs besides its tiles, in tiles: where the ranges of the CTAs are cut, units count as this much longer.
-// Queries, the first scores, masked halves and the results are some 15000 clocks. Prompt of 8192 tokens and a mixed step:
+// Its queries, first scores, masked halves and results. Prompt of 8192 tokens and a mixed step:
 // 3 552 and 100 us, 4 529 and 102, 5 525 and 102, 6 528 and 100.
 constexpr int kUnitCost = 6;
 
