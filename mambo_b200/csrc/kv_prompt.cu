@@ -267,10 +267,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
   }
-  // Behind the decode kernel (which waits for what came before it, and then lets this one start) there is nothing to wait
-  // for: they share nothing but the arguments. Its end is waited for at the end, so that this kernel's is the call's. (With
-  // the wait here a mixed step took 117 us for 111.)
-  if (p.few == 0) pdl_wait();
+  // Also behind the decode kernel of the same call, with which it shares nothing but the arguments: those are what kernels before
+  // that one have just written (cache, scales, lengths, queries), and only this wait makes their writes visible here.
+  pdl_wait();
   pdl_launch_dependents();
   // The whole work, and where this CTA's share begins: a warp has a run of sequences, a lane every 32nd unit of one.
   const int each = (p.seq.batch + 15) / 16, mine0 = min(p.seq.batch, warp * each), mine1 = min(p.seq.batch, mine0 + each);
@@ -983,7 +982,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::fence_after_sync();
     tc::dealloc(tmem, 512);
   }
-  if (p.few) pdl_wait();
 }
 
 size_t kv_prompt_partial_bytes(int sms) { return (size_t)sms * 4 * kPart * sizeof(float); }
