@@ -11,19 +11,28 @@
 //   S^T [128 positions x rows] = K Q^T        (keys: A, along K)
 //   O^T [head size x rows]    += V^T W^T      (values: A, along M)
 // with the rows as the MMA's N, and 128 positions or the head size as its M.
-// Queries and weights are two E4M3 terms each (kv_tc.cuh): the queries are
-// exact, the weights are rounded to 8 bits or more, as good as bf16. A thread
-// of the softmax has one position and all rows; S^T goes to it through TMEM,
-// the weights go back through shared memory, 16 bytes a term.
+// Queries are two E4M3 terms (kv_tc.cuh). Weights are three, each of what the
+// one before leaves, at 1, 2^4 and 2^8 times its size: columns of their own in
+// one MMA of N = 3 times the rows, so that the values are read from shared
+// memory once, and added up with their factors where a unit ends. A thread of
+// the softmax has one position and all rows; S^T goes to it through TMEM, the
+// weights go back through shared memory, 16 bytes a term.
 //
 // The softmax works with x = score * log2(e) + (exponent of the position's
 // value scale), so that the value scale needs no multiplication anywhere:
 //   w = 2^(x - m), O += w * code, l += w * 2^-exponent.
 // m need not be the maximum: it is moved (and O rescaled in TMEM) only when a
 // weight would pass 2^8.7, which a vote of the four warps finds out, so that
-// the common tile has no reduction over positions. m starts at the maximum of
-// the first tile less 4, which leaves weights of the maximum 2^4: the smallest
-// weights that matter, 2^-13 of that, still have 2 bits.
+// the common tile has no reduction over positions. It is moved to the maximum
+// less 6, so that the largest weight is at least 2^6.
+//
+// A weight's error is 2^-11 of it (f16, on the way to its terms) or, of the
+// smallest, 2^-18 (half the last term's step, 2^-9 of 2^-8): 2^-24 of the row's
+// largest weight. It must be that small because weights add up: beside a
+// position that has half of the mass, as the first one often does, each of n
+// others has 1/n of it, and 2^-24 n is the most that they lose together. (Two
+// terms of one size, with steps of 2^-9, lost up to a third of the result at
+// 32768 positions.)
 //
 // Work: the 128-position tiles of all (sequence, head) units in a row, cut into
 // one equal range per SM whatever the lengths are (they are on the device).
@@ -44,20 +53,22 @@ constexpr int kThreads = 256;
 constexpr int kMaxStages = 8;
 constexpr float kNone = -3e38f;      // m of a row that has seen nothing
 constexpr float kHeadroom = 8.7f;    // 2^8.7 < 448
-constexpr float kStart = 4.f;
+constexpr float kStart = 6.f;
+constexpr int kTerms = 3;            // of a weight, each 2^4 times as large as it counts beside the one before
+constexpr uint32_t kTermStep = 0x4C004C00u;  // 2^4, twice in f16
 
 template <int N>
 struct Cfg {
   static constexpr int kCtas = N == 16 ? 2 : 1;       // of an SM
   static constexpr uint32_t kStage = 2 * kKvTileBytes;
   static constexpr uint32_t kQ = N * 128u;            // bytes of a term of the queries
-  static constexpr uint32_t kW = 128u * N;            // of the weights: [N / 16][128 positions][16]
-  static constexpr uint32_t kTmem = 128;              // O: N columns, S: two of N
+  static constexpr uint32_t kW = 128u * N;            // of a term of the weights: [N / 16][128 positions][16]
+  static constexpr uint32_t kTmem = N == 16 ? 128 : 256;  // O: N columns for each term of the weights, S: two of N
   static constexpr uint32_t kMeta = 2 * N * 16;       // two units' row factors, places, tokens and heads
-  static constexpr uint32_t kScales = 2 * 32 * 16;    // two batches of pages
+  static constexpr uint32_t kScales = 2 * 32 * 8;     // two batches of pages
   static constexpr uint32_t kRed = (4 * N + 16) * 4;  // maxima or sums of the warps; the first tile, a flag
   static constexpr int kNumBars = 3 * kMaxStages + 15;
-  static constexpr uint32_t kFixed = 1024 + 4 * kQ + 2 * kW + kMeta + kScales + kRed + kNumBars * 8 + 16;
+  static constexpr uint32_t kFixed = 1024 + 4 * kQ + kTerms * kW + kMeta + kScales + kRed + kNumBars * 8 + 16;
   static constexpr int kPart = N * 130;               // floats of a part: O [N][128], m, l
 };
 
@@ -94,32 +105,24 @@ struct Walk {
   }
 };
 
-// O^T += V^T W^T over the 128 positions of a tile: values along M (128-byte swizzle, 32 positions in 4096 bytes), weights
-// along N (no swizzle, 32 positions in 512 bytes) in two terms w0, w1; and the arrivals once it is done.
-__device__ __forceinline__ void mma_values(uint32_t d, uint32_t v, uint32_t w0, uint32_t w1, uint32_t idesc, uint32_t acc,
-                                           uint32_t done0, uint32_t done1) {
+// O^T += V^T W^T over the 128 positions of a tile: values along M (128-byte swizzle, 32 positions in 4096 bytes), all terms of
+// the weights along N (no swizzle, 32 positions in 512 bytes); and the arrivals once it is done.
+__device__ __forceinline__ void mma_values(uint32_t d, uint32_t v, uint32_t w, uint32_t idesc, uint32_t acc, uint32_t done0,
+                                           uint32_t done1) {
   asm volatile(
-      "{\n\t.reg .pred p, t;\n\t.reg .b32 a, x, y;\n\t.reg .b64 da, dx, dy;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
-      "mov.b64 da, {%1, %6};\n\tmov.b64 dx, {%2, %7};\n\tmov.b64 dy, {%3, %7};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, dx, %4, p;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, dy, %4, t;\n\t"
-      "add.u32 a, %1, 256;\n\tadd.u32 x, %2, 32;\n\tadd.u32 y, %3, 32;\n\t"
-      "mov.b64 da, {a, %6};\n\tmov.b64 dx, {x, %7};\n\tmov.b64 dy, {y, %7};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, dx, %4, t;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, dy, %4, t;\n\t"
-      "add.u32 a, %1, 512;\n\tadd.u32 x, %2, 64;\n\tadd.u32 y, %3, 64;\n\t"
-      "mov.b64 da, {a, %6};\n\tmov.b64 dx, {x, %7};\n\tmov.b64 dy, {y, %7};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, dx, %4, t;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, dy, %4, t;\n\t"
-      "add.u32 a, %1, 768;\n\tadd.u32 x, %2, 96;\n\tadd.u32 y, %3, 96;\n\t"
-      "mov.b64 da, {a, %6};\n\tmov.b64 dx, {x, %7};\n\tmov.b64 dy, {y, %7};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, dx, %4, t;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, dy, %4, t;\n\t"
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%8];\n\t"
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%9];\n\t}" ::"r"(d),
-      "r"(v), "r"(w0), "r"(w1), "r"(idesc), "r"(acc), "r"(desc_high(1024, true)), "r"(desc_high(2048, false)), "r"(done0),
-      "r"(done1)
+      "{\n\t.reg .pred p, t;\n\t.reg .b32 a, x;\n\t.reg .b64 da, dx;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 dx, {%2, %6};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, dx, %3, p;\n\t"
+      "add.u32 a, %1, 256;\n\tadd.u32 x, %2, 32;\n\tmov.b64 da, {a, %5};\n\tmov.b64 dx, {x, %6};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, dx, %3, t;\n\t"
+      "add.u32 a, %1, 512;\n\tadd.u32 x, %2, 64;\n\tmov.b64 da, {a, %5};\n\tmov.b64 dx, {x, %6};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, dx, %3, t;\n\t"
+      "add.u32 a, %1, 768;\n\tadd.u32 x, %2, 96;\n\tmov.b64 da, {a, %5};\n\tmov.b64 dx, {x, %6};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, dx, %3, t;\n\t"
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t"
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%8];\n\t}" ::"r"(d),
+      "r"(v), "r"(w), "r"(idesc), "r"(acc), "r"(desc_high(1024, true)), "r"(desc_high(2048, false)), "r"(done0), "r"(done1)
       : "memory");
 }
 
@@ -154,11 +157,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* tiles0 = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* qs = tiles0 + (size_t)stages * C::kStage;  // [2 units][hi, lo][N][128]
-  uint8_t* ws = qs + 4 * C::kQ;                       // [hi, lo][N / 16][128][16]
-  float* factors = reinterpret_cast<float*>(ws + 2 * C::kW);   // [2][N]
+  uint8_t* ws = qs + 4 * C::kQ;                       // [terms][N / 16][128][16]
+  float* factors = reinterpret_cast<float*>(ws + kTerms * C::kW);  // [2][N]
   int* places = reinterpret_cast<int*>(factors + 2 * N);       // [2][N]
   int2* owners = reinterpret_cast<int2*>(places + 2 * N);      // [2][N]: the row's token and query head
-  float4* scales = reinterpret_cast<float4*>(owners + 2 * N);  // [2][32]: key factor, value exponent, 2^-exponent, is there
+  float2* scales = reinterpret_cast<float2*>(owners + 2 * N);  // [2][32]: key factor, value exponent (minus infinity: no page)
   float* red = reinterpret_cast<float*>(scales + 2 * 32);      // [4][N]
   int* begin = reinterpret_cast<int*>(red + 4 * N);            // the first tile: sequence, head, tile, tiles, start; a flag
   int* warp_sums = begin + 8;                                  // [8]
@@ -276,7 +279,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
   } else if (warp == 5) {
     // -------------------------------------------------------------- MMA
     if (walk.valid() && tm::elect_one()) {
-      constexpr uint32_t kIdS = tc::idesc_e4m3_f32(128, N), kIdO = kIdS | kIdescAlongM | kIdescAlongN;
+      constexpr uint32_t kIdS = tc::idesc_e4m3_f32(128, N);
+      constexpr uint32_t kIdO = tc::idesc_e4m3_f32(128, kTerms * N) | kIdescAlongM | kIdescAlongN;
       const bool wide = p.cache.dim > 64;
       const uint32_t stage0 = smem_u32(tiles0), q0 = smem_u32(qs), w0 = smem_u32(ws);
       KvRing kr, vr, sr, qr;
@@ -284,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
       bool ok = true, first_unit = true, v_first = false;
       // The scores of a tile are formed before the weights of the one before it are waited for.
       auto scores = [&](const Walk& w) {
-        uint32_t d = tmem + N + sr.at * N, a = desc_low(stage0 + kr.at * C::kStage, 16);
+        uint32_t d = tmem + kTerms * N + sr.at * N, a = desc_low(stage0 + kr.at * C::kStage, 16);
         uint32_t b = desc_low(q0 + qr.at * 2 * C::kQ, 16);
         asm volatile("" : "+r"(d), "+r"(a), "+r"(b));  // before the waits
         if (w.first && !kv_wait(kQfull + 8 * qr.at, qr.phase, kSiteKvFull)) return false;
@@ -316,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
           first_unit = false;
         }
         tc::fence_after_sync();
-        mma_values(tmem, v, w, w + (C::kW >> 4), kIdO, !first, kWfree, kEmpty + 8 * vr.at);
+        mma_values(tmem, v, w, kIdO, !first, kWfree, kEmpty + 8 * vr.at);
         vr.next(stages);
         return true;
       };
@@ -410,13 +414,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
         walk.next();
       }
       const int page = at >= 0 ? __ldg(p.seq.table + at) : -1;
-      float4 v = make_float4(0.f, 0.f, 1.f, 0.f);
+      float2 v = make_float2(0.f, -INFINITY);
       if (page >= 0 && page < p.cache.pages) {
         const int64_t row = (int64_t)page * p.cache.heads + h;
         const uint32_t kc = max((uint32_t)__ldg(p.cache.scales[0] + row), kKvMinCode);
         const uint32_t vc = max((uint32_t)__ldg(p.cache.scales[1] + row), kKvMinCode);
-        v = make_float4(kc == 255u ? NAN : e8m0_to_float(kc), vc == 255u ? NAN : (float)((int)vc - 127),
-                        vc == 255u ? 1.f : e8m0_to_float(254u - vc), 1.f);
+        v = make_float2(kc == 255u ? NAN : e8m0_to_float(kc), vc == 255u ? NAN : (float)((int)vc - 127));
       }
       if (step >= 2 && !(ok = kv_warp_wait(kMfree + 8 * ring.at, ring.phase ^ 1, kSiteKvEmpty))) break;
       scales[ring.at * 32 + lane] = v;
@@ -432,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
     uint32_t wphase = 1;  // of the last tile's MMAs on the values: a fresh barrier's previous phase counts as over
     KvRing mr;
     int in_batch = 0;
-    float m[N], l[N], cq[N];
+    float m[N], l[N];
     int place_lo = 0, place_hi = 0;
     bool failed = false;
     while (walk.valid()) {
@@ -442,7 +445,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
         failed |= !kv_warp_wait(kQfull + 8 * qr.at, qr.phase, kSiteKvFull);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-          cq[n] = factors[qr.at * N + n];
           m[n] = kNone;
           l[n] = 0.f;
         }
@@ -450,9 +452,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
         place_hi = pl[N - 1];
       }
       if (in_batch == 0) failed |= !kv_warp_wait(kMfull + 8 * mr.at, mr.phase, kSiteKvFull);
-      const float4 sc = scales[mr.at * 32 + in_batch * per_tile + (j >> log_page)];
-      const float ck = sc.x, ev = sc.y, back = sc.z;
-      const bool there = sc.w != 0.f;
+      const float2 sc = scales[mr.at * 32 + in_batch * per_tile + (j >> log_page)];
+      const float ck = sc.x, ev = sc.y;
+      const bool there = ev != -INFINITY;
+      const float back = there ? e8m0_to_float((uint32_t)(127 - (int)ev)) : 1.f;  // 2^-ev; of a NaN 1
       if (++in_batch == batch) {
         in_batch = 0;
         __syncwarp();
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
       failed |= !kv_warp_wait(kSfull + 8 * sr.at, sr.phase, kSiteKvFull);
       tc::fence_after_sync();
       uint32_t raw[N];
-      kv_ld<N>(tq + N + sr.at * N, raw);
+      kv_ld<N>(tq + kTerms * N + sr.at * N, raw);
       kv_wait_ld();
       kv_tie(raw);
       tc::fence_before_sync();
@@ -471,9 +474,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
 
       const int64_t j0 = (int64_t)(walk.start + walk.t) * kKvTile, jj = j0 + j;
       const bool edge = j0 + kKvTile - 1 > place_lo || (p.window && j0 <= (int64_t)place_hi - p.window);
+      // The rows' factors from shared memory: in registers they made the form of 16 rows spill (64 x 1 token 138 us for 129).
       float x[N];
 #pragma unroll
-      for (int n = 0; n < N; ++n) x[n] = fmaf(__uint_as_float(raw[n]) * cq[n], ck, ev);
+      for (int n = 0; n < N; n += 4) {
+        const float4 c = *reinterpret_cast<const float4*>(factors + qr.at * N + n);
+        x[n] = fmaf(__uint_as_float(raw[n]) * c.x, ck, ev), x[n + 1] = fmaf(__uint_as_float(raw[n + 1]) * c.y, ck, ev);
+        x[n + 2] = fmaf(__uint_as_float(raw[n + 2]) * c.z, ck, ev), x[n + 3] = fmaf(__uint_as_float(raw[n + 3]) * c.w, ck, ev);
+      }
       if (edge || !__all_sync(0xFFFFFFFFu, there)) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
@@ -511,12 +519,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
           // O holds all tiles before once the last one's MMAs are done.
           failed |= !kv_warp_wait(kWfree, wphase, kSiteKvFull);
           tc::fence_after_sync();
-          kv_ld<N>(tq, raw);
-          kv_wait_ld();
-          kv_tie(raw);
+#pragma unroll 1
+          for (uint32_t to = tq; to < tq + kTerms * N; to += N) {
+            kv_ld<N>(to, raw);
+            kv_wait_ld();
+            kv_tie(raw);
 #pragma unroll
-          for (int n = 0; n < N; ++n) raw[n] = __float_as_uint(__uint_as_float(raw[n]) * f[n]);
-          tc::st_cols<N>(tq, raw);
+            for (int n = 0; n < N; ++n) raw[n] = __float_as_uint(__uint_as_float(raw[n]) * f[n]);
+            tc::st_cols<N>(to, raw);
+          }
           tc::wait_st();
           tc::fence_before_sync();
         }
@@ -535,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
       uint8_t* w = ws + j * 16;
 #pragma unroll
       for (int g = 0; g < N / 16; ++g) {
-        uint32_t hi[4], lo[4];
+        uint32_t term[kTerms][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int n = 16 * g + 4 * i;
@@ -545,14 +556,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
             e[k] = ex2(x[n + k] - m[n + k]);
             l[n + k] = fmaf(e[k], back, l[n + k]);
           }
-          const uint32_t a = f16x2_of(e[0], e[1]), b = f16x2_of(e[2], e[3]);
-          const uint32_t ha = e4m3x2_of_f16x2(a), hb = e4m3x2_of_f16x2(b);
-          hi[i] = ha | (hb << 16);
-          lo[i] = e4m3x2_of_f16x2(sub_f16x2(a, f16x2_of_e4m3x2(ha))) |
-                  (e4m3x2_of_f16x2(sub_f16x2(b, f16x2_of_e4m3x2(hb))) << 16);
+          uint32_t a = f16x2_of(e[0], e[1]), b = f16x2_of(e[2], e[3]);
+#pragma unroll
+          for (int t = 0;; ++t) {
+            const uint32_t ha = e4m3x2_of_f16x2(a), hb = e4m3x2_of_f16x2(b);
+            term[t][i] = ha | (hb << 16);
+            if (t == kTerms - 1) break;
+            a = mul_f16x2(sub_f16x2(a, f16x2_of_e4m3x2(ha)), kTermStep);  // exact, both
+            b = mul_f16x2(sub_f16x2(b, f16x2_of_e4m3x2(hb)), kTermStep);
+          }
         }
-        *reinterpret_cast<uint4*>(w + g * 2048) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(w + C::kW + g * 2048) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+        for (int t = 0; t < kTerms; ++t)
+          *reinterpret_cast<uint4*>(w + t * C::kW + g * 2048) = make_uint4(term[t][0], term[t][1], term[t][2], term[t][3]);
       }
       fence_proxy_async_shared();
       __syncwarp();
@@ -574,9 +590,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
         red[warp * N + column] = reduce_columns<N>(l, lane, [](float a, float b) { return a + b; });
         failed |= !kv_warp_wait(kWfree, wphase, kSiteKvFull);
         tc::fence_after_sync();
-        kv_ld<N>(tq, raw);
+        // The terms' sums with their factors, the smallest first.
+        kv_ld<N>(tq + (kTerms - 1) * N, raw);
         kv_wait_ld();
         kv_tie(raw);
+#pragma unroll
+        for (int t = kTerms - 2; t >= 0; --t) {
+          uint32_t more[N];
+          kv_ld<N>(tq + t * N, more);
+          kv_wait_ld();
+          kv_tie(more);
+#pragma unroll
+          for (int n = 0; n < N; ++n) raw[n] = __float_as_uint(fmaf(__uint_as_float(raw[n]), 0.0625f, __uint_as_float(more[n])));
+        }
         tc::fence_before_sync();
         if (lane == 0) mbar_arrive(kOfree);
         kv_bar_sync(1, 128);

@@ -78,6 +78,12 @@ __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
   return d;
 }
 
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
 // The UE8M0 code of the power of two that brings a bf16 magnitude (its bits) to at most 448, 255 for NaN and infinity; as
 // mxfp8_scale_code, but for zero, and without branches: those keep the compiler from overlapping the chains of several
 // rows, and a row's chain (shuffles, code, conversions) is some 400 clocks.
