@@ -658,9 +658,11 @@ MAMBO_API int mambo_kv_append(const MamboKvCache* cache, const void* k, int64_t 
  *   out = sum_j softmax_j(scale * q . k_j) v_j   (bf16),   lse = log sum_j exp(scale * q . k_j)   (f32, may be null).
  * A query that sees nothing has zeros and an lse of minus infinity; rows that
  * no sequence covers are not written. Positions of a page outside the cache do
- * not exist; what no query sees may hold anything. Value scales of the pages
- * that a query sees may be 2^100 apart. out may be q, with its strides. The heads of q and out are 16-byte
- * aligned (strides in multiples of 8). scale: a positive number. workspace:
+ * not exist; what no query sees may hold anything. exp(..) times the page's
+ * value scale is rounded by 2^-11 of itself or 2^-24 of the row's largest such
+ * product; lse is right with value scales up to 2^100 apart. out may be q, with
+ * its strides. The heads of q and out are 16-byte aligned (strides in
+ * multiples of 8). scale: a positive number. workspace:
  * mambo_kv_attention_workspace_bytes(ragged: with offsets), zero-filled once,
  * shared with the other calls of the stream.
  */

@@ -165,10 +165,17 @@ def fp8_paged_attention(q, cache: Fp8KvCache, page_table, lengths, *, offsets=No
     A query sees the positions up to its own, with ``window`` the last
     ``window`` of them. Query head h reads key head h // (Hq / H). ``scale``
     (1/sqrt(D)) multiplies the scores. A query that sees nothing has zeros.
-    Positions of a page outside the cache do not exist. The value scales of the
-    pages that a query sees may be 2^100 apart: positions whose scale is smaller
-    by more are lost from the sum. ``out`` may be q; tokens that no sequence has
-    keep what it holds (without it, and in the logarithms, anything).
+    Positions of a page outside the cache do not exist. ``out`` may be q; tokens
+    that no sequence has keep what it holds (without it, and in the logarithms,
+    anything).
+
+    Scores and sums are float32. A position's weight times its page's value
+    scale is rounded by 2^-11 of itself or 2^-24 of the row's largest such
+    product, whichever is more: 8 bits are left of one that is 2^-16 of the
+    largest, and nothing behind 2^-24. So where a query sees pages whose value
+    scales are further apart than that, dimensions in which those of the large
+    scale hold zeros lose what the others hold. The logarithms are right with
+    scales up to 2^100 apart.
 
     ``return_lse``: also the float32 [T,Hq] logarithms of the sums of the
     exponentials (minus infinity where a query sees nothing), with which

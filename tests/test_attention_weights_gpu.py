@@ -153,6 +153,20 @@ def test_pages_of_small_values(cuda_device, kv, group, dim, tokens, apart):
         assert float((got.double() - want)[..., small].norm() / want[..., small].norm()) < 2.0 ** -7
 
 
+@pytest.mark.parametrize("apart", [18, 20])
+@pytest.mark.parametrize("kv,group,dim,tokens", FORMS)
+def test_pages_of_far_smaller_values(cuda_device, kv, group, dim, tokens, apart):
+    """The same with values of which few bits are left: the bound is an eighth and half of the others' values."""
+    gen = torch.Generator(device="cuda").manual_seed(apart)
+    n = 2048
+    k = torch.randn(kv, n, dim, generator=gen, device="cuda")
+    v = torch.rand(kv, n, dim, generator=gen, device="cuda") + 0.5
+    v[:, 5 * PAGE:6 * PAGE] = 0
+    v[:, 5 * PAGE + 7, 3] = 2.0 ** apart
+    q = torch.randn(64 * tokens, kv * group, dim, generator=gen, device="cuda").bfloat16()
+    verify(q, k, v, tokens, 64)
+
+
 @pytest.mark.parametrize("share", [0.5, 0.9])
 @pytest.mark.parametrize("group", [4, 20])
 def test_a_token_alone_and_in_a_prompt(cuda_device, group, share):
