@@ -162,22 +162,30 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&b);
 }
 
+// The words of the pairs that turn (all eight, or the first of an interleaved unit's, whose pair i is word i in 16 bits and
+// words 2 i and 2 i + 1 in 32) from lo and hi, the others as they came: bit for bit, whatever their neighbours are.
 template <bool k16>
-__device__ __forceinline__ void unit_store(void* out, int64_t at, const RotaryUnit& u, const float (&lo)[8],
-                                           const float (&hi)[8]) {
-  if constexpr (k16) {
-    uint16_t* p = reinterpret_cast<uint16_t*>(out) + at;
-    *reinterpret_cast<uint4*>(p + u.a) =
-        make_uint4(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7]));
-    *reinterpret_cast<uint4*>(p + u.b) =
-        make_uint4(pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3]), pack_bf16(hi[4], hi[5]), pack_bf16(hi[6], hi[7]));
-  } else {
-    float* p = reinterpret_cast<float*>(out) + at;
+__device__ __forceinline__ void unit_store(void* out, int64_t at, const RotaryUnit& u, const RawUnit<k16>& raw,
+                                           const float (&lo)[8], const float (&hi)[8]) {
+  constexpr int kWords = k16 ? 8 : 16, kHalf = kWords / 8;
+  uint32_t w[kWords];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      reinterpret_cast<float4*>(p + u.a)[i] = make_float4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
-      reinterpret_cast<float4*>(p + u.b)[i] = make_float4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-    }
+  for (int i = 0; i < kWords; ++i) {
+    const float* v = i < kWords / 2 ? lo : hi;
+    const int k = i % (kWords / 2);
+    w[i] = k16 ? pack_bf16(v[(2 * k) % 8], v[(2 * k + 1) % 8]) : __float_as_uint(v[k]);
+  }
+  if (u.turned < 8) {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(raw.w);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = i / kHalf < u.turned ? w[i] : r[i];
+  }
+  uint8_t* p = reinterpret_cast<uint8_t*>(out) + at * (k16 ? 2 : 4);
+#pragma unroll
+  for (int i = 0; i < kHalf; ++i) {
+    const int j = 4 * i, k = 4 * (kHalf + i);
+    reinterpret_cast<uint4*>(p + u.a * (k16 ? 2 : 4))[i] = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+    reinterpret_cast<uint4*>(p + u.b * (k16 ? 2 : 4))[i] = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
   }
 }
 
@@ -213,7 +221,7 @@ __global__ void __launch_bounds__(256, kPer == 4 && k16 ? 3 : 1) rotary_kernel(c
       float lo[8], hi[8];
       raw[i].get(lo, hi);
       if (turns) unit_turn(p.rot.interleaved, c, s, lo, hi);
-      unit_store<k16>(p.out, to + h * p.os_h, u, lo, hi);
+      unit_store<k16>(p.out, to + h * p.os_h, u, raw[i], lo, hi);
     }
   }
 }
