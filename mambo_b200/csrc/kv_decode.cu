@@ -479,8 +479,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
 #pragma unroll
       for (int n = 0; n < N; n += 4) {
         const float4 c = *reinterpret_cast<const float4*>(factors + qr.at * N + n);
-        x[n] = fmaf(__uint_as_float(raw[n]) * c.x, ck, ev), x[n + 1] = fmaf(__uint_as_float(raw[n + 1]) * c.y, ck, ev);
-        x[n + 2] = fmaf(__uint_as_float(raw[n + 2]) * c.z, ck, ev), x[n + 3] = fmaf(__uint_as_float(raw[n + 3]) * c.w, ck, ev);
+        // The factors' product first: large queries over small keys have scores that a product with one of them alone may pass.
+        x[n] = fmaf(__uint_as_float(raw[n]), c.x * ck, ev), x[n + 1] = fmaf(__uint_as_float(raw[n + 1]), c.y * ck, ev);
+        x[n + 2] = fmaf(__uint_as_float(raw[n + 2]), c.z * ck, ev), x[n + 3] = fmaf(__uint_as_float(raw[n + 3]), c.w * ck, ev);
       }
       if (edge || !__all_sync(0xFFFFFFFFu, there)) {
 #pragma unroll

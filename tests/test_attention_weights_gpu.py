@@ -184,3 +184,27 @@ def test_a_token_alone_and_in_a_prompt(cuda_device, group, share):
     chunk = verify(q, k, v, tokens, 1)[0]
     for alone in verify(q[-1:].repeat(batch, 1, 1), k, v, 1, batch):
         assert float((alone[0][0].double() - chunk[0][-1].double()).norm() / chunk[1][-1].norm()) < 2.0 ** -8
+
+
+@pytest.mark.parametrize("qe,ke", [(122, -64), (100, -64), (-100, 60), (-120, 100)])
+@pytest.mark.parametrize("kv,group,dim,tokens", FORMS)
+def test_large_queries_over_small_keys(cuda_device, kv, group, dim, tokens, qe, ke):
+    """Queries and keys near either end of float32 whose products are not: one position has all of the weight."""
+    n, at = 512, 333
+    k = torch.zeros(kv, n, dim, device="cuda")
+    k[:, at] = 1
+    codes, _ = quantized(k, PAGE)
+    values = torch.arange(n, device="cuda").float().remainder(16)[None, :, None].expand(kv, n, dim)
+    vc, vs = quantized(values, PAGE)
+    cache = {"keys": codes, "values": vc, "key_scales": torch.full_like(vs, 127 + ke), "value_scales": vs}
+    q = torch.full((8 * tokens, kv * group, dim), 2.0 ** qe, device="cuda", dtype=torch.bfloat16)
+    # codes of 2^8: scores of 2^(8 + qe + ke) times the head size at that position, zero at the others
+    scale = max(1.0, 2.0 ** -(qe + ke))
+    assert float(codes.view(torch.float8_e4m3fn).float().max()) == 256
+    table = torch.arange(n // PAGE, dtype=torch.int32, device="cuda")[None].repeat(8, 1)
+    lengths = torch.full((8,), n, dtype=torch.int32, device="cuda")
+    offsets = None if tokens == 1 else torch.arange(0, 8 * tokens + 1, tokens, dtype=torch.int32, device="cuda")
+    got, lse = fp8_paged_attention(q, cache, table, lengths, offsets=offsets, scale=scale, return_lse=True)
+    assert (got == at % 16).all()
+    want = scale * 2.0 ** (8 + qe + ke) * dim
+    assert (lse.double() / want - 1).abs().max() < 2.0 ** -20
