@@ -621,7 +621,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t qphase = 1;              // a fresh barrier's previous phase counts as over
     // Of the unit's queries this warp's 32 rows, split into two terms, to shared memory: a half warp a row, eight dimensions
     // a lane. The rows come as they are to where their terms go (a row of bf16 is as large as both), all at once and
-    // asynchronously, and are split in place. The factor of this thread's row is returned.
+    // asynchronously, and are split in place. The factor of this thread's row is returned; minus zero stands for a row that is
+    // not finite, whose sum becomes NaN at the unit's end if it sees anything.
     const int step_t = 2 / p.group, step_h = 2 - step_t * p.group;  // two rows on: tokens and heads
     auto queries = [&](const Unit& u) {
       const int c = lane & 15, r0 = 32 * (warp & 3) + (lane >> 4);
@@ -696,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_proxy_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(kQfull + 8 * q);
-      return bad ? NAN : p.scale * 1.4426950408889634f * e8m0_to_float(code);
+      return bad ? -0.f : p.scale * 1.4426950408889634f * e8m0_to_float(code);
     };
     // Through the units, one behind: the next one's queries are on their way before this one's results are waited for.
     float m = kNone, l = 0.f, cq = 0.f;
@@ -884,6 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int cta0 = whole ? 0 : kv_owner(unit.x, total, ctas);
         const int cta1 = whole ? 0 : kv_owner(unit.x + unit.tiles - 1, total, ctas);
         auto part = [&](int cta) { return partials + ((int64_t)(cta * 2 + (cta == cta0)) * 2 + q) * kPart; };
+        if (l != 0.f && __float_as_uint(cq) == 0x80000000u) l = NAN;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         uint32_t o[32];
         if (started) kv_ld<32>(to_, o);

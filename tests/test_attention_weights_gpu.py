@@ -208,3 +208,30 @@ def test_large_queries_over_small_keys(cuda_device, kv, group, dim, tokens, qe, 
     assert (got == at % 16).all()
     want = scale * 2.0 ** (8 + qe + ke) * dim
     assert (lse.double() / want - 1).abs().max() < 2.0 ** -20
+
+
+@pytest.mark.parametrize("kv,group,dim,tokens", FORMS)
+def test_not_finite_and_nothing_to_see(cuda_device, kv, group, dim, tokens):
+    """A query that is not finite and sees nothing has zeros like any other: all of its pages are outside the cache, or
+    those in its window. One that sees anything is NaN."""
+    n, batch = 4 * PAGE, 4
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    (kc, ks), (vc, vs) = (quantized(torch.randn(kv, n, dim, generator=gen, device="cuda"), PAGE) for _ in range(2))
+    cache = {"keys": kc, "values": vc, "key_scales": ks, "value_scales": vs}
+    table = torch.tensor([[-1, 9, -1, 1 << 30], [0, 1, 2, 3], [0, 1, 2, -1], [-1, -1, -1, 3]], dtype=torch.int32, device="cuda")
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    offsets = None if tokens == 1 else torch.arange(0, batch * tokens + 1, tokens, dtype=torch.int32, device="cuda")
+    for bad in (math.nan, math.inf):
+        q = torch.randn(batch, tokens, kv * group, dim, generator=gen, device="cuda").bfloat16()
+        q[:, :, 1, 3] = bad
+        got, lse = fp8_paged_attention(q.view(-1, kv * group, dim), cache, table, lengths, offsets=offsets, return_lse=True)
+        got, lse = got.view(q.shape), lse.view(q.shape[:3])
+        assert (got[0] == 0).all() and (lse[0] == -math.inf).all()
+        assert got[1:, :, 1].isnan().all() and lse[1:, :, 1].isnan().all()
+        others = [h for h in range(kv * group) if h != 1]
+        assert got[1:, :, others].isfinite().all() and lse[1:, :, others].isfinite().all()
+        got, lse = fp8_paged_attention(q.view(-1, kv * group, dim), cache, table, lengths, offsets=offsets, window=20,
+                                       return_lse=True)
+        got, lse = got.view(q.shape), lse.view(q.shape[:3])
+        assert (got[2] == 0).all() and (lse[2] == -math.inf).all()
+        assert got[3, :, 1].isnan().all() and got[3, :, others].isfinite().all()
