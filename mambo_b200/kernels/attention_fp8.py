@@ -84,7 +84,7 @@ def _sequences(page_table, lengths, offsets, tokens: int, device: int) -> tuple[
     if not lengths.is_contiguous():
         lengths = lengths.contiguous()
     stride, unit = table.stride()
-    if unit != 1 and columns > 1:
+    if (unit != 1 and columns > 1) or (stride < columns and batch > 1):  # also rows that share memory (expanded)
         table = table.contiguous()
         stride = columns
     at = None
