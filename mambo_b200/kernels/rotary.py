@@ -101,8 +101,10 @@ def prepare_rotary_fields(rotary_dim: int, *, base: float = 10000.0, interleaved
 
 
 def _check_rope(rope: RotaryFields, dim: int, device: torch.device) -> None:
-    if not isinstance(rope, dict) or "rotary" not in rope:
+    if not isinstance(rope, dict) or "rotary" not in rope or "turns" not in rope:
         raise TypeError("rope must come from prepare_rotary_fields")
+    if rope["rotary"].turns != rope["turns"].data_ptr():  # a copy of the fields: the kernels would read the first one's table
+        raise ValueError("rope's tensors were replaced: call prepare_rotary_fields again")
     if rope["rotary_dim"] > dim:
         raise ValueError("the rotated part is larger than the head")
     if rope["turns"].get_device() != device.index:
