@@ -35,7 +35,7 @@ int check_cache(const MamboKvCache* c) {
   if (c->head_dim < 16 || c->head_dim % 16 || c->head_dim > kKvMaxDim)
     return api_fail(MAMBO_EINVAL, "the head size must be a multiple of 16, at most %d", kKvMaxDim);
   if (c->kv_heads < 1 || c->kv_heads > kMaxHeads) return api_fail(MAMBO_EINVAL, "1 to %d heads", (int)kMaxHeads);
-  if (c->pages < 1 || c->pages * c->kv_heads > kMaxPages) return api_fail(MAMBO_EINVAL, "pages * heads must be in [1, 2^31]");
+  if (c->pages < 1 || c->pages > kMaxPages / c->kv_heads) return api_fail(MAMBO_EINVAL, "pages * heads must be in [1, 2^31]");
   if (!aligned(c->keys, 16) || !aligned(c->values, 16)) return api_fail(MAMBO_EINVAL, "the cache must be 16-byte aligned");
   return MAMBO_OK;
 }

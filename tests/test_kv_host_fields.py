@@ -1,4 +1,4 @@
-"""CPU: rotary fields whose tensor was replaced are refused before anything is launched."""
+"""CPU: rotary fields whose tensor was replaced, and cache sizes past 64 bits, are refused before anything is launched."""
 
 from __future__ import annotations
 
@@ -10,6 +10,7 @@ import torch
 from mambo_b200 import _lib
 from mambo_b200.kernels import rotary
 
+P = 4096  # a pointer that no refused call follows
 CPU = types.SimpleNamespace(index=-1)  # the device of tensors that have none
 
 
@@ -26,3 +27,17 @@ def test_replaced_tables_are_refused():
     for missing in ("turns", "rotary"):
         with pytest.raises(TypeError):
             rotary._check_rope({k: v for k, v in rope.items() if k != missing}, 8, CPU)
+
+
+@pytest.mark.parametrize("pages,heads", [(1 << 54, 1024), (1 << 62, 4), (1 << 63 - 1, 2), ((1 << 62) + 1, 4), (1 << 31, 2)])
+def test_cache_sizes_past_64_bits(pages, heads):
+    """Pages times heads that wrap to something small."""
+    lib = _lib.load()
+    cache = _lib.MamboKvCache(P, P, P, P, pages, heads, 16, 64)
+    seq = _lib.MamboKvSequences(P, 4, 4, P, None, 3)
+    assert lib.mambo_kv_append(cache, P, 128, 64, P, 128, 64, _lib.MAMBO_BF16, 3, seq, None, None) == _lib.MAMBO_EINVAL
+    assert "pages" in _lib.last_error()
+    need = lib.mambo_kv_attention_workspace_bytes(heads, heads, 0)
+    assert lib.mambo_kv_attention(P, 64 * heads, 64, 3, heads, cache, seq, 0, 1.0, P, 64 * heads, 64, None, heads, 1, P, need,
+                                  None) == _lib.MAMBO_EINVAL
+    assert "pages" in _lib.last_error()
