@@ -23,8 +23,8 @@
 //   w = 2^(x - m), O += w * code, l += w * 2^-exponent.
 // m need not be the maximum: it is moved (and O rescaled in TMEM) only when a
 // weight would pass 2^8.7, which a vote of the four warps finds out, so that
-// the common tile has no reduction over positions. It is moved to the maximum
-// less 6, so that the largest weight is at least 2^6.
+// the common tile has no reduction over positions. A row's m is moved to its
+// maximum less 6, so that its largest weight is at least 2^6.
 //
 // A weight's error is 2^-11 of it (f16, on the way to its terms) or, of the
 // smallest, 2^-18 (half the last term's step, 2^-9 of 2^-8): 2^-24 of the row's
@@ -510,10 +510,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float to = fmaxf(m[n + k], t[k] - kStart);
-            f[n + k] = ex2(m[n + k] - to);
-            m[n + k] = to;
-            l[n + k] *= f[n + k];
+            // Only where the row itself asks for it: its bits must not depend on the others', of which those behind the last
+            // one hold whatever was in shared memory.
+            f[n + k] = 1.f;
+            if (t[k] > m[n + k] + kHeadroom) {
+              f[n + k] = ex2(m[n + k] - (t[k] - kStart));
+              m[n + k] = t[k] - kStart;
+              l[n + k] *= f[n + k];
+            }
           }
         }
         if (!first) {
