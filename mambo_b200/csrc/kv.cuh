@@ -39,7 +39,7 @@ struct RotaryCall {
   int64_t xs_t, xs_h, os_t, os_h;  // strides in elements
   const void* positions;
   int positions64;
-  int units, per, groups;  // units of 16 dimensions of a head, heads of a thread, threads' head groups
+  int units, groups;  // of a head: units of 16 dimensions, or pairs of values where rows are not made of aligned vectors; of its heads
 };
 cudaError_t launch_rotary(RotaryCall p, cudaStream_t stream);
 

@@ -41,28 +41,23 @@ __device__ __forceinline__ void turn_cos_sin(uint64_t phase, float& c, float& s)
 
 // Where the 16 dimensions of a unit lie in a head. Interleaved pairs: dimensions a .. a+15, of which the first `turned`
 // pairs turn. Halves: dimensions a .. a+7 and b .. b+7, `turned` pairs; behind the rotated part a .. a+15, unchanged.
-// n: valid dimensions from a on (adjacent units).
 struct RotaryUnit {
-  int a, b, n, turned;
-  bool adjacent;
+  int a, b, turned;
 };
 __host__ __device__ __forceinline__ int rotary_units(const RotaryParams& r, int dim) {
   const int pairs = r.turns ? r.pairs : 0;
   return r.interleaved ? (dim + 15) / 16 : (pairs + 7) / 8 + (dim - 2 * pairs + 15) / 16;
 }
-__device__ __forceinline__ RotaryUnit rotary_unit(const RotaryParams& r, int dim, int u) {
+__device__ __forceinline__ RotaryUnit rotary_unit(const RotaryParams& r, int u) {
   RotaryUnit v;
   const int pairs = r.turns ? r.pairs : 0, first = r.interleaved ? 0 : (pairs + 7) / 8;
-  v.adjacent = u >= first;
-  if (v.adjacent) {
+  if (u >= first) {
     v.a = (r.interleaved ? 0 : 2 * pairs) + 16 * (u - first);
     v.b = v.a + 8;
-    v.n = min(16, dim - v.a);
     v.turned = r.interleaved ? max(min(8, pairs - 8 * u), 0) : 0;
   } else {
     v.a = 8 * u;
     v.b = pairs + 8 * u;
-    v.n = 0;
     v.turned = min(8, pairs - 8 * u);
   }
   return v;
@@ -199,7 +194,7 @@ __global__ void __launch_bounds__(256, kPer == 4 && k16 ? 3 : 1) rotary_kernel(c
   pdl_launch_dependents();
   if (token >= p.tokens) return;
   const int in = (int)(job - token * per_token), g = in / p.units, unit = in - g * p.units;
-  const RotaryUnit u = rotary_unit(p.rot, p.dim, unit);
+  const RotaryUnit u = rotary_unit(p.rot, unit);
   RawUnit<k16> raw[kPer];
   const int64_t from = token * p.xs_t, to = token * p.os_t;
 #pragma unroll
@@ -382,7 +377,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
   const int rows = row < p.rows_each ? (count - row + p.rows_each - 1) / p.rows_each : 0;  // of this thread
   if constexpr (kVec) {
     if (rows > 0) {
-      u = rotary_unit(rot, dim, unit);
+      u = rotary_unit(rot, unit);
       if constexpr (kAhead) raw.load(p.x[which], from + head0 * xs_h, u);
       if (u.turned > 0) unit_angles(rot, u, 8 * unit, t0 + row, c, s);
     }

@@ -109,9 +109,6 @@ __device__ __forceinline__ void split_e4m3x4(const float (&v)[4], uint32_t& hi, 
 // 16-byte unit). With the 128-byte swizzle: rows of 128 bytes along M or N, one per K; `sbo` between groups of 8 K,
 // `lbo` between the 128-byte columns of M or N. Without: 16-byte rows, 8 K in 128 bytes; `lbo` between groups of 8 K,
 // `sbo` between 16-byte columns.
-__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return tc::smem_desc(saddr, lbo, sbo) | (uint64_t)2 << 61;
-}
 constexpr uint32_t kIdescAlongM = 1u << 15, kIdescAlongN = 1u << 16;
 
 // Instructions whose operands sit in uniform registers issue in a few clocks each; descriptors formed one by one in a loop
