@@ -60,7 +60,7 @@ constexpr float kMostSum = 2048.f;    // of 16 weights, before m is moved: f16 h
 constexpr float kMostPoly = 100.f;    // of the exponents that the polynomial takes: a larger one would not show in its sum
 // What a unit costs besides its tiles, in tiles: where the ranges of the CTAs are cut, units count as this much longer.
 // Its queries, first scores, masked halves and results. Prompt of 8192 tokens and a mixed step:
-// 3 552 and 100 us, 4 529 and 102, 5 525 and 102, 6 528 and 100.
+// 3 557 and 110 us, 4 533 and 105, 5 529 and 114, 6 529 and 109 to 114 (the mixed step with its 31 us of the decode kernel).
 constexpr int kUnitCost = 6;
 
 // Shared memory: queries [2 tiles][hi, lo][128][128], keys, values as they come and in f16 [2 halves of D][128][128 bytes].
