@@ -715,7 +715,8 @@ template <int N>
 cudaError_t launch_decode(const KvAttentionCall& p, const CUtensorMap& k, const CUtensorMap& v, int sms, int smem_optin,
                           float* partials, int* counters, cudaStream_t stream) {
   using C = Cfg<N>;
-  // As many stages as fit the SM's shared memory, of which each CTA has 1 KB besides.
+  // As many stages as fit the SM's shared memory, of which each CTA has 1 KB besides: of two CTAs three each, with 376 bytes
+  // to spare, of one six.
   const uint32_t room = ((uint32_t)smem_optin + 1024) / C::kCtas - 1024;
   const int stages = min(kMaxStages, (int)((room - C::kFixed) / C::kStage));
   const uint32_t smem = C::kFixed + stages * C::kStage;

@@ -235,3 +235,32 @@ def test_not_finite_and_nothing_to_see(cuda_device, kv, group, dim, tokens):
         got, lse = got.view(q.shape), lse.view(q.shape[:3])
         assert (got[2] == 0).all() and (lse[2] == -math.inf).all()
         assert got[3, :, 1].isnan().all() and got[3, :, others].isfinite().all()
+
+
+@pytest.mark.parametrize("first", ["small", "large"])
+@pytest.mark.parametrize("kv,group,dim,tokens", FORMS)
+def test_logarithms_over_scales_far_apart(cuda_device, kv, group, dim, tokens, first):
+    """Half of the pages have a value scale 2^100 times as large as the others': the sum of the exponentials counts all
+    positions. Off by float32 sums of 64 exponentials a lane and page (2^-17 with room) and arguments of up to 2^8 (2^-15)."""
+    n, batch = 40 * PAGE, 8
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    kc, ks = quantized(torch.randn(kv, n, dim, generator=gen, device="cuda"), PAGE)
+    vc, _ = quantized(torch.randn(kv, n, dim, generator=gen, device="cuda"), PAGE)
+    vs = torch.full_like(ks, 127 - 64)
+    vs[(0 if first == "large" else 1)::2] = 127 + 36
+    cache = {"keys": kc, "values": vc, "key_scales": ks, "value_scales": vs}
+    table = torch.arange(n // PAGE, dtype=torch.int32, device="cuda")[None].repeat(batch, 1)
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    offsets = None if tokens == 1 else torch.arange(0, batch * tokens + 1, tokens, dtype=torch.int32, device="cuda")
+    q = torch.randn(batch * tokens, kv * group, dim, generator=gen, device="cuda").bfloat16()
+    _, lse = fp8_paged_attention(q, cache, table, lengths, offsets=offsets, return_lse=True)
+    k = dequantized(kc, ks)
+    for b in (0, batch - 1):
+        rows = slice(b * tokens, (b + 1) * tokens)
+        qs = q[rows].double().view(tokens, kv, group, dim)
+        s = torch.einsum("nhgd,hjd->nhgj", qs, k) * dim ** -0.5
+        seen = torch.arange(n, device="cuda")[None] <= n - tokens + torch.arange(tokens, device="cuda")[:, None]
+        want = torch.logsumexp(torch.where(seen[:, None, None], s, torch.full_like(s, -math.inf)), dim=-1)
+        es = 2.0 ** -18 * qs.abs().amax(dim=-1) * k.abs().sum(dim=-1).amax(dim=-1)[None, :, None] * dim ** -0.5
+        off = (lse[rows].double() - want.reshape(tokens, -1)).abs()
+        assert (off <= es.reshape(tokens, -1) + 2.0 ** -14).all(), float(off.max())
