@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
       }
       bool up = failed;
 #pragma unroll
-      for (int n = 0; n < N; ++n) up |= x[n] > m[n] + kHeadroom;
+      for (int n = 0; n < N; ++n) up |= x[n] - m[n] > kHeadroom;  // m + kHeadroom may round to 16 more than m, of scores near 2^27
       if (kv_bar_any(1, 128, up)) {
         if (kv_bar_any(1, 128, failed)) break;  // all four warps leave together
         float f[N];
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<N>::kCtas)
             // Only where the row itself asks for it: its bits must not depend on the others', of which those behind the last
             // one hold whatever was in shared memory.
             f[n + k] = 1.f;
-            if (t[k] > m[n + k] + kHeadroom) {
+            if (t[k] - m[n + k] > kHeadroom) {
               f[n + k] = ex2(m[n + k] - (t[k] - kStart));
               m[n + k] = t[k] - kStart;
               l[n + k] *= f[n + k];

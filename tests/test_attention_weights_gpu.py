@@ -264,3 +264,29 @@ def test_logarithms_over_scales_far_apart(cuda_device, kv, group, dim, tokens, f
         es = 2.0 ** -18 * qs.abs().amax(dim=-1) * k.abs().sum(dim=-1).amax(dim=-1)[None, :, None] * dim ** -0.5
         off = (lse[rows].double() - want.reshape(tokens, -1)).abs()
         assert (off <= es.reshape(tokens, -1) + 2.0 ** -14).all(), float(off.max())
+
+
+@pytest.mark.parametrize("power", list(range(20, 34)) + [60, 100])
+@pytest.mark.parametrize("kv,group,dim,tokens", FORMS)
+def test_scores_a_step_apart(cuda_device, kv, group, dim, tokens, power):
+    """Scores so large that neighbours in float32 are as far apart as the weights' range reaches. The values are all one, in
+    tiles of scale 2^-8 and 2^9 by turns, whose exponents move a score by a step or none: a result is one whatever
+    the scores round to."""
+    n, batch = 1024, 64 if tokens == 1 else 8
+    k = torch.zeros(kv, n, dim, device="cuda")
+    k[..., 0] = 256
+    kc, ks = quantized(k, PAGE)
+    ve = torch.where(torch.arange(n // PAGE, device="cuda") // 2 % 2 == 0, -8, 9)
+    vc = torch.exp2(-ve.float())[:, None, None, None].expand(-1, kv, PAGE, dim).to(torch.float8_e4m3fn).view(torch.uint8)
+    cache = {"keys": kc, "values": vc.contiguous(), "key_scales": ks,
+             "value_scales": (127 + ve).to(torch.uint8)[:, None].expand(-1, kv).contiguous()}
+    assert (dequantized(cache["values"], cache["value_scales"]) == 1).all()
+    q = torch.zeros(batch * tokens, kv * group, dim, device="cuda", dtype=torch.bfloat16)
+    q[..., 0] = 1 + torch.arange(q[..., 0].numel(), device="cuda").view(q.shape[:2]) % 128 / 128
+    table = torch.arange(n // PAGE, dtype=torch.int32, device="cuda")[None].repeat(batch, 1)
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    offsets = None if tokens == 1 else torch.arange(0, batch * tokens + 1, tokens, dtype=torch.int32, device="cuda")
+    for sign in (1, -1):  # scores of 2^power to 2^(power + 1) in powers of two, of either sign
+        got = fp8_paged_attention(sign * q, cache, table, lengths, offsets=offsets, scale=math.log(2) * 2.0 ** (power - 8))
+        # f16 weights and their terms, sums, bf16: 2^-10 + 2^-12 + 2^-8 at most
+        assert ((got.double() - 1).abs() < 2.0 ** -7).all(), (sign, float(got.min()), float(got.max()))
