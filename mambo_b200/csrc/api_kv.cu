@@ -72,7 +72,7 @@ KvSequences sequence_params(const MamboKvSequences* s, int64_t tokens) {
 // Rows of a sequence (tokens times query heads of a key head) that the decode kernel takes at most: it has forms for 16
 // and for 32 rows, and where the heads alone are more, none. Single tokens of 64 sequences, in the decode kernel, in the
 // prompt kernel and as the cache's bytes would take them, us: 4096 to 8191 positions, 8 key heads of 16 rows 137, 275 and
-// 123, 2 key heads of 20 rows 77, 87 and 31; 400 to 900 positions, 8 key heads of 16 rows 49, 82 and 13, 2 key heads of 20
+// 123, 2 key heads of 20 rows 75, 87 and 31; 400 to 900 positions, 8 key heads of 16 rows 49, 82 and 13, 2 key heads of 20
 // rows 32, 37 and 3.
 int few_rows(int group) { return group <= 16 ? 16 : group <= 32 ? 32 : 0; }
 size_t decode_bytes(int group) { return few_rows(group) ? (kv_decode_partial_bytes(group, kSmsBound) + 255) / 256 * 256 : 0; }

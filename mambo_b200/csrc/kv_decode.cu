@@ -7,7 +7,7 @@
 // heads: 133 us, 6.03 TB/s, 0.92 of a measured copy; one of 131072, 64 query
 // heads: 59 us, 0.69, the rest its start and the join of 37 parts a head).
 // With head size 64 (113 us, 0.55) or 17 to 32 rows (20 rows of 2 key heads:
-// 77 us, 0.40) by a tile's chain of scores, vote, weights and their terms.
+// 75 us, 0.41) by a tile's chain of scores, vote, weights and their terms.
 // So keys and values go from memory through tensor copies into shared
 // memory and from there straight into the tensor core, 8 bits as they are:
 //   S^T [128 positions x rows] = K Q^T        (keys: A, along K)
